@@ -272,6 +272,112 @@ int tfa_column_sums_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
 int tfa_column_sums(int64_t rows, int64_t cols, const float* re, const float* im, float* out_re, float* out_im,
                     void* workspace, tfa_stream stream);
 
+/* ---- Operators of models on frames (no counterpart in the reference) ---------------------------------------------
+ *
+ * What a model that is trained on STFT frames needs next to the transforms and the complex products: a mixing over
+ * frames with memory, a normalisation of channels-last features, and the optimizer's step.  Element types: */
+#define TFA_DTYPE_F32 0
+#define TFA_DTYPE_BF16 1
+#define TFA_DTYPE_F16 2
+
+/*
+ * Linear attention with a decay for each head, over (batch, tokens, heads, features) operands:
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   out_t = scale S_t^T q_t
+ * q, k (key_dim features) and v (value_dim) may have fewer heads than the call: head h reads head h / (heads / own).
+ * Their strides are in elements, for batch, token and head; features are contiguous.  State tensors are fp32 (batch,
+ * heads, key_dim, value_dim), the outputs contiguous (batch, tokens, heads, value_dim).  log_decay: (heads) device fp32, at most 0
+ * (-inf: no memory; above 0 the state grows).  lengths: (batch) device int64 or NULL; tokens at and past a sequence's
+ * length are padding: never read, zero in the outputs and gradients, and the state is the one at the length.  Products of
+ * bf16 operands are exact, scores, states and sums are fp32 for every type.  Head dimensions up to 256.
+ */
+typedef struct tfa_attn_desc {
+  int32_t dtype; /* TFA_DTYPE_* of q, k, v, out and their gradients */
+  int32_t heads, q_heads, k_heads, v_heads;
+  int32_t key_dim, value_dim;
+  float scale; /* finite, not zero */
+  int64_t batch, tokens;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, token, head */
+} tfa_attn_desc;
+
+/* Device workspace (bytes) of tfa_linear_attention (backward = 0) or its backward (1). */
+int tfa_linear_attention_workspace_size(const tfa_attn_desc* desc, int32_t backward, size_t* bytes);
+/* state_in may be NULL (zeros), state_out NULL (not wanted; must not be state_in otherwise). */
+int tfa_linear_attention(const tfa_attn_desc* desc, const void* q, const void* k, const void* v, const float* log_decay,
+                         const int64_t* lengths, const float* state_in, void* out, float* state_out, void* workspace,
+                         tfa_stream stream);
+/* Gradients of a loss whose gradients by out and state_out are grad_out (contiguous, as out) and grad_state_out (NULL:
+ * zero).  grad_q, grad_k, grad_v: contiguous (batch, tokens, own heads, features); each gradient may be NULL, but
+ * grad_log_decay needs grad_q and grad_state_in needs grad_v. */
+int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, const void* k, const void* v,
+                                  const float* log_decay, const int64_t* lengths, const float* state_in,
+                                  const void* grad_out, const float* grad_state_out, void* grad_q, void* grad_k,
+                                  void* grad_v, float* grad_log_decay, float* grad_state_in, void* workspace,
+                                  tfa_stream stream);
+/* One token of every stream (tokens = 1): state is updated in place, out = scale S^T q of the new state. */
+int tfa_linear_attention_step(const tfa_attn_desc* desc, const void* q, const void* k, const void* v,
+                              const float* log_decay, float* state, void* out, tfa_stream stream);
+
+/*
+ * Group norm with an activation on contiguous channels-last data (batch, positions, channels):
+ *   y = act((x - mean) rstd weight + bias), mean and rstd over the positions and the channels of a group
+ * weight, bias: fp32 (channels) or NULL; mean, rstd: fp32 (batch, groups), written by the forward, read by the backward.
+ * lengths: (batch) device int64 or NULL; positions at and past lengths[n] * inner are padding: never read, no part of the
+ * statistics, zeros in y and grad_x.
+ */
+#define TFA_ACT_NONE 0
+#define TFA_ACT_SILU 1
+#define TFA_ACT_GELU 2 /* z Phi(z), by the error function */
+#define TFA_ACT_RELU 3
+typedef struct tfa_norm_desc {
+  int32_t dtype; /* of x, y and their gradients */
+  int32_t channels, groups, activation;
+  int64_t batch, positions, inner;
+  float eps;
+  int32_t reserved;
+} tfa_norm_desc;
+
+int tfa_group_norm_workspace_size(const tfa_norm_desc* desc, int32_t backward, size_t* bytes);
+int tfa_group_norm(const tfa_norm_desc* desc, const void* x, const float* weight, const float* bias,
+                   const int64_t* lengths, void* y, float* mean, float* rstd, void* workspace, tfa_stream stream);
+/* grad_weight and grad_bias may be NULL. */
+int tfa_group_norm_backward(const tfa_norm_desc* desc, const void* x, const void* grad_y, const float* weight,
+                            const float* bias, const int64_t* lengths, const float* mean, const float* rstd,
+                            void* grad_x, float* grad_weight, float* grad_bias, void* workspace, tfa_stream stream);
+
+/*
+ * One AdamW step (decoupled weight decay) over many contiguous tensors:
+ *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * in fp32.  states: fp32, or 8-bit codes with one fp32 scale s per 256 values of a tensor: m = s sgn(c) (c / 127)^2 of int8
+ * codes, v = s (c / 255)^4 of uint8 codes, s the largest magnitude of the block.  With a master copy (fp32) the step is
+ * taken on it and param receives it rounded.  The tables are host memory, read before the call returns.
+ */
+typedef struct tfa_adam_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale; /* 8-bit states: ceil(n / 256) scales each; else NULL */
+  float* exp_avg_sq_scale;
+  float* master; /* or NULL */
+  int64_t n;
+} tfa_adam_tensor;
+typedef struct tfa_adam_desc {
+  int32_t param_dtype, grad_dtype, state_bits, reserved;
+  int64_t step; /* from 1 */
+  double lr, beta1, beta2, eps, weight_decay;
+} tfa_adam_desc;
+typedef struct tfa_code_tensor {
+  const void* codes;
+  const float* scales;
+  float* out;
+  int64_t n;
+} tfa_code_tensor;
+
+int tfa_adamw_step(int64_t count, const tfa_adam_tensor* tensors, const tfa_adam_desc* desc, tfa_stream stream);
+/* The fp32 values that 8-bit states stand for (squares = 0: exp_avg, 1: exp_avg_sq). */
+int tfa_adamw_state_values(int64_t count, const tfa_code_tensor* tensors, int32_t squares, tfa_stream stream);
+
 /* Thread-local message describing the last failure on this thread ("" if none). */
 const char* tfa_last_error(void);
 

@@ -25,8 +25,11 @@ from .api import (
     rfftn,
     stft,
 )
+from .attention import linear_attention, linear_attention_step
 from .complex import ComplexTensor, complex_matmul
 from .dispatch import HAS_HIP, HAS_NKI, complex_gemm, complex_linear, get_backend, hip_accepts, set_backend
+from .norm import group_norm
+from .optim import adamw_state_values, adamw_step
 from .plan import FFTAlgorithm, FFTPlan, clear_plan_cache, create_plan
 from .precision import get_precision, set_ozaki_product_precision_verified, set_precision
 
@@ -54,6 +57,11 @@ __all__ = [
     "clear_plan_cache",
     "FFTPlan",
     "FFTAlgorithm",
+    "linear_attention",
+    "linear_attention_step",
+    "group_norm",
+    "adamw_step",
+    "adamw_state_values",
     "HAS_HIP",
     "HAS_NKI",
     "set_backend",

@@ -57,9 +57,22 @@ EXPORTS = (
     "tfa_complex_gemm_ws",
     "tfa_column_sums_workspace_size",
     "tfa_column_sums",
+    "tfa_linear_attention_workspace_size",
+    "tfa_linear_attention",
+    "tfa_linear_attention_backward",
+    "tfa_linear_attention_step",
+    "tfa_group_norm_workspace_size",
+    "tfa_group_norm",
+    "tfa_group_norm_backward",
+    "tfa_adamw_step",
+    "tfa_adamw_state_values",
     "tfa_last_error",
     "tfa_abi_version",
 )
+
+# element types and activations of the operators of models
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+ACT_NONE, ACT_SILU, ACT_GELU, ACT_RELU = 0, 1, 2, 3
 
 
 class PlanDesc(ctypes.Structure):
@@ -71,6 +84,53 @@ class PlanDesc(ctypes.Structure):
         ("flags", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
         ("n2", ctypes.c_int64),
+    ]
+
+
+class AttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("v_heads", ctypes.c_int32),
+        ("key_dim", ctypes.c_int32),
+        ("value_dim", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+    ]
+
+
+class NormDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("channels", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("positions", ctypes.c_int64),
+        ("inner", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class AdamDesc(ctypes.Structure):
+    _fields_ = [
+        ("param_dtype", ctypes.c_int32),
+        ("grad_dtype", ctypes.c_int32),
+        ("state_bits", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("step", ctypes.c_int64),
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
     ]
 
 
@@ -131,6 +191,20 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.tfa_column_sums.restype = ctypes.c_int
     lib.tfa_execute_noalloc.argtypes = [_vp, _i64, _vp, _vp, _vp, _vp, _vp]
     lib.tfa_execute_noalloc.restype = ctypes.c_int
+    size_p = ctypes.POINTER(ctypes.c_size_t)
+    lib.tfa_linear_attention_workspace_size.argtypes = [ctypes.POINTER(AttnDesc), _i32, size_p]
+    lib.tfa_linear_attention.argtypes = [ctypes.POINTER(AttnDesc)] + [_vp] * 10
+    lib.tfa_linear_attention_backward.argtypes = [ctypes.POINTER(AttnDesc)] + [_vp] * 15
+    lib.tfa_linear_attention_step.argtypes = [ctypes.POINTER(AttnDesc)] + [_vp] * 7
+    lib.tfa_group_norm_workspace_size.argtypes = [ctypes.POINTER(NormDesc), _i32, size_p]
+    lib.tfa_group_norm.argtypes = [ctypes.POINTER(NormDesc)] + [_vp] * 9
+    lib.tfa_group_norm_backward.argtypes = [ctypes.POINTER(NormDesc)] + [_vp] * 12
+    # the tables of the multi-tensor steps (tfa_adam_tensor, tfa_code_tensor) are passed as packed 64-bit words
+    lib.tfa_adamw_step.argtypes = [_i64, _vp, ctypes.POINTER(AdamDesc), _vp]
+    lib.tfa_adamw_state_values.argtypes = [_i64, _vp, _i32, _vp]
+    for name in EXPORTS:
+        if name.startswith(("tfa_linear_attention", "tfa_group_norm", "tfa_adamw")):
+            getattr(lib, name).restype = ctypes.c_int
     lib.tfa_last_error.argtypes = []
     lib.tfa_last_error.restype = ctypes.c_char_p
     lib.tfa_abi_version.argtypes = []

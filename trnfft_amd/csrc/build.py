@@ -31,6 +31,10 @@ SOURCES = [
     "kernels_smooth_stft.hip",
     "kernels_smooth_istft.hip",
     "kernels_smooth_c2c.hip",
+    "model_ops.hip",
+    "kernels_attention.hip",
+    "kernels_norm.hip",
+    "kernels_adamw.hip",
 ]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -1,0 +1,317 @@
+// Linear attention with a decay for each head.
+//
+//   S_t = gamma S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t,   gamma = exp(log_decay[h])
+//
+// Forward and gradients are one form, out_t = scale sum_s gamma^|t-s| (a_t . b_s) c_s, over s <= t or, with time
+// reversed, s >= t:
+//          a   b   c   order     state M = sum gamma^(..) b c^T
+//   o      q   k   v   forward   S            from S_0, ends as S_T
+//   dq     do  v   k   forward   S^T          from S_0^T
+//   dk     v   do  q   reversed  (dS)^T       from dS_T^T
+//   dv     k   q   do  reversed  dS           from dS_T, ends as dS_0
+// (forward, a state reaches token t with gamma^(t+1); reversed, dS_T reaches token s with gamma^(T-1-s): the decay
+// comes after the token instead of before it).  Scores, states and sums are fp32 whatever the inputs' type.
+//
+// The log decay's gradient is the sum over all pairs of lag * flow; forward in time it is carried by the tangent
+// dM/dg: M' <- gamma (M' + M), with each token's out contribution a M' . x (the dq pass, x = q), and M' . dS_T^T at
+// the end.  All its terms have their true lags as weights, so nothing cancels that does not cancel in the sum itself.
+#include "model_ops.h"
+
+namespace tfa {
+
+// gamma as a sum of two fp32: powers of it over a long memory keep fp32's precision (a rounded gamma of a memory of
+// 256 tokens would be off by 256 half ulps, 8e-6).
+struct Decay {
+  float hi, lo;
+  __device__ __forceinline__ explicit Decay(double x) : hi((float)x), lo((float)(x - (double)(float)x)) {}
+  __device__ __forceinline__ float times(float m) const { return __builtin_fmaf(m, hi, m * lo); }
+};
+
+// log decays of -inf (no memory) are taken as -1e5: gamma^0 stays 1 and every other power is 0
+__device__ __forceinline__ float log_decay_of(const float* g, int h) { return fmaxf(g[h], -1e5f); }
+
+template <typename T>
+__device__ __forceinline__ const T* head_base(const HeadsView& v, long long b, int h) {
+  return static_cast<const T*>(v.p) + b * v.sb + (long long)(h / v.group) * v.sh;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Token by token.  A workgroup carries 32 columns of one head's state: thread (column, row group) holds RPT rows of
+// its column in registers, 16 tokens are staged in LDS at a time, and the row groups' parts of the outputs are
+// joined once per 16 tokens.  Bound by the fp32 FMAs (3 a state element and token, 6 with the tangent).
+// ------------------------------------------------------------------------------------------------
+
+constexpr int kScanCols = 32, kScanGroups = 8, kScanTokens = 16;
+
+template <typename T, int RPT, bool TANGENT>
+__global__ __launch_bounds__(256) void attn_scan_kernel(AttnPass p, int slices) {
+  constexpr int R = RPT * kScanGroups;
+  __shared__ float sa[kScanTokens][R], sb[kScanTokens][R], sc[kScanTokens][kScanCols], sx[kScanTokens][kScanCols];
+  __shared__ float part[kScanTokens][kScanGroups][kScanCols];
+  const int t = threadIdx.x, col = t % kScanCols, rg = t / kScanCols;
+  const int slice = blockIdx.x % slices;
+  const long long bh = blockIdx.x / slices, b = bh / p.heads;
+  const int h = (int)(bh % p.heads), n = slice * kScanCols + col;
+  const long long len = p.lengths ? min(max(p.lengths[b], 0LL), p.tokens) : p.tokens;
+  const T* A = head_base<T>(p.a, b, h);
+  const T* B = head_base<T>(p.b, b, h);
+  const T* C = head_base<T>(p.c, b, h);
+  const T* X = TANGENT ? head_base<T>(p.x, b, h) : nullptr;
+  const Decay gamma(exp((double)log_decay_of(p.log_decay, h)));
+  const long long m0 = bh * p.rows * p.cols;
+
+  float m[RPT], tm[RPT];
+#pragma unroll
+  for (int j = 0; j < RPT; ++j) {
+    const int r = rg + kScanGroups * j;
+    m[j] = p.m_in && r < p.rows && n < p.cols ? p.m_in[m0 + r * p.m_r + n * p.m_n] * p.m_in_scale : 0.0f;
+    tm[j] = 0.0f;
+  }
+  double dg = 0.0;
+  const long long o_t = (long long)p.heads * p.cols, o0 = b * p.tokens * o_t + (long long)h * p.cols;
+  for (long long t0 = 0; t0 < len; t0 += kScanTokens) {
+    const int count = (int)min((long long)kScanTokens, len - t0);
+    for (int i = t; i < kScanTokens * R; i += 256) {
+      const int k = i / R, r = i % R;
+      const bool in = k < count && r < p.rows;
+      const long long at = p.reverse ? len - 1 - t0 - k : t0 + k;
+      sa[k][r] = in ? to_f32(A[at * p.a.st + r]) : 0.0f;
+      sb[k][r] = in ? to_f32(B[at * p.b.st + r]) : 0.0f;
+    }
+    for (int i = t; i < kScanTokens * kScanCols; i += 256) {
+      const int k = i / kScanCols, cn = slice * kScanCols + i % kScanCols;
+      const bool in = k < count && cn < p.cols;
+      const long long at = p.reverse ? len - 1 - t0 - k : t0 + k;
+      sc[k][i % kScanCols] = in ? to_f32(C[at * p.c.st + cn]) : 0.0f;
+      if (TANGENT) sx[k][i % kScanCols] = in ? to_f32(X[at * p.x.st + cn]) : 0.0f;
+    }
+    __syncthreads();
+    float dgt = 0.0f;
+    for (int k = 0; k < count; ++k) {
+      const float c = sc[k][col];
+      float acc = 0.0f, tacc = 0.0f;
+#pragma unroll
+      for (int j = 0; j < RPT; ++j) {
+        const float a = sa[k][rg + kScanGroups * j], bb = sb[k][rg + kScanGroups * j];
+        if (TANGENT) {
+          tm[j] = gamma.times(tm[j] + m[j]);
+          tacc = __builtin_fmaf(a, tm[j], tacc);
+        }
+        if (p.reverse) {
+          m[j] = __builtin_fmaf(bb, c, m[j]);
+          acc = __builtin_fmaf(a, m[j], acc);
+          m[j] = gamma.times(m[j]);
+        } else {
+          m[j] = __builtin_fmaf(bb, c, gamma.times(m[j]));
+          acc = __builtin_fmaf(a, m[j], acc);
+        }
+      }
+      part[k][rg][col] = acc;
+      if (TANGENT) dgt = __builtin_fmaf(tacc, sx[k][col], dgt);
+    }
+    if (TANGENT) dg += (double)dgt * (double)p.scale;
+    __syncthreads();
+    for (int k = rg; k < count; k += kScanGroups) {
+      float s = 0.0f;
+#pragma unroll
+      for (int g = 0; g < kScanGroups; ++g) s += part[k][g][col];
+      const long long at = p.reverse ? len - 1 - t0 - k : t0 + k;
+      if (n < p.cols) {
+        if (p.out_f32)
+          static_cast<float*>(p.out)[o0 + at * o_t + n] = s * p.scale;
+        else
+          static_cast<T*>(p.out)[o0 + at * o_t + n] = from_f32<T>(s * p.scale);
+      }
+    }
+  }
+  // padding: nothing was read there, and its outputs are zeros
+  for (long long at = len + rg; at < p.tokens; at += kScanGroups)
+    if (n < p.cols) {
+      if (p.out_f32)
+        static_cast<float*>(p.out)[o0 + at * o_t + n] = 0.0f;
+      else
+        static_cast<T*>(p.out)[o0 + at * o_t + n] = from_f32<T>(0.0f);
+    }
+#pragma unroll
+  for (int j = 0; j < RPT; ++j) {
+    const int r = rg + kScanGroups * j;
+    if (r < p.rows && n < p.cols) {
+      if (p.m_out) p.m_out[m0 + r * p.m_r + n * p.m_n] = m[j] * p.m_out_scale;
+      if (TANGENT && p.m_sink) dg += (double)tm[j] * (double)p.m_sink[m0 + r * p.m_r + n * p.m_n];
+    }
+  }
+  if (TANGENT) {
+    __shared__ double sum[256];
+    sum[t] = dg;
+    __syncthreads();
+    for (int s = 128; s > 0; s /= 2) {
+      if (t < s) sum[t] += sum[t + s];
+      __syncthreads();
+    }
+    if (t == 0) p.dg_part[blockIdx.x] = sum[0];
+  }
+}
+
+int attn_dg_parts(const AttnPass& p) { return (p.cols + kScanCols - 1) / kScanCols; }
+
+template <typename T, int RPT>
+static hipError_t scan_launch(const AttnPass& p) {
+  const int slices = (p.cols + kScanCols - 1) / kScanCols;
+  const dim3 grid((unsigned)(p.batch * p.heads * slices)), block(256);
+  if (p.dg_part)
+    hipLaunchKernelGGL((attn_scan_kernel<T, RPT, true>), grid, block, 0, p.stream, p, slices);
+  else
+    hipLaunchKernelGGL((attn_scan_kernel<T, RPT, false>), grid, block, 0, p.stream, p, slices);
+  return hipGetLastError();
+}
+
+template <typename T>
+static hipError_t scan_rows(const AttnPass& p) {
+  if (p.rows <= 8 * kScanGroups) return scan_launch<T, 8>(p);
+  return p.rows <= 16 * kScanGroups ? scan_launch<T, 16>(p) : scan_launch<T, 32>(p);
+}
+
+hipError_t launch_attn_scan(const AttnPass& p) {
+  if (p.dtype == 0) return scan_rows<float>(p);
+  return p.dtype == 1 ? scan_rows<__bf16>(p) : scan_rows<_Float16>(p);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Sums of the gradients' parts, in a fixed order.
+// ------------------------------------------------------------------------------------------------
+
+__global__ __launch_bounds__(256) void attn_dg_sum_kernel(const double* __restrict__ parts, float* __restrict__ out,
+                                                          long long batch, int heads, int each) {
+  __shared__ double sum[256];
+  const int h = blockIdx.x, t = threadIdx.x;
+  double s = 0.0;
+  for (long long i = t; i < batch * each; i += 256) s += parts[((i / each) * heads + h) * each + i % each];
+  sum[t] = s;
+  __syncthreads();
+  for (int k = 128; k > 0; k /= 2) {
+    if (t < k) sum[t] += sum[t + k];
+    __syncthreads();
+  }
+  if (t == 0) out[h] = (float)sum[0];
+}
+
+hipError_t launch_attn_dg_sum(const double* parts, float* out, long long batch, int heads, int each,
+                              hipStream_t stream) {
+  hipLaunchKernelGGL(attn_dg_sum_kernel, dim3(heads), dim3(256), 0, stream, parts, out, batch, heads, each);
+  return hipGetLastError();
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void attn_head_sum_kernel(const float* __restrict__ in, T* __restrict__ out,
+                                                            long long total, int group, int d) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const float* src = in + (i / d) * group * d + i % d;
+  float s = 0.0f;
+  for (int g = 0; g < group; ++g) s += src[(long long)g * d];
+  out[i] = from_f32<T>(s);
+}
+
+hipError_t launch_attn_head_sum(const float* in, void* out, int dtype, long long rows, int heads_out, int group, int d,
+                                hipStream_t stream) {
+  const long long total = rows * heads_out * d;
+  const dim3 grid((unsigned)((total + 255) / 256)), block(256);
+  if (dtype == 0)
+    hipLaunchKernelGGL((attn_head_sum_kernel<float>), grid, block, 0, stream, in, static_cast<float*>(out), total, group, d);
+  else if (dtype == 1)
+    hipLaunchKernelGGL((attn_head_sum_kernel<__bf16>), grid, block, 0, stream, in, static_cast<__bf16*>(out), total, group, d);
+  else
+    hipLaunchKernelGGL((attn_head_sum_kernel<_Float16>), grid, block, 0, stream, in, static_cast<_Float16*>(out), total, group, d);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------
+// One token of every stream: S <- gamma S + k v^T in place, o = scale S^T q.  Bound by reading and writing the states
+// (8 bytes an element).  A workgroup takes 32 columns: 8 lanes of four columns, 32 row groups of 4 rows a pass.
+// ------------------------------------------------------------------------------------------------
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void attn_step_kernel(AttnStep p, int slices) {
+  __shared__ float part[4][32];
+  const int t = threadIdx.x, c4 = t % 8, rg = t / 8, wave = t / 64;
+  const int slice = blockIdx.x % slices;
+  const long long bh = blockIdx.x / slices, b = bh / p.heads;
+  const int h = (int)(bh % p.heads), n = slice * 32 + c4 * 4;
+  const T* q = static_cast<const T*>(p.q) + b * p.q_sb + (long long)(h / p.q_group) * p.q_sh;
+  const T* k = static_cast<const T*>(p.k) + b * p.k_sb + (long long)(h / p.k_group) * p.k_sh;
+  const T* v = static_cast<const T*>(p.v) + b * p.v_sb + (long long)(h / p.v_group) * p.v_sh;
+  float* S = p.state + bh * p.rows * p.cols;
+  const float gamma = expf(log_decay_of(p.log_decay, h));
+  float vv[4], acc[4] = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) vv[j] = n + j < p.cols ? to_f32(v[n + j]) : 0.0f;
+  for (int r0 = 0; r0 < p.rows; r0 += 128) {
+    float s[4][4], qr[4], kr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + rg + 32 * i;
+      const bool in = r < p.rows;
+      qr[i] = in ? to_f32(q[r]) : 0.0f;
+      kr[i] = in ? to_f32(k[r]) : 0.0f;
+      const float* src = S + (long long)r * p.cols + n;
+      if (VEC) {
+        const float4 x = in && n < p.cols ? *reinterpret_cast<const float4*>(src) : make_float4(0, 0, 0, 0);
+        s[i][0] = x.x; s[i][1] = x.y; s[i][2] = x.z; s[i][3] = x.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = in && n + j < p.cols ? src[j] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + rg + 32 * i;
+      float* dst = S + (long long)r * p.cols + n;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = __builtin_fmaf(kr[i], vv[j], gamma * s[i][j]);
+        acc[j] = __builtin_fmaf(qr[i], s[i][j], acc[j]);
+      }
+      if (r < p.rows) {
+        if (VEC) {
+          if (n < p.cols) *reinterpret_cast<float4*>(dst) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < p.cols) dst[j] = s[i][j];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int o = 8; o < 64; o *= 2) acc[j] += __shfl_xor(acc[j], o);
+    if (t % 64 < 8) part[wave][c4 * 4 + j] = acc[j];
+  }
+  __syncthreads();
+  if (t < 32 && slice * 32 + t < p.cols)
+    static_cast<T*>(p.out)[bh * p.cols + slice * 32 + t] =
+        from_f32<T>((part[0][t] + part[1][t] + part[2][t] + part[3][t]) * p.scale);
+}
+
+template <typename T>
+static void step_launch(const AttnStep& p) {
+  const int slices = (p.cols + 31) / 32;
+  const dim3 grid((unsigned)(p.batch * p.heads * slices)), block(256);
+  if (p.cols % 4 == 0 && reinterpret_cast<uintptr_t>(p.state) % 16 == 0)
+    hipLaunchKernelGGL((attn_step_kernel<T, true>), grid, block, 0, p.stream, p, slices);
+  else
+    hipLaunchKernelGGL((attn_step_kernel<T, false>), grid, block, 0, p.stream, p, slices);
+}
+
+hipError_t launch_attn_step(const AttnStep& p) {
+  if (p.dtype == 0)
+    step_launch<float>(p);
+  else if (p.dtype == 1)
+    step_launch<__bf16>(p);
+  else
+    step_launch<_Float16>(p);
+  return hipGetLastError();
+}
+
+}  // namespace tfa

@@ -1,0 +1,144 @@
+// Operators of models on frames: decayed linear attention, group norm with an activation, AdamW steps.
+// Argument blocks and launch functions shared by the kernels (kernels_attention.hip, kernels_norm.hip,
+// kernels_adamw.hip) and their C entry points (model_ops.hip).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace tfa {
+
+// Sets the calling thread's error text (tfa_last_error) and returns `code`; never throws.
+int set_error(int code, const char* text) noexcept;
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x) {
+  return static_cast<float>(x);
+}
+template <>
+__device__ __forceinline__ float to_f32<__bf16>(__bf16 x) {
+  return __uint_as_float((unsigned)__builtin_bit_cast(unsigned short, x) << 16);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float x) {
+  return static_cast<T>(x);  // to nearest, ties to even
+}
+
+// ------------------------------------------------------------------------------------------------
+// decayed linear attention
+// ------------------------------------------------------------------------------------------------
+
+// (batch, token, head, feature) operand: strides in elements, features contiguous; head h of the call reads h / group
+struct HeadsView {
+  const void* p;
+  long long sb, st, sh;
+  int group;
+};
+
+// One pass  out_t = scale (sum_s gamma^|t-s| (a_t . b_s) c_s + gamma^(..) a_t M_in)  over s <= t, or s >= t when
+// `reverse`; M is the (R, N) state sum_s gamma^(..) b_s c_s^T that the pass carries.  The forward of the attention and
+// each of its gradients is one such pass (the table is in kernels_attention.hip).
+struct AttnPass {
+  HeadsView a, b, c;
+  int rows, cols;  // R: features of a and b, N: features of c
+  bool reverse;
+  int dtype;
+  long long batch, tokens;
+  int heads;
+  const float* log_decay;      // (heads)
+  const long long* lengths;    // (batch) or nullptr: tokens at and past it are padding
+  const float* m_in;           // (batch, heads, ...) or nullptr; element (r, n) at r * m_r + n * m_n
+  float* m_out;                // or nullptr; laid out as m_in, must not alias it
+  long long m_r, m_n;
+  float m_in_scale, m_out_scale;
+  void* out;                   // (batch, tokens, heads, N), fp32 where out_f32, else `dtype`
+  bool out_f32;
+  float scale;
+  // tangent pass (the decays' gradient): x (batch, token, head, N), per workgroup
+  //   dg_part[..] = sum over pairs of lag * flow into out . x, and into m_sink (as m_in) where there is one
+  HeadsView x;
+  const float* m_sink;
+  double* dg_part;             // attn_dg_parts(pass) values for each (batch, head)
+  hipStream_t stream;
+};
+
+int attn_dg_parts(const AttnPass& p);
+hipError_t launch_attn_scan(const AttnPass& p);
+// dlog_decay[h] = sum over batch and parts
+hipError_t launch_attn_dg_sum(const double* parts, float* out, long long batch, int heads, int each, hipStream_t stream);
+// out (rows, heads_out, d) of `dtype` = sums of `group` neighbouring heads of (rows, heads_out * group, d) fp32
+hipError_t launch_attn_head_sum(const float* in, void* out, int dtype, long long rows, int heads_out, int group, int d,
+                                hipStream_t stream);
+
+struct AttnStep {
+  const void *q, *k, *v;  // (batch, q_heads, rows), (batch, k_heads, rows), (batch, v_heads, cols)
+  long long q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;
+  int q_group, k_group, v_group;
+  int rows, cols, heads, dtype;
+  long long batch;
+  const float* log_decay;
+  float* state;  // (batch, heads, rows, cols)
+  void* out;     // (batch, heads, cols)
+  float scale;
+  hipStream_t stream;
+};
+hipError_t launch_attn_step(const AttnStep& p);
+
+// ------------------------------------------------------------------------------------------------
+// group norm with an activation, channels last
+// ------------------------------------------------------------------------------------------------
+
+struct NormArgs {
+  const void* x;  // (batch, positions, channels)
+  const void* dy;
+  void* y;        // forward: y; backward: dx
+  const float* weight;  // or nullptr: 1
+  const float* bias;    // or nullptr: 0
+  float* mean;    // (batch, groups)
+  float* rstd;
+  float* dweight;  // backward, or nullptr
+  float* dbias;
+  const long long* lengths;  // (batch) or nullptr: positions at and past lengths[n] * inner are padding
+  long long batch, positions, inner;
+  int channels, groups, act, dtype;
+  float eps;
+  float* ws;  // norm_workspace_bytes
+  hipStream_t stream;
+};
+size_t norm_workspace_bytes(const NormArgs& a, bool backward);
+hipError_t launch_norm_forward(const NormArgs& a);
+hipError_t launch_norm_backward(const NormArgs& a);
+
+// ------------------------------------------------------------------------------------------------
+// AdamW over many tensors
+// ------------------------------------------------------------------------------------------------
+
+struct AdamTensor {
+  void* p;
+  const void* g;
+  void* m;         // fp32, or int8 codes
+  void* v;         // fp32, or uint8 codes
+  float* m_scale;  // 8 bits: one per block of 256
+  float* v_scale;
+  float* master;   // or nullptr
+  long long n;
+};
+struct AdamArgs {
+  int p_dtype, g_dtype, bits;
+  float decay;             // 1 - lr * weight_decay
+  float beta1, one_beta1, beta2, one_beta2;
+  float step_size;         // lr / (1 - beta1^step)
+  float root_bc2, eps;     // sqrt(1 - beta2^step)
+};
+hipError_t launch_adamw(const AdamTensor* tensors, long long count, const AdamArgs& a, hipStream_t stream);
+// out[i] = the values that 8-bit codes stand for (second moments where `squares`)
+struct CodeTensor {
+  const void* codes;
+  const float* scales;
+  float* out;
+  long long n;
+};
+hipError_t launch_adam_values(const CodeTensor* tensors, long long count, bool squares, hipStream_t stream);
+
+}  // namespace tfa

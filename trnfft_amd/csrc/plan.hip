@@ -12,6 +12,7 @@
 
 #include "../../include/trnfft_amd.h"
 #include "kernels.h"
+#include "model_ops.h"
 #include "smooth.h"
 
 using tfa::LdsShape;
@@ -461,6 +462,16 @@ int scratch_setup(int dev) {
 }
 
 }  // namespace
+
+namespace tfa {
+int set_error(int code, const char* text) noexcept {
+  try {
+    g_last_error = text;
+  } catch (...) {  // no memory for the text: the code still says what failed
+  }
+  return code;
+}
+}  // namespace tfa
 
 extern "C" {
 
