@@ -33,6 +33,7 @@ SOURCES = [
     "kernels_smooth_c2c.hip",
     "model_ops.hip",
     "kernels_attention.hip",
+    "kernels_attention_blocks.hip",
     "kernels_norm.hip",
     "kernels_adamw.hip",
 ]

@@ -15,25 +15,9 @@
 // The log decay's gradient is the sum over all pairs of lag * flow; forward in time it is carried by the tangent
 // dM/dg: M' <- gamma (M' + M), with each token's out contribution a M' . x (the dq pass, x = q), and M' . dS_T^T at
 // the end.  All its terms have their true lags as weights, so nothing cancels that does not cancel in the sum itself.
-#include "model_ops.h"
+#include "attention_device.h"
 
 namespace tfa {
-
-// gamma as a sum of two fp32: powers of it over a long memory keep fp32's precision (a rounded gamma of a memory of
-// 256 tokens would be off by 256 half ulps, 8e-6).
-struct Decay {
-  float hi, lo;
-  __device__ __forceinline__ explicit Decay(double x) : hi((float)x), lo((float)(x - (double)(float)x)) {}
-  __device__ __forceinline__ float times(float m) const { return __builtin_fmaf(m, hi, m * lo); }
-};
-
-// log decays of -inf (no memory) are taken as -1e5: gamma^0 stays 1 and every other power is 0
-__device__ __forceinline__ float log_decay_of(const float* g, int h) { return fmaxf(g[h], -1e5f); }
-
-template <typename T>
-__device__ __forceinline__ const T* head_base(const HeadsView& v, long long b, int h) {
-  return static_cast<const T*>(v.p) + b * v.sb + (long long)(h / v.group) * v.sh;
-}
 
 // ------------------------------------------------------------------------------------------------
 // Token by token.  A workgroup carries 32 columns of one head's state: thread (column, row group) holds RPT rows of
@@ -52,7 +36,7 @@ __global__ __launch_bounds__(256) void attn_scan_kernel(AttnPass p, int slices) 
   const int slice = blockIdx.x % slices;
   const long long bh = blockIdx.x / slices, b = bh / p.heads;
   const int h = (int)(bh % p.heads), n = slice * kScanCols + col;
-  const long long len = p.lengths ? min(max(p.lengths[b], 0LL), p.tokens) : p.tokens;
+  const long long len = live_tokens(p, b);
   const T* A = head_base<T>(p.a, b, h);
   const T* B = head_base<T>(p.b, b, h);
   const T* C = head_base<T>(p.c, b, h);
@@ -152,7 +136,7 @@ __global__ __launch_bounds__(256) void attn_scan_kernel(AttnPass p, int slices) 
   }
 }
 
-int attn_dg_parts(const AttnPass& p) { return (p.cols + kScanCols - 1) / kScanCols; }
+int attn_scan_dg_parts(const AttnPass& p) { return (p.cols + kScanCols - 1) / kScanCols; }
 
 template <typename T, int RPT>
 static hipError_t scan_launch(const AttnPass& p) {

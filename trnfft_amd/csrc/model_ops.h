@@ -59,12 +59,24 @@ struct AttnPass {
   //   dg_part[..] = sum over pairs of lag * flow into out . x, and into m_sink (as m_in) where there is one
   HeadsView x;
   const float* m_sink;
-  double* dg_part;             // attn_dg_parts(pass) values for each (batch, head)
+  double* dg_part;             // attn_*_dg_parts(pass) values for each (batch, head)
+  // A long sequence in segments of seg_tokens (a multiple of 64), each a workgroup of its own: seg_state (segments,
+  // batch, heads, ...) are the states they start from, laid out as m_in.  out = nullptr: writes the segments' own sums there.
+  int segments;
+  long long seg_tokens;
+  float* seg_state;
+  const float* seg_sink;       // with a tangent: the gradient of the state after each segment, over `scale`
   hipStream_t stream;
 };
 
-int attn_dg_parts(const AttnPass& p);
+// token by token (any dimensions up to 256)
 hipError_t launch_attn_scan(const AttnPass& p);
+int attn_scan_dg_parts(const AttnPass& p);
+// in blocks of tokens on the matrix cores: dimensions up to 128, token strides of 0 to 2^24 - 1 elements
+int attn_blocks_dg_parts(const AttnPass& p);
+hipError_t launch_attn_blocks(const AttnPass& p);
+// the states that segments of a long sequence start from, p.seg_state, from the segments' own sums: in place
+hipError_t launch_attn_join(const AttnPass& p);
 // dlog_decay[h] = sum over batch and parts
 hipError_t launch_attn_dg_sum(const double* parts, float* out, long long batch, int heads, int each, hipStream_t stream);
 // out (rows, heads_out, d) of `dtype` = sums of `group` neighbouring heads of (rows, heads_out * group, d) fp32

@@ -1,6 +1,7 @@
 // C entry points of the operators of models on frames (include/trnfft_amd.h): argument checks, workspaces, launches.
 #include "model_ops.h"
 
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/trnfft_amd.h"
@@ -62,21 +63,77 @@ tfa::AttnPass pass_of(const tfa_attn_desc* d, const float* log_decay, const int6
   return p;
 }
 
+// Sequences of up to kScanTokens go token by token, longer ones in blocks on the matrix cores.
+constexpr int64_t kScanTokens = 16;
+// A long sequence is cut into segments where batch * heads alone leave compute units idle: about kWantBlocks
+// workgroups in all, segments of at least kSegTokens.
+constexpr int64_t kWantBlocks = 512, kSegTokens = 128;
+
+struct Plan {
+  bool blocks;
+  int segments;
+  int64_t seg_tokens;
+  size_t state_bytes;  // of the segments' states
+};
+
+Plan plan_of(const tfa_attn_desc* d) {
+  Plan plan{false, 1, std::max<int64_t>(1, (d->tokens + 63) / 64 * 64), 0};
+  plan.blocks = d->tokens > kScanTokens && d->key_dim <= 128 && d->value_dim <= 128;
+  for (const int64_t* stride : {d->q_stride, d->k_stride, d->v_stride})  // (32-bit offsets inside a block of tokens)
+    if (stride[1] < 0 || stride[1] >= (1 << 24)) plan.blocks = false;
+  if ((int64_t)d->heads * std::max(d->key_dim, d->value_dim) >= (1 << 24)) plan.blocks = false;
+  if (!plan.blocks || d->batch == 0) return plan;
+  const int64_t rows = d->batch * d->heads;
+  const int64_t want = std::min((kWantBlocks + rows - 1) / rows, d->tokens / kSegTokens);
+  if (want > 1) {
+    plan.seg_tokens = ((d->tokens + want - 1) / want + 63) / 64 * 64;
+    plan.segments = (int)((d->tokens + plan.seg_tokens - 1) / plan.seg_tokens);
+    plan.state_bytes = align256((size_t)plan.segments * rows * d->key_dim * d->value_dim * sizeof(float));
+  }
+  return plan;
+}
+
+hipError_t run_pass(tfa::AttnPass p, const Plan& plan, float* states) {
+  p.segments = plan.segments;
+  p.seg_tokens = plan.seg_tokens;
+  p.seg_state = states;
+  return plan.blocks ? tfa::launch_attn_blocks(p) : tfa::launch_attn_scan(p);
+}
+
+// the states that a pass's segments start from
+hipError_t segment_states(tfa::AttnPass p, const Plan& plan, float* states) {
+  if (plan.segments == 1) return hipSuccess;
+  p.out = nullptr;
+  p.dg_part = nullptr;
+  const hipError_t e = run_pass(p, plan, states);
+  if (e != hipSuccess) return e;
+  p.segments = plan.segments;
+  p.seg_tokens = plan.seg_tokens;
+  p.seg_state = states;
+  return tfa::launch_attn_join(p);
+}
+
 struct BackwardSpace {
   size_t dq = 0, dk = 0, dv = 0, dg = 0, total = 0;  // offsets; gradients of shared heads before their sum
+  size_t states = 0, grad_states = 0;
   int dg_each = 0;
+  Plan plan;
 };
 
 BackwardSpace backward_space(const tfa_attn_desc* d) {
   BackwardSpace s;
+  s.plan = plan_of(d);
   const size_t rows = (size_t)d->batch * d->tokens * d->heads * sizeof(float);
   if (d->q_heads != d->heads) s.dq = s.total, s.total += align256(rows * d->key_dim);
   if (d->k_heads != d->heads) s.dk = s.total, s.total += align256(rows * d->key_dim);
   if (d->v_heads != d->heads) s.dv = s.total, s.total += align256(rows * d->value_dim);
+  s.states = s.total, s.total += s.plan.state_bytes;
+  s.grad_states = s.total, s.total += s.plan.state_bytes;
   tfa::AttnPass p{};
   p.rows = d->value_dim;
   p.cols = d->key_dim;
-  s.dg_each = tfa::attn_dg_parts(p);
+  p.segments = s.plan.segments;
+  s.dg_each = s.plan.blocks ? tfa::attn_blocks_dg_parts(p) : tfa::attn_scan_dg_parts(p);
   s.dg = s.total;
   s.total += align256((size_t)d->batch * d->heads * s.dg_each * sizeof(double));
   return s;
@@ -90,7 +147,7 @@ int tfa_linear_attention_workspace_size(const tfa_attn_desc* desc, int32_t backw
   if (!bytes) return set_error(TFA_ERR_INVALID, "null bytes pointer");
   *bytes = 0;
   if (const int rc = check_heads(desc)) return rc;
-  if (backward) *bytes = backward_space(desc).total;
+  *bytes = backward ? backward_space(desc).total : plan_of(desc).state_bytes;
   return TFA_OK;
 }
 
@@ -98,7 +155,6 @@ int tfa_linear_attention(const tfa_attn_desc* desc, const void* q, const void* k
                          const int64_t* lengths, const float* state_in, void* out, float* state_out, void* workspace,
                          tfa_stream stream) {
   if (const int rc = check_heads(desc)) return rc;
-  (void)workspace;
   if (desc->batch == 0) return TFA_OK;
   if (!log_decay || (desc->tokens > 0 && (!q || !k || !v || !out))) return set_error(TFA_ERR_INVALID, "null data pointer");
   if (state_out && state_out == state_in) return set_error(TFA_ERR_INVALID, "state_out must not be state_in");
@@ -113,7 +169,11 @@ int tfa_linear_attention(const tfa_attn_desc* desc, const void* q, const void* k
   p.m_r = desc->value_dim;
   p.m_n = 1;
   p.out = out;
-  return launched(tfa::launch_attn_scan(p), "linear attention");
+  const Plan plan = plan_of(desc);
+  if (plan.state_bytes && !workspace) return set_error(TFA_ERR_INVALID, "null workspace");
+  float* states = static_cast<float*>(workspace);
+  if (const hipError_t e = segment_states(p, plan, states)) return launched(e, "segments");
+  return launched(run_pass(p, plan, states), "linear attention");
 }
 
 int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, const void* k, const void* v,
@@ -133,6 +193,37 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
   const long long rows = (long long)d.batch * d.tokens;
   const tfa::HeadsView qv = view(q, d.q_stride, d.heads, d.q_heads), kv = view(k, d.k_stride, d.heads, d.k_heads),
                        vv = view(v, d.v_stride, d.heads, d.v_heads), gv = dense(grad_out, desc, d.value_dim);
+  const Plan& plan = space.plan;
+  float* states = reinterpret_cast<float*>(ws + space.states);
+  float* grad_states = reinterpret_cast<float*>(ws + space.grad_states);
+  // the value gradient's pass; its states are those of the key gradient too, and where the decays' tangent ends
+  tfa::AttnPass pv = pass_of(desc, log_decay, lengths, stream);
+  pv.a = kv;
+  pv.b = qv;
+  pv.c = gv;
+  pv.rows = d.key_dim;
+  pv.cols = d.value_dim;
+  pv.reverse = true;
+  pv.m_in = grad_state_out;
+  pv.m_out = grad_state_in;
+  pv.m_in_scale = 1.0f / d.scale;
+  pv.m_out_scale = d.scale;
+  pv.m_r = d.value_dim;
+  pv.m_n = 1;
+  if (d.batch > 0 && plan.segments > 1) {
+    if (const hipError_t e = segment_states(pv, plan, grad_states)) return launched(e, "gradient segments");
+    if (grad_q || grad_log_decay) {
+      tfa::AttnPass p = pass_of(desc, log_decay, lengths, stream);
+      p.b = kv;
+      p.c = vv;
+      p.rows = d.key_dim;
+      p.cols = d.value_dim;
+      p.m_in = state_in;
+      p.m_r = d.value_dim;
+      p.m_n = 1;
+      if (const hipError_t e = segment_states(p, plan, states)) return launched(e, "segments");
+    }
+  }
   if (d.batch > 0 && (grad_q || grad_log_decay)) {
     tfa::AttnPass p = pass_of(desc, log_decay, lengths, stream);
     p.a = gv;
@@ -149,9 +240,10 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
     if (grad_log_decay) {
       p.x = qv;
       p.m_sink = grad_state_out;
+      p.seg_sink = grad_states;
       p.dg_part = parts;
     }
-    if (const hipError_t e = tfa::launch_attn_scan(p)) return launched(e, "query gradient");
+    if (const hipError_t e = run_pass(p, plan, states)) return launched(e, "query gradient");
     if (p.out_f32 && grad_q && rows)
       if (const hipError_t e = tfa::launch_attn_head_sum(reinterpret_cast<const float*>(ws + space.dq), grad_q, d.dtype, rows,
                                                          d.q_heads, d.heads / d.q_heads, d.key_dim, s))
@@ -175,30 +267,18 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
     p.m_n = d.value_dim;
     p.out_f32 = d.k_heads != d.heads;
     p.out = p.out_f32 ? ws + space.dk : grad_k;
-    if (const hipError_t e = tfa::launch_attn_scan(p)) return launched(e, "key gradient");
+    if (const hipError_t e = run_pass(p, plan, grad_states)) return launched(e, "key gradient");
     if (p.out_f32 && rows)
       if (const hipError_t e = tfa::launch_attn_head_sum(reinterpret_cast<const float*>(ws + space.dk), grad_k, d.dtype, rows,
                                                          d.k_heads, d.heads / d.k_heads, d.key_dim, s))
         return launched(e, "key gradient sum");
   }
   if (grad_v || grad_state_in) {
-    tfa::AttnPass p = pass_of(desc, log_decay, lengths, stream);
-    p.a = kv;
-    p.b = qv;
-    p.c = gv;
-    p.rows = d.key_dim;
-    p.cols = d.value_dim;
-    p.reverse = true;
-    p.m_in = grad_state_out;
-    p.m_out = grad_state_in;
-    p.m_in_scale = 1.0f / d.scale;
-    p.m_out_scale = d.scale;
-    p.m_r = d.value_dim;
-    p.m_n = 1;
+    tfa::AttnPass p = pv;
     p.out_f32 = d.v_heads != d.heads;
     p.out = p.out_f32 ? ws + space.dv : grad_v;
     if (!p.out) return set_error(TFA_ERR_INVALID, "grad_state_in needs grad_v");
-    if (const hipError_t e = tfa::launch_attn_scan(p)) return launched(e, "value gradient");
+    if (const hipError_t e = run_pass(p, plan, grad_states)) return launched(e, "value gradient");
     if (p.out_f32 && grad_v && rows)
       if (const hipError_t e = tfa::launch_attn_head_sum(reinterpret_cast<const float*>(ws + space.dv), grad_v, d.dtype, rows,
                                                          d.v_heads, d.heads / d.v_heads, d.value_dim, s))
