@@ -10,6 +10,8 @@
 // unrounded m and v for the parameter, and only then encodes.  Every operation is one IEEE fp32 operation in
 // the written order (no contraction): codes do not depend on the compiler.
 // Memory bound: 28 bytes a value with fp32 parameters and states, 16 with 8-bit states.
+#include <type_traits>
+
 #include "model_ops.h"
 
 #pragma clang fp contract(off)
@@ -27,17 +29,28 @@ struct AdamTable {
 };
 static_assert(sizeof(AdamTable) + sizeof(AdamArgs) <= 4000, "kernel arguments");
 
-__device__ __forceinline__ float load_as_f32(const void* p, int dtype, long long i) {
-  if (dtype == 0) return static_cast<const float*>(p)[i];
-  return dtype == 1 ? to_f32(static_cast<const __bf16*>(p)[i]) : to_f32(static_cast<const _Float16*>(p)[i]);
+// four consecutive values: one access where `whole` (aligned, all inside), else one by one below n
+template <typename T>
+struct __attribute__((aligned(4 * sizeof(T)))) Four {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ Four<T> load4(const T* p, long long i, long long n, bool whole) {
+  if (whole) return *reinterpret_cast<const Four<T>*>(p + i);
+  Four<T> x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x.v[j] = i + j < n ? p[i + j] : T(0);
+  return x;
 }
-__device__ __forceinline__ void store_from_f32(void* p, int dtype, long long i, float x) {
-  if (dtype == 0)
-    static_cast<float*>(p)[i] = x;
-  else if (dtype == 1)
-    static_cast<__bf16*>(p)[i] = from_f32<__bf16>(x);
-  else
-    static_cast<_Float16*>(p)[i] = from_f32<_Float16>(x);
+template <typename T>
+__device__ __forceinline__ void store4(T* p, long long i, long long n, bool whole, const Four<T>& x) {
+  if (whole) {
+    *reinterpret_cast<Four<T>*>(p + i) = x;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) p[i + j] = x.v[j];
+  }
 }
 
 __device__ __forceinline__ float code_value(int c, float top, float s, bool fourth) {
@@ -73,62 +86,120 @@ __device__ __forceinline__ int tensor_of(const unsigned* first, int count, unsig
 }
 
 template <int BITS>
+struct StateTypes {
+  typedef float M;
+  typedef float V;
+};
+template <>
+struct StateTypes<8> {
+  typedef signed char M;
+  typedef unsigned char V;
+};
+
+// A workgroup takes 4096 values of one tensor, a wave four blocks of 256, a lane four neighbours of each: 16-byte accesses
+// for fp32, all of a wave's loads ahead of its arithmetic.
+template <int BITS, typename P, typename G>
 __global__ __launch_bounds__(256) void adamw_kernel(AdamTable tab, AdamArgs a) {
+  typedef typename StateTypes<BITS>::M M;
+  typedef typename StateTypes<BITS>::V V;
+  constexpr int U = kAdamChunk / kQBlock / 4;
   const int k = tensor_of(tab.first, tab.count, blockIdx.x);
   const AdamTensor& t = tab.t[k];
-  const long long base = (long long)(blockIdx.x - tab.first[k]) * kAdamChunk;
+  const long long n = t.n, base = (long long)(blockIdx.x - tab.first[k]) * kAdamChunk;
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  for (int q = wave; q < kAdamChunk / kQBlock; q += 4) {
-    const long long start = base + (long long)q * kQBlock;
-    if (start >= t.n) break;
-    float ms = 0.0f, vs = 0.0f;
-    if (BITS == 8) ms = t.m_scale[start / kQBlock], vs = t.v_scale[start / kQBlock];
-    float mm[4], vv[4];
+  P* const tp = static_cast<P*>(t.p);
+  const G* const tg = static_cast<const G*>(t.g);
+  M* const tm = static_cast<M*>(t.m);
+  V* const tv = static_cast<V*>(t.v);
+  float* const master = t.master;
+  const uintptr_t odd = reinterpret_cast<uintptr_t>(tp) % (4 * sizeof(P)) | reinterpret_cast<uintptr_t>(tg) % (4 * sizeof(G)) |
+                        reinterpret_cast<uintptr_t>(tm) % (4 * sizeof(M)) | reinterpret_cast<uintptr_t>(tv) % (4 * sizeof(V)) |
+                        reinterpret_cast<uintptr_t>(master) % 16;
+  const bool whole = odd == 0 && base + kAdamChunk <= n;
+
+  Four<P> p4[U];
+  Four<float> w4[U];
+  Four<G> g4[U];
+  Four<M> m4[U];
+  Four<V> v4[U];
+  float ms[U], vs[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long start = base + (wave + 4 * u) * kQBlock, i = start + lane * 4;
+    if (master)
+      w4[u] = load4(master, i, n, whole);
+    else
+      p4[u] = load4(tp, i, n, whole);
+    g4[u] = load4(tg, i, n, whole);
+    m4[u] = load4(tm, i, n, whole);
+    v4[u] = load4(tv, i, n, whole);
+    ms[u] = vs[u] = 0.0f;
+    if (BITS == 8 && start < n) ms[u] = t.m_scale[start / kQBlock], vs[u] = t.v_scale[start / kQBlock];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long start = base + (wave + 4 * u) * kQBlock, i = start + lane * 4;
+    if (start >= n) break;
+    Four<float> mo, vo, po;
     unsigned top_m = 0, top_v = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const long long i = start + lane * 4 + j;
-      mm[j] = vv[j] = 0.0f;
-      if (i >= t.n) continue;
-      const float g = load_as_f32(t.g, a.g_dtype, i);
-      float m, v;
-      if (BITS == 8) {
-        m = code_value(static_cast<const signed char*>(t.m)[i], 127.0f, ms, false);
-        v = code_value(static_cast<const unsigned char*>(t.v)[i], 255.0f, vs, true);
-      } else {
-        m = static_cast<const float*>(t.m)[i];
-        v = static_cast<const float*>(t.v)[i];
-      }
+      const float g = to_f32(g4[u].v[j]);
+      float m = BITS == 8 ? code_value((int)m4[u].v[j], 127.0f, ms[u], false) : (float)m4[u].v[j];
+      float v = BITS == 8 ? code_value((int)v4[u].v[j], 255.0f, vs[u], true) : (float)v4[u].v[j];
       m = m * a.beta1 + g * a.one_beta1;
       v = v * a.beta2 + (g * g) * a.one_beta2;
-      float p = t.master ? t.master[i] : load_as_f32(t.p, a.p_dtype, i);
-      p = p * a.decay - a.step_size * (m / (sqrtf(v) / a.root_bc2 + a.eps));
-      if (t.master) t.master[i] = p;
-      store_from_f32(t.p, a.p_dtype, i, p);
-      if (BITS == 32) {
-        static_cast<float*>(t.m)[i] = m;
-        static_cast<float*>(t.v)[i] = v;
+      const float p = master ? w4[u].v[j] : to_f32(p4[u].v[j]);
+      po.v[j] = p * a.decay - a.step_size * (m / (sqrtf(v) / a.root_bc2 + a.eps));
+      mo.v[j] = m;
+      vo.v[j] = v;
+      if (i + j < n) {  // (past the end: nothing may enter the block's scale)
+        top_m = max(top_m, __float_as_uint(fabsf(m)));
+        top_v = max(top_v, __float_as_uint(fabsf(v)));
       }
-      mm[j] = m;
-      vv[j] = v;
-      top_m = max(top_m, __float_as_uint(fabsf(m)));
-      top_v = max(top_v, __float_as_uint(fabsf(v)));
     }
-    if (BITS == 8) {
+    if (master) store4(master, i, n, whole, po);
+    Four<P> pr;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) pr.v[j] = from_f32<P>(po.v[j]);
+    store4(tp, i, n, whole, pr);
+    if constexpr (BITS == 32) {
+      store4(tm, i, n, whole, mo);
+      store4(tv, i, n, whole, vo);
+    } else {
       const float sm = __uint_as_float(wave_max(top_m)), sv = __uint_as_float(wave_max(top_v));
+      Four<M> mc;
+      Four<V> vc;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const long long i = start + lane * 4 + j;
-        if (i >= t.n) continue;
-        static_cast<signed char*>(t.m)[i] = (signed char)value_code(mm[j], sm, 127.0f, false);
-        static_cast<unsigned char*>(t.v)[i] = (unsigned char)value_code(vv[j], sv, 255.0f, true);
+        mc.v[j] = (M)value_code(mo.v[j], sm, 127.0f, false);
+        vc.v[j] = (V)value_code(vo.v[j], sv, 255.0f, true);
       }
+      store4(tm, i, n, whole, mc);
+      store4(tv, i, n, whole, vc);
       if (lane == 0) {
         t.m_scale[start / kQBlock] = sm;
         t.v_scale[start / kQBlock] = sv;
       }
     }
   }
+}
+
+template <int BITS, typename P>
+static void adamw_typed(const AdamTable& tab, const AdamArgs& a, unsigned blocks, hipStream_t stream) {
+  if (a.g_dtype == a.p_dtype)
+    hipLaunchKernelGGL((adamw_kernel<BITS, P, P>), dim3(blocks), dim3(256), 0, stream, tab, a);
+  else
+    hipLaunchKernelGGL((adamw_kernel<BITS, P, float>), dim3(blocks), dim3(256), 0, stream, tab, a);
+}
+template <int BITS>
+static void adamw_bits(const AdamTable& tab, const AdamArgs& a, unsigned blocks, hipStream_t stream) {
+  if (a.p_dtype == 0)
+    hipLaunchKernelGGL((adamw_kernel<BITS, float, float>), dim3(blocks), dim3(256), 0, stream, tab, a);
+  else if (a.p_dtype == 1)
+    adamw_typed<BITS, __bf16>(tab, a, blocks, stream);
+  else
+    adamw_typed<BITS, _Float16>(tab, a, blocks, stream);
 }
 
 hipError_t launch_adamw(const AdamTensor* tensors, long long count, const AdamArgs& a, hipStream_t stream) {
@@ -152,9 +223,9 @@ hipError_t launch_adamw(const AdamTensor* tensors, long long count, const AdamAr
       break;
     }
     if (a.bits == 8)
-      hipLaunchKernelGGL(adamw_kernel<8>, dim3((unsigned)blocks), dim3(256), 0, stream, tab, a);
+      adamw_bits<8>(tab, a, (unsigned)blocks, stream);
     else
-      hipLaunchKernelGGL(adamw_kernel<32>, dim3((unsigned)blocks), dim3(256), 0, stream, tab, a);
+      adamw_bits<32>(tab, a, (unsigned)blocks, stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -174,9 +245,26 @@ __global__ __launch_bounds__(256) void adam_values_kernel(CodeTable tab) {
   const int k = tensor_of(tab.first, tab.count, blockIdx.x);
   const CodeTensor& t = tab.t[k];
   const long long base = (long long)(blockIdx.x - tab.first[k]) * kAdamChunk;
-  for (long long i = base + threadIdx.x; i < min(base + kAdamChunk, t.n); i += 256) {
-    const int c = SQUARES ? (int)static_cast<const unsigned char*>(t.codes)[i] : (int)static_cast<const signed char*>(t.codes)[i];
-    t.out[i] = code_value(c, SQUARES ? 255.0f : 127.0f, t.scales[i / kQBlock], SQUARES);
+  typedef typename StateTypes<8>::M S;
+  typedef typename StateTypes<8>::V U;
+  typedef std::conditional_t<SQUARES, U, S> Code;
+  const Code* codes = static_cast<const Code*>(t.codes);
+  const bool whole = base + kAdamChunk <= t.n && reinterpret_cast<uintptr_t>(codes) % 4 == 0 && reinterpret_cast<uintptr_t>(t.out) % 16 == 0;
+  Four<Code> c[4];
+  float s[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const long long i = base + u * 1024 + threadIdx.x * 4;
+    c[u] = load4(codes, i, t.n, whole);
+    s[u] = i < t.n ? t.scales[i / kQBlock] : 0.0f;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const long long i = base + u * 1024 + threadIdx.x * 4;
+    Four<float> x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.v[j] = code_value((int)c[u].v[j], SQUARES ? 255.0f : 127.0f, s[u], SQUARES);
+    store4(t.out, i, t.n, whole, x);
   }
 }
 
