@@ -52,7 +52,10 @@ def _scale(scale, key_dim: int, what: str) -> float:
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+    """x with contiguous features at a 16-byte boundary (x itself where it is so)."""
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _desc(q, k, v, heads: int, scale: float) -> _lib.AttnDesc:
@@ -97,7 +100,7 @@ class _LinearAttentionFn(torch.autograd.Function):
         desc = _desc(q, k, v, heads, ctx.scale)
         if g_out is None:
             g_out = q.new_zeros(*q.shape[:2], heads, v.shape[3])
-        g_out = g_out.contiguous()
+        g_out = _rows(g_out.contiguous())
         g_last = None if g_last is None else g_last.contiguous()
         # (the decays' gradient comes with the queries', the state's with the values')
         d_q = torch.empty(q.shape, dtype=q.dtype, device=dev) if need[0] or need[3] else None

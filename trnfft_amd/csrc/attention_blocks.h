@@ -1,0 +1,677 @@
+// Linear attention with decays in blocks of C tokens on the bf16 matrix cores: one pass (model_ops.h, AttnPass)
+//
+//   out_i = scale ( sum_{j <= i} gamma^(i-j) (a_i . b_j) c_j  +  gamma^(i+e) a_i M ),
+//   M    <- gamma^L M + sum_j gamma^(L-e-j) b_j c_j^T             i, j < L: places in the block, in the pass's order
+//
+// with e = 1 forward and 0 in a reversed pass (a state reaches its first token undecayed there).  The tangent pass carries
+// M' = dM/dg as well: M' <- gamma^L (M' + L M) + sum_j (L-1-j) gamma^(L-1-j) b_j c_j^T, and dg collects x_i against
+// scale ( sum_j (i-j) gamma^(i-j) (a_i . b_j) c_j + gamma^(i+1) a_i (M' + (i+1) M) ).
+//
+// A workgroup carries one head's state for 32 columns a wave, all R rows of them in registers (32 x 32 accumulators of
+// v_mfma_f32_32x32x16_bf16), through its tokens.  The accumulator layout (lane: column, register: row) is also the
+// layout of a matrix operand (lane: column or row, register: contraction) up to an exchange of index bits 2 and 3, so with the
+// rows that feed the product taken in that order (pi below) the state goes from accumulators to operands without leaving
+// the registers.  Of a 64-token block's three 32 x 32 score tiles each wave computes its share and leaves it in LDS, where
+// a and b were; a 32-token block's one tile is computed by every wave.  Outputs are computed transposed (lane: token), so
+// that decays by token are one factor a lane and stores are 16 bytes.
+//
+// Operands in LDS: a and b by token (contraction over features), b and c by feature (contraction over tokens); the next
+// block is on its way in registers while one is computed.
+//
+// Precision: operands are exact sums of bf16 pieces (bf16: 1, fp16: 2, fp32: 3).  Scores, states and decayed c's are split into
+// pieces to nearest as they enter a product: two for 16-bit outputs (2^-17, nothing beside their rounding), three for fp32
+// outputs and for what enters states.  Products of pieces i, j are taken where i + j is within the piece count, into fp32.
+#pragma once
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_device.h"
+
+namespace tfa {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16;
+
+__device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// two fp32 as N packed pairs of bf16 pieces
+template <int N>
+__device__ __forceinline__ void split_pair(float x, float y, unsigned (&p)[N]) {
+  floatx2 r = {x, y};
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    p[q] = __builtin_bit_cast(unsigned, __builtin_convertvector(r, bf16x2));
+    if (q + 1 < N) {
+      r[0] -= __uint_as_float(p[q] << 16);
+      r[1] -= __uint_as_float(p[q] & 0xffff0000u);
+    }
+  }
+}
+// eight fp32 as an operand of N pieces
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], uint4 (&out)[N]) {
+  unsigned p[4][N];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split_pair<N>(x[2 * i], x[2 * i + 1], p[i]);
+#pragma unroll
+  for (int q = 0; q < N; ++q) out[q] = make_uint4(p[0][q], p[1][q], p[2][q], p[3][q]);
+}
+
+// index bits 2 and 3 exchanged: the row that accumulator place m stands for
+__device__ __forceinline__ int pi(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
+
+// a value that the compiler takes as new: what follows from it is computed again, not kept in registers over a loop
+__device__ __forceinline__ unsigned opaque(unsigned x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+template <typename T>
+struct Kind;
+template <>
+struct Kind<__bf16> {
+  static constexpr int pieces = 1, block = 64, out_pieces = 2;
+};
+template <>
+struct Kind<_Float16> {
+  static constexpr int pieces = 2, block = 32, out_pieces = 2;
+};
+template <>
+struct Kind<float> {
+  static constexpr int pieces = 3, block = 32, out_pieces = 3;
+};
+
+// Modes of the kernel: a pass with its outputs, the same with the decays' tangent, or only the segments' own states
+enum { kPass = 0, kTangent = 1, kSums = 2 };
+
+// pieces of two neighbouring features, from their raw bits: packed (f, f + 1)
+template <typename T>
+__device__ __forceinline__ void pair_pieces(const unsigned* w, unsigned (&p)[Kind<T>::pieces]) {
+  if constexpr (sizeof(T) == 4)
+    split_pair<3>(__uint_as_float(w[0]), __uint_as_float(w[1]), p);
+  else if constexpr (Kind<T>::pieces == 2)
+    split_pair<2>((float)__builtin_bit_cast(_Float16, (u16)w[0]), (float)__builtin_bit_cast(_Float16, (u16)(w[0] >> 16)), p);
+  else
+    p[0] = w[0];
+}
+
+template <typename T, int RP, int NW, int MODE>
+struct Blocks {
+  static constexpr bool out = MODE != kSums, tangent = MODE == kTangent;
+  static constexpr int NP = Kind<T>::pieces, C = Kind<T>::block, J = Kind<T>::out_pieces;
+  static constexpr int CP = 32 * NW, threads = 64 * NW, TI = C / 32, RB = RP / 32;
+  static constexpr bool shared_scores = TI == 2;
+  static constexpr int PJ = tangent ? 3 : J;                    // pieces of a shared score
+  static constexpr int tiles = shared_scores ? (3 + NW - 1) / NW : 1;  // score tiles of a wave
+  static constexpr int W = sizeof(T) / 2;                       // dwords of two features
+  static constexpr int pitch_row = RP + 8, pitch_tok = C + 8;   // 16-bit units: rows start 4 banks apart, modulo 64
+  static constexpr int row_plane = C * pitch_row, b_plane = RP * pitch_tok, c_plane = CP * pitch_tok, s_plane = C * pitch_tok;
+  static constexpr int off_b = out ? NP * row_plane : 0, rows_end = 2 * off_b;
+  static constexpr int scores_end = out && shared_scores ? PJ * s_plane : 0;  // in the rows' place
+  static constexpr int off_bt = rows_end > scores_end ? rows_end : scores_end;
+  static constexpr int off_ct = off_bt + NP * b_plane, off_end = off_ct + NP * c_plane;
+  // tables: gamma^(i - j) by i - j + C (zero before C), gamma^(L - e - j) by j
+  static constexpr int bytes = off_end * 2 + 3 * C * 4;
+  static constexpr int V = 16 / sizeof(T), a_lanes = RP / V, a_rows = threads / a_lanes, a_passes = C / a_rows;
+  static_assert(C % a_rows == 0, "whole passes");
+  // an operand taken by feature pairs: lanes over the pairs, 8 tokens a thread and pass
+  template <int F>
+  struct Pairs {
+    static constexpr int lanes = F / 2, at_once = threads / lanes, passes = (C / 8 + at_once - 1) / at_once;
+    static constexpr bool partial = C / 8 < at_once;  // some threads have no tokens
+    unsigned w[passes][8][W];
+  };
+};
+
+template <typename T, int RP, int NW, int MODE>
+__global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks_kernel(AttnPass p, int first_seg, int segs,
+                                                                                     bool whole_o, bool whole_x) {
+  using B = Blocks<T, RP, NW, MODE>;
+  constexpr int NP = B::NP, C = B::C, J = B::J, TI = B::TI, RB = B::RB, V = B::V, W = B::W;
+  constexpr bool OUT = B::out, TAN = B::tangent;
+  __shared__ __align__(16) unsigned char lds[B::bytes];
+  u16* const L16 = reinterpret_cast<u16*>(lds);
+  float* const pow_tab = reinterpret_cast<float*>(lds + B::off_end * 2);
+  float* const upd_tab = pow_tab + 2 * C;
+
+  const int t = threadIdx.x, lane = t & 63, half = lane >> 5, l32 = lane & 31, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int seg = first_seg + (int)(blockIdx.x % segs);
+  const long long bh = blockIdx.x / segs, b = bh / p.heads;
+  const int h = (int)(bh % p.heads);
+  const long long len = live_tokens(p, b);
+  const long long seg_lo = seg * p.seg_tokens, seg_end = min(seg_lo + p.seg_tokens, p.tokens);
+  const long long lo = min(seg_lo, len), hi = min(seg_end, len);
+  const int rows = p.rows, cols = p.cols, e = p.reverse ? 0 : 1;
+  const bool reverse = p.reverse;
+  const double g = (double)log_decay_of(p.log_decay, h);
+
+  for (int i = t; i < 2 * C; i += B::threads) pow_tab[i] = i < C ? 0.0f : (float)exp(g * (double)(i - C));
+
+  // the state: column 32 wave + l32, register r of block rb: row 32 rb + 16 (r / 8) + 8 half + r % 8
+  floatx16 m[RB], tm[TAN ? RB : 1];
+  const int ncol = 32 * wave + l32;
+  const size_t m0 = (size_t)bh * rows * cols, seg_size = (size_t)p.batch * p.heads * rows * cols;
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 32 * rb + 16 * (r >> 3) + 8 * half + (r & 7);
+      float x = 0.0f;
+      if (OUT && row < rows && ncol < cols) {
+        const size_t at = m0 + (size_t)(row * p.m_r + ncol * p.m_n);
+        if (p.segments > 1)
+          x = p.seg_state[seg * seg_size + at];
+        else if (p.m_in)
+          x = p.m_in[at] * p.m_in_scale;
+      }
+      m[rb][r] = x;
+      if (TAN) tm[rb][r] = 0.0f;
+    }
+  double dg = 0.0;
+
+  using PB = typename B::template Pairs<RP>;
+  using PC = typename B::template Pairs<B::CP>;
+  uint4 ra[OUT ? B::a_passes : 1];
+  PB rb_raw;
+  PC rc_raw;
+  const int a_f = (t % B::a_lanes) * V, a_u = t / B::a_lanes;
+  const int b_f = (t % PB::lanes) * 2, b_g = t / PB::lanes, c_f = (t % PC::lanes) * 2, c_g = t / PC::lanes;
+  const bool a_on = a_f < rows, b_on = b_f < rows, c_on = c_f < cols;
+  const bool b_has = !PB::partial || b_g < C / 8, c_has = !PC::partial || c_g < C / 8;  // (threads without tokens read group 0)
+
+  // Row u of a block (in the pass's order) is u, or reversed C - 1 - u, token strides above the block's base; a partial
+  // reversed block's base lies before its tokens, whose rows are not read.  Offsets in a block are 32-bit bytes.  Threads
+  // past the features read feature 0 and keep zeros.
+  const char* const base_a = OUT ? reinterpret_cast<const char*>(head_base<T>(p.a, b, h)) : nullptr;
+  const char* const base_b = reinterpret_cast<const char*>(head_base<T>(p.b, b, h));
+  const char* const base_c = reinterpret_cast<const char*>(head_base<T>(p.c, b, h));
+  const long long st_a = OUT ? p.a.st * (long long)sizeof(T) : 0, st_b = p.b.st * (long long)sizeof(T), st_c = p.c.st * (long long)sizeof(T);
+  const unsigned step_a = reverse ? 0u - (unsigned)st_a : (unsigned)st_a, step_b = reverse ? 0u - (unsigned)st_b : (unsigned)st_b,
+                 step_c = reverse ? 0u - (unsigned)st_c : (unsigned)st_c;
+  const unsigned off_a = (unsigned)(reverse ? C - 1 : 0) * (unsigned)st_a + (unsigned)a_u * step_a + (a_on ? a_f : 0) * (unsigned)sizeof(T);
+  const unsigned off_b = (unsigned)(reverse ? C - 1 : 0) * (unsigned)st_b + (unsigned)(b_has ? b_g * 8 : 0) * step_b + (b_on ? b_f : 0) * (unsigned)sizeof(T);
+  const unsigned off_c = (unsigned)(reverse ? C - 1 : 0) * (unsigned)st_c + (unsigned)(c_has ? c_g * 8 : 0) * step_c + (c_on ? c_f : 0) * (unsigned)sizeof(T);
+
+  auto load_pair = [](const char* base, unsigned off, unsigned (&w)[W]) {
+    if constexpr (W == 1) {
+      w[0] = *reinterpret_cast<const unsigned*>(base + off);
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(base + off);
+      w[0] = v.x;
+      w[1] = v.y;
+    }
+  };
+  // blocks in the pass's order; their borders are the same tokens in both directions
+  const int total = (int)((hi - lo + C - 1) / C);
+  auto block_lo = [&](int i) { return lo + (long long)(reverse ? total - 1 - i : i) * C; };
+
+  // (ALL: a whole block; else rows past the last one are zeros)
+  auto fetch_rows = [&](long long at, int count, auto all) {
+    constexpr bool ALL = decltype(all)::value;
+    if constexpr (OUT) {
+      const char* base = base_a + at * st_a;
+      unsigned off = opaque(off_a);
+#pragma unroll
+      for (int q = 0; q < B::a_passes; ++q, off += (unsigned)B::a_rows * step_a) {
+        if (!ALL) ra[q] = make_uint4(0, 0, 0, 0);
+        if (ALL || a_u + q * B::a_rows < count) ra[q] = *reinterpret_cast<const uint4*>(base + off);
+      }
+    }
+    const char* const bb = base_b + at * st_b;
+#pragma unroll
+    for (int q = 0; q < PB::passes; ++q) {
+      unsigned off = opaque(off_b) + (unsigned)(8 * q * PB::at_once) * step_b;
+#pragma unroll
+      for (int k = 0; k < 8; ++k, off += step_b) {
+        if (!ALL)
+          for (unsigned& z : rb_raw.w[q][k]) z = 0;
+        if (ALL || (b_g + q * PB::at_once) * 8 + k < count) load_pair(bb, off, rb_raw.w[q][k]);
+      }
+    }
+    const char* const bc = base_c + at * st_c;
+#pragma unroll
+    for (int q = 0; q < PC::passes; ++q) {
+      unsigned off = opaque(off_c) + (unsigned)(8 * q * PC::at_once) * step_c;
+#pragma unroll
+      for (int k = 0; k < 8; ++k, off += step_c) {
+        if (!ALL)
+          for (unsigned& z : rc_raw.w[q][k]) z = 0;
+        if (ALL || (c_g + q * PC::at_once) * 8 + k < count) load_pair(bc, off, rc_raw.w[q][k]);
+      }
+    }
+  };
+  auto fetch = [&](int i) {
+    const long long c0 = block_lo(i);
+    const int count = (int)min((long long)C, hi - c0);
+    if (count == C)
+      fetch_rows(c0, C, std::true_type{});
+    else
+      fetch_rows(reverse ? c0 - (C - count) : c0, count, std::false_type{});
+  };
+
+  // eight tokens of a feature pair: by feature (two rows of 8 tokens) and, where rows0, by token
+  auto put_pairs = [&](const unsigned(&r)[8][W], bool on, u16* plane0, int plane, int f, int tok, u16* rows0) {
+    unsigned pc[8][NP];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      unsigned w[W];
+#pragma unroll
+      for (int z = 0; z < W; ++z) w[z] = on ? r[k][z] : 0u;
+      pair_pieces<T>(w, pc[k]);
+    }
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      unsigned lo4[4], hi4[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        lo4[k] = (pc[2 * k][q] & 0xffffu) | (pc[2 * k + 1][q] << 16);
+        hi4[k] = (pc[2 * k][q] >> 16) | (pc[2 * k + 1][q] & 0xffff0000u);
+      }
+      u16* dst = plane0 + q * plane + f * B::pitch_tok + tok;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
+      *reinterpret_cast<uint4*>(dst + B::pitch_tok) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
+      if (rows0)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<unsigned*>(rows0 + q * B::row_plane + (tok + k) * B::pitch_row + f) = pc[k][q];
+    }
+  };
+  auto stage = [&]() {
+    if constexpr (OUT) {
+#pragma unroll
+      for (int q = 0; q < B::a_passes; ++q) {
+        u16* dst = L16 + (a_u + q * B::a_rows) * B::pitch_row + a_f;
+        if constexpr (NP == 1) {
+          *reinterpret_cast<uint4*>(dst) = a_on ? ra[q] : make_uint4(0, 0, 0, 0);
+        } else {
+          const unsigned w[4] = {a_on ? ra[q].x : 0u, a_on ? ra[q].y : 0u, a_on ? ra[q].z : 0u, a_on ? ra[q].w : 0u};
+          unsigned pc[V / 2][NP];
+#pragma unroll
+          for (int k = 0; k < V / 2; ++k) pair_pieces<T>(w + k * W, pc[k]);
+#pragma unroll
+          for (int z = 0; z < NP; ++z)
+            if constexpr (V == 8)
+              *reinterpret_cast<uint4*>(dst + z * B::row_plane) = make_uint4(pc[0][z], pc[1][z], pc[2][z], pc[3][z]);
+            else
+              *reinterpret_cast<uint2*>(dst + z * B::row_plane) = make_uint2(pc[0][z], pc[1][z]);
+        }
+      }
+    }
+    if (b_has)
+#pragma unroll
+      for (int q = 0; q < PB::passes; ++q)
+        put_pairs(rb_raw.w[q], b_on, L16 + B::off_bt, B::b_plane, b_f, (b_g + q * PB::at_once) * 8, OUT ? L16 + B::off_b : nullptr);
+    if (c_has)
+#pragma unroll
+      for (int q = 0; q < PC::passes; ++q)
+        put_pairs(rc_raw.w[q], c_on, L16 + B::off_ct, B::c_plane, c_f, (c_g + q * PC::at_once) * 8, nullptr);
+  };
+
+  const Decay gamma_full(exp(g * (double)C)), gamma_part(exp(g * (double)((hi - lo) % C)));
+  const int n4 = 32 * wave + 4 * half;  // the lane's first output column
+  int table_for = 0;
+  if (total > 0) fetch(0);
+  for (int i = 0; i < total; ++i) {
+    const long long c0 = block_lo(i);
+    const int count = (int)min((long long)C, hi - c0);
+    __syncthreads();  // the block before is done with LDS
+    if (table_for != count) {
+      table_for = count;
+      for (int j = t; j < C; j += B::threads) upd_tab[j] = j < count ? (float)exp(g * (double)(count - e - j)) : 0.0f;
+    }
+    stage();
+    __syncthreads();
+    if (i + 1 < total) fetch(i + 1);
+
+    floatx16 o[OUT ? TI : 1], s[OUT ? B::tiles : 1], ol[TAN ? TI : 1];
+    if constexpr (OUT) {
+#pragma unroll
+      for (int x = 0; x < TI; ++x) {
+        o[x] = floatx16{};
+        if (TAN) ol[x] = floatx16{};
+      }
+#pragma unroll
+      for (int k = 0; k < B::tiles; ++k) s[k] = floatx16{};
+      // over the features: scores^T = b a^T (rows in the order pi) and out^T = M^T a^T
+#pragma unroll
+      for (int ks = 0; ks < RP / 16; ++ks) {
+        __builtin_amdgcn_sched_barrier(0);  // (one step's operands at a time: registers)
+        uint4 fa[NP][TI], fm[J];
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+          for (int x = 0; x < TI; ++x)
+            fa[q][x] = *reinterpret_cast<const uint4*>(L16 + q * B::row_plane + (32 * x + l32) * B::pitch_row + 16 * ks + 8 * half);
+#pragma unroll
+        for (int k = 0; k < B::tiles; ++k) {
+          const int id = wave + NW * k;  // tiles (x, y): (0, 0), (1, 0), (1, 1)
+          if (B::shared_scores && id > 2) break;
+          const int y = B::shared_scores ? id >> 1 : 0;
+          uint4 fb[NP];
+#pragma unroll
+          for (int q = 0; q < NP; ++q)
+            fb[q] = *reinterpret_cast<const uint4*>(L16 + B::off_b + q * B::row_plane + (32 * y + pi(l32)) * B::pitch_row + 16 * ks + 8 * half);
+#pragma unroll
+          for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int z = 0; z < NP; ++z)
+              if (q + z < 3) {
+                if constexpr (B::shared_scores) {
+                  if (id == 0)
+                    s[k] = mfma(fb[q], fa[z][0], s[k]);
+                  else
+                    s[k] = mfma(fb[q], fa[z][TI - 1], s[k]);
+                } else {
+                  s[k] = mfma(fb[q], fa[z][0], s[k]);
+                }
+              }
+        }
+        float mv[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mv[k] = m[ks / 2][8 * (ks & 1) + k];
+        split8<J>(mv, fm);
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+          for (int z = 0; z < J; ++z)
+            if (q + z < J)
+#pragma unroll
+              for (int x = 0; x < TI; ++x) o[x] = mfma(fm[z], fa[q][x], o[x]);
+        if constexpr (TAN) {
+          uint4 fr[3];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mv[k] = tm[ks / 2][8 * (ks & 1) + k];
+          split8<3>(mv, fr);
+#pragma unroll
+          for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int z = 0; z < 3; ++z)
+              if (q + z < 3)
+#pragma unroll
+                for (int x = 0; x < TI; ++x) ol[x] = mfma(fr[z], fa[q][x], ol[x]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // a state reaches token i with gamma^(i + e)
+#pragma unroll
+      for (int x = 0; x < TI; ++x) {
+        const float w = e ? pow_tab[C + 32 * x + l32] * pow_tab[C + 1] : pow_tab[C + 32 * x + l32];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          o[x][r] *= w;
+          if (TAN) ol[x][r] = __builtin_fmaf(ol[x][r], w, (float)(32 * x + l32 + 1) * o[x][r]);
+        }
+      }
+      // scores take gamma^(i - j), j = 32 y + 16 (r / 8) + 8 half + r % 8
+#pragma unroll
+      for (int k = 0; k < B::tiles; ++k) {
+        const int id = wave + NW * k;
+        if (B::shared_scores && id > 2) break;
+        const int lag = (B::shared_scores && id == 1 ? 32 : 0) + l32 - 8 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[k][r] *= pow_tab[C + lag - 16 * (r >> 3) - (r & 7)];
+      }
+      if constexpr (B::shared_scores) {
+        __syncthreads();  // a and b by token are done with: the scores take their place
+#pragma unroll
+        for (int k = 0; k < B::tiles; ++k) {
+          const int id = wave + NW * k;
+          if (id > 2) break;
+          const int x = id ? 1 : 0, y = id >> 1;
+#pragma unroll
+          for (int r0 = 0; r0 < 16; r0 += 8) {
+            float w[8];
+            uint4 fp[B::PJ];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) w[r] = s[k][r0 + r];
+            split8<B::PJ>(w, fp);
+#pragma unroll
+            for (int q = 0; q < B::PJ; ++q)
+              *reinterpret_cast<uint4*>(L16 + q * B::s_plane + (32 * x + l32) * B::pitch_tok + 32 * y + 2 * r0 + 8 * half) = fp[q];
+          }
+        }
+        __syncthreads();
+      }
+    }
+    // the state takes gamma^L M, its tangent gamma^L (M' + L M)
+    {
+      const Decay gamma = count == C ? gamma_full : gamma_part;
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (TAN) tm[rb][r] = gamma.times(__builtin_fmaf((float)count, m[rb][r], tm[rb][r]));
+          m[rb][r] = gamma.times(m[rb][r]);
+        }
+    }
+    // over the tokens: out^T += c^T scores^T, M += b^T (decayed c)
+#pragma unroll
+    for (int kk = 0; kk < C / 16; ++kk) {
+      __builtin_amdgcn_sched_barrier(0);
+      uint4 fc[NP];
+#pragma unroll
+      for (int q = 0; q < NP; ++q)
+        fc[q] = *reinterpret_cast<const uint4*>(L16 + B::off_ct + q * B::c_plane + ncol * B::pitch_tok + 16 * kk + 8 * half);
+      if constexpr (OUT) {
+#pragma unroll
+        for (int x = kk / 2; x < TI; ++x) {
+          uint4 fp[B::PJ];
+          float w[8];
+          if constexpr (B::shared_scores) {
+#pragma unroll
+            for (int q = 0; q < B::PJ; ++q)
+              fp[q] = *reinterpret_cast<const uint4*>(L16 + q * B::s_plane + (32 * x + l32) * B::pitch_tok + 16 * kk + 8 * half);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = s[0][8 * kk + k];
+            split8<B::PJ>(w, fp);
+          }
+#pragma unroll
+          for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int z = 0; z < J; ++z)
+              if (q + z < J) o[x] = mfma(fc[q], fp[z], o[x]);
+          if constexpr (TAN) {
+            if constexpr (B::shared_scores) {  // (three pieces are the score itself)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) w[k] = 0.0f;
+#pragma unroll
+              for (int q = B::PJ - 1; q >= 0; --q) {
+                const unsigned d[4] = {fp[q].x, fp[q].y, fp[q].z, fp[q].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  w[2 * k] += __uint_as_float(d[k] << 16);
+                  w[2 * k + 1] += __uint_as_float(d[k] & 0xffff0000u);
+                }
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] *= (float)(32 * x + l32 - 16 * kk - 8 * half - k);
+            uint4 fl[3];
+            split8<3>(w, fl);
+#pragma unroll
+            for (int q = 0; q < NP; ++q)
+#pragma unroll
+              for (int z = 0; z < 3; ++z)
+                if (q + z < 3) ol[x] = mfma(fc[q], fl[z], ol[x]);
+          }
+        }
+      }
+      float cv[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) cv[k] = 0.0f;
+#pragma unroll
+      for (int q = NP - 1; q >= 0; --q) {
+        const unsigned d[4] = {fc[q].x, fc[q].y, fc[q].z, fc[q].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          cv[2 * k] += __uint_as_float(d[k] << 16);
+          cv[2 * k + 1] += __uint_as_float(d[k] & 0xffff0000u);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) cv[k] *= upd_tab[16 * kk + 8 * half + k];
+      uint4 fu[3], ft[TAN ? 3 : 1];
+      split8<3>(cv, fu);
+      if constexpr (TAN) {
+        float tv[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) tv[k] = cv[k] * (float)(count - 1 - 16 * kk - 8 * half - k);
+        split8<3>(tv, ft);
+      }
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+          const uint4 fbt = *reinterpret_cast<const uint4*>(L16 + B::off_bt + q * B::b_plane + (32 * rb + pi(l32)) * B::pitch_tok + 16 * kk + 8 * half);
+#pragma unroll
+          for (int z = 0; z < 3; ++z)
+            if (q + z < 3) {
+              m[rb] = mfma(fbt, fu[z], m[rb]);
+              if constexpr (TAN) tm[rb] = mfma(fbt, ft[z], tm[rb]);
+            }
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (OUT) {
+      // out: lane: token 32 x + l32, register r: column n4 + 8 (r / 4) + r % 4
+#pragma unroll
+      for (int x = 0; x < TI; ++x) {
+        const int u = 32 * x + l32;
+        const bool live = u < count;
+        const long long tok = reverse ? c0 + count - 1 - u : c0 + u;
+        if constexpr (TAN) {
+          float sum = 0.0f;
+          if (live) {
+            const T* xr = head_base<T>(p.x, b, h) + tok * p.x.st + n4;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              T xv[4];
+              if (whole_x && n4 + 8 * q < cols) {
+                __builtin_memcpy(xv, __builtin_assume_aligned(xr + 8 * q, 4 * sizeof(T)), sizeof(xv));
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) xv[k] = n4 + 8 * q + k < cols ? xr[8 * q + k] : T(0.0f);
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) sum = __builtin_fmaf(to_f32(xv[k]), ol[x][4 * q + k], sum);
+            }
+          }
+          dg += (double)sum * (double)p.scale;
+        }
+        float ov[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ov[r] = o[x][r] * p.scale;
+        const size_t row = (((size_t)b * p.tokens + tok) * p.heads + h) * cols;
+        if (sizeof(T) == 4 || p.out_f32) {
+          float* dst = static_cast<float*>(p.out) + row + n4;
+          if (live)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              if (whole_o) {
+                if (n4 + 8 * q < cols) *reinterpret_cast<float4*>(dst + 8 * q) = make_float4(ov[4 * q], ov[4 * q + 1], ov[4 * q + 2], ov[4 * q + 3]);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if (n4 + 8 * q + k < cols) dst[8 * q + k] = ov[4 * q + k];
+              }
+            }
+        } else if constexpr (sizeof(T) == 2) {
+          unsigned d[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            d[k] = __builtin_bit_cast(u16, from_f32<T>(ov[2 * k])) | (unsigned)__builtin_bit_cast(u16, from_f32<T>(ov[2 * k + 1])) << 16;
+          if (whole_o) {
+            // the halves exchange so that each has 8 consecutive columns: 16 (q / 2) + 8 half
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+              const auto s0 = __builtin_amdgcn_permlane32_swap(d[2 * q], d[2 * q + 2], false, false);
+              const auto s1 = __builtin_amdgcn_permlane32_swap(d[2 * q + 1], d[2 * q + 3], false, false);
+              const int n = 32 * wave + 8 * q + 8 * half;
+              if (live && n < cols) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row + n) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+            }
+          } else if (live) {
+            u16* dst = static_cast<u16*>(p.out) + row + n4;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int n = 8 * (k / 2) + 2 * (k % 2);
+              if (n4 + n < cols) dst[n] = (u16)d[k];
+              if (n4 + n + 1 < cols) dst[n + 1] = (u16)(d[k] >> 16);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // padding: zeros
+  if (OUT)
+    for (long long tok = max(len, seg_lo) + t / 32; tok < seg_end; tok += B::threads / 32)
+      for (int n = t % 32; n < cols; n += 32) {
+        const size_t at = (((size_t)b * p.tokens + tok) * p.heads + h) * cols + n;
+        if (p.out_f32)
+          static_cast<float*>(p.out)[at] = 0.0f;
+        else
+          static_cast<T*>(p.out)[at] = from_f32<T>(0.0f);
+      }
+  const bool last = seg == (reverse ? 0 : p.segments - 1);
+  const int row0 = (int)opaque(8u * half);
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 32 * rb + 16 * (r >> 3) + row0 + (r & 7);
+      if (row >= rows || ncol >= cols) continue;
+      const size_t at = m0 + (size_t)(row * p.m_r + ncol * p.m_n);
+      if (!OUT)
+        p.seg_state[seg * seg_size + at] = m[rb][r];
+      else if (last && p.m_out)
+        p.m_out[at] = m[rb][r] * p.m_out_scale;
+      if (TAN) {
+        const float sink = p.segments > 1 ? p.seg_sink[seg * seg_size + at] * p.scale : p.m_sink ? p.m_sink[at] : 0.0f;
+        dg += (double)tm[rb][r] * (double)sink;
+      }
+    }
+  if constexpr (TAN) {
+    double* sum = reinterpret_cast<double*>(lds);
+    __syncthreads();
+    sum[t] = dg;
+    __syncthreads();
+    if (t == 0) {
+      double all = 0.0;
+      for (int k = 0; k < B::threads; ++k) all += sum[k];
+      p.dg_part[bh * p.segments + seg] = all;
+    }
+  }
+}
+
+template <typename T, int RP, int NW, int MODE>
+static hipError_t blocks_launch(const AttnPass& p) {
+  const int osize = p.out_f32 || sizeof(T) == 4 ? 4 : 2;
+  const bool wo = p.cols % (16 / osize) == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+  const bool wx = MODE == kTangent && p.cols % 4 == 0 && whole_view(p.x, (int)sizeof(T), 4 * (int)sizeof(T));
+  const int first = MODE == kSums && p.reverse ? 1 : 0, segs = MODE == kSums ? p.segments - 1 : p.segments;
+  const long long grid = p.batch * p.heads * segs;
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((attn_blocks_kernel<T, RP, NW, MODE>), dim3((unsigned)grid), dim3(64 * NW), 0, p.stream, p, first, segs, wo, wx);
+  return hipGetLastError();
+}
+
+template <typename T, int MODE>
+static hipError_t blocks_dims(const AttnPass& p) {
+  if (p.rows <= 64) return p.cols <= 64 ? blocks_launch<T, 64, 2, MODE>(p) : blocks_launch<T, 64, 4, MODE>(p);
+  return p.cols <= 64 ? blocks_launch<T, 128, 2, MODE>(p) : blocks_launch<T, 128, 4, MODE>(p);
+}
+
+template <typename T>
+static hipError_t blocks_modes(const AttnPass& p) {
+  if (!p.out) return blocks_dims<T, kSums>(p);
+  return p.dg_part ? blocks_dims<T, kTangent>(p) : blocks_dims<T, kPass>(p);
+}
+
+}  // namespace tfa

@@ -33,7 +33,9 @@ SOURCES = [
     "kernels_smooth_c2c.hip",
     "model_ops.hip",
     "kernels_attention.hip",
-    "kernels_attention_blocks.hip",
+    "kernels_attention_f32.hip",
+    "kernels_attention_bf16.hip",
+    "kernels_attention_f16.hip",
     "kernels_norm.hip",
     "kernels_adamw.hip",
 ]

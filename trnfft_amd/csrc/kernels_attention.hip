@@ -161,6 +161,74 @@ hipError_t launch_attn_scan(const AttnPass& p) {
 }
 
 // ------------------------------------------------------------------------------------------------
+// In blocks of tokens (attention_blocks.h): dispatch, and what surrounds the segments of a long sequence.
+// ------------------------------------------------------------------------------------------------
+
+hipError_t launch_attn_blocks_f32(const AttnPass& p);
+hipError_t launch_attn_blocks_bf16(const AttnPass& p);
+hipError_t launch_attn_blocks_f16(const AttnPass& p);
+
+hipError_t launch_attn_blocks(const AttnPass& p) {
+  if (p.dtype == 0) return launch_attn_blocks_f32(p);
+  return p.dtype == 1 ? launch_attn_blocks_bf16(p) : launch_attn_blocks_f16(p);
+}
+
+int attn_blocks_dg_parts(const AttnPass& p) { return p.segments; }
+
+// seg_state[s] of each segment's own sum becomes the state it starts from; one thread an element
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnPass p) {
+  const size_t size = (size_t)p.rows * p.cols, all = (size_t)p.batch * p.heads * size;
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= all) return;
+  const long long bh = (long long)(i / size), len = live_tokens(p, bh / p.heads);
+  const double g = (double)log_decay_of(p.log_decay, (int)(bh % p.heads));
+  const Decay whole(exp(g * (double)p.seg_tokens));
+  float m = p.m_in ? p.m_in[i] * p.m_in_scale : 0.0f;
+  for (int k = 0; k < p.segments; ++k) {
+    const int s = p.reverse ? p.segments - 1 - k : k;
+    float* at = p.seg_state + s * all + i;
+    const bool end = k == p.segments - 1;
+    const float own = end ? 0.0f : *at;
+    *at = m;
+    const long long tokens = min(max(len - s * p.seg_tokens, 0LL), p.seg_tokens);
+    m = (tokens == p.seg_tokens ? whole : Decay(exp(g * (double)tokens))).times(m) + own;
+  }
+}
+
+hipError_t launch_attn_join(const AttnPass& p) {
+  const size_t all = (size_t)p.batch * p.heads * p.rows * p.cols, blocks = (all + 255) / 256;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)blocks), dim3(256), 0, p.stream, p);
+  return hipGetLastError();
+}
+
+// (batch, token, head, features) of any strides as a dense tensor of `padded` features, zeros past the last
+template <typename U>
+__global__ __launch_bounds__(256) void attn_pack_kernel(const U* __restrict__ in, U* __restrict__ out, long long total,
+                                                        long long tokens, int heads, int features, int padded, long long sb,
+                                                        long long st, long long sh) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int f = (int)(i % padded);
+  const long long r = i / padded, h = r % heads, bt = r / heads;
+  out[i] = f < features ? in[bt / tokens * sb + bt % tokens * st + h * sh + f] : U(0);
+}
+
+hipError_t launch_attn_pack(const HeadsView& v, void* out, int dtype, long long batch, long long tokens, int heads, int features,
+                            int padded, hipStream_t stream) {
+  const long long total = batch * tokens * heads * padded, blocks = (total + 255) / 256;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)blocks), block(256);
+  if (dtype == 0)
+    hipLaunchKernelGGL((attn_pack_kernel<unsigned>), grid, block, 0, stream, static_cast<const unsigned*>(v.p),
+                       static_cast<unsigned*>(out), total, tokens, heads, features, padded, v.sb, v.st, v.sh);
+  else
+    hipLaunchKernelGGL((attn_pack_kernel<unsigned short>), grid, block, 0, stream, static_cast<const unsigned short*>(v.p),
+                       static_cast<unsigned short*>(out), total, tokens, heads, features, padded, v.sb, v.st, v.sh);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------
 // Sums of the gradients' parts, in a fixed order.
 // ------------------------------------------------------------------------------------------------
 

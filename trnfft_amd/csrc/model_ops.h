@@ -72,9 +72,17 @@ struct AttnPass {
 // token by token (any dimensions up to 256)
 hipError_t launch_attn_scan(const AttnPass& p);
 int attn_scan_dg_parts(const AttnPass& p);
-// in blocks of tokens on the matrix cores: dimensions up to 128, token strides of 0 to 2^24 - 1 elements
+// in blocks of tokens on the matrix cores: dimensions up to 128; a, b and c "whole" (addresses, strides and features are
+// multiples of 16 bytes, or stride 0) with token strides below 2^24 elements
 int attn_blocks_dg_parts(const AttnPass& p);
 hipError_t launch_attn_blocks(const AttnPass& p);
+inline bool whole_view(const HeadsView& v, int size, int bytes) {
+  const int n = bytes / size;
+  return reinterpret_cast<uintptr_t>(v.p) % bytes == 0 && v.sb % n == 0 && v.st % n == 0 && v.sh % n == 0;
+}
+// a dense copy (batch, tokens, heads, padded) of an operand, zeros past its features
+hipError_t launch_attn_pack(const HeadsView& v, void* out, int dtype, long long batch, long long tokens, int heads, int features,
+                            int padded, hipStream_t stream);
 // the states that segments of a long sequence start from, p.seg_state, from the segments' own sums: in place
 hipError_t launch_attn_join(const AttnPass& p);
 // dlog_decay[h] = sum over batch and parts

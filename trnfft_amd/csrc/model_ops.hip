@@ -40,8 +40,9 @@ int check_heads(const tfa_attn_desc* d) {
   return TFA_OK;
 }
 
-tfa::HeadsView view(const void* p, const int64_t* stride, int32_t heads, int32_t own) {
-  return {p, stride[0], stride[1], stride[2], heads / own};
+tfa::HeadsView view(const void* p, const tfa_attn_desc* d, const int64_t* stride, int32_t own) {
+  // (a stride along one row says nothing)
+  return {p, d->batch > 1 ? stride[0] : 0, d->tokens > 1 ? stride[1] : 0, own > 1 ? stride[2] : 0, d->heads / own};
 }
 
 tfa::HeadsView dense(const void* p, const tfa_attn_desc* d, int32_t features) {
@@ -74,23 +75,57 @@ struct Plan {
   int segments;
   int64_t seg_tokens;
   size_t state_bytes;  // of the segments' states
+  // operands q, k, v, grad_out that are not laid out in whole 16-byte pieces are copied so first
+  int padded[4];        // features of the copy, 0: taken as it is
+  size_t pack_bytes[4];
 };
 
-Plan plan_of(const tfa_attn_desc* d) {
-  Plan plan{false, 1, std::max<int64_t>(1, (d->tokens + 63) / 64 * 64), 0};
+Plan plan_of(const tfa_attn_desc* d, bool backward) {
+  Plan plan{};
+  plan.segments = 1;
+  plan.seg_tokens = std::max<int64_t>(1, (d->tokens + 63) / 64 * 64);
   plan.blocks = d->tokens > kScanTokens && d->key_dim <= 128 && d->value_dim <= 128;
-  for (const int64_t* stride : {d->q_stride, d->k_stride, d->v_stride})  // (32-bit offsets inside a block of tokens)
-    if (stride[1] < 0 || stride[1] >= (1 << 24)) plan.blocks = false;
-  if ((int64_t)d->heads * std::max(d->key_dim, d->value_dim) >= (1 << 24)) plan.blocks = false;
   if (!plan.blocks || d->batch == 0) return plan;
+  const int piece = 16 / (int)dtype_size(d->dtype);
+  const int64_t* strides[3] = {d->q_stride, d->k_stride, d->v_stride};
+  const int32_t own[4] = {d->q_heads, d->k_heads, d->v_heads, d->heads};
+  for (int i = 0; i < (backward ? 4 : 3); ++i) {
+    const int32_t features = i < 2 ? d->key_dim : d->value_dim;
+    bool whole = features % piece == 0;
+    if (i < 3) {
+      const tfa::HeadsView v = view(nullptr, d, strides[i], own[i]);
+      whole = whole && v.sb % piece == 0 && v.st % piece == 0 && v.sh % piece == 0 && v.st >= 0 && v.st < (1 << 24);
+    }
+    if (whole) continue;
+    plan.padded[i] = (features + piece - 1) / piece * piece;
+    plan.pack_bytes[i] = align256((size_t)d->batch * d->tokens * own[i] * plan.padded[i] * dtype_size(d->dtype));
+  }
   const int64_t rows = d->batch * d->heads;
   const int64_t want = std::min((kWantBlocks + rows - 1) / rows, d->tokens / kSegTokens);
   if (want > 1) {
     plan.seg_tokens = ((d->tokens + want - 1) / want + 63) / 64 * 64;
     plan.segments = (int)((d->tokens + plan.seg_tokens - 1) / plan.seg_tokens);
-    plan.state_bytes = align256((size_t)plan.segments * rows * d->key_dim * d->value_dim * sizeof(float));
+    if (plan.segments > 1) plan.state_bytes = align256((size_t)plan.segments * rows * d->key_dim * d->value_dim * sizeof(float));
   }
   return plan;
+}
+
+size_t packed_bytes(const Plan& plan) { return plan.pack_bytes[0] + plan.pack_bytes[1] + plan.pack_bytes[2] + plan.pack_bytes[3]; }
+
+// Operand i as the kernels take it, copied to `*space` where the plan says so; `*space` moves past the copy.
+int operand(const tfa_attn_desc* d, const Plan& plan, int i, int32_t own, int32_t features, tfa::HeadsView* v, char** space,
+            hipStream_t stream) {
+  if (!plan.blocks) return TFA_OK;
+  if (!plan.padded[i]) {
+    if (reinterpret_cast<uintptr_t>(v->p) % 16) return set_error(TFA_ERR_INVALID, "operands must be 16-byte aligned");
+    return TFA_OK;
+  }
+  const hipError_t e = tfa::launch_attn_pack(*v, *space, d->dtype, d->batch, d->tokens, own, features, plan.padded[i], stream);
+  if (e != hipSuccess) return launched(e, "operand copy");
+  const long long row = (long long)own * plan.padded[i];
+  *v = {*space, d->tokens * row, row, plan.padded[i], v->group};
+  *space += plan.pack_bytes[i];
+  return TFA_OK;
 }
 
 hipError_t run_pass(tfa::AttnPass p, const Plan& plan, float* states) {
@@ -115,18 +150,19 @@ hipError_t segment_states(tfa::AttnPass p, const Plan& plan, float* states) {
 
 struct BackwardSpace {
   size_t dq = 0, dk = 0, dv = 0, dg = 0, total = 0;  // offsets; gradients of shared heads before their sum
-  size_t states = 0, grad_states = 0;
+  size_t packed = 0, states = 0, grad_states = 0;
   int dg_each = 0;
   Plan plan;
 };
 
 BackwardSpace backward_space(const tfa_attn_desc* d) {
   BackwardSpace s;
-  s.plan = plan_of(d);
+  s.plan = plan_of(d, true);
   const size_t rows = (size_t)d->batch * d->tokens * d->heads * sizeof(float);
   if (d->q_heads != d->heads) s.dq = s.total, s.total += align256(rows * d->key_dim);
   if (d->k_heads != d->heads) s.dk = s.total, s.total += align256(rows * d->key_dim);
   if (d->v_heads != d->heads) s.dv = s.total, s.total += align256(rows * d->value_dim);
+  s.packed = s.total, s.total += packed_bytes(s.plan);
   s.states = s.total, s.total += s.plan.state_bytes;
   s.grad_states = s.total, s.total += s.plan.state_bytes;
   tfa::AttnPass p{};
@@ -147,7 +183,12 @@ int tfa_linear_attention_workspace_size(const tfa_attn_desc* desc, int32_t backw
   if (!bytes) return set_error(TFA_ERR_INVALID, "null bytes pointer");
   *bytes = 0;
   if (const int rc = check_heads(desc)) return rc;
-  *bytes = backward ? backward_space(desc).total : plan_of(desc).state_bytes;
+  if (backward) {
+    *bytes = backward_space(desc).total;
+  } else {
+    const Plan plan = plan_of(desc, false);
+    *bytes = packed_bytes(plan) + plan.state_bytes;
+  }
   return TFA_OK;
 }
 
@@ -159,9 +200,9 @@ int tfa_linear_attention(const tfa_attn_desc* desc, const void* q, const void* k
   if (!log_decay || (desc->tokens > 0 && (!q || !k || !v || !out))) return set_error(TFA_ERR_INVALID, "null data pointer");
   if (state_out && state_out == state_in) return set_error(TFA_ERR_INVALID, "state_out must not be state_in");
   tfa::AttnPass p = pass_of(desc, log_decay, lengths, stream);
-  p.a = view(q, desc->q_stride, desc->heads, desc->q_heads);
-  p.b = view(k, desc->k_stride, desc->heads, desc->k_heads);
-  p.c = view(v, desc->v_stride, desc->heads, desc->v_heads);
+  p.a = view(q, desc, desc->q_stride, desc->q_heads);
+  p.b = view(k, desc, desc->k_stride, desc->k_heads);
+  p.c = view(v, desc, desc->v_stride, desc->v_heads);
   p.rows = desc->key_dim;
   p.cols = desc->value_dim;
   p.m_in = state_in;
@@ -169,9 +210,13 @@ int tfa_linear_attention(const tfa_attn_desc* desc, const void* q, const void* k
   p.m_r = desc->value_dim;
   p.m_n = 1;
   p.out = out;
-  const Plan plan = plan_of(desc);
-  if (plan.state_bytes && !workspace) return set_error(TFA_ERR_INVALID, "null workspace");
-  float* states = static_cast<float*>(workspace);
+  const Plan plan = plan_of(desc, false);
+  if (packed_bytes(plan) + plan.state_bytes && !workspace) return set_error(TFA_ERR_INVALID, "null workspace");
+  char* space = static_cast<char*>(workspace);
+  if (const int rc = operand(desc, plan, 0, desc->q_heads, desc->key_dim, &p.a, &space, p.stream)) return rc;
+  if (const int rc = operand(desc, plan, 1, desc->k_heads, desc->key_dim, &p.b, &space, p.stream)) return rc;
+  if (const int rc = operand(desc, plan, 2, desc->v_heads, desc->value_dim, &p.c, &space, p.stream)) return rc;
+  float* states = reinterpret_cast<float*>(space);
   if (const hipError_t e = segment_states(p, plan, states)) return launched(e, "segments");
   return launched(run_pass(p, plan, states), "linear attention");
 }
@@ -191,9 +236,16 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
   char* ws = static_cast<char*>(workspace);
   double* parts = reinterpret_cast<double*>(ws + space.dg);
   const long long rows = (long long)d.batch * d.tokens;
-  const tfa::HeadsView qv = view(q, d.q_stride, d.heads, d.q_heads), kv = view(k, d.k_stride, d.heads, d.k_heads),
-                       vv = view(v, d.v_stride, d.heads, d.v_heads), gv = dense(grad_out, desc, d.value_dim);
+  tfa::HeadsView qv = view(q, desc, d.q_stride, d.q_heads), kv = view(k, desc, d.k_stride, d.k_heads),
+                       vv = view(v, desc, d.v_stride, d.v_heads), gv = dense(grad_out, desc, d.value_dim);
   const Plan& plan = space.plan;
+  if (d.batch > 0) {
+    char* packed = ws + space.packed;
+    if (const int rc = operand(desc, plan, 0, d.q_heads, d.key_dim, &qv, &packed, s)) return rc;
+    if (const int rc = operand(desc, plan, 1, d.k_heads, d.key_dim, &kv, &packed, s)) return rc;
+    if (const int rc = operand(desc, plan, 2, d.v_heads, d.value_dim, &vv, &packed, s)) return rc;
+    if (const int rc = operand(desc, plan, 3, d.heads, d.value_dim, &gv, &packed, s)) return rc;
+  }
   float* states = reinterpret_cast<float*>(ws + space.states);
   float* grad_states = reinterpret_cast<float*>(ws + space.grad_states);
   // the value gradient's pass; its states are those of the key gradient too, and where the decays' tangent ends
@@ -368,6 +420,8 @@ int tfa_adamw_step(int64_t count, const tfa_adam_tensor* tensors, const tfa_adam
   if (count < 0 || !desc || (count > 0 && !tensors)) return set_error(TFA_ERR_INVALID, "bad argument");
   const tfa_adam_desc& d = *desc;
   if (!dtype_ok(d.param_dtype) || !dtype_ok(d.grad_dtype)) return set_error(TFA_ERR_INVALID, "dtype must be TFA_DTYPE_F32, _BF16 or _F16");
+  if (d.grad_dtype != d.param_dtype && d.grad_dtype != TFA_DTYPE_F32)
+    return set_error(TFA_ERR_UNSUPPORTED, "gradients must have the parameters' type or be fp32");
   if (d.state_bits != 32 && d.state_bits != 8) return set_error(TFA_ERR_INVALID, "states have 32 or 8 bits");
   if (d.step < 1) return set_error(TFA_ERR_INVALID, "steps count from 1");
   if (!(d.beta1 >= 0.0 && d.beta1 < 1.0 && d.beta2 >= 0.0 && d.beta2 < 1.0)) return set_error(TFA_ERR_INVALID, "betas must be in [0, 1)");
