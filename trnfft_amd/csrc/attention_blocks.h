@@ -106,16 +106,16 @@ struct Blocks {
   static constexpr int NP = Kind<T>::pieces, C = Kind<T>::block, J = Kind<T>::out_pieces;
   static constexpr int CP = 32 * NW, threads = 64 * NW, TI = C / 32, RB = RP / 32;
   static constexpr bool shared_scores = TI == 2;
-  static constexpr int PJ = tangent ? 3 : J;                    // pieces of a shared score
+  static constexpr int PL = tangent ? 3 : 0;                    // pieces of a shared score times its lag
   static constexpr int tiles = shared_scores ? (3 + NW - 1) / NW : 1;  // score tiles of a wave
   static constexpr int W = sizeof(T) / 2;                       // dwords of two features
   static constexpr int pitch_row = RP + 8, pitch_tok = C + 8;   // 16-bit units: rows start 4 banks apart, modulo 64
   static constexpr int row_plane = C * pitch_row, b_plane = RP * pitch_tok, c_plane = CP * pitch_tok, s_plane = C * pitch_tok;
   static constexpr int off_b = out ? NP * row_plane : 0, rows_end = 2 * off_b;
-  static constexpr int scores_end = out && shared_scores ? PJ * s_plane : 0;  // in the rows' place
+  static constexpr int scores_end = out && shared_scores ? (J + PL) * s_plane : 0;  // in the rows' place
   static constexpr int off_bt = rows_end > scores_end ? rows_end : scores_end;
   static constexpr int off_ct = off_bt + NP * b_plane, off_end = off_ct + NP * c_plane;
-  // tables: gamma^(i - j) by i - j + C (zero before C), gamma^(L - e - j) by j
+  // tables: scale gamma^(i - j) by i - j + C (zero before C), gamma^(L - e - j) by j
   static constexpr int bytes = off_end * 2 + 3 * C * 4;
   static constexpr int V = 16 / sizeof(T), a_lanes = RP / V, a_rows = threads / a_lanes, a_passes = C / a_rows;
   static_assert(C % a_rows == 0, "whole passes");
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
   const bool reverse = p.reverse;
   const double g = (double)log_decay_of(p.log_decay, h);
 
-  for (int i = t; i < 2 * C; i += B::threads) pow_tab[i] = i < C ? 0.0f : (float)exp(g * (double)(i - C));
+  for (int i = t; i < 2 * C; i += B::threads) pow_tab[i] = i < C ? 0.0f : (float)(exp(g * (double)(i - C)) * (double)p.scale);
 
   // the state: column 32 wave + l32, register r of block rb: row 32 rb + 16 (r / 8) + 8 half + r % 8
   floatx16 m[RB], tm[TAN ? RB : 1];
@@ -269,8 +269,8 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
       unsigned lo4[4], hi4[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        lo4[k] = (pc[2 * k][q] & 0xffffu) | (pc[2 * k + 1][q] << 16);
-        hi4[k] = (pc[2 * k][q] >> 16) | (pc[2 * k + 1][q] & 0xffff0000u);
+        lo4[k] = __builtin_amdgcn_perm(pc[2 * k + 1][q], pc[2 * k][q], 0x05040100);
+        hi4[k] = __builtin_amdgcn_perm(pc[2 * k + 1][q], pc[2 * k][q], 0x07060302);
       }
       u16* dst = plane0 + q * plane + f * B::pitch_tok + tok;
       *reinterpret_cast<uint4*>(dst) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
@@ -312,8 +312,18 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
         put_pairs(rc_raw.w[q], c_on, L16 + B::off_ct, B::c_plane, c_f, (c_g + q * PC::at_once) * 8, nullptr);
   };
 
-  const Decay gamma_full(exp(g * (double)C)), gamma_part(exp(g * (double)((hi - lo) % C)));
+  // the wave's score tiles (x, y) of (0, 0), (1, 0), (1, 1); past the last it computes that one again, for nothing
+  int tile_x[B::tiles], tile_y[B::tiles];
+#pragma unroll
+  for (int k = 0; k < B::tiles; ++k) {
+    const int id = min(wave + NW * k, 2);
+    tile_x[k] = B::shared_scores && id ? 1 : 0;
+    tile_y[k] = B::shared_scores ? id >> 1 : 0;
+  }
+  DecaySteps gamma_full(exp(g * (double)C));
+  const float gamma_part = (float)exp(g * (double)((hi - lo) % C));
   const int n4 = 32 * wave + 4 * half;  // the lane's first output column
+  const float first = (float)exp(g * (double)e);
   int table_for = 0;
   if (total > 0) fetch(0);
   for (int i = 0; i < total; ++i) {
@@ -349,27 +359,17 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
             fa[q][x] = *reinterpret_cast<const uint4*>(L16 + q * B::row_plane + (32 * x + l32) * B::pitch_row + 16 * ks + 8 * half);
 #pragma unroll
         for (int k = 0; k < B::tiles; ++k) {
-          const int id = wave + NW * k;  // tiles (x, y): (0, 0), (1, 0), (1, 1)
-          if (B::shared_scores && id > 2) break;
-          const int y = B::shared_scores ? id >> 1 : 0;
-          uint4 fb[NP];
+          uint4 fb[NP], fs[NP];
 #pragma unroll
-          for (int q = 0; q < NP; ++q)
-            fb[q] = *reinterpret_cast<const uint4*>(L16 + B::off_b + q * B::row_plane + (32 * y + pi(l32)) * B::pitch_row + 16 * ks + 8 * half);
+          for (int q = 0; q < NP; ++q) {
+            fb[q] = *reinterpret_cast<const uint4*>(L16 + B::off_b + q * B::row_plane + (32 * tile_y[k] + pi(l32)) * B::pitch_row + 16 * ks + 8 * half);
+            fs[q] = B::shared_scores ? *reinterpret_cast<const uint4*>(L16 + q * B::row_plane + (32 * tile_x[k] + l32) * B::pitch_row + 16 * ks + 8 * half) : fa[q][0];
+          }
 #pragma unroll
           for (int q = 0; q < NP; ++q)
 #pragma unroll
             for (int z = 0; z < NP; ++z)
-              if (q + z < 3) {
-                if constexpr (B::shared_scores) {
-                  if (id == 0)
-                    s[k] = mfma(fb[q], fa[z][0], s[k]);
-                  else
-                    s[k] = mfma(fb[q], fa[z][TI - 1], s[k]);
-                } else {
-                  s[k] = mfma(fb[q], fa[z][0], s[k]);
-                }
-              }
+              if (q + z < 3) s[k] = mfma(fb[q], fs[z], s[k]);
         }
         float mv[8];
 #pragma unroll
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
       // a state reaches token i with gamma^(i + e)
 #pragma unroll
       for (int x = 0; x < TI; ++x) {
-        const float w = e ? pow_tab[C + 32 * x + l32] * pow_tab[C + 1] : pow_tab[C + 32 * x + l32];
+        const float w = pow_tab[C + 32 * x + l32] * first;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           o[x][r] *= w;
@@ -410,9 +410,7 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
       // scores take gamma^(i - j), j = 32 y + 16 (r / 8) + 8 half + r % 8
 #pragma unroll
       for (int k = 0; k < B::tiles; ++k) {
-        const int id = wave + NW * k;
-        if (B::shared_scores && id > 2) break;
-        const int lag = (B::shared_scores && id == 1 ? 32 : 0) + l32 - 8 * half;
+        const int lag = 32 * (tile_x[k] - tile_y[k]) + l32 - 8 * half;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[k][r] *= pow_tab[C + lag - 16 * (r >> 3) - (r & 7)];
       }
@@ -426,13 +424,18 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
 #pragma unroll
           for (int r0 = 0; r0 < 16; r0 += 8) {
             float w[8];
-            uint4 fp[B::PJ];
+            uint4 fp[J + B::PL], *const fl = fp + J;
+            u16* const dst = L16 + (32 * x + l32) * B::pitch_tok + 32 * y + 2 * r0 + 8 * half;
 #pragma unroll
             for (int r = 0; r < 8; ++r) w[r] = s[k][r0 + r];
-            split8<B::PJ>(w, fp);
+            split8<J>(w, *reinterpret_cast<uint4(*)[J]>(fp));
+            if constexpr (TAN) {
 #pragma unroll
-            for (int q = 0; q < B::PJ; ++q)
-              *reinterpret_cast<uint4*>(L16 + q * B::s_plane + (32 * x + l32) * B::pitch_tok + 32 * y + 2 * r0 + 8 * half) = fp[q];
+              for (int r = 0; r < 8; ++r) w[r] *= (float)(32 * (x - y) + l32 - 2 * r0 - 8 * half - r);
+              split8<3>(w, *reinterpret_cast<uint4(*)[3]>(fl));
+            }
+#pragma unroll
+            for (int q = 0; q < J + B::PL; ++q) *reinterpret_cast<uint4*>(dst + q * B::s_plane) = fp[q];
           }
         }
         __syncthreads();
@@ -440,13 +443,13 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
     }
     // the state takes gamma^L M, its tangent gamma^L (M' + L M)
     {
-      const Decay gamma = count == C ? gamma_full : gamma_part;
+      const float gamma = count == C ? gamma_full.next() : gamma_part;
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          if (TAN) tm[rb][r] = gamma.times(__builtin_fmaf((float)count, m[rb][r], tm[rb][r]));
-          m[rb][r] = gamma.times(m[rb][r]);
+          if (TAN) tm[rb][r] = gamma * __builtin_fmaf((float)count, m[rb][r], tm[rb][r]);
+          m[rb][r] *= gamma;
         }
     }
     // over the tokens: out^T += c^T scores^T, M += b^T (decayed c)
@@ -460,46 +463,36 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
       if constexpr (OUT) {
 #pragma unroll
         for (int x = kk / 2; x < TI; ++x) {
-          uint4 fp[B::PJ];
-          float w[8];
+          uint4 fp[J], fl[TAN ? 3 : 1];
           if constexpr (B::shared_scores) {
+            const u16* const src = L16 + (32 * x + l32) * B::pitch_tok + 16 * kk + 8 * half;
 #pragma unroll
-            for (int q = 0; q < B::PJ; ++q)
-              fp[q] = *reinterpret_cast<const uint4*>(L16 + q * B::s_plane + (32 * x + l32) * B::pitch_tok + 16 * kk + 8 * half);
+            for (int q = 0; q < J; ++q) fp[q] = *reinterpret_cast<const uint4*>(src + q * B::s_plane);
+            if constexpr (TAN)
+#pragma unroll
+              for (int q = 0; q < 3; ++q) fl[q] = *reinterpret_cast<const uint4*>(src + (J + q) * B::s_plane);
           } else {
+            float w[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) w[k] = s[0][8 * kk + k];
-            split8<B::PJ>(w, fp);
+            split8<J>(w, fp);
+            if constexpr (TAN) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) w[k] *= (float)(l32 - 16 * kk - 8 * half - k);
+              split8<3>(w, fl);
+            }
           }
 #pragma unroll
           for (int q = 0; q < NP; ++q)
 #pragma unroll
             for (int z = 0; z < J; ++z)
               if (q + z < J) o[x] = mfma(fc[q], fp[z], o[x]);
-          if constexpr (TAN) {
-            if constexpr (B::shared_scores) {  // (three pieces are the score itself)
-#pragma unroll
-              for (int k = 0; k < 8; ++k) w[k] = 0.0f;
-#pragma unroll
-              for (int q = B::PJ - 1; q >= 0; --q) {
-                const unsigned d[4] = {fp[q].x, fp[q].y, fp[q].z, fp[q].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  w[2 * k] += __uint_as_float(d[k] << 16);
-                  w[2 * k + 1] += __uint_as_float(d[k] & 0xffff0000u);
-                }
-              }
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] *= (float)(32 * x + l32 - 16 * kk - 8 * half - k);
-            uint4 fl[3];
-            split8<3>(w, fl);
+          if constexpr (TAN)
 #pragma unroll
             for (int q = 0; q < NP; ++q)
 #pragma unroll
               for (int z = 0; z < 3; ++z)
                 if (q + z < 3) ol[x] = mfma(fc[q], fl[z], ol[x]);
-          }
         }
       }
       float cv[8];
@@ -562,11 +555,9 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
               for (int k = 0; k < 4; ++k) sum = __builtin_fmaf(to_f32(xv[k]), ol[x][4 * q + k], sum);
             }
           }
-          dg += (double)sum * (double)p.scale;
+          dg += (double)sum;
         }
-        float ov[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ov[r] = o[x][r] * p.scale;
+        const floatx16 ov = o[x];
         const size_t row = (((size_t)b * p.tokens + tok) * p.heads + h) * cols;
         if (sizeof(T) == 4 || p.out_f32) {
           float* dst = static_cast<float*>(p.out) + row + n4;

@@ -12,6 +12,24 @@ struct Decay {
   __device__ __forceinline__ float times(float m) const { return __builtin_fmaf(m, hi, m * lo); }
 };
 
+// The same as one fp32 factor a step: of the two fp32 around gamma, the one that brings the product so far nearer to the
+// power, so that the product stays within a half ulp of it however many steps there are.
+struct DecaySteps {
+  float below, above, err_below, err_above, err = 0.0f;
+  __device__ __forceinline__ explicit DecaySteps(double x) {
+    const float near = (float)x;
+    below = (double)near <= x ? near : __uint_as_float(__float_as_uint(near) - 1);
+    above = (double)near >= x ? near : __uint_as_float(__float_as_uint(near) + 1);
+    err_below = x > 0.0 ? (float)(((double)below - x) / x) : 0.0f;
+    err_above = x > 0.0 ? (float)(((double)above - x) / x) : 0.0f;
+  }
+  __device__ __forceinline__ float next() {
+    const bool down = err > 0.0f;
+    err += down ? err_below : err_above;
+    return down ? below : above;
+  }
+};
+
 // log decays of -inf (no memory) are taken as -1e5: gamma^0 stays 1 and every other power is 0
 __device__ __forceinline__ float log_decay_of(const float* g, int h) { return fmaxf(g[h], -1e5f); }
 
