@@ -7,8 +7,8 @@
 // (c over its top is c times the rounded reciprocal.)  The square law spends the codes where moments are (their logarithm is what varies): a step is 1.6 % of a value at the
 // top of a block and values down to 6e-5 (m) and 2e-10 (v) of it keep a code; v's are the squares of m's in range, so that
 // a value's m rounds to zero before its v does.  A step decodes, updates in fp32 from the decoded values, uses the
-// unrounded m and v for the parameter, and only then encodes.  Every operation is one IEEE fp32 operation in
-// the written order (no contraction): codes do not depend on the compiler.
+// unrounded m and v for the parameter, and only then encodes.  m, v and the codes are what IEEE fp32 operations in the
+// written order give (no contraction): they do not depend on the compiler.
 // Memory bound: 28 bytes a value with fp32 parameters and states, 16 with 8-bit states.
 #include <type_traits>
 
@@ -65,13 +65,24 @@ __device__ __forceinline__ unsigned wave_max(unsigned x) {
   for (int o = 32; o > 0; o /= 2) x = max(x, (unsigned)__shfl_xor((int)x, o));
   return x;
 }
-__device__ __forceinline__ int value_code(float x, float s, float top, bool fourth) {
-  const float r = s > 0.0f ? fabsf(x) / s : 0.0f;
-  float t = sqrtf(r);
+// the code by its definition: IEEE division, roots and product, each rounded
+__device__ __noinline__ float root_place(float x, float s, float top, bool fourth) {
+  float t = sqrtf(fabsf(x) / s);
   if (fourth) t = sqrtf(t);
-  t = rintf(t * top);
-  return t <= top ? (x < 0.0f ? -(int)t : (int)t) : 0;  // NaN: 0 (the scale says it)
+  return rintf(t * top);
 }
+// The same code by approximate division and roots (all of it within 8 ulp, 2e-4 of a code's step) wherever that is 1e-3 of a step
+// and more from the middle between two codes; elsewhere by the definition.  inv: approximate 1 / s, 0 where s is 0 or
+// not normal enough for it (the definition decides then).
+__device__ __forceinline__ int value_code(float x, float s, float inv, float top, bool fourth) {
+  float t = __builtin_amdgcn_sqrtf(fabsf(x) * inv);
+  if (fourth) t = __builtin_amdgcn_sqrtf(t);
+  const float u = t * top, f = __builtin_amdgcn_fractf(u);
+  float c = rintf(u);
+  if (!(fabsf(f - 0.5f) > 1e-3f) || inv == 0.0f) c = s > 0.0f ? root_place(x, s, top, fourth) : 0.0f;
+  return c <= top ? (x < 0.0f ? -(int)c : (int)c) : 0;  // NaN: 0 (the scale says it)
+}
+__device__ __forceinline__ float scale_inverse(float s) { return s > 1e-30f && s < 1e30f ? __builtin_amdgcn_rcpf(s) : 0.0f; }
 
 __device__ __forceinline__ int tensor_of(const unsigned* first, int count, unsigned block) {
   int lo = 0, hi = count;  // the last tensor whose first workgroup is not past this one
@@ -150,7 +161,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamTable tab, AdamArgs a) {
       m = m * a.beta1 + g * a.one_beta1;
       v = v * a.beta2 + (g * g) * a.one_beta2;
       const float p = master ? w4[u].v[j] : to_f32(p4[u].v[j]);
-      po.v[j] = p * a.decay - a.step_size * (m / (sqrtf(v) / a.root_bc2 + a.eps));
+      // (root and quotient of the step are the hardware's, 1 ulp each: 1e-7 of a step)
+      po.v[j] = p * a.decay - a.step_size * (m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * a.inv_root_bc2 + a.eps));
       mo.v[j] = m;
       vo.v[j] = v;
       if (i + j < n) {  // (past the end: nothing may enter the block's scale)
@@ -168,12 +180,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamTable tab, AdamArgs a) {
       store4(tv, i, n, whole, vo);
     } else {
       const float sm = __uint_as_float(wave_max(top_m)), sv = __uint_as_float(wave_max(top_v));
+      const float im = scale_inverse(sm), iv = scale_inverse(sv);
       Four<M> mc;
       Four<V> vc;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        mc.v[j] = (M)value_code(mo.v[j], sm, 127.0f, false);
-        vc.v[j] = (V)value_code(vo.v[j], sv, 255.0f, true);
+        mc.v[j] = (M)value_code(mo.v[j], sm, im, 127.0f, false);
+        vc.v[j] = (V)value_code(vo.v[j], sv, iv, 255.0f, true);
       }
       store4(tm, i, n, whole, mc);
       store4(tv, i, n, whole, vc);

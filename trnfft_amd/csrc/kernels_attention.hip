@@ -184,14 +184,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPass p) {
   const double g = (double)log_decay_of(p.log_decay, (int)(bh % p.heads));
   const Decay whole(exp(g * (double)p.seg_tokens));
   float m = p.m_in ? p.m_in[i] * p.m_in_scale : 0.0f;
-  for (int k = 0; k < p.segments; ++k) {
-    const int s = p.reverse ? p.segments - 1 - k : k;
-    float* at = p.seg_state + s * all + i;
-    const bool end = k == p.segments - 1;
-    const float own = end ? 0.0f : *at;
-    *at = m;
-    const long long tokens = min(max(len - s * p.seg_tokens, 0LL), p.seg_tokens);
-    m = (tokens == p.seg_tokens ? whole : Decay(exp(g * (double)tokens))).times(m) + own;
+  constexpr int U = 8;  // sums on their way at a time
+  for (int k0 = 0; k0 < p.segments; k0 += U) {
+    float own[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u, s = p.reverse ? p.segments - 1 - k : k;
+      own[u] = k < p.segments - 1 ? p.seg_state[s * all + i] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u, s = p.reverse ? p.segments - 1 - k : k;
+      if (k >= p.segments) break;
+      p.seg_state[s * all + i] = m;
+      const long long tokens = min(max(len - s * p.seg_tokens, 0LL), p.seg_tokens);
+      m = (tokens == p.seg_tokens ? whole : Decay(exp(g * (double)tokens))).times(m) + own[u];
+    }
   }
 }
 

@@ -9,25 +9,49 @@
 #include "model_ops.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tfa {
 
 enum { kActNone = 0, kActSilu = 1, kActGelu = 2, kActRelu = 3 };
 
+// e^-x by the hardware's exp2, a few 1e-7 of the result where it matters (x from -20 to 20)
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * -1.4426950408889634f); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_neg(z)); }
+
+// Phi(z), the normal distribution: 1 - erf by Abramowitz and Stegun 7.1.26 (1.5e-7 absolute), on the side where it
+// is small, so that nothing cancels; `bell` receives e^(-z^2 / 2), which the slope needs too.
+__device__ __forceinline__ float normal_cdf(float z, float& bell) {
+  const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+  bell = exp_neg(x * x);
+  float q = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+  q = __builtin_fmaf(t, q, 1.421413741f);
+  q = __builtin_fmaf(t, q, -0.284496736f);
+  q = __builtin_fmaf(t, q, 0.254829592f);
+  const float tail = 0.5f * q * t * bell;
+  return z < 0.0f ? tail : 1.0f - tail;  // (NaN stays: it is in tail)
+}
+
 __device__ __forceinline__ float activate(float z, int act) {
-  if (act == kActSilu) return z / (1.0f + expf(-z));
-  if (act == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if (act == kActSilu) return z * sigmoid(z);
+  if (act == kActGelu) {
+    float bell;
+    return z * normal_cdf(z, bell);
+  }
   if (act == kActRelu) return z > 0.0f ? z : z != z ? z : 0.0f;  // NaN stays
   return z;
 }
 
 __device__ __forceinline__ float activation_slope(float z, int act) {
   if (act == kActSilu) {
-    const float s = 1.0f / (1.0f + expf(-z));
-    return s * (1.0f + z * (1.0f - s));
+    const float s = sigmoid(z);
+    return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
   }
-  if (act == kActGelu)
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+  if (act == kActGelu) {
+    float bell;
+    const float cdf = normal_cdf(z, bell);
+    return __builtin_fmaf(z * 0.39894228040143268f, bell, cdf);
+  }
   if (act == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
   return 1.0f;
 }
@@ -97,26 +121,42 @@ __global__ __launch_bounds__(kNormThreads) void norm_stats_kernel(NormArgs a, lo
   if (s.on)
     for (long long r = r0 + s.lane; r < r1; r += (long long)U * s.lanes) {
       float v[U][V];
-      const int full = (int)min((long long)U, (r1 - r + s.lanes - 1) / s.lanes);
+      const bool whole = r + (long long)(U - 1) * s.lanes < r1;
+      const int full = whole ? U : (int)((r1 - r + s.lanes - 1) / s.lanes);
+      if (whole) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)  // (rows past the end repeat the last: in bounds, weight 0)
-        load_pack<T, V>(x + (r + (long long)min(u, full - 1) * s.lanes) * a.channels, v[u]);
-      const float inv = 1.0f / (float)full, f = (float)full / (count + (float)full);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float sum = 0.0f, sq = 0.0f;
-#pragma unroll
-        for (int u = 0; u < U; ++u) sum += u < full ? v[u][i] : 0.0f;
-        sum *= inv;
+        for (int u = 0; u < U; ++u) load_pack<T, V>(x + (r + (long long)u * s.lanes) * a.channels, v[u]);
+      } else {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const float d = u < full ? v[u][i] - sum : 0.0f;
-          sq = __builtin_fmaf(d, d, sq);
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[u][i] = 0.0f;
+          if (u < full) load_pack<T, V>(x + (r + (long long)u * s.lanes) * a.channels, v[u]);
         }
-        const float d = sum - mean[i];
-        mean[i] = __builtin_fmaf(d, f, mean[i]);
-        m2[i] += sq + d * d * count * f;
       }
+      const float inv = 1.0f / (float)full, f = (float)full / (count + (float)full);
+      auto add = [&](auto all) {
+        constexpr bool ALL = decltype(all)::value;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float sum = 0.0f, sq = 0.0f;
+#pragma unroll
+          for (int u = 0; u < U; ++u) sum += v[u][i];
+          sum *= inv;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const float d = ALL || u < full ? v[u][i] - sum : 0.0f;
+            sq = __builtin_fmaf(d, d, sq);
+          }
+          const float d = sum - mean[i];
+          mean[i] = __builtin_fmaf(d, f, mean[i]);
+          m2[i] += sq + d * d * count * f;
+        }
+      };
+      if (whole)
+        add(std::true_type{});
+      else
+        add(std::false_type{});
       count += (float)full;
     }
   if (s.on)
@@ -163,12 +203,14 @@ __global__ __launch_bounds__(64) void norm_join_kernel(NormArgs a, int splits, l
   }
 }
 
+// (from the last rows to the first: what the statistics read last is still in the Infinity Cache)
 template <typename T, int V>
 __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, long long rows_each, unsigned splits) {
   const Slab s = slab_of<V>(a.channels);
   if (!s.on) return;
-  const long long n = blockIdx.x / splits, live = live_positions(a, n);
-  const long long r0 = (blockIdx.x % splits) * rows_each, r1 = min(r0 + rows_each, a.positions);
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const long long n = block / splits, live = live_positions(a, n);
+  const long long r0 = (block % splits) * rows_each, r1 = min(r0 + rows_each, a.positions);
   const int each = a.channels / a.groups;
   float mean[V], mul[V], add[V];
 #pragma unroll
@@ -181,14 +223,24 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, lo
   const size_t at = (size_t)n * a.positions * a.channels + s.col;
   const T* x = static_cast<const T*>(a.x) + at;
   T* y = static_cast<T*>(a.y) + at;
-  for (long long r = r0 + s.lane; r < r1; r += s.lanes) {
-    float v[V] = {};
-    if (r < live) {
-      load_pack<T, V>(x + r * a.channels, v);
+  constexpr int U = 4;
+  for (long long r = r0 + s.lane; r < r1; r += (long long)U * s.lanes) {
+    Pack<T, V> v[U];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = activate(__builtin_fmaf(v[i] - mean[i], mul[i], add[i]), a.act);
+    for (int u = 0; u < U; ++u) {
+      const long long q = r + (long long)u * s.lanes;
+      if (q < r1 && q < live) v[u] = *reinterpret_cast<const Pack<T, V>*>(x + q * a.channels);
     }
-    store_pack<T, V>(y + r * a.channels, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long q = r + (long long)u * s.lanes;
+      if (q >= r1) break;
+      float z[V] = {};
+      if (q < live)
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = activate(__builtin_fmaf(to_f32(v[u].v[i]) - mean[i], mul[i], add[i]), a.act);
+      store_pack<T, V>(y + q * a.channels, z);
+    }
   }
 }
 
@@ -265,23 +317,32 @@ __global__ __launch_bounds__(64) void norm_grad_join_kernel(NormArgs a, int spli
 }
 
 // dbias[c], dweight[c]: 32 channels a workgroup, the partials of all samples and splits in a fixed order
-__global__ __launch_bounds__(256) void norm_weight_grad_kernel(NormArgs a, long long parts) {
-  __shared__ float red[2][8][32];
-  const int c = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
+__global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* __restrict__ partial, float* __restrict__ dweight,
+                                                                float* __restrict__ dbias, int channels, long long parts) {
+  __shared__ float red[2][32][33];
+  const int cl = threadIdx.x % 32, c = blockIdx.x * 32 + cl, lane = threadIdx.x / 32;
+  constexpr int U = 8;
   float u = 0.0f, q = 0.0f;
-  if (c < a.channels)
-    for (long long i = lane; i < parts; i += 8) {
-      const float* src = a.ws + i * 2 * a.channels + c;
-      u += src[0];
-      q += src[a.channels];
+  if (c < channels)
+    for (long long i = lane; i < parts; i += 32 * U) {
+      float p[U], r[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const bool in = i + 32 * k < parts;
+        const float* src = partial + (i + 32 * k) * 2 * channels + c;
+        p[k] = in ? src[0] : 0.0f;
+        r[k] = in ? src[channels] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) u += p[k], q += r[k];
     }
-  red[0][lane][threadIdx.x % 32] = u;
-  red[1][lane][threadIdx.x % 32] = q;
+  red[0][lane][cl] = u;
+  red[1][lane][cl] = q;
   __syncthreads();
-  if (lane == 0 && c < a.channels) {
-    for (int l = 1; l < 8; ++l) u += red[0][l][threadIdx.x], q += red[1][l][threadIdx.x];
-    if (a.dbias) a.dbias[c] = u;
-    if (a.dweight) a.dweight[c] = q;
+  if (lane == 0 && c < channels) {
+    for (int l = 1; l < 32; ++l) u += red[0][l][cl], q += red[1][l][cl];
+    if (dbias) dbias[c] = u;
+    if (dweight) dweight[c] = q;
   }
 }
 
@@ -289,8 +350,9 @@ template <typename T, int V>
 __global__ __launch_bounds__(kNormThreads) void norm_grad_kernel(NormArgs a, long long rows_each, unsigned splits, const float* joined) {
   const Slab s = slab_of<V>(a.channels);
   if (!s.on) return;
-  const long long n = blockIdx.x / splits, live = live_positions(a, n);
-  const long long r0 = (blockIdx.x % splits) * rows_each, r1 = min(r0 + rows_each, a.positions);
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const long long n = block / splits, live = live_positions(a, n);
+  const long long r0 = (block % splits) * rows_each, r1 = min(r0 + rows_each, a.positions);
   const int each = a.channels / a.groups;
   float mean[V], rstd[V], w[V], b[V], c1[V], c2[V];
 #pragma unroll
@@ -324,6 +386,209 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_kernel(NormArgs a, lon
 }
 
 // ------------------------------------------------------------------------------------------------
+// Samples that fit a workgroup's registers: one launch, every value read once.  A workgroup takes whole groups of one
+// sample, some 128 bytes of each position (a cache line), K 16-byte vectors a thread.  Statistics are two passes over the
+// registers.  Gradients keep x and dy; the activation's slope is computed twice, which is cheaper than keeping it.
+// ------------------------------------------------------------------------------------------------
+
+struct NormTile {
+  int threads, vecs, lanes, groups, k;  // vectors of a position in the tile, as lanes: a power of two; groups of a tile; K
+  unsigned tiles;
+};
+
+// (sum over the rows and the group's vectors of two values a thread; lanes of one vector are `lanes` apart)
+template <int W>
+__device__ __forceinline__ void group_sum(float& u, float& q, float (*red)[64][2], int lanes, int col, int group_vecs, int vecs) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int o = lanes; o < 64; o *= 2) u += __shfl_xor(u, o), q += __shfl_xor(q, o);
+  __syncthreads();
+  if (lane < lanes) red[wave][lane][0] = u, red[wave][lane][1] = q;
+  __syncthreads();
+  u = q = 0.0f;
+  const int c0 = col / group_vecs * group_vecs;
+  if (col < vecs)
+    for (int w = 0; w < W; ++w)
+      for (int c = 0; c < group_vecs; ++c) u += red[w][c0 + c][0], q += red[w][c0 + c][1];
+}
+
+template <typename T, int V, int K, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_whole_kernel(NormArgs a, NormTile t) {
+  __shared__ float red[THREADS / 64][64][2];
+  const long long n = blockIdx.x / t.tiles;
+  const int each = a.channels / a.groups, group_vecs = each / V;
+  const int g0 = (int)(blockIdx.x % t.tiles) * t.groups, vecs = min(t.groups, a.groups - g0) * group_vecs;
+  const int col = threadIdx.x % t.lanes, row = threadIdx.x / t.lanes, rows = THREADS / t.lanes;
+  const int live = (int)live_positions(a, n), positions = (int)a.positions;
+  const bool on = col < vecs;
+  const int ch = g0 * each + col * V, g = g0 + (on ? col / group_vecs : 0);
+  const size_t at = (size_t)n * a.positions * a.channels + ch;
+  const T* x = static_cast<const T*>(a.x) + at;
+  Pack<T, V> v[K];
+  float sum = 0.0f, unused = 0.0f;
+  // (sums are of distances from one of the group's values: a mean far from zero costs nothing)
+  const float pivot = on && live ? to_f32(static_cast<const T*>(a.x)[(size_t)n * a.positions * a.channels + g * each]) : 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[k].v[i] = from_f32<T>(0.0f);
+    const int r = row + k * rows;
+    if (on && r < live) v[k] = *reinterpret_cast<const Pack<T, V>*>(x + (size_t)r * a.channels);
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (on && row + k * rows < live)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum += to_f32(v[k].v[i]) - pivot;
+  group_sum<THREADS / 64>(sum, unused, red, t.lanes, col, group_vecs, vecs);
+  const float count = (float)live * (float)each, mean = live ? pivot + sum / count : 0.0f;
+  float m2 = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (row + k * rows < live)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = to_f32(v[k].v[i]) - mean;
+        m2 = __builtin_fmaf(d, d, m2);
+      }
+  if (!on) m2 = 0.0f;
+  group_sum<THREADS / 64>(m2, unused, red, t.lanes, col, group_vecs, vecs);
+  const float rstd = 1.0f / sqrtf((live ? m2 / count : 0.0f) + a.eps);
+  if (!on) return;
+  if (row == 0 && col % group_vecs == 0) {
+    a.mean[n * a.groups + g] = mean;
+    a.rstd[n * a.groups + g] = rstd;
+  }
+  float mul[V], add[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    mul[i] = rstd * (a.weight ? a.weight[ch + i] : 1.0f);
+    add[i] = a.bias ? a.bias[ch + i] : 0.0f;
+  }
+  T* y = static_cast<T*>(a.y) + at;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int r = row + k * rows;
+    if (r >= positions) break;
+    float z[V] = {};
+    if (r < live)
+#pragma unroll
+      for (int i = 0; i < V; ++i) z[i] = activate(__builtin_fmaf(to_f32(v[k].v[i]) - mean, mul[i], add[i]), a.act);
+    store_pack<T, V>(y + (size_t)r * a.channels, z);
+  }
+}
+
+// the same for the gradients; partial sums of dz and dz xhat by channel at ws[(n * 2 + {0, 1}) * channels + c]
+template <typename T, int V, int K, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_whole_grad_kernel(NormArgs a, NormTile t) {
+  __shared__ float red[THREADS / 64][64][2];
+  __shared__ float part[THREADS / 64][64 * V];
+  const long long n = blockIdx.x / t.tiles;
+  const int each = a.channels / a.groups, group_vecs = each / V;
+  const int g0 = (int)(blockIdx.x % t.tiles) * t.groups, vecs = min(t.groups, a.groups - g0) * group_vecs;
+  const int col = threadIdx.x % t.lanes, row = threadIdx.x / t.lanes, rows = THREADS / t.lanes;
+  const int live = (int)live_positions(a, n), positions = (int)a.positions;
+  const bool on = col < vecs;
+  const int ch = on ? g0 * each + col * V : g0 * each, g = g0 + (on ? col / group_vecs : 0);
+  const size_t at = (size_t)n * a.positions * a.channels + ch;
+  const T* x = static_cast<const T*>(a.x) + at;
+  const T* dy = static_cast<const T*>(a.dy) + at;
+  Pack<T, V> v[K], d[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int r = row + k * rows;
+    if (on && r < live) {
+      v[k] = *reinterpret_cast<const Pack<T, V>*>(x + (size_t)r * a.channels);
+      d[k] = *reinterpret_cast<const Pack<T, V>*>(dy + (size_t)r * a.channels);
+    }
+  }
+  const float mean = a.mean[n * a.groups + g], rstd = a.rstd[n * a.groups + g];
+  float w[V], b[V], s1[V] = {}, s2[V] = {};
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    w[i] = a.weight ? a.weight[ch + i] : 1.0f;
+    b[i] = a.bias ? a.bias[ch + i] : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    __builtin_amdgcn_sched_barrier(0);  // (one vector at a time: registers)
+    if (on && row + k * rows < live)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float xh = (to_f32(v[k].v[i]) - mean) * rstd;
+        const float dz = to_f32(d[k].v[i]) * activation_slope(__builtin_fmaf(xh, w[i], b[i]), a.act);
+        s1[i] += dz;
+        s2[i] = __builtin_fmaf(dz, xh, s2[i]);
+      }
+  }
+  float u = 0.0f, q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) u = __builtin_fmaf(w[i], s1[i], u), q = __builtin_fmaf(w[i], s2[i], q);
+  group_sum<THREADS / 64>(u, q, red, t.lanes, col, group_vecs, vecs);
+  const float count = (float)live * (float)each;
+  const float c1 = live ? u / count : 0.0f, c2 = live ? q / count : 0.0f;
+  if (a.dweight || a.dbias) {
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float s = z ? s2[i] : s1[i];
+        for (int o = t.lanes; o < 64; o *= 2) s += __shfl_xor(s, o);
+        if ((int)(threadIdx.x & 63) < t.lanes) part[threadIdx.x >> 6][(threadIdx.x & 63) * V + i] = s;
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < vecs * V; c += THREADS) {
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < THREADS / 64; ++k) s += part[k][c];
+        a.ws[(n * 2 + z) * a.channels + g0 * each + c] = s;
+      }
+      __syncthreads();
+    }
+  }
+  if (!on) return;
+  // (as new values: xhat and the slope are computed again, not kept for all of K in registers)
+  float mean2 = mean, rstd2 = rstd;
+  asm volatile("" : "+v"(mean2), "+v"(rstd2));
+  T* dx = static_cast<T*>(a.y) + at;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    __builtin_amdgcn_sched_barrier(0);
+    const int r = row + k * rows;
+    if (r >= positions) break;
+    float z[V] = {};
+    if (r < live)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float xh = (to_f32(v[k].v[i]) - mean2) * rstd2;
+        const float e = to_f32(d[k].v[i]) * activation_slope(__builtin_fmaf(xh, w[i], b[i]), a.act) * w[i];
+        z[i] = rstd2 * (e - c1 - xh * c2);
+      }
+    store_pack<T, V>(dx + (size_t)r * a.channels, z);
+  }
+}
+
+// The tile of a sample that a workgroup can hold (threads = 0: none can): K vectors a thread at most 8, of one tensor or two
+static NormTile norm_tile(const NormArgs& a, int size) {
+  NormTile t{};
+  const int V = 16 / size, each = a.channels / a.groups;
+  if (a.channels % V || each % V || each / V > 64) return t;
+  const int group_vecs = each / V;
+  t.groups = std::min(a.groups, std::max(1, 8 / group_vecs));
+  t.vecs = t.groups * group_vecs;
+  t.lanes = 1;
+  while (t.lanes < t.vecs) t.lanes *= 2;
+  t.tiles = (unsigned)((a.groups + t.groups - 1) / t.groups);
+  for (const int threads : {256, 1024}) {
+    const long long rows = threads / t.lanes, k = (a.positions + rows - 1) / rows;
+    if (k > 8 || (threads == 256 && k > 4)) continue;
+    t.threads = threads;
+    t.k = k <= 2 ? 2 : k <= 4 ? 4 : 8;
+    break;
+  }
+  return t;
+}
+
+// ------------------------------------------------------------------------------------------------
 
 // rows of a workgroup: about 2048 workgroups in all, at least 32 rows each, at most 65535 splits
 static long long norm_rows_each(const NormArgs& a) {
@@ -338,6 +603,7 @@ static long long norm_splits(const NormArgs& a) {
 
 size_t norm_workspace_bytes(const NormArgs& a, bool backward) {
   if (a.batch == 0 || a.positions == 0) return 0;
+  // (for the three passes also where whole samples fit: the data's addresses, which have a say in it, are not known here)
   const size_t parts = (size_t)a.batch * norm_splits(a) * 2 * a.channels;
   return sizeof(float) * (parts + (backward ? (size_t)a.batch * a.groups * 2 : 0));
 }
@@ -347,6 +613,30 @@ static bool norm_vectors(const NormArgs& a) {
   constexpr int V = 16 / sizeof(T);
   const uintptr_t any = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.dy);
   return a.channels % V == 0 && any % 16 == 0;
+}
+
+static void weight_grad_launch(const NormArgs& a, long long parts) {
+  hipLaunchKernelGGL(norm_weight_grad_kernel, dim3((a.channels + 31) / 32), dim3(1024), 0, a.stream, a.ws, a.dweight, a.dbias,
+                     a.channels, parts);
+}
+
+template <typename T, int V, int K, int THREADS>
+static hipError_t whole_launch(const NormArgs& a, const NormTile& t, bool backward) {
+  const dim3 grid((unsigned)a.batch * t.tiles), block(THREADS);
+  if (!backward) {
+    hipLaunchKernelGGL((norm_whole_kernel<T, V, K, THREADS>), grid, block, 0, a.stream, a, t);
+  } else {
+    hipLaunchKernelGGL((norm_whole_grad_kernel<T, V, K, THREADS>), grid, block, 0, a.stream, a, t);
+    if (a.dweight || a.dbias) weight_grad_launch(a, a.batch);
+  }
+  return hipGetLastError();
+}
+
+template <typename T, int V>
+static hipError_t whole_sizes(const NormArgs& a, const NormTile& t, bool backward) {
+  if (t.threads == 256) return t.k == 2 ? whole_launch<T, V, 2, 256>(a, t, backward) : whole_launch<T, V, 4, 256>(a, t, backward);
+  if (t.k == 2) return whole_launch<T, V, 2, 1024>(a, t, backward);
+  return t.k == 4 ? whole_launch<T, V, 4, 1024>(a, t, backward) : whole_launch<T, V, 8, 1024>(a, t, backward);
 }
 
 template <typename T, int V>
@@ -369,7 +659,7 @@ static hipError_t backward_launch(const NormArgs& a) {
   hipLaunchKernelGGL((norm_grad_sums_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
   hipLaunchKernelGGL(norm_grad_join_kernel, dim3((unsigned)(a.batch * a.groups)), dim3(64), 0, a.stream, a, (int)splits, joined);
   if (a.dweight || a.dbias)
-    hipLaunchKernelGGL(norm_weight_grad_kernel, dim3((a.channels + 31) / 32), dim3(256), 0, a.stream, a, a.batch * splits);
+    weight_grad_launch(a, a.batch * splits);
   hipLaunchKernelGGL((norm_grad_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits, joined);
   return hipGetLastError();
 }
@@ -377,7 +667,11 @@ static hipError_t backward_launch(const NormArgs& a) {
 template <typename T>
 static hipError_t norm_typed(const NormArgs& a, bool backward) {
   constexpr int V = 16 / sizeof(T);
-  if (norm_vectors<T>(a)) return backward ? backward_launch<T, V>(a) : forward_launch<T, V>(a);
+  if (norm_vectors<T>(a)) {
+    const NormTile t = norm_tile(a, sizeof(T));
+    if (t.threads) return whole_sizes<T, V>(a, t, backward);
+    return backward ? backward_launch<T, V>(a) : forward_launch<T, V>(a);
+  }
   return backward ? backward_launch<T, 1>(a) : forward_launch<T, 1>(a);
 }
 

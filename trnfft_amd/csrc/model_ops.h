@@ -149,7 +149,7 @@ struct AdamArgs {
   float decay;             // 1 - lr * weight_decay
   float beta1, one_beta1, beta2, one_beta2;
   float step_size;         // lr / (1 - beta1^step)
-  float root_bc2, eps;     // sqrt(1 - beta2^step)
+  float inv_root_bc2, eps;  // 1 / sqrt(1 - beta2^step)
 };
 hipError_t launch_adamw(const AdamTensor* tensors, long long count, const AdamArgs& a, hipStream_t stream);
 // out[i] = the values that 8-bit codes stand for (second moments where `squares`)

@@ -438,7 +438,7 @@ int tfa_adamw_step(int64_t count, const tfa_adam_tensor* tensors, const tfa_adam
   a.decay = (float)(1.0 - d.lr * d.weight_decay);
   a.beta1 = (float)d.beta1, a.one_beta1 = (float)(1.0 - d.beta1), a.beta2 = (float)d.beta2, a.one_beta2 = (float)(1.0 - d.beta2);
   a.step_size = (float)(d.lr / (1.0 - std::pow(d.beta1, (double)d.step)));
-  a.root_bc2 = (float)std::sqrt(1.0 - std::pow(d.beta2, (double)d.step));
+  a.inv_root_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(d.beta2, (double)d.step)));
   a.eps = (float)d.eps;
   static_assert(sizeof(tfa_adam_tensor) == sizeof(tfa::AdamTensor), "one layout");
   const hipError_t e = tfa::launch_adamw(reinterpret_cast<const tfa::AdamTensor*>(tensors), count, a, static_cast<hipStream_t>(stream));
