@@ -75,6 +75,20 @@ __device__ __forceinline__ void store_pack(T* p, const float (&x)[V]) {
   *reinterpret_cast<Pack<T, V>*>(p) = u;
 }
 
+// a vector as it lies in memory, so that one waits in registers at its own size
+template <typename T, int V>
+struct __attribute__((aligned(V * sizeof(T)))) Raw {
+  unsigned w[V * sizeof(T) / 4];
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    const unsigned u = w[i / 2];
+    if constexpr (std::is_same_v<T, __bf16>)
+      return __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16);
+    else
+      return (float)__builtin_bit_cast(_Float16, (unsigned short)(i % 2 ? u >> 16 : u));
+  }
+};
+
 __device__ __forceinline__ long long live_positions(const NormArgs& a, long long n) {
   if (!a.lengths) return a.positions;
   return min(max(a.lengths[n], 0LL), a.positions / a.inner) * a.inner;
@@ -423,22 +437,21 @@ __global__ __launch_bounds__(THREADS) void norm_whole_kernel(NormArgs a, NormTil
   const int ch = g0 * each + col * V, g = g0 + (on ? col / group_vecs : 0);
   const size_t at = (size_t)n * a.positions * a.channels + ch;
   const T* x = static_cast<const T*>(a.x) + at;
-  Pack<T, V> v[K];
+  Raw<T, V> v[K];
   float sum = 0.0f, unused = 0.0f;
   // (sums are of distances from one of the group's values: a mean far from zero costs nothing)
   const float pivot = on && live ? to_f32(static_cast<const T*>(a.x)[(size_t)n * a.positions * a.channels + g * each]) : 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[k].v[i] = from_f32<T>(0.0f);
+    for (unsigned& w : v[k].w) w = 0;
     const int r = row + k * rows;
-    if (on && r < live) v[k] = *reinterpret_cast<const Pack<T, V>*>(x + (size_t)r * a.channels);
+    if (on && r < live) v[k] = *reinterpret_cast<const Raw<T, V>*>(x + (size_t)r * a.channels);
   }
 #pragma unroll
   for (int k = 0; k < K; ++k)
     if (on && row + k * rows < live)
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum += to_f32(v[k].v[i]) - pivot;
+      for (int i = 0; i < V; ++i) sum += v[k].at(i) - pivot;
   group_sum<THREADS / 64>(sum, unused, red, t.lanes, col, group_vecs, vecs);
   const float count = (float)live * (float)each, mean = live ? pivot + sum / count : 0.0f;
   float m2 = 0.0f;
@@ -447,7 +460,7 @@ __global__ __launch_bounds__(THREADS) void norm_whole_kernel(NormArgs a, NormTil
     if (row + k * rows < live)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float d = to_f32(v[k].v[i]) - mean;
+        const float d = v[k].at(i) - mean;
         m2 = __builtin_fmaf(d, d, m2);
       }
   if (!on) m2 = 0.0f;
@@ -467,12 +480,13 @@ __global__ __launch_bounds__(THREADS) void norm_whole_kernel(NormArgs a, NormTil
   T* y = static_cast<T*>(a.y) + at;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
+    __builtin_amdgcn_sched_barrier(0);  // (one vector at a time: registers)
     const int r = row + k * rows;
     if (r >= positions) break;
     float z[V] = {};
     if (r < live)
 #pragma unroll
-      for (int i = 0; i < V; ++i) z[i] = activate(__builtin_fmaf(to_f32(v[k].v[i]) - mean, mul[i], add[i]), a.act);
+      for (int i = 0; i < V; ++i) z[i] = activate(__builtin_fmaf(v[k].at(i) - mean, mul[i], add[i]), a.act);
     store_pack<T, V>(y + (size_t)r * a.channels, z);
   }
 }
@@ -492,13 +506,13 @@ __global__ __launch_bounds__(THREADS) void norm_whole_grad_kernel(NormArgs a, No
   const size_t at = (size_t)n * a.positions * a.channels + ch;
   const T* x = static_cast<const T*>(a.x) + at;
   const T* dy = static_cast<const T*>(a.dy) + at;
-  Pack<T, V> v[K], d[K];
+  Raw<T, V> v[K], d[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int r = row + k * rows;
     if (on && r < live) {
-      v[k] = *reinterpret_cast<const Pack<T, V>*>(x + (size_t)r * a.channels);
-      d[k] = *reinterpret_cast<const Pack<T, V>*>(dy + (size_t)r * a.channels);
+      v[k] = *reinterpret_cast<const Raw<T, V>*>(x + (size_t)r * a.channels);
+      d[k] = *reinterpret_cast<const Raw<T, V>*>(dy + (size_t)r * a.channels);
     }
   }
   const float mean = a.mean[n * a.groups + g], rstd = a.rstd[n * a.groups + g];
@@ -514,8 +528,8 @@ __global__ __launch_bounds__(THREADS) void norm_whole_grad_kernel(NormArgs a, No
     if (on && row + k * rows < live)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float xh = (to_f32(v[k].v[i]) - mean) * rstd;
-        const float dz = to_f32(d[k].v[i]) * activation_slope(__builtin_fmaf(xh, w[i], b[i]), a.act);
+        const float xh = (v[k].at(i) - mean) * rstd;
+        const float dz = d[k].at(i) * activation_slope(__builtin_fmaf(xh, w[i], b[i]), a.act);
         s1[i] += dz;
         s2[i] = __builtin_fmaf(dz, xh, s2[i]);
       }
@@ -559,15 +573,16 @@ __global__ __launch_bounds__(THREADS) void norm_whole_grad_kernel(NormArgs a, No
     if (r < live)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float xh = (to_f32(v[k].v[i]) - mean2) * rstd2;
-        const float e = to_f32(d[k].v[i]) * activation_slope(__builtin_fmaf(xh, w[i], b[i]), a.act) * w[i];
+        const float xh = (v[k].at(i) - mean2) * rstd2;
+        const float e = d[k].at(i) * activation_slope(__builtin_fmaf(xh, w[i], b[i]), a.act) * w[i];
         z[i] = rstd2 * (e - c1 - xh * c2);
       }
     store_pack<T, V>(dx + (size_t)r * a.channels, z);
   }
 }
 
-// The tile of a sample that a workgroup can hold (threads = 0: none can): K vectors a thread at most 8, of one tensor or two
+// The tile of a sample that a workgroup can hold (threads = 0: none can): K vectors a thread, of one tensor or two. Few threads with many vectors
+// leave room for several workgroups a compute unit, which cover each other's reductions (1024 threads of 5 vectors: one fits)
 static NormTile norm_tile(const NormArgs& a, int size) {
   NormTile t{};
   const int V = 16 / size, each = a.channels / a.groups;
@@ -578,11 +593,11 @@ static NormTile norm_tile(const NormArgs& a, int size) {
   t.lanes = 1;
   while (t.lanes < t.vecs) t.lanes *= 2;
   t.tiles = (unsigned)((a.groups + t.groups - 1) / t.groups);
-  for (const int threads : {256, 1024}) {
+  for (const int threads : {256, 512}) {
     const long long rows = threads / t.lanes, k = (a.positions + rows - 1) / rows;
-    if (k > 8 || (threads == 256 && k > 4)) continue;
+    if (k > (threads == 256 ? 20 : 16)) continue;  // (20: the most that leaves the backward two waves a SIMD)
     t.threads = threads;
-    t.k = k <= 2 ? 2 : k <= 4 ? 4 : 8;
+    t.k = threads == 512 ? 16 : k <= 2 ? 2 : k <= 8 ? 8 : k <= 14 ? 14 : 20;
     break;
   }
   return t;
@@ -634,9 +649,9 @@ static hipError_t whole_launch(const NormArgs& a, const NormTile& t, bool backwa
 
 template <typename T, int V>
 static hipError_t whole_sizes(const NormArgs& a, const NormTile& t, bool backward) {
-  if (t.threads == 256) return t.k == 2 ? whole_launch<T, V, 2, 256>(a, t, backward) : whole_launch<T, V, 4, 256>(a, t, backward);
-  if (t.k == 2) return whole_launch<T, V, 2, 1024>(a, t, backward);
-  return t.k == 4 ? whole_launch<T, V, 4, 1024>(a, t, backward) : whole_launch<T, V, 8, 1024>(a, t, backward);
+  if (t.threads == 512) return whole_launch<T, V, 16, 512>(a, t, backward);
+  if (t.k <= 8) return t.k == 2 ? whole_launch<T, V, 2, 256>(a, t, backward) : whole_launch<T, V, 8, 256>(a, t, backward);
+  return t.k == 14 ? whole_launch<T, V, 14, 256>(a, t, backward) : whole_launch<T, V, 20, 256>(a, t, backward);
 }
 
 template <typename T, int V>

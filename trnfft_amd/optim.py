@@ -8,6 +8,7 @@ s (c / 255)^4 of uint8 codes.  The reference has no counterpart.
 from __future__ import annotations
 
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -22,20 +23,20 @@ def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
+_dtype = attrgetter("dtype")
+
+
 def _same(what: str, name: str, tensors, sizes, dtype, dev) -> list[int]:
-    """Addresses of a list whose tensors have to match the parameters'."""
+    """Addresses of a list whose tensors have to match the parameters' (checked in bulk: hundreds of tensors a step)."""
     if len(tensors) != len(sizes):
         raise ValueError(f"{what}: {len(sizes)} parameters, but {len(tensors)} {name}")
-    addresses = []
-    for t, n in zip(tensors, sizes):
-        if t.dtype != dtype:
-            raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
-        if t.device != dev:
-            raise ValueError(f"{what}: {name} must be on {dev}, got {t.device}")
-        if t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be contiguous, with the size its parameter asks for")
-        addresses.append(t.data_ptr())
-    return addresses
+    if set(map(_dtype, tensors)) != {dtype}:
+        raise TypeError(f"{what}: {name} must be {dtype}, got {set(map(_dtype, tensors)) - {dtype}}")
+    if set(map(torch.Tensor.get_device, tensors)) != {dev.index}:
+        raise ValueError(f"{what}: {name} must be on {dev}")
+    if list(map(torch.Tensor.numel, tensors)) != sizes or not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise ValueError(f"{what}: {name} must be contiguous, with the size its parameter asks for")
+    return list(map(torch.Tensor.data_ptr, tensors))
 
 
 def _table(columns, count: int) -> array:
@@ -75,12 +76,12 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
     _require_hip(what)
     if dev.type != "cuda":
         raise ValueError(f"{what}: the parameters are updated in place and must be on the GPU")
-    sizes = [p.numel() for p in params]
+    sizes = list(map(torch.Tensor.numel, params))
     columns = [_same(what, "params", params, sizes, p_dtype, dev), _same(what, "grads", grads, sizes, g_dtype, dev),
                _same(what, "exp_avgs", exp_avgs, sizes, torch.int8 if eight else torch.float32, dev),
                _same(what, "exp_avg_sqs", exp_avg_sqs, sizes, torch.uint8 if eight else torch.float32, dev)]
     if eight:
-        blocks = [_blocks(n) for n in sizes]
+        blocks = [-(-n // BLOCK) for n in sizes]
         columns += [_same(what, "exp_avg_scales", exp_avg_scales, blocks, torch.float32, dev),
                     _same(what, "exp_avg_sq_scales", exp_avg_sq_scales, blocks, torch.float32, dev)]
     else:
@@ -92,7 +93,6 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
     launch(what, dev, _lib.lib().tfa_adamw_step, len(params), table.buffer_info()[0], desc)
     # (autograd sees the update as it sees any in-place operation)
     torch.autograd.graph.increment_version(params)
-    torch.autograd.graph.increment_version(list(exp_avgs) + list(exp_avg_sqs))
     if masters is not None:
         torch.autograd.graph.increment_version(list(masters))
 
