@@ -15,8 +15,9 @@
 // a and b were; a 32-token block's one tile is computed by every wave.  Outputs are computed transposed (lane: token), so
 // that decays by token are one factor a lane and stores are 16 bytes.
 //
-// Operands in LDS: a and b by token (contraction over features), b and c by feature (contraction over tokens); the next
-// block is on its way in registers while one is computed.
+// Operands lie in LDS by token; products over features read them as they are, products over tokens through the transposing
+// LDS read (ds_read_b64_tr_b16: 16 lanes take 4 tokens x 16 features, each receives one feature's 4 tokens).  The next block
+// is on its way in registers while one is computed.
 //
 // Precision: operands are exact sums of bf16 pieces (bf16: 1, fp16: 2, fp32: 3).  Scores, states and decayed c's are split into
 // pieces to nearest as they enter a product: two for 16-bit outputs (2^-17, nothing beside their rounding), three for fp32
@@ -60,6 +61,15 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 (&out)[N]) {
   for (int i = 0; i < 4; ++i) split_pair<N>(x[2 * i], x[2 * i + 1], p[i]);
 #pragma unroll
   for (int q = 0; q < N; ++q) out[q] = make_uint4(p[0][q], p[1][q], p[2][q], p[3][q]);
+}
+
+// four tokens (rows `pitch` apart) of the lane's feature and the four after them
+__device__ __forceinline__ uint4 read_transposed(const u16* src, int pitch) {
+  typedef short shortx4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) shortx4* Lds;
+  const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)src));
+  const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(src + 4 * pitch)));
+  return make_uint4(x.x, x.y, y.x, y.y);
 }
 
 // index bits 2 and 3 exchanged: the row that accumulator place m stands for
@@ -108,23 +118,21 @@ struct Blocks {
   static constexpr bool shared_scores = TI == 2;
   static constexpr int PL = tangent ? 3 : 0;                    // pieces of a shared score times its lag
   static constexpr int tiles = shared_scores ? (3 + NW - 1) / NW : 1;  // score tiles of a wave
-  static constexpr int W = sizeof(T) / 2;                       // dwords of two features
-  static constexpr int pitch_row = RP + 8, pitch_tok = C + 8;   // 16-bit units: rows start 4 banks apart, modulo 64
-  static constexpr int row_plane = C * pitch_row, b_plane = RP * pitch_tok, c_plane = CP * pitch_tok, s_plane = C * pitch_tok;
-  static constexpr int off_b = out ? NP * row_plane : 0, rows_end = 2 * off_b;
-  static constexpr int scores_end = out && shared_scores ? (J + PL) * s_plane : 0;  // in the rows' place
-  static constexpr int off_bt = rows_end > scores_end ? rows_end : scores_end;
-  static constexpr int off_ct = off_bt + NP * b_plane, off_end = off_ct + NP * c_plane;
+  static constexpr int V = 16 / sizeof(T);
+  // LDS in 16-bit units; rows start 4 banks apart, modulo 64
+  static constexpr int pitch = RP + 8, pitch_c = CP + 8, pitch_s = C + 8;
+  static constexpr int plane = C * pitch, plane_c = C * pitch_c, plane_s = C * pitch_s;
+  static constexpr int a_end = out ? NP * plane : 0, scores_end = out && shared_scores ? (J + PL) * plane_s : 0;  // in a's place
+  static constexpr int off_b = a_end > scores_end ? a_end : scores_end;
+  static constexpr int off_c = off_b + NP * plane, off_end = off_c + NP * plane_c;
   // tables: scale gamma^(i - j) by i - j + C (zero before C), gamma^(L - e - j) by j
   static constexpr int bytes = off_end * 2 + 3 * C * 4;
-  static constexpr int V = 16 / sizeof(T), a_lanes = RP / V, a_rows = threads / a_lanes, a_passes = C / a_rows;
-  static_assert(C % a_rows == 0, "whole passes");
-  // an operand taken by feature pairs: lanes over the pairs, 8 tokens a thread and pass
+  // an operand's rows in 16-byte pieces: lanes over the features, then over the tokens
   template <int F>
-  struct Pairs {
-    static constexpr int lanes = F / 2, at_once = threads / lanes, passes = (C / 8 + at_once - 1) / at_once;
-    static constexpr bool partial = C / 8 < at_once;  // some threads have no tokens
-    unsigned w[passes][8][W];
+  struct Rows {
+    static constexpr int lanes = F / V, at_once = threads / lanes, passes = C / at_once;
+    static_assert(C % at_once == 0, "whole passes");
+    uint4 w[passes];
   };
 };
 
@@ -132,7 +140,7 @@ template <typename T, int RP, int NW, int MODE>
 __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks_kernel(AttnPass p, int first_seg, int segs,
                                                                                      bool whole_o, bool whole_x) {
   using B = Blocks<T, RP, NW, MODE>;
-  constexpr int NP = B::NP, C = B::C, J = B::J, TI = B::TI, RB = B::RB, V = B::V, W = B::W;
+  constexpr int NP = B::NP, C = B::C, J = B::J, TI = B::TI, RB = B::RB, V = B::V;
   constexpr bool OUT = B::out, TAN = B::tangent;
   __shared__ __align__(16) unsigned char lds[B::bytes];
   u16* const L16 = reinterpret_cast<u16*>(lds);
@@ -174,15 +182,12 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
     }
   double dg = 0.0;
 
-  using PB = typename B::template Pairs<RP>;
-  using PC = typename B::template Pairs<B::CP>;
-  uint4 ra[OUT ? B::a_passes : 1];
-  PB rb_raw;
-  PC rc_raw;
-  const int a_f = (t % B::a_lanes) * V, a_u = t / B::a_lanes;
-  const int b_f = (t % PB::lanes) * 2, b_g = t / PB::lanes, c_f = (t % PC::lanes) * 2, c_g = t / PC::lanes;
-  const bool a_on = a_f < rows, b_on = b_f < rows, c_on = c_f < cols;
-  const bool b_has = !PB::partial || b_g < C / 8, c_has = !PC::partial || c_g < C / 8;  // (threads without tokens read group 0)
+  using RowsB = typename B::template Rows<RP>;
+  using RowsC = typename B::template Rows<B::CP>;
+  RowsB ra, rb_raw;
+  RowsC rc_raw;
+  const int b_f = (t % RowsB::lanes) * V, b_u = t / RowsB::lanes, c_f = (t % RowsC::lanes) * V, c_u = t / RowsC::lanes;
+  const bool b_on = b_f < rows, c_on = c_f < cols;
 
   // Row u of a block (in the pass's order) is u, or reversed C - 1 - u, token strides above the block's base; a partial
   // reversed block's base lies before its tokens, whose rows are not read.  Offsets in a block are 32-bit bytes.  Threads
@@ -191,126 +196,70 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
   const char* const base_b = reinterpret_cast<const char*>(head_base<T>(p.b, b, h));
   const char* const base_c = reinterpret_cast<const char*>(head_base<T>(p.c, b, h));
   const long long st_a = OUT ? p.a.st * (long long)sizeof(T) : 0, st_b = p.b.st * (long long)sizeof(T), st_c = p.c.st * (long long)sizeof(T);
-  const unsigned step_a = reverse ? 0u - (unsigned)st_a : (unsigned)st_a, step_b = reverse ? 0u - (unsigned)st_b : (unsigned)st_b,
-                 step_c = reverse ? 0u - (unsigned)st_c : (unsigned)st_c;
-  const unsigned off_a = (unsigned)(reverse ? C - 1 : 0) * (unsigned)st_a + (unsigned)a_u * step_a + (a_on ? a_f : 0) * (unsigned)sizeof(T);
-  const unsigned off_b = (unsigned)(reverse ? C - 1 : 0) * (unsigned)st_b + (unsigned)(b_has ? b_g * 8 : 0) * step_b + (b_on ? b_f : 0) * (unsigned)sizeof(T);
-  const unsigned off_c = (unsigned)(reverse ? C - 1 : 0) * (unsigned)st_c + (unsigned)(c_has ? c_g * 8 : 0) * step_c + (c_on ? c_f : 0) * (unsigned)sizeof(T);
-
-  auto load_pair = [](const char* base, unsigned off, unsigned (&w)[W]) {
-    if constexpr (W == 1) {
-      w[0] = *reinterpret_cast<const unsigned*>(base + off);
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(base + off);
-      w[0] = v.x;
-      w[1] = v.y;
-    }
+  auto offset = [&](long long st, int u, int f) {
+    return (unsigned)(reverse ? C - 1 - u : u) * (unsigned)st + (unsigned)f * (unsigned)sizeof(T);
   };
+  const unsigned off_a = offset(st_a, b_u, b_on ? b_f : 0), off_b = offset(st_b, b_u, b_on ? b_f : 0), off_c = offset(st_c, c_u, c_on ? c_f : 0);
+
   // blocks in the pass's order; their borders are the same tokens in both directions
   const int total = (int)((hi - lo + C - 1) / C);
   auto block_lo = [&](int i) { return lo + (long long)(reverse ? total - 1 - i : i) * C; };
-
-  // (ALL: a whole block; else rows past the last one are zeros)
-  auto fetch_rows = [&](long long at, int count, auto all) {
-    constexpr bool ALL = decltype(all)::value;
-    if constexpr (OUT) {
-      const char* base = base_a + at * st_a;
-      unsigned off = opaque(off_a);
+  // (all: a whole block; else rows past the last one are zeros)
+  auto fetch_rows = [&](auto& r, const char* base, unsigned off0, long long st, int u0, int count, auto all) {
+    using R = std::remove_reference_t<decltype(r)>;
+    const unsigned step = (unsigned)R::at_once * (reverse ? 0u - (unsigned)st : (unsigned)st);
+    unsigned off = opaque(off0);
 #pragma unroll
-      for (int q = 0; q < B::a_passes; ++q, off += (unsigned)B::a_rows * step_a) {
-        if (!ALL) ra[q] = make_uint4(0, 0, 0, 0);
-        if (ALL || a_u + q * B::a_rows < count) ra[q] = *reinterpret_cast<const uint4*>(base + off);
-      }
-    }
-    const char* const bb = base_b + at * st_b;
-#pragma unroll
-    for (int q = 0; q < PB::passes; ++q) {
-      unsigned off = opaque(off_b) + (unsigned)(8 * q * PB::at_once) * step_b;
-#pragma unroll
-      for (int k = 0; k < 8; ++k, off += step_b) {
-        if (!ALL)
-          for (unsigned& z : rb_raw.w[q][k]) z = 0;
-        if (ALL || (b_g + q * PB::at_once) * 8 + k < count) load_pair(bb, off, rb_raw.w[q][k]);
-      }
-    }
-    const char* const bc = base_c + at * st_c;
-#pragma unroll
-    for (int q = 0; q < PC::passes; ++q) {
-      unsigned off = opaque(off_c) + (unsigned)(8 * q * PC::at_once) * step_c;
-#pragma unroll
-      for (int k = 0; k < 8; ++k, off += step_c) {
-        if (!ALL)
-          for (unsigned& z : rc_raw.w[q][k]) z = 0;
-        if (ALL || (c_g + q * PC::at_once) * 8 + k < count) load_pair(bc, off, rc_raw.w[q][k]);
-      }
+    for (int q = 0; q < R::passes; ++q, off += step) {
+      if (!decltype(all)::value) r.w[q] = make_uint4(0, 0, 0, 0);
+      if (decltype(all)::value || u0 + q * R::at_once < count) r.w[q] = *reinterpret_cast<const uint4*>(base + off);
     }
   };
   auto fetch = [&](int i) {
     const long long c0 = block_lo(i);
     const int count = (int)min((long long)C, hi - c0);
+    const long long at = reverse ? c0 - (C - count) : c0;
+    auto each = [&](auto all) {
+      if constexpr (OUT) fetch_rows(ra, base_a + at * st_a, off_a, st_a, b_u, count, all);
+      fetch_rows(rb_raw, base_b + at * st_b, off_b, st_b, b_u, count, all);
+      fetch_rows(rc_raw, base_c + at * st_c, off_c, st_c, c_u, count, all);
+    };
     if (count == C)
-      fetch_rows(c0, C, std::true_type{});
+      each(std::true_type{});
     else
-      fetch_rows(reverse ? c0 - (C - count) : c0, count, std::false_type{});
+      each(std::false_type{});
   };
-
-  // eight tokens of a feature pair: by feature (two rows of 8 tokens) and, where rows0, by token
-  auto put_pairs = [&](const unsigned(&r)[8][W], bool on, u16* plane0, int plane, int f, int tok, u16* rows0) {
-    unsigned pc[8][NP];
+  // rows from registers to LDS, in pieces
+  auto stage_rows = [&](const auto& r, u16* dst, int step, int plane, bool on) {
+    using R = std::remove_cv_t<std::remove_reference_t<decltype(r)>>;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      unsigned w[W];
+    for (int q = 0; q < R::passes; ++q, dst += step) {
+      const uint4 v = on ? r.w[q] : make_uint4(0, 0, 0, 0);
+      if constexpr (NP == 1) {
+        *reinterpret_cast<uint4*>(dst) = v;
+      } else {
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+        unsigned pc[V / 2][NP];
 #pragma unroll
-      for (int z = 0; z < W; ++z) w[z] = on ? r[k][z] : 0u;
-      pair_pieces<T>(w, pc[k]);
-    }
+        for (int k = 0; k < V / 2; ++k) pair_pieces<T>(w + k * (int)sizeof(T) / 2, pc[k]);
 #pragma unroll
-    for (int q = 0; q < NP; ++q) {
-      unsigned lo4[4], hi4[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        lo4[k] = __builtin_amdgcn_perm(pc[2 * k + 1][q], pc[2 * k][q], 0x05040100);
-        hi4[k] = __builtin_amdgcn_perm(pc[2 * k + 1][q], pc[2 * k][q], 0x07060302);
+        for (int z = 0; z < NP; ++z)
+          if constexpr (V == 8)
+            *reinterpret_cast<uint4*>(dst + z * plane) = make_uint4(pc[0][z], pc[1][z], pc[2][z], pc[3][z]);
+          else
+            *reinterpret_cast<uint2*>(dst + z * plane) = make_uint2(pc[0][z], pc[1][z]);
       }
-      u16* dst = plane0 + q * plane + f * B::pitch_tok + tok;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
-      *reinterpret_cast<uint4*>(dst + B::pitch_tok) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
-      if (rows0)
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          *reinterpret_cast<unsigned*>(rows0 + q * B::row_plane + (tok + k) * B::pitch_row + f) = pc[k][q];
     }
   };
   auto stage = [&]() {
-    if constexpr (OUT) {
-#pragma unroll
-      for (int q = 0; q < B::a_passes; ++q) {
-        u16* dst = L16 + (a_u + q * B::a_rows) * B::pitch_row + a_f;
-        if constexpr (NP == 1) {
-          *reinterpret_cast<uint4*>(dst) = a_on ? ra[q] : make_uint4(0, 0, 0, 0);
-        } else {
-          const unsigned w[4] = {a_on ? ra[q].x : 0u, a_on ? ra[q].y : 0u, a_on ? ra[q].z : 0u, a_on ? ra[q].w : 0u};
-          unsigned pc[V / 2][NP];
-#pragma unroll
-          for (int k = 0; k < V / 2; ++k) pair_pieces<T>(w + k * W, pc[k]);
-#pragma unroll
-          for (int z = 0; z < NP; ++z)
-            if constexpr (V == 8)
-              *reinterpret_cast<uint4*>(dst + z * B::row_plane) = make_uint4(pc[0][z], pc[1][z], pc[2][z], pc[3][z]);
-            else
-              *reinterpret_cast<uint2*>(dst + z * B::row_plane) = make_uint2(pc[0][z], pc[1][z]);
-        }
-      }
-    }
-    if (b_has)
-#pragma unroll
-      for (int q = 0; q < PB::passes; ++q)
-        put_pairs(rb_raw.w[q], b_on, L16 + B::off_bt, B::b_plane, b_f, (b_g + q * PB::at_once) * 8, OUT ? L16 + B::off_b : nullptr);
-    if (c_has)
-#pragma unroll
-      for (int q = 0; q < PC::passes; ++q)
-        put_pairs(rc_raw.w[q], c_on, L16 + B::off_ct, B::c_plane, c_f, (c_g + q * PC::at_once) * 8, nullptr);
+    const int at = b_u * B::pitch + b_f, step = RowsB::at_once * B::pitch;
+    if constexpr (OUT) stage_rows(ra, L16 + at, step, B::plane, b_on);
+    stage_rows(rb_raw, L16 + B::off_b + at, step, B::plane, b_on);
+    stage_rows(rc_raw, L16 + B::off_c + c_u * B::pitch_c + c_f, RowsC::at_once * B::pitch_c, B::plane_c, c_on);
   };
+  // transposed operands: lane's row (feature) l32, in the order pi for b, tokens 8 half + 0 .. 7 of the sixteen from `src`
+  const int tr_tok = 8 * half + ((lane & 15) >> 2), tr_f = lane & 16;
+  const int tr_b = tr_tok * B::pitch + tr_f + 8 * (lane & 1) + 2 * (lane & 2), tr_c = tr_tok * B::pitch_c + tr_f + 4 * (lane & 3);
 
   // the wave's score tiles (x, y) of (0, 0), (1, 0), (1, 1); past the last it computes that one again, for nothing
   int tile_x[B::tiles], tile_y[B::tiles];
@@ -356,14 +305,14 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
         for (int q = 0; q < NP; ++q)
 #pragma unroll
           for (int x = 0; x < TI; ++x)
-            fa[q][x] = *reinterpret_cast<const uint4*>(L16 + q * B::row_plane + (32 * x + l32) * B::pitch_row + 16 * ks + 8 * half);
+            fa[q][x] = *reinterpret_cast<const uint4*>(L16 + q * B::plane + (32 * x + l32) * B::pitch + 16 * ks + 8 * half);
 #pragma unroll
         for (int k = 0; k < B::tiles; ++k) {
           uint4 fb[NP], fs[NP];
 #pragma unroll
           for (int q = 0; q < NP; ++q) {
-            fb[q] = *reinterpret_cast<const uint4*>(L16 + B::off_b + q * B::row_plane + (32 * tile_y[k] + pi(l32)) * B::pitch_row + 16 * ks + 8 * half);
-            fs[q] = B::shared_scores ? *reinterpret_cast<const uint4*>(L16 + q * B::row_plane + (32 * tile_x[k] + l32) * B::pitch_row + 16 * ks + 8 * half) : fa[q][0];
+            fb[q] = *reinterpret_cast<const uint4*>(L16 + B::off_b + q * B::plane + (32 * tile_y[k] + pi(l32)) * B::pitch + 16 * ks + 8 * half);
+            fs[q] = B::shared_scores ? *reinterpret_cast<const uint4*>(L16 + q * B::plane + (32 * tile_x[k] + l32) * B::pitch + 16 * ks + 8 * half) : fa[q][0];
           }
 #pragma unroll
           for (int q = 0; q < NP; ++q)
@@ -415,7 +364,7 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
         for (int r = 0; r < 16; ++r) s[k][r] *= pow_tab[C + lag - 16 * (r >> 3) - (r & 7)];
       }
       if constexpr (B::shared_scores) {
-        __syncthreads();  // a and b by token are done with: the scores take their place
+        __syncthreads();  // a is done with: the scores take its place
 #pragma unroll
         for (int k = 0; k < B::tiles; ++k) {
           const int id = wave + NW * k;
@@ -425,7 +374,7 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
           for (int r0 = 0; r0 < 16; r0 += 8) {
             float w[8];
             uint4 fp[J + B::PL], *const fl = fp + J;
-            u16* const dst = L16 + (32 * x + l32) * B::pitch_tok + 32 * y + 2 * r0 + 8 * half;
+            u16* const dst = L16 + (32 * x + l32) * B::pitch_s + 32 * y + 2 * r0 + 8 * half;
 #pragma unroll
             for (int r = 0; r < 8; ++r) w[r] = s[k][r0 + r];
             split8<J>(w, *reinterpret_cast<uint4(*)[J]>(fp));
@@ -435,7 +384,7 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
               split8<3>(w, *reinterpret_cast<uint4(*)[3]>(fl));
             }
 #pragma unroll
-            for (int q = 0; q < J + B::PL; ++q) *reinterpret_cast<uint4*>(dst + q * B::s_plane) = fp[q];
+            for (int q = 0; q < J + B::PL; ++q) *reinterpret_cast<uint4*>(dst + q * B::plane_s) = fp[q];
           }
         }
         __syncthreads();
@@ -459,18 +408,18 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
       uint4 fc[NP];
 #pragma unroll
       for (int q = 0; q < NP; ++q)
-        fc[q] = *reinterpret_cast<const uint4*>(L16 + B::off_ct + q * B::c_plane + ncol * B::pitch_tok + 16 * kk + 8 * half);
+        fc[q] = read_transposed(L16 + B::off_c + q * B::plane_c + 16 * kk * B::pitch_c + 32 * wave + tr_c, B::pitch_c);
       if constexpr (OUT) {
 #pragma unroll
         for (int x = kk / 2; x < TI; ++x) {
           uint4 fp[J], fl[TAN ? 3 : 1];
           if constexpr (B::shared_scores) {
-            const u16* const src = L16 + (32 * x + l32) * B::pitch_tok + 16 * kk + 8 * half;
+            const u16* const src = L16 + (32 * x + l32) * B::pitch_s + 16 * kk + 8 * half;
 #pragma unroll
-            for (int q = 0; q < J; ++q) fp[q] = *reinterpret_cast<const uint4*>(src + q * B::s_plane);
+            for (int q = 0; q < J; ++q) fp[q] = *reinterpret_cast<const uint4*>(src + q * B::plane_s);
             if constexpr (TAN)
 #pragma unroll
-              for (int q = 0; q < 3; ++q) fl[q] = *reinterpret_cast<const uint4*>(src + (J + q) * B::s_plane);
+              for (int q = 0; q < 3; ++q) fl[q] = *reinterpret_cast<const uint4*>(src + (J + q) * B::plane_s);
           } else {
             float w[8];
 #pragma unroll
@@ -521,7 +470,7 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
-          const uint4 fbt = *reinterpret_cast<const uint4*>(L16 + B::off_bt + q * B::b_plane + (32 * rb + pi(l32)) * B::pitch_tok + 16 * kk + 8 * half);
+          const uint4 fbt = read_transposed(L16 + B::off_b + q * B::plane + 16 * kk * B::pitch + 32 * rb + tr_b, B::pitch);
 #pragma unroll
           for (int z = 0; z < 3; ++z)
             if (q + z < 3) {
