@@ -300,7 +300,7 @@ typedef struct tfa_attn_desc {
   int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, token, head */
 } tfa_attn_desc;
 
-/* Device workspace (bytes) of tfa_linear_attention (backward = 0) or its backward (1). */
+/* Device workspace (bytes) of tfa_linear_attention (backward = 0), of its backward without grad_log_decay (1) or with (2). */
 int tfa_linear_attention_workspace_size(const tfa_attn_desc* desc, int32_t backward, size_t* bytes);
 /* state_in may be NULL (zeros), state_out NULL (not wanted; must not be state_in otherwise). */
 int tfa_linear_attention(const tfa_attn_desc* desc, const void* q, const void* k, const void* v, const float* log_decay,
@@ -308,7 +308,7 @@ int tfa_linear_attention(const tfa_attn_desc* desc, const void* q, const void* k
                          tfa_stream stream);
 /* Gradients of a loss whose gradients by out and state_out are grad_out (contiguous, as out) and grad_state_out (NULL:
  * zero).  grad_q, grad_k, grad_v: contiguous (batch, tokens, own heads, features); each gradient may be NULL, but
- * grad_log_decay needs grad_q and grad_state_in needs grad_v. */
+ * grad_log_decay needs grad_q and grad_k, and grad_state_in needs grad_v. */
 int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, const void* k, const void* v,
                                   const float* log_decay, const int64_t* lengths, const float* state_in,
                                   const void* grad_out, const float* grad_state_out, void* grad_q, void* grad_k,

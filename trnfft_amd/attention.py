@@ -102,17 +102,17 @@ class _LinearAttentionFn(torch.autograd.Function):
             g_out = q.new_zeros(*q.shape[:2], heads, v.shape[3])
         g_out = _rows(g_out.contiguous())
         g_last = None if g_last is None else g_last.contiguous()
-        # (the decays' gradient comes with the queries', the state's with the values')
+        # (the decays' gradient comes with the queries' and keys', the state's with the values')
         d_q = torch.empty(q.shape, dtype=q.dtype, device=dev) if need[0] or need[3] else None
-        d_k = torch.empty(k.shape, dtype=q.dtype, device=dev) if need[1] else None
+        d_k = torch.empty(k.shape, dtype=q.dtype, device=dev) if need[1] or need[3] else None
         d_state = torch.empty_like(state) if state is not None and need[4] else None
         d_v = torch.empty(v.shape, dtype=q.dtype, device=dev) if need[2] or d_state is not None else None
         d_g = torch.empty_like(log_decay) if need[3] else None
-        ws = _workspace(desc, 1, dev, what)
+        ws = _workspace(desc, 2 if need[3] else 1, dev, what)
         launch(what, dev, _lib.lib().tfa_linear_attention_backward, desc, addr(q), addr(k), addr(v), addr(log_decay),
                addr(lengths), addr(state), addr(g_out), addr(g_last), addr(d_q), addr(d_k), addr(d_v), addr(d_g),
                addr(d_state), addr(ws))
-        return d_q if need[0] else None, d_k, d_v if need[2] else None, d_g, d_state, None, None
+        return d_q if need[0] else None, d_k if need[1] else None, d_v if need[2] else None, d_g, d_state, None, None
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, *,

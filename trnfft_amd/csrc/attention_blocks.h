@@ -3,17 +3,27 @@
 //   out_i = scale ( sum_{j <= i} gamma^(i-j) (a_i . b_j) c_j  +  gamma^(i+e) a_i M ),
 //   M    <- gamma^L M + sum_j gamma^(L-e-j) b_j c_j^T             i, j < L: places in the block, in the pass's order
 //
-// with e = 1 forward and 0 in a reversed pass (a state reaches its first token undecayed there).  The tangent pass carries
-// M' = dM/dg as well: M' <- gamma^L (M' + L M) + sum_j (L-1-j) gamma^(L-1-j) b_j c_j^T, and dg collects x_i against
-// scale ( sum_j (i-j) gamma^(i-j) (a_i . b_j) c_j + gamma^(i+1) a_i (M' + (i+1) M) ).
+// with e = 1 forward and 0 in a reversed pass (a state reaches its first token undecayed there).
 //
-// A workgroup carries one head's state for 32 columns a wave, all R rows of them in registers (32 x 32 accumulators of
+// A workgroup carries one head's state, 32 columns a wave with all R rows of them in registers (accumulators of
 // v_mfma_f32_32x32x16_bf16), through its tokens.  The accumulator layout (lane: column, register: row) is also the
 // layout of a matrix operand (lane: column or row, register: contraction) up to an exchange of index bits 2 and 3, so with the
 // rows that feed the product taken in that order (pi below) the state goes from accumulators to operands without leaving
-// the registers.  Of a 64-token block's three 32 x 32 score tiles each wave computes its share and leaves it in LDS, where
-// a and b were; a 32-token block's one tile is computed by every wave.  Outputs are computed transposed (lane: token), so
-// that decays by token are one factor a lane and stores are 16 bytes.
+// the registers.  Scores are 16 x 16 tiles (v_mfma_f32_16x16x32_bf16), shared out over the waves and joined in LDS.
+// Outputs are computed transposed (lane: token), so that decays by token are one factor a lane and stores are 16 bytes.
+//
+// The log decay's gradient is the sum over all pairs of lag * flow, a flow being what a source (a token's b c^T, or
+// the first state) contributes through a sink (a token's out . x, or the last state's gradient dS_T).  Pairs in one block: the
+// query gradient's pass has their scores a . b, multiplies c . x out likewise, and sums lag gamma^lag of the two.  Pairs of
+// different blocks: with the tokens in stretches of `stretch`, places in a stretch counted from 1, lag = (sink's stretch -
+// source's) * stretch + sink's place - source's place, so their sum is
+//   stretch * sum over the borders of S . dS  +  sum_t place_t q_t . dq_t  -  sum_s place_s k_s . dk_s
+// of gradients through states alone.  The query gradient's pass adds the second sum and leaves the states S at the borders in
+// memory; the key gradient's pass, which meets the same borders with dS, adds the first and the third.  (dS_T is a sink of place
+// (T - 1) % stretch + 1 for all blocks but the last, whose tokens are told by their distance from the end.)  Places are at most
+// 256 where lags are a head's memory: rounding counts some 256 / lag times in these, so states enter such passes in all
+// their pieces (1e-7, not 1e-5), and a head without memory gets an exact 0.  (The state's derivative carried along in registers
+// took the query gradient's pass from 150 to 500 us at 8 x 4096 tokens of 16 heads of 128.)
 //
 // Operands lie in LDS by token; products over features read them as they are, products over tokens through the transposing
 // LDS read (ds_read_b64_tr_b16: 16 lanes take 4 tokens x 16 features, each receives one feature's 4 tokens).  The next block
@@ -31,6 +41,7 @@
 namespace tfa {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -38,6 +49,10 @@ typedef unsigned short u16;
 
 __device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ floatx4 mfma(uint4 a, uint4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
 // two fp32 as N packed pairs of bf16 pieces
@@ -81,6 +96,13 @@ __device__ __forceinline__ unsigned opaque(unsigned x) {
   return x;
 }
 
+// the lane's number, computed where it is used
+__device__ __forceinline__ int lane_again() {
+  int x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+  return x;
+}
+
 template <typename T>
 struct Kind;
 template <>
@@ -96,8 +118,8 @@ struct Kind<float> {
   static constexpr int pieces = 3, block = 32, out_pieces = 3;
 };
 
-// Modes of the kernel: a pass with its outputs, the same with the decays' tangent, or only the segments' own states
-enum { kPass = 0, kTangent = 1, kSums = 2 };
+// Modes of the kernel: a pass with its outputs, the same with its part of the decays' gradient, or only the segments' own states
+enum { kPass = 0, kLags = 1, kSums = 2 };
 
 // pieces of two neighbouring features, from their raw bits: packed (f, f + 1)
 template <typename T>
@@ -112,21 +134,25 @@ __device__ __forceinline__ void pair_pieces(const unsigned* w, unsigned (&p)[Kin
 
 template <typename T, int RP, int NW, int MODE>
 struct Blocks {
-  static constexpr bool out = MODE != kSums, tangent = MODE == kTangent;
-  static constexpr int NP = Kind<T>::pieces, C = Kind<T>::block, J = Kind<T>::out_pieces;
+  static constexpr bool out = MODE != kSums, lags = MODE == kLags;
+  static constexpr int NP = Kind<T>::pieces, C = Kind<T>::block, JP = Kind<T>::out_pieces;
+  static constexpr int J = lags ? 3 : JP;  // pieces of a state; of a score: JP
   static constexpr int CP = 32 * NW, threads = 64 * NW, TI = C / 32, RB = RP / 32;
-  static constexpr bool shared_scores = TI == 2;
-  static constexpr int PL = tangent ? 3 : 0;                    // pieces of a shared score times its lag
-  static constexpr int tiles = shared_scores ? (3 + NW - 1) / NW : 1;  // score tiles of a wave
+  // score tiles (x, y, z): tokens i = 16 x + l against j = 32 y + 8 g + 4 z + r (lane l of group g, register r)
+  static constexpr int all_tiles = TI == 2 ? 12 : 4, tiles = all_tiles / NW;
+  static_assert(all_tiles % NW == 0, "the waves have equal shares");
   static constexpr int V = 16 / sizeof(T);
   // LDS in 16-bit units; rows start 4 banks apart, modulo 64
   static constexpr int pitch = RP + 8, pitch_c = CP + 8, pitch_s = C + 8;
   static constexpr int plane = C * pitch, plane_c = C * pitch_c, plane_s = C * pitch_s;
-  static constexpr int a_end = out ? NP * plane : 0, scores_end = out && shared_scores ? (J + PL) * plane_s : 0;  // in a's place
-  static constexpr int off_b = a_end > scores_end ? a_end : scores_end;
+  static constexpr int a_end = out ? NP * plane : 0, s_size = out ? JP * plane_s : 0, bc_size = NP * (plane + plane_c);
+  // scores have a place of their own where two workgroups then still fit a compute unit; else a's, once a is done with
+  static constexpr bool own_scores = (a_end + s_size + bc_size) * 2 + 4 * C * 4 <= 80 * 1024;
+  static constexpr int off_s = own_scores ? a_end : 0;
+  static constexpr int off_b = own_scores ? a_end + s_size : a_end > s_size ? a_end : s_size;
   static constexpr int off_c = off_b + NP * plane, off_end = off_c + NP * plane_c;
-  // tables: scale gamma^(i - j) by i - j + C (zero before C), gamma^(L - e - j) by j
-  static constexpr int bytes = off_end * 2 + 3 * C * 4;
+  // tables: scale gamma^(i - j) by i - j + C (zero before C), gamma^(C - e - j) by j (zero from C on)
+  static constexpr int bytes = off_end * 2 + 4 * C * 4;
   // an operand's rows in 16-byte pieces: lanes over the features, then over the tokens
   template <int F>
   struct Rows {
@@ -137,20 +163,25 @@ struct Blocks {
 };
 
 template <typename T, int RP, int NW, int MODE>
-__global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks_kernel(AttnPass p, int first_seg, int segs,
-                                                                                     bool whole_o, bool whole_x) {
+__global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_blocks_kernel(AttnPass p, int first_seg, int segs,
+                                                                                              bool whole_o) {
   using B = Blocks<T, RP, NW, MODE>;
-  constexpr int NP = B::NP, C = B::C, J = B::J, TI = B::TI, RB = B::RB, V = B::V;
-  constexpr bool OUT = B::out, TAN = B::tangent;
+  constexpr int NP = B::NP, C = B::C, J = B::J, JP = B::JP, TI = B::TI, RB = B::RB, V = B::V;
+  constexpr int STEPS = MODE == kPass ? 100 : 1;
+  constexpr bool OUT = B::out, LAGS = B::lags;
   __shared__ __align__(16) unsigned char lds[B::bytes];
   u16* const L16 = reinterpret_cast<u16*>(lds);
   float* const pow_tab = reinterpret_cast<float*>(lds + B::off_end * 2);
   float* const upd_tab = pow_tab + 2 * C;
 
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5, l32 = lane & 31, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int seg = first_seg + (int)(blockIdx.x % segs);
-  const long long bh = blockIdx.x / segs, b = bh / p.heads;
-  const int h = (int)(bh % p.heads);
+  // Heads vary fastest and neighbours run on one XCD: tokens are rows of all heads, and one head alone keeps to few of an
+  // L2's channels (16 heads of 256 bytes on 8 XCDs, head by XCD: two of its sixteen).
+  unsigned block = xcd_tile_remap32(blockIdx.x, gridDim.x);
+  const int h = (int)(block % p.heads);
+  block /= p.heads;
+  const int seg = first_seg + (int)(block % segs);
+  const long long b = block / segs, bh = b * p.heads + h;
   const long long len = live_tokens(p, b);
   const long long seg_lo = seg * p.seg_tokens, seg_end = min(seg_lo + p.seg_tokens, p.tokens);
   const long long lo = min(seg_lo, len), hi = min(seg_end, len);
@@ -158,10 +189,13 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
   const bool reverse = p.reverse;
   const double g = (double)log_decay_of(p.log_decay, h);
 
-  for (int i = t; i < 2 * C; i += B::threads) pow_tab[i] = i < C ? 0.0f : (float)(exp(g * (double)(i - C)) * (double)p.scale);
+  for (int i = t; i < 2 * C; i += B::threads) {
+    pow_tab[i] = i < C ? 0.0f : (float)(exp(g * (double)(i - C)) * (double)p.scale);
+    upd_tab[i] = i < C ? (float)exp(g * (double)(C - e - i)) : 0.0f;
+  }
 
   // the state: column 32 wave + l32, register r of block rb: row 32 rb + 16 (r / 8) + 8 half + r % 8
-  floatx16 m[RB], tm[TAN ? RB : 1];
+  floatx16 m[RB];
   const int ncol = 32 * wave + l32;
   const size_t m0 = (size_t)bh * rows * cols, seg_size = (size_t)p.batch * p.heads * rows * cols;
 #pragma unroll
@@ -178,7 +212,6 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
           x = p.m_in[at] * p.m_in_scale;
       }
       m[rb][r] = x;
-      if (TAN) tm[rb][r] = 0.0f;
     }
   double dg = 0.0;
 
@@ -261,65 +294,127 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
   const int tr_tok = 8 * half + ((lane & 15) >> 2), tr_f = lane & 16;
   const int tr_b = tr_tok * B::pitch + tr_f + 8 * (lane & 1) + 2 * (lane & 2), tr_c = tr_tok * B::pitch_c + tr_f + 4 * (lane & 3);
 
-  // the wave's score tiles (x, y) of (0, 0), (1, 0), (1, 1); past the last it computes that one again, for nothing
-  int tile_x[B::tiles], tile_y[B::tiles];
+  // score tiles: token by l16, features 8 g + 0 .. 7; a score row stands for token 8 (l16 / 4) + l16 % 4
+  const int l16 = lane & 15, grp = lane >> 4;
+  const int at_a = l16 * B::pitch + 8 * grp, at_b = (8 * (l16 >> 2) + (l16 & 3)) * B::pitch + 8 * grp;
+  int tile_x[B::tiles], tile_y[B::tiles], tile_z[B::tiles];
 #pragma unroll
   for (int k = 0; k < B::tiles; ++k) {
-    const int id = min(wave + NW * k, 2);
-    tile_x[k] = B::shared_scores && id ? 1 : 0;
-    tile_y[k] = B::shared_scores ? id >> 1 : 0;
+    const int id = wave + NW * k, u = id >> 1;  // u: (0, 0), (1, 0), (2, 0), (3, 0), (2, 1), (3, 1)
+    tile_z[k] = id & 1;
+    tile_y[k] = u >> 2;
+    tile_x[k] = u < 4 ? u : u - 2;
   }
+  // states at the borders of stretches, as the lanes hold them
+  float* const border = LAGS ? p.border_state + (size_t)bh * p.borders * (RB * 16 * B::threads) + t : nullptr;
   DecaySteps gamma_full(exp(g * (double)C));
-  const float gamma_part = (float)exp(g * (double)((hi - lo) % C));
-  const int n4 = 32 * wave + 4 * half;  // the lane's first output column
-  const float first = (float)exp(g * (double)e);
-  int table_for = 0;
+  const float gamma_part = scalar((float)exp(g * (double)((hi - lo) % C)));
+  const float first = scalar((float)exp(g * (double)e));
   if (total > 0) fetch(0);
   for (int i = 0; i < total; ++i) {
     const long long c0 = block_lo(i);
     const int count = (int)min((long long)C, hi - c0);
     __syncthreads();  // the block before is done with LDS
-    if (table_for != count) {
-      table_for = count;
-      for (int j = t; j < C; j += B::threads) upd_tab[j] = j < count ? (float)exp(g * (double)(count - e - j)) : 0.0f;
-    }
     stage();
     __syncthreads();
     if (i + 1 < total) fetch(i + 1);
 
-    floatx16 o[OUT ? TI : 1], s[OUT ? B::tiles : 1], ol[TAN ? TI : 1];
+    const bool at_border = LAGS && c0 > 0 && c0 % p.stretch == 0;
+    float* const held = LAGS && at_border ? border + (size_t)(c0 / p.stretch) * (RB * 16 * B::threads) : nullptr;
+    if constexpr (LAGS)
+      if (at_border && !reverse)
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) held[(rb * 16 + r) * B::threads] = m[rb][r];
+
+    floatx16 o[OUT ? TI : 1];
     if constexpr (OUT) {
+      // scores^T = b a^T, with their gamma^(i - j)
+      floatx4 s[B::tiles];
 #pragma unroll
-      for (int x = 0; x < TI; ++x) {
-        o[x] = floatx16{};
-        if (TAN) ol[x] = floatx16{};
+      for (int k = 0; k < B::tiles; ++k) {
+        s[k] = floatx4{};
+#pragma unroll
+        for (int ks = 0; ks < RP / 32; ++ks) {
+          uint4 fa[NP], fb[NP];
+#pragma unroll
+          for (int q = 0; q < NP; ++q) {
+            fa[q] = *reinterpret_cast<const uint4*>(L16 + q * B::plane + 16 * tile_x[k] * B::pitch + 32 * ks + at_a);
+            fb[q] = *reinterpret_cast<const uint4*>(L16 + B::off_b + q * B::plane + (32 * tile_y[k] + 4 * tile_z[k]) * B::pitch + 32 * ks + at_b);
+          }
+#pragma unroll
+          for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int z = 0; z < NP; ++z)
+              if (q + z < 3) s[k] = mfma(fb[q], fa[z], s[k]);
+        }
       }
+      if constexpr (LAGS)
+        if (!reverse) {
+          // pairs in the block: c . x beside a . b
+          float sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < B::tiles; ++k) s[k] = floatx16{};
-      // over the features: scores^T = b a^T (rows in the order pi) and out^T = M^T a^T
+          for (int k = 0; k < B::tiles; ++k) {
+            floatx4 s2 = {};
+            const int i = 16 * tile_x[k] + l16;
+            const char* const xr = reinterpret_cast<const char*>(head_base<T>(p.x, b, h) + (c0 + min(i, count - 1)) * p.x.st);
+#pragma unroll
+            for (int ks = 0; ks < B::CP / 32; ++ks) {
+              const int f = 32 * ks + 8 * grp;
+              unsigned raw[4 * sizeof(T) / 2];
+#pragma unroll
+              for (int y = 0; y < (int)sizeof(T) / 2; ++y) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (i < count && f + y * V < cols) v = *reinterpret_cast<const uint4*>(xr + f * (int)sizeof(T) + 16 * y);
+                raw[4 * y] = v.x, raw[4 * y + 1] = v.y, raw[4 * y + 2] = v.z, raw[4 * y + 3] = v.w;
+              }
+              unsigned pc[4][NP];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) pair_pieces<T>(raw + y * (int)sizeof(T) / 2, pc[y]);
+#pragma unroll
+              for (int q = 0; q < NP; ++q) {
+                const uint4 fc = *reinterpret_cast<const uint4*>(L16 + B::off_c + q * B::plane_c + (32 * tile_y[k] + 4 * tile_z[k] + 8 * (l16 >> 2) + (l16 & 3)) * B::pitch_c + f);
+#pragma unroll
+                for (int z = 0; z < NP; ++z)
+                  if (q + z < 3) s2 = mfma(fc, make_uint4(pc[0][z], pc[1][z], pc[2][z], pc[3][z]), s2);
+              }
+            }
+            const int lag = 16 * (tile_x[k] - 2 * tile_y[k]) - 4 * tile_z[k] + l16 - 8 * grp;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(s[k][r] * pow_tab[C + lag - r] * (float)(lag - r), s2[r], sum);
+          }
+          dg += (double)sum;
+        }
+      auto put_scores = [&]() {
+#pragma unroll
+        for (int k = 0; k < B::tiles; ++k) {
+          const int own = lane_again(), i16 = own & 15, j8 = 8 * (own >> 4);
+          const int j0 = 32 * tile_y[k] + 4 * tile_z[k], lag = 16 * tile_x[k] - j0 + i16 - j8;
+          u16* const dst = L16 + B::off_s + (16 * tile_x[k] * B::pitch_s + j0) + (i16 * B::pitch_s + j8);
+          float w[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[r] = s[k][r] * pow_tab[C + lag - r];
+          unsigned p0[JP], p1[JP];
+          split_pair<JP>(w[0], w[1], p0);
+          split_pair<JP>(w[2], w[3], p1);
+#pragma unroll
+          for (int q = 0; q < JP; ++q) *reinterpret_cast<uint2*>(dst + q * B::plane_s) = make_uint2(p0[q], p1[q]);
+        }
+      };
+      if constexpr (B::own_scores) put_scores();
+      // over the features: out^T = M^T a^T
+#pragma unroll
+      for (int x = 0; x < TI; ++x) o[x] = floatx16{};
 #pragma unroll
       for (int ks = 0; ks < RP / 16; ++ks) {
-        __builtin_amdgcn_sched_barrier(0);  // (one step's operands at a time: registers)
+        if (ks % STEPS == 0) __builtin_amdgcn_sched_barrier(0);  // (a few steps' operands at a time: registers)
         uint4 fa[NP][TI], fm[J];
 #pragma unroll
         for (int q = 0; q < NP; ++q)
 #pragma unroll
           for (int x = 0; x < TI; ++x)
             fa[q][x] = *reinterpret_cast<const uint4*>(L16 + q * B::plane + (32 * x + l32) * B::pitch + 16 * ks + 8 * half);
-#pragma unroll
-        for (int k = 0; k < B::tiles; ++k) {
-          uint4 fb[NP], fs[NP];
-#pragma unroll
-          for (int q = 0; q < NP; ++q) {
-            fb[q] = *reinterpret_cast<const uint4*>(L16 + B::off_b + q * B::plane + (32 * tile_y[k] + pi(l32)) * B::pitch + 16 * ks + 8 * half);
-            fs[q] = B::shared_scores ? *reinterpret_cast<const uint4*>(L16 + q * B::plane + (32 * tile_x[k] + l32) * B::pitch + 16 * ks + 8 * half) : fa[q][0];
-          }
-#pragma unroll
-          for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int z = 0; z < NP; ++z)
-              if (q + z < 3) s[k] = mfma(fb[q], fs[z], s[k]);
-        }
         float mv[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) mv[k] = m[ks / 2][8 * (ks & 1) + k];
@@ -331,19 +426,6 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
             if (q + z < J)
 #pragma unroll
               for (int x = 0; x < TI; ++x) o[x] = mfma(fm[z], fa[q][x], o[x]);
-        if constexpr (TAN) {
-          uint4 fr[3];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) mv[k] = tm[ks / 2][8 * (ks & 1) + k];
-          split8<3>(mv, fr);
-#pragma unroll
-          for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int z = 0; z < 3; ++z)
-              if (q + z < 3)
-#pragma unroll
-                for (int x = 0; x < TI; ++x) ol[x] = mfma(fr[z], fa[q][x], ol[x]);
-        }
       }
       __builtin_amdgcn_sched_barrier(0);
       // a state reaches token i with gamma^(i + e)
@@ -351,97 +433,71 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
       for (int x = 0; x < TI; ++x) {
         const float w = pow_tab[C + 32 * x + l32] * first;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          o[x][r] *= w;
-          if (TAN) ol[x][r] = __builtin_fmaf(ol[x][r], w, (float)(32 * x + l32 + 1) * o[x][r]);
-        }
-      }
-      // scores take gamma^(i - j), j = 32 y + 16 (r / 8) + 8 half + r % 8
+        for (int r = 0; r < 16; ++r) o[x][r] *= w;
+        if constexpr (LAGS) {
+          const int own = lane_again(), u = 32 * x + (own & 31), n4 = 32 * wave + 4 * (own >> 5);
+          if (u < count) {
+            const long long tok = reverse ? c0 + count - 1 - u : c0 + u;
+            const T* xr = head_base<T>(p.x, b, h) + tok * p.x.st + n4;
+            float sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < B::tiles; ++k) {
-        const int lag = 32 * (tile_x[k] - tile_y[k]) + l32 - 8 * half;
+            for (int q = 0; q < 4; ++q)
+              if (n4 + 8 * q < cols) {
+                T xv[4];
+                __builtin_memcpy(xv, __builtin_assume_aligned(xr + 8 * q, 4 * sizeof(T)), sizeof(xv));
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[k][r] *= pow_tab[C + lag - 16 * (r >> 3) - (r & 7)];
-      }
-      if constexpr (B::shared_scores) {
-        __syncthreads();  // a is done with: the scores take its place
-#pragma unroll
-        for (int k = 0; k < B::tiles; ++k) {
-          const int id = wave + NW * k;
-          if (id > 2) break;
-          const int x = id ? 1 : 0, y = id >> 1;
-#pragma unroll
-          for (int r0 = 0; r0 < 16; r0 += 8) {
-            float w[8];
-            uint4 fp[J + B::PL], *const fl = fp + J;
-            u16* const dst = L16 + (32 * x + l32) * B::pitch_s + 32 * y + 2 * r0 + 8 * half;
-#pragma unroll
-            for (int r = 0; r < 8; ++r) w[r] = s[k][r0 + r];
-            split8<J>(w, *reinterpret_cast<uint4(*)[J]>(fp));
-            if constexpr (TAN) {
-#pragma unroll
-              for (int r = 0; r < 8; ++r) w[r] *= (float)(32 * (x - y) + l32 - 2 * r0 - 8 * half - r);
-              split8<3>(w, *reinterpret_cast<uint4(*)[3]>(fl));
-            }
-#pragma unroll
-            for (int q = 0; q < J + B::PL; ++q) *reinterpret_cast<uint4*>(dst + q * B::plane_s) = fp[q];
+                for (int k = 0; k < 4; ++k) sum = __builtin_fmaf(to_f32(xv[k]), o[x][4 * q + k], sum);
+              }
+            const int place = (int)(tok % p.stretch) + 1;
+            dg += (double)sum * (double)(!reverse ? place : c0 + count == len ? u : -place);
           }
         }
-        __syncthreads();
       }
+      if constexpr (!B::own_scores) {
+        __syncthreads();  // a is done with
+        put_scores();
+      }
+      __syncthreads();
     }
-    // the state takes gamma^L M, its tangent gamma^L (M' + L M)
     {
       const float gamma = count == C ? gamma_full.next() : gamma_part;
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          if (TAN) tm[rb][r] = gamma * __builtin_fmaf((float)count, m[rb][r], tm[rb][r]);
-          m[rb][r] *= gamma;
+        for (int r = 0; r < 16; ++r) m[rb][r] *= gamma;
+      if constexpr (LAGS)
+        if (!reverse && p.m_sink && c0 + count == len) {  // dS_T as a sink of all blocks but this, the last
+          const int row0 = (int)opaque(8u * half);
+          float sum = 0.0f;
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int row = 32 * rb + 16 * (r >> 3) + row0 + (r & 7);
+              if (row < rows && ncol < cols) sum = __builtin_fmaf(m[rb][r], p.m_sink[m0 + (size_t)(row * p.m_r + ncol * p.m_n)], sum);
+            }
+          dg += (double)sum * (double)((len - 1) % p.stretch + 1);
         }
     }
     // over the tokens: out^T += c^T scores^T, M += b^T (decayed c)
 #pragma unroll
     for (int kk = 0; kk < C / 16; ++kk) {
-      __builtin_amdgcn_sched_barrier(0);
+      if (kk % STEPS == 0) __builtin_amdgcn_sched_barrier(0);
       uint4 fc[NP];
 #pragma unroll
-      for (int q = 0; q < NP; ++q)
-        fc[q] = read_transposed(L16 + B::off_c + q * B::plane_c + 16 * kk * B::pitch_c + 32 * wave + tr_c, B::pitch_c);
+      for (int q = 0; q < NP; ++q) fc[q] = read_transposed(L16 + B::off_c + q * B::plane_c + 16 * kk * B::pitch_c + 32 * wave + tr_c, B::pitch_c);
       if constexpr (OUT) {
 #pragma unroll
         for (int x = kk / 2; x < TI; ++x) {
-          uint4 fp[J], fl[TAN ? 3 : 1];
-          if constexpr (B::shared_scores) {
-            const u16* const src = L16 + (32 * x + l32) * B::pitch_s + 16 * kk + 8 * half;
+          uint4 fp[JP];
 #pragma unroll
-            for (int q = 0; q < J; ++q) fp[q] = *reinterpret_cast<const uint4*>(src + q * B::plane_s);
-            if constexpr (TAN)
-#pragma unroll
-              for (int q = 0; q < 3; ++q) fl[q] = *reinterpret_cast<const uint4*>(src + (J + q) * B::plane_s);
-          } else {
-            float w[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = s[0][8 * kk + k];
-            split8<J>(w, fp);
-            if constexpr (TAN) {
-#pragma unroll
-              for (int k = 0; k < 8; ++k) w[k] *= (float)(l32 - 16 * kk - 8 * half - k);
-              split8<3>(w, fl);
-            }
-          }
+          for (int q = 0; q < JP; ++q)
+            fp[q] = *reinterpret_cast<const uint4*>(L16 + B::off_s + q * B::plane_s + (32 * x + l32) * B::pitch_s + 16 * kk + 8 * half);
 #pragma unroll
           for (int q = 0; q < NP; ++q)
 #pragma unroll
-            for (int z = 0; z < J; ++z)
-              if (q + z < J) o[x] = mfma(fc[q], fp[z], o[x]);
-          if constexpr (TAN)
-#pragma unroll
-            for (int q = 0; q < NP; ++q)
-#pragma unroll
-              for (int z = 0; z < 3; ++z)
-                if (q + z < 3) ol[x] = mfma(fc[q], fl[z], ol[x]);
+            for (int z = 0; z < JP; ++z)
+              if (q + z < JP) o[x] = mfma(fc[q], fp[z], o[x]);
         }
       }
       float cv[8];
@@ -457,15 +513,9 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
         }
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) cv[k] *= upd_tab[16 * kk + 8 * half + k];
-      uint4 fu[3], ft[TAN ? 3 : 1];
+      for (int k = 0; k < 8; ++k) cv[k] *= upd_tab[C - count + 16 * kk + 8 * half + k];
+      uint4 fu[3];
       split8<3>(cv, fu);
-      if constexpr (TAN) {
-        float tv[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) tv[k] = cv[k] * (float)(count - 1 - 16 * kk - 8 * half - k);
-        split8<3>(tv, ft);
-      }
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
@@ -473,40 +523,27 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
           const uint4 fbt = read_transposed(L16 + B::off_b + q * B::plane + 16 * kk * B::pitch + 32 * rb + tr_b, B::pitch);
 #pragma unroll
           for (int z = 0; z < 3; ++z)
-            if (q + z < 3) {
-              m[rb] = mfma(fbt, fu[z], m[rb]);
-              if constexpr (TAN) tm[rb] = mfma(fbt, ft[z], tm[rb]);
-            }
+            if (q + z < 3) m[rb] = mfma(fbt, fu[z], m[rb]);
         }
     }
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (LAGS)
+      if (at_border && reverse) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum = __builtin_fmaf(held[(rb * 16 + r) * B::threads], m[rb][r], sum);
+        dg += (double)sum * (double)p.scale * (double)p.stretch;
+      }
     if constexpr (OUT) {
       // out: lane: token 32 x + l32, register r: column n4 + 8 (r / 4) + r % 4
+      const int own = lane_again(), l32 = own & 31, half = own >> 5, n4 = 32 * wave + 4 * half;
 #pragma unroll
       for (int x = 0; x < TI; ++x) {
         const int u = 32 * x + l32;
         const bool live = u < count;
         const long long tok = reverse ? c0 + count - 1 - u : c0 + u;
-        if constexpr (TAN) {
-          float sum = 0.0f;
-          if (live) {
-            const T* xr = head_base<T>(p.x, b, h) + tok * p.x.st + n4;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              T xv[4];
-              if (whole_x && n4 + 8 * q < cols) {
-                __builtin_memcpy(xv, __builtin_assume_aligned(xr + 8 * q, 4 * sizeof(T)), sizeof(xv));
-              } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) xv[k] = n4 + 8 * q + k < cols ? xr[8 * q + k] : T(0.0f);
-              }
-#pragma unroll
-              for (int k = 0; k < 4; ++k) sum = __builtin_fmaf(to_f32(xv[k]), ol[x][4 * q + k], sum);
-            }
-          }
-          dg += (double)sum;
-        }
-        const floatx16 ov = o[x];
         const size_t row = (((size_t)b * p.tokens + tok) * p.heads + h) * cols;
         if (sizeof(T) == 4 || p.out_f32) {
           float* dst = static_cast<float*>(p.out) + row + n4;
@@ -514,18 +551,18 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               if (whole_o) {
-                if (n4 + 8 * q < cols) *reinterpret_cast<float4*>(dst + 8 * q) = make_float4(ov[4 * q], ov[4 * q + 1], ov[4 * q + 2], ov[4 * q + 3]);
+                if (n4 + 8 * q < cols) *reinterpret_cast<float4*>(dst + 8 * q) = make_float4(o[x][4 * q], o[x][4 * q + 1], o[x][4 * q + 2], o[x][4 * q + 3]);
               } else {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  if (n4 + 8 * q + k < cols) dst[8 * q + k] = ov[4 * q + k];
+                  if (n4 + 8 * q + k < cols) dst[8 * q + k] = o[x][4 * q + k];
               }
             }
         } else if constexpr (sizeof(T) == 2) {
           unsigned d[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            d[k] = __builtin_bit_cast(u16, from_f32<T>(ov[2 * k])) | (unsigned)__builtin_bit_cast(u16, from_f32<T>(ov[2 * k + 1])) << 16;
+            d[k] = __builtin_bit_cast(u16, from_f32<T>(o[x][2 * k])) | (unsigned)__builtin_bit_cast(u16, from_f32<T>(o[x][2 * k + 1])) << 16;
           if (whole_o) {
             // the halves exchange so that each has 8 consecutive columns: 16 (q / 2) + 8 half
 #pragma unroll
@@ -572,12 +609,8 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
         p.seg_state[seg * seg_size + at] = m[rb][r];
       else if (last && p.m_out)
         p.m_out[at] = m[rb][r] * p.m_out_scale;
-      if (TAN) {
-        const float sink = p.segments > 1 ? p.seg_sink[seg * seg_size + at] * p.scale : p.m_sink ? p.m_sink[at] : 0.0f;
-        dg += (double)tm[rb][r] * (double)sink;
-      }
     }
-  if constexpr (TAN) {
+  if constexpr (LAGS) {
     double* sum = reinterpret_cast<double*>(lds);
     __syncthreads();
     sum[t] = dg;
@@ -585,7 +618,7 @@ __global__ __launch_bounds__(64 * NW, MODE == kTangent ? 1 : 2) void attn_blocks
     if (t == 0) {
       double all = 0.0;
       for (int k = 0; k < B::threads; ++k) all += sum[k];
-      p.dg_part[bh * p.segments + seg] = all;
+      p.dg_part[(bh * p.segments + seg) * 2 + (reverse ? 1 : 0)] = all;
     }
   }
 }
@@ -594,11 +627,10 @@ template <typename T, int RP, int NW, int MODE>
 static hipError_t blocks_launch(const AttnPass& p) {
   const int osize = p.out_f32 || sizeof(T) == 4 ? 4 : 2;
   const bool wo = p.cols % (16 / osize) == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-  const bool wx = MODE == kTangent && p.cols % 4 == 0 && whole_view(p.x, (int)sizeof(T), 4 * (int)sizeof(T));
   const int first = MODE == kSums && p.reverse ? 1 : 0, segs = MODE == kSums ? p.segments - 1 : p.segments;
   const long long grid = p.batch * p.heads * segs;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((attn_blocks_kernel<T, RP, NW, MODE>), dim3((unsigned)grid), dim3(64 * NW), 0, p.stream, p, first, segs, wo, wx);
+  hipLaunchKernelGGL((attn_blocks_kernel<T, RP, NW, MODE>), dim3((unsigned)grid), dim3(64 * NW), 0, p.stream, p, first, segs, wo);
   return hipGetLastError();
 }
 
@@ -611,7 +643,7 @@ static hipError_t blocks_dims(const AttnPass& p) {
 template <typename T>
 static hipError_t blocks_modes(const AttnPass& p) {
   if (!p.out) return blocks_dims<T, kSums>(p);
-  return p.dg_part ? blocks_dims<T, kTangent>(p) : blocks_dims<T, kPass>(p);
+  return p.dg_part ? blocks_dims<T, kLags>(p) : blocks_dims<T, kPass>(p);
 }
 
 }  // namespace tfa

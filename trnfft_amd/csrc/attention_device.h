@@ -1,5 +1,6 @@
 // Device helpers shared by the linear attention kernels.
 #pragma once
+#include "kernels.h"
 #include "model_ops.h"
 
 namespace tfa {
@@ -14,17 +15,24 @@ struct Decay {
 
 // The same as one fp32 factor a step: of the two fp32 around gamma, the one that brings the product so far nearer to the
 // power, so that the product stays within a half ulp of it however many steps there are.
+// (All of it the same in every lane, and kept in scalar registers: the errors, below 2^-23 of gamma, count in 2^-44ths.)
+__device__ __forceinline__ float scalar(float x) {
+  return __uint_as_float((unsigned)__builtin_amdgcn_readfirstlane((int)__float_as_uint(x)));
+}
 struct DecaySteps {
-  float below, above, err_below, err_above, err = 0.0f;
+  float below, above;
+  int err_below, err_above, err = 0;
   __device__ __forceinline__ explicit DecaySteps(double x) {
     const float near = (float)x;
-    below = (double)near <= x ? near : __uint_as_float(__float_as_uint(near) - 1);
-    above = (double)near >= x ? near : __uint_as_float(__float_as_uint(near) + 1);
-    err_below = x > 0.0 ? (float)(((double)below - x) / x) : 0.0f;
-    err_above = x > 0.0 ? (float)(((double)above - x) / x) : 0.0f;
+    below = scalar((double)near <= x ? near : __uint_as_float(__float_as_uint(near) - 1));
+    above = scalar((double)near >= x ? near : __uint_as_float(__float_as_uint(near) + 1));
+    // (a gamma in the denormals or zero forgets all it carries: no error to keep account of)
+    const double unit = x > 1e-30 ? 0x1p44 / x : 0.0;
+    err_below = __builtin_amdgcn_readfirstlane((int)(((double)below - x) * unit));
+    err_above = __builtin_amdgcn_readfirstlane((int)(((double)above - x) * unit));
   }
   __device__ __forceinline__ float next() {
-    const bool down = err > 0.0f;
+    const bool down = err > 0;
     err += down ? err_below : err_above;
     return down ? below : above;
   }

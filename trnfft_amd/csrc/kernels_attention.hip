@@ -12,9 +12,9 @@
 // (forward, a state reaches token t with gamma^(t+1); reversed, dS_T reaches token s with gamma^(T-1-s): the decay
 // comes after the token instead of before it).  Scores, states and sums are fp32 whatever the inputs' type.
 //
-// The log decay's gradient is the sum over all pairs of lag * flow; forward in time it is carried by the tangent
-// dM/dg: M' <- gamma (M' + M), with each token's out contribution a M' . x (the dq pass, x = q), and M' . dS_T^T at
-// the end.  All its terms have their true lags as weights, so nothing cancels that does not cancel in the sum itself.
+// The log decay's gradient is the sum over all pairs of lag * flow.  Token by token it is carried by the state's derivative
+// dM/dg: M' <- gamma (M' + M), with each token's contribution a M' . x (the dq pass, x = q), and M' . dS_T^T at the end; in
+// blocks it comes from the query and key gradients themselves (attention_blocks.h).
 #include "attention_device.h"
 
 namespace tfa {
@@ -173,7 +173,8 @@ hipError_t launch_attn_blocks(const AttnPass& p) {
   return p.dtype == 1 ? launch_attn_blocks_bf16(p) : launch_attn_blocks_f16(p);
 }
 
-int attn_blocks_dg_parts(const AttnPass& p) { return p.segments; }
+int attn_blocks_dg_parts(const AttnPass& p) { return 2 * p.segments; }
+size_t attn_border_bytes(int rows, int cols) { return sizeof(float) * (rows <= 64 ? 64 : 128) * (cols <= 64 ? 64 : 128); }
 
 // seg_state[s] of each segment's own sum becomes the state it starts from; one thread an element
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnPass p) {

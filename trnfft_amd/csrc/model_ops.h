@@ -55,17 +55,20 @@ struct AttnPass {
   void* out;                   // (batch, tokens, heads, N), fp32 where out_f32, else `dtype`
   bool out_f32;
   float scale;
-  // tangent pass (the decays' gradient): x (batch, token, head, N), per workgroup
-  //   dg_part[..] = sum over pairs of lag * flow into out . x, and into m_sink (as m_in) where there is one
+  // the decays' gradient, sum over pairs of lag * flow: x (batch, token, head, N) the operand that `out` is the gradient of,
+  // m_sink the gradient of the end state (laid out as m_in) or nullptr, dg_part attn_*_dg_parts(pass) values for each (batch, head)
   HeadsView x;
   const float* m_sink;
-  double* dg_part;             // attn_*_dg_parts(pass) values for each (batch, head)
+  double* dg_part;
   // A long sequence in segments of seg_tokens (a multiple of 64), each a workgroup of its own: seg_state (segments,
   // batch, heads, ...) are the states they start from, laid out as m_in.  out = nullptr: writes the segments' own sums there.
   int segments;
   long long seg_tokens;
   float* seg_state;
-  const float* seg_sink;       // with a tangent: the gradient of the state after each segment, over `scale`
+  // In blocks, with dg_part: the forward pass of the query gradient leaves the states at every `stretch` tokens (a divisor of
+  // seg_tokens), `borders` of them for each (batch, head), for the reversed pass of the key gradient
+  float* border_state;
+  long long borders, stretch;
   hipStream_t stream;
 };
 
@@ -75,6 +78,7 @@ int attn_scan_dg_parts(const AttnPass& p);
 // in blocks of tokens on the matrix cores: dimensions up to 128; a, b and c "whole" (addresses, strides and features are
 // multiples of 16 bytes, or stride 0) with token strides below 2^24 elements
 int attn_blocks_dg_parts(const AttnPass& p);
+size_t attn_border_bytes(int rows, int cols);  // of one border's state
 hipError_t launch_attn_blocks(const AttnPass& p);
 inline bool whole_view(const HeadsView& v, int size, int bytes) {
   const int n = bytes / size;

@@ -69,6 +69,8 @@ constexpr int64_t kScanTokens = 16;
 // A long sequence is cut into segments where batch * heads alone leave compute units idle: about kWantBlocks
 // workgroups in all, segments of at least kSegTokens.
 constexpr int64_t kWantBlocks = 512, kSegTokens = 128;
+// Tokens between the states that the decays' gradient keeps: a quarter of the traffic of keeping each 64-token block's.
+constexpr int64_t kStretch = 256;
 
 struct Plan {
   bool blocks;
@@ -150,12 +152,13 @@ hipError_t segment_states(tfa::AttnPass p, const Plan& plan, float* states) {
 
 struct BackwardSpace {
   size_t dq = 0, dk = 0, dv = 0, dg = 0, total = 0;  // offsets; gradients of shared heads before their sum
-  size_t packed = 0, states = 0, grad_states = 0;
+  size_t packed = 0, states = 0, grad_states = 0, border = 0;
+  int64_t stretch = 0, borders = 0;
   int dg_each = 0;
   Plan plan;
 };
 
-BackwardSpace backward_space(const tfa_attn_desc* d) {
+BackwardSpace backward_space(const tfa_attn_desc* d, bool decays) {
   BackwardSpace s;
   s.plan = plan_of(d, true);
   const size_t rows = (size_t)d->batch * d->tokens * d->heads * sizeof(float);
@@ -172,6 +175,13 @@ BackwardSpace backward_space(const tfa_attn_desc* d) {
   s.dg_each = s.plan.blocks ? tfa::attn_blocks_dg_parts(p) : tfa::attn_scan_dg_parts(p);
   s.dg = s.total;
   s.total += align256((size_t)d->batch * d->heads * s.dg_each * sizeof(double));
+  if (decays && s.plan.blocks) {
+    s.stretch = kStretch;
+    while (s.plan.seg_tokens % s.stretch) s.stretch /= 2;
+    s.borders = (d->tokens + s.stretch - 1) / s.stretch;
+    s.border = s.total;
+    s.total += align256((size_t)d->batch * d->heads * s.borders * tfa::attn_border_bytes(p.rows, p.cols));
+  }
   return s;
 }
 
@@ -184,7 +194,7 @@ int tfa_linear_attention_workspace_size(const tfa_attn_desc* desc, int32_t backw
   *bytes = 0;
   if (const int rc = check_heads(desc)) return rc;
   if (backward) {
-    *bytes = backward_space(desc).total;
+    *bytes = backward_space(desc, backward == 2).total;
   } else {
     const Plan plan = plan_of(desc, false);
     *bytes = packed_bytes(plan) + plan.state_bytes;
@@ -229,9 +239,10 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
   if (const int rc = check_heads(desc)) return rc;
   const tfa_attn_desc& d = *desc;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const BackwardSpace space = backward_space(desc);
+  const BackwardSpace space = backward_space(desc, grad_log_decay != nullptr);
   if (!log_decay || (!workspace && space.total)) return set_error(TFA_ERR_INVALID, "null data pointer");
   if (d.batch > 0 && d.tokens > 0 && (!q || !k || !v || !grad_out)) return set_error(TFA_ERR_INVALID, "null data pointer");
+  if (grad_log_decay && d.batch > 0 && d.tokens > 0 && (!grad_q || !grad_k)) return set_error(TFA_ERR_INVALID, "grad_log_decay needs grad_q and grad_k");
   if (grad_state_in && grad_state_in == grad_state_out) return set_error(TFA_ERR_INVALID, "grad_state_in must not be grad_state_out");
   char* ws = static_cast<char*>(workspace);
   double* parts = reinterpret_cast<double*>(ws + space.dg);
@@ -288,12 +299,13 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
     p.m_n = d.value_dim;
     p.out_f32 = d.q_heads != d.heads;
     p.out = p.out_f32 ? ws + space.dq : grad_q;
-    if (!p.out) return set_error(TFA_ERR_INVALID, "grad_log_decay needs grad_q");
     if (grad_log_decay) {
       p.x = qv;
       p.m_sink = grad_state_out;
-      p.seg_sink = grad_states;
       p.dg_part = parts;
+      p.border_state = reinterpret_cast<float*>(ws + space.border);
+      p.borders = space.borders;
+      p.stretch = space.stretch;
     }
     if (const hipError_t e = run_pass(p, plan, states)) return launched(e, "query gradient");
     if (p.out_f32 && grad_q && rows)
@@ -301,11 +313,7 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
                                                          d.q_heads, d.heads / d.q_heads, d.key_dim, s))
         return launched(e, "query gradient sum");
   }
-  if (grad_log_decay)
-    if (const hipError_t e = tfa::launch_attn_dg_sum(parts, grad_log_decay, d.batch, d.heads, space.dg_each, s))
-      return launched(e, "decay gradient sum");
-  if (d.batch == 0) return TFA_OK;
-  if (grad_k) {
+  if (d.batch > 0 && (grad_k || grad_log_decay)) {
     tfa::AttnPass p = pass_of(desc, log_decay, lengths, stream);
     p.a = vv;
     p.b = gv;
@@ -319,13 +327,23 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
     p.m_n = d.value_dim;
     p.out_f32 = d.k_heads != d.heads;
     p.out = p.out_f32 ? ws + space.dk : grad_k;
+    if (grad_log_decay && plan.blocks) {
+      p.x = kv;
+      p.dg_part = parts;
+      p.border_state = reinterpret_cast<float*>(ws + space.border);
+      p.borders = space.borders;
+      p.stretch = space.stretch;
+    }
     if (const hipError_t e = run_pass(p, plan, grad_states)) return launched(e, "key gradient");
     if (p.out_f32 && rows)
       if (const hipError_t e = tfa::launch_attn_head_sum(reinterpret_cast<const float*>(ws + space.dk), grad_k, d.dtype, rows,
                                                          d.k_heads, d.heads / d.k_heads, d.key_dim, s))
         return launched(e, "key gradient sum");
   }
-  if (grad_v || grad_state_in) {
+  if (grad_log_decay)
+    if (const hipError_t e = tfa::launch_attn_dg_sum(parts, grad_log_decay, d.batch, d.heads, space.dg_each, s))
+      return launched(e, "decay gradient sum");
+  if (d.batch > 0 && (grad_v || grad_state_in)) {
     tfa::AttnPass p = pv;
     p.out_f32 = d.v_heads != d.heads;
     p.out = p.out_f32 ? ws + space.dv : grad_v;
