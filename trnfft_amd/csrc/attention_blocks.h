@@ -146,10 +146,15 @@ struct Blocks {
   static constexpr int pitch = RP + 8, pitch_c = CP + 8, pitch_s = C + 8;
   static constexpr int plane = C * pitch, plane_c = C * pitch_c, plane_s = C * pitch_s;
   static constexpr int a_end = out ? NP * plane : 0, s_size = out ? JP * plane_s : 0, bc_size = NP * (plane + plane_c);
-  // scores have a place of their own where two workgroups then still fit a compute unit; else a's, once a is done with
-  static constexpr bool own_scores = (a_end + s_size + bc_size) * 2 + 4 * C * 4 <= 80 * 1024;
+  // x as it is in memory (16-bit units; rows 16 bytes longer than they need), before the scores take its place
+  static constexpr int W = sizeof(T) / 2, pitch_x = (CP + V) * W, x_size = lags ? C * pitch_x : 0;
+  // scores (and x) have a place of their own where two workgroups then still fit a compute unit; else a's, once a is done
+  // with (and x is read from memory)
+  static constexpr int sx_size = s_size > x_size ? s_size : x_size;
+  static constexpr bool own_scores = (a_end + sx_size + bc_size) * 2 + 4 * C * 4 <= 80 * 1024;
+  static constexpr bool x_in_lds = lags && own_scores;
   static constexpr int off_s = own_scores ? a_end : 0;
-  static constexpr int off_b = own_scores ? a_end + s_size : a_end > s_size ? a_end : s_size;
+  static constexpr int off_b = own_scores ? a_end + sx_size : a_end > s_size ? a_end : s_size;
   static constexpr int off_c = off_b + NP * plane, off_end = off_c + NP * plane_c;
   // tables: scale gamma^(i - j) by i - j + C (zero before C), gamma^(C - e - j) by j (zero from C on)
   static constexpr int bytes = off_end * 2 + 4 * C * 4;
@@ -218,7 +223,7 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
   using RowsB = typename B::template Rows<RP>;
   using RowsC = typename B::template Rows<B::CP>;
   RowsB ra, rb_raw;
-  RowsC rc_raw;
+  RowsC rc_raw, rx;
   const int b_f = (t % RowsB::lanes) * V, b_u = t / RowsB::lanes, c_f = (t % RowsC::lanes) * V, c_u = t / RowsC::lanes;
   const bool b_on = b_f < rows, c_on = c_f < cols;
 
@@ -228,11 +233,14 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
   const char* const base_a = OUT ? reinterpret_cast<const char*>(head_base<T>(p.a, b, h)) : nullptr;
   const char* const base_b = reinterpret_cast<const char*>(head_base<T>(p.b, b, h));
   const char* const base_c = reinterpret_cast<const char*>(head_base<T>(p.c, b, h));
+  const char* const base_x = B::x_in_lds ? reinterpret_cast<const char*>(head_base<T>(p.x, b, h)) : nullptr;
+  const long long st_x = B::x_in_lds ? p.x.st * (long long)sizeof(T) : 0;
   const long long st_a = OUT ? p.a.st * (long long)sizeof(T) : 0, st_b = p.b.st * (long long)sizeof(T), st_c = p.c.st * (long long)sizeof(T);
   auto offset = [&](long long st, int u, int f) {
     return (unsigned)(reverse ? C - 1 - u : u) * (unsigned)st + (unsigned)f * (unsigned)sizeof(T);
   };
-  const unsigned off_a = offset(st_a, b_u, b_on ? b_f : 0), off_b = offset(st_b, b_u, b_on ? b_f : 0), off_c = offset(st_c, c_u, c_on ? c_f : 0);
+  const unsigned off_a = offset(st_a, b_u, b_on ? b_f : 0), off_b = offset(st_b, b_u, b_on ? b_f : 0), off_c = offset(st_c, c_u, c_on ? c_f : 0),
+                 off_x = offset(st_x, c_u, c_on ? c_f : 0);
 
   // blocks in the pass's order; their borders are the same tokens in both directions
   const int total = (int)((hi - lo + C - 1) / C);
@@ -256,6 +264,7 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
       if constexpr (OUT) fetch_rows(ra, base_a + at * st_a, off_a, st_a, b_u, count, all);
       fetch_rows(rb_raw, base_b + at * st_b, off_b, st_b, b_u, count, all);
       fetch_rows(rc_raw, base_c + at * st_c, off_c, st_c, c_u, count, all);
+      if constexpr (B::x_in_lds) fetch_rows(rx, base_x + at * st_x, off_x, st_x, c_u, count, all);
     };
     if (count == C)
       each(std::true_type{});
@@ -288,6 +297,12 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
     const int at = b_u * B::pitch + b_f, step = RowsB::at_once * B::pitch;
     if constexpr (OUT) stage_rows(ra, L16 + at, step, B::plane, b_on);
     stage_rows(rb_raw, L16 + B::off_b + at, step, B::plane, b_on);
+    if constexpr (B::x_in_lds) {
+      u16* dst = L16 + B::off_s + c_u * B::pitch_x + c_f * B::W;
+#pragma unroll
+      for (int q = 0; q < RowsC::passes; ++q, dst += RowsC::at_once * B::pitch_x)
+        *reinterpret_cast<uint4*>(dst) = c_on ? rx.w[q] : make_uint4(0, 0, 0, 0);
+    }
     stage_rows(rc_raw, L16 + B::off_c + c_u * B::pitch_c + c_f, RowsC::at_once * B::pitch_c, B::plane_c, c_on);
   };
   // transposed operands: lane's row (feature) l32, in the order pi for b, tokens 8 half + 0 .. 7 of the sixteen from `src`
@@ -319,8 +334,8 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
     __syncthreads();
     if (i + 1 < total) fetch(i + 1);
 
-    const bool at_border = LAGS && c0 > 0 && c0 % p.stretch == 0;
-    float* const held = LAGS && at_border ? border + (size_t)(c0 / p.stretch) * (RB * 16 * B::threads) : nullptr;
+    const bool at_border = LAGS && c0 > 0 && (c0 & (p.stretch - 1)) == 0;
+    float* const held = LAGS && at_border ? border + (size_t)(c0 >> p.log_stretch) * (RB * 16 * B::threads) : nullptr;
     if constexpr (LAGS)
       if (at_border && !reverse)
 #pragma unroll
@@ -358,7 +373,8 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
           for (int k = 0; k < B::tiles; ++k) {
             floatx4 s2 = {};
             const int i = 16 * tile_x[k] + l16;
-            const char* const xr = reinterpret_cast<const char*>(head_base<T>(p.x, b, h) + (c0 + min(i, count - 1)) * p.x.st);
+            const char* const xr = B::x_in_lds ? nullptr : reinterpret_cast<const char*>(head_base<T>(p.x, b, h) + (c0 + min(i, count - 1)) * p.x.st);
+            (void)xr;
 #pragma unroll
             for (int ks = 0; ks < B::CP / 32; ++ks) {
               const int f = 32 * ks + 8 * grp;
@@ -366,7 +382,10 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
 #pragma unroll
               for (int y = 0; y < (int)sizeof(T) / 2; ++y) {
                 uint4 v = make_uint4(0, 0, 0, 0);
-                if (i < count && f + y * V < cols) v = *reinterpret_cast<const uint4*>(xr + f * (int)sizeof(T) + 16 * y);
+                if constexpr (B::x_in_lds)
+                  v = *reinterpret_cast<const uint4*>(L16 + B::off_s + i * B::pitch_x + f * B::W + 8 * y);
+                else if (i < count && f + y * V < cols)
+                  v = *reinterpret_cast<const uint4*>(xr + f * (int)sizeof(T) + 16 * y);
                 raw[4 * y] = v.x, raw[4 * y + 1] = v.y, raw[4 * y + 2] = v.z, raw[4 * y + 3] = v.w;
               }
               unsigned pc[4][NP];
@@ -402,7 +421,7 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
           for (int q = 0; q < JP; ++q) *reinterpret_cast<uint2*>(dst + q * B::plane_s) = make_uint2(p0[q], p1[q]);
         }
       };
-      if constexpr (B::own_scores) put_scores();
+      if constexpr (B::own_scores && !LAGS) put_scores();
       // over the features: out^T = M^T a^T
 #pragma unroll
       for (int x = 0; x < TI; ++x) o[x] = floatx16{};
@@ -438,23 +457,23 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
           const int own = lane_again(), u = 32 * x + (own & 31), n4 = 32 * wave + 4 * (own >> 5);
           if (u < count) {
             const long long tok = reverse ? c0 + count - 1 - u : c0 + u;
-            const T* xr = head_base<T>(p.x, b, h) + tok * p.x.st + n4;
+            const T* const xr = B::x_in_lds ? reinterpret_cast<const T*>(L16 + B::off_s + u * B::pitch_x) + n4 : head_base<T>(p.x, b, h) + tok * p.x.st + n4;
             float sum = 0.0f;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              if (n4 + 8 * q < cols) {
+              if (B::x_in_lds || n4 + 8 * q < cols) {
                 T xv[4];
                 __builtin_memcpy(xv, __builtin_assume_aligned(xr + 8 * q, 4 * sizeof(T)), sizeof(xv));
 #pragma unroll
                 for (int k = 0; k < 4; ++k) sum = __builtin_fmaf(to_f32(xv[k]), o[x][4 * q + k], sum);
               }
-            const int place = (int)(tok % p.stretch) + 1;
+            const int place = ((int)tok & (p.stretch - 1)) + 1;
             dg += (double)sum * (double)(!reverse ? place : c0 + count == len ? u : -place);
           }
         }
       }
-      if constexpr (!B::own_scores) {
-        __syncthreads();  // a is done with
+      if constexpr (!B::own_scores || LAGS) {
+        __syncthreads();  // a, or x, is done with
         put_scores();
       }
       __syncthreads();
@@ -476,7 +495,7 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
               const int row = 32 * rb + 16 * (r >> 3) + row0 + (r & 7);
               if (row < rows && ncol < cols) sum = __builtin_fmaf(m[rb][r], p.m_sink[m0 + (size_t)(row * p.m_r + ncol * p.m_n)], sum);
             }
-          dg += (double)sum * (double)((len - 1) % p.stretch + 1);
+          dg += (double)sum * (double)(((int)(len - 1) & (p.stretch - 1)) + 1);
         }
     }
     // over the tokens: out^T += c^T scores^T, M += b^T (decayed c)

@@ -68,7 +68,8 @@ struct AttnPass {
   // In blocks, with dg_part: the forward pass of the query gradient leaves the states at every `stretch` tokens (a divisor of
   // seg_tokens), `borders` of them for each (batch, head), for the reversed pass of the key gradient
   float* border_state;
-  long long borders, stretch;
+  long long borders;
+  int stretch, log_stretch;  // a power of two
   hipStream_t stream;
 };
 

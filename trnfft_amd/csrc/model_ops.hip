@@ -305,7 +305,8 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
       p.dg_part = parts;
       p.border_state = reinterpret_cast<float*>(ws + space.border);
       p.borders = space.borders;
-      p.stretch = space.stretch;
+      p.stretch = (int)space.stretch;
+      p.log_stretch = __builtin_ctz((unsigned)space.stretch);
     }
     if (const hipError_t e = run_pass(p, plan, states)) return launched(e, "query gradient");
     if (p.out_f32 && grad_q && rows)
@@ -332,7 +333,8 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
       p.dg_part = parts;
       p.border_state = reinterpret_cast<float*>(ws + space.border);
       p.borders = space.borders;
-      p.stretch = space.stretch;
+      p.stretch = (int)space.stretch;
+      p.log_stretch = __builtin_ctz((unsigned)space.stretch);
     }
     if (const hipError_t e = run_pass(p, plan, grad_states)) return launched(e, "key gradient");
     if (p.out_f32 && rows)
