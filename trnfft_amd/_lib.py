@@ -99,9 +99,8 @@ class AttnDesc(ctypes.Structure):
         ("scale", ctypes.c_float),
         ("batch", ctypes.c_int64),
         ("tokens", ctypes.c_int64),
-        ("q_stride", ctypes.c_int64 * 3),
-        ("k_stride", ctypes.c_int64 * 3),
-        ("v_stride", ctypes.c_int64 * 3),
+        # (batch, token, head) strides of q, k, v; nine fields, since arrays of them take three times as long to fill
+        *((f"{name}_stride_{axis}", ctypes.c_int64) for name in "qkv" for axis in ("batch", "token", "head")),
     ]
 
 

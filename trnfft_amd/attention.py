@@ -24,23 +24,26 @@ DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.
 
 def _check_operands(what: str, q, k, v, log_decay, dims: int) -> int:
     """Shapes and types of a call; returns the number of heads."""
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        if x.dim() != dims:
-            raise ValueError(f"{what}: {name} must have {dims} dimensions, got {x.dim()}")
-        if x.dtype != q.dtype:
-            raise TypeError(f"{what}: q, k and v must have one dtype, got {q.dtype} and {x.dtype}")
-    if q.dtype not in DTYPES:
-        raise TypeError(f"{what}: float32, bfloat16 or float16 expected, got {q.dtype}")
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if not len(qs) == len(ks) == len(vs) == dims:
+        raise ValueError(f"{what}: q, k and v must have {dims} dimensions, got {len(qs)}, {len(ks)} and {len(vs)}")
+    dtype = q.dtype
+    if dtype not in DTYPES:
+        raise TypeError(f"{what}: float32, bfloat16 or float16 expected, got {dtype}")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"{what}: q, k and v must have one dtype, got {dtype}, {k.dtype} and {v.dtype}")
     if log_decay.dim() != 1 or log_decay.dtype != torch.float32:
         raise TypeError(f"{what}: log_decay must be a float32 vector, one value for each head")
-    if k.shape[:-2] != q.shape[:-2] or v.shape[:-2] != q.shape[:-2]:
+    if not qs[:-2] == ks[:-2] == vs[:-2]:
         raise ValueError(f"{what}: q, k and v must agree up to their heads")
-    if q.shape[-1] != k.shape[-1]:
-        raise ValueError(f"{what}: q and k must have the same features, got {q.shape[-1]} and {k.shape[-1]}")
-    heads = log_decay.numel()
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        if x.shape[-2] < 1 or x.shape[-1] < 1 or heads < 1 or heads % x.shape[-2]:
-            raise ValueError(f"{what}: the {heads} heads of log_decay must be a multiple of {name}'s {x.shape[-2]}")
+    if qs[-1] != ks[-1]:
+        raise ValueError(f"{what}: q and k must have the same features, got {qs[-1]} and {ks[-1]}")
+    if qs[-1] < 1 or vs[-1] < 1:
+        raise ValueError(f"{what}: heads must have features")
+    heads = log_decay.shape[0]
+    for n in (qs[-2], ks[-2], vs[-2]):
+        if n < 1 or heads < 1 or heads % n:
+            raise ValueError(f"{what}: the {heads} heads of log_decay must be a multiple of q's, k's and v's ({n})")
     return heads
 
 
@@ -51,18 +54,22 @@ def _scale(scale, key_dim: int, what: str) -> float:
     return scale
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x with contiguous features at a 16-byte boundary (x itself where it is so)."""
+def _on(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    return x if x.device == dev else x.to(dev)
+
+
+def _rows(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """x on dev with contiguous features at a 16-byte boundary (x itself where it is so)."""
+    x = _on(x, dev)
     if x.stride(-1) != 1 and x.shape[-1] > 1:
         x = x.contiguous()
     return x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _desc(q, k, v, heads: int, scale: float) -> _lib.AttnDesc:
-    b, t = q.shape[:2]
-    strides = [x.stride()[:3] for x in (q, k, v)]
-    return _lib.AttnDesc(DTYPES[q.dtype], heads, q.shape[2], k.shape[2], v.shape[2], q.shape[3], v.shape[3], scale, b, t,
-                         *((ctypes.c_int64 * 3)(*s) for s in strides))
+    (b, t, qh, dk), kh, (vh, dv) = q.shape, k.shape[2], v.shape[2:]
+    return _lib.AttnDesc(DTYPES[q.dtype], heads, qh, kh, vh, dk, dv, scale, b, t, *q.stride()[:3], *k.stride()[:3],
+                         *v.stride()[:3])
 
 
 def _workspace(desc: _lib.AttnDesc, backward: int, dev: torch.device, what: str) -> torch.Tensor | None:
@@ -100,7 +107,7 @@ class _LinearAttentionFn(torch.autograd.Function):
         desc = _desc(q, k, v, heads, ctx.scale)
         if g_out is None:
             g_out = q.new_zeros(*q.shape[:2], heads, v.shape[3])
-        g_out = _rows(g_out.contiguous())
+        g_out = _rows(g_out.contiguous(), dev)
         g_last = None if g_last is None else g_last.contiguous()
         # (the decays' gradient comes with the queries' and keys', the state's with the values')
         d_q = torch.empty(q.shape, dtype=q.dtype, device=dev) if need[0] or need[3] else None
@@ -146,9 +153,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
             raise TypeError(f"{what}: lengths must be whole numbers, got {lengths.dtype}")
     _require_hip(what)
     dev, out_dev = target_device(q, k, v), q.device
-    q, k, v = (_rows(x.to(dev)) for x in (q, k, v))
-    log_decay = log_decay.to(dev).contiguous()
-    state = None if initial_state is None else initial_state.to(dev).contiguous()
+    q, k, v = _rows(q, dev), _rows(k, dev), _rows(v, dev)
+    log_decay = _on(log_decay, dev).contiguous()
+    state = None if initial_state is None else _on(initial_state, dev).contiguous()
     lengths = None if lengths is None else lengths.to(dev, torch.int64).contiguous()
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, log_decay, state)):
         out, last = _LinearAttentionFn.apply(q, k, v, log_decay, state, lengths, scale)
@@ -168,21 +175,23 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     """
     what = "linear_attention_step"
     heads = _check_operands(what, q, k, v, log_decay, 3)
-    scale = _scale(scale, q.shape[-1], what)
-    if state.shape != (q.shape[0], heads, q.shape[-1], v.shape[-1]):
+    (b, qh, dk), kh, (vh, dv) = q.shape, k.shape[1], v.shape[1:]
+    scale = _scale(scale, dk, what)
+    if state.shape != (b, heads, dk, dv):
         raise ValueError(f"{what}: state must be (batch, heads, key_dim, value_dim), got {tuple(state.shape)}")
     if state.dtype != torch.float32:
         raise TypeError(f"{what}: states are float32, got {state.dtype}")
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, log_decay, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or state.requires_grad):
         raise RuntimeError(f"{what}: no gradients; use linear_attention, or torch.no_grad()")
     _require_hip(what)
     if not state.is_cuda or not state.is_contiguous():
         raise ValueError(f"{what}: the state is updated in place and must be contiguous on the GPU")
     dev, out_dev = state.device, q.device
-    q, k, v = (_rows(x.to(dev)).unsqueeze(1) for x in (q, k, v))
-    log_decay = log_decay.to(dev).contiguous()
-    desc = _desc(q, k, v, heads, scale)
-    out = q.new_empty(q.shape[0], heads, v.shape[3])
+    q, k, v, log_decay = _rows(q, dev), _rows(k, dev), _rows(v, dev), _on(log_decay, dev).contiguous()
+    (qb, qs, _), (kb, ks, _), (vb, vs, _) = q.stride(), k.stride(), v.stride()
+    desc = _lib.AttnDesc(DTYPES[q.dtype], heads, qh, kh, vh, dk, dv, scale, b, 1, qb, 0, qs, kb, 0, ks, vb, 0, vs)
+    out = q.new_empty(b, heads, dv)
     launch(what, dev, _lib.lib().tfa_linear_attention_step, desc, addr(q), addr(k), addr(v), addr(log_decay), addr(state),
            addr(out))
     torch.autograd.graph.increment_version(state)

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .attention import DTYPES
+from .attention import DTYPES, _on
 from .dispatch import _require_hip, addr, launch, target_device
 
 ACTIVATIONS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "relu": _lib.ACT_RELU}
@@ -28,11 +28,16 @@ def _workspace(desc: _lib.NormDesc, backward: int, dev: torch.device, what: str)
 
 def _forward(x, weight, bias, lengths, desc):
     y = torch.empty_like(x)
-    mean = torch.empty(2, desc.batch, desc.groups, dtype=torch.float32, device=x.device)
+    stats = torch.empty(2, desc.batch, desc.groups, dtype=torch.float32, device=x.device)
     ws = _workspace(desc, 0, x.device, "group_norm")
     launch("group_norm", x.device, _lib.lib().tfa_group_norm, desc, addr(x), addr(weight), addr(bias), addr(lengths),
-           addr(y), addr(mean[0]), addr(mean[1]), addr(ws))
-    return y, mean
+           addr(y), *_mean_rstd(stats), addr(ws))
+    return y, stats
+
+
+def _mean_rstd(stats: torch.Tensor) -> tuple[int, int]:
+    at = stats.data_ptr()
+    return at, at + 2 * stats.numel()  # (two halves of 4-byte values)
 
 
 class _GroupNormFn(torch.autograd.Function):
@@ -50,11 +55,12 @@ class _GroupNormFn(torch.autograd.Function):
         what, dev, desc, need = "group_norm backward", x.device, ctx.desc, ctx.needs_input_grad
         g = g.contiguous()
         dx = torch.empty_like(x)
-        dw = torch.zeros_like(weight) if weight is not None and need[1] else None
-        db = torch.zeros_like(bias) if bias is not None and need[2] else None
+        fresh = torch.empty_like if x.numel() else torch.zeros_like  # (of no data there is no launch)
+        dw = fresh(weight) if weight is not None and need[1] else None
+        db = fresh(bias) if bias is not None and need[2] else None
         ws = _workspace(desc, 1, dev, what)
         launch(what, dev, _lib.lib().tfa_group_norm_backward, desc, addr(x), addr(g), addr(weight), addr(bias),
-               addr(lengths), addr(stats[0]), addr(stats[1]), addr(dx), addr(dw), addr(db), addr(ws))
+               addr(lengths), *_mean_rstd(stats), addr(dx), addr(dw), addr(db), addr(ws))
         return dx if need[0] else None, dw, db, None, None
 
 
@@ -93,8 +99,10 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
             raise TypeError(f"{what}: lengths must be whole numbers, got {lengths.dtype}")
     _require_hip(what)
     dev, out_dev = target_device(x), x.device
-    x = x.to(dev).contiguous()
-    weight, bias = (None if w is None else w.to(dev, torch.float32).contiguous() for w in (weight, bias))
+    x = _on(x, dev).contiguous()
+    weight, bias = (w if w is None or (w.dtype == torch.float32 and w.device == dev) else w.to(dev, torch.float32)
+                    for w in (weight, bias))
+    weight, bias = (None if w is None else w.contiguous() for w in (weight, bias))
     lengths = None if lengths is None else lengths.to(dev, torch.int64).contiguous()
     positions = math.prod(x.shape[1:-1])
     inner = max(1, math.prod(x.shape[2:-1])) if x.dim() > 2 else 1

@@ -42,11 +42,11 @@ def _same(what: str, name: str, tensors, sizes, dtype, dev) -> list[int]:
 def _table(columns, count: int) -> array:
     """Host table of 64-bit words, one row for each tensor."""
     width = len(columns)
-    table = array("q", bytes(8 * width * count))
+    words = [0] * (width * count)
     for i, column in enumerate(columns):
         if column is not None:
-            table[i::width] = array("q", column)
-    return table
+            words[i::width] = column
+    return array("q", words)
 
 
 @torch.no_grad()
