@@ -319,7 +319,7 @@ int tfa_linear_attention_step(const tfa_attn_desc* desc, const void* q, const vo
                               const float* log_decay, float* state, void* out, tfa_stream stream);
 
 /*
- * Group norm with an activation on contiguous channels-last data (batch, positions, channels):
+ * Group norm with an activation on contiguous channels-last data (batch, positions, channels), 16-byte aligned:
  *   y = act((x - mean) rstd weight + bias), mean and rstd over the positions and the channels of a group
  * weight, bias: fp32 (channels) or NULL; mean, rstd: fp32 (batch, groups), written by the forward, read by the backward.
  * lengths: (batch) device int64 or NULL; positions at and past lengths[n] * inner are padding: never read, no part of the

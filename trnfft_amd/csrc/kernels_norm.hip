@@ -89,6 +89,20 @@ struct __attribute__((aligned(V * sizeof(T)))) Raw {
   }
 };
 
+// (past the caches where these may still hold what the next rows' loads want)
+template <typename T, int V>
+__device__ __forceinline__ void stream_pack(T* p, const float (&x)[V]) {
+  if constexpr (V * sizeof(T) == 16) {
+    typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+    Pack<T, V> u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) u.v[i] = from_f32<T>(x[i]);
+    __builtin_nontemporal_store(__builtin_bit_cast(uintx4, u), reinterpret_cast<uintx4*>(p));
+  } else {
+    store_pack<T, V>(p, x);
+  }
+}
+
 __device__ __forceinline__ long long live_positions(const NormArgs& a, long long n) {
   if (!a.lengths) return a.positions;
   return min(max(a.lengths[n], 0LL), a.positions / a.inner) * a.inner;
@@ -253,7 +267,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, lo
       if (q < live)
 #pragma unroll
         for (int i = 0; i < V; ++i) z[i] = activate(__builtin_fmaf(to_f32(v[u].v[i]) - mean[i], mul[i], add[i]), a.act);
-      store_pack<T, V>(y + q * a.channels, z);
+      stream_pack<T, V>(y + q * a.channels, z);
     }
   }
 }
@@ -616,18 +630,21 @@ static long long norm_splits(const NormArgs& a) {
   return (a.positions + each - 1) / each;
 }
 
-size_t norm_workspace_bytes(const NormArgs& a, bool backward) {
-  if (a.batch == 0 || a.positions == 0) return 0;
-  // (for the three passes also where whole samples fit: the data's addresses, which have a say in it, are not known here)
-  const size_t parts = (size_t)a.batch * norm_splits(a) * 2 * a.channels;
-  return sizeof(float) * (parts + (backward ? (size_t)a.batch * a.groups * 2 : 0));
-}
-
 template <typename T>
 static bool norm_vectors(const NormArgs& a) {
-  constexpr int V = 16 / sizeof(T);
+  return a.channels % (16 / (int)sizeof(T)) == 0;
+}
+
+bool norm_aligned(const NormArgs& a) {
   const uintptr_t any = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.dy);
-  return a.channels % V == 0 && any % 16 == 0;
+  return any % 16 == 0;
+}
+
+size_t norm_workspace_bytes(const NormArgs& a, bool backward) {
+  if (a.batch == 0 || a.positions == 0) return 0;
+  if (norm_tile(a, a.dtype == 0 ? 4 : 2).threads) return backward ? sizeof(float) * (size_t)a.batch * 2 * a.channels : 0;
+  const size_t parts = (size_t)a.batch * norm_splits(a) * 2 * a.channels;
+  return sizeof(float) * (parts + (backward ? (size_t)a.batch * a.groups * 2 : 0));
 }
 
 static void weight_grad_launch(const NormArgs& a, long long parts) {

@@ -132,6 +132,7 @@ struct NormArgs {
   hipStream_t stream;
 };
 size_t norm_workspace_bytes(const NormArgs& a, bool backward);
+bool norm_aligned(const NormArgs& a);
 hipError_t launch_norm_forward(const NormArgs& a);
 hipError_t launch_norm_backward(const NormArgs& a);
 

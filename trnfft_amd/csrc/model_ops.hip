@@ -412,11 +412,13 @@ int tfa_group_norm(const tfa_norm_desc* desc, const void* x, const float* weight
                    const int64_t* lengths, void* y, float* mean, float* rstd, void* workspace, tfa_stream stream) {
   if (const int rc = check_norm(desc)) return rc;
   if (desc->batch == 0 || desc->positions == 0) return TFA_OK;
-  if (!x || !y || !mean || !rstd || !workspace) return set_error(TFA_ERR_INVALID, "null data pointer");
   tfa::NormArgs a = norm_args(desc);
+  if (!x || !y || !mean || !rstd || (!workspace && tfa::norm_workspace_bytes(a, false)))
+    return set_error(TFA_ERR_INVALID, "null data pointer");
   a.x = x, a.y = y, a.weight = weight, a.bias = bias, a.mean = mean, a.rstd = rstd;
   a.lengths = reinterpret_cast<const long long*>(lengths);
   a.ws = static_cast<float*>(workspace), a.stream = static_cast<hipStream_t>(stream);
+  if (!tfa::norm_aligned(a)) return set_error(TFA_ERR_INVALID, "x and y must be 16-byte aligned");
   return launched(tfa::launch_norm_forward(a), "group norm");
 }
 
@@ -431,6 +433,7 @@ int tfa_group_norm_backward(const tfa_norm_desc* desc, const void* x, const void
   a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd), a.dweight = grad_weight, a.dbias = grad_bias;
   a.lengths = reinterpret_cast<const long long*>(lengths);
   a.ws = static_cast<float*>(workspace), a.stream = static_cast<hipStream_t>(stream);
+  if (!tfa::norm_aligned(a)) return set_error(TFA_ERR_INVALID, "x, grad_y and grad_x must be 16-byte aligned");
   return launched(tfa::launch_norm_backward(a), "group norm gradient");
 }
 

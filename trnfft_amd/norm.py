@@ -20,6 +20,10 @@ from .dispatch import _require_hip, addr, launch, target_device
 ACTIVATIONS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "relu": _lib.ACT_RELU}
 
 
+def _whole(x: torch.Tensor) -> torch.Tensor:
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
 def _workspace(desc: _lib.NormDesc, backward: int, dev: torch.device, what: str) -> torch.Tensor | None:
     nbytes = ctypes.c_size_t()
     _lib.check(_lib.lib().tfa_group_norm_workspace_size(desc, backward, nbytes), what)
@@ -53,7 +57,7 @@ class _GroupNormFn(torch.autograd.Function):
     def backward(ctx, g):
         x, weight, bias, lengths, stats = ctx.saved_tensors
         what, dev, desc, need = "group_norm backward", x.device, ctx.desc, ctx.needs_input_grad
-        g = g.contiguous()
+        g = _whole(g.contiguous())
         dx = torch.empty_like(x)
         fresh = torch.empty_like if x.numel() else torch.zeros_like  # (of no data there is no launch)
         dw = fresh(weight) if weight is not None and need[1] else None
@@ -99,7 +103,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
             raise TypeError(f"{what}: lengths must be whole numbers, got {lengths.dtype}")
     _require_hip(what)
     dev, out_dev = target_device(x), x.device
-    x = _on(x, dev).contiguous()
+    x = _whole(_on(x, dev).contiguous())
     weight, bias = (w if w is None or (w.dtype == torch.float32 and w.device == dev) else w.to(dev, torch.float32)
                     for w in (weight, bias))
     weight, bias = (None if w is None else w.contiguous() for w in (weight, bias))
