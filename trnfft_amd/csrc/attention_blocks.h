@@ -172,7 +172,7 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
                                                                                               bool whole_o) {
   using B = Blocks<T, RP, NW, MODE>;
   constexpr int NP = B::NP, C = B::C, J = B::J, JP = B::JP, TI = B::TI, RB = B::RB, V = B::V;
-  constexpr int STEPS = MODE == kPass ? 100 : 1;
+  constexpr int STEPS = MODE == kPass ? 100 : 1, DEEP = 1;
   constexpr bool OUT = B::out, LAGS = B::lags;
   __shared__ __align__(16) unsigned char lds[B::bytes];
   u16* const L16 = reinterpret_cast<u16*>(lds);
@@ -222,8 +222,10 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
 
   using RowsB = typename B::template Rows<RP>;
   using RowsC = typename B::template Rows<B::CP>;
-  RowsB ra, rb_raw;
-  RowsC rc_raw, rx;
+  struct Set {
+    RowsB a, b;
+    RowsC c, x;
+  };
   const int b_f = (t % RowsB::lanes) * V, b_u = t / RowsB::lanes, c_f = (t % RowsC::lanes) * V, c_u = t / RowsC::lanes;
   const bool b_on = b_f < rows, c_on = c_f < cols;
 
@@ -256,15 +258,15 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
       if (decltype(all)::value || u0 + q * R::at_once < count) r.w[q] = *reinterpret_cast<const uint4*>(base + off);
     }
   };
-  auto fetch = [&](int i) {
+  auto fetch = [&](int i, Set& set) {
     const long long c0 = block_lo(i);
     const int count = (int)min((long long)C, hi - c0);
     const long long at = reverse ? c0 - (C - count) : c0;
     auto each = [&](auto all) {
-      if constexpr (OUT) fetch_rows(ra, base_a + at * st_a, off_a, st_a, b_u, count, all);
-      fetch_rows(rb_raw, base_b + at * st_b, off_b, st_b, b_u, count, all);
-      fetch_rows(rc_raw, base_c + at * st_c, off_c, st_c, c_u, count, all);
-      if constexpr (B::x_in_lds) fetch_rows(rx, base_x + at * st_x, off_x, st_x, c_u, count, all);
+      if constexpr (OUT) fetch_rows(set.a, base_a + at * st_a, off_a, st_a, b_u, count, all);
+      fetch_rows(set.b, base_b + at * st_b, off_b, st_b, b_u, count, all);
+      fetch_rows(set.c, base_c + at * st_c, off_c, st_c, c_u, count, all);
+      if constexpr (B::x_in_lds) fetch_rows(set.x, base_x + at * st_x, off_x, st_x, c_u, count, all);
     };
     if (count == C)
       each(std::true_type{});
@@ -293,17 +295,17 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
       }
     }
   };
-  auto stage = [&]() {
+  auto stage = [&](const Set& set) {
     const int at = b_u * B::pitch + b_f, step = RowsB::at_once * B::pitch;
-    if constexpr (OUT) stage_rows(ra, L16 + at, step, B::plane, b_on);
-    stage_rows(rb_raw, L16 + B::off_b + at, step, B::plane, b_on);
+    if constexpr (OUT) stage_rows(set.a, L16 + at, step, B::plane, b_on);
+    stage_rows(set.b, L16 + B::off_b + at, step, B::plane, b_on);
     if constexpr (B::x_in_lds) {
       u16* dst = L16 + B::off_s + c_u * B::pitch_x + c_f * B::W;
 #pragma unroll
       for (int q = 0; q < RowsC::passes; ++q, dst += RowsC::at_once * B::pitch_x)
-        *reinterpret_cast<uint4*>(dst) = c_on ? rx.w[q] : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst) = c_on ? set.x.w[q] : make_uint4(0, 0, 0, 0);
     }
-    stage_rows(rc_raw, L16 + B::off_c + c_u * B::pitch_c + c_f, RowsC::at_once * B::pitch_c, B::plane_c, c_on);
+    stage_rows(set.c, L16 + B::off_c + c_u * B::pitch_c + c_f, RowsC::at_once * B::pitch_c, B::plane_c, c_on);
   };
   // transposed operands: lane's row (feature) l32, in the order pi for b, tokens 8 half + 0 .. 7 of the sixteen from `src`
   const int tr_tok = 8 * half + ((lane & 15) >> 2), tr_f = lane & 16;
@@ -325,14 +327,13 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
   DecaySteps gamma_full(exp(g * (double)C));
   const float gamma_part = scalar((float)exp(g * (double)((hi - lo) % C)));
   const float first = scalar((float)exp(g * (double)e));
-  if (total > 0) fetch(0);
-  for (int i = 0; i < total; ++i) {
+  auto compute = [&](int i, Set& set) {
     const long long c0 = block_lo(i);
     const int count = (int)min((long long)C, hi - c0);
     __syncthreads();  // the block before is done with LDS
-    stage();
+    stage(set);
     __syncthreads();
-    if (i + 1 < total) fetch(i + 1);
+    if (i + DEEP < total) fetch(i + DEEP, set);
 
     const bool at_border = LAGS && c0 > 0 && (c0 & (p.stretch - 1)) == 0;
     float* const held = LAGS && at_border ? border + (size_t)(c0 >> p.log_stretch) * (RB * 16 * B::threads) : nullptr;
@@ -348,22 +349,24 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
       // scores^T = b a^T, with their gamma^(i - j)
       floatx4 s[B::tiles];
 #pragma unroll
-      for (int k = 0; k < B::tiles; ++k) {
-        s[k] = floatx4{};
+      for (int k = 0; k < B::tiles; ++k) s[k] = floatx4{};
 #pragma unroll
-        for (int ks = 0; ks < RP / 32; ++ks) {
-          uint4 fa[NP], fb[NP];
+      for (int ks = 0; ks < RP / 32; ++ks) {
+        uint4 fa[B::tiles][NP], fb[B::tiles][NP];
+#pragma unroll
+        for (int k = 0; k < B::tiles; ++k)
 #pragma unroll
           for (int q = 0; q < NP; ++q) {
-            fa[q] = *reinterpret_cast<const uint4*>(L16 + q * B::plane + 16 * tile_x[k] * B::pitch + 32 * ks + at_a);
-            fb[q] = *reinterpret_cast<const uint4*>(L16 + B::off_b + q * B::plane + (32 * tile_y[k] + 4 * tile_z[k]) * B::pitch + 32 * ks + at_b);
+            fa[k][q] = *reinterpret_cast<const uint4*>(L16 + q * B::plane + 16 * tile_x[k] * B::pitch + 32 * ks + at_a);
+            fb[k][q] = *reinterpret_cast<const uint4*>(L16 + B::off_b + q * B::plane + (32 * tile_y[k] + 4 * tile_z[k]) * B::pitch + 32 * ks + at_b);
           }
 #pragma unroll
-          for (int q = 0; q < NP; ++q)
+        for (int q = 0; q < NP; ++q)
 #pragma unroll
-            for (int z = 0; z < NP; ++z)
-              if (q + z < 3) s[k] = mfma(fb[q], fa[z], s[k]);
-        }
+          for (int z = 0; z < NP; ++z)
+            if (q + z < 3)
+#pragma unroll
+              for (int k = 0; k < B::tiles; ++k) s[k] = mfma(fb[k][q], fa[k][z], s[k]);  // (neighbours do not wait for each other)
       }
       if constexpr (LAGS)
         if (!reverse) {
@@ -506,18 +509,19 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
 #pragma unroll
       for (int q = 0; q < NP; ++q) fc[q] = read_transposed(L16 + B::off_c + q * B::plane_c + 16 * kk * B::pitch_c + 32 * wave + tr_c, B::pitch_c);
       if constexpr (OUT) {
+        uint4 fp[JP][TI];
 #pragma unroll
-        for (int x = kk / 2; x < TI; ++x) {
-          uint4 fp[JP];
+        for (int q = 0; q < JP; ++q)
 #pragma unroll
-          for (int q = 0; q < JP; ++q)
-            fp[q] = *reinterpret_cast<const uint4*>(L16 + B::off_s + q * B::plane_s + (32 * x + l32) * B::pitch_s + 16 * kk + 8 * half);
+          for (int x = kk / 2; x < TI; ++x)
+            fp[q][x] = *reinterpret_cast<const uint4*>(L16 + B::off_s + q * B::plane_s + (32 * x + l32) * B::pitch_s + 16 * kk + 8 * half);
 #pragma unroll
-          for (int q = 0; q < NP; ++q)
+        for (int q = 0; q < NP; ++q)
 #pragma unroll
-            for (int z = 0; z < JP; ++z)
-              if (q + z < JP) o[x] = mfma(fc[q], fp[z], o[x]);
-        }
+          for (int z = 0; z < JP; ++z)
+            if (q + z < JP)
+#pragma unroll
+              for (int x = kk / 2; x < TI; ++x) o[x] = mfma(fc[q], fp[z][x], o[x]);
       }
       float cv[8];
 #pragma unroll
@@ -536,14 +540,17 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
       uint4 fu[3];
       split8<3>(cv, fu);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
+      for (int q = 0; q < NP; ++q) {
+        uint4 fbt[RB];
 #pragma unroll
-        for (int q = 0; q < NP; ++q) {
-          const uint4 fbt = read_transposed(L16 + B::off_b + q * B::plane + 16 * kk * B::pitch + 32 * rb + tr_b, B::pitch);
+        for (int rb = 0; rb < RB; ++rb)
+          fbt[rb] = read_transposed(L16 + B::off_b + q * B::plane + 16 * kk * B::pitch + 32 * rb + tr_b, B::pitch);
 #pragma unroll
-          for (int z = 0; z < 3; ++z)
-            if (q + z < 3) m[rb] = mfma(fbt, fu[z], m[rb]);
-        }
+        for (int z = 0; z < 3; ++z)
+          if (q + z < 3)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) m[rb] = mfma(fbt[rb], fu[z], m[rb]);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (LAGS)
@@ -603,6 +610,20 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
         }
       }
     }
+  };
+
+  if constexpr (DEEP == 2) {
+    Set even, odd;
+    if (total > 0) fetch(0, even);
+    if (total > 1) fetch(1, odd);
+    for (int i = 0; i < total; i += 2) {
+      compute(i, even);
+      if (i + 1 < total) compute(i + 1, odd);
+    }
+  } else {
+    Set set;
+    if (total > 0) fetch(0, set);
+    for (int i = 0; i < total; ++i) compute(i, set);
   }
 
   // padding: zeros
