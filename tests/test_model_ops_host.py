@@ -173,3 +173,26 @@ def test_c_entries_refuse_bad_descriptors():
     assert lib.tfa_adamw_step(0, None, adam(), None) == _lib.TFA_OK
     assert lib.tfa_adamw_state_values(1, (ctypes.c_int64 * 4)(far, 0, far, 5), 0, None) == _lib.TFA_ERR_INVALID
     assert lib.tfa_last_error()
+
+
+def test_tensor_table_refusals():
+    """The builder of AdamW's tables reads the lists itself: what it refuses it names, without a GPU."""
+    from trnfft_amd import _lib
+
+    table = _lib.tensor_table()
+    x, f32 = torch.zeros(3), torch.float32
+    with pytest.raises(TypeError, match="op: states must be torch.int8, got torch.float32"):
+        table("op", ("states",), ([x],), (torch.int8,), 0)
+    with pytest.raises(ValueError, match="op: states must be on the GPU"):
+        table("op", ("states",), ([x],), (f32,), 0)
+    with pytest.raises(TypeError, match="op: states must be tensors"):
+        table("op", ("states",), ([3],), (f32,), 0)
+    with pytest.raises(ValueError, match="op: 0 a, but 1 b"):
+        table("op", ("a", "b"), ([], [x]), (f32, f32), 0)
+    with pytest.raises(ValueError, match="must agree"):
+        table("op", ("a",), (), (), 0)
+    with pytest.raises(TypeError, match="lists of tensors"):
+        table("op", ("a", "b"), ([], (x,)), (f32, f32), 0)
+    with pytest.raises(TypeError, match="lists of tensors"):
+        table("op", ("a",), ([x],), ("float32",), 0)
+    assert table("op", ("a", "b"), ([], None), (f32, f32), 0) == b""

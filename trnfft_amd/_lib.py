@@ -134,6 +134,7 @@ class AdamDesc(ctypes.Structure):
 
 
 _lib = None
+_table = None
 _lock = threading.Lock()
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -230,6 +231,19 @@ def lib() -> ctypes.CDLL:
             _declare(handle)
             _lib = handle
     return _lib
+
+
+def tensor_table():
+    """The table builder for lists of tensors (csrc/tensor_table.cpp), loaded once."""
+    global _table
+    if _table is None:
+        try:
+            from ._tensor_table import table
+        except ImportError as e:
+            raise RuntimeError("trnfft_amd: _tensor_table.so is missing or was built for another torch; run "
+                               "`python -m trnfft_amd.csrc.build`") from e
+        _table = table
+    return _table
 
 
 def check(rc: int, what: str) -> None:

@@ -1,5 +1,6 @@
 """Build libtrnfft_amd.so (all HIP kernels + the C ABI) for gfx950 with hipcc, in-tree, and
-libtfa_copy.so, the plain-copy kernels bench.py measures the achievable memory rate with.
+libtfa_copy.so, the plain-copy kernels bench.py measures the achievable memory rate with; and, with the host compiler,
+_tensor_table.so, which reads lists of tensors for the operators that take them.
 
 Usage: python -m trnfft_amd.csrc.build   (or trnfft_amd.csrc.build.build()).
 """
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -17,6 +19,8 @@ PKG = os.path.dirname(HERE)
 LIB = os.path.join(PKG, "libtrnfft_amd.so")
 COPY_LIB = os.path.join(PKG, "libtfa_copy.so")
 COPY_SOURCE = "bench_copy.hip"
+TABLE_LIB = os.path.join(PKG, "_tensor_table.so")
+TABLE_SOURCE = "tensor_table.cpp"
 SOURCES = [
     "plan.hip",
     "kernels_c2c.hip",
@@ -40,6 +44,7 @@ SOURCES = [
     "kernels_adamw.hip",
 ]
 
+CXX = os.environ.get("CXX", "g++")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "-O3",
@@ -78,6 +83,22 @@ def _link(objs: list[str], out: str) -> None:
     os.replace(tmp, out)
 
 
+def _build_table() -> None:
+    """The CPython module on torch's own headers (torch is loaded before it: its libraries need no search path)."""
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    tmp = TABLE_LIB + ".tmp"
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    for path in (*include_paths(), sysconfig.get_path("include")):
+        cmd += ["-isystem", path]
+    cmd += [os.path.join(HERE, TABLE_SOURCE), "-o", tmp, *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{CXX} failed for {TABLE_SOURCE}:\n{res.stderr}")
+    os.replace(tmp, TABLE_LIB)
+
+
 def build(verbose: bool = False) -> str:
     """Compile every source and link the shared libraries; returns the main library's path."""
     if not shutil.which(HIPCC) and not os.path.exists(HIPCC):
@@ -87,11 +108,13 @@ def build(verbose: bool = False) -> str:
     srcs = SOURCES + [COPY_SOURCE]
     objs = [os.path.join(objdir, s.rsplit(".", 1)[0] + ".o") for s in srcs]
     with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 1)) as ex:
+        table = ex.submit(_build_table)
         list(ex.map(lambda so: _compile(*so), zip(srcs, objs)))
+        table.result()
     _link(objs[:-1], LIB)
     _link(objs[-1:], COPY_LIB)
     if verbose:
-        print(f"built {LIB} and {COPY_LIB}")
+        print(f"built {LIB}, {COPY_LIB} and {TABLE_LIB}")
     return LIB
 
 

@@ -7,9 +7,6 @@ s (c / 255)^4 of uint8 codes.  The reference has no counterpart.
 
 from __future__ import annotations
 
-from array import array
-from operator import attrgetter
-
 import torch
 
 from . import _lib
@@ -23,30 +20,11 @@ def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-_dtype = attrgetter("dtype")
+def _listed(tensors):
+    return tensors if tensors is None or type(tensors) is list else list(tensors)
 
 
-def _same(what: str, name: str, tensors, sizes, dtype, dev) -> list[int]:
-    """Addresses of a list whose tensors have to match the parameters' (checked in bulk: hundreds of tensors a step)."""
-    if len(tensors) != len(sizes):
-        raise ValueError(f"{what}: {len(sizes)} parameters, but {len(tensors)} {name}")
-    if set(map(_dtype, tensors)) != {dtype}:
-        raise TypeError(f"{what}: {name} must be {dtype}, got {set(map(_dtype, tensors)) - {dtype}}")
-    if set(map(torch.Tensor.get_device, tensors)) != {dev.index}:
-        raise ValueError(f"{what}: {name} must be on {dev}")
-    if list(map(torch.Tensor.numel, tensors)) != sizes or not all(map(torch.Tensor.is_contiguous, tensors)):
-        raise ValueError(f"{what}: {name} must be contiguous, with the size its parameter asks for")
-    return list(map(torch.Tensor.data_ptr, tensors))
-
-
-def _table(columns, count: int) -> array:
-    """Host table of 64-bit words, one row for each tensor."""
-    width = len(columns)
-    words = [0] * (width * count)
-    for i, column in enumerate(columns):
-        if column is not None:
-            words[i::width] = column
-    return array("q", words)
+_ADAM_LISTS = ("params", "grads", "exp_avgs", "exp_avg_sqs", "exp_avg_scales", "exp_avg_sq_scales", "masters")
 
 
 @torch.no_grad()
@@ -76,21 +54,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
     _require_hip(what)
     if dev.type != "cuda":
         raise ValueError(f"{what}: the parameters are updated in place and must be on the GPU")
-    sizes = list(map(torch.Tensor.numel, params))
-    columns = [_same(what, "params", params, sizes, p_dtype, dev), _same(what, "grads", grads, sizes, g_dtype, dev),
-               _same(what, "exp_avgs", exp_avgs, sizes, torch.int8 if eight else torch.float32, dev),
-               _same(what, "exp_avg_sqs", exp_avg_sqs, sizes, torch.uint8 if eight else torch.float32, dev)]
-    if eight:
-        blocks = [-(-n // BLOCK) for n in sizes]
-        columns += [_same(what, "exp_avg_scales", exp_avg_scales, blocks, torch.float32, dev),
-                    _same(what, "exp_avg_sq_scales", exp_avg_sq_scales, blocks, torch.float32, dev)]
-    else:
-        columns += [None, None]
-    columns.append(None if masters is None else _same(what, "masters", masters, sizes, torch.float32, dev))
-    table = _table(columns + [sizes], len(params))
+    moments = (torch.int8, torch.uint8) if eight else (torch.float32, torch.float32)
+    table = _lib.tensor_table()(what, _ADAM_LISTS,
+                                (params, grads, *map(_listed, (exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, masters))),
+                                (p_dtype, g_dtype, *moments, torch.float32, torch.float32, torch.float32), dev.index)
     desc = _lib.AdamDesc(DTYPES[p_dtype], DTYPES[g_dtype], 8 if eight else 32, 0, int(step), lr, betas[0], betas[1], eps,
                          weight_decay)
-    launch(what, dev, _lib.lib().tfa_adamw_step, len(params), table.buffer_info()[0], desc)
+    launch(what, dev, _lib.lib().tfa_adamw_step, len(params), table, desc)
     # (autograd sees the update as it sees any in-place operation)
     torch.autograd.graph.increment_version(params)
     if masters is not None:
@@ -112,11 +82,9 @@ def adamw_state_values(codes, scales, out=None) -> list[torch.Tensor]:
         raise ValueError(f"{what}: the states must be on the GPU")
     if out is None:
         out = [torch.empty(c.shape, dtype=torch.float32, device=dev) for c in codes]
-    sizes = [c.numel() for c in codes]
-    table = _table([_same(what, "codes", codes, sizes, dtype, dev),
-                    _same(what, "scales", scales, [_blocks(n) for n in sizes], torch.float32, dev),
-                    _same(what, "out", out, sizes, torch.float32, dev), sizes], len(codes))
-    launch(what, dev, _lib.lib().tfa_adamw_state_values, len(codes), table.buffer_info()[0], int(dtype == torch.uint8))
+    table = _lib.tensor_table()(what, ("codes", "scales", "out"), (codes, _listed(scales), _listed(out)),
+                                (dtype, torch.float32, torch.float32), dev.index)
+    launch(what, dev, _lib.lib().tfa_adamw_state_values, len(codes), table, int(dtype == torch.uint8))
     torch.autograd.graph.increment_version(out)
     return out
 
