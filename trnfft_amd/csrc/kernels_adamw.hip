@@ -19,7 +19,8 @@
 namespace tfa {
 
 constexpr int kQBlock = 256;       // values of a scale
-constexpr int kAdamChunk = 4096;   // values of a workgroup: 4 waves of 4 blocks
+constexpr int kAdamChunk = 4096;   // values of a workgroup: 4 waves of 4 blocks; with 8-bit states 2 blocks
+constexpr int adam_chunk(int bits) { return bits == 8 ? kAdamChunk / 2 : kAdamChunk; }
 constexpr int kAdamTensors = 52;   // per launch: their table travels in the kernel's arguments (4 KB at most)
 
 struct AdamTable {
@@ -59,28 +60,56 @@ __device__ __forceinline__ float code_value(int c, float top, float s, bool four
   if (fourth) t = t * t;
   return t * s;
 }
-// magnitudes compare as their bits; a NaN is above infinity, so it becomes the block's scale and the block decodes to NaN
+// Magnitudes compare as their bits; a NaN is above infinity, so it becomes the block's scale and the block decodes to NaN.
+// Within rows of 16 lanes by lane permutations, over the rows in scalar registers: no shared memory.
 __device__ __forceinline__ unsigned wave_max(unsigned x) {
-#pragma unroll
-  for (int o = 32; o > 0; o /= 2) x = max(x, (unsigned)__shfl_xor((int)x, o));
-  return x;
+  x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 15, 15, true));   // lanes 1 apart
+  x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 15, 15, true));   // 2 apart
+  x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x141, 15, 15, true));  // mirrored halves of a row
+  x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x140, 15, 15, true));  // mirrored rows
+  const unsigned a = __builtin_amdgcn_readlane((int)x, 0), b = __builtin_amdgcn_readlane((int)x, 16);
+  const unsigned c = __builtin_amdgcn_readlane((int)x, 32), d = __builtin_amdgcn_readlane((int)x, 48);
+  return max(max(a, b), max(c, d));
 }
 // the code by its definition: IEEE division, roots and product, each rounded
-__device__ __noinline__ float root_place(float x, float s, float top, bool fourth) {
+__device__ __forceinline__ int code_of_place(float c, float x, float top) {
+  return c <= top ? (x < 0.0f ? -(int)c : (int)c) : 0;  // NaN: 0 (the scale says it)
+}
+__device__ __forceinline__ int root_place(float x, float s, float top, bool fourth) {
   float t = sqrtf(fabsf(x) / s);
   if (fourth) t = sqrtf(t);
-  return rintf(t * top);
+  return code_of_place(s > 0.0f ? rintf(t * top) : 0.0f, x, top);
 }
-// The same code by approximate division and roots (all of it within 8 ulp, 2e-4 of a code's step) wherever that is 1e-3 of a step
-// and more from the middle between two codes; elsewhere by the definition.  inv: approximate 1 / s, 0 where s is 0 or
-// not normal enough for it (the definition decides then).
-__device__ __forceinline__ int value_code(float x, float s, float inv, float top, bool fourth) {
-  float t = __builtin_amdgcn_sqrtf(fabsf(x) * inv);
-  if (fourth) t = __builtin_amdgcn_sqrtf(t);
-  const float u = t * top, f = __builtin_amdgcn_fractf(u);
-  float c = rintf(u);
-  if (!(fabsf(f - 0.5f) > 1e-3f) || inv == 0.0f) c = s > 0.0f ? root_place(x, s, top, fourth) : 0.0f;
-  return c <= top ? (x < 0.0f ? -(int)c : (int)c) : 0;  // NaN: 0 (the scale says it)
+// four codes by the definition, a byte each (out of line: seldom run)
+template <bool SQUARES>
+__device__ __noinline__ unsigned root_places(float x0, float x1, float x2, float x3, float s) {
+  constexpr float top = SQUARES ? 255.0f : 127.0f;
+  unsigned r = root_place(x0, s, top, SQUARES) & 255;
+  r |= (root_place(x1, s, top, SQUARES) & 255) << 8;
+  r |= (root_place(x2, s, top, SQUARES) & 255) << 16;
+  return r | (unsigned)root_place(x3, s, top, SQUARES) << 24;
+}
+// The same four codes by approximate division and roots wherever they are kDoubt of a step and more from the middle between two codes
+// (relative errors of 2^-23 for the quotient, each root and the product, halved by each root: 2e-4 of a
+// step at most); where one of a wave's is not, by the definition: one wave's block in seven.  inv: approximate 1 / s, 0
+// where s is 0 or not normal enough for it (the definition decides then).
+constexpr float kDoubt = 2.5e-4f;
+template <bool SQUARES>
+__device__ __forceinline__ unsigned value_codes(const float (&x)[4], float s, float inv) {
+  constexpr float top = SQUARES ? 255.0f : 127.0f;
+  unsigned r = 0;
+  float least = 1.0f;  // distance from a middle
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float t = __builtin_amdgcn_sqrtf(fabsf(x[j]) * inv);
+    if (SQUARES) t = __builtin_amdgcn_sqrtf(t);
+    const float u = t * top;
+    least = fminf(least, fabsf(__builtin_amdgcn_fractf(u) - 0.5f));
+    const int c = (int)rintf(u);
+    r |= (unsigned)((!SQUARES && x[j] < 0.0f ? -c : c) & 255) << (8 * j);
+  }
+  if (__any(!(least > kDoubt)) || inv == 0.0f) r = root_places<SQUARES>(x[0], x[1], x[2], x[3], s);
+  return r;
 }
 __device__ __forceinline__ float scale_inverse(float s) { return s > 1e-30f && s < 1e30f ? __builtin_amdgcn_rcpf(s) : 0.0f; }
 
@@ -107,16 +136,20 @@ struct StateTypes<8> {
   typedef unsigned char V;
 };
 
-// A workgroup takes 4096 values of one tensor, a wave four blocks of 256, a lane four neighbours of each: 16-byte accesses
-// for fp32, all of a wave's loads ahead of its arithmetic.
+// A wave takes blocks of 256 of one tensor, a lane four neighbours of each: 16-byte accesses for fp32, and all of a wave's loads
+// ahead of its arithmetic, with fp32 states four blocks.  With 8-bit states two: their arithmetic (five roots and reciprocals
+// a value) then leaves eight waves a SIMD to overlap it with other waves' loads; four blocks took 457 us where two take 350
+// (50 tensors of 2.4M fp32 values: 5.5 TB/s), and the wave's whole block decides by itself whether its codes need the
+// definition (a branch for each value took 100 us more).  bfloat16 parameters and gradients: 353 us, bound by that arithmetic.
+// fp32 states: 5.0 TB/s, as a large copy (17.4M values with bf16 parameters and masters 97 us).
 template <int BITS, typename P, typename G>
 __global__ __launch_bounds__(256) void adamw_kernel(AdamTable tab, AdamArgs a) {
   typedef typename StateTypes<BITS>::M M;
   typedef typename StateTypes<BITS>::V V;
-  constexpr int U = kAdamChunk / kQBlock / 4;
+  constexpr int kChunk = adam_chunk(BITS), U = kChunk / kQBlock / 4;
   const int k = tensor_of(tab.first, tab.count, blockIdx.x);
   const AdamTensor& t = tab.t[k];
-  const long long n = t.n, base = (long long)(blockIdx.x - tab.first[k]) * kAdamChunk;
+  const long long n = t.n, base = (long long)(blockIdx.x - tab.first[k]) * kChunk;
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   P* const tp = static_cast<P*>(t.p);
   const G* const tg = static_cast<const G*>(t.g);
@@ -126,7 +159,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamTable tab, AdamArgs a) {
   const uintptr_t odd = reinterpret_cast<uintptr_t>(tp) % (4 * sizeof(P)) | reinterpret_cast<uintptr_t>(tg) % (4 * sizeof(G)) |
                         reinterpret_cast<uintptr_t>(tm) % (4 * sizeof(M)) | reinterpret_cast<uintptr_t>(tv) % (4 * sizeof(V)) |
                         reinterpret_cast<uintptr_t>(master) % 16;
-  const bool whole = odd == 0 && base + kAdamChunk <= n;
+  const bool whole = odd == 0 && base + kChunk <= n;
 
   Four<P> p4[U];
   Four<float> w4[U];
@@ -181,15 +214,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamTable tab, AdamArgs a) {
     } else {
       const float sm = __uint_as_float(wave_max(top_m)), sv = __uint_as_float(wave_max(top_v));
       const float im = scale_inverse(sm), iv = scale_inverse(sv);
-      Four<M> mc;
-      Four<V> vc;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        mc.v[j] = (M)value_code(mo.v[j], sm, im, 127.0f, false);
-        vc.v[j] = (V)value_code(vo.v[j], sv, iv, 255.0f, true);
-      }
-      store4(tm, i, n, whole, mc);
-      store4(tv, i, n, whole, vc);
+      store4(tm, i, n, whole, __builtin_bit_cast(Four<M>, value_codes<false>(mo.v, sm, im)));
+      store4(tv, i, n, whole, __builtin_bit_cast(Four<V>, value_codes<true>(vo.v, sv, iv)));
       if (lane == 0) {
         t.m_scale[start / kQBlock] = sm;
         t.v_scale[start / kQBlock] = sv;
@@ -216,13 +242,14 @@ static void adamw_bits(const AdamTable& tab, const AdamArgs& a, unsigned blocks,
 }
 
 hipError_t launch_adamw(const AdamTensor* tensors, long long count, const AdamArgs& a, hipStream_t stream) {
+  const int chunk = adam_chunk(a.bits);
   for (long long i = 0; i < count;) {
     AdamTable tab;
     tab.count = 0;
     unsigned long long blocks = 0;
     while (i < count && tab.count < kAdamTensors) {
       const AdamTensor& t = tensors[i];
-      const unsigned long long more = (unsigned long long)((t.n + kAdamChunk - 1) / kAdamChunk);
+      const unsigned long long more = (unsigned long long)((t.n + chunk - 1) / chunk);
       if (blocks + more > 0x7fffffffull) break;
       if (more) {
         tab.t[tab.count] = t;
