@@ -235,3 +235,27 @@ def test_module_and_cpu_inputs():
     assert layer.weight.grad.shape == (32,) and math.isfinite(float(layer.weight.grad.sum()))
     layer = layer.cuda()
     assert rel(layer(x.cuda()), y.detach().double()) <= 2e-6
+
+
+# many samples of few positions: groups of one vector and of 64, of sizes that are no power of two, fewer groups than a tile holds
+FEW = [((700, 1, 64), 4), ((300, 2, 120), 5), ((40, 7, 144), 3), ((5000, 1, 512), 1), ((33, 13, 64), 2), ((65, 30, 48), 3),
+       ((9, 3, 5, 16), 1), ((2100, 1, 256), 8)]
+
+
+@pytest.mark.parametrize("dtype", list(TOL))
+@pytest.mark.parametrize("shape,groups", FEW, ids=str)
+def test_samples_of_few_positions(shape, groups, dtype):
+    x, w, b, dy = make(shape, dtype, seed=11)
+    n = torch.randint(0, shape[1] + 1, (shape[0],), generator=torch.Generator().manual_seed(12)) if shape[1] > 1 else None
+    ref_in = [t.double().requires_grad_() for t in (x, w, b)]
+    ref = reference(ref_in[0], groups, ref_in[1], ref_in[2], 1e-5, "silu", n)
+    expected = torch.autograd.grad(ref, ref_in, dy.double())
+    if n is not None:
+        for i, end in enumerate(n.tolist()):
+            x[i, end:], dy[i, end:] = float("nan"), float("inf")
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = trnfft_amd.group_norm(leaves[0], groups, leaves[1], leaves[2], activation="silu", lengths=None if n is None else n.cuda())
+    got = torch.autograd.grad(y, leaves, dy.cuda())
+    assert rel(y, ref) <= TOL[dtype] and rel(got[0], expected[0]) <= TOL[dtype]
+    for g, e in zip(got[1:], expected[1:]):
+        assert rel(g, e) <= 3e-6

@@ -29,6 +29,14 @@
 // LDS read (ds_read_b64_tr_b16: 16 lanes take 4 tokens x 16 features, each receives one feature's 4 tokens).  The next block
 // is on its way in registers while one is computed.
 //
+// What it measures: 32 x 1024 tokens of 16 bf16 heads of 128 forward 157 us (3.4 TB/s of operands and results; at the copy's rate
+// 104), of 64 96 us (52); fp16 221 us, fp32 (3.1 TB/s) 342 us.  A training pass of 8 x 4096 tokens of 16 heads of 128: 1.05 ms, 2.1 in
+// fp32.  What bounds it: a block's chain of dependent steps (stage, scores, decays and pieces, outputs, state) with two waves a SIMD,
+// as the state leaves registers for no more: the matrix units are 30 to 44 % busy, vector units and memory less than that.
+// Two blocks on their way instead of one, or heads in another order over the L2s, change nothing; 16 columns a wave (four
+// waves a SIMD) read each operand from LDS twice as often: bf16 229 us for the 162 of 32, fp32 the other way (137 for 205 at
+// 64 features).  One layout is kept for all types.
+//
 // Precision: operands are exact sums of bf16 pieces (bf16: 1, fp16: 2, fp32: 3).  Scores, states and decayed c's are split into
 // pieces to nearest as they enter a product: two for 16-bit outputs (2^-17, nothing beside their rounding), three for fp32
 // outputs and for what enters states.  Products of pieces i, j are taken where i + j is within the piece count, into fp32.
@@ -172,7 +180,7 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
                                                                                               bool whole_o) {
   using B = Blocks<T, RP, NW, MODE>;
   constexpr int NP = B::NP, C = B::C, J = B::J, JP = B::JP, TI = B::TI, RB = B::RB, V = B::V;
-  constexpr int STEPS = MODE == kPass ? 100 : 1, DEEP = 1;
+  constexpr int STEPS = MODE == kPass ? 100 : 1;
   constexpr bool OUT = B::out, LAGS = B::lags;
   __shared__ __align__(16) unsigned char lds[B::bytes];
   u16* const L16 = reinterpret_cast<u16*>(lds);
@@ -333,7 +341,7 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
     __syncthreads();  // the block before is done with LDS
     stage(set);
     __syncthreads();
-    if (i + DEEP < total) fetch(i + DEEP, set);
+    if (i + 1 < total) fetch(i + 1, set);
 
     const bool at_border = LAGS && c0 > 0 && (c0 & (p.stretch - 1)) == 0;
     float* const held = LAGS && at_border ? border + (size_t)(c0 >> p.log_stretch) * (RB * 16 * B::threads) : nullptr;
@@ -612,19 +620,9 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
     }
   };
 
-  if constexpr (DEEP == 2) {
-    Set even, odd;
-    if (total > 0) fetch(0, even);
-    if (total > 1) fetch(1, odd);
-    for (int i = 0; i < total; i += 2) {
-      compute(i, even);
-      if (i + 1 < total) compute(i + 1, odd);
-    }
-  } else {
-    Set set;
-    if (total > 0) fetch(0, set);
-    for (int i = 0; i < total; ++i) compute(i, set);
-  }
+  Set set;
+  if (total > 0) fetch(0, set);
+  for (int i = 0; i < total; ++i) compute(i, set);
 
   // padding: zeros
   if (OUT)

@@ -20,9 +20,11 @@
 namespace tfa {
 
 // ------------------------------------------------------------------------------------------------
-// Token by token.  A workgroup carries 32 columns of one head's state: thread (column, row group) holds RPT rows of
-// its column in registers, 16 tokens are staged in LDS at a time, and the row groups' parts of the outputs are
-// joined once per 16 tokens.  Bound by the fp32 FMAs (3 a state element and token, 6 with the tangent).
+// Token by token, for heads of 129 to 256 features (and where there is no token: states and zeros only).  A workgroup carries 32
+// columns of one head's state: thread (column, row group) holds RPT rows of its column in registers, 16 tokens are
+// staged in LDS at a time, and the row groups' parts of the outputs are joined once per 16 tokens.  Bound by the fp32
+// FMAs (3 a state element and token, 6 with the tangent) and, more, by their LDS operands: 8 x 1024 tokens of 8 bf16 heads of 256,
+// 3.2 ms, 8 TFLOP/s.
 // ------------------------------------------------------------------------------------------------
 
 constexpr int kScanCols = 32, kScanGroups = 8, kScanTokens = 16;
@@ -176,7 +178,8 @@ hipError_t launch_attn_blocks(const AttnPass& p) {
 int attn_blocks_dg_parts(const AttnPass& p) { return 2 * p.segments; }
 size_t attn_border_bytes(int rows, int cols) { return sizeof(float) * (rows <= 64 ? 64 : 128) * (cols <= 64 ? 64 : 128); }
 
-// seg_state[s] of each segment's own sum becomes the state it starts from; one thread an element
+// seg_state[s] of each segment's own sum becomes the state it starts from; one thread an element, 8 segments' sums on their way at a
+// time.  Bound by memory: 4 segments of 128 heads of 128 x 128, 17 us, 3.9 TB/s.
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnPass p) {
   const size_t size = (size_t)p.rows * p.cols, all = (size_t)p.batch * p.heads * size;
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -211,29 +214,46 @@ hipError_t launch_attn_join(const AttnPass& p) {
   return hipGetLastError();
 }
 
-// (batch, token, head, features) of any strides as a dense tensor of `padded` features, zeros past the last
+// (batch, token, head, features) of any strides as a dense tensor of `padded` features, zeros past the last: operands that are
+// not in whole 16-byte pieces, which the blocks' loads need.  32 x 1024 tokens of 16 bf16 heads of 127: 3 copies and a
+// pass 415 us (a value a thread: 860), where heads of 128 take 157.
+// A thread writes one piece of 16 bytes, and reads it in one load (at whatever address: the hardware takes any) where it is whole.
 template <typename U>
 __global__ __launch_bounds__(256) void attn_pack_kernel(const U* __restrict__ in, U* __restrict__ out, long long total,
-                                                        long long tokens, int heads, int features, int padded, long long sb,
+                                                        unsigned tokens, unsigned heads, int features, unsigned pieces, long long sb,
                                                         long long st, long long sh) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const int f = (int)(i % padded);
-  const long long r = i / padded, h = r % heads, bt = r / heads;
-  out[i] = f < features ? in[bt / tokens * sb + bt % tokens * st + h * sh + f] : U(0);
+  constexpr int N = 16 / sizeof(U);
+  struct __attribute__((aligned(sizeof(U)))) Any {
+    U v[N];
+  };
+  const long long i0 = (long long)blockIdx.x * 256, row = (long long)heads * pieces, bt0 = i0 / row, b0 = bt0 / tokens;
+  if (i0 + threadIdx.x >= total) return;
+  const unsigned p = (unsigned)(i0 - bt0 * row) + threadIdx.x, r = p % (unsigned)row;
+  const unsigned t = (unsigned)(bt0 - b0 * tokens) + p / (unsigned)row, h = r / pieces;
+  const int f = (int)(r % pieces) * N;
+  const U* src = in + (b0 + t / tokens) * sb + (long long)(t % tokens) * st + h * sh + f;
+  Any x;
+  if (f + N <= features) {
+    x = *reinterpret_cast<const Any*>(src);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x.v[j] = f + j < features ? src[j] : U(0);
+  }
+  *reinterpret_cast<uint4*>(out + (i0 + threadIdx.x) * N) = __builtin_bit_cast(uint4, x);
 }
 
 hipError_t launch_attn_pack(const HeadsView& v, void* out, int dtype, long long batch, long long tokens, int heads, int features,
                             int padded, hipStream_t stream) {
-  const long long total = batch * tokens * heads * padded, blocks = (total + 255) / 256;
+  const int pieces = padded / (dtype == 0 ? 4 : 8);
+  const long long total = batch * tokens * heads * pieces, blocks = (total + 255) / 256;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   const dim3 grid((unsigned)blocks), block(256);
   if (dtype == 0)
     hipLaunchKernelGGL((attn_pack_kernel<unsigned>), grid, block, 0, stream, static_cast<const unsigned*>(v.p),
-                       static_cast<unsigned*>(out), total, tokens, heads, features, padded, v.sb, v.st, v.sh);
+                       static_cast<unsigned*>(out), total, (unsigned)tokens, (unsigned)heads, features, (unsigned)pieces, v.sb, v.st, v.sh);
   else
     hipLaunchKernelGGL((attn_pack_kernel<unsigned short>), grid, block, 0, stream, static_cast<const unsigned short*>(v.p),
-                       static_cast<unsigned short*>(out), total, tokens, heads, features, padded, v.sb, v.st, v.sh);
+                       static_cast<unsigned short*>(out), total, (unsigned)tokens, (unsigned)heads, features, (unsigned)pieces, v.sb, v.st, v.sh);
   return hipGetLastError();
 }
 
@@ -288,8 +308,16 @@ hipError_t launch_attn_head_sum(const float* in, void* out, int dtype, long long
 
 // ------------------------------------------------------------------------------------------------
 // One token of every stream: S <- gamma S + k v^T in place, o = scale S^T q.  Bound by reading and writing the states
-// (8 bytes an element).  A workgroup takes 32 columns: 8 lanes of four columns, 32 row groups of 4 rows a pass.
+// (8 bytes an element), each of them once: 256 streams of 16 heads of 128 x 128, 109 us, 4.9 TB/s.  A workgroup takes 32 columns,
+// so that one stream of 8 heads of 64 is 16 workgroups: 8 lanes of four columns (a 128-byte line together), 32 row groups of 4
+// rows a pass, all of a pass's 16-byte loads ahead of its arithmetic.  (At addresses that are no multiples of 16 bytes the same
+// accesses take 163 us.  Where columns are no multiple of 4 a row's last ones go by the value: 126 columns, 180 us; all of them so, 199.)
 // ------------------------------------------------------------------------------------------------
+
+// four neighbours at any address of a float (one access: the hardware asks for no more)
+struct __attribute__((aligned(4))) AnyFour {
+  float v[4];
+};
 
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void attn_step_kernel(AttnStep p, int slices) {
@@ -315,12 +343,13 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnStep p, int slices) 
       qr[i] = in ? to_f32(q[r]) : 0.0f;
       kr[i] = in ? to_f32(k[r]) : 0.0f;
       const float* src = S + (long long)r * p.cols + n;
-      if (VEC) {
-        const float4 x = in && n < p.cols ? *reinterpret_cast<const float4*>(src) : make_float4(0, 0, 0, 0);
-        s[i][0] = x.x; s[i][1] = x.y; s[i][2] = x.z; s[i][3] = x.w;
+      if (in && (VEC ? n < p.cols : n + 3 < p.cols)) {
+        const AnyFour x = *reinterpret_cast<const AnyFour*>(src);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = x.v[j];
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = in && n + j < p.cols ? src[j] : 0.0f;
+        for (int j = 0; j < 4; ++j) s[i][j] = !VEC && in && n + j < p.cols ? src[j] : 0.0f;
       }
     }
 #pragma unroll
@@ -333,9 +362,9 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnStep p, int slices) 
         acc[j] = __builtin_fmaf(qr[i], s[i][j], acc[j]);
       }
       if (r < p.rows) {
-        if (VEC) {
-          if (n < p.cols) *reinterpret_cast<float4*>(dst) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
-        } else {
+        if (VEC ? n < p.cols : n + 3 < p.cols) {
+          *reinterpret_cast<AnyFour*>(dst) = AnyFour{{s[i][0], s[i][1], s[i][2], s[i][3]}};
+        } else if (!VEC) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (n + j < p.cols) dst[j] = s[i][j];
@@ -359,7 +388,7 @@ template <typename T>
 static void step_launch(const AttnStep& p) {
   const int slices = (p.cols + 31) / 32;
   const dim3 grid((unsigned)(p.batch * p.heads * slices)), block(256);
-  if (p.cols % 4 == 0 && reinterpret_cast<uintptr_t>(p.state) % 16 == 0)
+  if (p.cols % 4 == 0)
     hipLaunchKernelGGL((attn_step_kernel<T, true>), grid, block, 0, p.stream, p, slices);
   else
     hipLaunchKernelGGL((attn_step_kernel<T, false>), grid, block, 0, p.stream, p, slices);

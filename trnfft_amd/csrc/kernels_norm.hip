@@ -3,7 +3,8 @@
 //   xhat = (x - mean) rstd over the positions and the channels of a group, z = xhat w + b, y = act(z)
 //   dz = dy act'(z), db = sum dz, dw = sum dz xhat, dx = rstd (dz w - mean(dz w) - xhat mean(dz w xhat))
 //
-// Memory bound: forward x and y once, backward x, dy and dx once is the floor.  Statistics are fp32 (mean, sum of squared
+// Memory bound: forward x and y once, backward x, dy and dx once is the floor.  Three ways, by what of a sample fits where:
+// a team of lanes (norm_rows), a workgroup's registers (norm_tile), or several passes over memory.  Statistics are fp32 (mean, sum of squared
 // deviations) pairs that are merged, never a difference of sums of squares.  With lengths, positions at and past
 // lengths[n] * inner are padding: not read, zeros in y and dx.
 #include "model_ops.h"
@@ -414,7 +415,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_kernel(NormArgs a, lon
 }
 
 // ------------------------------------------------------------------------------------------------
-// Samples that fit a workgroup's registers: one launch, every value read once.  A workgroup takes whole groups of one
+// Samples that fit a workgroup's registers: one launch, every value read once (64 x 1000 x 512 in 32 groups, bf16: 33 us, 3.9 TB/s;
+// in passes 63; 64 x 626 x 512 29 against 45, a training pass with all of its host work 118 against 136; past 1280 positions of such a tile only passes remain).  A workgroup takes whole groups of one
 // sample, some 128 bytes of each position (a cache line), K 16-byte vectors a thread.  Statistics are two passes over the
 // registers.  Gradients keep x and dy; the activation's slope is computed twice, which is cheaper than keeping it.
 // ------------------------------------------------------------------------------------------------
@@ -595,6 +597,199 @@ __global__ __launch_bounds__(THREADS) void norm_whole_grad_kernel(NormArgs a, No
   }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Samples of few positions (a frame of a stream, or every frame normalised by itself): several to a wave.  A team of S <= 64 lanes takes one
+// tile of one sample, K vectors a lane; its sums are lane exchanges, without shared memory or barriers.  Teams go on to
+// further samples of the same tile, and so sum the weights' gradients in registers: the partial sums that reach memory are one row a
+// workgroup, where a row a sample would be twice as much as x itself.  40064 samples of 256 features, bf16: 24 us in one group, 17 in 4
+// (a workgroup a sample and 8 vectors: 372 and 728); with gradients 65 and 56 (814 and 1707).  For what it takes it is never slower.
+// ------------------------------------------------------------------------------------------------
+
+struct NormRows {
+  int slot, lanes, rows, groups, k;  // lanes of a group (a power of two), of a tile, positions at a time; groups of a tile; K (0: not taken)
+  unsigned tiles, parts;             // workgroups of a tile: rows of the weights' partial sums
+};
+constexpr int kRowsThreads = 256;
+
+struct TeamLane {
+  int row, ch, g;
+  long long n, step;  // first sample of the team, samples apart
+  bool on, first;     // has channels; is its group's first lane
+};
+template <int V>
+__device__ __forceinline__ TeamLane team_lane(const NormArgs& a, const NormRows& t) {
+  const int size = t.lanes * t.rows, lane = threadIdx.x % size % t.lanes, each = a.channels / a.groups;
+  const int teams = kRowsThreads / size, group = (int)(blockIdx.x % t.tiles) * t.groups + lane / t.slot, vec = lane % t.slot;
+  TeamLane m;
+  m.row = threadIdx.x % size / t.lanes;
+  m.on = group < a.groups && vec * V < each;
+  m.first = vec == 0 && m.row == 0;
+  m.g = m.on ? group : 0;
+  m.ch = m.on ? group * each + vec * V : 0;
+  m.n = (long long)(blockIdx.x / t.tiles) * teams + threadIdx.x / size;
+  m.step = (long long)t.parts * teams;
+  return m;
+}
+__device__ __forceinline__ float team_sum(float u, const NormRows& t) {
+  for (int o = 1; o < t.slot; o *= 2) u += __shfl_xor(u, o);
+  for (int o = t.lanes; o < t.lanes * t.rows; o *= 2) u += __shfl_xor(u, o);
+  return u;
+}
+
+template <typename T, int V, int K>
+__global__ __launch_bounds__(kRowsThreads) void norm_rows_kernel(NormArgs a, NormRows t) {
+  const TeamLane m = team_lane<V>(a, t);
+  const int each = a.channels / a.groups, positions = (int)a.positions;
+  float w[V], b[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    w[i] = a.weight ? a.weight[m.ch + i] : 1.0f;
+    b[i] = a.bias ? a.bias[m.ch + i] : 0.0f;
+  }
+  for (long long n = m.n; n < a.batch; n += m.step) {
+    const int live = (int)live_positions(a, n);
+    const size_t at = (size_t)n * a.positions * a.channels + m.ch;
+    const T* x = static_cast<const T*>(a.x) + at;
+    Raw<T, V> v[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      for (unsigned& u : v[k].w) u = 0;
+      const int r = m.row + k * t.rows;
+      if (m.on && r < live) v[k] = *reinterpret_cast<const Raw<T, V>*>(x + (size_t)r * a.channels);
+    }
+    // (distances from the group's first value, as above)
+    const float pivot = __shfl(v[0].at(0), (int)(threadIdx.x & 63) / (t.lanes * t.rows) * (t.lanes * t.rows) + threadIdx.x % t.lanes / t.slot * t.slot);
+    float sum = 0.0f, m2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (m.on && m.row + k * t.rows < live)
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum += v[k].at(i) - pivot;
+    const float count = (float)live * (float)each, mean = live ? pivot + team_sum(sum, t) / count : 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (m.on && m.row + k * t.rows < live)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = v[k].at(i) - mean;
+          m2 = __builtin_fmaf(d, d, m2);
+        }
+    m2 = team_sum(m2, t);
+    const float rstd = 1.0f / sqrtf((live ? m2 / count : 0.0f) + a.eps);
+    if (m.on && m.first) {
+      a.mean[n * a.groups + m.g] = mean;
+      a.rstd[n * a.groups + m.g] = rstd;
+    }
+    T* y = static_cast<T*>(a.y) + at;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int r = m.row + k * t.rows;
+      if (!m.on || r >= positions) continue;
+      float z[V] = {};
+      if (r < live)
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = activate(__builtin_fmaf(v[k].at(i) - mean, rstd * w[i], b[i]), a.act);
+      store_pack<T, V>(y + (size_t)r * a.channels, z);
+    }
+  }
+}
+
+// the same for the gradients; partial sums of dz and dz xhat by channel at ws[(part * 2 + {0, 1}) * channels + c]
+template <typename T, int V, int K>
+__global__ __launch_bounds__(kRowsThreads) void norm_rows_grad_kernel(NormArgs a, NormRows t) {
+  __shared__ float part[kRowsThreads / 64][64 * V];
+  const TeamLane m = team_lane<V>(a, t);
+  const int each = a.channels / a.groups, positions = (int)a.positions;
+  float w[V], b[V], db[V] = {}, dw[V] = {};
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    w[i] = a.weight ? a.weight[m.ch + i] : 1.0f;
+    b[i] = a.bias ? a.bias[m.ch + i] : 0.0f;
+  }
+  for (long long n = m.n; n < a.batch; n += m.step) {
+    const int live = (int)live_positions(a, n);
+    const size_t at = (size_t)n * a.positions * a.channels + m.ch;
+    const T* x = static_cast<const T*>(a.x) + at;
+    const T* dy = static_cast<const T*>(a.dy) + at;
+    Raw<T, V> v[K], d[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int r = m.row + k * t.rows;
+      if (m.on && r < live) {
+        v[k] = *reinterpret_cast<const Raw<T, V>*>(x + (size_t)r * a.channels);
+        d[k] = *reinterpret_cast<const Raw<T, V>*>(dy + (size_t)r * a.channels);
+      }
+    }
+    const float mean = a.mean[n * a.groups + m.g], rstd = a.rstd[n * a.groups + m.g];
+    float e[K][V], xh[K][V], u = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        e[k][i] = xh[k][i] = 0.0f;
+        if (m.on && m.row + k * t.rows < live) {
+          xh[k][i] = (v[k].at(i) - mean) * rstd;
+          const float dz = d[k].at(i) * activation_slope(__builtin_fmaf(xh[k][i], w[i], b[i]), a.act);
+          db[i] += dz;
+          dw[i] = __builtin_fmaf(dz, xh[k][i], dw[i]);
+          e[k][i] = dz * w[i];
+          u += e[k][i];
+          q = __builtin_fmaf(e[k][i], xh[k][i], q);
+        }
+      }
+    const float count = (float)live * (float)each;
+    u = team_sum(u, t), q = team_sum(q, t);
+    const float c1 = live ? u / count : 0.0f, c2 = live ? q / count : 0.0f;
+    T* dx = static_cast<T*>(a.y) + at;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int r = m.row + k * t.rows;
+      if (!m.on || r >= positions) continue;
+      float z[V] = {};
+      if (r < live)
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = rstd * (e[k][i] - c1 - xh[k][i] * c2);
+      store_pack<T, V>(dx + (size_t)r * a.channels, z);
+    }
+  }
+  if (!a.dweight && !a.dbias) return;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int z = 0; z < 2; ++z) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float s = z ? dw[i] : db[i];
+      for (int o = t.lanes; o < 64; o *= 2) s += __shfl_xor(s, o);
+      if (lane < t.lanes) part[threadIdx.x >> 6][lane * V + i] = s;
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < t.lanes * V; c += kRowsThreads) {
+      const int own = c / V, group = (int)(blockIdx.x % t.tiles) * t.groups + own / t.slot, at = own % t.slot * V;
+      if (group < a.groups && at < each)
+        a.ws[((size_t)(blockIdx.x / t.tiles) * 2 + z) * a.channels + group * each + at + c % V] = part[0][c] + part[1][c] + part[2][c] + part[3][c];
+    }
+    __syncthreads();
+  }
+}
+
+// The tile of a sample that a team takes, where four vectors a lane hold all positions.
+static NormRows norm_rows(const NormArgs& a, int size) {
+  NormRows t{};
+  const int V = 16 / size, each = a.channels / a.groups;
+  if (each % V || each / V > 64) return t;
+  for (t.slot = 1; t.slot < each / V;) t.slot *= 2;
+  for (t.groups = 1; t.groups < a.groups && t.groups * t.slot < 8;) t.groups *= 2;  // (128 bytes of a position, a cache line)
+  t.lanes = t.groups * t.slot;
+  for (t.rows = 1; t.rows < a.positions && t.rows * t.lanes < 64;) t.rows *= 2;
+  const long long k = (a.positions + t.rows - 1) / t.rows;
+  if (k > 4) return t;
+  t.k = k == 1 ? 1 : 4;
+  t.tiles = (unsigned)((a.groups + t.groups - 1) / t.groups);
+  const long long teams = kRowsThreads / (t.lanes * t.rows), need = (a.batch + teams - 1) / teams;
+  t.parts = (unsigned)std::min(need, std::max(1LL, 2048LL / t.tiles));  // (2048: eight waves a SIMD)
+  return t;
+}
+
 // The tile of a sample that a workgroup can hold (threads = 0: none can): K vectors a thread, of one tensor or two. Few threads with many vectors
 // leave room for several workgroups a compute unit, which cover each other's reductions (1024 threads of 5 vectors: one fits)
 static NormTile norm_tile(const NormArgs& a, int size) {
@@ -642,7 +837,9 @@ bool norm_aligned(const NormArgs& a) {
 
 size_t norm_workspace_bytes(const NormArgs& a, bool backward) {
   if (a.batch == 0 || a.positions == 0) return 0;
-  if (norm_tile(a, a.dtype == 0 ? 4 : 2).threads) return backward ? sizeof(float) * (size_t)a.batch * 2 * a.channels : 0;
+  const int size = a.dtype == 0 ? 4 : 2;
+  if (const NormRows t = norm_rows(a, size); t.k) return backward ? sizeof(float) * (size_t)t.parts * 2 * a.channels : 0;
+  if (norm_tile(a, size).threads) return backward ? sizeof(float) * (size_t)a.batch * 2 * a.channels : 0;
   const size_t parts = (size_t)a.batch * norm_splits(a) * 2 * a.channels;
   return sizeof(float) * (parts + (backward ? (size_t)a.batch * a.groups * 2 : 0));
 }
@@ -660,6 +857,18 @@ static hipError_t whole_launch(const NormArgs& a, const NormTile& t, bool backwa
   } else {
     hipLaunchKernelGGL((norm_whole_grad_kernel<T, V, K, THREADS>), grid, block, 0, a.stream, a, t);
     if (a.dweight || a.dbias) weight_grad_launch(a, a.batch);
+  }
+  return hipGetLastError();
+}
+
+template <typename T, int V, int K>
+static hipError_t rows_launch(const NormArgs& a, const NormRows& t, bool backward) {
+  const dim3 grid(t.parts * t.tiles), block(kRowsThreads);
+  if (!backward) {
+    hipLaunchKernelGGL((norm_rows_kernel<T, V, K>), grid, block, 0, a.stream, a, t);
+  } else {
+    hipLaunchKernelGGL((norm_rows_grad_kernel<T, V, K>), grid, block, 0, a.stream, a, t);
+    if (a.dweight || a.dbias) weight_grad_launch(a, t.parts);
   }
   return hipGetLastError();
 }
@@ -700,6 +909,8 @@ template <typename T>
 static hipError_t norm_typed(const NormArgs& a, bool backward) {
   constexpr int V = 16 / sizeof(T);
   if (norm_vectors<T>(a)) {
+    if (const NormRows t = norm_rows(a, sizeof(T)); t.k)
+      return t.k == 1 ? rows_launch<T, V, 1>(a, t, backward) : rows_launch<T, V, 4>(a, t, backward);
     const NormTile t = norm_tile(a, sizeof(T));
     if (t.threads) return whole_sizes<T, V>(a, t, backward);
     return backward ? backward_launch<T, V>(a) : forward_launch<T, V>(a);

@@ -81,10 +81,6 @@ int attn_scan_dg_parts(const AttnPass& p);
 int attn_blocks_dg_parts(const AttnPass& p);
 size_t attn_border_bytes(int rows, int cols);  // of one border's state
 hipError_t launch_attn_blocks(const AttnPass& p);
-inline bool whole_view(const HeadsView& v, int size, int bytes) {
-  const int n = bytes / size;
-  return reinterpret_cast<uintptr_t>(v.p) % bytes == 0 && v.sb % n == 0 && v.st % n == 0 && v.sh % n == 0;
-}
 // a dense copy (batch, tokens, heads, padded) of an operand, zeros past its features
 hipError_t launch_attn_pack(const HeadsView& v, void* out, int dtype, long long batch, long long tokens, int heads, int features,
                             int padded, hipStream_t stream);

@@ -10,11 +10,7 @@ using tfa::set_error;
 
 namespace {
 
-int launched(hipError_t e, const char* what) {
-  if (e == hipSuccess) return TFA_OK;
-  (void)what;
-  return set_error(TFA_ERR_HIP, hipGetErrorString(e));
-}
+int launched(hipError_t e) { return e == hipSuccess ? TFA_OK : set_error(TFA_ERR_HIP, hipGetErrorString(e)); }
 
 bool dtype_ok(int32_t d) { return d == TFA_DTYPE_F32 || d == TFA_DTYPE_BF16 || d == TFA_DTYPE_F16; }
 size_t dtype_size(int32_t d) { return d == TFA_DTYPE_F32 ? 4 : 2; }
@@ -64,12 +60,17 @@ tfa::AttnPass pass_of(const tfa_attn_desc* d, const float* log_decay, const int6
   return p;
 }
 
-// Sequences of up to kScanTokens go token by token, longer ones in blocks on the matrix cores.
-constexpr int64_t kScanTokens = 16;
+// Heads of up to kBlockDim features go in blocks of tokens on the matrix cores, wider ones (whose state does not fit a wave's
+// registers) token by token.  Blocks are the better choice from the first token on: 256 x 4 tokens of 16 bf16 heads of 128, 136 against 168 us,
+// training 538 against 1037; 16 tokens 137 against 422 us; 64 x 4 of 8 heads of 64, 16 against 15 us.
+constexpr int32_t kBlockDim = 128;
 // A long sequence is cut into segments where batch * heads alone leave compute units idle: about kWantBlocks
-// workgroups in all, segments of at least kSegTokens.
+// workgroups in all, segments of at least kSegTokens.  Twice as many workgroups: 64 x 626 tokens of 8 heads of 64 99 against
+// 71 us, 1 x 65536 of 16 heads of 128 487 against 454, training on 8 x 4096 1205 against 1040 (sums and joins repeat the
+// keys' and values' reading).  Segments of at least 256: training on 4 x 1001 of 6 fp32 heads 350 against 223 us.
 constexpr int64_t kWantBlocks = 512, kSegTokens = 128;
-// Tokens between the states that the decays' gradient keeps: a quarter of the traffic of keeping each 64-token block's.
+// Tokens between the states that the decays' gradient keeps: a quarter of the traffic of keeping each 64-token block's
+// (training on 8 x 4096 tokens of 16 heads of 128: 1017 us, with 64 tokens 1383; 64 x 626 of 8 heads of 64: 341 and 398).
 constexpr int64_t kStretch = 256;
 
 struct Plan {
@@ -86,7 +87,7 @@ Plan plan_of(const tfa_attn_desc* d, bool backward) {
   Plan plan{};
   plan.segments = 1;
   plan.seg_tokens = std::max<int64_t>(1, (d->tokens + 63) / 64 * 64);
-  plan.blocks = d->tokens > kScanTokens && d->key_dim <= 128 && d->value_dim <= 128;
+  plan.blocks = d->tokens > 0 && d->key_dim <= kBlockDim && d->value_dim <= kBlockDim;
   if (!plan.blocks || d->batch == 0) return plan;
   const int piece = 16 / (int)dtype_size(d->dtype);
   const int64_t* strides[3] = {d->q_stride, d->k_stride, d->v_stride};
@@ -123,7 +124,7 @@ int operand(const tfa_attn_desc* d, const Plan& plan, int i, int32_t own, int32_
     return TFA_OK;
   }
   const hipError_t e = tfa::launch_attn_pack(*v, *space, d->dtype, d->batch, d->tokens, own, features, plan.padded[i], stream);
-  if (e != hipSuccess) return launched(e, "operand copy");
+  if (e != hipSuccess) return launched(e);
   const long long row = (long long)own * plan.padded[i];
   *v = {*space, d->tokens * row, row, plan.padded[i], v->group};
   *space += plan.pack_bytes[i];
@@ -227,8 +228,8 @@ int tfa_linear_attention(const tfa_attn_desc* desc, const void* q, const void* k
   if (const int rc = operand(desc, plan, 1, desc->k_heads, desc->key_dim, &p.b, &space, p.stream)) return rc;
   if (const int rc = operand(desc, plan, 2, desc->v_heads, desc->value_dim, &p.c, &space, p.stream)) return rc;
   float* states = reinterpret_cast<float*>(space);
-  if (const hipError_t e = segment_states(p, plan, states)) return launched(e, "segments");
-  return launched(run_pass(p, plan, states), "linear attention");
+  if (const hipError_t e = segment_states(p, plan, states)) return launched(e);
+  return launched(run_pass(p, plan, states));
 }
 
 int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, const void* k, const void* v,
@@ -274,7 +275,7 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
   pv.m_r = d.value_dim;
   pv.m_n = 1;
   if (d.batch > 0 && plan.segments > 1) {
-    if (const hipError_t e = segment_states(pv, plan, grad_states)) return launched(e, "gradient segments");
+    if (const hipError_t e = segment_states(pv, plan, grad_states)) return launched(e);
     if (grad_q || grad_log_decay) {
       tfa::AttnPass p = pass_of(desc, log_decay, lengths, stream);
       p.b = kv;
@@ -284,7 +285,7 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
       p.m_in = state_in;
       p.m_r = d.value_dim;
       p.m_n = 1;
-      if (const hipError_t e = segment_states(p, plan, states)) return launched(e, "segments");
+      if (const hipError_t e = segment_states(p, plan, states)) return launched(e);
     }
   }
   if (d.batch > 0 && (grad_q || grad_log_decay)) {
@@ -308,11 +309,11 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
       p.stretch = (int)space.stretch;
       p.log_stretch = __builtin_ctz((unsigned)space.stretch);
     }
-    if (const hipError_t e = run_pass(p, plan, states)) return launched(e, "query gradient");
+    if (const hipError_t e = run_pass(p, plan, states)) return launched(e);
     if (p.out_f32 && grad_q && rows)
       if (const hipError_t e = tfa::launch_attn_head_sum(reinterpret_cast<const float*>(ws + space.dq), grad_q, d.dtype, rows,
                                                          d.q_heads, d.heads / d.q_heads, d.key_dim, s))
-        return launched(e, "query gradient sum");
+        return launched(e);
   }
   if (d.batch > 0 && (grad_k || grad_log_decay)) {
     tfa::AttnPass p = pass_of(desc, log_decay, lengths, stream);
@@ -336,25 +337,25 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
       p.stretch = (int)space.stretch;
       p.log_stretch = __builtin_ctz((unsigned)space.stretch);
     }
-    if (const hipError_t e = run_pass(p, plan, grad_states)) return launched(e, "key gradient");
+    if (const hipError_t e = run_pass(p, plan, grad_states)) return launched(e);
     if (p.out_f32 && rows)
       if (const hipError_t e = tfa::launch_attn_head_sum(reinterpret_cast<const float*>(ws + space.dk), grad_k, d.dtype, rows,
                                                          d.k_heads, d.heads / d.k_heads, d.key_dim, s))
-        return launched(e, "key gradient sum");
+        return launched(e);
   }
   if (grad_log_decay)
     if (const hipError_t e = tfa::launch_attn_dg_sum(parts, grad_log_decay, d.batch, d.heads, space.dg_each, s))
-      return launched(e, "decay gradient sum");
+      return launched(e);
   if (d.batch > 0 && (grad_v || grad_state_in)) {
     tfa::AttnPass p = pv;
     p.out_f32 = d.v_heads != d.heads;
     p.out = p.out_f32 ? ws + space.dv : grad_v;
     if (!p.out) return set_error(TFA_ERR_INVALID, "grad_state_in needs grad_v");
-    if (const hipError_t e = run_pass(p, plan, grad_states)) return launched(e, "value gradient");
+    if (const hipError_t e = run_pass(p, plan, grad_states)) return launched(e);
     if (p.out_f32 && grad_v && rows)
       if (const hipError_t e = tfa::launch_attn_head_sum(reinterpret_cast<const float*>(ws + space.dv), grad_v, d.dtype, rows,
                                                          d.v_heads, d.heads / d.v_heads, d.value_dim, s))
-        return launched(e, "value gradient sum");
+        return launched(e);
   }
   return TFA_OK;
 }
@@ -374,7 +375,7 @@ int tfa_linear_attention_step(const tfa_attn_desc* desc, const void* q, const vo
   p.rows = d.key_dim, p.cols = d.value_dim, p.heads = d.heads, p.dtype = d.dtype, p.batch = d.batch;
   p.log_decay = log_decay, p.state = state, p.out = out, p.scale = d.scale;
   p.stream = static_cast<hipStream_t>(stream);
-  return launched(tfa::launch_attn_step(p), "linear attention step");
+  return launched(tfa::launch_attn_step(p));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -419,7 +420,7 @@ int tfa_group_norm(const tfa_norm_desc* desc, const void* x, const float* weight
   a.lengths = reinterpret_cast<const long long*>(lengths);
   a.ws = static_cast<float*>(workspace), a.stream = static_cast<hipStream_t>(stream);
   if (!tfa::norm_aligned(a)) return set_error(TFA_ERR_INVALID, "x and y must be 16-byte aligned");
-  return launched(tfa::launch_norm_forward(a), "group norm");
+  return launched(tfa::launch_norm_forward(a));
 }
 
 int tfa_group_norm_backward(const tfa_norm_desc* desc, const void* x, const void* grad_y, const float* weight,
@@ -434,7 +435,7 @@ int tfa_group_norm_backward(const tfa_norm_desc* desc, const void* x, const void
   a.lengths = reinterpret_cast<const long long*>(lengths);
   a.ws = static_cast<float*>(workspace), a.stream = static_cast<hipStream_t>(stream);
   if (!tfa::norm_aligned(a)) return set_error(TFA_ERR_INVALID, "x, grad_y and grad_x must be 16-byte aligned");
-  return launched(tfa::launch_norm_backward(a), "group norm gradient");
+  return launched(tfa::launch_norm_backward(a));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -466,7 +467,7 @@ int tfa_adamw_step(int64_t count, const tfa_adam_tensor* tensors, const tfa_adam
   static_assert(sizeof(tfa_adam_tensor) == sizeof(tfa::AdamTensor), "one layout");
   const hipError_t e = tfa::launch_adamw(reinterpret_cast<const tfa::AdamTensor*>(tensors), count, a, static_cast<hipStream_t>(stream));
   if (e == hipErrorInvalidValue) return set_error(TFA_ERR_UNSUPPORTED, "tensor beyond the launch grid");
-  return launched(e, "AdamW step");
+  return launched(e);
 }
 
 int tfa_adamw_state_values(int64_t count, const tfa_code_tensor* tensors, int32_t squares, tfa_stream stream) {
@@ -479,7 +480,7 @@ int tfa_adamw_state_values(int64_t count, const tfa_code_tensor* tensors, int32_
   const hipError_t e = tfa::launch_adam_values(reinterpret_cast<const tfa::CodeTensor*>(tensors), count, squares != 0,
                                                static_cast<hipStream_t>(stream));
   if (e == hipErrorInvalidValue) return set_error(TFA_ERR_UNSUPPORTED, "tensor beyond the launch grid");
-  return launched(e, "state values");
+  return launched(e);
 }
 
 }  // extern "C"
