@@ -119,8 +119,10 @@ __device__ __forceinline__ void merge(float& mean, float& m2, float& count, floa
   count = total;
 }
 
-// A workgroup takes rows [r0, r1) of one sample and up to 256 vectors of V channels; a thread keeps its channels
-// over its rows: kLane rows apart.
+// Passes over memory: statistics, join, result; backward sums, join, weights' gradients, result.  A workgroup takes rows [r0, r1) of one
+// sample and up to 256 vectors of V channels (V = 16 bytes, or 1 where the channels are no multiple of that); a thread keeps its
+// channels over its rows, `lanes` apart.  32 x 160882 x 32 (330 MB of bf16, more than the caches hold): statistics
+// 72 us, 4.6 TB/s, result 132 us, 5.0 TB/s, a large copy's rate.
 constexpr int kNormThreads = 256;
 struct Slab {
   int col, lane, lanes;  // first channel of the thread's vector, row lane, row lanes
@@ -210,29 +212,49 @@ __device__ __forceinline__ float rows_of(long long split, long long rows_each, l
   return (float)max(0LL, min(rows_each, live - split * rows_each));
 }
 
-// joins the partials of one (sample, group): a wave each
-__global__ __launch_bounds__(64) void norm_join_kernel(NormArgs a, int splits, long long rows_each) {
+// Joins the partials of one (sample, group).  A wave takes them where they are few; else 1024 threads, several splits on their way
+// each: 1 x 160882 x 32 in 8 groups, whose 8 joins had 8192 partials (2048 splits), 43 us; with a wave each, 92.
+constexpr int kJoinFew = 512;
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_join_kernel(NormArgs a, int splits, long long rows_each) {
+  __shared__ float red[3][THREADS / 64];
   const long long n = blockIdx.x / a.groups;
   const int g = (int)(blockIdx.x % a.groups), each = a.channels / a.groups;
   const long long live = live_positions(a, n);
+  const int width = min(each, THREADS), lanes = THREADS / width, lane = threadIdx.x / width;
+  // (means as distances from the first one: merging rounds the distance, not a mean far from zero)
+  const float pivot = a.ws[n * splits * 2 * a.channels + g * each];
   float mean = 0.0f, m2 = 0.0f, count = 0.0f;
-  for (long long i = threadIdx.x; i < (long long)splits * each; i += 64) {
-    const long long split = i / each;
-    const float* src = a.ws + (n * splits + split) * 2 * a.channels + g * each + i % each;
-    merge(mean, m2, count, src[0], src[a.channels], rows_of(split, rows_each, live));
-  }
+  constexpr int U = 4;
+  if (lane < lanes)
+    for (int c = threadIdx.x % width; c < each; c += width)
+      for (int s = lane; s < splits; s += U * lanes) {
+        float x[U], q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float* src = a.ws + (n * splits + min(s + u * lanes, splits - 1)) * 2 * a.channels + g * each + c;
+          x[u] = src[0] - pivot, q[u] = src[a.channels];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (s + u * lanes < splits) merge(mean, m2, count, x[u], q[u], rows_of(s + u * lanes, rows_each, live));
+      }
 #pragma unroll
   for (int o = 32; o > 0; o /= 2) {
     const float mb = __shfl_down(mean, o), qb = __shfl_down(m2, o), cb = __shfl_down(count, o);
     merge(mean, m2, count, mb, qb, cb);
   }
+  if (threadIdx.x % 64 == 0) red[0][threadIdx.x / 64] = mean, red[1][threadIdx.x / 64] = m2, red[2][threadIdx.x / 64] = count;
+  __syncthreads();
   if (threadIdx.x == 0) {
-    a.mean[blockIdx.x] = mean;
+    for (int w = 1; w < THREADS / 64; ++w) merge(mean, m2, count, red[0][w], red[1][w], red[2][w]);
+    a.mean[blockIdx.x] = count > 0.0f ? pivot + mean : 0.0f;
     a.rstd[blockIdx.x] = 1.0f / sqrtf((count > 0.0f ? m2 / count : 0.0f) + a.eps);
   }
 }
 
-// (from the last rows to the first: what the statistics read last is still in the Infinity Cache)
+// (from the last rows to the first: what the statistics read last is still in the Infinity Cache; and results past it, so that they
+// do not displace it: with both 200 us for the above, with neither 227)
 template <typename T, int V>
 __global__ __launch_bounds__(kNormThreads) void norm_apply_kernel(NormArgs a, long long rows_each, unsigned splits) {
   const Slab s = slab_of<V>(a.channels);
@@ -325,20 +347,30 @@ __global__ __launch_bounds__(kNormThreads) void norm_grad_sums_kernel(NormArgs a
 }
 
 // mean(dz w) and mean(dz w xhat) of one (sample, group): a wave each, behind the partials
-__global__ __launch_bounds__(64) void norm_grad_join_kernel(NormArgs a, int splits, float* joined) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_grad_join_kernel(NormArgs a, int splits, float* joined) {
+  __shared__ float red[2][THREADS / 64];
   const long long n = blockIdx.x / a.groups;
   const int g = (int)(blockIdx.x % a.groups), each = a.channels / a.groups;
+  const int width = min(each, THREADS), lanes = THREADS / width, lane = threadIdx.x / width;
   float u = 0.0f, q = 0.0f;
-  for (long long i = threadIdx.x; i < (long long)splits * each; i += 64) {
-    const int c = g * each + (int)(i % each);
-    const float* src = a.ws + (n * splits + i / each) * 2 * a.channels + c;
-    const float w = a.weight ? a.weight[c] : 1.0f;
-    u = __builtin_fmaf(w, src[0], u);
-    q = __builtin_fmaf(w, src[a.channels], q);
-  }
+  if (lane < lanes)
+    for (int c = threadIdx.x % width; c < each; c += width) {
+      const float w = a.weight ? a.weight[g * each + c] : 1.0f;
+      float cu = 0.0f, cq = 0.0f;
+#pragma unroll 4
+      for (int s = lane; s < splits; s += lanes) {
+        const float* src = a.ws + (n * splits + s) * 2 * a.channels + g * each + c;
+        cu += src[0], cq += src[a.channels];
+      }
+      u = __builtin_fmaf(w, cu, u), q = __builtin_fmaf(w, cq, q);
+    }
 #pragma unroll
   for (int o = 32; o > 0; o /= 2) u += __shfl_down(u, o), q += __shfl_down(q, o);
+  if (threadIdx.x % 64 == 0) red[0][threadIdx.x / 64] = u, red[1][threadIdx.x / 64] = q;
+  __syncthreads();
   if (threadIdx.x == 0) {
+    for (int w = 1; w < THREADS / 64; ++w) u += red[0][w], q += red[1][w];
     const float count = (float)live_positions(a, n) * (float)each;
     joined[2 * blockIdx.x] = count > 0.0f ? u / count : 0.0f;
     joined[2 * blockIdx.x + 1] = count > 0.0f ? q / count : 0.0f;
@@ -814,9 +846,11 @@ static NormTile norm_tile(const NormArgs& a, int size) {
 
 // ------------------------------------------------------------------------------------------------
 
-// rows of a workgroup: about 2048 workgroups in all, at least 32 rows each, at most 65535 splits
+// Rows of a workgroup: about 1024 workgroups in all, at least 32 rows each, at most 65535 splits.  bf16, forward, with 1024, 2048 and 4096:
+// 1 x 160882 x 32 in 8 groups 30, 43 and 61 us (the joins), 64 x 2000 x 512 in 32 82, 89 and 113; 32 x 160882 x 32 203, 203
+// and 207, its training pass 562, 539 and 544.
 static long long norm_rows_each(const NormArgs& a) {
-  const long long want = std::max(1LL, 2048 / std::max(1LL, a.batch));
+  const long long want = std::max(1LL, 1024 / std::max(1LL, a.batch));
   const long long splits = std::min({want, std::max(1LL, a.positions / 32), 65535LL});
   return (a.positions + splits - 1) / splits;
 }
@@ -886,7 +920,11 @@ static hipError_t forward_launch(const NormArgs& a) {
   const int vecs = a.channels / V;
   const dim3 grid((unsigned)(splits * a.batch), 1, (unsigned)((vecs + kNormThreads - 1) / kNormThreads)), block(kNormThreads);
   hipLaunchKernelGGL((norm_stats_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
-  hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(a.batch * a.groups)), dim3(64), 0, a.stream, a, (int)splits, each);
+  const dim3 joins((unsigned)(a.batch * a.groups));
+  if (splits * (a.channels / a.groups) <= kJoinFew)
+    hipLaunchKernelGGL(norm_join_kernel<64>, joins, dim3(64), 0, a.stream, a, (int)splits, each);
+  else
+    hipLaunchKernelGGL(norm_join_kernel<1024>, joins, dim3(1024), 0, a.stream, a, (int)splits, each);
   hipLaunchKernelGGL((norm_apply_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
   return hipGetLastError();
 }
@@ -898,7 +936,11 @@ static hipError_t backward_launch(const NormArgs& a) {
   const dim3 grid((unsigned)(splits * a.batch), 1, (unsigned)((vecs + kNormThreads - 1) / kNormThreads)), block(kNormThreads);
   float* joined = a.ws + (size_t)a.batch * splits * 2 * a.channels;
   hipLaunchKernelGGL((norm_grad_sums_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
-  hipLaunchKernelGGL(norm_grad_join_kernel, dim3((unsigned)(a.batch * a.groups)), dim3(64), 0, a.stream, a, (int)splits, joined);
+  const dim3 joins((unsigned)(a.batch * a.groups));
+  if (splits * (a.channels / a.groups) <= kJoinFew)
+    hipLaunchKernelGGL(norm_grad_join_kernel<64>, joins, dim3(64), 0, a.stream, a, (int)splits, joined);
+  else
+    hipLaunchKernelGGL(norm_grad_join_kernel<1024>, joins, dim3(1024), 0, a.stream, a, (int)splits, joined);
   if (a.dweight || a.dbias)
     weight_grad_launch(a, a.batch * splits);
   hipLaunchKernelGGL((norm_grad_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits, joined);
