@@ -213,7 +213,8 @@ __device__ __forceinline__ float rows_of(long long split, long long rows_each, l
 }
 
 // Joins the partials of one (sample, group).  A wave takes them where they are few; else 1024 threads, several splits on their way
-// each: 1 x 160882 x 32 in 8 groups, whose 8 joins had 8192 partials (2048 splits), 43 us; with a wave each, 92.
+// each: 1 x 160882 x 32 in 8 groups, 8 joins of 4096 partials, 30 us, with a wave each 38 (more with more splits); 64 x 2000 x 512 in 32
+// groups, 2048 joins of 256 partials, 80 us, with 1024 threads each 88.
 constexpr int kJoinFew = 512;
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_join_kernel(NormArgs a, int splits, long long rows_each) {
