@@ -194,7 +194,7 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
   const int h = (int)(block % p.heads);
   block /= p.heads;
   const int seg = first_seg + (int)(block % segs);
-  const long long b = block / segs, bh = b * p.heads + h;
+  const long long b = p.first + block / segs, bh = b * p.heads + h;
   const long long len = live_tokens(p, b);
   const long long seg_lo = seg * p.seg_tokens, seg_end = min(seg_lo + p.seg_tokens, p.tokens);
   const long long lo = min(seg_lo, len), hi = min(seg_end, len);
@@ -666,10 +666,9 @@ static hipError_t blocks_launch(const AttnPass& p) {
   const int osize = p.out_f32 || sizeof(T) == 4 ? 4 : 2;
   const bool wo = p.cols % (16 / osize) == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
   const int first = MODE == kSums && p.reverse ? 1 : 0, segs = MODE == kSums ? p.segments - 1 : p.segments;
-  const long long grid = p.batch * p.heads * segs;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((attn_blocks_kernel<T, RP, NW, MODE>), dim3((unsigned)grid), dim3(64 * NW), 0, p.stream, p, first, segs, wo);
-  return hipGetLastError();
+  return for_batches(p, (long long)p.heads * segs, 64 * NW, [&](const AttnPass& q, dim3 grid) {
+    hipLaunchKernelGGL((attn_blocks_kernel<T, RP, NW, MODE>), grid, dim3(64 * NW), 0, q.stream, q, first, segs, wo);
+  });
 }
 
 template <typename T, int MODE>

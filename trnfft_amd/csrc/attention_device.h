@@ -50,4 +50,16 @@ __device__ __forceinline__ long long live_tokens(const AttnPass& p, long long b)
   return p.lengths ? min(max(p.lengths[b], 0LL), p.tokens) : p.tokens;
 }
 
+// Launches of `each` workgroups for every batch row, as many rows at a time as a launch holds.  (One row always fits: heads are
+// below 2^16, slices of a head at most 8, and segments for few heads only.)
+template <typename Args, typename Launch>
+hipError_t for_batches(Args p, long long each, int threads, Launch launch) {
+  const long long most = max_blocks(threads) / each;
+  for (p.first = 0; p.first < p.batch; p.first += most) {
+    launch(p, dim3((unsigned)(each * (p.batch - p.first < most ? p.batch - p.first : most))));
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 }  // namespace tfa

@@ -246,11 +246,11 @@ hipError_t launch_adamw(const AdamTensor* tensors, long long count, const AdamAr
   for (long long i = 0; i < count;) {
     AdamTable tab;
     tab.count = 0;
-    unsigned long long blocks = 0;
+    long long blocks = 0;
     while (i < count && tab.count < kAdamTensors) {
       const AdamTensor& t = tensors[i];
-      const unsigned long long more = (unsigned long long)((t.n + chunk - 1) / chunk);
-      if (blocks + more > 0x7fffffffull) break;
+      const long long more = (t.n + chunk - 1) / chunk;
+      if (blocks + more > max_blocks(256)) break;
       if (more) {
         tab.t[tab.count] = t;
         tab.first[tab.count++] = (unsigned)blocks;
@@ -312,10 +312,10 @@ hipError_t launch_adam_values(const CodeTensor* tensors, long long count, bool s
   for (long long i = 0; i < count;) {
     CodeTable tab;
     tab.count = 0;
-    unsigned long long blocks = 0;
+    long long blocks = 0;
     while (i < count && tab.count < kCodeTensors) {
-      const unsigned long long more = (unsigned long long)((tensors[i].n + kAdamChunk - 1) / kAdamChunk);
-      if (blocks + more > 0x7fffffffull) break;
+      const long long more = (tensors[i].n + kAdamChunk - 1) / kAdamChunk;
+      if (blocks + more > max_blocks(256)) break;
       if (more) {
         tab.t[tab.count] = tensors[i];
         tab.first[tab.count++] = (unsigned)blocks;

@@ -17,6 +17,8 @@
 // blocks it comes from the query and key gradients themselves (attention_blocks.h).
 #include "attention_device.h"
 
+#include <algorithm>
+
 namespace tfa {
 
 // ------------------------------------------------------------------------------------------------
@@ -36,7 +38,7 @@ __global__ __launch_bounds__(256) void attn_scan_kernel(AttnPass p, int slices) 
   __shared__ float part[kScanTokens][kScanGroups][kScanCols];
   const int t = threadIdx.x, col = t % kScanCols, rg = t / kScanCols;
   const int slice = blockIdx.x % slices;
-  const long long bh = blockIdx.x / slices, b = bh / p.heads;
+  const long long bh = p.first * p.heads + blockIdx.x / slices, b = bh / p.heads;
   const int h = (int)(bh % p.heads), n = slice * kScanCols + col;
   const long long len = live_tokens(p, b);
   const T* A = head_base<T>(p.a, b, h);
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(256) void attn_scan_kernel(AttnPass p, int slices) 
       if (t < s) sum[t] += sum[t + s];
       __syncthreads();
     }
-    if (t == 0) p.dg_part[blockIdx.x] = sum[0];
+    if (t == 0) p.dg_part[bh * slices + slice] = sum[0];
   }
 }
 
@@ -143,12 +145,12 @@ int attn_scan_dg_parts(const AttnPass& p) { return (p.cols + kScanCols - 1) / kS
 template <typename T, int RPT>
 static hipError_t scan_launch(const AttnPass& p) {
   const int slices = (p.cols + kScanCols - 1) / kScanCols;
-  const dim3 grid((unsigned)(p.batch * p.heads * slices)), block(256);
-  if (p.dg_part)
-    hipLaunchKernelGGL((attn_scan_kernel<T, RPT, true>), grid, block, 0, p.stream, p, slices);
-  else
-    hipLaunchKernelGGL((attn_scan_kernel<T, RPT, false>), grid, block, 0, p.stream, p, slices);
-  return hipGetLastError();
+  return for_batches(p, (long long)p.heads * slices, 256, [&](const AttnPass& q, dim3 grid) {
+    if (q.dg_part)
+      hipLaunchKernelGGL((attn_scan_kernel<T, RPT, true>), grid, dim3(256), 0, q.stream, q, slices);
+    else
+      hipLaunchKernelGGL((attn_scan_kernel<T, RPT, false>), grid, dim3(256), 0, q.stream, q, slices);
+  });
 }
 
 template <typename T>
@@ -209,10 +211,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPass p) {
 
 hipError_t launch_attn_join(const AttnPass& p) {
   const size_t all = (size_t)p.batch * p.heads * p.rows * p.cols, blocks = (all + 255) / 256;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  if ((long long)blocks > max_blocks(256)) return hipErrorInvalidValue;  // (segments are for few heads)
   hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)blocks), dim3(256), 0, p.stream, p);
   return hipGetLastError();
 }
+
+// Workgroups of 256 for `total` threads' work, in a loop past 2^20 of them
+static unsigned looping_blocks(long long total) { return (unsigned)std::min((total + 255) / 256, 1LL << 20); }
 
 // (batch, token, head, features) of any strides as a dense tensor of `padded` features, zeros past the last: operands that are
 // not in whole 16-byte pieces, which the blocks' loads need.  32 x 1024 tokens of 16 bf16 heads of 127: 3 copies and a
@@ -226,28 +231,28 @@ __global__ __launch_bounds__(256) void attn_pack_kernel(const U* __restrict__ in
   struct __attribute__((aligned(sizeof(U)))) Any {
     U v[N];
   };
-  const long long i0 = (long long)blockIdx.x * 256, row = (long long)heads * pieces, bt0 = i0 / row, b0 = bt0 / tokens;
-  if (i0 + threadIdx.x >= total) return;
-  const unsigned p = (unsigned)(i0 - bt0 * row) + threadIdx.x, r = p % (unsigned)row;
-  const unsigned t = (unsigned)(bt0 - b0 * tokens) + p / (unsigned)row, h = r / pieces;
-  const int f = (int)(r % pieces) * N;
-  const U* src = in + (b0 + t / tokens) * sb + (long long)(t % tokens) * st + h * sh + f;
-  Any x;
-  if (f + N <= features) {
-    x = *reinterpret_cast<const Any*>(src);
-  } else {
+  for (long long i0 = (long long)blockIdx.x * 256; i0 + threadIdx.x < total; i0 += (long long)gridDim.x * 256) {
+    const long long row = (long long)heads * pieces, bt0 = i0 / row, b0 = bt0 / tokens;
+    const unsigned p = (unsigned)(i0 - bt0 * row) + threadIdx.x, r = p % (unsigned)row;
+    const unsigned t = (unsigned)(bt0 - b0 * tokens) + p / (unsigned)row, h = r / pieces;
+    const int f = (int)(r % pieces) * N;
+    const U* src = in + (b0 + t / tokens) * sb + (long long)(t % tokens) * st + h * sh + f;
+    Any x;
+    if (f + N <= features) {
+      x = *reinterpret_cast<const Any*>(src);
+    } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) x.v[j] = f + j < features ? src[j] : U(0);
+      for (int j = 0; j < N; ++j) x.v[j] = f + j < features ? src[j] : U(0);
+    }
+    *reinterpret_cast<uint4*>(out + (i0 + threadIdx.x) * N) = __builtin_bit_cast(uint4, x);
   }
-  *reinterpret_cast<uint4*>(out + (i0 + threadIdx.x) * N) = __builtin_bit_cast(uint4, x);
 }
 
 hipError_t launch_attn_pack(const HeadsView& v, void* out, int dtype, long long batch, long long tokens, int heads, int features,
                             int padded, hipStream_t stream) {
   const int pieces = padded / (dtype == 0 ? 4 : 8);
-  const long long total = batch * tokens * heads * pieces, blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)blocks), block(256);
+  const long long total = batch * tokens * heads * pieces;
+  const dim3 grid(looping_blocks(total)), block(256);
   if (dtype == 0)
     hipLaunchKernelGGL((attn_pack_kernel<unsigned>), grid, block, 0, stream, static_cast<const unsigned*>(v.p),
                        static_cast<unsigned*>(out), total, (unsigned)tokens, (unsigned)heads, features, (unsigned)pieces, v.sb, v.st, v.sh);
@@ -285,18 +290,18 @@ hipError_t launch_attn_dg_sum(const double* parts, float* out, long long batch, 
 template <typename T>
 __global__ __launch_bounds__(256) void attn_head_sum_kernel(const float* __restrict__ in, T* __restrict__ out,
                                                             long long total, int group, int d) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const float* src = in + (i / d) * group * d + i % d;
-  float s = 0.0f;
-  for (int g = 0; g < group; ++g) s += src[(long long)g * d];
-  out[i] = from_f32<T>(s);
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const float* src = in + (i / d) * group * d + i % d;
+    float s = 0.0f;
+    for (int g = 0; g < group; ++g) s += src[(long long)g * d];
+    out[i] = from_f32<T>(s);
+  }
 }
 
 hipError_t launch_attn_head_sum(const float* in, void* out, int dtype, long long rows, int heads_out, int group, int d,
                                 hipStream_t stream) {
   const long long total = rows * heads_out * d;
-  const dim3 grid((unsigned)((total + 255) / 256)), block(256);
+  const dim3 grid(looping_blocks(total)), block(256);
   if (dtype == 0)
     hipLaunchKernelGGL((attn_head_sum_kernel<float>), grid, block, 0, stream, in, static_cast<float*>(out), total, group, d);
   else if (dtype == 1)
@@ -324,7 +329,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnStep p, int slices) 
   __shared__ float part[4][32];
   const int t = threadIdx.x, c4 = t % 8, rg = t / 8, wave = t / 64;
   const int slice = blockIdx.x % slices;
-  const long long bh = blockIdx.x / slices, b = bh / p.heads;
+  const long long bh = p.first * p.heads + blockIdx.x / slices, b = bh / p.heads;
   const int h = (int)(bh % p.heads), n = slice * 32 + c4 * 4;
   const T* q = static_cast<const T*>(p.q) + b * p.q_sb + (long long)(h / p.q_group) * p.q_sh;
   const T* k = static_cast<const T*>(p.k) + b * p.k_sb + (long long)(h / p.k_group) * p.k_sh;
@@ -385,23 +390,19 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnStep p, int slices) 
 }
 
 template <typename T>
-static void step_launch(const AttnStep& p) {
+static hipError_t step_launch(const AttnStep& p) {
   const int slices = (p.cols + 31) / 32;
-  const dim3 grid((unsigned)(p.batch * p.heads * slices)), block(256);
-  if (p.cols % 4 == 0)
-    hipLaunchKernelGGL((attn_step_kernel<T, true>), grid, block, 0, p.stream, p, slices);
-  else
-    hipLaunchKernelGGL((attn_step_kernel<T, false>), grid, block, 0, p.stream, p, slices);
+  return for_batches(p, (long long)p.heads * slices, 256, [&](const AttnStep& q, dim3 grid) {
+    if (q.cols % 4 == 0)
+      hipLaunchKernelGGL((attn_step_kernel<T, true>), grid, dim3(256), 0, q.stream, q, slices);
+    else
+      hipLaunchKernelGGL((attn_step_kernel<T, false>), grid, dim3(256), 0, q.stream, q, slices);
+  });
 }
 
 hipError_t launch_attn_step(const AttnStep& p) {
-  if (p.dtype == 0)
-    step_launch<float>(p);
-  else if (p.dtype == 1)
-    step_launch<__bf16>(p);
-  else
-    step_launch<_Float16>(p);
-  return hipGetLastError();
+  if (p.dtype == 0) return step_launch<float>(p);
+  return p.dtype == 1 ? step_launch<__bf16>(p) : step_launch<_Float16>(p);
 }
 
 }  // namespace tfa

@@ -884,15 +884,33 @@ static void weight_grad_launch(const NormArgs& a, long long parts) {
                      a.channels, parts);
 }
 
+// The samples [first, first + most) of a, whose workspace holds `parts` rows of partial sums a sample.
+template <typename T>
+static NormArgs samples_of(NormArgs a, long long first, long long most, long long parts) {
+  const size_t at = (size_t)first * a.positions * a.channels;
+  a.x = static_cast<const T*>(a.x) + at;
+  a.y = static_cast<T*>(a.y) + at;
+  if (a.dy) a.dy = static_cast<const T*>(a.dy) + at;
+  a.mean += first * a.groups;
+  a.rstd += first * a.groups;
+  if (a.lengths) a.lengths += first;
+  if (a.ws) a.ws += (size_t)first * parts * 2 * a.channels;
+  a.batch = std::min(most, a.batch - first);
+  return a;
+}
+
 template <typename T, int V, int K, int THREADS>
-static hipError_t whole_launch(const NormArgs& a, const NormTile& t, bool backward) {
-  const dim3 grid((unsigned)a.batch * t.tiles), block(THREADS);
-  if (!backward) {
-    hipLaunchKernelGGL((norm_whole_kernel<T, V, K, THREADS>), grid, block, 0, a.stream, a, t);
-  } else {
-    hipLaunchKernelGGL((norm_whole_grad_kernel<T, V, K, THREADS>), grid, block, 0, a.stream, a, t);
-    if (a.dweight || a.dbias) weight_grad_launch(a, a.batch);
+static hipError_t whole_launch(const NormArgs& all, const NormTile& t, bool backward) {
+  const long long most = max_blocks(THREADS) / t.tiles;  // samples of a launch (tiles are below 2^20)
+  for (long long first = 0; first < all.batch; first += most) {
+    const NormArgs a = samples_of<T>(all, first, most, 1);
+    const dim3 grid((unsigned)a.batch * t.tiles), block(THREADS);
+    if (!backward)
+      hipLaunchKernelGGL((norm_whole_kernel<T, V, K, THREADS>), grid, block, 0, a.stream, a, t);
+    else
+      hipLaunchKernelGGL((norm_whole_grad_kernel<T, V, K, THREADS>), grid, block, 0, a.stream, a, t);
   }
+  if (backward && (all.dweight || all.dbias)) weight_grad_launch(all, all.batch);
   return hipGetLastError();
 }
 
@@ -915,36 +933,51 @@ static hipError_t whole_sizes(const NormArgs& a, const NormTile& t, bool backwar
   return t.k == 14 ? whole_launch<T, V, 14, 256>(a, t, backward) : whole_launch<T, V, 20, 256>(a, t, backward);
 }
 
+// In passes: the samples of a launch (one always fits: splits are below 2^16, groups 2^20 at most)
+static long long pass_samples(const NormArgs& a, long long splits, bool few) {
+  return std::min(max_blocks(kNormThreads) / splits, max_blocks(few ? 64 : 1024) / a.groups);
+}
+
 template <typename T, int V>
-static hipError_t forward_launch(const NormArgs& a) {
-  const long long each = norm_rows_each(a), splits = norm_splits(a);
-  const int vecs = a.channels / V;
-  const dim3 grid((unsigned)(splits * a.batch), 1, (unsigned)((vecs + kNormThreads - 1) / kNormThreads)), block(kNormThreads);
-  hipLaunchKernelGGL((norm_stats_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
-  const dim3 joins((unsigned)(a.batch * a.groups));
-  if (splits * (a.channels / a.groups) <= kJoinFew)
-    hipLaunchKernelGGL(norm_join_kernel<64>, joins, dim3(64), 0, a.stream, a, (int)splits, each);
-  else
-    hipLaunchKernelGGL(norm_join_kernel<1024>, joins, dim3(1024), 0, a.stream, a, (int)splits, each);
-  hipLaunchKernelGGL((norm_apply_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
+static hipError_t forward_launch(const NormArgs& all) {
+  const long long each = norm_rows_each(all), splits = norm_splits(all);
+  const int vecs = all.channels / V;
+  const bool few = splits * (all.channels / all.groups) <= kJoinFew;
+  const long long most = pass_samples(all, splits, few);
+  for (long long first = 0; first < all.batch; first += most) {
+    const NormArgs a = samples_of<T>(all, first, most, splits);
+    const dim3 grid((unsigned)(splits * a.batch), 1, (unsigned)((vecs + kNormThreads - 1) / kNormThreads)), block(kNormThreads);
+    hipLaunchKernelGGL((norm_stats_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
+    const dim3 joins((unsigned)(a.batch * a.groups));
+    if (few)
+      hipLaunchKernelGGL(norm_join_kernel<64>, joins, dim3(64), 0, a.stream, a, (int)splits, each);
+    else
+      hipLaunchKernelGGL(norm_join_kernel<1024>, joins, dim3(1024), 0, a.stream, a, (int)splits, each);
+    hipLaunchKernelGGL((norm_apply_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
+  }
   return hipGetLastError();
 }
 
 template <typename T, int V>
-static hipError_t backward_launch(const NormArgs& a) {
-  const long long each = norm_rows_each(a), splits = norm_splits(a);
-  const int vecs = a.channels / V;
-  const dim3 grid((unsigned)(splits * a.batch), 1, (unsigned)((vecs + kNormThreads - 1) / kNormThreads)), block(kNormThreads);
-  float* joined = a.ws + (size_t)a.batch * splits * 2 * a.channels;
-  hipLaunchKernelGGL((norm_grad_sums_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
-  const dim3 joins((unsigned)(a.batch * a.groups));
-  if (splits * (a.channels / a.groups) <= kJoinFew)
-    hipLaunchKernelGGL(norm_grad_join_kernel<64>, joins, dim3(64), 0, a.stream, a, (int)splits, joined);
-  else
-    hipLaunchKernelGGL(norm_grad_join_kernel<1024>, joins, dim3(1024), 0, a.stream, a, (int)splits, joined);
-  if (a.dweight || a.dbias)
-    weight_grad_launch(a, a.batch * splits);
-  hipLaunchKernelGGL((norm_grad_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits, joined);
+static hipError_t backward_launch(const NormArgs& all) {
+  const long long each = norm_rows_each(all), splits = norm_splits(all);
+  const int vecs = all.channels / V;
+  const bool few = splits * (all.channels / all.groups) <= kJoinFew;
+  const long long most = pass_samples(all, splits, few);
+  float* const joins_at = all.ws + (size_t)all.batch * splits * 2 * all.channels;
+  for (long long first = 0; first < all.batch; first += most) {
+    const NormArgs a = samples_of<T>(all, first, most, splits);
+    const dim3 grid((unsigned)(splits * a.batch), 1, (unsigned)((vecs + kNormThreads - 1) / kNormThreads)), block(kNormThreads);
+    float* const joined = joins_at + (size_t)first * a.groups * 2;
+    hipLaunchKernelGGL((norm_grad_sums_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits);
+    const dim3 joins((unsigned)(a.batch * a.groups));
+    if (few)
+      hipLaunchKernelGGL(norm_grad_join_kernel<64>, joins, dim3(64), 0, a.stream, a, (int)splits, joined);
+    else
+      hipLaunchKernelGGL(norm_grad_join_kernel<1024>, joins, dim3(1024), 0, a.stream, a, (int)splits, joined);
+    hipLaunchKernelGGL((norm_grad_kernel<T, V>), grid, block, 0, a.stream, a, each, (unsigned)splits, joined);
+  }
+  if (all.dweight || all.dbias) weight_grad_launch(all, all.batch * splits);
   return hipGetLastError();
 }
 

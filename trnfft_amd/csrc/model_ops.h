@@ -9,6 +9,9 @@
 
 namespace tfa {
 
+// Workgroups of a launch: a dispatch counts its threads along x in 32 bits, and what is past them is dropped without an error.
+constexpr long long max_blocks(int threads) { return 0xffffffffLL / threads; }
+
 // Sets the calling thread's error text (tfa_last_error) and returns `code`; never throws.
 int set_error(int code, const char* text) noexcept;
 
@@ -45,6 +48,7 @@ struct AttnPass {
   bool reverse;
   int dtype;
   long long batch, tokens;
+  long long first;             // batch row of the launch's first workgroup (launches set it)
   int heads;
   const float* log_decay;      // (heads)
   const long long* lengths;    // (batch) or nullptr: tokens at and past it are padding
@@ -98,6 +102,7 @@ struct AttnStep {
   int q_group, k_group, v_group;
   int rows, cols, heads, dtype;
   long long batch;
+  long long first;  // as AttnPass's
   const float* log_decay;
   float* state;  // (batch, heads, rows, cols)
   void* out;     // (batch, heads, cols)
