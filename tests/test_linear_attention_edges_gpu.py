@@ -1,0 +1,80 @@
+"""Linear attention where its inputs are at an end: values that are not finite in live frames.  What a value that is not finite reaches is what the recurrence in 64 bits says; all else is
+equal bits to the same call without it."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import trnfft_amd
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def recurrence(a, b, c, g, reverse=False):
+    """out_t = sum gamma^|t - s| (a_t . b_s) c_s over s <= t (or s >= t) and the end state, token by token, (batch, token, head, feature)."""
+    a, b, c = (x.double() for x in (a, b, c))
+    gamma = torch.exp(g.double())[:, None, None]
+    order = range(a.shape[1])
+    m = torch.zeros(*b.shape[:1], *b.shape[2:], c.shape[-1], dtype=torch.float64)
+    out = [None] * a.shape[1]
+    for t in reversed(order) if reverse else order:
+        m = gamma * m + b[:, t, :, :, None] * c[:, t, :, None, :]
+        out[t] = (a[:, t, :, None, :] @ m)[..., 0, :]
+    return torch.stack(out, 1), m
+
+
+def same_but_where_not_finite(got, clean, ref):
+    """got is not finite exactly where ref is not, and clean's bits elsewhere."""
+    bad = ~torch.isfinite(ref)
+    got, clean = got.detach().cpu(), clean.detach().cpu()
+    assert torch.equal(~torch.isfinite(got), bad)
+    assert torch.equal(torch.where(bad, 0.0, got), torch.where(bad, 0.0, clean))
+
+
+def run(parts, g, do, decays):
+    leaves = [x.cuda().requires_grad_() for x in parts]
+    g = g.cuda().requires_grad_(decays)
+    o, last = trnfft_amd.linear_attention(*leaves, g, scale=1.0, return_state=True)
+    grads = torch.autograd.grad(o, leaves + ([g] if decays else []), do.cuda())
+    return o, last, *grads
+
+
+# (a head of 160 features goes token by token; 600 frames of one sequence are shared out over segments)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,dk,dv", [(150, 32, 48), (600, 64, 128), (90, 160, 16)])
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+@pytest.mark.parametrize("name,value", [("k", math.nan), ("v", math.inf), ("v", math.nan), ("q", -math.inf), ("do", math.inf)])
+def test_what_is_not_finite_does_not_reach_back(dtype, t, dk, dv, where, name, value):
+    r = torch.Generator().manual_seed(t + dk)
+    q, k, v, do = (torch.randn(1, t, 2, d, generator=r).to(dtype) for d in (dk, dk, dv, dv))
+    g = torch.tensor([-0.02, -0.3])
+    clean = {decays: run((q, k, v), g, do, decays) for decays in (False, True)}
+    at = {"first": 0, "middle": t // 2 + 2, "last": t - 1}[where]
+    dirty = {"q": q.clone(), "k": k.clone(), "v": v.clone(), "do": do.clone()}
+    dirty[name][0, at, 0, 5 if name in "qk" else dv - 2] = value
+    q, k, v, do = (dirty[n] for n in ("q", "k", "v", "do"))
+    o, last = recurrence(q, k, v, g)
+    refs = [o, last, recurrence(do, v, k, g)[0], recurrence(v, do, q, g, True)[0], recurrence(k, q, do, g, True)[0]]
+    for decays in (False, True):
+        got = run((q, k, v), g, do, decays)
+        for x, y, ref in zip(got, clean[decays], refs):
+            same_but_where_not_finite(x, y, ref)
+        if decays:
+            assert torch.equal(got[5][1], clean[True][5][1])  # the other head's decay
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_near_the_largest_stay_in_their_frames(dtype):
+    # the largest finite value of the type, in a value that later frames alone may see
+    q, k, v = (torch.randn(1, 100, 1, 32, generator=torch.Generator().manual_seed(i)).to(dtype) for i in range(3))
+    g = torch.tensor([-0.1])
+    clean = trnfft_amd.linear_attention(*(x.cuda() for x in (q, k, v, g)))
+    v[0, 40, 0, 3] = torch.finfo(dtype).max
+    got = trnfft_amd.linear_attention(*(x.cuda() for x in (q, k, v, g)))
+    assert torch.equal(got[:, :40], clean[:, :40])
+    assert torch.equal(got[..., :3], clean[..., :3]) and torch.equal(got[..., 4:], clean[..., 4:])

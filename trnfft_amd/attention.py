@@ -135,6 +135,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 
     Returns o (batch, frames, heads, value_dim) in q's dtype, and with return_state the state after each
     sequence's last frame (float32).  States and sums are fp32.  Gradients cannot be differentiated again.
+    A value that is not finite makes NaN (or infinities) of what depends on it by the recurrence: its frame and those after it.
     """
     what = "linear_attention"
     heads = _check_operands(what, q, k, v, log_decay, 4)
