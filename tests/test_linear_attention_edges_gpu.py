@@ -1,5 +1,6 @@
-"""Linear attention where its inputs are at an end: values that are not finite in live frames.  What a value that is not finite reaches is what the recurrence in 64 bits says; all else is
-equal bits to the same call without it."""
+"""Linear attention where its inputs are at an end: values that are not finite in live frames, decays that are NaN.
+What a value that is not finite reaches is what the recurrence in 64 bits says; all else is equal bits to the same call
+without it."""
 
 from __future__ import annotations
 
@@ -78,3 +79,23 @@ def test_values_near_the_largest_stay_in_their_frames(dtype):
     got = trnfft_amd.linear_attention(*(x.cuda() for x in (q, k, v, g)))
     assert torch.equal(got[:, :40], clean[:, :40])
     assert torch.equal(got[..., :3], clean[..., :3]) and torch.equal(got[..., 4:], clean[..., 4:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,d", [(1, 64), (100, 64), (600, 32), (20, 160)])
+def test_a_decay_that_is_nan_shows(dtype, t, d):
+    r = torch.Generator().manual_seed(t)
+    parts = [torch.randn(2, t, 3, d, generator=r).to(dtype) for _ in range(3)]
+    do = torch.randn(2, t, 3, d, generator=r).to(dtype)
+    g = torch.tensor([-0.1, math.nan, -math.inf])
+    got, clean = run(parts, g, do, True), run(parts, torch.tensor([-0.1, -0.2, -math.inf]), do, True)
+    for i, (x, y) in enumerate(zip(got, clean)):
+        axis = {1: 1, 5: 0}.get(i, 2)  # (of the heads)
+        x, y = x.movedim(axis, 0), y.movedim(axis, 0)
+        nan = x[1][:, :-1] if i in (3, 4) else x[1]  # (the last frame's keys and values reach its output undecayed)
+        assert nan.isnan().all()
+        assert torch.equal(x[0], y[0]) and torch.equal(x[2], y[2])
+    state = torch.zeros(2, 3, d, d, device="cuda")
+    o = trnfft_amd.linear_attention_step(*(x[:, 0].cuda() for x in parts), g.cuda(), state)
+    assert o[:, 1].isnan().all() and state[:, 1].isnan().all()
+    assert torch.isfinite(o[:, ::2]).all() and torch.isfinite(state[:, ::2]).all()

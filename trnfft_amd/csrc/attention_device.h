@@ -26,10 +26,10 @@ struct DecaySteps {
     const float near = (float)x;
     below = scalar((double)near <= x ? near : __uint_as_float(__float_as_uint(near) - 1));
     above = scalar((double)near >= x ? near : __uint_as_float(__float_as_uint(near) + 1));
-    // (a gamma in the denormals or zero forgets all it carries: no error to keep account of)
-    const double unit = x > 1e-30 ? 0x1p44 / x : 0.0;
-    err_below = __builtin_amdgcn_readfirstlane((int)(((double)below - x) * unit));
-    err_above = __builtin_amdgcn_readfirstlane((int)(((double)above - x) * unit));
+    // (a gamma in the denormals or zero forgets all it carries: no error to keep account of; nor of NaN)
+    const double unit = 0x1p44 / x;
+    err_below = __builtin_amdgcn_readfirstlane(x > 1e-30 ? (int)(((double)below - x) * unit) : 0);
+    err_above = __builtin_amdgcn_readfirstlane(x > 1e-30 ? (int)(((double)above - x) * unit) : 0);
   }
   __device__ __forceinline__ float next() {
     const bool down = err > 0;
@@ -38,8 +38,9 @@ struct DecaySteps {
   }
 };
 
-// log decays of -inf (no memory) are taken as -1e5: gamma^0 stays 1 and every other power is 0
-__device__ __forceinline__ float log_decay_of(const float* g, int h) { return fmaxf(g[h], -1e5f); }
+// log decays of -inf (no memory) are taken as -1e5: gamma^0 stays 1 and every other power is 0.  (By a comparison that lets NaN through:
+// a decay that has diverged is to be seen.)
+__device__ __forceinline__ float log_decay_of(const float* g, int h) { return g[h] < -1e5f ? -1e5f : g[h]; }
 
 template <typename T>
 __device__ __forceinline__ const T* head_base(const HeadsView& v, long long b, int h) {

@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnPass p) {
       if (k >= p.segments) break;
       p.seg_state[s * all + i] = m;
       const long long tokens = min(max(len - s * p.seg_tokens, 0LL), p.seg_tokens);
-      m = (tokens == p.seg_tokens ? whole : Decay(exp(g * (double)tokens))).times(m) + own[u];
+      if (tokens > 0) m = (tokens == p.seg_tokens ? whole : Decay(exp(g * (double)tokens))).times(m) + own[u];
     }
   }
 }
