@@ -1,4 +1,4 @@
-"""Linear attention where its inputs are at an end: values that are not finite in live frames, decays that are NaN.
+"""Linear attention where its inputs are at an end: values that are not finite in live frames, decays that are NaN, no frames.
 What a value that is not finite reaches is what the recurrence in 64 bits says; all else is equal bits to the same call
 without it."""
 
@@ -99,3 +99,20 @@ def test_a_decay_that_is_nan_shows(dtype, t, d):
     o = trnfft_amd.linear_attention_step(*(x[:, 0].cuda() for x in parts), g.cuda(), state)
     assert o[:, 1].isnan().all() and state[:, 1].isnan().all()
     assert torch.isfinite(o[:, ::2]).all() and torch.isfinite(state[:, ::2]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [(2, 2, 2), (2, 1, 1), (1, 2, 1)])
+def test_gradients_of_no_frames(dtype, heads):
+    # the state goes through: its gradient is the end state's (divided by the scale and multiplied again: three roundings), the
+    # decays' has no lag to count
+    q, k, v = (torch.empty(2, 0, n, d, device="cuda", dtype=dtype, requires_grad=True) for n, d in zip(heads, (8, 8, 16)))
+    g = torch.tensor([-0.1, -0.2], device="cuda", requires_grad=True)
+    s = torch.randn(2, 2, 8, 16, device="cuda", requires_grad=True)
+    ds = torch.randn(2, 2, 8, 16, device="cuda")
+    o, last = trnfft_amd.linear_attention(q, k, v, g, initial_state=s, return_state=True)
+    got = torch.autograd.grad([o, last], [q, k, v, g, s], [torch.empty_like(o), ds])
+    assert all(x.shape == y.shape for x, y in zip(got, (q, k, v, g, s)))
+    assert not got[3].any() and ((got[4] - ds).abs() <= 2.0**-22 * ds.abs()).all()
+    (only,) = torch.autograd.grad(trnfft_amd.linear_attention(q, k, v, g.detach(), initial_state=s, return_state=True)[1], s, ds)
+    assert torch.equal(only, got[4])

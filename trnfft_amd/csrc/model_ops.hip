@@ -350,7 +350,7 @@ int tfa_linear_attention_backward(const tfa_attn_desc* desc, const void* q, cons
     tfa::AttnPass p = pv;
     p.out_f32 = d.v_heads != d.heads;
     p.out = p.out_f32 ? ws + space.dv : grad_v;
-    if (!p.out) return set_error(TFA_ERR_INVALID, "grad_state_in needs grad_v");
+    if (!p.out && rows) return set_error(TFA_ERR_INVALID, "grad_state_in needs grad_v");
     if (const hipError_t e = run_pass(p, plan, grad_states)) return launched(e);
     if (p.out_f32 && grad_v && rows)
       if (const hipError_t e = tfa::launch_attn_head_sum(reinterpret_cast<const float*>(ws + space.dv), grad_v, d.dtype, rows,
