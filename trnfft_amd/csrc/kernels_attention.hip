@@ -335,7 +335,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnStep p, int slices) 
   const T* k = static_cast<const T*>(p.k) + b * p.k_sb + (long long)(h / p.k_group) * p.k_sh;
   const T* v = static_cast<const T*>(p.v) + b * p.v_sb + (long long)(h / p.v_group) * p.v_sh;
   float* S = p.state + bh * p.rows * p.cols;
-  const float gamma = expf(log_decay_of(p.log_decay, h));
+  const Decay gamma(exp((double)log_decay_of(p.log_decay, h)));  // (rounded once more at every frame, it would add up)
   float vv[4], acc[4] = {};
 #pragma unroll
   for (int j = 0; j < 4; ++j) vv[j] = n + j < p.cols ? to_f32(v[n + j]) : 0.0f;
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnStep p, int slices) 
       float* dst = S + (long long)r * p.cols + n;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = __builtin_fmaf(kr[i], vv[j], gamma * s[i][j]);
+        s[i][j] = __builtin_fmaf(kr[i], vv[j], gamma.times(s[i][j]));
         acc[j] = __builtin_fmaf(qr[i], s[i][j], acc[j]);
       }
       if (r < p.rows) {
