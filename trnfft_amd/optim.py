@@ -34,7 +34,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
 
     params: one dtype of float32, bfloat16, float16; grads: one dtype, the parameters' or float32.  exp_avgs and exp_avg_sqs:
     float32, or int8 and uint8 codes with their exp_avg_scales and exp_avg_sq_scales (float32, one for every 256 values).
-    masters: float32 copies that the step is taken on; params then receive them rounded.  step counts from 1.
+    masters: float32 copies that the step is taken on; params then receive them rounded.  step counts from 1; it, lr and the other
+    numbers are those of the call, so a captured call replays the same step, bias correction included.
     A gradient that is not finite makes its 8-bit block NaN, as it makes a float32 state.
     """
     what = "adamw_step"
@@ -95,6 +96,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits: 32, or 8 for states of a quarter of the size (tensors below 4096 values keep 32 bits: they cost nothing, and
     norms and biases are the most sensitive).  master_weights: float32 copies of 16-bit parameters, on which
     the step is taken (without them updates below half a unit in the last place of a 16-bit parameter are lost).
+    The step count and lr live on the host: ``step`` is refused while a graph is captured, whose replays would repeat one step's.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
@@ -125,6 +127,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: step cannot be captured in a graph: its replays would repeat this step's bias correction")
         loss = None
         if closure is not None:
             with torch.enable_grad():
