@@ -350,8 +350,9 @@ int tfa_group_norm_backward(const tfa_norm_desc* desc, const void* x, const void
  *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
  *   p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)
  * in fp32.  states: fp32, or 8-bit codes with one fp32 scale s per 256 values of a tensor: m = s sgn(c) (c / 127)^2 of int8
- * codes, v = s (c / 255)^4 of uint8 codes, s the largest magnitude of the block.  With a master copy (fp32) the step is
- * taken on it and param receives it rounded.  The tables are host memory, read before the call returns.
+ * codes, v = s (c / 255)^4 of uint8 codes, s the largest magnitude of the block, c to nearest and at least 1 where v > 0.
+ * With a master copy (fp32) the step is taken on it and param receives it rounded.  The tables are host memory, read before
+ * the call returns.
  */
 typedef struct tfa_adam_tensor {
   void* param;

@@ -1,10 +1,11 @@
-"""The AdamW step where its callers are at an end: captures."""
+"""The AdamW step where its callers and its 8-bit states are at an end: captures, outliers in a block."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
+import trnfft_amd
 from trnfft_amd.optim import AdamW
 
 pytestmark = pytest.mark.gpu
@@ -31,3 +32,42 @@ def test_the_optimizer_refuses_to_be_captured():
     straight.step()
     straight.step()
     assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("ratio", [1e5, 5e5, 1e6, 1e8])
+@pytest.mark.parametrize("on", [1, 200])
+@pytest.mark.parametrize("stop", [False, True])
+def test_an_outlier_in_a_block_does_not_blow_up_its_neighbours(dtype, ratio, on, stop):
+    # One value's gradients are `ratio` times its neighbours' for `on` steps; the neighbours' stop 20 steps later, or go on.  fp32 states keep
+    # updates of the neighbours within 1.1 lr.  Codes to nearest hold second moments still that grow slowly, worth 11 lr at most
+    # by the same steps in 64 bits with these codes; moments kept beside second moments lost would be worth thousands.
+    n, steps, lr = 512, 600, 1e-3
+    r = torch.Generator().manual_seed(1)
+    p = [torch.zeros(n, device="cuda", dtype=dtype)]
+    mc, vc = [torch.zeros(n, dtype=torch.int8, device="cuda")], [torch.zeros(n, dtype=torch.uint8, device="cuda")]
+    ms, vs = [torch.zeros(2, device="cuda")], [torch.zeros(2, device="cuda")]
+    worst = torch.zeros((), device="cuda")
+    for t in range(steps):
+        g = torch.randn(n, generator=r) * 1e-4
+        if stop and t >= on + 20:
+            g[:] = 0
+        if t < on:
+            g[7] = 1e-4 * ratio
+        p[0].zero_()
+        trnfft_amd.adamw_step(p, [g.to("cuda", dtype)], mc, vc, step=t + 1, lr=lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
+                              exp_avg_scales=ms, exp_avg_sq_scales=vs)
+        p[0][7] = 0
+        worst = torch.maximum(worst, p[0].abs().max().float())
+    assert float(worst) <= 15 * lr
+
+
+def test_second_moments_that_are_not_zero_keep_a_code():
+    g = torch.full((256,), 1e-12, device="cuda")
+    g[0], g[1], g[2] = 1.0, 0.0, 1e-5
+    p = [torch.zeros(256, device="cuda")]
+    mc, vc = [torch.zeros(256, dtype=torch.int8, device="cuda")], [torch.zeros(256, dtype=torch.uint8, device="cuda")]
+    ms, vs = [torch.zeros(1, device="cuda")], [torch.zeros(1, device="cuda")]
+    trnfft_amd.adamw_step(p, [g], mc, vc, step=1, exp_avg_scales=ms, exp_avg_sq_scales=vs)
+    assert vc[0].tolist() == [255, 0, 1] + [1] * 253
+    assert mc[0][:4].tolist() == [127, 0, 0, 0]

@@ -3,10 +3,14 @@
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // States are fp32, or 8-bit codes with one fp32 scale s (the largest magnitude) per block of 256 values:
-//   m = s sgn(c) (c / 127)^2,  v = s (c / 255)^4,   c = round(127 sqrt(|m| / s)),  c = round(255 (v / s)^(1/4)).
+//   m = s sgn(c) (c / 127)^2,  v = s (c / 255)^4,   c = round(127 sqrt(|m| / s)),  c = round(255 (v / s)^(1/4)), 1 at least where v > 0.
 // (c over its top is c times the rounded reciprocal.)  The square law spends the codes where moments are (their logarithm is what varies): a step is 1.6 % of a value at the
-// top of a block and values down to 6e-5 (m) and 2e-10 (v) of it keep a code; v's are the squares of m's in range, so that
-// a value's m rounds to zero before its v does.  A step decodes, updates in fp32 from the decoded values, uses the
+// top of a block and values down to 6e-5 (m) and 2e-10 (v) of it keep a code.  v's are the squares of m's in range, but the two scales
+// fall at different rates (beta1, beta2): behind an outlier a value's m has a code again long before its v would have one, and an update by
+// m over a v of zero is thousands of lr.  So no v is lost: the least one stands for 2e-10 of the block's largest, and smaller ones update by
+// less.  (What codes to nearest still do: v stays where a step changes it by less than half a code, so that a value next to one 1e3 to 1e5 times
+// larger may update by up to 13 lr where fp32 states give 1, until the larger one's share of the scale is forgotten.)
+// A step decodes, updates in fp32 from the decoded values, uses the
 // unrounded m and v for the parameter, and only then encodes.  m, v and the codes are what IEEE fp32 operations in the
 // written order give (no contraction): they do not depend on the compiler.
 // Memory bound: 28 bytes a value with fp32 parameters and states, 16 with 8-bit states.
@@ -78,7 +82,9 @@ __device__ __forceinline__ int code_of_place(float c, float x, float top) {
 __device__ __forceinline__ int root_place(float x, float s, float top, bool fourth) {
   float t = sqrtf(fabsf(x) / s);
   if (fourth) t = sqrtf(t);
-  return code_of_place(s > 0.0f ? rintf(t * top) : 0.0f, x, top);
+  float c = s > 0.0f ? rintf(t * top) : 0.0f;
+  if (fourth && c == 0.0f && x > 0.0f && s < __builtin_inff()) c = 1.0f;
+  return code_of_place(c, x, top);
 }
 // four codes by the definition, a byte each (out of line: seldom run)
 template <bool SQUARES>
@@ -105,7 +111,8 @@ __device__ __forceinline__ unsigned value_codes(const float (&x)[4], float s, fl
     if (SQUARES) t = __builtin_amdgcn_sqrtf(t);
     const float u = t * top;
     least = fminf(least, fabsf(__builtin_amdgcn_fractf(u) - 0.5f));
-    const int c = (int)rintf(u);
+    int c = (int)rintf(u);
+    if (SQUARES) c = max(c, x[j] > 0.0f ? 1 : 0);
     r |= (unsigned)((!SQUARES && x[j] < 0.0f ? -c : c) & 255) << (8 * j);
   }
   if (__any(!(least > kDoubt)) || inv == 0.0f) r = root_places<SQUARES>(x[0], x[1], x[2], x[3], s);
