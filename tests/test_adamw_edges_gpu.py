@@ -71,3 +71,16 @@ def test_second_moments_that_are_not_zero_keep_a_code():
     trnfft_amd.adamw_step(p, [g], mc, vc, step=1, exp_avg_scales=ms, exp_avg_sq_scales=vs)
     assert vc[0].tolist() == [255, 0, 1] + [1] * 253
     assert mc[0][:4].tolist() == [127, 0, 0, 0]
+
+
+def test_a_gradient_that_negates_what_it_reads():
+    # autograd hands the imaginary part of a conjugated tensor on as a view with the negative bit, contiguous where it has one value
+    for bits in (32, 8):
+        w = torch.nn.Parameter(torch.ones(1, device="cuda"))
+        z = torch.complex(torch.ones(1, device="cuda"), w)
+        (z.conj() * torch.tensor([1 + 2j], device="cuda")).abs().sum().backward()
+        assert w.grad.is_neg() and float(w.grad) > 0
+        AdamW([w], lr=0.1, weight_decay=0.0, state_bits=bits).step()
+        assert abs(float(w) - 0.9) < 1e-6
+        with pytest.raises(ValueError, match="negating"):
+            trnfft_amd.adamw_step([w.detach()], [w.grad], [torch.zeros(1, device="cuda")], [torch.zeros(1, device="cuda")], step=1)

@@ -136,3 +136,23 @@ def test_a_long_stream_keeps_the_precision_of_its_state(dtype):
         trnfft_amd.linear_attention_step(qc[i], kc[i], vc[i], gc, state)
     off = (state.double().cpu() - ref).flatten(2).norm(dim=2) / ref.flatten(2).norm(dim=2)
     assert (off <= 4e-6).all(), off
+
+
+def test_views_that_negate_what_they_read():
+    # one value each: contiguous, and still the negative of its memory
+    one = torch.ones(1, 1, 1, 1, device="cuda")
+    minus = torch.complex(one, one).conj().imag
+    assert minus.is_neg() and minus.is_contiguous()
+    g = torch.complex(torch.zeros(1, device="cuda"), torch.ones(1, device="cuda")).conj().imag
+    o, last = trnfft_amd.linear_attention(one, one, one, g, initial_state=minus, return_state=True)
+    expect = 1.0 - math.exp(-1.0)
+    assert abs(float(o) - expect) < 1e-6 and abs(float(last) - expect) < 1e-6
+    assert abs(float(trnfft_amd.linear_attention_step(one[0], minus[0], one[0], g, one.clone())) - (math.exp(-1.0) - 1.0)) < 1e-6
+    with pytest.raises(ValueError):
+        trnfft_amd.linear_attention_step(one[0], one[0], one[0], g, minus)
+    leaves = [x.clone().requires_grad_() for x in (one, one, one, one)]
+    out = trnfft_amd.linear_attention(*leaves[:3], g, initial_state=leaves[3], return_state=True)
+    grads = torch.autograd.grad(out, leaves, [minus, minus])
+    # d(o + last) with o = q (v k + gamma s), last = v k + gamma s, all ones, times -1
+    for x, expect in zip(grads, (-1.0 - math.exp(-1.0), -2.0, -2.0, -2.0 * math.exp(-1.0))):
+        assert abs(float(x) - expect) < 1e-6

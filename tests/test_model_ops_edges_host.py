@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from trnfft_amd import _lib
 from trnfft_amd.optim import AdamW
 
 
@@ -17,3 +18,10 @@ def test_the_optimizer_refuses_to_be_captured(monkeypatch):
     with pytest.raises(RuntimeError, match="captured"):
         opt.step()
     assert not opt.state[p]
+
+
+def test_lists_of_tensors_hold_no_negating_views():
+    minus = torch.complex(torch.ones(1), torch.ones(1)).conj().imag
+    assert minus.is_neg() and minus.is_contiguous()
+    with pytest.raises(ValueError, match="negating"):
+        _lib.tensor_table()("op", ("states",), ([minus],), (torch.float32,), 0)

@@ -55,6 +55,8 @@ def _scale(scale, key_dim: int, what: str) -> float:
 
 
 def _on(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """x on dev, as its memory says it (the imaginary part of a conjugated tensor is a view that negates what it reads)."""
+    x = x.resolve_neg() if x.is_neg() else x
     return x if x.device == dev else x.to(dev)
 
 
@@ -107,8 +109,8 @@ class _LinearAttentionFn(torch.autograd.Function):
         desc = _desc(q, k, v, heads, ctx.scale)
         if g_out is None:
             g_out = q.new_zeros(*q.shape[:2], heads, v.shape[3])
-        g_out = _rows(g_out.contiguous(), dev)
-        g_last = None if g_last is None else g_last.contiguous()
+        g_out = _rows(_on(g_out, dev).contiguous(), dev)
+        g_last = None if g_last is None else _on(g_last, dev).contiguous()
         # (the decays' gradient comes with the queries' and keys', the state's with the values')
         d_q = torch.empty(q.shape, dtype=q.dtype, device=dev) if need[0] or need[3] else None
         d_k = torch.empty(k.shape, dtype=q.dtype, device=dev) if need[1] or need[3] else None
@@ -186,7 +188,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
                                     or state.requires_grad):
         raise RuntimeError(f"{what}: no gradients; use linear_attention, or torch.no_grad()")
     _require_hip(what)
-    if not state.is_cuda or not state.is_contiguous():
+    if not state.is_cuda or not state.is_contiguous() or state.is_neg():
         raise ValueError(f"{what}: the state is updated in place and must be contiguous on the GPU")
     dev, out_dev = state.device, q.device
     q, k, v, log_decay = _rows(q, dev), _rows(k, dev), _rows(v, dev), _on(log_decay, dev).contiguous()

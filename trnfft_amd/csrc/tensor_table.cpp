@@ -17,8 +17,8 @@ constexpr int64_t kBlock = 256;  // values that share a scale
 
 const char kDoc[] =
     "table(what, names, lists, dtypes, device) -> bytes: rows of 64-bit words, one for each tensor of lists[0]: the address\n"
-    "of its entry in each list (0 where a list is None), then its size.  Tensors must be contiguous, on the GPU of that index\n"
-    "and of the list's dtype, with as many values as lists[0]'s (a name that ends in 'scales': one for every 256).";
+    "of its entry in each list (0 where a list is None), then its size.  Tensors must be contiguous, no negating views, on the GPU of that\n"
+    "index and of the list's dtype, with as many values as lists[0]'s (a name that ends in 'scales': one for every 256).";
 
 // An error of list `name` (a new Python exception of the given type).
 PyObject* refuse(PyObject* type, PyObject* what, PyObject* name, const char* text) {
@@ -80,6 +80,7 @@ PyObject* table_of(PyObject* args) {
         PyErr_Format(PyExc_TypeError, "%U: %U must be %S, got %S", what, name, dtype, reinterpret_cast<PyObject*>(torch::getTHPDtype(t.scalar_type())));
         return nullptr;
       }
+      if (t.is_neg()) return refuse(PyExc_ValueError, what, name, "must not be negating views (resolve_neg)");
       if (!t.is_cuda() || t.get_device() != device) return refuse(PyExc_ValueError, what, name, "must be on the GPU of the first");
       if (t.layout() != at::kStrided || !t.is_contiguous()) return refuse(PyExc_ValueError, what, name, "must be contiguous");
       const int64_t n = t.numel();

@@ -57,7 +57,7 @@ class _GroupNormFn(torch.autograd.Function):
     def backward(ctx, g):
         x, weight, bias, lengths, stats = ctx.saved_tensors
         what, dev, desc, need = "group_norm backward", x.device, ctx.desc, ctx.needs_input_grad
-        g = _whole(g.contiguous())
+        g = _whole(_on(g, dev).contiguous())
         dx = torch.empty_like(x)
         fresh = torch.empty_like if x.numel() else torch.zeros_like  # (of no data there is no launch)
         dw = fresh(weight) if weight is not None and need[1] else None
@@ -104,9 +104,8 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
     _require_hip(what)
     dev, out_dev = target_device(x), x.device
     x = _whole(_on(x, dev).contiguous())
-    weight, bias = (w if w is None or (w.dtype == torch.float32 and w.device == dev) else w.to(dev, torch.float32)
-                    for w in (weight, bias))
-    weight, bias = (None if w is None else w.contiguous() for w in (weight, bias))
+    weight, bias = (w if w is None or w.dtype == torch.float32 else w.to(dev, torch.float32) for w in (weight, bias))
+    weight, bias = (None if w is None else _on(w, dev).contiguous() for w in (weight, bias))
     lengths = None if lengths is None else lengths.to(dev, torch.int64).contiguous()
     positions = math.prod(x.shape[1:-1])
     inner = max(1, math.prod(x.shape[2:-1])) if x.dim() > 2 else 1

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .attention import DTYPES
+from .attention import DTYPES, _on
 from .dispatch import _require_hip, launch
 
 BLOCK = 256  # values that share a scale
@@ -144,7 +144,7 @@ class AdamW(torch.optim.Optimizer):
                 state = self._state_of(p, group)
                 state["step"] += 1
                 key = (p.dtype, p.grad.dtype, p.device, state["step"], "exp_avg_scale" in state, "master" in state)
-                calls.setdefault(key, []).append((p, p.grad.contiguous(), state))
+                calls.setdefault(key, []).append((p, _on(p.grad, p.device).contiguous(), state))
             for (_, _, _, step, eight, master), items in calls.items():
                 states = [s for _, _, s in items]
                 adamw_step([p for p, _, _ in items], [g for _, g, _ in items], [s["exp_avg"] for s in states],
