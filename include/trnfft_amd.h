@@ -285,9 +285,9 @@ int tfa_column_sums(int64_t rows, int64_t cols, const float* re, const float* im
  *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   out_t = scale S_t^T q_t
  * q, k (key_dim features) and v (value_dim) may have fewer heads than the call: head h reads head h / (heads / own).
  * Their strides are in elements, for batch, token and head; features are contiguous and q, k, v, grad_out 16-byte aligned
- * (operands whose features or strides are not multiples of 16 bytes are copied to the workspace first).  State tensors are fp32 (batch,
- * heads, key_dim, value_dim), the outputs contiguous (batch, tokens, heads, value_dim).  log_decay: (heads) device fp32, at most 0
- * (-inf: no memory; above 0 the state grows).  lengths: (batch) device int64 or NULL; tokens at and past a sequence's
+ * (a step's operands may lie anywhere; operands whose features or strides are not multiples of 16 bytes are copied to the
+ * workspace first).  State tensors are fp32 (batch, heads, key_dim, value_dim), the outputs contiguous (batch, tokens,
+ * heads, value_dim).  log_decay: (heads) device fp32, at most 0 (-inf: no memory; above 0 the state grows).  lengths: (batch) device int64 or NULL; tokens at and past a sequence's
  * length are padding: never read, zero in the outputs and gradients, and the state is the one at the length.  Products of
  * bf16 operands are exact, scores, states and sums are fp32 for every type.  Head dimensions up to 256.
  */

@@ -156,3 +156,19 @@ def test_views_that_negate_what_they_read():
     # d(o + last) with o = q (v k + gamma s), last = v k + gamma s, all ones, times -1
     for x, expect in zip(grads, (-1.0 - math.exp(-1.0), -2.0, -2.0, -2.0 * math.exp(-1.0))):
         assert abs(float(x) - expect) < 1e-6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_step_takes_its_operands_where_they_lie(dtype):
+    # three heads of 20 features in a row of a projection, at odd addresses: no copies, the output is all that is allocated
+    r = torch.Generator().manual_seed(0)
+    packed = torch.randn(2, 1 + 3 * 3 * 20, generator=r).to(dtype)
+    g, s = torch.tensor([-0.1, -0.2, -0.3]), torch.randn(2, 3, 20, 20, generator=r)
+    q, k, v = (x.unflatten(-1, (3, 20)) for x in packed.cuda()[:, 1:].split(60, dim=-1))
+    assert all(x.data_ptr() % 16 for x in (q, k, v))
+    gc, state, dense = g.cuda(), s.cuda(), s.cuda()
+    expected = trnfft_amd.linear_attention_step(q.contiguous(), k.contiguous(), v.contiguous(), gc, dense)
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    o = trnfft_amd.linear_attention_step(q, k, v, gc, state)
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before + 1
+    assert torch.equal(o, expected) and torch.equal(state, dense)

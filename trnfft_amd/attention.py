@@ -60,11 +60,15 @@ def _on(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
     return x if x.device == dev else x.to(dev)
 
 
-def _rows(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    """x on dev with contiguous features at a 16-byte boundary (x itself where it is so)."""
+def _features(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """x on dev with contiguous features (x itself where it is so)."""
     x = _on(x, dev)
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
-        x = x.contiguous()
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def _rows(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """The same at a 16-byte boundary."""
+    x = _features(x, dev)
     return x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
@@ -191,7 +195,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     if not state.is_cuda or not state.is_contiguous() or state.is_neg():
         raise ValueError(f"{what}: the state is updated in place and must be contiguous on the GPU")
     dev, out_dev = state.device, q.device
-    q, k, v, log_decay = _rows(q, dev), _rows(k, dev), _rows(v, dev), _on(log_decay, dev).contiguous()
+    q, k, v, log_decay = _features(q, dev), _features(k, dev), _features(v, dev), _on(log_decay, dev).contiguous()
     (qb, qs, _), (kb, ks, _), (vb, vs, _) = q.stride(), k.stride(), v.stride()
     desc = _lib.AttnDesc(DTYPES[q.dtype], heads, qh, kh, vh, dk, dv, scale, b, 1, qb, 0, qs, kb, 0, ks, vb, 0, vs)
     out = q.new_empty(b, heads, dv)
