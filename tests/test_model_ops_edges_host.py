@@ -4,7 +4,9 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
+import trnfft_amd
 from trnfft_amd import _lib
 from trnfft_amd.optim import AdamW
 
@@ -25,3 +27,18 @@ def test_lists_of_tensors_hold_no_negating_views():
     assert minus.is_neg() and minus.is_contiguous()
     with pytest.raises(ValueError, match="negating"):
         _lib.tensor_table()("op", ("states",), ([minus],), (torch.float32,), 0)
+
+
+def test_forward_mode_tangents_are_not_dropped():
+    q, g, s, x, w = (torch.zeros(n) for n in ((1, 4, 2, 8), (2,), (1, 2, 8, 8), (2, 5, 4), (4,)))
+    with forward_ad.dual_level():
+        for i in range(5):
+            a = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate((q, q, q, g, s))]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                trnfft_amd.linear_attention(*a[:4], initial_state=a[4])
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                trnfft_amd.linear_attention_step(*(t[:, 0] for t in a[:3]), a[3], a[4])
+        for i in range(3):
+            a = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate((x, w, w))]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                trnfft_amd.group_norm(a[0], 2, a[1], a[2])

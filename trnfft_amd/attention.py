@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .dispatch import _require_hip, addr, launch, target_device
+from .dispatch import _require_hip, addr, launch, refuse_tangents, target_device
 
 DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
@@ -140,7 +140,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     numbers; frames at and past a sequence's length are padding, whatever they hold: outputs and gradients are zero there.
 
     Returns o (batch, frames, heads, value_dim) in q's dtype, and with return_state the state after each
-    sequence's last frame (float32).  States and sums are fp32.  Gradients cannot be differentiated again.
+    sequence's last frame (float32).  States and sums are fp32.  Gradients cannot be differentiated again, and there is no
+    forward mode.
     A value that is not finite makes NaN (or infinities) of what depends on it by the recurrence: its frame and those after it.
     """
     what = "linear_attention"
@@ -158,6 +159,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
             raise ValueError(f"{what}: lengths must be ({b},), got {tuple(lengths.shape)}")
         if lengths.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8):
             raise TypeError(f"{what}: lengths must be whole numbers, got {lengths.dtype}")
+    refuse_tangents(what, q, k, v, log_decay, initial_state)
     _require_hip(what)
     dev, out_dev = target_device(q, k, v), q.device
     q, k, v = _rows(q, dev), _rows(k, dev), _rows(v, dev)
@@ -191,6 +193,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or state.requires_grad):
         raise RuntimeError(f"{what}: no gradients; use linear_attention, or torch.no_grad()")
+    refuse_tangents(what, q, k, v, log_decay, state)
     _require_hip(what)
     if not state.is_cuda or not state.is_contiguous() or state.is_neg():
         raise ValueError(f"{what}: the state is updated in place and must be contiguous on the GPU")

@@ -18,6 +18,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .complex import ComplexTensor
@@ -104,6 +105,14 @@ def _require_hip(what: str) -> None:
             "visible gfx950 GPU); no CPU fallback exists in this package"
         )
     _lib.lib()
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raises where an input carries a forward-mode tangent, which a call that knows none would drop."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
 
 
 def target_device(*tensors: torch.Tensor) -> torch.device:

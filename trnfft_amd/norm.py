@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .attention import DTYPES, _on
-from .dispatch import _require_hip, addr, launch, target_device
+from .dispatch import _require_hip, addr, launch, refuse_tangents, target_device
 
 ACTIVATIONS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU, "relu": _lib.ACT_RELU}
 
@@ -75,7 +75,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
     Statistics are those of a sample's group of channels / num_groups channels over all positions.  x: float32, bfloat16 or
     float16; weight and bias (channels,) in float32 or x's dtype; activation: None, "silu", "gelu" (by the error function)
     or "relu".  lengths: (batch,) whole numbers, the positions along axis 1 that are no padding: padding is not read, takes
-    no part in the statistics and is zero in the result.  Gradients cannot be differentiated again.
+    no part in the statistics and is zero in the result.  Gradients cannot be differentiated again, and there is no forward mode.
     """
     what = "group_norm"
     if x.dtype not in DTYPES:
@@ -101,6 +101,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
             raise ValueError(f"{what}: lengths must be ({batch},) for (batch, positions, ..., channels) data")
         if lengths.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8):
             raise TypeError(f"{what}: lengths must be whole numbers, got {lengths.dtype}")
+    refuse_tangents(what, x, weight, bias)
     _require_hip(what)
     dev, out_dev = target_device(x), x.device
     x = _whole(_on(x, dev).contiguous())
