@@ -42,3 +42,20 @@ def test_forward_mode_tangents_are_not_dropped():
             a = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate((x, w, w))]
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 trnfft_amd.group_norm(a[0], 2, a[1], a[2])
+
+
+def test_the_c_library_is_built_where_the_table_cannot_be(monkeypatch, tmp_path):
+    from trnfft_amd.csrc import build
+
+    linked = []
+
+    def no_headers():
+        raise RuntimeError("Python.h: No such file or directory")
+
+    monkeypatch.setattr(build, "HERE", str(tmp_path))
+    monkeypatch.setattr(build, "_build_table", no_headers)
+    monkeypatch.setattr(build, "_compile", lambda src, obj: None)
+    monkeypatch.setattr(build, "_link", lambda objs, out: linked.append(out))
+    with pytest.raises(RuntimeError, match="Python.h"):
+        build.build()
+    assert linked == [build.LIB, build.COPY_LIB]

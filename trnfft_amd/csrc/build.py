@@ -110,9 +110,10 @@ def build(verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 1)) as ex:
         table = ex.submit(_build_table)
         list(ex.map(lambda so: _compile(*so), zip(srcs, objs)))
-        table.result()
+    # (the C ABI needs neither torch's headers nor Python's: it is there also where the table fails)
     _link(objs[:-1], LIB)
     _link(objs[-1:], COPY_LIB)
+    table.result()
     if verbose:
         print(f"built {LIB}, {COPY_LIB} and {TABLE_LIB}")
     return LIB
