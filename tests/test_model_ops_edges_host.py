@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -59,3 +61,17 @@ def test_the_c_library_is_built_where_the_table_cannot_be(monkeypatch, tmp_path)
     with pytest.raises(RuntimeError, match="Python.h"):
         build.build()
     assert linked == [build.LIB, build.COPY_LIB]
+
+
+@pytest.mark.parametrize("tokens,states", [(1, 0), (64, 0), (256, 0), (512, 1), (1024, 3)])
+def test_the_decays_gradient_keeps_states_between_tokens_alone(tokens, states):
+    # (many short sequences: a state for each, 64 KB of no use, was more than the card holds)
+    batch, heads, dim = 40064, 16, 128
+    desc = _lib.AttnDesc(_lib.DTYPE_BF16, heads, heads, heads, heads, dim, dim, 1.0, batch, tokens,
+                         *((tokens * heads * dim, heads * dim, dim) * 3))
+    size = {}
+    for kind in (1, 2):
+        out = ctypes.c_size_t()
+        assert _lib.lib().tfa_linear_attention_workspace_size(desc, kind, out) == _lib.TFA_OK
+        size[kind] = out.value
+    assert size[2] - size[1] == states * batch * heads * dim * dim * 4

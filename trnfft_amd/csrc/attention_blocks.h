@@ -395,7 +395,7 @@ __global__ __launch_bounds__(64 * NW, NW == 2 && RP == 128 ? 1 : 2) void attn_bl
     if (i + 1 < total) fetch(i + 1, set);
 
     const bool at_border = LAGS && c0 > 0 && (c0 & (p.stretch - 1)) == 0;
-    float* const held = LAGS && at_border ? border + (size_t)(c0 >> p.log_stretch) * (RB * 16 * B::threads) : nullptr;
+    float* const held = LAGS && at_border ? border + (size_t)((c0 >> p.log_stretch) - 1) * (RB * 16 * B::threads) : nullptr;
     if constexpr (LAGS)
       if (at_border && !reverse)
 #pragma unroll

@@ -70,7 +70,7 @@ struct AttnPass {
   long long seg_tokens;
   float* seg_state;
   // In blocks, with dg_part: the forward pass of the query gradient leaves the states at every `stretch` tokens (a divisor of
-  // seg_tokens), `borders` of them for each (batch, head), for the reversed pass of the key gradient
+  // seg_tokens) but the first, `borders` of them for each (batch, head), for the reversed pass of the key gradient
   float* border_state;
   long long borders;
   int stretch, log_stretch;  // a power of two

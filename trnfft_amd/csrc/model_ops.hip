@@ -179,7 +179,7 @@ BackwardSpace backward_space(const tfa_attn_desc* d, bool decays) {
   if (decays && s.plan.blocks) {
     s.stretch = kStretch;
     while (s.plan.seg_tokens % s.stretch) s.stretch /= 2;
-    s.borders = (d->tokens + s.stretch - 1) / s.stretch;
+    s.borders = (d->tokens - 1) / s.stretch;
     s.border = s.total;
     s.total += align256((size_t)d->batch * d->heads * s.borders * tfa::attn_border_bytes(p.rows, p.cols));
   }
