@@ -84,3 +84,18 @@ def test_a_gradient_that_negates_what_it_reads():
         assert abs(float(w) - 0.9) < 1e-6
         with pytest.raises(ValueError, match="negating"):
             trnfft_amd.adamw_step([w.detach()], [w.grad], [torch.zeros(1, device="cuda")], [torch.zeros(1, device="cuda")], step=1)
+
+
+def test_lists_that_can_be_read_once():
+    n = 600
+    p, g = torch.ones(n, device="cuda", dtype=torch.bfloat16), torch.ones(n, device="cuda")
+    mc, vc = torch.zeros(n, dtype=torch.int8, device="cuda"), torch.zeros(n, dtype=torch.uint8, device="cuda")
+    ms, vs = torch.zeros(3, device="cuda"), torch.zeros(3, device="cuda")
+    master, values = p.float(), torch.zeros(n, device="cuda")
+    versions = master._version, values._version
+    trnfft_amd.adamw_step(*(iter([t]) for t in (p, g, mc, vc)), step=1, exp_avg_scales=iter([ms]), exp_avg_sq_scales=iter([vs]),
+                          masters=iter([master]))
+    out = trnfft_amd.adamw_state_values(iter([mc]), iter([ms]), iter([values]))
+    assert (master != 1).all() and torch.equal(p, master.to(p.dtype))
+    assert len(out) == 1 and out[0] is values and (values != 0).all()
+    assert master._version > versions[0] and values._version > versions[1]

@@ -39,7 +39,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
     A gradient that is not finite makes its 8-bit block NaN, as it makes a float32 state.
     """
     what = "adamw_step"
-    params, grads = list(params), list(grads)
+    params, grads, masters = list(params), list(grads), _listed(masters)
     if not params:
         return
     eight = exp_avg_scales is not None
@@ -57,7 +57,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
         raise ValueError(f"{what}: the parameters are updated in place and must be on the GPU")
     moments = (torch.int8, torch.uint8) if eight else (torch.float32, torch.float32)
     table = _lib.tensor_table()(what, _ADAM_LISTS,
-                                (params, grads, *map(_listed, (exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, masters))),
+                                (params, grads, *map(_listed, (exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales)), masters),
                                 (p_dtype, g_dtype, *moments, torch.float32, torch.float32, torch.float32), dev.index)
     desc = _lib.AdamDesc(DTYPES[p_dtype], DTYPES[g_dtype], 8 if eight else 32, 0, int(step), lr, betas[0], betas[1], eps,
                          weight_decay)
@@ -65,7 +65,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1
     # (autograd sees the update as it sees any in-place operation)
     torch.autograd.graph.increment_version(params)
     if masters is not None:
-        torch.autograd.graph.increment_version(list(masters))
+        torch.autograd.graph.increment_version(masters)
 
 
 @torch.no_grad()
@@ -81,9 +81,8 @@ def adamw_state_values(codes, scales, out=None) -> list[torch.Tensor]:
     _require_hip(what)
     if dev.type != "cuda":
         raise ValueError(f"{what}: the states must be on the GPU")
-    if out is None:
-        out = [torch.empty(c.shape, dtype=torch.float32, device=dev) for c in codes]
-    table = _lib.tensor_table()(what, ("codes", "scales", "out"), (codes, _listed(scales), _listed(out)),
+    out = [torch.empty(c.shape, dtype=torch.float32, device=dev) for c in codes] if out is None else _listed(out)
+    table = _lib.tensor_table()(what, ("codes", "scales", "out"), (codes, _listed(scales), out),
                                 (dtype, torch.float32, torch.float32), dev.index)
     launch(what, dev, _lib.lib().tfa_adamw_state_values, len(codes), table, int(dtype == torch.uint8))
     torch.autograd.graph.increment_version(out)
