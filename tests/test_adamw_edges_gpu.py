@@ -99,3 +99,33 @@ def test_lists_that_can_be_read_once():
     assert (master != 1).all() and torch.equal(p, master.to(p.dtype))
     assert len(out) == 1 and out[0] is values and (values != 0).all()
     assert master._version > versions[0] and values._version > versions[1]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_parameters_written_between_steps_keep_what_was_written(dtype):
+    # as with torch's optimizer, which has no masters: weights that are loaded or clamped are where the next step starts
+    torch.manual_seed(0)
+    p = torch.nn.Parameter(torch.randn(300, device="cuda").to(dtype))
+    opt = AdamW([p], lr=1e-3, weight_decay=0.0)
+    r = torch.Generator().manual_seed(0)
+    for _ in range(3):
+        p.grad = torch.randn(300, generator=r).to("cuda", dtype)
+        opt.step()
+    kept, before = opt.state[p]["master"][100:].clone(), p.detach().clone()
+    with torch.no_grad():
+        p[:100] = 7.0
+    p.grad = torch.zeros(300, device="cuda", dtype=dtype)
+    opt.step()
+    # (a zero gradient moves by the momentum alone: 3 lr at most)
+    assert ((p[:100].float() - 7.0).abs() <= 7.0 * 2.0**-8).all()
+    assert ((opt.state[p]["master"][:100] - 7.0).abs() <= 3e-3).all()
+    assert ((opt.state[p]["master"][100:] - kept).abs() <= 3e-3).all() and (kept != before[100:].float()).any()
+    # and what a checkpoint brings back is its own
+    saved, weights = opt.state_dict(), p.detach().clone()
+    again = torch.nn.Parameter(weights)
+    other = AdamW([again], lr=1e-3, weight_decay=0.0)
+    other.load_state_dict(saved)
+    for q, o in ((p, opt), (again, other)):
+        q.grad = torch.ones(300, device="cuda", dtype=dtype)
+        o.step()
+    assert torch.equal(opt.state[p]["master"], other.state[again]["master"]) and torch.equal(p, again)

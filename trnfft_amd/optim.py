@@ -94,9 +94,12 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits: 32, or 8 for states of a quarter of the size (tensors below 4096 values keep 32 bits: they cost nothing, and
     norms and biases are the most sensitive).  Values whose gradients are 1e3 to 1e5 times smaller than others of their 256 may
-    update several times faster with 8 bits (up to 13 lr for 1), still smaller ones slower.  master_weights: float32 copies of 16-bit parameters, on which
-    the step is taken (without them updates below half a unit in the last place of a 16-bit parameter are lost).
-    The step count and lr live on the host: ``step`` is refused while a graph is captured, whose replays would repeat one step's.
+    update several times faster with 8 bits (up to 13 lr for 1), still smaller ones slower.
+    master_weights: float32 copies of 16-bit parameters, on which the step is taken (without them updates below half a unit in
+    the last place of a 16-bit parameter are lost).  A parameter that was written between two steps (weights loaded, clamped)
+    takes its master along; writes through ``.data`` are not seen.
+    Parameters must be contiguous.  The step count and lr live on the host: ``step`` is refused while a graph is captured,
+    whose replays would repeat one step's.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
@@ -123,6 +126,10 @@ class AdamW(torch.optim.Optimizer):
                 state["exp_avg_sq_scale"] = torch.zeros(_blocks(p.numel()), **flat)
             if p.dtype != torch.float32 and group["master_weights"]:
                 state["master"] = p.detach().float().contiguous()
+        elif "master" in state and state.get("seen") != p._version:
+            # written since the last step (weights that were loaded, clamped, averaged): those values hold, others keep their master
+            master = state["master"]
+            master.copy_(torch.where(master.to(p.dtype) == p, master, p.float()))
         return state
 
     @torch.no_grad()
@@ -152,6 +159,9 @@ class AdamW(torch.optim.Optimizer):
                            exp_avg_scales=[s["exp_avg_scale"] for s in states] if eight else None,
                            exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states] if eight else None,
                            masters=[s["master"] for s in states] if master else None)
+                if master:
+                    for p, _, s in items:
+                        s["seen"] = p._version
         return loss
 
     def load_state_dict(self, state_dict):
@@ -162,3 +172,5 @@ class AdamW(torch.optim.Optimizer):
                 for name, value in state_dict["state"].get(index, {}).items():
                     if torch.is_tensor(value):
                         self.state[p][name] = value.to(p.device).clone()
+                if p in self.state:
+                    self.state[p].pop("seen", None)
