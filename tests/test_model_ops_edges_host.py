@@ -75,3 +75,14 @@ def test_the_decays_gradient_keeps_states_between_tokens_alone(tokens, states):
         assert _lib.lib().tfa_linear_attention_workspace_size(desc, kind, out) == _lib.TFA_OK
         size[kind] = out.value
     assert size[2] - size[1] == states * batch * heads * dim * dim * 4
+
+
+@pytest.mark.parametrize("bad", [dict(state_bits=4), dict(betas=(1.0, 0.9)), dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-1.0)])
+def test_a_group_of_parameters_with_options_of_its_own_is_checked(bad):
+    p, q = (torch.nn.Parameter(torch.zeros(3)) for _ in range(2))
+    with pytest.raises(ValueError):
+        AdamW([{"params": [p], **bad}])
+    opt = AdamW([{"params": [p], "state_bits": 8, "lr": 0.5}])
+    assert opt.param_groups[0]["state_bits"] == 8 and opt.param_groups[0]["lr"] == 0.5
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [q], **bad})

@@ -104,14 +104,19 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  state_bits: int = 32, master_weights: bool = True):
-        if state_bits not in (32, 8):
-            raise ValueError(f"AdamW: state_bits must be 32 or 8, got {state_bits}")
-        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
-            raise ValueError(f"AdamW: betas must be in [0, 1), got {betas}")
-        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
-            raise ValueError("AdamW: lr, eps and weight_decay must not be negative")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights))
+
+    def add_param_group(self, param_group):
+        own = {**self.defaults, **param_group}
+        betas = own["betas"]
+        if own["state_bits"] not in (32, 8):
+            raise ValueError(f"AdamW: state_bits must be 32 or 8, got {own['state_bits']}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"AdamW: betas must be in [0, 1), got {betas}")
+        if own["lr"] < 0.0 or own["eps"] < 0.0 or own["weight_decay"] < 0.0:
+            raise ValueError("AdamW: lr, eps and weight_decay must not be negative")
+        super().add_param_group(param_group)
 
     def _state_of(self, p: torch.Tensor, group: dict) -> dict:
         state = self.state[p]
