@@ -86,3 +86,14 @@ def test_a_group_of_parameters_with_options_of_its_own_is_checked(bad):
     assert opt.param_groups[0]["state_bits"] == 8 and opt.param_groups[0]["lr"] == 0.5
     with pytest.raises(ValueError):
         opt.add_param_group({"params": [q], **bad})
+
+
+def test_a_refused_step_does_not_count():
+    # (on the CPU: there is no GPU, or the parameters are not on it; not contiguous anywhere)
+    p = torch.nn.Parameter(torch.zeros(4, 6).t())
+    p.grad = torch.ones(6, 4)
+    opt = AdamW([p])
+    for _ in range(2):
+        with pytest.raises((RuntimeError, ValueError)):
+            opt.step()
+    assert opt.state[p]["step"] == 0

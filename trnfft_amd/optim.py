@@ -153,8 +153,7 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise RuntimeError("AdamW: sparse gradients are not supported")
                 state = self._state_of(p, group)
-                state["step"] += 1
-                key = (p.dtype, p.grad.dtype, p.device, state["step"], "exp_avg_scale" in state, "master" in state)
+                key = (p.dtype, p.grad.dtype, p.device, state["step"] + 1, "exp_avg_scale" in state, "master" in state)
                 calls.setdefault(key, []).append((p, _on(p.grad, p.device).contiguous(), state))
             for (_, _, _, step, eight, master), items in calls.items():
                 states = [s for _, _, s in items]
@@ -164,8 +163,9 @@ class AdamW(torch.optim.Optimizer):
                            exp_avg_scales=[s["exp_avg_scale"] for s in states] if eight else None,
                            exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states] if eight else None,
                            masters=[s["master"] for s in states] if master else None)
-                if master:
-                    for p, _, s in items:
+                for p, _, s in items:
+                    s["step"] = step
+                    if master:
                         s["seen"] = p._version
         return loss
 
