@@ -24,6 +24,10 @@ def _whole(x: torch.Tensor) -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
+def _channels(w: torch.Tensor | None, dev: torch.device) -> torch.Tensor | None:
+    return None if w is None else _on(w if w.dtype == torch.float32 else w.float(), dev).contiguous()
+
+
 def _workspace(desc: _lib.NormDesc, backward: int, dev: torch.device, what: str) -> torch.Tensor | None:
     nbytes = ctypes.c_size_t()
     _lib.check(_lib.lib().tfa_group_norm_workspace_size(desc, backward, nbytes), what)
@@ -105,8 +109,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
     _require_hip(what)
     dev, out_dev = target_device(x), x.device
     x = _whole(_on(x, dev).contiguous())
-    weight, bias = (w if w is None or w.dtype == torch.float32 else w.to(dev, torch.float32) for w in (weight, bias))
-    weight, bias = (None if w is None else _on(w, dev).contiguous() for w in (weight, bias))
+    weight, bias = _channels(weight, dev), _channels(bias, dev)
     lengths = None if lengths is None else lengths.to(dev, torch.int64).contiguous()
     positions = math.prod(x.shape[1:-1])
     inner = max(1, math.prod(x.shape[2:-1])) if x.dim() > 2 else 1
