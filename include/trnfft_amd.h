@@ -287,9 +287,11 @@ int tfa_column_sums(int64_t rows, int64_t cols, const float* re, const float* im
  * Their strides are in elements, for batch, token and head; features are contiguous and q, k, v, grad_out 16-byte aligned
  * (a step's operands may lie anywhere; operands whose features or strides are not multiples of 16 bytes are copied to the
  * workspace first).  State tensors are fp32 (batch, heads, key_dim, value_dim), the outputs contiguous (batch, tokens,
- * heads, value_dim).  log_decay: (heads) device fp32, at most 0 (-inf: no memory; above 0 the state grows).  lengths: (batch) device int64 or NULL; tokens at and past a sequence's
- * length are padding: never read, zero in the outputs and gradients, and the state is the one at the length.  Products of
- * bf16 operands are exact, scores, states and sums are fp32 for every type.  Head dimensions up to 256.
+ * heads, value_dim).  log_decay: (heads) device fp32, at most 0 (-inf: no memory; above 0 the state grows).  lengths: (batch)
+ * device int64 or NULL; tokens at and past a sequence's length are padding: never read, zero in the outputs and gradients,
+ * and the state is the one at the length.  Products of bf16 operands are exact; scores, states and sums are held in fp32
+ * for every type, and up to 128 features enter the products of 16-bit outputs with 16 to 17 bits.  What is not finite makes
+ * NaN or infinities of what depends on it by the recurrence: its token and later ones.  Head dimensions up to 256.
  */
 typedef struct tfa_attn_desc {
   int32_t dtype; /* TFA_DTYPE_* of q, k, v, out and their gradients */

@@ -29,17 +29,19 @@
 // LDS read (ds_read_b64_tr_b16: 16 lanes take 4 tokens x 16 features, each receives one feature's 4 tokens).  The next block
 // is on its way in registers while one is computed.
 //
-// What it measures: 32 x 1024 tokens of 16 bf16 heads of 128 forward 157 us (3.4 TB/s of operands and results; at the copy's rate
-// 104), of 64 96 us (52); fp16 221 us, fp32 (3.1 TB/s) 342 us.  A training pass of 8 x 4096 tokens of 16 heads of 128: 1.05 ms, 2.1 in
-// fp32.  What bounds it: a block's chain of dependent steps (stage, scores, decays and pieces, outputs, state) with two waves a SIMD,
-// as the state leaves registers for no more: the matrix units are 30 to 44 % busy, vector units and memory less than that.
+// What it measures: 32 x 1024 tokens of 16 bf16 heads of 128 forward 181 us (3.0 TB/s of operands and results; at the copy's rate
+// 104), of 64 98 us (52); fp16 230 us, fp32 (3.1 TB/s) 345 us.  A training pass of 8 x 4096 tokens of 16 heads of 128: 1.09 ms, 1.4 in
+// fp16, 2.1 in fp32.  What bounds it: a block's chain of dependent steps (stage, scores, decays and pieces, outputs, state) with two waves a
+// SIMD at most, as the state leaves registers for no more (one where 512 workgroups of two waves are all there is: 64 columns and fewer): the
+// matrix units are 30 to 44 % busy, vector units and memory less than that.
 // Two blocks on their way instead of one, or heads in another order over the L2s, change nothing; 16 columns a wave (four
 // waves a SIMD) read each operand from LDS twice as often: bf16 229 us for the 162 of 32, fp32 the other way (137 for 205 at
 // 64 features).  One layout is kept for all types.
 //
-// Precision: operands are exact sums of bf16 pieces (bf16: 1, fp16: 2, fp32: 3).  Scores, states and decayed c's are split into
-// pieces to nearest as they enter a product: two for 16-bit outputs (2^-17, nothing beside their rounding), three for fp32
-// outputs and for what enters states.  Products of pieces i, j are taken where i + j is within the piece count, into fp32.
+// Precision: operands are exact sums of bf16 pieces (bf16: 1, fp16: 2, fp32: 3).  Scores, states and decayed c's are fp32 where they
+// are summed and kept, and are split into pieces to nearest as they enter a product: two for 16-bit outputs (2^-17, nothing beside their
+// rounding), three for fp32 outputs and for what enters states.  Products of pieces i, j are taken where i + j is within the piece count,
+// into fp32.
 //
 // What is not finite reaches what the recurrence lets it reach, and no token before it: scores of later tokens are replaced by zeros, and
 // a c that is not finite (or rounds to infinity as bf16: fp32 above 3.39e38) is looked for as it is staged, taken out of its block and put

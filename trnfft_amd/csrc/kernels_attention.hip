@@ -10,7 +10,8 @@
 //   dk     v   do  q   reversed  (dS)^T       from dS_T^T
 //   dv     k   q   do  reversed  dS           from dS_T, ends as dS_0
 // (forward, a state reaches token t with gamma^(t+1); reversed, dS_T reaches token s with gamma^(T-1-s): the decay
-// comes after the token instead of before it).  Scores, states and sums are fp32 whatever the inputs' type.
+// comes after the token instead of before it).  Scores, states and sums are held in fp32 whatever the inputs' type; in blocks they enter
+// the products of 16-bit outputs as 16 to 17 bits of theirs (attention_blocks.h).
 //
 // The log decay's gradient is the sum over all pairs of lag * flow.  Token by token it is carried by the state's derivative
 // dM/dg: M' <- gamma (M' + M), with each token's contribution a M' . x (the dq pass, x = q), and M' . dS_T^T at the end; in
@@ -221,7 +222,7 @@ static unsigned looping_blocks(long long total) { return (unsigned)std::min((tot
 
 // (batch, token, head, features) of any strides as a dense tensor of `padded` features, zeros past the last: operands that are
 // not in whole 16-byte pieces, which the blocks' loads need.  32 x 1024 tokens of 16 bf16 heads of 127: 3 copies and a
-// pass 415 us (a value a thread: 860), where heads of 128 take 157.
+// pass 415 us (a value a thread: 860), where heads of 128 take 181.
 // A thread writes one piece of 16 bytes, and reads it in one load (at whatever address: the hardware takes any) where it is whole.
 template <typename U>
 __global__ __launch_bounds__(256) void attn_pack_kernel(const U* __restrict__ in, U* __restrict__ out, long long total,
@@ -313,7 +314,7 @@ hipError_t launch_attn_head_sum(const float* in, void* out, int dtype, long long
 
 // ------------------------------------------------------------------------------------------------
 // One token of every stream: S <- gamma S + k v^T in place, o = scale S^T q.  Bound by reading and writing the states
-// (8 bytes an element), each of them once: 256 streams of 16 heads of 128 x 128, 109 us, 4.9 TB/s.  A workgroup takes 32 columns,
+// (8 bytes an element), each of them once: 256 streams of 16 heads of 128 x 128, 108 us, 4.9 TB/s.  A workgroup takes 32 columns,
 // so that one stream of 8 heads of 64 is 16 workgroups: 8 lanes of four columns (a 128-byte line together), 32 row groups of 4
 // rows a pass, all of a pass's 16-byte loads ahead of its arithmetic.  (At addresses that are no multiples of 16 bytes the same
 // accesses take 163 us.  Where columns are no multiple of 4 a row's last ones go by the value: 126 columns, 180 us; all of them so, 199.)
