@@ -109,7 +109,7 @@ def _require_hip(what: str) -> None:
 
 def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
     """Raises where an input carries a forward-mode tangent, which a call that knows none would drop."""
-    if forward_ad._current_level >= 0:
+    if getattr(forward_ad, "_current_level", 0) >= 0:
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
