@@ -47,7 +47,7 @@ def run(parts, g, do, decays):
 
 # (a head of 160 features goes token by token; 600 frames of one sequence are shared out over segments)
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("t,dk,dv", [(150, 32, 48), (600, 64, 128), (90, 160, 16)])
+@pytest.mark.parametrize("t,dk,dv", [(150, 32, 48), (600, 64, 128), (130, 128, 128), (90, 160, 16)])
 @pytest.mark.parametrize("where", ["first", "middle", "last"])
 @pytest.mark.parametrize("name,value", [("k", math.nan), ("v", math.inf), ("v", math.nan), ("q", -math.inf), ("do", math.inf)])
 def test_what_is_not_finite_does_not_reach_back(dtype, t, dk, dv, where, name, value):
