@@ -382,6 +382,97 @@ int tfa_adamw_step(int64_t count, const tfa_adam_tensor* tensors, const tfa_adam
 /* The fp32 values that 8-bit states stand for (squares = 0: exp_avg, 1: exp_avg_sq). */
 int tfa_adamw_state_values(int64_t count, const tfa_code_tensor* tensors, int32_t squares, tfa_stream stream);
 
+/*
+ * Causal convolution along frames with a short filter for each channel, channels last, and an activation:
+ *   y_t = act(bias + sum_j weight[c][j] x_{t - width + 1 + j}),  j < width
+ * x: (batch, tokens, channels) at strides of batch and token (in elements; channels contiguous, any address); y and the
+ * gradients are contiguous.  weight: fp32 (channels, width), bias: fp32 (channels) or NULL.  States hold the last width - 1
+ * inputs, (batch, width - 1, channels) of the call's type: state_in (NULL: zeros) is what came before the first token,
+ * state_out (NULL: not wanted; must not be state_in) what a sequence ends with.  lengths: (batch) device int64 or NULL; tokens at and
+ * past a sequence's length are padding: never read, zeros in y and the gradients.  Sums are fp32.  Widths 1 to 8.
+ */
+typedef struct tfa_conv_desc {
+  int32_t dtype; /* TFA_DTYPE_* of x, y, states and their gradients */
+  int32_t channels, width, activation;
+  int64_t batch, tokens;
+  int64_t x_stride[2]; /* batch, token */
+} tfa_conv_desc;
+
+int tfa_causal_conv(const tfa_conv_desc* desc, const void* x, const float* weight, const float* bias, const int64_t* lengths,
+                    const void* state_in, void* y, void* state_out, tfa_stream stream);
+/* Gradients of a loss whose gradients by y and state_out are grad_y (contiguous) and grad_state_out (NULL: zero); each may be
+ * NULL.  workspace: device memory of the size that tfa_causal_conv_workspace_size gives. */
+int tfa_causal_conv_workspace_size(const tfa_conv_desc* desc, size_t* bytes);
+int tfa_causal_conv_backward(const tfa_conv_desc* desc, const void* x, const float* weight, const float* bias,
+                             const int64_t* lengths, const void* state_in, const void* grad_y, const void* grad_state_out,
+                             void* grad_x, float* grad_weight, float* grad_bias, void* grad_state_in, void* workspace,
+                             tfa_stream stream);
+/* One token of every stream (tokens = 1): state is shifted in place. */
+int tfa_causal_conv_step(const tfa_conv_desc* desc, const void* x, const float* weight, const float* bias, void* state, void* y,
+                         tfa_stream stream);
+
+/*
+ * The selective scan of a state space layer, `states` values a channel:
+ *   s_t = softplus(dt_t + dt_bias) (or dt_t + dt_bias),  h_t = exp(s_t a) h_{t-1} + s_t x_t b_t,
+ *   y_t = (c_t . h_t + d x_t) silu(z_t)
+ * x, dt, z: (batch, tokens, channels) at strides of batch and token, channels contiguous; b, c: (batch, tokens, groups, states) at
+ * strides of batch, token and group, states contiguous, shared by channels / groups neighbouring channels; all of one type, at any
+ * address.  a: fp32 (channels, states); d, dt_bias: fp32 (channels) or NULL (zero); z may be NULL (no gate).  State tensors are fp32
+ * (batch, channels, states).  lengths: (batch) device int64 or NULL; tokens at and past a sequence's length are padding: never
+ * read, zeros in y and the gradients, and the state is the one at the length.  States, exponentials and sums are fp32 for every
+ * type.  What is not finite makes NaN or infinities of its channel from its token on.  Up to 64 states.
+ */
+typedef struct tfa_scan_desc {
+  int32_t dtype; /* TFA_DTYPE_* of x, dt, z, b, c, y and their gradients */
+  int32_t channels, groups, states;
+  int32_t softplus, reserved;
+  int64_t batch, tokens;
+  int64_t x_stride[2], dt_stride[2], z_stride[2]; /* batch, token */
+  int64_t b_stride[3], c_stride[3];               /* batch, token, group */
+} tfa_scan_desc;
+
+/* Bytes of the states that a backward needs of its forward, and of the workspaces of both. */
+int tfa_selective_scan_sizes(const tfa_scan_desc* desc, size_t* kept, size_t* workspace, size_t* backward_workspace);
+/* state_in may be NULL (zeros), state_out NULL (not wanted; must not be state_in), kept NULL (no backward follows). */
+int tfa_selective_scan(const tfa_scan_desc* desc, const void* x, const void* dt, const float* a, const void* b, const void* c,
+                       const float* d, const void* z, const float* dt_bias, const int64_t* lengths, const float* state_in,
+                       void* y, float* state_out, void* kept, void* workspace, tfa_stream stream);
+/* Where the gradients of a loss by y (contiguous) and state_out (NULL: zero) go; all contiguous in the layout of what they are
+ * gradients of, NULL where not wanted (grad_state_in must not be grad_state_out). */
+typedef struct tfa_scan_grads {
+  const void* grad_y;
+  const float* grad_state_out;
+  void *x, *dt, *b, *c, *z;
+  float *a, *d, *dt_bias, *state_in;
+} tfa_scan_grads;
+int tfa_selective_scan_backward(const tfa_scan_desc* desc, const void* x, const void* dt, const float* a, const void* b,
+                                const void* c, const float* d, const void* z, const float* dt_bias, const int64_t* lengths,
+                                const float* state_in, const void* kept, const tfa_scan_grads* grads, void* workspace,
+                                tfa_stream stream);
+/* One token of every stream (tokens = 1): state is updated in place. */
+int tfa_selective_scan_step(const tfa_scan_desc* desc, const void* x, const void* dt, const float* a, const void* b,
+                            const void* c, const float* d, const void* z, const float* dt_bias, float* state, void* y,
+                            tfa_stream stream);
+
+/*
+ * The norm of all values of many contiguous tensors, norm[0] = sqrt(sum of squares) with squares summed in 64 bits, and their
+ * clipping: every value times min(1, max_norm / (norm + 1e-6)), in place.  A norm that is not finite makes gradients NaN or zero.
+ * tensors[d], count[d]: those of type d (TFA_DTYPE_*); host memory, read before the call returns.  norm: device fp32.
+ * parts: device workspace of the size that tfa_grad_norm_workspace_size gives.  Sums are added in one order whatever the timing.
+ */
+typedef struct tfa_grad_tensor {
+  void* data;
+  int64_t n;
+} tfa_grad_tensor;
+typedef struct tfa_grad_lists {
+  const tfa_grad_tensor* tensors[3];
+  int64_t count[3];
+} tfa_grad_lists;
+int tfa_grad_norm_workspace_size(const tfa_grad_lists* grads, size_t* bytes);
+int tfa_grad_norm(const tfa_grad_lists* grads, float* norm, void* workspace, tfa_stream stream);
+/* max_norm: at least 0.  Tensors must not overlap. */
+int tfa_clip_grads(const tfa_grad_lists* grads, double max_norm, float* norm, void* workspace, tfa_stream stream);
+
 /* Thread-local message describing the last failure on this thread ("" if none). */
 const char* tfa_last_error(void);
 

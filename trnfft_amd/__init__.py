@@ -29,9 +29,10 @@ from .attention import linear_attention, linear_attention_step
 from .complex import ComplexTensor, complex_matmul
 from .dispatch import HAS_HIP, HAS_NKI, complex_gemm, complex_linear, get_backend, hip_accepts, set_backend
 from .norm import group_norm
-from .optim import adamw_state_values, adamw_step
+from .optim import adamw_state_values, adamw_step, clip_grads, grad_norm
 from .plan import FFTAlgorithm, FFTPlan, clear_plan_cache, create_plan
 from .precision import get_precision, set_ozaki_product_precision_verified, set_precision
+from .state_space import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
 __all__ = [
     "fft",
@@ -62,6 +63,12 @@ __all__ = [
     "group_norm",
     "adamw_step",
     "adamw_state_values",
+    "grad_norm",
+    "clip_grads",
+    "causal_conv",
+    "causal_conv_step",
+    "selective_scan",
+    "selective_scan_step",
     "HAS_HIP",
     "HAS_NKI",
     "set_backend",

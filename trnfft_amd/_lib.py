@@ -66,6 +66,17 @@ EXPORTS = (
     "tfa_group_norm_backward",
     "tfa_adamw_step",
     "tfa_adamw_state_values",
+    "tfa_causal_conv",
+    "tfa_causal_conv_workspace_size",
+    "tfa_causal_conv_backward",
+    "tfa_causal_conv_step",
+    "tfa_selective_scan_sizes",
+    "tfa_selective_scan",
+    "tfa_selective_scan_backward",
+    "tfa_selective_scan_step",
+    "tfa_grad_norm_workspace_size",
+    "tfa_grad_norm",
+    "tfa_clip_grads",
     "tfa_last_error",
     "tfa_abi_version",
 )
@@ -131,6 +142,43 @@ class AdamDesc(ctypes.Structure):
         ("eps", ctypes.c_double),
         ("weight_decay", ctypes.c_double),
     ]
+
+
+class ConvDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("channels", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("x_stride_batch", ctypes.c_int64),
+        ("x_stride_token", ctypes.c_int64),
+    ]
+
+
+class ScanDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("channels", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("states", ctypes.c_int32),
+        ("softplus", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        *((f"{name}_stride_{axis}", ctypes.c_int64) for name in ("x", "dt", "z") for axis in ("batch", "token")),
+        *((f"{name}_stride_{axis}", ctypes.c_int64) for name in "bc" for axis in ("batch", "token", "group")),
+    ]
+
+
+class ScanGrads(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("grad_y", "grad_state_out", "x", "dt", "b", "c", "z", "a", "d", "dt_bias",
+                                                     "state_in")]
+
+
+class GradLists(ctypes.Structure):
+    _fields_ = [("tensors", ctypes.c_char_p * 3), ("count", ctypes.c_int64 * 3)]
 
 
 _lib = None
@@ -202,8 +250,20 @@ def _declare(lib: ctypes.CDLL) -> None:
     # the tables of the multi-tensor steps (tfa_adam_tensor, tfa_code_tensor) are passed as packed 64-bit words
     lib.tfa_adamw_step.argtypes = [_i64, _vp, ctypes.POINTER(AdamDesc), _vp]
     lib.tfa_adamw_state_values.argtypes = [_i64, _vp, _i32, _vp]
+    lib.tfa_causal_conv.argtypes = [ctypes.POINTER(ConvDesc)] + [_vp] * 8
+    lib.tfa_causal_conv_workspace_size.argtypes = [ctypes.POINTER(ConvDesc), size_p]
+    lib.tfa_causal_conv_backward.argtypes = [ctypes.POINTER(ConvDesc)] + [_vp] * 13
+    lib.tfa_causal_conv_step.argtypes = [ctypes.POINTER(ConvDesc)] + [_vp] * 6
+    lib.tfa_selective_scan_sizes.argtypes = [ctypes.POINTER(ScanDesc), size_p, size_p, size_p]
+    lib.tfa_selective_scan.argtypes = [ctypes.POINTER(ScanDesc)] + [_vp] * 15
+    lib.tfa_selective_scan_backward.argtypes = [ctypes.POINTER(ScanDesc)] + [_vp] * 11 + [ctypes.POINTER(ScanGrads), _vp, _vp]
+    lib.tfa_selective_scan_step.argtypes = [ctypes.POINTER(ScanDesc)] + [_vp] * 11
+    lib.tfa_grad_norm_workspace_size.argtypes = [ctypes.POINTER(GradLists), size_p]
+    lib.tfa_grad_norm.argtypes = [ctypes.POINTER(GradLists), _vp, _vp, _vp]
+    lib.tfa_clip_grads.argtypes = [ctypes.POINTER(GradLists), ctypes.c_double, _vp, _vp, _vp]
     for name in EXPORTS:
-        if name.startswith(("tfa_linear_attention", "tfa_group_norm", "tfa_adamw")):
+        if name.startswith(("tfa_linear_attention", "tfa_group_norm", "tfa_adamw", "tfa_causal_conv", "tfa_selective_scan",
+                            "tfa_grad_norm", "tfa_clip_grads")):
             getattr(lib, name).restype = ctypes.c_int
     lib.tfa_last_error.argtypes = []
     lib.tfa_last_error.restype = ctypes.c_char_p

@@ -42,6 +42,13 @@ SOURCES = [
     "kernels_attention_f16.hip",
     "kernels_norm.hip",
     "kernels_adamw.hip",
+    "state_space_ops.hip",
+    "kernels_conv.hip",
+    "kernels_scan.hip",
+    "kernels_scan_f32.hip",
+    "kernels_scan_bf16.hip",
+    "kernels_scan_f16.hip",
+    "kernels_clip.hip",
 ]
 
 CXX = os.environ.get("CXX", "g++")

@@ -1,0 +1,217 @@
+// The selective scan's step for one token of every stream, and what joins the parts of whole sequences (scan_blocks.h).
+#include "scan_blocks.h"
+
+namespace tfa {
+
+// The states that segments start from, in place of their own sums; reversed, the gradients that they end with.  A thread takes a lane of a
+// wave's states over the segments, one after the other.
+__global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, int lanes, bool reverse, long long first) {
+  const long long id = (first + blockIdx.x) * 256 + threadIdx.x, unit = id / 64;
+  const int lane = (int)(id % 64), channels = 64 / lanes, q = lane / channels, each = p.channels / p.groups;
+  const int tiles = (each + channels - 1) / channels;
+  const long long units = p.batch * p.groups * tiles;
+  if (unit >= units) return;
+  const int own = (int)(unit % tiles) * channels + lane % channels;
+  const long long row = unit / tiles / p.groups;
+  const bool valid = own < each;
+  const int channel = (int)(unit / tiles % p.groups) * each + (valid ? own : 0);
+  const Four32 a = load_states(p.a + (long long)channel * p.n, p.n, q, valid);
+  const float* from = reverse ? p.dstate_out : p.state_in;
+  Four32 s = {};
+  if (from) s = load_states(from + (row * p.channels + channel) * p.n, p.n, q, valid);
+  for (int k = 0; k < p.segments; ++k) {
+    const long long at = ((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane;
+    const Four32 sum = reinterpret_cast<Four32*>(p.seg_state)[at];
+    const float steps = p.seg_steps[at] * kLog2E;
+    reinterpret_cast<Four32*>(p.seg_state)[at] = s;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s.v[r] = __builtin_fmaf(__builtin_amdgcn_exp2f(steps * a.v[r]), s.v[r], sum.v[r]);
+  }
+}
+
+// db and dc from the workgroups' shares: a thread for each value, zeros where there is padding
+template <typename T>
+__global__ __launch_bounds__(256) void scan_shares_kernel(ScanArgs p, int lanes, long long parts, long long first) {
+  const long long id = (first + blockIdx.x) * 256 + threadIdx.x, width = (long long)p.groups * 8 * lanes, cells = p.batch * p.tokens;
+  const long long cell = id / width;
+  if (cell >= cells) return;
+  const int at = (int)(id % width), group = at / (8 * lanes), which = at / (4 * lanes) % 2, k = at % (4 * lanes);
+  T* const out = static_cast<T*>(which ? p.dc : p.db);
+  if (!out || k >= p.n) return;
+  float sum = 0.0f;
+  if (cell % p.tokens < scan_end(p, cell / p.tokens))
+    for (long long i = 0; i < parts; ++i) sum += p.shared_parts[i * cells * width + id];
+  out[(cell * p.groups + group) * p.n + k] = from_f32<T>(sum);
+}
+
+// da, dd and ddt_bias from the rows' and segments' sums
+__global__ __launch_bounds__(256) void scan_channels_kernel(ScanArgs p, int lanes) {
+  const int channels = 64 / lanes, each = p.channels / p.groups, tiles = (each + channels - 1) / channels;
+  const long long id = blockIdx.x * 256LL + threadIdx.x, of_row = (long long)p.groups * tiles * 64;
+  if (id >= of_row) return;
+  const int lane = (int)(id % 64), q = lane / channels, own = (int)(id / 64 % tiles) * channels + lane % channels;
+  if (own >= each) return;
+  const int channel = (int)(id / 64 / tiles) * each + own;
+  const long long count = p.segments * p.batch, all = count * of_row;
+  Four32 da = {};
+  float dd = 0.0f, dbias = 0.0f;
+  for (long long i = 0; i < count; ++i) {
+    const long long at = i * of_row + id;
+    const Four32 v = reinterpret_cast<const Four32*>(p.channel_parts)[at];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) da.v[r] += v.v[r];
+    dd += p.channel_parts[4 * all + at];
+    dbias += p.channel_parts[5 * all + at];
+  }
+  if (p.da) store_states(p.da + (long long)channel * p.n, p.n, q, true, da);
+  if (q == 0 && p.dd) p.dd[channel] = dd;
+  if (q == 0 && p.ddt_bias) p.ddt_bias[channel] = dbias;
+}
+
+template <typename F>
+static hipError_t scan_launches(long long threads, F f) {
+  const long long blocks = (threads + 255) / 256;
+  for (long long first = 0; first < blocks; first += max_blocks(256)) {
+    f(first, (unsigned)std::min(blocks - first, max_blocks(256)));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+static hipError_t scan_mode(const ScanArgs& p, ScanMode mode) {
+  return p.dtype == 0 ? scan_f32(p, mode) : p.dtype == 1 ? scan_bf16(p, mode) : scan_f16(p, mode);
+}
+
+static long long scan_tiles(const ScanArgs& p) {
+  const int channels = 64 / scan_lanes(p.n);
+  return (p.channels / p.groups + channels - 1) / channels;
+}
+long long scan_waves(const ScanArgs& p) { return p.batch * p.groups * scan_tiles(p); }
+
+static long long share_parts(const ScanArgs& p) {
+  const int waves = scan_lanes(p.n) <= 4 ? kBackWaves<4> : kBackWaves<8>;
+  return (scan_tiles(p) + waves - 1) / waves;
+}
+
+ScanSizes scan_sizes(const ScanArgs& p) {
+  ScanSizes s;
+  const size_t lanes = (size_t)scan_waves(p) * 64, of_segments = p.segments > 1 ? p.segments * lanes : 0;
+  s.kept = p.tokens > 0 ? (p.tokens - 1) / kScanStretch * lanes * 4 * sizeof(float) : 0;
+  s.seg_state = of_segments * 4 * sizeof(float);
+  s.seg_steps = of_segments * sizeof(float);
+  s.shared_parts = (size_t)share_parts(p) * p.batch * p.tokens * p.groups * 8 * scan_lanes(p.n) * sizeof(float);
+  s.channel_parts = (size_t)p.segments * lanes * 6 * sizeof(float);
+  return s;
+}
+
+static hipError_t scan_segments(const ScanArgs& p, bool reverse) {
+  if (p.segments == 1) return hipSuccess;
+  const hipError_t e = scan_mode(p, reverse ? kScanBackSums : kScanSums);
+  if (e != hipSuccess) return e;
+  return scan_launches(scan_waves(p) * 64, [&](long long first, unsigned n) {
+    hipLaunchKernelGGL(scan_join_kernel, dim3(n), dim3(256), 0, p.stream, p, scan_lanes(p.n), reverse, first);
+  });
+}
+
+hipError_t launch_scan_forward(const ScanArgs& p) {
+  const hipError_t e = scan_segments(p, false);
+  return e != hipSuccess ? e : scan_mode(p, kScanForward);
+}
+
+hipError_t launch_scan_backward(const ScanArgs& p) {
+  hipError_t e = scan_segments(p, true);
+  if (e != hipSuccess) return e;
+  e = scan_mode(p, kScanBackward);
+  if (e != hipSuccess) return e;
+  const int lanes = scan_lanes(p.n);
+  if (p.shared_parts) {
+    e = scan_launches(p.batch * p.tokens * p.groups * 8 * lanes, [&](long long first, unsigned n) {
+      if (p.dtype == 0) hipLaunchKernelGGL(scan_shares_kernel<float>, dim3(n), dim3(256), 0, p.stream, p, lanes, share_parts(p), first);
+      if (p.dtype == 1) hipLaunchKernelGGL(scan_shares_kernel<__bf16>, dim3(n), dim3(256), 0, p.stream, p, lanes, share_parts(p), first);
+      if (p.dtype == 2) hipLaunchKernelGGL(scan_shares_kernel<_Float16>, dim3(n), dim3(256), 0, p.stream, p, lanes, share_parts(p), first);
+    });
+    if (e != hipSuccess) return e;
+  }
+  if (!p.da && !p.dd && !p.ddt_bias) return hipSuccess;
+  const long long threads = p.groups * scan_tiles(p) * 64;
+  hipLaunchKernelGGL(scan_channels_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, p.stream, p, lanes);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------
+
+// sum over Q neighbouring lanes, in all of them
+template <int Q>
+__device__ __forceinline__ float sum_lanes(float v) {
+  if constexpr (Q >= 2) v += lane_xor<1>(v);
+  if constexpr (Q >= 4) v += lane_xor<2>(v);
+  if constexpr (Q >= 8) v += lane_xor<7>(v);
+  if constexpr (Q >= 16) v += lane_xor<8>(v);
+  return v;
+}
+
+// Q neighbouring lanes a channel, 4 states each, so that a wave reads and writes its states in one piece.  Memory bound by the states.
+template <typename T, int Q>
+__global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, bool whole, long long first) {
+  const long long id = ((first + blockIdx.x) * 256 + threadIdx.x) / Q, row = id / p.channels;
+  const int q = threadIdx.x % Q;
+  if (row >= p.batch) return;
+  const int channel = (int)(id % p.channels), group = channel / (p.channels / p.groups);
+  float* const state = p.state + (row * p.channels + channel) * p.n;
+  const float* const pa = p.a + (long long)channel * p.n;
+  const T* const pb = static_cast<const T*>(p.b) + row * p.b_sb + group * p.b_sg;
+  const T* const pc = static_cast<const T*>(p.c) + row * p.c_sb + group * p.c_sg;
+  Four32 h, a;
+  if (whole && 4 * q < p.n) {
+    h = *reinterpret_cast<const Four32*>(state + 4 * q);
+    a = *reinterpret_cast<const Four32*>(pa + 4 * q);
+  } else {
+    h = load_states(state, p.n, q, true);
+    a = load_states(pa, p.n, q, true);
+  }
+  const float x = to_f32(static_cast<const T*>(p.x)[row * p.x_sb + channel]);
+  float slope;
+  const float s = step_of(to_f32(static_cast<const T*>(p.dt)[row * p.dt_sb + channel]), p.dt_bias ? p.dt_bias[channel] : 0.0f, p.softplus, slope);
+  const float u = s * x;
+  float y = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int k = 4 * q + r;
+    if (k >= p.n) continue;
+    h.v[r] = __builtin_fmaf(decay_of(s, a.v[r] * kLog2E), h.v[r], u * to_f32(pb[k]));
+    y = __builtin_fmaf(to_f32(pc[k]), h.v[r], y);
+  }
+  if (whole && 4 * q < p.n)
+    *reinterpret_cast<Four32*>(state + 4 * q) = h;
+  else
+    store_states(state, p.n, q, true, h);
+  y = sum_lanes<Q>(y);
+  if (q) return;
+  if (p.d) y = __builtin_fmaf(p.d[channel], x, y);
+  if (p.z) y *= activate(to_f32(static_cast<const T*>(p.z)[row * p.z_sb + channel]), kActSilu);
+  static_cast<T*>(p.y)[row * p.channels + channel] = from_f32<T>(y);
+}
+
+template <typename T, int Q>
+static hipError_t step_lanes(const ScanStep& p) {
+  const bool whole = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.state) | reinterpret_cast<uintptr_t>(p.a)) % 16 == 0;
+  return scan_launches(p.batch * p.channels * Q, [&](long long first, unsigned n) {
+    hipLaunchKernelGGL((scan_step_kernel<T, Q>), dim3(n), dim3(256), 0, p.stream, p, whole, first);
+  });
+}
+template <typename T>
+static hipError_t step_typed(const ScanStep& p) {
+  switch (scan_lanes(p.n)) {
+    case 1: return step_lanes<T, 1>(p);
+    case 2: return step_lanes<T, 2>(p);
+    case 4: return step_lanes<T, 4>(p);
+    case 8: return step_lanes<T, 8>(p);
+  }
+  return step_lanes<T, 16>(p);
+}
+hipError_t launch_scan_step(const ScanStep& p) {
+  return p.dtype == 0 ? step_typed<float>(p) : p.dtype == 1 ? step_typed<__bf16>(p) : step_typed<_Float16>(p);
+}
+
+}  // namespace tfa

@@ -1,6 +1,7 @@
-// Operators of models on frames: decayed linear attention, group norm with an activation, AdamW steps.
-// Argument blocks and launch functions shared by the kernels (kernels_attention.hip, kernels_norm.hip,
-// kernels_adamw.hip) and their C entry points (model_ops.hip).
+// Operators of models on frames: decayed linear attention, group norm with an activation, AdamW steps, causal convolution,
+// selective scan, gradient norms.  Argument blocks and launch functions shared by the kernels (kernels_attention.hip,
+// kernels_norm.hip, kernels_adamw.hip, kernels_conv.hip, kernels_scan.hip, kernels_clip.hip) and their C entry points
+// (model_ops.hip, state_space_ops.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -26,6 +27,26 @@ __device__ __forceinline__ float to_f32<__bf16>(__bf16 x) {
 template <typename T>
 __device__ __forceinline__ T from_f32(float x) {
   return static_cast<T>(x);  // to nearest, ties to even
+}
+
+// V neighbouring values, one access
+template <typename T, int V>
+struct __attribute__((aligned(V * sizeof(T)))) Pack {
+  T v[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_pack(const T* p, float (&x)[V]) {
+  const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = to_f32(u.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const float (&x)[V]) {
+  Pack<T, V> u;
+#pragma unroll
+  for (int i = 0; i < V; ++i) u.v[i] = from_f32<T>(x[i]);
+  *reinterpret_cast<Pack<T, V>*>(p) = u;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -167,5 +188,113 @@ struct CodeTensor {
   long long n;
 };
 hipError_t launch_adam_values(const CodeTensor* tensors, long long count, bool squares, hipStream_t stream);
+
+// ------------------------------------------------------------------------------------------------
+// causal convolution along frames, a filter for each channel
+// ------------------------------------------------------------------------------------------------
+
+struct ConvArgs {
+  const void* x;  // (batch, tokens, channels) at x_sb, x_st
+  long long x_sb, x_st;
+  const float* weight;  // (channels, width)
+  const float* bias;    // or nullptr
+  const long long* lengths;
+  const void* state_in;  // (batch, width - 1, channels) or nullptr: zeros
+  void* y;               // contiguous
+  void* state_out;       // or nullptr
+  int channels, width, act, dtype;
+  long long batch, tokens;
+  // backward: dy contiguous, dstate_out or nullptr; dx, dstate_in, dweight and dbias or nullptr
+  const void* dy;
+  const void* dstate_out;
+  void* dx;
+  void* dstate_in;
+  float* dweight;
+  float* dbias;
+  float* ws;  // conv_workspace_bytes
+  hipStream_t stream;
+};
+size_t conv_workspace_bytes(const ConvArgs& a);
+hipError_t launch_conv_forward(const ConvArgs& a);
+hipError_t launch_conv_backward(const ConvArgs& a);
+// one token: state_out (= state_in) is shifted in place
+hipError_t launch_conv_step(const ConvArgs& a);
+
+// ------------------------------------------------------------------------------------------------
+// selective scan
+// ------------------------------------------------------------------------------------------------
+
+struct ScanArgs {
+  // (batch, tokens, channels) at strides of batch and token, channels contiguous; z may be nullptr (no gate)
+  const void *x, *dt, *z;
+  long long x_sb, x_st, dt_sb, dt_st, z_sb, z_st;
+  // (batch, tokens, groups, n) at strides of batch, token and group, n contiguous
+  const void *b, *c;
+  long long b_sb, b_st, b_sg, c_sb, c_st, c_sg;
+  const float *a;             // (channels, n)
+  const float *d, *dt_bias;   // (channels) or nullptr
+  const long long* lengths;   // (batch) or nullptr
+  const float* state_in;      // (batch, channels, n) or nullptr: zeros
+  float* state_out;           // or nullptr
+  void* y;                    // contiguous
+  bool softplus;
+  int channels, groups, n, dtype;
+  long long batch, tokens;
+  // states at every kScanStretch tokens but the first, as the kernels lay them out: written by the forward, read by the backward
+  float* kept;
+  // a long sequence in segments: their own sums and decays, then the states they start from
+  float* seg_state;
+  float* seg_steps;
+  // backward: dy contiguous; dx, ddt, dz, db and dc contiguous (db, dc: (batch, tokens, groups, n)), or nullptr
+  const void* dy;
+  const float* dstate_out;
+  void *dx, *ddt, *dz, *db, *dc;
+  float *da, *dd, *ddt_bias, *dstate_in;
+  float* shared_parts;   // sums over workgroups' channels of db and dc
+  float* channel_parts;  // sums over rows and segments of da, dd and ddt_bias
+  int segments;
+  long long seg_tokens;  // a multiple of kScanStretch
+  hipStream_t stream;
+};
+constexpr int kScanTile = 16;     // tokens that are worked on together
+constexpr int kScanStretch = 16;  // tokens between kept states
+constexpr int kScanMostStates = 64;
+// Sizes in bytes of what a call needs (segments and seg_tokens set)
+struct ScanSizes {
+  size_t kept, seg_state, seg_steps, shared_parts, channel_parts;
+};
+long long scan_waves(const ScanArgs& p);  // of a segment
+ScanSizes scan_sizes(const ScanArgs& p);
+hipError_t launch_scan_forward(const ScanArgs& p);
+hipError_t launch_scan_backward(const ScanArgs& p);
+struct ScanStep {
+  const void *x, *dt, *z, *b, *c;
+  long long x_sb, dt_sb, z_sb, b_sb, b_sg, c_sb, c_sg;
+  const float *a, *d, *dt_bias;
+  float* state;
+  void* y;
+  bool softplus;
+  int channels, groups, n, dtype;
+  long long batch;
+  hipStream_t stream;
+};
+hipError_t launch_scan_step(const ScanStep& p);
+
+// ------------------------------------------------------------------------------------------------
+// the gradients' global norm and their clipping
+// ------------------------------------------------------------------------------------------------
+
+struct GradTensor {
+  void* p;
+  long long n;
+};
+// tensors of a dtype (the index), any number of each
+struct GradLists {
+  const GradTensor* tensors[3];
+  long long count[3];
+};
+long long grad_parts(const GradLists& g);  // doubles of the workspace
+// norm[0] = sqrt(sum of squares); then, where `scale`, every value times min(1, max_norm / (norm + 1e-6))
+hipError_t launch_grad_norm(const GradLists& g, double* parts, float* norm, bool scale, double max_norm, hipStream_t stream);
 
 }  // namespace tfa

@@ -1,4 +1,5 @@
-"""AdamW over all tensors of a model in few launches, states in 32 or 8 bits (csrc/kernels_adamw.hip).
+"""AdamW over all tensors of a model in few launches, states in 32 or 8 bits (csrc/kernels_adamw.hip), and the gradients' global
+norm and clipping (csrc/kernels_clip.hip).
 
 ``adamw_step`` is the step itself on lists of tensors, ``AdamW`` the torch optimizer on it.  8-bit states keep one fp32
 scale s for every 256 values of a tensor: first moments s sgn(c) (c / 127)^2 of int8 codes c, second moments
@@ -6,6 +7,8 @@ s (c / 255)^4 of uint8 codes (at least 1 where there is any).  The reference has
 """
 
 from __future__ import annotations
+
+import ctypes
 
 import torch
 
@@ -87,6 +90,72 @@ def adamw_state_values(codes, scales, out=None) -> list[torch.Tensor]:
     launch(what, dev, _lib.lib().tfa_adamw_state_values, len(codes), table, int(dtype == torch.uint8))
     torch.autograd.graph.increment_version(out)
     return out
+
+
+def _norm_call(what: str, grads: list, max_norm: float | None) -> torch.Tensor:
+    by_type: dict = {}
+    for g in grads:
+        by_type.setdefault(g.dtype, []).append(g)
+    for dtype in by_type:
+        if dtype not in DTYPES:
+            raise TypeError(f"{what}: float32, bfloat16 or float16 gradients expected, got {dtype}")
+    _require_hip(what)
+    dev = grads[0].device
+    if dev.type != "cuda":
+        raise ValueError(f"{what}: the gradients must be on the GPU")
+    lists = _lib.GradLists()
+    for dtype, own in by_type.items():
+        lists.tensors[DTYPES[dtype]] = _lib.tensor_table()(what, ("gradients",), (own,), (dtype,), dev.index)
+        lists.count[DTYPES[dtype]] = len(own)
+    nbytes = ctypes.c_size_t()
+    _lib.check(_lib.lib().tfa_grad_norm_workspace_size(lists, nbytes), what)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+    if max_norm is None:
+        launch(what, dev, _lib.lib().tfa_grad_norm, lists, norm.data_ptr(), ws.data_ptr())
+    else:
+        launch(what, dev, _lib.lib().tfa_clip_grads, lists, max_norm, norm.data_ptr(), ws.data_ptr())
+        torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+@torch.no_grad()
+def grad_norm(grads) -> torch.Tensor:
+    """The 2-norm of all values of a list of contiguous GPU tensors (float32, bfloat16, float16, mixed as they come), as a
+    float32 scalar on the GPU.  Squares are summed in 64 bits and in one order: the same gradients give the same norm."""
+    grads = list(grads)
+    return _norm_call("grad_norm", grads, None) if grads else torch.zeros(())
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm: float) -> torch.Tensor:
+    """Scales a list of contiguous GPU tensors in place by min(1, max_norm / (norm + 1e-6)); returns their norm before, as
+    grad_norm does.  Nothing is written where the norm is within the bound.  A norm that is infinite makes zeros of finite gradients
+    and NaN of the others, one that is NaN makes NaN of all.  The tensors must not overlap."""
+    what, grads, max_norm = "clip_grads", list(grads), float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"{what}: max_norm must not be negative, got {max_norm}")
+    return _norm_call(what, grads, max_norm) if grads else torch.zeros(())
+
+
+def _in_memory_order(g: torch.Tensor) -> torch.Tensor:
+    """A contiguous view of g where there is one (a gradient of a transposed weight is transposed)."""
+    return g if g.is_contiguous() else g.permute(sorted(range(g.dim()), key=g.stride, reverse=True))
+
+
+def clip_grad_norm_(parameters, max_norm: float, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Clips the gradients of parameters (a tensor or an iterable of them) by their global 2-norm, in place, as
+    torch.nn.utils.clip_grad_norm_ does; returns the norm before.  error_if_nonfinite waits for the GPU and raises where the norm
+    is not finite."""
+    what = "clip_grad_norm_"
+    parameters = [parameters] if torch.is_tensor(parameters) else list(dict.fromkeys(parameters))
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if any(g.is_sparse for g in grads):
+        raise RuntimeError(f"{what}: sparse gradients are not supported")
+    grads = [_in_memory_order(g) for g in grads]
+    if error_if_nonfinite and grads and not torch.isfinite(grad_norm(grads)):
+        raise RuntimeError(f"{what}: the gradients' norm is not finite, so they cannot be clipped")
+    return clip_grads(grads, max_norm)
 
 
 class AdamW(torch.optim.Optimizer):
