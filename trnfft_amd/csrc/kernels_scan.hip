@@ -5,6 +5,7 @@ namespace tfa {
 
 // The states that segments start from, in place of their own sums; reversed, the gradients that they end with.  A thread takes a lane of a
 // wave's states over the segments, one after the other.
+template <int R>
 __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, int lanes, bool reverse, long long first) {
   const long long id = (first + blockIdx.x) * 256 + threadIdx.x, unit = id / 64;
   const int lane = (int)(id % 64), channels = 64 / lanes, q = lane / channels, each = p.channels / p.groups;
@@ -15,27 +16,27 @@ __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, int lanes, b
   const long long row = unit / tiles / p.groups;
   const bool valid = own < each;
   const int channel = (int)(unit / tiles % p.groups) * each + (valid ? own : 0);
-  const Four32 a = load_states(p.a + (long long)channel * p.n, p.n, q, valid);
+  const States<R> a = load_states<R>(p.a + (long long)channel * p.n, p.n, q, valid);
   const float* from = reverse ? p.dstate_out : p.state_in;
-  Four32 s = {};
-  if (from) s = load_states(from + (row * p.channels + channel) * p.n, p.n, q, valid);
+  States<R> s = {};
+  if (from) s = load_states<R>(from + (row * p.channels + channel) * p.n, p.n, q, valid);
   for (int k = 0; k < p.segments; ++k) {
     const long long at = ((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane;
-    const Four32 sum = reinterpret_cast<Four32*>(p.seg_state)[at];
+    const States<R> sum = reinterpret_cast<States<R>*>(p.seg_state)[at];
     const float steps = p.seg_steps[at] * kLog2E;
-    reinterpret_cast<Four32*>(p.seg_state)[at] = s;
+    reinterpret_cast<States<R>*>(p.seg_state)[at] = s;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s.v[r] = __builtin_fmaf(__builtin_amdgcn_exp2f(steps * a.v[r]), s.v[r], sum.v[r]);
+    for (int r = 0; r < R; ++r) s.v[r] = __builtin_fmaf(__builtin_amdgcn_exp2f(steps * a.v[r]), s.v[r], sum.v[r]);
   }
 }
 
-// db and dc from the workgroups' shares: a thread for each value, zeros where there is padding
+// db and dc from the workgroups' shares (of `states` states, n and what fills up the lanes): a thread for each value, zeros where there is padding
 template <typename T>
-__global__ __launch_bounds__(256) void scan_shares_kernel(ScanArgs p, int lanes, long long parts, long long first) {
-  const long long id = (first + blockIdx.x) * 256 + threadIdx.x, width = (long long)p.groups * 8 * lanes, cells = p.batch * p.tokens;
+__global__ __launch_bounds__(256) void scan_shares_kernel(ScanArgs p, int states, long long parts, long long first) {
+  const long long id = (first + blockIdx.x) * 256 + threadIdx.x, width = (long long)p.groups * 2 * states, cells = p.batch * p.tokens;
   const long long cell = id / width;
   if (cell >= cells) return;
-  const int at = (int)(id % width), group = at / (8 * lanes), which = at / (4 * lanes) % 2, k = at % (4 * lanes);
+  const int at = (int)(id % width), group = at / (2 * states), which = at / states % 2, k = at % states;
   T* const out = static_cast<T*>(which ? p.dc : p.db);
   if (!out || k >= p.n) return;
   float sum = 0.0f;
@@ -45,6 +46,7 @@ __global__ __launch_bounds__(256) void scan_shares_kernel(ScanArgs p, int lanes,
 }
 
 // da, dd and ddt_bias from the rows' and segments' sums
+template <int R>
 __global__ __launch_bounds__(256) void scan_channels_kernel(ScanArgs p, int lanes) {
   const int channels = 64 / lanes, each = p.channels / p.groups, tiles = (each + channels - 1) / channels;
   const long long id = blockIdx.x * 256LL + threadIdx.x, of_row = (long long)p.groups * tiles * 64;
@@ -53,17 +55,17 @@ __global__ __launch_bounds__(256) void scan_channels_kernel(ScanArgs p, int lane
   if (own >= each) return;
   const int channel = (int)(id / 64 / tiles) * each + own;
   const long long count = p.segments * p.batch, all = count * of_row;
-  Four32 da = {};
+  States<R> da = {};
   float dd = 0.0f, dbias = 0.0f;
   for (long long i = 0; i < count; ++i) {
     const long long at = i * of_row + id;
-    const Four32 v = reinterpret_cast<const Four32*>(p.channel_parts)[at];
+    const States<R> v = reinterpret_cast<const States<R>*>(p.channel_parts)[at];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) da.v[r] += v.v[r];
-    dd += p.channel_parts[4 * all + at];
-    dbias += p.channel_parts[5 * all + at];
+    for (int r = 0; r < R; ++r) da.v[r] += v.v[r];
+    dd += p.channel_parts[R * all + at];
+    dbias += p.channel_parts[(R + 1) * all + at];
   }
-  if (p.da) store_states(p.da + (long long)channel * p.n, p.n, q, true, da);
+  if (p.da) store_states<R>(p.da + (long long)channel * p.n, p.n, q, true, da);
   if (q == 0 && p.dd) p.dd[channel] = dd;
   if (q == 0 && p.ddt_bias) p.ddt_bias[channel] = dbias;
 }
@@ -84,24 +86,25 @@ static hipError_t scan_mode(const ScanArgs& p, ScanMode mode) {
 }
 
 static long long scan_tiles(const ScanArgs& p) {
-  const int channels = 64 / scan_lanes(p.n);
+  const int channels = 64 / scan_shape(p.n).lanes;
   return (p.channels / p.groups + channels - 1) / channels;
 }
 long long scan_waves(const ScanArgs& p) { return p.batch * p.groups * scan_tiles(p); }
 
 static long long share_parts(const ScanArgs& p) {
-  const int waves = scan_lanes(p.n) <= 4 ? kBackWaves<4> : kBackWaves<8>;
+  const int lanes = scan_shape(p.n).lanes, waves = lanes == 4 ? kBackWaves<4> : lanes == 8 ? kBackWaves<8> : kBackWaves<16>;
   return (scan_tiles(p) + waves - 1) / waves;
 }
 
 ScanSizes scan_sizes(const ScanArgs& p) {
   ScanSizes s;
+  const ScanShape shape = scan_shape(p.n);
   const size_t lanes = (size_t)scan_waves(p) * 64, of_segments = p.segments > 1 ? p.segments * lanes : 0;
-  s.kept = p.tokens > 0 ? (p.tokens - 1) / kScanStretch * lanes * 4 * sizeof(float) : 0;
-  s.seg_state = of_segments * 4 * sizeof(float);
+  s.kept = p.tokens > 0 ? (p.tokens - 1) / kScanStretch * lanes * shape.each * sizeof(float) : 0;
+  s.seg_state = of_segments * shape.each * sizeof(float);
   s.seg_steps = of_segments * sizeof(float);
-  s.shared_parts = (size_t)share_parts(p) * p.batch * p.tokens * p.groups * 8 * scan_lanes(p.n) * sizeof(float);
-  s.channel_parts = (size_t)p.segments * lanes * 6 * sizeof(float);
+  s.shared_parts = (size_t)share_parts(p) * p.batch * p.tokens * p.groups * 2 * shape.lanes * shape.each * sizeof(float);
+  s.channel_parts = (size_t)p.segments * lanes * (shape.each + 2) * sizeof(float);
   return s;
 }
 
@@ -109,8 +112,10 @@ static hipError_t scan_segments(const ScanArgs& p, bool reverse) {
   if (p.segments == 1) return hipSuccess;
   const hipError_t e = scan_mode(p, reverse ? kScanBackSums : kScanSums);
   if (e != hipSuccess) return e;
+  const ScanShape s = scan_shape(p.n);
   return scan_launches(scan_waves(p) * 64, [&](long long first, unsigned n) {
-    hipLaunchKernelGGL(scan_join_kernel, dim3(n), dim3(256), 0, p.stream, p, scan_lanes(p.n), reverse, first);
+    const auto kernel = s.each == 1 ? scan_join_kernel<1> : s.each == 2 ? scan_join_kernel<2> : scan_join_kernel<4>;
+    hipLaunchKernelGGL(kernel, dim3(n), dim3(256), 0, p.stream, p, s.lanes, reverse, first);
   });
 }
 
@@ -124,18 +129,19 @@ hipError_t launch_scan_backward(const ScanArgs& p) {
   if (e != hipSuccess) return e;
   e = scan_mode(p, kScanBackward);
   if (e != hipSuccess) return e;
-  const int lanes = scan_lanes(p.n);
+  const ScanShape s = scan_shape(p.n);
   if (p.shared_parts) {
-    e = scan_launches(p.batch * p.tokens * p.groups * 8 * lanes, [&](long long first, unsigned n) {
-      if (p.dtype == 0) hipLaunchKernelGGL(scan_shares_kernel<float>, dim3(n), dim3(256), 0, p.stream, p, lanes, share_parts(p), first);
-      if (p.dtype == 1) hipLaunchKernelGGL(scan_shares_kernel<__bf16>, dim3(n), dim3(256), 0, p.stream, p, lanes, share_parts(p), first);
-      if (p.dtype == 2) hipLaunchKernelGGL(scan_shares_kernel<_Float16>, dim3(n), dim3(256), 0, p.stream, p, lanes, share_parts(p), first);
+    const int states = s.lanes * s.each;
+    e = scan_launches(p.batch * p.tokens * p.groups * 2 * states, [&](long long first, unsigned n) {
+      const auto kernel = p.dtype == 0 ? scan_shares_kernel<float> : p.dtype == 1 ? scan_shares_kernel<__bf16> : scan_shares_kernel<_Float16>;
+      hipLaunchKernelGGL(kernel, dim3(n), dim3(256), 0, p.stream, p, states, share_parts(p), first);
     });
     if (e != hipSuccess) return e;
   }
   if (!p.da && !p.dd && !p.ddt_bias) return hipSuccess;
   const long long threads = p.groups * scan_tiles(p) * 64;
-  hipLaunchKernelGGL(scan_channels_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, p.stream, p, lanes);
+  const auto kernel = s.each == 1 ? scan_channels_kernel<1> : s.each == 2 ? scan_channels_kernel<2> : scan_channels_kernel<4>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, p.stream, p, s.lanes);
   return hipGetLastError();
 }
 
@@ -167,12 +173,12 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, bool whole, 
     h = *reinterpret_cast<const Four32*>(state + 4 * q);
     a = *reinterpret_cast<const Four32*>(pa + 4 * q);
   } else {
-    h = load_states(state, p.n, q, true);
-    a = load_states(pa, p.n, q, true);
+    h = load_states<4>(state, p.n, q, true);
+    a = load_states<4>(pa, p.n, q, true);
   }
   const float x = to_f32(static_cast<const T*>(p.x)[row * p.x_sb + channel]);
-  float slope;
-  const float s = step_of(to_f32(static_cast<const T*>(p.dt)[row * p.dt_sb + channel]), p.dt_bias ? p.dt_bias[channel] : 0.0f, p.softplus, slope);
+  float s = to_f32(static_cast<const T*>(p.dt)[row * p.dt_sb + channel]) + (p.dt_bias ? p.dt_bias[channel] : 0.0f), slope;
+  if (p.softplus) s = softplus(s, slope);
   const float u = s * x;
   float y = 0.0f;
 #pragma unroll
@@ -185,7 +191,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, bool whole, 
   if (whole && 4 * q < p.n)
     *reinterpret_cast<Four32*>(state + 4 * q) = h;
   else
-    store_states(state, p.n, q, true, h);
+    store_states<4>(state, p.n, q, true, h);
   y = sum_lanes<Q>(y);
   if (q) return;
   if (p.d) y = __builtin_fmaf(p.d[channel], x, y);
@@ -202,13 +208,10 @@ static hipError_t step_lanes(const ScanStep& p) {
 }
 template <typename T>
 static hipError_t step_typed(const ScanStep& p) {
-  switch (scan_lanes(p.n)) {
-    case 1: return step_lanes<T, 1>(p);
-    case 2: return step_lanes<T, 2>(p);
-    case 4: return step_lanes<T, 4>(p);
-    case 8: return step_lanes<T, 8>(p);
-  }
-  return step_lanes<T, 16>(p);
+  if (p.n <= 4) return step_lanes<T, 1>(p);
+  if (p.n <= 8) return step_lanes<T, 2>(p);
+  if (p.n <= 16) return step_lanes<T, 4>(p);
+  return p.n <= 32 ? step_lanes<T, 8>(p) : step_lanes<T, 16>(p);
 }
 hipError_t launch_scan_step(const ScanStep& p) {
   return p.dtype == 0 ? step_typed<float>(p) : p.dtype == 1 ? step_typed<__bf16>(p) : step_typed<_Float16>(p);

@@ -6,11 +6,13 @@
 //   ds_t = x_t sum_n g_t[n] b_t[n] + sum_n a[n] f_t[n],  dx_t = s_t sum_n g_t[n] b_t[n] + d v_t,  da[n] = sum_t s_t f_t[n],
 //   where f_t = g_t e_t h_{t-1},  dz_t = dy_t silu'(z_t) (sum_n c_t[n] h_t[n] + d x_t)
 //
-// A wave takes 64 / Q channels of a row and group, Q lanes a channel with 4 states each (Q the least power of two that holds n), and walks
+// A wave takes 64 / Q channels of a row and group, Q lanes a channel with R states each (4 x 1, 2 or 4 up to 16 states, 8 and 16 x 4 above), and walks
 // along the tokens in tiles of 16.  For what belongs to a channel and token alone (softplus, gates, loads, stores) lane q of a channel takes
 // every Q-th token, so nothing of it is done twice; the tokens' s and s x go to the channel's lanes through LDS, as do b and
 // c, whose rows all channels of a group share.  Sums over the lanes of a channel are folded: Q tokens' sums at once, each ending in
 // the lane of its token.
+//
+// Bound by vector instructions (an exponential takes two instructions' time), not by memory.
 #pragma once
 #include "scan_device.h"
 
@@ -18,18 +20,23 @@
 
 namespace tfa {
 
-struct alignas(16) Four32 {
-  float v[4];
+template <int R>
+struct alignas(4 * R) States {
+  float v[R];
 };
+typedef States<4> Four32;
 
-// where a lane stands
+// Where a wave and its lane stand.  What is one for the wave is kept where the compiler sees it (scalar registers): addresses are a scalar
+// part and 32 bits of the lane's own.
 template <int Q>
 struct ScanPlace {
   static constexpr int kChannels = 64 / Q;
-  int lane, q, c;            // c: channel of the tile
+  int wave, lane, q, c;       // c: channel of the tile
   long long row;
-  int group, tile, channel;  // channel of the row
-  bool valid;                // whether there is such a channel
+  int group, tile, base;      // base: the tile's first channel
+  int own;                    // c, or where there is no such channel the last that there is
+  bool valid;                 // whether there is such a channel
+  bool idle;                  // whether there is no such tile
   long long unit, units;
   int seg;
 };
@@ -38,20 +45,23 @@ template <int Q>
 __device__ __forceinline__ ScanPlace<Q> scan_place(const ScanArgs& p, long long block, int waves) {
   ScanPlace<Q> s;
   const int each = p.channels / p.groups, tiles = (each + s.kChannels - 1) / s.kChannels, across = (tiles + waves - 1) / waves;
+  s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   s.lane = threadIdx.x % 64;
   s.q = s.lane / s.kChannels;
   s.c = s.lane % s.kChannels;
-  s.tile = (int)(block % across) * waves + threadIdx.x / 64;
+  s.tile = (int)(block % across) * waves + s.wave;
   block /= across;
   s.group = (int)(block % p.groups);
   block /= p.groups;
   s.row = block % p.batch;
   s.seg = (int)(block / p.batch);
-  const int own = s.tile * s.kChannels + s.c;
-  s.valid = own < each;
-  s.channel = s.group * each + (s.valid ? own : 0);
+  s.idle = s.tile >= tiles;
+  const int tile = min(s.tile, tiles - 1), left = each - tile * s.kChannels;
+  s.valid = !s.idle && s.c < left;
+  s.own = min(s.c, left - 1);
+  s.base = s.group * each + tile * s.kChannels;
   s.units = p.batch * p.groups * tiles;
-  s.unit = (s.row * p.groups + s.group) * tiles + min(s.tile, tiles - 1);
+  s.unit = (s.row * p.groups + s.group) * tiles + tile;
   return s;
 }
 
@@ -63,53 +73,157 @@ __device__ __forceinline__ void wave_order() {
 
 constexpr int kPlaneRow = kScanTile + 4;  // words of a channel's tokens: rows at 16 bytes that spread over the banks
 
-// A value of every channel and token of the tile: lane q puts tokens q, q + Q, ...; all lanes of a channel read four neighbours.
+// A value of every channel and token of the tile in LDS: lane q puts tokens q, q + Q, ...; all lanes of a channel read four neighbours.
 template <int Q>
-struct ScanPlane {
-  float own[Q == 1 ? kScanTile : 1];
-  __device__ __forceinline__ void put(float* lds, int q, int c, int i, float v) {
-    if constexpr (Q == 1)
-      own[i] = v;
-    else
-      lds[c * kPlaneRow + q + Q * i] = v;
-  }
-  __device__ __forceinline__ Four32 four(const float* lds, int c, int k) const {
-    if constexpr (Q == 1)
-      return {own[4 * k], own[4 * k + 1], own[4 * k + 2], own[4 * k + 3]};
-    else
-      return *reinterpret_cast<const Four32*>(lds + c * kPlaneRow + 4 * k);
-  }
-};
+__device__ __forceinline__ void put_token(float* lds, int q, int c, int i, float v) {
+  lds[c * kPlaneRow + q + Q * i] = v;
+}
+__device__ __forceinline__ Four32 four_tokens(const float* lds, int c, int k) {
+  return *reinterpret_cast<const Four32*>(lds + c * kPlaneRow + 4 * k);
+}
 template <int Q>
-constexpr int kPlaneWords = Q == 1 ? 0 : 64 / Q * kPlaneRow;
+constexpr int kPlaneWords = 64 / Q * kPlaneRow;
 
-// a tile's tokens q, q + Q, ... of one operand
+// p, the same for a wave, and a lane's own 32 bits of an address: one register and no arithmetic in 64 bits.  (The compiler must not see that
+// the lane's part stays as it is from tile to tile: it would keep the sums of both, in 64 bits, in vector registers.)
+template <typename T>
+__device__ __forceinline__ T* lane_address(T* p, unsigned bytes) {
+  asm volatile("" : "+v"(bytes));
+  typedef std::conditional_t<std::is_const_v<T>, const char, char> Byte;
+  return reinterpret_cast<T*>(reinterpret_cast<Byte*>(p) + bytes);
+}
+
+// The tokens q, q + Q, ... of a tile of one operand; those past the end are the last one's again.
 template <typename T, int Q>
 struct ScanTokens {
   T v[kScanTile / Q];
-  // p: token t0 + q of the channel
-  __device__ __forceinline__ void load(const T* p, long long st, long long first, long long end, bool valid) {
+  // p: the tile's first channel at its first token; left: tokens from there to the end, at least one
+  __device__ __forceinline__ void load(const T* p, long long st, const ScanPlace<Q>& s, int left) {
+    if (left >= kScanTile) {
+      const unsigned at = (s.q * (unsigned)st + s.own) * sizeof(T);
 #pragma unroll
-    for (int i = 0; i < kScanTile / Q; ++i) v[i] = valid && first + Q * i < end ? p[i * Q * st] : T(0);
-  }
-};
-// a tile's rows of b or c, 16 by 4 Q with zeros past n and past the end: lane l has elements l, l + 64, ...
-template <typename T, int Q>
-struct ScanRows {
-  T v[Q];
-  // p: token t0 of the row and group
-  __device__ __forceinline__ void load(const T* p, long long st, int n, int lane, long long t0, long long end) {
+      for (int i = 0; i < kScanTile / Q; ++i) v[i] = *lane_address(p + i * Q * st, at);
+    } else {
 #pragma unroll
-    for (int i = 0; i < Q; ++i) {
-      const int at = lane + 64 * i, t = at / (4 * Q), k = at % (4 * Q);
-      v[i] = k < n && t0 + t < end ? p[t * st + k] : T(0);
+      for (int i = 0; i < kScanTile / Q; ++i) v[i] = *lane_address(p, (min(s.q + Q * i, left - 1) * (unsigned)st + s.own) * (unsigned)sizeof(T));
+      // (keeps the compiler from making one load of both ways' with an address in 64 bits of registers)
+      asm volatile("");
     }
   }
-  __device__ __forceinline__ void put(float* lds, int lane) const {
+};
+// A tile's rows of b or c, 16 by Q R, zeros past n and past the end.  With 4 lanes a channel a row of 16 lanes has one q: lane l of it
+// keeps the R states of token l % 16, and products take them from there.  Else they go through LDS.
+template <int BYTES>
+struct WordsOf {
+  typedef unsigned Type __attribute__((ext_vector_type(BYTES / 4)));
+};
+template <>
+struct WordsOf<4> {
+  typedef unsigned Type;
+};
+template <>
+struct WordsOf<2> {
+  typedef unsigned short Type;
+};
+template <typename T, int Q, int R>
+struct ScanRows {
+  static constexpr int kParts = Q == 4 ? 1 : Q / 4, kBytes = R * (int)sizeof(T), kWords = kBytes < 4 ? 1 : kBytes / 4;
+  unsigned w[kParts][kWords];  // as they lie in memory, so that nothing waits for them before they are put to use
+  static __device__ __forceinline__ int token(int lane, int i) { return Q == 4 ? lane % 16 : (lane + 64 * i) / Q; }
+  static __device__ __forceinline__ int state(int lane, int i) { return (Q == 4 ? lane / 16 : (lane + 64 * i) % Q) * R; }
+  // p: the tile's first token; whole: R neighbours can be read at once, and n is a multiple of R
+  __device__ __forceinline__ void load(const T* p, long long st, int n, bool whole, int lane, int left) {
 #pragma unroll
-    for (int i = 0; i < Q; ++i) lds[lane + 64 * i] = to_f32(v[i]);
+    for (int i = 0; i < kParts; ++i) {
+      const int k = state(lane, i);
+      const unsigned at = (left >= kScanTile ? token(lane, i) : min(token(lane, i), left - 1)) * (unsigned)st;
+      if (whole) {
+        typedef typename WordsOf<kBytes>::Type Words;
+        const Words v = *reinterpret_cast<const Words*>(lane_address(p, (at + min(k, n - R)) * (unsigned)sizeof(T)));
+        if constexpr (kWords == 1) {
+          w[i][0] = v;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kWords; ++j) w[i][j] = v[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) w[i][j] = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const T v = *lane_address(p, (at + min(k + r, n - 1)) * (unsigned)sizeof(T));
+          if constexpr (sizeof(T) == 4)
+            w[i][r] = __builtin_bit_cast(unsigned, v);
+          else
+            w[i][r / 2] |= (unsigned)__builtin_bit_cast(unsigned short, v) << 16 * (r % 2);
+        }
+        asm volatile("");  // (as above)
+      }
+    }
+  }
+  __device__ __forceinline__ float value(int i, int r) const {
+    if constexpr (sizeof(T) == 4)
+      return __uint_as_float(w[i][r]);
+    else
+      return to_f32(__builtin_bit_cast(T, (unsigned short)(w[i][r / 2] >> 16 * (r % 2))));
   }
 };
+template <int Q, int R>
+struct ScanBank {
+  States<R> own;
+  template <typename T>
+  __device__ __forceinline__ void put(const ScanRows<T, Q, R>& rows, float* lds, int n, int lane, int left) {
+#pragma unroll
+    for (int i = 0; i < rows.kParts; ++i) {
+      const int t = rows.token(lane, i), k = rows.state(lane, i);
+#pragma unroll
+      for (int r = 0; r < R; ++r) own.v[r] = k + r < n && t < left ? rows.value(i, r) : 0.0f;
+      if (Q > 4) *reinterpret_cast<States<R>*>(lds + R * (lane + 64 * i)) = own;
+    }
+  }
+  __device__ __forceinline__ States<R> at(const float* lds, int t, int q) const {
+    return *reinterpret_cast<const States<R>*>(lds + (t * Q + q) * R);
+  }
+  // with the values of a lane's states at token t: their products with u, those added to sums, and the dot product with x
+  template <int t>
+  __device__ __forceinline__ void products(const float* lds, int q, float u, float (&out)[R]) const {
+    if constexpr (Q == 4) {
+      RowLane<t>::products(own.v, u, out);
+    } else {
+      const States<R> v = at(lds, t, q);
+#pragma unroll
+      for (int r = 0; r < R; ++r) out[r] = v.v[r] * u;
+    }
+  }
+  template <int t>
+  __device__ __forceinline__ void add(const float* lds, int q, float u, float (&sum)[R]) const {
+    if constexpr (Q == 4) {
+      RowLane<t>::add(own.v, u, sum);
+    } else {
+      const States<R> v = at(lds, t, q);
+#pragma unroll
+      for (int r = 0; r < R; ++r) sum[r] = __builtin_fmaf(v.v[r], u, sum[r]);
+    }
+  }
+  template <int t>
+  __device__ __forceinline__ float dot(const float* lds, int q, const float (&x)[R]) const {
+    float sum = 0.0f;
+    if constexpr (Q == 4) {
+      sum = RowLane<t>::dot(own.v, x);
+    } else {
+      const States<R> v = at(lds, t, q);
+#pragma unroll
+      for (int r = 0; r < R; ++r) sum = __builtin_fmaf(v.v[r], x[r], sum);
+    }
+    return sum;
+  }
+};
+template <int Q, int R>
+constexpr int kBankWords = Q == 4 ? 1 : 16 * Q * R;
+template <typename T, int R>
+__device__ __forceinline__ bool rows_whole(const void* p, long long sb, long long st, long long sg, int n) {
+  return (reinterpret_cast<uintptr_t>(p) % (R * sizeof(T)) | (sb | st | sg | n) % R) == 0;
+}
 
 // sums over a channel's lanes of Q values: lane q receives the q-th
 template <int Q, int MASK = 32>
@@ -132,17 +246,19 @@ __device__ __forceinline__ float sum_states(float v) {
     return sum_states<Q / 2, MASK / 2>(fold<MASK>(v));
 }
 
-// four states of a channel in (channels, n) fp32
-__device__ __forceinline__ Four32 load_states(const float* p, int n, int q, bool valid) {
-  Four32 s;
+// a lane's states of a channel in (channels, n) fp32
+template <int R>
+__device__ __forceinline__ States<R> load_states(const float* p, int n, int q, bool valid) {
+  States<R> s;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) s.v[r] = valid && 4 * q + r < n ? p[4 * q + r] : 0.0f;
+  for (int r = 0; r < R; ++r) s.v[r] = valid && R * q + r < n ? p[R * q + r] : 0.0f;
   return s;
 }
-__device__ __forceinline__ void store_states(float* p, int n, int q, bool valid, const Four32& s) {
+template <int R>
+__device__ __forceinline__ void store_states(float* p, int n, int q, bool valid, const States<R>& s) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (valid && 4 * q + r < n) p[4 * q + r] = s.v[r];
+  for (int r = 0; r < R; ++r)
+    if (valid && R * q + r < n) p[R * q + r] = s.v[r];
 }
 
 __device__ __forceinline__ long long scan_end(const ScanArgs& p, long long row) {
@@ -150,374 +266,430 @@ __device__ __forceinline__ long long scan_end(const ScanArgs& p, long long row) 
 }
 __device__ __forceinline__ long long kept_states(const ScanArgs& p) { return p.tokens > 0 ? (p.tokens - 1) / kScanStretch : 0; }
 
-// s_t and, where asked for, its slope by dt_t
-__device__ __forceinline__ float step_of(float dt, float bias, bool soft, float& slope) {
-  slope = 1.0f;
-  return soft ? softplus(dt + bias, slope) : dt + bias;
+// a tile's own steps s_t, zeros where they are not live, and their slopes by dt_t
+template <typename T, int Q, typename L>
+__device__ __forceinline__ void steps_of(const ScanTokens<T, Q>& dt, float bias, bool soft, L live, float (&step)[kScanTile / Q],
+                                         float (&slope)[kScanTile / Q]) {
+#pragma unroll
+  for (int i = 0; i < kScanTile / Q; ++i) step[i] = to_f32(dt.v[i]) + bias, slope[i] = 1.0f;
+  if (soft) {
+#pragma unroll
+    for (int i = 0; i < kScanTile / Q; ++i) step[i] = softplus(step[i], slope[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kScanTile / Q; ++i) step[i] = live(i) ? step[i] : 0.0f;
 }
+// The same tokens to a contiguous (batch, tokens, channels) operand; p as above; all: the wave has all of its channels and tokens.
+template <typename T, int Q>
+__device__ __forceinline__ void store_tokens(T* p, int st, const ScanPlace<Q>& s, int left, bool all, const float (&v)[kScanTile / Q]) {
+  const unsigned at = (s.q * (unsigned)st + s.own) * sizeof(T);
+  if (all) {
+#pragma unroll
+    for (int i = 0; i < kScanTile / Q; ++i) *lane_address(p + (long long)i * Q * st, at) = from_f32<T>(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kScanTile / Q; ++i)
+      if (s.valid && s.q + Q * i < left) *lane_address(p + (long long)i * Q * st, at) = from_f32<T>(v[i]);
+  }
+}
+// Zeros in the tokens from `from` to `to`; p: the wave's first channel at token 0
+template <typename T, int Q>
+__device__ __forceinline__ void zero_tokens(T* p, int st, const ScanPlace<Q>& s, long long from, long long to) {
+  if (s.valid)
+    for (long long t = from + s.q; t < to; t += Q) p[t * st + s.own] = T(0);
+}
+__device__ __forceinline__ int tile_left(long long end, long long t0) { return (int)min(end - t0, (long long)kScanTile); }
 
 constexpr int kScanWaves = 4;  // of a workgroup of the forward and the sums
 
 // OUT: the sequences, or their segments from seg_state's states.  Else the segments' own sums from zero, and their steps' sums.
-template <typename T, int Q, bool OUT>
+template <typename T, int Q, int R, bool OUT>
 __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs p, long long first_block) {
   constexpr int kOwn = kScanTile / Q;
-  __shared__ float rows[kScanWaves][2][64 * Q];
-  __shared__ float planes[kScanWaves][2][Q == 1 ? 1 : kPlaneWords<Q>];
+  __shared__ float rows[kScanWaves][2][kBankWords<Q, R>];
+  __shared__ float planes[kScanWaves][2][kPlaneWords<Q>];
   const ScanPlace<Q> s = scan_place<Q>(p, first_block + blockIdx.x, kScanWaves);
-  if (s.tile * s.kChannels >= p.channels / p.groups) return;
-  const int wave = threadIdx.x / 64;
-  float *const lb = rows[wave][0], *const lc = rows[wave][1], *const ls = planes[wave][0], *const lu = planes[wave][1];
+  if (s.idle) return;
+  float *const lb = rows[s.wave][0], *const lc = rows[s.wave][1], *const ls = planes[s.wave][0], *const lu = planes[s.wave][1];
   const long long seg_begin = s.seg * p.seg_tokens, seg_end = min(p.tokens, seg_begin + p.seg_tokens), end = min(scan_end(p, s.row), seg_end);
 
-  const T* px = static_cast<const T*>(p.x) + s.row * p.x_sb + (seg_begin + s.q) * p.x_st + s.channel;
-  const T* pdt = static_cast<const T*>(p.dt) + s.row * p.dt_sb + (seg_begin + s.q) * p.dt_st + s.channel;
-  const T* pz = p.z ? static_cast<const T*>(p.z) + s.row * p.z_sb + (seg_begin + s.q) * p.z_st + s.channel : nullptr;
+  const T* px = static_cast<const T*>(p.x) + s.row * p.x_sb + seg_begin * p.x_st + s.base;
+  const T* pdt = static_cast<const T*>(p.dt) + s.row * p.dt_sb + seg_begin * p.dt_st + s.base;
+  const T* pz = p.z ? static_cast<const T*>(p.z) + s.row * p.z_sb + seg_begin * p.z_st + s.base : nullptr;
   const T* pb = static_cast<const T*>(p.b) + s.row * p.b_sb + seg_begin * p.b_st + s.group * p.b_sg;
   const T* pc = static_cast<const T*>(p.c) + s.row * p.c_sb + seg_begin * p.c_st + s.group * p.c_sg;
-  T* py = OUT ? static_cast<T*>(p.y) + (s.row * p.tokens + seg_begin + s.q) * p.channels + s.channel : nullptr;
+  const bool b_whole = rows_whole<T, R>(p.b, p.b_sb, p.b_st, p.b_sg, p.n), c_whole = rows_whole<T, R>(p.c, p.c_sb, p.c_st, p.c_sg, p.n);
+  T* const y = OUT ? static_cast<T*>(p.y) + s.row * p.tokens * p.channels + s.base : nullptr;
+  const int channel = s.base + s.own;
 
-  Four32 a = load_states(p.a + (long long)s.channel * p.n, p.n, s.q, s.valid), h = {};
+  States<R> a = load_states<R>(p.a + (long long)channel * p.n, p.n, s.q, s.valid), h = {};
 #pragma unroll
-  for (int r = 0; r < 4; ++r) a.v[r] *= kLog2E;
-  const float bias = p.dt_bias ? p.dt_bias[s.channel] : 0.0f, skip = p.d ? p.d[s.channel] : 0.0f;
+  for (int r = 0; r < R; ++r) a.v[r] *= kLog2E;
+  const float bias = p.dt_bias ? p.dt_bias[channel] : 0.0f, skip = p.d ? p.d[channel] : 0.0f;
   if (OUT) {
     if (p.segments > 1)
-      h = reinterpret_cast<const Four32*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane];
+      h = reinterpret_cast<const States<R>*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane];
     else if (p.state_in)
-      h = load_states(p.state_in + (s.row * p.channels + s.channel) * p.n, p.n, s.q, s.valid);
+      h = load_states<R>(p.state_in + (s.row * p.channels + channel) * p.n, p.n, s.q, s.valid);
   }
+  States<R>* const kept = OUT && p.kept ? reinterpret_cast<States<R>*>(p.kept) + s.unit * kept_states(p) * 64 : nullptr;
+  const bool all_valid = __all(s.valid);
   float steps = 0.0f;
   ScanTokens<T, Q> x, dt, z;
-  ScanRows<T, Q> b, c;
-  const auto fetch = [&](long long t0) {
-    x.load(px, p.x_st, t0 + s.q, end, s.valid);
-    dt.load(pdt, p.dt_st, t0 + s.q, end, s.valid);
-    b.load(pb, p.b_st, p.n, s.lane, t0, end);
+  ScanRows<T, Q, R> b, c;
+  // the next tile, from where the pointers stand, of `left` tokens to the end
+  const auto fetch = [&](int left) {
+    x.load(px, p.x_st, s, left);
+    dt.load(pdt, p.dt_st, s, left);
+    b.load(pb, p.b_st, p.n, b_whole, s.lane, left);
     if (OUT) {
-      c.load(pc, p.c_st, p.n, s.lane, t0, end);
-      if (pz) z.load(pz, p.z_st, t0 + s.q, end, s.valid), pz += kScanTile * p.z_st;
+      c.load(pc, p.c_st, p.n, c_whole, s.lane, left);
+      if (pz) z.load(pz, p.z_st, s, left), pz += kScanTile * p.z_st;
     }
     px += kScanTile * p.x_st, pdt += kScanTile * p.dt_st, pb += kScanTile * p.b_st, pc += kScanTile * p.c_st;
   };
-  fetch(seg_begin);
+  if (seg_begin < end) fetch(tile_left(end, seg_begin));
+  // A tile's results wait in registers until the next one's loads have come: stores and loads are waited for in their order, and stores
+  // right ahead of the next tile would be waited for at once.
+  float ys[kOwn];
   for (long long t0 = seg_begin; t0 < end; t0 += kScanTile) {
-    if (OUT && p.kept && t0 > 0 && t0 % kScanStretch == 0)
-      reinterpret_cast<Four32*>(p.kept)[(s.unit * kept_states(p) + t0 / kScanStretch - 1) * 64 + s.lane] = h;
-    ScanPlane<Q> step, in;
-    float xs[kOwn], zs[kOwn];
+    if (OUT && kept && t0 > 0) *lane_address(kept + (t0 / kScanStretch - 1) * 64, s.lane * (unsigned)sizeof(h)) = h;
+    const int left = tile_left(end, t0);
+    const auto live = [&](int i) { return s.valid && s.q + Q * i < left; };
+    float xs[kOwn], zs[kOwn], own[kOwn], slope[kOwn];
+    steps_of<T, Q>(dt, bias, p.softplus, live, own, slope);
     wave_order();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      float slope;
       xs[i] = to_f32(x.v[i]);
-      const float v = s.valid && t0 + s.q + Q * i < end ? step_of(to_f32(dt.v[i]), bias, p.softplus, slope) : 0.0f;
-      step.put(ls, s.q, s.c, i, v);
-      in.put(lu, s.q, s.c, i, v * xs[i]);
-      steps += v;
-      if (OUT && pz) zs[i] = to_f32(z.v[i]);
+      put_token<Q>(ls, s.q, s.c, i, own[i]);
+      put_token<Q>(lu, s.q, s.c, i, live(i) ? own[i] * xs[i] : 0.0f);
+      steps += own[i];
+      zs[i] = 1.0f;
     }
-    b.put(lb, s.lane);
-    if (OUT) c.put(lc, s.lane);
-    wave_order();
-    fetch(t0 + kScanTile);
-    float part[kScanTile];
+    ScanBank<Q, R> bs, cs;
+    bs.put(b, lb, p.n, s.lane, left);
+    if (OUT) {
+      cs.put(c, lc, p.n, s.lane, left);
+      if (pz) {
 #pragma unroll
-    for (int k = 0; k < kScanTile / 4; ++k) {
-      const Four32 st = step.four(ls, s.c, k), u = in.four(lu, s.c, k);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = 4 * k + j;
-        const Four32 bt = *reinterpret_cast<const Four32*>(lb + t * 4 * Q + 4 * s.q);
-        Four32 ct;
-        if (OUT) ct = *reinterpret_cast<const Four32*>(lc + t * 4 * Q + 4 * s.q);
-        float y = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          h.v[r] = __builtin_fmaf(decay_of(st.v[j], a.v[r]), h.v[r], u.v[j] * bt.v[r]);
-          if (OUT) y = __builtin_fmaf(ct.v[r], h.v[r], y);
-        }
-        part[t] = y;
+        for (int i = 0; i < kOwn; ++i) zs[i] = activate(to_f32(z.v[i]), kActSilu);
       }
     }
+    wave_order();
+    if (OUT && t0 > seg_begin) store_tokens<T, Q>(y + (t0 - kScanTile) * p.channels, p.channels, s, kScanTile, all_valid, ys);
+    if (t0 + kScanTile < end) fetch(tile_left(end, t0 + kScanTile));
+    float part[kScanTile];
+    Four32 st, u;
+    for_each<kScanTile>([&](auto index) TFA_INLINE {
+      constexpr int t = index;
+      if constexpr (t % 4 == 0) st = four_tokens(ls, s.c, t / 4), u = four_tokens(lu, s.c, t / 4);
+      float in[R];
+      bs.template products<t>(lb, s.q, u.v[t % 4], in);
+#pragma unroll
+      for (int r = 0; r < R; ++r) h.v[r] = __builtin_fmaf(decay_of(st.v[t % 4], a.v[r]), h.v[r], in[r]);
+      if constexpr (OUT) part[t] = cs.template dot<t>(lc, s.q, h.v);
+    });
     if (!OUT) continue;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       float sums[Q];
 #pragma unroll
       for (int j = 0; j < Q; ++j) sums[j] = part[i * Q + j];
-      float y = __builtin_fmaf(skip, xs[i], fold_states<Q>(sums));
-      if (pz) y *= activate(zs[i], kActSilu);
-      if (s.valid && t0 + s.q + Q * i < end) py[(long long)i * Q * p.channels] = from_f32<T>(y);
+      ys[i] = __builtin_fmaf(skip, xs[i], fold_states<Q>(sums)) * zs[i];
     }
-    py += (long long)kScanTile * p.channels;
   }
   if (!OUT) {
-    reinterpret_cast<Four32*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane] = h;
+    reinterpret_cast<States<R>*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane] = h;
     p.seg_steps[(s.seg * s.units + s.unit) * 64 + s.lane] = sum_states<Q>(steps);
     return;
   }
-  T* const y = static_cast<T*>(p.y) + s.row * p.tokens * p.channels + s.channel;
-  for (long long t = max(end, seg_begin) + s.q; t < seg_end; t += Q)
-    if (s.valid) y[t * p.channels] = T(0);
+  if (seg_begin < end) {
+    const long long t0 = seg_begin + (end - 1 - seg_begin) / kScanTile * kScanTile;
+    const int left = tile_left(end, t0);
+    store_tokens<T, Q>(y + t0 * p.channels, p.channels, s, left, all_valid && left == kScanTile, ys);
+  }
+  zero_tokens<T, Q>(y, p.channels, s, max(end, seg_begin), seg_end);
   if (p.state_out && s.seg == p.segments - 1)
-    store_states(p.state_out + (s.row * p.channels + s.channel) * p.n, p.n, s.q, s.valid, h);
+    store_states<R>(p.state_out + (s.row * p.channels + channel) * p.n, p.n, s.q, s.valid, h);
 }
 
-// Waves of a workgroup of the backward: their channels' shares of db and dc are added in LDS, so at least 32 channels
+// Waves of a workgroup of the backward: their channels' shares of db and dc are added in LDS, those of 64 channels where LDS holds them
 template <int Q>
-constexpr int kBackWaves = Q <= 4 ? 4 : 8;
+constexpr int kBackWaves = Q == 8 ? 8 : 4;
 
 // The gradients, tile by tile from the last: a tile's states are computed again from the kept one before it.
 // SUM: the segments' own sums of e g from zero at their ends, and their steps' sums.
-template <typename T, int Q, bool SUM>
-__global__ __launch_bounds__(64 * kBackWaves<Q>) void scan_backward_kernel(ScanArgs p, long long first_block) {
+template <typename T, int Q, int R, bool SUM>
+__global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(ScanArgs p, long long first_block) {
   constexpr int kOwn = kScanTile / Q, kWaves = kBackWaves<Q>, kChannels = 64 / Q;
-  __shared__ float rows[kWaves][2][64 * Q];
-  __shared__ float planes[kWaves][3][Q == 1 ? 1 : kPlaneWords<Q>];
-  __shared__ float shares[SUM ? 1 : kWaves][SUM ? 1 : kScanTile * 8 * Q];
+  __shared__ float rows[kWaves][2][kBankWords<Q, R>];
+  __shared__ float planes[kWaves][SUM ? 2 : 6][kPlaneWords<Q>];
+  __shared__ float shares[2][SUM ? 1 : kWaves][SUM ? 1 : kScanTile * 2 * Q * R];  // of this tile and the one before
   const ScanPlace<Q> s = scan_place<Q>(p, first_block + blockIdx.x, kWaves);
-  const bool idle = s.tile * kChannels >= p.channels / p.groups;  // (takes part in the barriers)
-  if (SUM && idle) return;
-  const int wave = threadIdx.x / 64;
-  float *const lb = rows[wave][0], *const lc = rows[wave][1];
-  float *const ls = planes[wave][0], *const lu = planes[wave][1], *const lv = planes[wave][2];
+  if (SUM && s.idle) return;  // (else it takes part in the barriers)
+  float *const lb = rows[s.wave][0], *const lc = rows[s.wave][1];
+  // of every channel and token: s, dy silu(z), s x, and what its own lane needs again: x, the slope of s by dt, dy silu'(z)
+  float *const ls = planes[s.wave][0], *const lv = planes[s.wave][1], *const lu = planes[s.wave][SUM ? 0 : 2];
+  float *const lx = planes[s.wave][SUM ? 0 : 3], *const lslope = planes[s.wave][SUM ? 0 : 4], *const lz = planes[s.wave][SUM ? 0 : 5];
   const long long seg_begin = s.seg * p.seg_tokens, seg_end = min(p.tokens, seg_begin + p.seg_tokens), end = min(scan_end(p, s.row), seg_end);
 
-  const T* const px = static_cast<const T*>(p.x) + s.row * p.x_sb + s.channel;
-  const T* const pdt = static_cast<const T*>(p.dt) + s.row * p.dt_sb + s.channel;
-  const T* const pz = p.z ? static_cast<const T*>(p.z) + s.row * p.z_sb + s.channel : nullptr;
+  const T* const px = static_cast<const T*>(p.x) + s.row * p.x_sb + s.base;
+  const T* const pdt = static_cast<const T*>(p.dt) + s.row * p.dt_sb + s.base;
+  const T* const pz = p.z ? static_cast<const T*>(p.z) + s.row * p.z_sb + s.base : nullptr;
   const T* const pb = static_cast<const T*>(p.b) + s.row * p.b_sb + s.group * p.b_sg;
   const T* const pc = static_cast<const T*>(p.c) + s.row * p.c_sb + s.group * p.c_sg;
-  const long long plane = s.row * p.tokens * p.channels + s.channel;  // of contiguous (batch, tokens, channels)
+  const long long plane = s.row * p.tokens * p.channels + s.base;  // of contiguous (batch, tokens, channels)
   const T* const pdy = static_cast<const T*>(p.dy) + plane;
-  const Four32* const kept = reinterpret_cast<const Four32*>(p.kept) + s.unit * kept_states(p) * 64 + s.lane;
+  const bool b_whole = rows_whole<T, R>(p.b, p.b_sb, p.b_st, p.b_sg, p.n), c_whole = rows_whole<T, R>(p.c, p.c_sb, p.c_st, p.c_sg, p.n);
+  const States<R>* const kept = reinterpret_cast<const States<R>*>(p.kept) + s.unit * kept_states(p) * 64;
+  const int channel = s.base + s.own;
 
-  Four32 a = load_states(p.a + (long long)s.channel * p.n, p.n, s.q, s.valid), carry = {}, da = {};
+  States<R> a = load_states<R>(p.a + (long long)channel * p.n, p.n, s.q, s.valid), carry = {}, da = {};
 #pragma unroll
-  for (int r = 0; r < 4; ++r) a.v[r] *= kLog2E;
-  const float bias = p.dt_bias ? p.dt_bias[s.channel] : 0.0f, skip = p.d ? p.d[s.channel] : 0.0f;
+  for (int r = 0; r < R; ++r) a.v[r] *= kLog2E;
+  const float bias = p.dt_bias ? p.dt_bias[channel] : 0.0f, skip = p.d ? p.d[channel] : 0.0f;
   if (!SUM) {
     if (p.segments > 1)
-      carry = reinterpret_cast<const Four32*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane];
+      carry = reinterpret_cast<const States<R>*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane];
     else if (p.dstate_out)
-      carry = load_states(p.dstate_out + (s.row * p.channels + s.channel) * p.n, p.n, s.q, s.valid);
+      carry = load_states<R>(p.dstate_out + (s.row * p.channels + channel) * p.n, p.n, s.q, s.valid);
   }
+  const bool all_valid = __all(s.valid);
   float steps = 0.0f, dskip = 0.0f, dbias = 0.0f;
   ScanTokens<T, Q> x, dt, z, dy;
-  ScanRows<T, Q> b, c;
-  Four32 h0 = {};
+  ScanRows<T, Q, R> b, c;
+  States<R> h0 = {};
   const auto fetch = [&](long long t0) {
-    const long long t = t0 + s.q;
-    dt.load(pdt + t * p.dt_st, p.dt_st, t, end, s.valid);
-    dy.load(pdy + t * p.channels, p.channels, t, end, s.valid);
-    c.load(pc + t0 * p.c_st, p.c_st, p.n, s.lane, t0, end);
-    if (pz) z.load(pz + t * p.z_st, p.z_st, t, end, s.valid);
+    const int left = tile_left(end, t0);
+    dt.load(pdt + t0 * p.dt_st, p.dt_st, s, left);
+    dy.load(pdy + t0 * p.channels, p.channels, s, left);
+    c.load(pc + t0 * p.c_st, p.c_st, p.n, c_whole, s.lane, left);
+    if (pz) z.load(pz + t0 * p.z_st, p.z_st, s, left);
     if (!SUM) {
-      x.load(px + t * p.x_st, p.x_st, t, end, s.valid);
-      b.load(pb + t0 * p.b_st, p.b_st, p.n, s.lane, t0, end);
+      x.load(px + t0 * p.x_st, p.x_st, s, left);
+      b.load(pb + t0 * p.b_st, p.b_st, p.n, b_whole, s.lane, left);
       if (t0 > 0)
-        h0 = s.valid ? kept[(t0 / kScanStretch - 1) * 64] : Four32{};
+        h0 = *lane_address(kept + (t0 / kScanStretch - 1) * 64, s.lane * (unsigned)sizeof(h0));
       else
-        h0 = p.state_in ? load_states(p.state_in + (s.row * p.channels + s.channel) * p.n, p.n, s.q, s.valid) : Four32{};
+        h0 = p.state_in ? load_states<R>(p.state_in + (s.row * p.channels + channel) * p.n, p.n, s.q, s.valid) : States<R>{};
+    }
+  };
+  // Results of the tile at t0, which wait in registers and LDS until the next one's loads have come (as in the forward)
+  float gb[kOwn], ga[kOwn], ys[kOwn];
+  int turn = 0;  // the half of `shares` that is written next
+  const auto results = [&](long long t0) {
+    const int left = tile_left(end, t0);
+    const bool all = all_valid && left == kScanTile;
+    const long long at = plane + t0 * p.channels;
+    if (p.dx) store_tokens<T, Q>(static_cast<T*>(p.dx) + at, p.channels, s, left, all, gb);
+    if (p.ddt) store_tokens<T, Q>(static_cast<T*>(p.ddt) + at, p.channels, s, left, all, ga);
+    if (p.dz) store_tokens<T, Q>(static_cast<T*>(p.dz) + at, p.channels, s, left, all, ys);
+    if (!p.shared_parts) return;
+    __syncthreads();
+    constexpr int kRow = 2 * Q * R;
+    float* const to = p.shared_parts + (((s.tile / kWaves * p.batch + s.row) * p.tokens + t0) * p.groups + s.group) * kRow;
+    for (int i = threadIdx.x; i < left * kRow; i += 64 * kWaves) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) sum += shares[turn ^ 1][w][i];
+      to[(long long)(i / kRow) * p.groups * kRow + i % kRow] = sum;
     }
   };
   const long long last = end > seg_begin ? seg_begin + (end - 1 - seg_begin) / kScanTile * kScanTile : seg_begin - kScanTile;
   if (last >= seg_begin) fetch(last);
   for (long long t0 = last; t0 >= seg_begin; t0 -= kScanTile) {
-    ScanPlane<Q> step, in, out;
-    float xs[kOwn], ss[kOwn], slope[kOwn], vs[kOwn], zs[kOwn];  // zs: dy silu'(z)
+    const int left = tile_left(end, t0);
+    // (channels past the last and tokens past the end take no part in anything that is shared)
+    const auto live = [&](int i) { return s.valid && s.q + Q * i < left; };
+    float own[kOwn], slope[kOwn], vs[kOwn], zs[kOwn];
+    steps_of<T, Q>(dt, bias, p.softplus, live, own, slope);
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) vs[i] = to_f32(dy.v[i]), zs[i] = 0.0f;
+    if (pz) {
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const float zi = to_f32(z.v[i]), gate = sigmoid(zi);
+        zs[i] = vs[i] * gate * __builtin_fmaf(zi, 1.0f - gate, 1.0f);
+        vs[i] *= zi * gate;
+      }
+    }
     wave_order();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const bool live = s.valid && t0 + s.q + Q * i < end;
-      const float v = step_of(to_f32(dt.v[i]), bias, p.softplus, slope[i]);
-      ss[i] = live ? v : 0.0f;
-      step.put(ls, s.q, s.c, i, ss[i]);
-      steps += ss[i];
-      vs[i] = to_f32(dy.v[i]);
-      zs[i] = 0.0f;
-      if (pz) {
-        const float zi = to_f32(z.v[i]);
-        zs[i] = vs[i] * activation_slope(zi, kActSilu);
-        vs[i] *= activate(zi, kActSilu);
-      }
-      out.put(lv, s.q, s.c, i, vs[i]);
-      if (!SUM) {
-        xs[i] = to_f32(x.v[i]);
-        in.put(lu, s.q, s.c, i, ss[i] * xs[i]);
+      put_token<Q>(ls, s.q, s.c, i, own[i]);
+      put_token<Q>(lv, s.q, s.c, i, live(i) ? vs[i] : 0.0f);
+      if (SUM) {
+        steps += own[i];
+      } else {
+        const float xi = live(i) ? to_f32(x.v[i]) : 0.0f;
+        put_token<Q>(lu, s.q, s.c, i, own[i] * xi);
+        put_token<Q>(lx, s.q, s.c, i, xi);
+        put_token<Q>(lslope, s.q, s.c, i, slope[i]);
+        put_token<Q>(lz, s.q, s.c, i, zs[i]);
       }
     }
-    c.put(lc, s.lane);
-    if (!SUM) b.put(lb, s.lane);
+    ScanBank<Q, R> bs, cs;
+    cs.put(c, lc, p.n, s.lane, left);
+    if (!SUM) bs.put(b, lb, p.n, s.lane, left);
     wave_order();
-    const Four32 start = h0;
+    const States<R> start = s.valid ? h0 : States<R>{};
+    if (!SUM && t0 < last) results(t0 + kScanTile);
     if (t0 > seg_begin) fetch(t0 - kScanTile);
     if constexpr (SUM) {
+      Four32 st, vt;
+      for_each<kScanTile>([&](auto index) TFA_INLINE {
+        constexpr int t = kScanTile - 1 - index;
+        if constexpr (t % 4 == 3) st = four_tokens(ls, s.c, t / 4), vt = four_tokens(lv, s.c, t / 4);
+        cs.template add<t>(lc, s.q, vt.v[t % 4], carry.v);
 #pragma unroll
-      for (int k = kScanTile / 4 - 1; k >= 0; --k) {
-        const Four32 st = step.four(ls, s.c, k), vt = out.four(lv, s.c, k);
-#pragma unroll
-        for (int j = 3; j >= 0; --j) {
-          const Four32 ct = *reinterpret_cast<const Four32*>(lc + (4 * k + j) * 4 * Q + 4 * s.q);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            carry.v[r] = decay_of(st.v[j], a.v[r]) * __builtin_fmaf(ct.v[r], vt.v[j], carry.v[r]);
-        }
-      }
+        for (int r = 0; r < R; ++r) carry.v[r] *= decay_of(st.v[t % 4], a.v[r]);
+      });
     } else {
-      Four32 hs[kScanTile], h = start, da_tile = {};
+      States<R> hs[kScanTile], es[kScanTile], h = start, da_tile = {};
+      // (the next four tokens' values are read while these are worked on)
+      Four32 st = four_tokens(ls, s.c, 0), u = four_tokens(lu, s.c, 0), vt = {}, st_next = {}, u_next = {}, vt_next = {};
+      for_each<kScanTile>([&](auto index) TFA_INLINE {
+        constexpr int t = index, k = t / 4;
+        if constexpr (t % 4 == 0 && k + 1 < kScanTile / 4) st_next = four_tokens(ls, s.c, k + 1), u_next = four_tokens(lu, s.c, k + 1);
+        if constexpr (t % 4 == 0 && k + 1 == kScanTile / 4) vt = four_tokens(lv, s.c, k);
+        float in[R];
+        bs.template products<t>(lb, s.q, u.v[t % 4], in);
 #pragma unroll
-      for (int k = 0; k < kScanTile / 4; ++k) {
-        const Four32 st = step.four(ls, s.c, k), u = in.four(lu, s.c, k);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const Four32 bt = *reinterpret_cast<const Four32*>(lb + (4 * k + j) * 4 * Q + 4 * s.q);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            h.v[r] = __builtin_fmaf(decay_of(st.v[j], a.v[r]), h.v[r], u.v[j] * bt.v[r]);
-          hs[4 * k + j] = h;
+        for (int r = 0; r < R; ++r) {
+          es[t].v[r] = decay_of(st.v[t % 4], a.v[r]);
+          h.v[r] = __builtin_fmaf(es[t].v[r], h.v[r], in[r]);
         }
-      }
-      float sum_b[kScanTile], sum_a[kScanTile], sum_y[kScanTile];
+        hs[t] = h;
+        if constexpr (t % 4 == 3) {
+          if constexpr (k + 1 < kScanTile / 4) st = st_next, u = u_next;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      });
+      // sums over the states for a token: of Q tokens at least before they are folded
+      float sum_b[Q], sum_a[Q], sum_y[Q];
+      for_each<kScanTile>([&](auto index) TFA_INLINE {
+        constexpr int t = kScanTile - 1 - index, k = t / 4, at = t % Q;
+        if constexpr (t % 4 == 3 && k > 0)
+          st_next = four_tokens(ls, s.c, k - 1), u_next = four_tokens(lu, s.c, k - 1), vt_next = four_tokens(lv, s.c, k - 1);
+        const States<R>& before = t ? hs[t ? t - 1 : 0] : start;
+        float v[2 * R];
+        cs.template add<t>(lc, s.q, vt.v[t % 4], carry.v);  // (now g)
+        sum_b[at] = bs.template dot<t>(lb, s.q, carry.v);
+        sum_y[at] = cs.template dot<t>(lc, s.q, hs[t].v);
+        sum_a[at] = 0.0f;
 #pragma unroll
-      for (int k = kScanTile / 4 - 1; k >= 0; --k) {
-        const Four32 st = step.four(ls, s.c, k), u = in.four(lu, s.c, k), vt = out.four(lv, s.c, k);
-#pragma unroll
-        for (int j = 3; j >= 0; --j) {
-          const int t = 4 * k + j;
-          const Four32 bt = *reinterpret_cast<const Four32*>(lb + t * 4 * Q + 4 * s.q);
-          const Four32 ct = *reinterpret_cast<const Four32*>(lc + t * 4 * Q + 4 * s.q);
-          const Four32 before = t ? hs[t ? t - 1 : 0] : start;
-          float v[8];
-          sum_b[t] = sum_a[t] = sum_y[t] = 0.0f;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float g = __builtin_fmaf(ct.v[r], vt.v[j], carry.v[r]);
-            carry.v[r] = decay_of(st.v[j], a.v[r]) * g;
-            const float flow = carry.v[r] * before.v[r];
-            sum_b[t] = __builtin_fmaf(g, bt.v[r], sum_b[t]);
-            sum_a[t] = __builtin_fmaf(flow, a.v[r], sum_a[t]);
-            sum_y[t] = __builtin_fmaf(ct.v[r], hs[t].v[r], sum_y[t]);
-            da_tile.v[r] = __builtin_fmaf(flow, st.v[j], da_tile.v[r]);
-            v[r] = g * u.v[j];
-            v[4 + r] = vt.v[j] * hs[t].v[r];
-          }
-          // over the channels: db's and dc's shares part at the first level, their states at the next two
-          constexpr int kTop = kChannels / 2 == 4 ? 7 : kChannels / 2, kMid = kChannels / 4 == 4 ? 7 : kChannels / 4;
-          float w[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) w[r] = fold<kTop>(v[r], v[r + 4]);
-          w[0] = fold<kMid>(w[0], w[2]);
-          w[1] = fold<kMid>(w[1], w[3]);
-          const int which = s.c / (kChannels / 2), half = s.c / (kChannels / 4) % 2;
-          float* const to = shares[wave] + t * 8 * Q + which * 4 * Q + 4 * s.q + 2 * half;
+        for (int r = 0; r < R; ++r) {
+          v[r] = carry.v[r] * u.v[t % 4];
+          v[R + r] = vt.v[t % 4] * hs[t].v[r];
+          carry.v[r] *= es[t].v[r];
+          const float flow = carry.v[r] * before.v[r];
+          sum_a[at] = __builtin_fmaf(flow, a.v[r], sum_a[at]);
+          da_tile.v[r] = __builtin_fmaf(flow, st.v[t % 4], da_tile.v[r]);
+        }
+        // over the channels: db's and dc's shares part at the first level, their states at the next
+        float* const to = shares[turn][s.wave] + (2 * t + s.c / (kChannels / 2)) * Q * R + R * s.q;
+        constexpr int kTop = kChannels / 2 == 4 ? 7 : kChannels / 2, kMid = kChannels / 4 == 4 ? 7 : kChannels / 4;
+        float w[R];
+        fold_pairs<kTop, R>(v, w);
+        // (lanes with the same sum write the same bits)
+        if constexpr (R == 1) {
+          to[0] = fold<1>(fold<2>(fold<kMid>(w[0])));
+        } else if constexpr (R == 2) {
+          to[s.c / (kChannels / 4) % 2] = fold<1>(fold<2>(fold<kMid>(w[0], w[1])));
+        } else {
+          float* const half = to + s.c / (kChannels / 4) % 2 * 2;
+          float x2[2];
+          fold_pairs<kMid, 2>(w, x2);
           if constexpr (kChannels == 4) {
-            to[0] = w[0];
-            to[1] = w[1];
+            half[0] = x2[0];
+            half[1] = x2[1];
           } else {
-            constexpr int kLow = kChannels / 8 == 4 ? 7 : kChannels / 8;
-            float sum = fold<kLow>(w[0], w[1]);
-            if constexpr (kChannels >= 64) sum = fold<7>(sum);
-            if constexpr (kChannels >= 32) sum = fold<2>(sum);
-            if constexpr (kChannels >= 16) sum = fold<1>(sum);
-            if (s.c % (kChannels / 8) == 0) to[s.c / (kChannels / 8) % 2] = sum;
+            constexpr int kLow = kChannels / 8;
+            float sum = fold<kLow>(x2[0], x2[1]);
+            if constexpr (kChannels == 16) sum = fold<1>(sum);
+            half[s.c / kLow % 2] = sum;
           }
         }
-      }
+        if constexpr (t % Q == 0) gb[t / Q] = fold_states<Q>(sum_b), ga[t / Q] = fold_states<Q>(sum_a), ys[t / Q] = fold_states<Q>(sum_y);
+        if constexpr (t % 4 == 0) {
+          st = st_next, u = u_next, vt = vt_next;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      });
       float dskip_tile = 0.0f, dbias_tile = 0.0f;
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
-        float vb[Q], va[Q], vy[Q];
-#pragma unroll
-        for (int j = 0; j < Q; ++j) vb[j] = sum_b[i * Q + j], va[j] = sum_a[i * Q + j], vy[j] = sum_y[i * Q + j];
-        const float gb = fold_states<Q>(vb), ga = fold_states<Q>(va) * (1.0f / kLog2E);
-        const float y = pz ? __builtin_fmaf(skip, xs[i], fold_states<Q>(vy)) : 0.0f;
-        const float ddt = __builtin_fmaf(xs[i], gb, ga) * slope[i];
-        if (s.valid && t0 + s.q + Q * i < end) {
-          const long long at = plane + (t0 + s.q + Q * i) * p.channels;
-          if (p.dx) static_cast<T*>(p.dx)[at] = from_f32<T>(__builtin_fmaf(ss[i], gb, skip * vs[i]));
-          if (p.ddt) static_cast<T*>(p.ddt)[at] = from_f32<T>(ddt);
-          if (p.dz) static_cast<T*>(p.dz)[at] = from_f32<T>(zs[i] * y);
-          dskip_tile = __builtin_fmaf(vs[i], xs[i], dskip_tile);
-          dbias_tile += ddt;
-        }
+        const int at = s.c * kPlaneRow + s.q + Q * i;
+        const float xi = lx[at], vi = lv[at];
+        ys[i] = lz[at] * __builtin_fmaf(skip, xi, ys[i]);
+        ga[i] = __builtin_fmaf(xi, gb[i], ga[i] * (1.0f / kLog2E)) * lslope[at];
+        gb[i] = __builtin_fmaf(ls[at], gb[i], skip * vi);
+        dskip_tile = __builtin_fmaf(vi, xi, dskip_tile);
+        dbias_tile += live(i) ? ga[i] : 0.0f;
       }
       // (a tile's terms by themselves first: long sums keep their last bits)
       dskip += dskip_tile;
       dbias += dbias_tile;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) da.v[r] += da_tile.v[r];
-      if (p.shared_parts) {
-        __syncthreads();
-        const long long part = s.tile / kWaves;
-        float* const to = p.shared_parts + ((part * p.batch + s.row) * p.tokens + t0) * p.groups * 8 * Q + s.group * 8 * Q;
-        for (int i = threadIdx.x; i < kScanTile * 8 * Q; i += 64 * kWaves) {
-          if (t0 + i / (8 * Q) >= end) break;
-          float sum = 0.0f;
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) sum += shares[w][i];
-          to[(long long)(i / (8 * Q)) * p.groups * 8 * Q + i % (8 * Q)] = sum;
-        }
-        __syncthreads();
-      }
+      for (int r = 0; r < R; ++r) da.v[r] += da_tile.v[r];
+      turn ^= 1;
     }
   }
+  if (!SUM && last >= seg_begin) results(seg_begin);
   if (SUM) {
-    reinterpret_cast<Four32*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane] = carry;
+    reinterpret_cast<States<R>*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane] = carry;
     p.seg_steps[(s.seg * s.units + s.unit) * 64 + s.lane] = sum_states<Q>(steps);
     return;
   }
-  if (idle) return;
-  if (s.valid)
-    for (long long t = max(end, seg_begin) + s.q; t < seg_end; t += Q) {
-      const long long at = plane + t * p.channels;
-      if (p.dx) static_cast<T*>(p.dx)[at] = T(0);
-      if (p.ddt) static_cast<T*>(p.ddt)[at] = T(0);
-      if (p.dz) static_cast<T*>(p.dz)[at] = T(0);
-    }
+  if (s.idle) return;
+  for (void* const out : {p.dx, p.ddt, p.dz})
+    if (out) zero_tokens<T, Q>(static_cast<T*>(out) + plane, p.channels, s, max(end, seg_begin), seg_end);
   if (p.dstate_in && s.seg == 0)
-    store_states(p.dstate_in + (s.row * p.channels + s.channel) * p.n, p.n, s.q, s.valid, carry);
+    store_states<R>(p.dstate_in + (s.row * p.channels + channel) * p.n, p.n, s.q, s.valid, carry);
   if (p.channel_parts) {
-    // (seg, unit, lane): four of da, then dd and ddt_bias
+    // (seg, unit, lane): those of da, then dd and ddt_bias
     const long long at = (s.seg * s.units + s.unit) * 64 + s.lane, all = p.segments * s.units * 64;
-    reinterpret_cast<Four32*>(p.channel_parts)[at] = da;
-    p.channel_parts[4 * all + at] = sum_states<Q>(dskip);
-    p.channel_parts[5 * all + at] = sum_states<Q>(dbias);
+    reinterpret_cast<States<R>*>(p.channel_parts)[at] = da;
+    p.channel_parts[R * all + at] = sum_states<Q>(dskip);
+    p.channel_parts[(R + 1) * all + at] = sum_states<Q>(dbias);
   }
 }
 
 enum ScanMode { kScanSums, kScanForward, kScanBackSums, kScanBackward };
 
-template <typename T, int Q>
+template <typename T, int Q, int R>
 hipError_t scan_launch(const ScanArgs& p, ScanMode mode) {
   const int waves = mode == kScanBackSums || mode == kScanBackward ? kBackWaves<Q> : kScanWaves;
   const long long tiles = (p.channels / p.groups + 64 / Q - 1) / (64 / Q);
   const long long blocks = (tiles + waves - 1) / waves * p.groups * p.batch * p.segments;
   for (long long first = 0; first < blocks; first += max_blocks(64 * waves)) {
     const dim3 grid((unsigned)std::min(blocks - first, max_blocks(64 * waves))), block(64 * waves);
-    if (mode == kScanSums) hipLaunchKernelGGL((scan_forward_kernel<T, Q, false>), grid, block, 0, p.stream, p, first);
-    if (mode == kScanForward) hipLaunchKernelGGL((scan_forward_kernel<T, Q, true>), grid, block, 0, p.stream, p, first);
-    if (mode == kScanBackSums) hipLaunchKernelGGL((scan_backward_kernel<T, Q, true>), grid, block, 0, p.stream, p, first);
-    if (mode == kScanBackward) hipLaunchKernelGGL((scan_backward_kernel<T, Q, false>), grid, block, 0, p.stream, p, first);
+    if (mode == kScanSums) hipLaunchKernelGGL((scan_forward_kernel<T, Q, R, false>), grid, block, 0, p.stream, p, first);
+    if (mode == kScanForward) hipLaunchKernelGGL((scan_forward_kernel<T, Q, R, true>), grid, block, 0, p.stream, p, first);
+    if (mode == kScanBackSums) hipLaunchKernelGGL((scan_backward_kernel<T, Q, R, true>), grid, block, 0, p.stream, p, first);
+    if (mode == kScanBackward) hipLaunchKernelGGL((scan_backward_kernel<T, Q, R, false>), grid, block, 0, p.stream, p, first);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }
 
-// lanes of a channel
-inline int scan_lanes(int n) { return n <= 4 ? 1 : n <= 8 ? 2 : n <= 16 ? 4 : n <= 32 ? 8 : 16; }
+// Lanes of a channel, and the states that each has
+struct ScanShape {
+  int lanes, each;
+};
+inline ScanShape scan_shape(int n) {
+  return n <= 4 ? ScanShape{4, 1} : n <= 8 ? ScanShape{4, 2} : n <= 16 ? ScanShape{4, 4} : n <= 32 ? ScanShape{8, 4} : ScanShape{16, 4};
+}
 
 template <typename T>
 hipError_t scan_typed(const ScanArgs& p, ScanMode mode) {
-  switch (scan_lanes(p.n)) {
-    case 1: return scan_launch<T, 1>(p, mode);
-    case 2: return scan_launch<T, 2>(p, mode);
-    case 4: return scan_launch<T, 4>(p, mode);
-    case 8: return scan_launch<T, 8>(p, mode);
-  }
-  return scan_launch<T, 16>(p, mode);
+  const ScanShape s = scan_shape(p.n);
+  if (s.lanes == 4 && s.each == 1) return scan_launch<T, 4, 1>(p, mode);
+  if (s.lanes == 4 && s.each == 2) return scan_launch<T, 4, 2>(p, mode);
+  if (s.lanes == 4) return scan_launch<T, 4, 4>(p, mode);
+  return s.lanes == 8 ? scan_launch<T, 8, 4>(p, mode) : scan_launch<T, 16, 4>(p, mode);
 }
 
 hipError_t scan_f32(const ScanArgs& p, ScanMode mode);

@@ -94,6 +94,13 @@ void scan_inputs(P& p, const tfa_scan_desc* d, const ScanInputs& in) {
   p.b_sb = rows ? d->b_stride[0] : 0, p.c_sb = rows ? d->c_stride[0] : 0;
   p.b_sg = groups ? d->b_stride[2] : 0, p.c_sg = groups ? d->c_stride[2] : 0;
 }
+// (a lane's own part of an address has 32 bits: tokens of a tile are less than 2^32 bytes apart)
+int check_token_strides(const tfa_scan_desc* d) {
+  if (d->tokens < 2) return TFA_OK;
+  for (const int64_t st : {d->x_stride[1], d->dt_stride[1], d->z_stride[1], d->b_stride[1], d->c_stride[1], (int64_t)d->channels})
+    if (st < 0 || st >= 1 << 24) return set_error(TFA_ERR_UNSUPPORTED, "token strides must be from 0 to 2^24 - 1 elements");
+  return TFA_OK;
+}
 void scan_tokens(tfa::ScanArgs& p, const tfa_scan_desc* d) {
   const bool many = d->tokens > 1;
   p.x_st = many ? d->x_stride[1] : 0, p.dt_st = many ? d->dt_stride[1] : 0, p.z_st = many ? d->z_stride[1] : 0;
@@ -212,6 +219,7 @@ int tfa_selective_scan(const tfa_scan_desc* desc, const void* x, const void* dt,
                        const float* d, const void* z, const float* dt_bias, const int64_t* lengths, const float* state_in,
                        void* y, float* state_out, void* kept, void* workspace, tfa_stream stream) {
   if (const int rc = check_scan(desc)) return rc;
+  if (const int rc = check_token_strides(desc)) return rc;
   if (desc->batch == 0) return TFA_OK;
   if (!a || (desc->tokens > 0 && (!x || !dt || !b || !c || !y))) return set_error(TFA_ERR_INVALID, "null data pointer");
   if (state_out && state_out == state_in) return set_error(TFA_ERR_INVALID, "state_out must not be state_in");
@@ -234,6 +242,7 @@ int tfa_selective_scan_backward(const tfa_scan_desc* desc, const void* x, const 
                                 const float* state_in, const void* kept, const tfa_scan_grads* grads, void* workspace,
                                 tfa_stream stream) {
   if (const int rc = check_scan(desc)) return rc;
+  if (const int rc = check_token_strides(desc)) return rc;
   if (!grads) return set_error(TFA_ERR_INVALID, "null gradients");
   const tfa_scan_grads& g = *grads;
   const bool some = desc->batch > 0 && desc->tokens > 0;

@@ -54,6 +54,12 @@ def _dense(g: torch.Tensor | None, dev: torch.device) -> torch.Tensor | None:
     return None if g is None else _on(g, dev).contiguous()
 
 
+def _tokens(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """x on dev with contiguous channels and frames less than 2^24 values apart (x itself where it is so)."""
+    x = _features(x, dev)
+    return x if x.stride(1) < 1 << 24 or x.shape[1] == 1 else x.contiguous()
+
+
 def _check_state(what: str, state: torch.Tensor) -> torch.device:
     """The device of a state that is updated in place."""
     if not state.is_cuda or not state.is_contiguous() or state.is_neg():
@@ -293,8 +299,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     refuse_tangents(what, x, dt, a, b, c, d, z, dt_bias, initial_state)
     _require_hip(what)
     dev, out_dev = target_device(x, dt, b, c), x.device
-    x, dt, b, c = _features(x, dev), _features(dt, dev), _features(b, dev), _features(c, dev)
-    z = None if z is None else _features(z, dev)
+    x, dt, b, c = _tokens(x, dev), _tokens(dt, dev), _tokens(b, dev), _tokens(c, dev)
+    z = None if z is None else _tokens(z, dev)
     a, d, dt_bias = _dense(a, dev), _channels(d, dev), _channels(dt_bias, dev)
     state, lengths = _dense(initial_state, dev), _whole_numbers(lengths, dev)
     if _wants(x, dt, a, b, c, d, z, dt_bias, state):
