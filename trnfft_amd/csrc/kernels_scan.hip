@@ -20,10 +20,11 @@ __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, int lanes, b
   const float* from = reverse ? p.dstate_out : p.state_in;
   States<R> s = {};
   if (from) s = load_states<R>(from + (row * p.channels + channel) * p.n, p.n, q, valid);
-  for (int k = 0; k < p.segments; ++k) {
+  for (int k = 0; k < p.segments; ++k) {  // (the last one's sums are not there, and nothing comes behind it)
     const long long at = ((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane;
-    const States<R> sum = reinterpret_cast<States<R>*>(p.seg_state)[at];
-    const float steps = p.seg_steps[at] * kLog2E;
+    const bool last = k + 1 == p.segments;
+    const States<R> sum = last ? States<R>{} : reinterpret_cast<States<R>*>(p.seg_state)[at];
+    const float steps = last ? 0.0f : p.seg_steps[at] * kLog2E;
     reinterpret_cast<States<R>*>(p.seg_state)[at] = s;
 #pragma unroll
     for (int r = 0; r < R; ++r) s.v[r] = __builtin_fmaf(__builtin_amdgcn_exp2f(steps * a.v[r]), s.v[r], sum.v[r]);

@@ -105,7 +105,7 @@ struct ScanTokens {
       for (int i = 0; i < kScanTile / Q; ++i) v[i] = *lane_address(p + i * Q * st, at);
     } else {
 #pragma unroll
-      for (int i = 0; i < kScanTile / Q; ++i) v[i] = *lane_address(p, (min(s.q + Q * i, left - 1) * (unsigned)st + s.own) * (unsigned)sizeof(T));
+      for (int i = 0; i < kScanTile / Q; ++i) v[i] = *lane_address(p, (__umul24(min(s.q + Q * i, left - 1), st) + s.own) * (unsigned)sizeof(T));
       // (keeps the compiler from making one load of both ways' with an address in 64 bits of registers)
       asm volatile("");
     }
@@ -136,7 +136,7 @@ struct ScanRows {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
       const int k = state(lane, i);
-      const unsigned at = (left >= kScanTile ? token(lane, i) : min(token(lane, i), left - 1)) * (unsigned)st;
+      const unsigned at = __umul24(min(token(lane, i), left - 1), st);
       if (whole) {
         typedef typename WordsOf<kBytes>::Type Words;
         const Words v = *reinterpret_cast<const Words*>(lane_address(p, (at + min(k, n - R)) * (unsigned)sizeof(T)));
@@ -173,11 +173,16 @@ struct ScanBank {
   States<R> own;
   template <typename T>
   __device__ __forceinline__ void put(const ScanRows<T, Q, R>& rows, float* lds, int n, int lane, int left) {
+    const bool all = n == Q * R && left == kScanTile;
 #pragma unroll
     for (int i = 0; i < rows.kParts; ++i) {
-      const int t = rows.token(lane, i), k = rows.state(lane, i);
 #pragma unroll
-      for (int r = 0; r < R; ++r) own.v[r] = k + r < n && t < left ? rows.value(i, r) : 0.0f;
+      for (int r = 0; r < R; ++r) own.v[r] = rows.value(i, r);
+      if (!all) {
+        const int t = rows.token(lane, i), k = rows.state(lane, i);
+#pragma unroll
+        for (int r = 0; r < R; ++r) own.v[r] = k + r < n && t < left ? own.v[r] : 0.0f;
+      }
       if (Q > 4) *reinterpret_cast<States<R>*>(lds + R * (lane + 64 * i)) = own;
     }
   }
@@ -266,18 +271,21 @@ __device__ __forceinline__ long long scan_end(const ScanArgs& p, long long row) 
 }
 __device__ __forceinline__ long long kept_states(const ScanArgs& p) { return p.tokens > 0 ? (p.tokens - 1) / kScanStretch : 0; }
 
-// a tile's own steps s_t, zeros where they are not live, and their slopes by dt_t
-template <typename T, int Q, typename L>
-__device__ __forceinline__ void steps_of(const ScanTokens<T, Q>& dt, float bias, bool soft, L live, float (&step)[kScanTile / Q],
-                                         float (&slope)[kScanTile / Q]) {
+// a tile's own steps s_t and their slopes by dt_t
+template <typename T, int Q>
+__device__ __forceinline__ void steps_of(const ScanTokens<T, Q>& dt, float bias, bool soft, float (&step)[kScanTile / Q], float (&slope)[kScanTile / Q]) {
 #pragma unroll
   for (int i = 0; i < kScanTile / Q; ++i) step[i] = to_f32(dt.v[i]) + bias, slope[i] = 1.0f;
   if (soft) {
 #pragma unroll
     for (int i = 0; i < kScanTile / Q; ++i) step[i] = softplus(step[i], slope[i]);
   }
+}
+// zeros in the tokens past the end and the channels past the last, which take no part in anything that is shared
+template <int Q>
+__device__ __forceinline__ void clear_dead(const ScanPlace<Q>& s, int left, float (&v)[kScanTile / Q]) {
 #pragma unroll
-  for (int i = 0; i < kScanTile / Q; ++i) step[i] = live(i) ? step[i] : 0.0f;
+  for (int i = 0; i < kScanTile / Q; ++i) v[i] = s.valid && s.q + Q * i < left ? v[i] : 0.0f;
 }
 // The same tokens to a contiguous (batch, tokens, channels) operand; p as above; all: the wave has all of its channels and tokens.
 template <typename T, int Q>
@@ -355,17 +363,18 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
   for (long long t0 = seg_begin; t0 < end; t0 += kScanTile) {
     if (OUT && kept && t0 > 0) *lane_address(kept + (t0 / kScanStretch - 1) * 64, s.lane * (unsigned)sizeof(h)) = h;
     const int left = tile_left(end, t0);
-    const auto live = [&](int i) { return s.valid && s.q + Q * i < left; };
+    const bool full = all_valid && left == kScanTile;
     float xs[kOwn], zs[kOwn], own[kOwn], slope[kOwn];
-    steps_of<T, Q>(dt, bias, p.softplus, live, own, slope);
+    steps_of<T, Q>(dt, bias, p.softplus, own, slope);
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) xs[i] = to_f32(x.v[i]), zs[i] = 1.0f;
+    if (!full) clear_dead<Q>(s, left, own), clear_dead<Q>(s, left, xs);
     wave_order();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      xs[i] = to_f32(x.v[i]);
       put_token<Q>(ls, s.q, s.c, i, own[i]);
-      put_token<Q>(lu, s.q, s.c, i, live(i) ? own[i] * xs[i] : 0.0f);
-      steps += own[i];
-      zs[i] = 1.0f;
+      put_token<Q>(lu, s.q, s.c, i, own[i] * xs[i]);
+      if (!OUT) steps += own[i];
     }
     ScanBank<Q, R> bs, cs;
     bs.put(b, lb, p.n, s.lane, left);
@@ -426,7 +435,8 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
   __shared__ float rows[kWaves][2][kBankWords<Q, R>];
   __shared__ float planes[kWaves][SUM ? 2 : 6][kPlaneWords<Q>];
   __shared__ float shares[2][SUM ? 1 : kWaves][SUM ? 1 : kScanTile * 2 * Q * R];  // of this tile and the one before
-  const ScanPlace<Q> s = scan_place<Q>(p, first_block + blockIdx.x, kWaves);
+  ScanPlace<Q> s = scan_place<Q>(p, first_block + blockIdx.x, kWaves);
+  if (SUM) ++s.seg;  // (nothing comes before the first segment)
   if (SUM && s.idle) return;  // (else it takes part in the barriers)
   float *const lb = rows[s.wave][0], *const lc = rows[s.wave][1];
   // of every channel and token: s, dy silu(z), s x, and what its own lane needs again: x, the slope of s by dt, dy silu'(z)
@@ -500,10 +510,9 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
   if (last >= seg_begin) fetch(last);
   for (long long t0 = last; t0 >= seg_begin; t0 -= kScanTile) {
     const int left = tile_left(end, t0);
-    // (channels past the last and tokens past the end take no part in anything that is shared)
-    const auto live = [&](int i) { return s.valid && s.q + Q * i < left; };
-    float own[kOwn], slope[kOwn], vs[kOwn], zs[kOwn];
-    steps_of<T, Q>(dt, bias, p.softplus, live, own, slope);
+    const bool full = all_valid && left == kScanTile;
+    float xs[kOwn], own[kOwn], slope[kOwn], vs[kOwn], zs[kOwn];
+    steps_of<T, Q>(dt, bias, p.softplus, own, slope);
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) vs[i] = to_f32(dy.v[i]), zs[i] = 0.0f;
     if (pz) {
@@ -514,17 +523,19 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
         vs[i] *= zi * gate;
       }
     }
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) xs[i] = SUM ? 0.0f : to_f32(x.v[i]);
+    if (!full) clear_dead<Q>(s, left, own), clear_dead<Q>(s, left, vs), clear_dead<Q>(s, left, xs), clear_dead<Q>(s, left, slope);
     wave_order();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       put_token<Q>(ls, s.q, s.c, i, own[i]);
-      put_token<Q>(lv, s.q, s.c, i, live(i) ? vs[i] : 0.0f);
+      put_token<Q>(lv, s.q, s.c, i, vs[i]);
       if (SUM) {
         steps += own[i];
       } else {
-        const float xi = live(i) ? to_f32(x.v[i]) : 0.0f;
-        put_token<Q>(lu, s.q, s.c, i, own[i] * xi);
-        put_token<Q>(lx, s.q, s.c, i, xi);
+        put_token<Q>(lu, s.q, s.c, i, own[i] * xs[i]);
+        put_token<Q>(lx, s.q, s.c, i, xs[i]);
         put_token<Q>(lslope, s.q, s.c, i, slope[i]);
         put_token<Q>(lz, s.q, s.c, i, zs[i]);
       }
@@ -626,7 +637,7 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
         ga[i] = __builtin_fmaf(xi, gb[i], ga[i] * (1.0f / kLog2E)) * lslope[at];
         gb[i] = __builtin_fmaf(ls[at], gb[i], skip * vi);
         dskip_tile = __builtin_fmaf(vi, xi, dskip_tile);
-        dbias_tile += live(i) ? ga[i] : 0.0f;
+        dbias_tile += ga[i];  // (where there is no token or channel the slope is 0)
       }
       // (a tile's terms by themselves first: long sums keep their last bits)
       dskip += dskip_tile;
@@ -662,7 +673,9 @@ template <typename T, int Q, int R>
 hipError_t scan_launch(const ScanArgs& p, ScanMode mode) {
   const int waves = mode == kScanBackSums || mode == kScanBackward ? kBackWaves<Q> : kScanWaves;
   const long long tiles = (p.channels / p.groups + 64 / Q - 1) / (64 / Q);
-  const long long blocks = (tiles + waves - 1) / waves * p.groups * p.batch * p.segments;
+  // (the last segment's sums are not needed, nor are the first's backwards)
+  const int segments = mode == kScanSums || mode == kScanBackSums ? p.segments - 1 : p.segments;
+  const long long blocks = (tiles + waves - 1) / waves * p.groups * p.batch * segments;
   for (long long first = 0; first < blocks; first += max_blocks(64 * waves)) {
     const dim3 grid((unsigned)std::min(blocks - first, max_blocks(64 * waves))), block(64 * waves);
     if (mode == kScanSums) hipLaunchKernelGGL((scan_forward_kernel<T, Q, R, false>), grid, block, 0, p.stream, p, first);
