@@ -20,14 +20,27 @@ __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, int lanes, b
   const float* from = reverse ? p.dstate_out : p.state_in;
   States<R> s = {};
   if (from) s = load_states<R>(from + (row * p.channels + channel) * p.n, p.n, q, valid);
-  for (int k = 0; k < p.segments; ++k) {  // (the last one's sums are not there, and nothing comes behind it)
-    const long long at = ((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane;
-    const bool last = k + 1 == p.segments;
-    const States<R> sum = last ? States<R>{} : reinterpret_cast<States<R>*>(p.seg_state)[at];
-    const float steps = last ? 0.0f : p.seg_steps[at] * kLog2E;
-    reinterpret_cast<States<R>*>(p.seg_state)[at] = s;
+  // eight segments' sums on their way at a time (the last one's are not there, and nothing comes behind it)
+  constexpr int U = 8;
+  for (int k0 = 0; k0 < p.segments; k0 += U) {
+    States<R> sum[U];
+    float steps[U];
 #pragma unroll
-    for (int r = 0; r < R; ++r) s.v[r] = __builtin_fmaf(__builtin_amdgcn_exp2f(steps * a.v[r]), s.v[r], sum.v[r]);
+    for (int i = 0; i < U; ++i) {
+      const int k = k0 + i;
+      const long long at = ((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane;
+      const bool there = k + 1 < p.segments;
+      sum[i] = there ? reinterpret_cast<const States<R>*>(p.seg_state)[at] : States<R>{};
+      steps[i] = there ? p.seg_steps[at] * kLog2E : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = k0 + i;
+      if (k >= p.segments) break;
+      reinterpret_cast<States<R>*>(p.seg_state)[((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane] = s;
+#pragma unroll
+      for (int r = 0; r < R; ++r) s.v[r] = __builtin_fmaf(__builtin_amdgcn_exp2f(steps[i] * a.v[r]), s.v[r], sum[i].v[r]);
+    }
   }
 }
 

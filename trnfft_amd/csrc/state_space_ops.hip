@@ -63,9 +63,14 @@ int check_scan(const tfa_scan_desc* d) {
   return TFA_OK;
 }
 
-// A sequence is cut into segments where its rows and channels alone leave the vector units idle: about kWantWaves waves in all,
-// segments of at least kSegTokens.
-constexpr int64_t kWantWaves = 2048, kSegTokens = 256;
+// A sequence is cut into segments where its rows and channels alone leave the vector units idle, at a cost: the segments' sums are 0.6 (forward)
+// and 0.25 (backward) of the pass itself.  Forward below 1024 waves into segments that make about 4096, backward below 2048 into
+// such that make 2048 (a wave takes half of a SIMD's registers there), at most 64 of at least 64 tokens, of sequences of at least 256.
+// 16 states, bf16: 8 x 4096 tokens of 2048 channels (1024 waves) forward 505 us whole, 533 in 2 segments, 505 in 4; backward 1340 whole, 1110 in 2,
+// 1142 in 4.  64 x 626 of 512 (2048 waves) 92 whole, 122 in 2.  1 x 65536 of 1024 (64 waves) 753 in 16, 544 in 32, 491 in 64.
+// 1 x 16384 of 256 (16 waves) 83 in 64, 131 in 256.  1 x 1000 of 512 73 in 3, 40 in 7, 30 in 15.  1 x 128 of 1024 21 whole, 27 in 2.
+constexpr int64_t kForwardWaves = 1024, kForwardWant = 4096, kBackwardWaves = 2048, kBackwardWant = 2048;
+constexpr int64_t kMostSegments = 64, kSegTokens = 64, kSplitTokens = 256;
 
 tfa::ScanArgs scan_args(const tfa_scan_desc* d, bool backward) {
   tfa::ScanArgs p{};
@@ -74,7 +79,9 @@ tfa::ScanArgs scan_args(const tfa_scan_desc* d, bool backward) {
   p.segments = 1;
   p.seg_tokens = std::max<int64_t>(1, (d->tokens + tfa::kScanStretch - 1) / tfa::kScanStretch) * tfa::kScanStretch;
   if (d->batch == 0) return p;
-  const int64_t waves = tfa::scan_waves(p), want = std::min((kWantWaves + waves - 1) / waves, d->tokens / kSegTokens);
+  const int64_t waves = tfa::scan_waves(p);
+  if (waves >= (backward ? kBackwardWaves : kForwardWaves) || d->tokens < kSplitTokens) return p;
+  const int64_t want = std::min({((backward ? kBackwardWant : kForwardWant) + waves - 1) / waves, d->tokens / kSegTokens, kMostSegments});
   if (want > 1) {
     p.seg_tokens = ((d->tokens + want - 1) / want + tfa::kScanStretch - 1) / tfa::kScanStretch * tfa::kScanStretch;
     p.segments = (int)((d->tokens + p.seg_tokens - 1) / p.seg_tokens);
