@@ -8,15 +8,20 @@
 // norm does not depend on timing.  Memory bound: one reading for the norm, one reading and writing where gradients are scaled.
 #include "model_ops.h"
 
+#include <algorithm>
+
 namespace tfa {
 
 constexpr int kGradTensors = 180;  // per launch: their table travels in the kernel's arguments (4 KB at most)
-constexpr int kGradChunk = 16384;  // values of a workgroup
+// Values of a workgroup: as many as make about kGradBlocks workgroups (small models: no fewer than keep the compute units busy; large ones: the
+// loads of a next batch cover the sums of this one)
+constexpr int kLeastChunk = 4096, kMostChunk = 65536;
+constexpr long long kGradBlocks = 2048;
 
 struct GradTable {
   GradTensor t[kGradTensors];
   unsigned first[kGradTensors];  // first workgroup
-  int count;
+  int count, chunk;
 };
 static_assert(sizeof(GradTable) <= 3900, "kernel arguments");
 
@@ -32,7 +37,7 @@ __device__ __forceinline__ int grad_tensor_of(const GradTable& tab, unsigned blo
   return lo;
 }
 
-// sum over the workgroup's 256 threads, in thread 0
+// sum over the workgroup's 256 threads, in all of them
 __device__ __forceinline__ double block_sum(double x) {
   __shared__ double parts[4];
 #pragma unroll
@@ -42,98 +47,130 @@ __device__ __forceinline__ double block_sum(double x) {
   return parts[0] + parts[1] + parts[2] + parts[3];
 }
 
+// a workgroup's stretch of a tensor: `head` values up to a 16-byte boundary, `vectors` of 16 bytes, and what is left behind them
+template <typename T>
+struct GradStretch {
+  static constexpr int V = 16 / (int)sizeof(T);
+  T* p;
+  int n, head, vectors;
+  __device__ __forceinline__ GradStretch(const GradTable& tab) {
+    const int k = grad_tensor_of(tab, blockIdx.x);
+    const long long base = (long long)(blockIdx.x - tab.first[k]) * tab.chunk;
+    p = static_cast<T*>(tab.t[k].p) + base;
+    n = (int)min((long long)tab.chunk, tab.t[k].n - base);
+    head = min(n, (int)((16 - reinterpret_cast<uintptr_t>(p) % 16) % 16 / sizeof(T)));
+    vectors = (n - head) / V;
+  }
+  // f on every value that is in no vector
+  template <typename F>
+  __device__ __forceinline__ void rest(F f) const {
+    const int behind = head + vectors * V;
+    if ((int)threadIdx.x < head) f(p[threadIdx.x]);
+    if ((int)threadIdx.x < n - behind) f(p[behind + threadIdx.x]);  // (less than a vector)
+  }
+};
+constexpr int kGradBatch = 4;  // vectors of a thread whose loads are on their way together
+
 template <typename T>
 __global__ __launch_bounds__(256) void grad_squares_kernel(GradTable tab, double* parts) {
-  constexpr int V = 16 / sizeof(T);
-  const int k = grad_tensor_of(tab, blockIdx.x);
-  const long long base = (long long)(blockIdx.x - tab.first[k]) * kGradChunk;
-  const T* const p = static_cast<const T*>(tab.t[k].p) + base;
-  const int n = (int)min((long long)kGradChunk, tab.t[k].n - base);
-  double sum = 0.0;
-  if (n == kGradChunk && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-    constexpr int U = 8;
+  constexpr int V = GradStretch<T>::V;
+  const GradStretch<T> s(tab);
+  const Pack<T, V>* const v = reinterpret_cast<const Pack<T, V>*>(s.p + s.head);
+  const auto load = [&](int i, Pack<T, V>(&x)[kGradBatch]) {
 #pragma unroll
-    for (int i = 0; i < kGradChunk; i += U * V * 256) {
-      Pack<T, V> v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const Pack<T, V>*>(p + i + (u * 256 + threadIdx.x) * V);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const double g = to_f32(v[u].v[j]);
-          sum = __builtin_fma(g, g, sum);
-        }
+    for (int u = 0; u < kGradBatch; ++u) {
+      const int at = i + u * 256 + threadIdx.x;
+      x[u] = at < s.vectors ? v[at] : Pack<T, V>{};
     }
-  } else {
-    for (int i = threadIdx.x; i < n; i += 256) {
-      const double g = to_f32(p[i]);
-      sum = __builtin_fma(g, g, sum);
+  };
+  double sum = 0.0;
+  Pack<T, V> x[kGradBatch], next[kGradBatch];
+  load(0, x);
+  for (int i = 0; i < s.vectors; i += kGradBatch * 256) {
+    load(i + kGradBatch * 256, next);
+#pragma unroll
+    for (int u = 0; u < kGradBatch; ++u) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const double g = to_f32(x[u].v[j]);
+        sum = __builtin_fma(g, g, sum);
+      }
+      x[u] = next[u];
     }
   }
+  s.rest([&](const T& value) {
+    const double g = to_f32(value);
+    sum = __builtin_fma(g, g, sum);
+  });
   sum = block_sum(sum);
   if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 
-// out[0] the norm, coef[0] what gradients are multiplied with
-__global__ __launch_bounds__(256) void grad_norm_kernel(const double* parts, long long count, double max_norm, float* norm, float* coef) {
+__device__ __forceinline__ double norm_of_parts(const double* parts, long long count) {
   double sum = 0.0;
+#pragma unroll 8
   for (long long i = threadIdx.x; i < count; i += 256) sum += parts[i];
-  sum = block_sum(sum);
-  if (threadIdx.x == 0) {
-    const double root = sqrt(sum);
-    norm[0] = (float)root;
-    const double c = max_norm / (root + 1e-6);
-    if (coef) coef[0] = c < 1.0 || c != c ? (float)c : 1.0f;  // (a norm that is NaN makes every gradient NaN)
-  }
+  return sqrt(block_sum(sum));
 }
 
+__global__ __launch_bounds__(256) void grad_norm_kernel(const double* parts, long long count, float* norm) {
+  const double root = norm_of_parts(parts, count);
+  if (threadIdx.x == 0) norm[0] = (float)root;
+}
+
+// Every workgroup adds the parts itself, in the same order: one launch less, for some 2000 values out of the caches.
 template <typename T>
-__global__ __launch_bounds__(256) void grad_scale_kernel(GradTable tab, const float* coef) {
-  constexpr int V = 16 / sizeof(T);
-  const float c = coef[0];
-  if (c == 1.0f) return;  // times one: what is there
-  const int k = grad_tensor_of(tab, blockIdx.x);
-  const long long base = (long long)(blockIdx.x - tab.first[k]) * kGradChunk;
-  T* const p = static_cast<T*>(tab.t[k].p) + base;
-  const int n = (int)min((long long)kGradChunk, tab.t[k].n - base);
-  if (n == kGradChunk && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-    constexpr int U = 8;
+__global__ __launch_bounds__(256) void grad_scale_kernel(GradTable tab, const double* parts, long long count, double max_norm, float* norm) {
+  constexpr int V = GradStretch<T>::V;
+  const double root = norm_of_parts(parts, count), ratio = max_norm / (root + 1e-6);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)root;
+  if (ratio >= 1.0) return;  // times one: what is there  (a norm that is NaN makes every gradient NaN)
+  const float c = (float)ratio;
+  const GradStretch<T> s(tab);
+  Pack<T, V>* const v = reinterpret_cast<Pack<T, V>*>(s.p + s.head);
+  for (int i = threadIdx.x; i < s.vectors; i += kGradBatch * 256) {
+    Pack<T, V> x[kGradBatch];
 #pragma unroll
-    for (int i = 0; i < kGradChunk; i += U * V * 256) {
-      Pack<T, V> v[U];
+    for (int u = 0; u < kGradBatch; ++u)
+      if (i + u * 256 < s.vectors) x[u] = v[i + u * 256];
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const Pack<T, V>*>(p + i + (u * 256 + threadIdx.x) * V);
+    for (int u = 0; u < kGradBatch; ++u) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[u].v[j] = from_f32<T>(to_f32(v[u].v[j]) * c);
-        *reinterpret_cast<Pack<T, V>*>(p + i + (u * 256 + threadIdx.x) * V) = v[u];
-      }
+      for (int j = 0; j < V; ++j) x[u].v[j] = from_f32<T>(to_f32(x[u].v[j]) * c);
+      if (i + u * 256 < s.vectors) v[i + u * 256] = x[u];
     }
-  } else {
-    for (int i = threadIdx.x; i < n; i += 256) p[i] = from_f32<T>(to_f32(p[i]) * c);
   }
+  s.rest([&](T& value) { value = from_f32<T>(to_f32(value) * c); });
 }
 
-static long long chunks_of(const GradTensor& t) { return (t.n + kGradChunk - 1) / kGradChunk; }
-
-long long grad_parts(const GradLists& g) {
+static int grad_chunk(const GradLists& g) {
   long long total = 0;
   for (int d = 0; d < 3; ++d)
-    for (long long i = 0; i < g.count[d]; ++i) total += chunks_of(g.tensors[d][i]);
-  return total + 1;  // (and the factor)
+    for (long long i = 0; i < g.count[d]; ++i) total += g.tensors[d][i].n;
+  int chunk = kLeastChunk;
+  while (chunk < kMostChunk && total / chunk > kGradBlocks) chunk *= 2;
+  return chunk;
+}
+static long long chunks_of(const GradTensor& t, int chunk) { return (t.n + chunk - 1) / chunk; }
+
+long long grad_parts(const GradLists& g) {
+  const int chunk = grad_chunk(g);
+  long long total = 0;
+  for (int d = 0; d < 3; ++d)
+    for (long long i = 0; i < g.count[d]; ++i) total += chunks_of(g.tensors[d][i], chunk);
+  return std::max(1LL, total);
 }
 
 // f(table, workgroups, workgroups before it) for all tensors of a dtype, as many in a launch as the arguments and the grid hold
 template <typename F>
-static hipError_t each_table(const GradTensor* tensors, long long count, long long& before, F f) {
+static hipError_t each_table(const GradTensor* tensors, long long count, int chunk, long long& before, F f) {
   for (long long i = 0; i < count;) {
     GradTable tab;
     tab.count = 0;
+    tab.chunk = chunk;
     long long blocks = 0;
     while (i < count && tab.count < kGradTensors) {
-      const long long more = chunks_of(tensors[i]);
+      const long long more = chunks_of(tensors[i], chunk);
       if (blocks + more > max_blocks(256)) break;
       if (more) {
         tab.t[tab.count] = tensors[i];
@@ -155,27 +192,28 @@ static hipError_t each_table(const GradTensor* tensors, long long count, long lo
 }
 
 hipError_t launch_grad_norm(const GradLists& g, double* parts, float* norm, bool scale, double max_norm, hipStream_t stream) {
+  const int chunk = grad_chunk(g);
   long long done = 0;
   for (int d = 0; d < 3; ++d) {
-    const hipError_t e = each_table(g.tensors[d], g.count[d], done, [&](const GradTable& tab, unsigned blocks, long long before) {
-      if (d == 0) hipLaunchKernelGGL(grad_squares_kernel<float>, dim3(blocks), dim3(256), 0, stream, tab, parts + before);
-      if (d == 1) hipLaunchKernelGGL(grad_squares_kernel<__bf16>, dim3(blocks), dim3(256), 0, stream, tab, parts + before);
-      if (d == 2) hipLaunchKernelGGL(grad_squares_kernel<_Float16>, dim3(blocks), dim3(256), 0, stream, tab, parts + before);
+    const hipError_t e = each_table(g.tensors[d], g.count[d], chunk, done, [&](const GradTable& tab, unsigned blocks, long long before) {
+      const auto kernel = d == 0 ? grad_squares_kernel<float> : d == 1 ? grad_squares_kernel<__bf16> : grad_squares_kernel<_Float16>;
+      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, tab, parts + before);
     });
     if (e != hipSuccess) return e;
   }
-  float* const coef = scale ? reinterpret_cast<float*>(parts + done) : nullptr;
-  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, stream, parts, done, max_norm, norm, coef);
-  hipError_t e = hipGetLastError();
-  for (int d = 0; d < 3 && scale && e == hipSuccess; ++d) {
-    long long before = 0;
-    e = each_table(g.tensors[d], g.count[d], before, [&](const GradTable& tab, unsigned blocks, long long) {
-      if (d == 0) hipLaunchKernelGGL(grad_scale_kernel<float>, dim3(blocks), dim3(256), 0, stream, tab, coef);
-      if (d == 1) hipLaunchKernelGGL(grad_scale_kernel<__bf16>, dim3(blocks), dim3(256), 0, stream, tab, coef);
-      if (d == 2) hipLaunchKernelGGL(grad_scale_kernel<_Float16>, dim3(blocks), dim3(256), 0, stream, tab, coef);
-    });
+  if (!scale || !done) {
+    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, stream, parts, done, norm);
+    return hipGetLastError();
   }
-  return e;
+  for (int d = 0; d < 3; ++d) {
+    long long before = 0;
+    const hipError_t e = each_table(g.tensors[d], g.count[d], chunk, before, [&](const GradTable& tab, unsigned blocks, long long) {
+      const auto kernel = d == 0 ? grad_scale_kernel<float> : d == 1 ? grad_scale_kernel<__bf16> : grad_scale_kernel<_Float16>;
+      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, tab, parts, done, max_norm, norm);
+    });
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace tfa

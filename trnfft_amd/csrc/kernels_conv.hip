@@ -11,12 +11,16 @@
 #include "activations.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tfa {
 
 // Tokens of a thread's run: as many as leave about kConvThreads threads, the fewer the smaller the call.
-constexpr long long kConvThreads = 128 << 10;
-constexpr int kRunMost = 32;
+constexpr long long kConvThreads = 256 << 10;
+constexpr int kRunMost = 64;
+// Tokens whose loads are on their way together: forward 4 (8 and 2 are the same), backward 2, which leaves registers for more waves (8 x 4096
+// tokens of 2048 bf16 channels and 4 taps: 101 us, 4 tokens 122)
+constexpr int kConvBatch = 4, kConvBackBatch = 2;
 
 __device__ __forceinline__ long long conv_end(const long long* lengths, long long row, long long tokens) {
   return lengths ? min(max(lengths[row], 0LL), tokens) : tokens;
@@ -35,159 +39,210 @@ __device__ __forceinline__ void conv_frame(const T* x, long long st, const T* st
   }
 }
 
+// A workgroup takes `lanes` neighbouring vectors of channels (a power of two) over 256 / lanes runs.
+struct ConvPlace {
+  int vec, lane, slot;
+  long long part, row, t0, t1;
+};
+__device__ __forceinline__ ConvPlace conv_place(long long block, int lanes, int across, long long runs, int run, long long tokens) {
+  ConvPlace s;
+  s.lane = threadIdx.x % lanes;
+  s.slot = threadIdx.x / lanes;
+  s.vec = (int)(block % across) * lanes + s.lane;
+  s.part = block / across;
+  const long long cell = s.part * (256 / lanes) + s.slot;
+  s.row = cell / runs;
+  s.t0 = cell % runs * run;
+  s.t1 = min(s.t0 + run, tokens);
+  return s;
+}
+// The workgroup's filters through LDS: read in their order in memory, by their channels from there (each lane its 16 W V bytes at once
+// touched 64 cache lines an instruction).
+template <int V, int W>
+constexpr int kFilterWords = 64 * (V * W + 1);
+template <int V, int W>
+__device__ __forceinline__ void conv_filters(const ConvArgs& a, int lanes, int first, const ConvPlace& s, float* lds, float (&w)[V][W], float (&b)[V]) {
+  const int count = min(lanes * V, a.channels - first) * W;
+  for (int i = threadIdx.x; i < count; i += 256) lds[i / (V * W) * (V * W + 1) + i % (V * W)] = a.weight[(long long)first * W + i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = min(s.vec * V + i, a.channels - 1);
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[i][j] = lds[min(s.lane, (a.channels - first - 1) / V) * (V * W + 1) + i * W + j];
+    b[i] = a.bias ? a.bias[c] : 0.0f;
+  }
+}
+
 template <typename T, int V, int W>
-__global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a, int vectors, long long runs, int run, long long first) {
-  const long long id = (first + blockIdx.x) * 256 + threadIdx.x;
-  const long long cell = id / vectors, row = cell / runs;
-  if (row >= a.batch) return;
-  const int c = (int)(id % vectors) * V;
-  const long long t0 = cell % runs * run, t1 = min(t0 + run, a.tokens), end = conv_end(a.lengths, row, a.tokens);
-  const T* const x = static_cast<const T*>(a.x) + row * a.x_sb + c;
-  const T* const state = a.state_in ? static_cast<const T*>(a.state_in) + row * (W - 1) * a.channels + c : nullptr;
-  T* const y = static_cast<T*>(a.y) + row * a.tokens * a.channels + c;
-  if (a.state_out && t0 == 0) {  // the last W - 1 frames up to the end
-    T* const out = static_cast<T*>(a.state_out) + row * (W - 1) * a.channels + c;
+__global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a, int vectors, int lanes, int across, long long runs, int run, long long first) {
+  __shared__ float filters[kFilterWords<V, W>];
+  const ConvPlace s = conv_place(first + blockIdx.x, lanes, across, runs, run, a.tokens);
+  float w[V][W], b[V], win[W][V];
+  conv_filters<V, W>(a, lanes, (s.vec - s.lane) * V, s, filters, w, b);
+  if (s.vec >= vectors || s.row >= a.batch) return;
+  const int c = s.vec * V;
+  const long long end = conv_end(a.lengths, s.row, a.tokens), live = min(s.t1, end);
+  const T* const x = static_cast<const T*>(a.x) + s.row * a.x_sb + c;
+  const T* const state = a.state_in ? static_cast<const T*>(a.state_in) + s.row * (W - 1) * a.channels + c : nullptr;
+  T* const y = static_cast<T*>(a.y) + s.row * a.tokens * a.channels + c;
+  if (a.state_out && s.t0 == 0) {  // the last W - 1 frames up to the end
+    T* const out = static_cast<T*>(a.state_out) + s.row * (W - 1) * a.channels + c;
     for (int j = 0; j < W - 1; ++j) {
       float v[V];
       conv_frame<T, V, W>(x, a.x_st, state, a.channels, end + j - (W - 1), v);
       store_pack<T, V>(out + (long long)j * a.channels, v);
     }
   }
-  float w[V][W], b[V], win[W][V];
+  if (s.t0 < live) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) w[i][j] = a.weight[(long long)(c + i) * W + j];
-    b[i] = a.bias ? a.bias[c + i] : 0.0f;
+    for (int j = 0; j < W - 1; ++j) conv_frame<T, V, W>(x, a.x_st, state, a.channels, s.t0 + j - (W - 1), win[j]);
   }
-  const long long live = min(t1, end);
-  if (t0 < live) {
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j) conv_frame<T, V, W>(x, a.x_st, state, a.channels, t0 + j - (W - 1), win[j]);
-  }
-#pragma unroll 4
-  for (long long t = t0; t < live; ++t) {
-    load_pack<T, V>(x + t * a.x_st, win[W - 1]);
+  const auto token = [&](long long t, const Pack<T, V>& u) {
     float z[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      float s = b[i];
+      win[W - 1][i] = to_f32(u.v[i]);
+      float sum = b[i];
 #pragma unroll
-      for (int j = 0; j < W; ++j) s = __builtin_fmaf(w[i][j], win[j][i], s);
-      z[i] = activate(s, a.act);
+      for (int j = 0; j < W; ++j) sum = __builtin_fmaf(w[i][j], win[j][i], sum);
+      z[i] = activate(sum, a.act);
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
     }
     store_pack<T, V>(y + t * a.channels, z);
+  };
+  long long t = s.t0;
+  for (; t + kConvBatch <= live; t += kConvBatch) {
+    Pack<T, V> u[kConvBatch];
+#pragma unroll
+    for (int k = 0; k < kConvBatch; ++k) u[k] = *reinterpret_cast<const Pack<T, V>*>(x + (t + k) * a.x_st);
+#pragma unroll
+    for (int k = 0; k < kConvBatch; ++k) token(t + k, u[k]);
   }
+  for (; t < live; ++t) token(t, *reinterpret_cast<const Pack<T, V>*>(x + t * a.x_st));
   const float none[V] = {};
-  for (long long t = max(t0, live); t < t1; ++t) store_pack<T, V>(y + t * a.channels, none);
+  for (t = max(s.t0, live); t < s.t1; ++t) store_pack<T, V>(y + t * a.channels, none);
 }
 
-// A workgroup: `lanes` vectors of channels (a power of two) by 256 / lanes runs, whose filter gradients are added in LDS.
-// parts: (workgroups along the runs, channels, W + 1)
+// The workgroup's filter gradients are added in LDS.  parts: (workgroups along the runs, channels, W + 1)
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a, int vectors, int lanes, int across, long long runs, int run, long long first) {
-  const long long block = first + blockIdx.x;
-  const int lane = threadIdx.x % lanes, slot = threadIdx.x / lanes, slots = 256 / lanes;
-  const int vec = (int)(block % across) * lanes + lane;
-  const long long part = block / across, cell = part * slots + slot, row = cell / runs;
-  const int c = vec * V;
-  float dw[V][W], db[V];
+  constexpr int kSums = 256 * (V + 1);
+  __shared__ float lds[kSums > kFilterWords<V, W> ? kSums : kFilterWords<V, W>];
+  const ConvPlace s = conv_place(first + blockIdx.x, lanes, across, runs, run, a.tokens);
+  const int head = (s.vec - s.lane) * V;
+  float dw[V][W], db[V], w[V][W], b[V];
+  conv_filters<V, W>(a, lanes, head, s, lds, w, b);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
 #pragma unroll
     for (int j = 0; j < W; ++j) dw[i][j] = 0.0f;
     db[i] = 0.0f;
   }
-  if (vec < vectors && row < a.batch) {
-    const long long t0 = cell % runs * run, t1 = min(t0 + run, a.tokens), end = conv_end(a.lengths, row, a.tokens);
-    const T* const x = static_cast<const T*>(a.x) + row * a.x_sb + c;
-    const T* const state = a.state_in ? static_cast<const T*>(a.state_in) + row * (W - 1) * a.channels + c : nullptr;
-    const T* const dy = static_cast<const T*>(a.dy) + row * a.tokens * a.channels + c;
-    const T* const dlast = a.dstate_out ? static_cast<const T*>(a.dstate_out) + row * (W - 1) * a.channels + c : nullptr;
-    T* const dx = a.dx ? static_cast<T*>(a.dx) + row * a.tokens * a.channels + c : nullptr;
-    T* const dstate = a.dstate_in ? static_cast<T*>(a.dstate_in) + row * (W - 1) * a.channels + c : nullptr;
-    float w[V][W], b[V], win[W][V], dpre[W][V];
+  if (s.vec < vectors && s.row < a.batch) {
+    const int c = s.vec * V;
+    const long long end = conv_end(a.lengths, s.row, a.tokens), live = min(s.t1, end);
+    const T* const x = static_cast<const T*>(a.x) + s.row * a.x_sb + c;
+    const T* const state = a.state_in ? static_cast<const T*>(a.state_in) + s.row * (W - 1) * a.channels + c : nullptr;
+    const T* const dy = static_cast<const T*>(a.dy) + s.row * a.tokens * a.channels + c;
+    const T* const dlast = a.dstate_out ? static_cast<const T*>(a.dstate_out) + s.row * (W - 1) * a.channels + c : nullptr;
+    T* const dx = a.dx ? static_cast<T*>(a.dx) + s.row * a.tokens * a.channels + c : nullptr;
+    T* const dstate = a.dstate_in ? static_cast<T*>(a.dstate_in) + s.row * (W - 1) * a.channels + c : nullptr;
+    float win[W][V], dpre[W][V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int j = 0; j < W; ++j) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        w[i][j] = a.weight[(long long)(c + i) * W + j];
-        dpre[j][i] = 0.0f;
-      }
-      b[i] = a.bias ? a.bias[c + i] : 0.0f;
+      for (int i = 0; i < V; ++i) win[j][i] = dpre[j][i] = 0.0f;
+      if (j < W - 1 && s.t0 + j - (W - 1) < end) conv_frame<T, V, W>(x, a.x_st, state, a.channels, s.t0 + j - (W - 1), win[j]);
     }
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j) {
-      const long long t = t0 + j - (W - 1);
-      if (t < end) {
-        conv_frame<T, V, W>(x, a.x_st, state, a.channels, t, win[j]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) win[j][i] = 0.0f;
-      }
-    }
-    // frame s = t - (W - 1) is complete with dpre_t
-#pragma unroll 2
-    for (long long t = t0; t < t1 + W - 1; ++t) {
-      float g[V];
-      const bool in = t < end;
-      if (in) {
-        load_pack<T, V>(x + t * a.x_st, win[W - 1]);
-        load_pack<T, V>(dy + t * a.channels, g);
-      }
+    // dpre_t of a token before the end; `counts`: one of the run's own, whose filter gradients are its
+    const auto token = [&](const Pack<T, V>& u, const Pack<T, V>& g, auto counts) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float s = b[i];
+        win[W - 1][i] = to_f32(u.v[i]);
+        float sum = b[i];
 #pragma unroll
-        for (int j = 0; j < W; ++j) s = __builtin_fmaf(w[i][j], win[j][i], s);
-        dpre[W - 1][i] = in ? g[i] * activation_slope(s, a.act) : 0.0f;
-        if (in && t < t1) {
+        for (int j = 0; j < W; ++j) sum = __builtin_fmaf(w[i][j], win[j][i], sum);
+        const float d = to_f32(g.v[i]) * activation_slope(sum, a.act);
+        dpre[W - 1][i] = d;
+        if constexpr (counts) {
 #pragma unroll
-          for (int j = 0; j < W; ++j) dw[i][j] = __builtin_fmaf(dpre[W - 1][i], win[j][i], dw[i][j]);
-          db[i] += dpre[W - 1][i];
+          for (int j = 0; j < W; ++j) dw[i][j] = __builtin_fmaf(d, win[j][i], dw[i][j]);
+          db[i] += d;
         }
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
       }
-      const long long s = t - (W - 1);
-      const bool own = s >= t0 || t0 == 0;
-      if (own && (s >= 0 ? dx != nullptr : dstate != nullptr)) {
-        float d[V], last[V];
-        const long long k = s + (W - 1) - end;  // its place in the state at the end
-        const bool kept = dlast && k >= 0 && k < W - 1 && s < end;
-        if (kept) load_pack<T, V>(dlast + k * a.channels, last);
+    };
+    // the gradient of frame t - (W - 1), which is complete with dpre_t; then the next token's place
+    const auto frame = [&](T* to, const float (&more)[V]) {
+      float d[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          d[i] = 0.0f;
+      for (int i = 0; i < V; ++i) {
+        d[i] = more[i];
 #pragma unroll
-          for (int j = 0; j < W; ++j) d[i] = __builtin_fmaf(w[i][j], dpre[W - 1 - j][i], d[i]);
-          if (kept) d[i] += last[i];
-        }
-        store_pack<T, V>(s >= 0 ? dx + s * a.channels : dstate + (s + W - 1) * a.channels, d);
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i)
+        for (int j = 0; j < W; ++j) d[i] = __builtin_fmaf(w[i][j], dpre[W - 1 - j][i], d[i]);
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) dpre[j][i] = dpre[j + 1][i];
+      }
+      if (to) store_pack<T, V>(to, d);
+    };
+    const float none[V] = {};
+    // The first W - 1 tokens complete frames of the run before, or of the state before the first
+    long long t = s.t0;
+    for (; t < live && t < s.t0 + W - 1; ++t) {
+      token(*reinterpret_cast<const Pack<T, V>*>(x + t * a.x_st), *reinterpret_cast<const Pack<T, V>*>(dy + t * a.channels), std::true_type());
+      frame(s.t0 == 0 && dstate ? dstate + t * a.channels : nullptr, none);
+    }
+    for (; t + kConvBackBatch <= live; t += kConvBackBatch) {
+      Pack<T, V> u[kConvBackBatch], g[kConvBackBatch];
+#pragma unroll
+      for (int k = 0; k < kConvBackBatch; ++k) {
+        u[k] = *reinterpret_cast<const Pack<T, V>*>(x + (t + k) * a.x_st);
+        g[k] = *reinterpret_cast<const Pack<T, V>*>(dy + (t + k) * a.channels);
+      }
+#pragma unroll
+      for (int k = 0; k < kConvBackBatch; ++k) {
+        token(u[k], g[k], std::true_type());
+        frame(dx ? dx + (t + k - (W - 1)) * a.channels : nullptr, none);
+      }
+    }
+    // the rest of the run, the W - 1 tokens behind it, and padding
+    for (; t < s.t1 + W - 1; ++t) {
+      if (t < end) {
+        const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(x + t * a.x_st), g = *reinterpret_cast<const Pack<T, V>*>(dy + t * a.channels);
+        if (t < s.t1)
+          token(u, g, std::true_type());
+        else
+          token(u, g, std::false_type());
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) dpre[W - 1][i] = 0.0f;
+      }
+      const long long at = t - (W - 1), k = t - end;  // the frame, and its place in the state at the end
+      float more[V] = {};
+      if (dlast && k >= 0 && k < W - 1) load_pack<T, V>(dlast + k * a.channels, more);
+      T* to = nullptr;
+      if (at >= 0 ? at >= s.t0 : s.t0 == 0) to = at >= 0 ? (dx ? dx + at * a.channels : nullptr) : (dstate ? dstate + (at + W - 1) * a.channels : nullptr);
+      frame(to, more);
     }
   }
   if (!a.dweight && !a.dbias) return;
   // the runs' sums, in their order
-  __shared__ float sums[256][V + 1];
+  const int slots = 256 / lanes;
 #pragma unroll
   for (int j = 0; j <= W; ++j) {
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < V; ++i) sums[threadIdx.x][i] = j < W ? dw[i][j < W ? j : 0] : db[i];
+    for (int i = 0; i < V; ++i) lds[threadIdx.x * (V + 1) + i] = j < W ? dw[i][j < W ? j : 0] : db[i];
     __syncthreads();
     for (int i = threadIdx.x; i < lanes * V; i += 256) {
-      float s = 0.0f;
-      for (int k = 0; k < slots; ++k) s += sums[k * lanes + i / V][i % V];
-      const int channel = (int)(block % across) * lanes * V + i;
-      if (channel < a.channels) a.ws[(part * a.channels + channel) * (W + 1) + j] = s;
+      float sum = 0.0f;
+      for (int k = 0; k < slots; ++k) sum += lds[(k * lanes + i / V) * (V + 1) + i % V];
+      const int channel = head + i;
+      if (channel < a.channels) a.ws[(s.part * a.channels + channel) * (W + 1) + j] = sum;
     }
-    __syncthreads();
   }
 }
 
@@ -196,8 +251,10 @@ __global__ __launch_bounds__(256) void conv_join_kernel(const float* parts, long
   __shared__ float sums[8][32];
   const long long values = (long long)channels * (width + 1), i = (long long)blockIdx.x * 32 + threadIdx.x % 32;
   float s = 0.0f;
-  if (i < values)
+  if (i < values) {
+#pragma unroll 8
     for (long long k = threadIdx.x / 32; k < count; k += 8) s += parts[k * values + i];
+  }
   sums[threadIdx.x / 32][threadIdx.x % 32] = s;
   __syncthreads();
   if (threadIdx.x >= 32 || i >= values) return;
@@ -289,13 +346,12 @@ enum ConvMode { kConvForward, kConvBackward, kConvStep };
 template <ConvMode MODE, typename T, int V, int W>
 static hipError_t conv_width(const ConvArgs& a) {
   const ConvRuns r = conv_runs(a, V);
-  const long long threads = a.batch * r.vectors * (MODE == kConvStep ? 1 : r.runs), blocks = (threads + 255) / 256;
   if constexpr (MODE == kConvForward) {
-    return conv_launches(blocks, [&](long long first, unsigned n) {
-      hipLaunchKernelGGL((conv_forward_kernel<T, V, W>), dim3(n), dim3(256), 0, a.stream, a, r.vectors, r.runs, r.run, first);
+    return conv_launches(r.parts * r.across, [&](long long first, unsigned n) {
+      hipLaunchKernelGGL((conv_forward_kernel<T, V, W>), dim3(n), dim3(256), 0, a.stream, a, r.vectors, r.lanes, r.across, r.runs, r.run, first);
     });
   } else if constexpr (MODE == kConvStep) {
-    return conv_launches(blocks, [&](long long first, unsigned n) {
+    return conv_launches((a.batch * r.vectors + 255) / 256, [&](long long first, unsigned n) {
       hipLaunchKernelGGL((conv_step_kernel<T, V, W>), dim3(n), dim3(256), 0, a.stream, a, r.vectors, first);
     });
   } else {

@@ -93,41 +93,38 @@ def adamw_state_values(codes, scales, out=None) -> list[torch.Tensor]:
 
 
 def _norm_call(what: str, grads: list, max_norm: float | None) -> torch.Tensor:
-    by_type: dict = {}
-    for g in grads:
-        by_type.setdefault(g.dtype, []).append(g)
-    for dtype in by_type:
-        if dtype not in DTYPES:
-            raise TypeError(f"{what}: float32, bfloat16 or float16 gradients expected, got {dtype}")
+    types = {g.dtype for g in grads}
+    if not types <= DTYPES.keys():
+        raise TypeError(f"{what}: float32, bfloat16 or float16 gradients expected, got {(types - DTYPES.keys()).pop()}")
     _require_hip(what)
-    dev = grads[0].device
+    dev, lib = grads[0].device, _lib.lib()
     if dev.type != "cuda":
         raise ValueError(f"{what}: the gradients must be on the GPU")
-    lists = _lib.GradLists()
-    for dtype, own in by_type.items():
-        lists.tensors[DTYPES[dtype]] = _lib.tensor_table()(what, ("gradients",), (own,), (dtype,), dev.index)
+    lists, table = _lib.GradLists(), _lib.tensor_table()
+    for dtype in types:
+        own = grads if len(types) == 1 else [g for g in grads if g.dtype == dtype]
+        lists.tensors[DTYPES[dtype]] = table(what, ("gradients",), (own,), (dtype,), dev.index)
         lists.count[DTYPES[dtype]] = len(own)
     nbytes = ctypes.c_size_t()
-    _lib.check(_lib.lib().tfa_grad_norm_workspace_size(lists, nbytes), what)
+    _lib.check(lib.tfa_grad_norm_workspace_size(lists, nbytes), what)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
     if max_norm is None:
-        launch(what, dev, _lib.lib().tfa_grad_norm, lists, norm.data_ptr(), ws.data_ptr())
+        launch(what, dev, lib.tfa_grad_norm, lists, norm.data_ptr(), ws.data_ptr())
     else:
-        launch(what, dev, _lib.lib().tfa_clip_grads, lists, max_norm, norm.data_ptr(), ws.data_ptr())
+        launch(what, dev, lib.tfa_clip_grads, lists, max_norm, norm.data_ptr(), ws.data_ptr())
         torch.autograd.graph.increment_version(grads)
     return norm
 
 
-@torch.no_grad()
 def grad_norm(grads) -> torch.Tensor:
     """The 2-norm of all values of a list of contiguous GPU tensors (float32, bfloat16, float16, mixed as they come), as a
-    float32 scalar on the GPU.  Squares are summed in 64 bits and in one order: the same gradients give the same norm."""
+    float32 scalar on the GPU, without a gradient.  Squares are summed in 64 bits and in one order: the same gradients give the
+    same norm."""
     grads = list(grads)
     return _norm_call("grad_norm", grads, None) if grads else torch.zeros(())
 
 
-@torch.no_grad()
 def clip_grads(grads, max_norm: float) -> torch.Tensor:
     """Scales a list of contiguous GPU tensors in place by min(1, max_norm / (norm + 1e-6)); returns their norm before, as
     grad_norm does.  Nothing is written where the norm is within the bound.  A norm that is infinite makes zeros of finite gradients
