@@ -171,54 +171,87 @@ __device__ __forceinline__ float sum_lanes(float v) {
   return v;
 }
 
-// Q neighbouring lanes a channel, 4 states each, so that a wave reads and writes its states in one piece.  Memory bound by the states.
-template <typename T, int Q>
-__global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, bool whole, long long first) {
-  const long long id = ((first + blockIdx.x) * 256 + threadIdx.x) / Q, row = id / p.channels;
+// Q neighbouring lanes a channel, 4 states each, so that a wave reads and writes its states in one piece; ROWS streams a thread, whose states
+// are on their way together and for which a, d and dt_bias are read once.  Memory bound by the states.  256 streams of 2048 channels of 16
+// states, bf16: 16.9 us (72 MB); with one stream a thread 19.0, four 19.7, eight 28.0.
+// whole: states and a, b and c can be read by fours
+template <typename T, int Q, int ROWS>
+__global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, bool whole, bool rows_whole, long long first) {
+  const long long id = ((first + blockIdx.x) * 256 + threadIdx.x) / Q, row0 = id / p.channels * ROWS;
   const int q = threadIdx.x % Q;
-  if (row >= p.batch) return;
-  const int channel = (int)(id % p.channels), group = channel / (p.channels / p.groups);
-  float* const state = p.state + (row * p.channels + channel) * p.n;
-  const float* const pa = p.a + (long long)channel * p.n;
-  const T* const pb = static_cast<const T*>(p.b) + row * p.b_sb + group * p.b_sg;
-  const T* const pc = static_cast<const T*>(p.c) + row * p.c_sb + group * p.c_sg;
-  Four32 h, a;
-  if (whole && 4 * q < p.n) {
-    h = *reinterpret_cast<const Four32*>(state + 4 * q);
-    a = *reinterpret_cast<const Four32*>(pa + 4 * q);
-  } else {
-    h = load_states<4>(state, p.n, q, true);
-    a = load_states<4>(pa, p.n, q, true);
-  }
-  const float x = to_f32(static_cast<const T*>(p.x)[row * p.x_sb + channel]);
-  float s = to_f32(static_cast<const T*>(p.dt)[row * p.dt_sb + channel]) + (p.dt_bias ? p.dt_bias[channel] : 0.0f), slope;
-  if (p.softplus) s = softplus(s, slope);
-  const float u = s * x;
-  float y = 0.0f;
+  if (row0 >= p.batch) return;
+  const int channel = (int)(id % p.channels), group = channel / (p.channels / p.groups), k0 = 4 * q;
+  const bool all = whole && k0 < p.n;
+  const auto states_of = [&](const float* at) { return all ? *reinterpret_cast<const Four32*>(at + k0) : load_states<4>(at, p.n, q, true); };
+  const auto rows_of = [&](const void* base, long long at) {
+    const T* const from = static_cast<const T*>(base) + at;
+    Four32 v;
+    if (rows_whole && k0 < p.n) {
+      const Pack<T, 4> u = *reinterpret_cast<const Pack<T, 4>*>(from + k0);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int k = 4 * q + r;
-    if (k >= p.n) continue;
-    h.v[r] = __builtin_fmaf(decay_of(s, a.v[r] * kLog2E), h.v[r], u * to_f32(pb[k]));
-    y = __builtin_fmaf(to_f32(pc[k]), h.v[r], y);
+      for (int r = 0; r < 4; ++r) v.v[r] = to_f32(u.v[r]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v.v[r] = k0 + r < p.n ? to_f32(from[k0 + r]) : 0.0f;
+    }
+    return v;
+  };
+  Four32 h[ROWS], b[ROWS], c[ROWS];
+  float x[ROWS], dt[ROWS], z[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const long long row = min(row0 + i, p.batch - 1);
+    h[i] = states_of(p.state + (row * p.channels + channel) * p.n);
+    b[i] = rows_of(p.b, row * p.b_sb + group * p.b_sg);
+    c[i] = rows_of(p.c, row * p.c_sb + group * p.c_sg);
+    x[i] = to_f32(static_cast<const T*>(p.x)[row * p.x_sb + channel]);
+    dt[i] = to_f32(static_cast<const T*>(p.dt)[row * p.dt_sb + channel]);
+    z[i] = p.z ? to_f32(static_cast<const T*>(p.z)[row * p.z_sb + channel]) : 0.0f;
   }
-  if (whole && 4 * q < p.n)
-    *reinterpret_cast<Four32*>(state + 4 * q) = h;
-  else
-    store_states<4>(state, p.n, q, true, h);
-  y = sum_lanes<Q>(y);
-  if (q) return;
-  if (p.d) y = __builtin_fmaf(p.d[channel], x, y);
-  if (p.z) y *= activate(to_f32(static_cast<const T*>(p.z)[row * p.z_sb + channel]), kActSilu);
-  static_cast<T*>(p.y)[row * p.channels + channel] = from_f32<T>(y);
+  Four32 a = states_of(p.a + (long long)channel * p.n);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) a.v[r] *= kLog2E;
+  const float skip = p.d ? p.d[channel] : 0.0f, bias = p.dt_bias ? p.dt_bias[channel] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const long long row = row0 + i;
+    if (ROWS > 1 && row >= p.batch) break;
+    float s = dt[i] + bias, slope;
+    if (p.softplus) s = softplus(s, slope);
+    const float u = s * x[i];
+    float y = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (k0 + r >= p.n) continue;  // (nothing of what fills a lane up: it may not be finite)
+      h[i].v[r] = __builtin_fmaf(decay_of(s, a.v[r]), h[i].v[r], u * b[i].v[r]);
+      y = __builtin_fmaf(c[i].v[r], h[i].v[r], y);
+    }
+    float* const state = p.state + (row * p.channels + channel) * p.n;
+    if (all)
+      *reinterpret_cast<Four32*>(state + k0) = h[i];
+    else
+      store_states<4>(state, p.n, q, true, h[i]);
+    y = sum_lanes<Q>(y);
+    if (q) continue;
+    y = __builtin_fmaf(skip, x[i], y);
+    if (p.z) y *= activate(z[i], kActSilu);
+    static_cast<T*>(p.y)[row * p.channels + channel] = from_f32<T>(y);
+  }
 }
 
+template <typename T, int Q, int ROWS>
+static hipError_t step_rows(const ScanStep& p) {
+  const bool whole = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.state) | reinterpret_cast<uintptr_t>(p.a)) % 16 == 0;
+  const bool rows = (reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.c)) % (4 * sizeof(T)) == 0 &&
+                    (p.b_sb | p.b_sg | p.c_sb | p.c_sg | p.n) % 4 == 0;
+  return scan_launches((p.batch + ROWS - 1) / ROWS * p.channels * Q, [&](long long first, unsigned n) {
+    hipLaunchKernelGGL((scan_step_kernel<T, Q, ROWS>), dim3(n), dim3(256), 0, p.stream, p, whole, rows, first);
+  });
+}
+// Two streams a thread where that leaves 2048 waves
 template <typename T, int Q>
 static hipError_t step_lanes(const ScanStep& p) {
-  const bool whole = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.state) | reinterpret_cast<uintptr_t>(p.a)) % 16 == 0;
-  return scan_launches(p.batch * p.channels * Q, [&](long long first, unsigned n) {
-    hipLaunchKernelGGL((scan_step_kernel<T, Q>), dim3(n), dim3(256), 0, p.stream, p, whole, first);
-  });
+  return p.batch / 2 * p.channels * Q >= 2048 * 64 ? step_rows<T, Q, 2>(p) : step_rows<T, Q, 1>(p);
 }
 template <typename T>
 static hipError_t step_typed(const ScanStep& p) {

@@ -47,11 +47,28 @@ def _whole_numbers(lengths: torch.Tensor | None, dev: torch.device) -> torch.Ten
 
 
 def _wants(*tensors: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _dense(g: torch.Tensor | None, dev: torch.device) -> torch.Tensor | None:
     return None if g is None else _on(g, dev).contiguous()
+
+
+# A step is a few microseconds of GPU work: operands that are as the kernels take them are passed through with as few questions as that takes.
+def _step_operand(x: torch.Tensor | None, dev: torch.device, index: int) -> torch.Tensor | None:
+    if x is None or (x.get_device() == index and x.stride(-1) == 1 and not x.is_neg()):
+        return x
+    return _features(x, dev)
+
+
+def _step_weights(w: torch.Tensor | None, dev: torch.device, index: int) -> torch.Tensor | None:
+    if w is None or (w.dtype == torch.float32 and w.get_device() == index and w.is_contiguous() and not w.is_neg()):
+        return w
+    return _channels(w, dev)
 
 
 def _tokens(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
@@ -82,7 +99,8 @@ def _check_conv(what: str, x, weight, bias, activation, dims: int) -> None:
         raise ValueError(f"{what}: weight must be (channels, width) for {c} channels, got {tuple(weight.shape)}")
     if weight.dtype not in (torch.float32, x.dtype):
         raise TypeError(f"{what}: weight must be float32 or {x.dtype}, got {weight.dtype}")
-    _check_channels(what, c, x.dtype, bias=bias)
+    if bias is not None:
+        _check_channels(what, c, x.dtype, bias=bias)
     if activation not in ACTIVATIONS:
         raise ValueError(f"{what}: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
 
@@ -184,7 +202,8 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     refuse_tangents(what, x, state, weight, bias)
     _require_hip(what)
     dev, out_dev = _check_state(what, state), x.device
-    x, weight, bias = _features(x, dev), _channels(weight, dev), _channels(bias, dev)
+    at = dev.index
+    x, weight, bias = _step_operand(x, dev, at), _step_weights(weight, dev, at), _step_weights(bias, dev, at)
     desc = _lib.ConvDesc(DTYPES[x.dtype], c, width, ACTIVATIONS[activation], b, 1, x.stride(0), 0)
     y = x.new_empty(b, c)
     launch(what, dev, _lib.lib().tfa_causal_conv_step, desc, addr(x), addr(weight), addr(bias), addr(state), addr(y))
@@ -200,25 +219,26 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
 def _check_scan(what: str, x, dt, a, b, c, d, z, dt_bias, dims: int) -> None:
     if x.dim() != dims:
         raise ValueError(f"{what}: x must have {dims} dimensions, got {x.dim()}")
-    dtype, lead, channels = x.dtype, x.shape[:-1], x.shape[-1]
+    dtype, shape = x.dtype, x.shape
+    lead, channels = shape[:-1], shape[-1]
     if dtype not in DTYPES:
         raise TypeError(f"{what}: float32, bfloat16 or float16 expected, got {dtype}")
     if a.dim() != 2 or a.shape[0] != channels or a.shape[1] < 1 or channels < 1:
         raise ValueError(f"{what}: a must be (channels, states) for {channels} channels, got {tuple(a.shape)}")
     if a.dtype != torch.float32:
         raise TypeError(f"{what}: a must be float32, got {a.dtype}")
-    for name, v in (("dt", dt), ("z", z)):
-        if v is not None and v.shape != x.shape:
-            raise ValueError(f"{what}: {name} must be {tuple(x.shape)} as x, got {tuple(v.shape)}")
-    if b.dim() != dims + 1 or b.shape[:-2] != lead or b.shape[-1] != a.shape[1] or b.shape[-2] < 1 or channels % b.shape[-2]:
+    if dt.shape != shape or (z is not None and z.shape != shape):
+        raise ValueError(f"{what}: dt and z must be {tuple(shape)} as x, got {tuple(dt.shape)} and {None if z is None else tuple(z.shape)}")
+    bs = b.shape
+    if len(bs) != dims + 1 or bs[:-2] != lead or bs[-1] != a.shape[1] or bs[-2] < 1 or channels % bs[-2]:
         raise ValueError(f"{what}: b must be (*{tuple(lead)}, groups, {a.shape[1]}) with groups that divide {channels} channels, "
-                         f"got {tuple(b.shape)}")
-    if c.shape != b.shape:
-        raise ValueError(f"{what}: c must be {tuple(b.shape)} as b, got {tuple(c.shape)}")
-    for name, v in (("dt", dt), ("b", b), ("c", c), ("z", z)):
-        if v is not None and v.dtype != dtype:
-            raise TypeError(f"{what}: {name} must be {dtype} as x, got {v.dtype}")
-    _check_channels(what, channels, dtype, d=d, dt_bias=dt_bias)
+                         f"got {tuple(bs)}")
+    if c.shape != bs:
+        raise ValueError(f"{what}: c must be {tuple(bs)} as b, got {tuple(c.shape)}")
+    if dt.dtype != dtype or b.dtype != dtype or c.dtype != dtype or (z is not None and z.dtype != dtype):
+        raise TypeError(f"{what}: dt, b, c and z must be {dtype} as x")
+    if d is not None or dt_bias is not None:
+        _check_channels(what, channels, dtype, d=d, dt_bias=dt_bias)
 
 
 def _scan_desc(x, dt, b, c, z, softplus: bool) -> _lib.ScanDesc:
@@ -332,9 +352,9 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     refuse_tangents(what, x, dt, a, b, c, state, d, z, dt_bias)
     _require_hip(what)
     dev, out_dev = _check_state(what, state), x.device
-    x, dt, b, c = _features(x, dev), _features(dt, dev), _features(b, dev), _features(c, dev)
-    z = None if z is None else _features(z, dev)
-    a, d, dt_bias = _dense(a, dev), _channels(d, dev), _channels(dt_bias, dev)
+    at = dev.index
+    x, dt, b, c, z = (_step_operand(v, dev, at) for v in (x, dt, b, c, z))
+    a, d, dt_bias = _step_weights(a, dev, at), _step_weights(d, dev, at), _step_weights(dt_bias, dev, at)
     (bs, bg, _), (cs, cg, _) = b.stride(), c.stride()
     desc = _lib.ScanDesc(DTYPES[x.dtype], channels, b.shape[1], a.shape[1], int(bool(softplus)), 0, rows, 1, x.stride(0), 0,
                          dt.stride(0), 0, 0 if z is None else z.stride(0), 0, bs, 0, bg, cs, 0, cg)
