@@ -1,11 +1,14 @@
 """A denoiser on STFT frames that is trained on whole signals and then runs on a stream, frame by frame.
 
     python examples/denoise.py [--steps 60] [--batch 16] [--seconds 2] [--dtype bfloat16] [--state-bits 8]
+                               [--mixer attention] [--max-norm 1]
 
 Signals are synthetic: gliding harmonics in white noise.  Frames-major spectra go through blocks of group norm and linear attention
-with learned decays; a mask per bin comes out and the inverse STFT gives the waveform back.  Training runs whole, ragged
-signals through ``linear_attention`` and its gradient, and steps with ``AdamW``.  Serving keeps one state a
-block and takes each new frame through ``linear_attention_step``; its masks equal those of the whole signal.
+with learned decays, or with ``--mixer state-space`` of group norm and a selective state space layer; a mask per bin comes out and
+the inverse STFT gives the waveform back.  Training runs whole, ragged signals through ``linear_attention`` (``causal_conv`` and
+``selective_scan``) and its gradient, clips the gradients where it is told to, and steps with ``AdamW``.  Serving keeps one state a
+block and takes each new frame through ``linear_attention_step`` (the other layer's steps); its masks equal those of the whole
+signal.
 """
 
 from __future__ import annotations
@@ -23,8 +26,8 @@ if __package__ in (None, ""):
     sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 import trnfft_amd
-from trnfft_amd.nn import GroupNorm
-from trnfft_amd.optim import AdamW
+from trnfft_amd.nn import GroupNorm, StateSpace
+from trnfft_amd.optim import AdamW, clip_grad_norm_
 
 N_FFT, HOP, RATE = 512, 160, 16000
 BINS = N_FFT // 2 + 1
@@ -72,11 +75,37 @@ class Block(nn.Module):
         return self._join(x, trnfft_amd.linear_attention_step(q, k, v, self._log_decay(), state, scale=1.0))
 
 
+    def state(self, streams: int, device) -> torch.Tensor:
+        return torch.zeros(streams, self.heads, self.key_dim, self.value_dim, device=device)
+
+
+class StateSpaceBlock(nn.Module):
+    """The block with a selective state space layer in the attention's place."""
+
+    def __init__(self, features: int):
+        super().__init__()
+        self.norm = FrameNorm(1, features)
+        self.mix = StateSpace(features)
+
+    def forward(self, x: torch.Tensor, lengths: torch.Tensor | None = None) -> torch.Tensor:
+        return x + self.mix(self.norm(x), lengths)
+
+    def step(self, x: torch.Tensor, state) -> torch.Tensor:
+        return x + self.mix.step(self.norm(x), state)
+
+    def state(self, streams: int, device):
+        return self.mix.state(streams, device)
+
+
+MIXERS = ("attention", "state-space")
+
+
 class Denoiser(nn.Module):
-    def __init__(self, features: int = 256, heads: int = 4, key_dim: int = 32, blocks: int = 2):
+    def __init__(self, features: int = 256, heads: int = 4, key_dim: int = 32, blocks: int = 2, mixer: str = "attention"):
         super().__init__()
         self.enter = nn.Linear(BINS, features)
-        self.blocks = nn.ModuleList(Block(features, heads, key_dim) for _ in range(blocks))
+        self.blocks = nn.ModuleList(Block(features, heads, key_dim) if mixer == "attention" else StateSpaceBlock(features)
+                                    for _ in range(blocks))
         self.leave = nn.Linear(features, BINS)
 
     def features(self, spectrum: trnfft_amd.ComplexTensor) -> torch.Tensor:
@@ -90,10 +119,10 @@ class Denoiser(nn.Module):
             x = block(x, lengths)
         return torch.sigmoid(self.leave(x).float())
 
-    def states(self, streams: int, device) -> list[torch.Tensor]:
-        return [torch.zeros(streams, b.heads, b.key_dim, b.value_dim, device=device) for b in self.blocks]
+    def states(self, streams: int, device) -> list:
+        return [b.state(streams, device) for b in self.blocks]
 
-    def step(self, frame: torch.Tensor, states: list[torch.Tensor]) -> torch.Tensor:
+    def step(self, frame: torch.Tensor, states: list) -> torch.Tensor:
         """Masks (streams, bins) of every stream's next frame; the states are updated."""
         x = self.enter(frame)
         for block, state in zip(self.blocks, states):
@@ -130,7 +159,8 @@ def signals(batch: int, length: int, g: torch.Generator, device):
     return clean, clean + 0.5 * torch.randn(batch, length, generator=g, device=device), ends
 
 
-def train(model: Denoiser, steps: int, batch: int, length: int, state_bits: int, seed: int = 0) -> list[float]:
+def train(model: Denoiser, steps: int, batch: int, length: int, state_bits: int, seed: int = 0,
+          max_norm: float | None = None) -> list[float]:
     device = model.enter.weight.device
     g = torch.Generator(device=device).manual_seed(seed)
     optimizer = AdamW(model.parameters(), lr=2e-3, state_bits=state_bits)
@@ -144,6 +174,8 @@ def train(model: Denoiser, steps: int, batch: int, length: int, state_bits: int,
         loss = error.square().mean()
         optimizer.zero_grad()
         loss.backward()
+        if max_norm is not None:
+            clip_grad_norm_(model.parameters(), max_norm)
         optimizer.step()
         losses.append(loss.detach())
     return torch.stack(losses).tolist() if losses else []
@@ -163,11 +195,13 @@ def main() -> None:
     ap.add_argument("--seconds", type=float, default=2.0)
     ap.add_argument("--dtype", choices=("float32", "bfloat16"), default="bfloat16")
     ap.add_argument("--state-bits", type=int, choices=(8, 32), default=8)
+    ap.add_argument("--mixer", choices=MIXERS, default="attention")
+    ap.add_argument("--max-norm", type=float, default=None)
     a = ap.parse_args()
     torch.manual_seed(0)
-    model = Denoiser().to("cuda", getattr(torch, a.dtype))
+    model = Denoiser(mixer=a.mixer).to("cuda", getattr(torch, a.dtype))
     length = int(a.seconds * RATE)
-    losses = train(model, a.steps, a.batch, length, a.state_bits)
+    losses = train(model, a.steps, a.batch, length, a.state_bits, max_norm=a.max_norm)
     if losses:
         print(f"loss {losses[0]:.4f} -> {losses[-1]:.4f} in {a.steps} steps")
     clean, noisy, _ = signals(2, length, torch.Generator(device="cuda").manual_seed(1), torch.device("cuda"))

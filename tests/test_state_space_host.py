@@ -183,3 +183,14 @@ def test_c_entries_refuse_bad_descriptors():
     assert lib.tfa_clip_grads(lists((far, 3)), -1.0, far, far, None) == _lib.TFA_ERR_INVALID
     assert lib.tfa_clip_grads(lists((far, 3), (far + 8, 3)), 1.0, far, far, None) == _lib.TFA_ERR_INVALID  # overlap
     assert b"overlap" in lib.tfa_last_error()
+
+
+def test_the_layer_refuses_sizes_below_one():
+    from trnfft_amd.nn import StateSpace
+
+    for bad in (dict(features=0), dict(features=4, states=0), dict(features=4, width=0), dict(features=4, expand=0),
+                dict(features=4, rank=0)):
+        with pytest.raises(ValueError):
+            StateSpace(**bad)
+    m = StateSpace(20)
+    assert m.rank == 2 and [s.shape for s in m.state(3)] == [(3, 3, 40), (3, 40, 16)]
