@@ -6,9 +6,9 @@ namespace tfa {
 // The states that segments start from, in place of their own sums; reversed, the gradients that they end with.  A thread takes a lane of a
 // wave's states over the segments, one after the other.
 template <int R>
-__global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, int lanes, bool reverse, long long first) {
-  const long long id = (first + blockIdx.x) * 256 + threadIdx.x, unit = id / 64;
-  const int lane = (int)(id % 64), channels = 64 / lanes, q = lane / channels, each = p.channels / p.groups;
+__global__ __launch_bounds__(64) void scan_join_kernel(ScanArgs p, int lanes, bool reverse, long long first) {
+  const long long unit = first + blockIdx.x;
+  const int lane = threadIdx.x, channels = 64 / lanes, q = lane / channels, each = p.channels / p.groups;
   const int tiles = (each + channels - 1) / channels;
   const long long units = p.batch * p.groups * tiles;
   if (unit >= units) return;
@@ -20,18 +20,17 @@ __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, int lanes, b
   const float* from = reverse ? p.dstate_out : p.state_in;
   States<R> s = {};
   if (from) s = load_states<R>(from + (row * p.channels + channel) * p.n, p.n, q, valid);
-  // eight segments' sums on their way at a time (the last one's are not there, and nothing comes behind it)
-  constexpr int U = 8;
+  // sixteen segments' sums on their way at a time (the last one has none, and nothing comes behind it)
+  constexpr int U = 16;
   for (int k0 = 0; k0 < p.segments; k0 += U) {
     States<R> sum[U];
     float steps[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int k = k0 + i;
+      const int k = min(k0 + i, p.segments - 2);
       const long long at = ((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane;
-      const bool there = k + 1 < p.segments;
-      sum[i] = there ? reinterpret_cast<const States<R>*>(p.seg_state)[at] : States<R>{};
-      steps[i] = there ? p.seg_steps[at] * kLog2E : 0.0f;
+      sum[i] = reinterpret_cast<const States<R>*>(p.seg_state)[at];
+      steps[i] = p.seg_steps[at] * kLog2E;
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -54,8 +53,10 @@ __global__ __launch_bounds__(256) void scan_shares_kernel(ScanArgs p, int states
   T* const out = static_cast<T*>(which ? p.dc : p.db);
   if (!out || k >= p.n) return;
   float sum = 0.0f;
-  if (cell % p.tokens < scan_end(p, cell / p.tokens))
+  if (cell % p.tokens < scan_end(p, cell / p.tokens)) {
+#pragma unroll 8
     for (long long i = 0; i < parts; ++i) sum += p.shared_parts[i * cells * width + id];
+  }
   out[(cell * p.groups + group) * p.n + k] = from_f32<T>(sum);
 }
 
@@ -71,6 +72,7 @@ __global__ __launch_bounds__(256) void scan_channels_kernel(ScanArgs p, int lane
   const long long count = p.segments * p.batch, all = count * of_row;
   States<R> da = {};
   float dd = 0.0f, dbias = 0.0f;
+#pragma unroll 4
   for (long long i = 0; i < count; ++i) {
     const long long at = i * of_row + id;
     const States<R> v = reinterpret_cast<const States<R>*>(p.channel_parts)[at];
@@ -84,11 +86,11 @@ __global__ __launch_bounds__(256) void scan_channels_kernel(ScanArgs p, int lane
   if (q == 0 && p.ddt_bias) p.ddt_bias[channel] = dbias;
 }
 
-template <typename F>
+template <int BLOCK = 256, typename F>
 static hipError_t scan_launches(long long threads, F f) {
-  const long long blocks = (threads + 255) / 256;
-  for (long long first = 0; first < blocks; first += max_blocks(256)) {
-    f(first, (unsigned)std::min(blocks - first, max_blocks(256)));
+  const long long blocks = (threads + BLOCK - 1) / BLOCK;
+  for (long long first = 0; first < blocks; first += max_blocks(BLOCK)) {
+    f(first, (unsigned)std::min(blocks - first, max_blocks(BLOCK)));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -127,9 +129,9 @@ static hipError_t scan_segments(const ScanArgs& p, bool reverse) {
   const hipError_t e = scan_mode(p, reverse ? kScanBackSums : kScanSums);
   if (e != hipSuccess) return e;
   const ScanShape s = scan_shape(p.n);
-  return scan_launches(scan_waves(p) * 64, [&](long long first, unsigned n) {
+  return scan_launches<64>(scan_waves(p) * 64, [&](long long first, unsigned n) {
     const auto kernel = s.each == 1 ? scan_join_kernel<1> : s.each == 2 ? scan_join_kernel<2> : scan_join_kernel<4>;
-    hipLaunchKernelGGL(kernel, dim3(n), dim3(256), 0, p.stream, p, s.lanes, reverse, first);
+    hipLaunchKernelGGL(kernel, dim3(n), dim3(64), 0, p.stream, p, s.lanes, reverse, first);
   });
 }
 

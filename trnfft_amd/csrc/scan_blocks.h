@@ -189,17 +189,29 @@ struct ScanBank {
   __device__ __forceinline__ States<R> at(const float* lds, int t, int q) const {
     return *reinterpret_cast<const States<R>*>(lds + (t * Q + q) * R);
   }
-  // with the values of a lane's states at token t: their products with u, those added to sums, and the dot product with x
+  // with the values of a lane's states at tokens t and t + 1: their products with u0 and u1, and the dot products with x0 and x1
   template <int t>
-  __device__ __forceinline__ void products(const float* lds, int q, float u, float (&out)[R]) const {
+  __device__ __forceinline__ void products(const float* lds, int q, float u0, float u1, float (&out0)[R], float (&out1)[R]) const {
     if constexpr (Q == 4) {
-      RowLane<t>::products(own.v, u, out);
+      RowLane<t>::products(own.v, u0, u1, out0, out1);
     } else {
-      const States<R> v = at(lds, t, q);
+      const States<R> v0 = at(lds, t, q), v1 = at(lds, t + 1, q);
 #pragma unroll
-      for (int r = 0; r < R; ++r) out[r] = v.v[r] * u;
+      for (int r = 0; r < R; ++r) out0[r] = v0.v[r] * u0, out1[r] = v1.v[r] * u1;
     }
   }
+  template <int t>
+  __device__ __forceinline__ void dots(const float* lds, int q, const float (&x0)[R], const float (&x1)[R], float& sum0, float& sum1) const {
+    if constexpr (Q == 4) {
+      RowLane<t>::dots(own.v, x0, x1, sum0, sum1);
+    } else {
+      const States<R> v0 = at(lds, t, q), v1 = at(lds, t + 1, q);
+      sum0 = sum1 = 0.0f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) sum0 = __builtin_fmaf(v0.v[r], x0[r], sum0), sum1 = __builtin_fmaf(v1.v[r], x1[r], sum1);
+    }
+  }
+  // token t's products with u, added to sums
   template <int t>
   __device__ __forceinline__ void add(const float* lds, int q, float u, float (&sum)[R]) const {
     if constexpr (Q == 4) {
@@ -210,19 +222,24 @@ struct ScanBank {
       for (int r = 0; r < R; ++r) sum[r] = __builtin_fmaf(v.v[r], u, sum[r]);
     }
   }
-  template <int t>
-  __device__ __forceinline__ float dot(const float* lds, int q, const float (&x)[R]) const {
-    float sum = 0.0f;
-    if constexpr (Q == 4) {
-      sum = RowLane<t>::dot(own.v, x);
-    } else {
-      const States<R> v = at(lds, t, q);
-#pragma unroll
-      for (int r = 0; r < R; ++r) sum = __builtin_fmaf(v.v[r], x[r], sum);
-    }
-    return sum;
-  }
 };
+// g += c_t u, then b_t . g and c_t . h
+template <int t, int Q, int R>
+__device__ __forceinline__ void reverse_token(const ScanBank<Q, R>& b, const float* lb, const ScanBank<Q, R>& c, const float* lc, int q, float u,
+                                              const States<R>& h, States<R>& g, float& sum_b, float& sum_c) {
+  if constexpr (Q == 4) {
+    RowLane<t>::reverse(b.own.v, c.own.v, u, h.v, g.v, sum_b, sum_c);
+  } else {
+    const States<R> bt = b.at(lb, t, q), ct = c.at(lc, t, q);
+    sum_b = sum_c = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      g.v[r] = __builtin_fmaf(ct.v[r], u, g.v[r]);
+      sum_b = __builtin_fmaf(bt.v[r], g.v[r], sum_b);
+      sum_c = __builtin_fmaf(ct.v[r], h.v[r], sum_c);
+    }
+  }
+}
 template <int Q, int R>
 constexpr int kBankWords = Q == 4 ? 1 : 16 * Q * R;
 template <typename T, int R>
@@ -390,14 +407,18 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
     if (t0 + kScanTile < end) fetch(tile_left(end, t0 + kScanTile));
     float part[kScanTile];
     Four32 st, u;
-    for_each<kScanTile>([&](auto index) TFA_INLINE {
-      constexpr int t = index;
-      if constexpr (t % 4 == 0) st = four_tokens(ls, s.c, t / 4), u = four_tokens(lu, s.c, t / 4);
-      float in[R];
-      bs.template products<t>(lb, s.q, u.v[t % 4], in);
+    for_each<kScanTile / 2>([&](auto index) TFA_INLINE {
+      constexpr int t = 2 * index, j = t % 4;
+      if constexpr (j == 0) st = four_tokens(ls, s.c, t / 4), u = four_tokens(lu, s.c, t / 4);
+      float in0[R], in1[R];
+      bs.template products<t>(lb, s.q, u.v[j], u.v[j + 1], in0, in1);
+      States<R> h0 = h;
 #pragma unroll
-      for (int r = 0; r < R; ++r) h.v[r] = __builtin_fmaf(decay_of(st.v[t % 4], a.v[r]), h.v[r], in[r]);
-      if constexpr (OUT) part[t] = cs.template dot<t>(lc, s.q, h.v);
+      for (int r = 0; r < R; ++r) {
+        h0.v[r] = __builtin_fmaf(decay_of(st.v[j], a.v[r]), h.v[r], in0[r]);
+        h.v[r] = __builtin_fmaf(decay_of(st.v[j + 1], a.v[r]), h0.v[r], in1[r]);
+      }
+      if constexpr (OUT) cs.template dots<t>(lc, s.q, h0.v, h.v, part[t], part[t + 1]);
     });
     if (!OUT) continue;
 #pragma unroll
@@ -405,6 +426,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
       float sums[Q];
 #pragma unroll
       for (int j = 0; j < Q; ++j) sums[j] = part[i * Q + j];
+      settle(sums);
       ys[i] = __builtin_fmaf(skip, xs[i], fold_states<Q>(sums)) * zs[i];
     }
   }
@@ -506,6 +528,42 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
       to[(long long)(i / kRow) * p.groups * kRow + i % kRow] = sum;
     }
   };
+  // Sums over the channels of two tokens' shares of db (the first R) and dc: these part at the first level, their states at the next ones.
+  // (Lanes with the same sum write the same bits.)
+  const auto fold_channels = [&](const float(&v)[2][2 * R], int t) TFA_INLINE {
+    float* const to = shares[turn][s.wave] + (2 * t + s.c / (kChannels / 2)) * Q * R + R * s.q;
+    constexpr int kNext = 2 * Q * R;  // from a token to the next
+    if constexpr (R == 4 && kChannels == 16) {
+      const int at = s.c / 4 % 2 * 2 + s.c / 2 % 2;
+      float sum0, sum1;
+      fold_row(v[0], v[1], 0xCCCCCCCCCCCCCCCCull, sum0, sum1);
+      to[at] = sum0;
+      to[kNext + at] = sum1;
+    } else {
+      constexpr int kTop = kChannels / 2 == 4 ? 7 : kChannels / 2, kMid = kChannels / 4 == 4 ? 7 : kChannels / 4;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float w[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) w[r] = fold<kTop>(v[i][r], v[i][R + r]);
+        float* const half = to + i * kNext;
+        if constexpr (R == 1) {
+          half[0] = fold<1>(fold<2>(fold<kMid>(w[0])));
+        } else if constexpr (R == 2) {
+          half[s.c / (kChannels / 4) % 2] = fold<1>(fold<2>(fold<kMid>(w[0], w[1])));
+        } else {
+          const int first = s.c / (kChannels / 4) % 2 * 2;
+          const float x0 = fold<kMid>(w[0], w[2]), x1 = fold<kMid>(w[1], w[3]);
+          if constexpr (kChannels == 4) {
+            half[first] = x0;
+            half[first + 1] = x1;
+          } else {
+            half[first + s.c % 2] = fold<1>(x0, x1);
+          }
+        }
+      }
+    }
+  };
   const long long last = end > seg_begin ? seg_begin + (end - 1 - seg_begin) / kScanTile * kScanTile : seg_begin - kScanTile;
   if (last >= seg_begin) fetch(last);
   for (long long t0 = last; t0 >= seg_begin; t0 -= kScanTile) {
@@ -560,70 +618,51 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
       States<R> hs[kScanTile], es[kScanTile], h = start, da_tile = {};
       // (the next four tokens' values are read while these are worked on)
       Four32 st = four_tokens(ls, s.c, 0), u = four_tokens(lu, s.c, 0), vt = {}, st_next = {}, u_next = {}, vt_next = {};
-      for_each<kScanTile>([&](auto index) TFA_INLINE {
-        constexpr int t = index, k = t / 4;
-        if constexpr (t % 4 == 0 && k + 1 < kScanTile / 4) st_next = four_tokens(ls, s.c, k + 1), u_next = four_tokens(lu, s.c, k + 1);
-        if constexpr (t % 4 == 0 && k + 1 == kScanTile / 4) vt = four_tokens(lv, s.c, k);
-        float in[R];
-        bs.template products<t>(lb, s.q, u.v[t % 4], in);
+      for_each<kScanTile / 2>([&](auto index) TFA_INLINE {
+        constexpr int t = 2 * index, k = t / 4, j = t % 4;
+        if constexpr (j == 0 && k + 1 < kScanTile / 4) st_next = four_tokens(ls, s.c, k + 1), u_next = four_tokens(lu, s.c, k + 1);
+        if constexpr (j == 0 && k + 1 == kScanTile / 4) vt = four_tokens(lv, s.c, k);
+        float in0[R], in1[R];
+        bs.template products<t>(lb, s.q, u.v[j], u.v[j + 1], in0, in1);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          es[t].v[r] = decay_of(st.v[t % 4], a.v[r]);
-          h.v[r] = __builtin_fmaf(es[t].v[r], h.v[r], in[r]);
+          es[t].v[r] = decay_of(st.v[j], a.v[r]);
+          es[t + 1].v[r] = decay_of(st.v[j + 1], a.v[r]);
+          hs[t].v[r] = __builtin_fmaf(es[t].v[r], h.v[r], in0[r]);
+          hs[t + 1].v[r] = __builtin_fmaf(es[t + 1].v[r], hs[t].v[r], in1[r]);
         }
-        hs[t] = h;
-        if constexpr (t % 4 == 3) {
+        h = hs[t + 1];
+        if constexpr (j == 2) {
           if constexpr (k + 1 < kScanTile / 4) st = st_next, u = u_next;
           __builtin_amdgcn_sched_barrier(0);
         }
       });
       // sums over the states for a token: of Q tokens at least before they are folded
       float sum_b[Q], sum_a[Q], sum_y[Q];
+      float v[2][2 * R];  // what two tokens' gradients by b and c sum up over the channels
       for_each<kScanTile>([&](auto index) TFA_INLINE {
-        constexpr int t = kScanTile - 1 - index, k = t / 4, at = t % Q;
-        if constexpr (t % 4 == 3 && k > 0)
+        constexpr int t = kScanTile - 1 - index, k = t / 4, j = t % 4, at = t % Q;
+        if constexpr (j == 3 && k > 0)
           st_next = four_tokens(ls, s.c, k - 1), u_next = four_tokens(lu, s.c, k - 1), vt_next = four_tokens(lv, s.c, k - 1);
         const States<R>& before = t ? hs[t ? t - 1 : 0] : start;
-        float v[2 * R];
-        cs.template add<t>(lc, s.q, vt.v[t % 4], carry.v);  // (now g)
-        sum_b[at] = bs.template dot<t>(lb, s.q, carry.v);
-        sum_y[at] = cs.template dot<t>(lc, s.q, hs[t].v);
+        float(&own)[2 * R] = v[t % 2];
+        reverse_token<t>(bs, lb, cs, lc, s.q, vt.v[j], hs[t], carry, sum_b[at], sum_y[at]);  // (carry is now g)
         sum_a[at] = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          v[r] = carry.v[r] * u.v[t % 4];
-          v[R + r] = vt.v[t % 4] * hs[t].v[r];
+          own[r] = carry.v[r] * u.v[j];
+          own[R + r] = vt.v[j] * hs[t].v[r];
           carry.v[r] *= es[t].v[r];
           const float flow = carry.v[r] * before.v[r];
           sum_a[at] = __builtin_fmaf(flow, a.v[r], sum_a[at]);
-          da_tile.v[r] = __builtin_fmaf(flow, st.v[t % 4], da_tile.v[r]);
+          da_tile.v[r] = __builtin_fmaf(flow, st.v[j], da_tile.v[r]);
         }
-        // over the channels: db's and dc's shares part at the first level, their states at the next
-        float* const to = shares[turn][s.wave] + (2 * t + s.c / (kChannels / 2)) * Q * R + R * s.q;
-        constexpr int kTop = kChannels / 2 == 4 ? 7 : kChannels / 2, kMid = kChannels / 4 == 4 ? 7 : kChannels / 4;
-        float w[R];
-        fold_pairs<kTop, R>(v, w);
-        // (lanes with the same sum write the same bits)
-        if constexpr (R == 1) {
-          to[0] = fold<1>(fold<2>(fold<kMid>(w[0])));
-        } else if constexpr (R == 2) {
-          to[s.c / (kChannels / 4) % 2] = fold<1>(fold<2>(fold<kMid>(w[0], w[1])));
-        } else {
-          float* const half = to + s.c / (kChannels / 4) % 2 * 2;
-          float x2[2];
-          fold_pairs<kMid, 2>(w, x2);
-          if constexpr (kChannels == 4) {
-            half[0] = x2[0];
-            half[1] = x2[1];
-          } else {
-            constexpr int kLow = kChannels / 8;
-            float sum = fold<kLow>(x2[0], x2[1]);
-            if constexpr (kChannels == 16) sum = fold<1>(sum);
-            half[s.c / kLow % 2] = sum;
-          }
+        if constexpr (t % 2 == 0) fold_channels(v, t);
+        if constexpr (at == 0) {
+          settle(sum_b), settle(sum_y);
+          gb[t / Q] = fold_states<Q>(sum_b), ga[t / Q] = fold_states<Q>(sum_a), ys[t / Q] = fold_states<Q>(sum_y);
         }
-        if constexpr (t % Q == 0) gb[t / Q] = fold_states<Q>(sum_b), ga[t / Q] = fold_states<Q>(sum_a), ys[t / Q] = fold_states<Q>(sum_y);
-        if constexpr (t % 4 == 0) {
+        if constexpr (j == 0) {
           st = st_next, u = u_next, vt = vt_next;
           __builtin_amdgcn_sched_barrier(0);
         }

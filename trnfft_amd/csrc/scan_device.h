@@ -33,64 +33,112 @@ __device__ __forceinline__ float lane_xor(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), ctrl, 15, 15, true));
 }
 
-// Products with x[r] of lane T of the lane's row of 16, which the instruction's operand takes from there.  (Waits as at
-// fold_pairs.)
+// A permutation of lanes takes values that are two instructions old; the compiler keeps to that for its own instructions, and does not
+// see those written here: they begin with a wait where what they permute may be new, and what they leave is made old by this before
+// a permutation that the compiler writes.
+template <int N>
+__device__ __forceinline__ void settle(float (&v)[N]) {
+  if constexpr (N == 4)
+    asm volatile("s_nop 1" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+  else
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("s_nop 1" : "+v"(v[i]));
+}
+
+// Products with x[r] of lanes T and T + 1 of the lane's row of 16, which the instructions' operands take from there.
+#define TFA_ROW_AT(lane) " row_newbcast:%c[" lane "] row_mask:0xf bank_mask:0xf\n\t"
 template <int T>
 struct RowLane {
-  template <int R>
-  static __device__ __forceinline__ void products(const float (&x)[R], float u, float (&out)[R]) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) out[r] = lane(x[r]) * u;
+  static __device__ __forceinline__ float lane(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + T, 15, 15, true));
   }
+  // out = x (of T) u0 and x (of T + 1) u1
+  template <int R>
+  static __device__ __forceinline__ void products(const float (&x)[R], float u0, float u1, float (&out0)[R], float (&out1)[R]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) out0[r] = lane(x[r]) * u0, out1[r] = RowLane<T + 1>::lane(x[r]) * u1;
+  }
+  static __device__ __forceinline__ void products(const float (&x)[4], float u0, float u1, float (&out0)[4], float (&out1)[4]) {
+    asm("s_nop 1\n\t"
+        "v_mul_f32_dpp %0, %8, %12" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %1, %9, %12" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %2, %10, %12" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %3, %11, %12" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %4, %8, %13" TFA_ROW_AT("n")
+        "v_mul_f32_dpp %5, %9, %13" TFA_ROW_AT("n")
+        "v_mul_f32_dpp %6, %10, %13" TFA_ROW_AT("n")
+        "v_mul_f32_dpp %7, %11, %13" TFA_ROW_AT("n")
+        : "=&v"(out0[0]), "=&v"(out0[1]), "=&v"(out0[2]), "=&v"(out0[3]), "=&v"(out1[0]), "=&v"(out1[1]), "=&v"(out1[2]), "=&v"(out1[3])
+        : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(u0), "v"(u1), [t] "n"(T), [n] "n"(T + 1));
+  }
+  // sum0 = x (of T) . y0, sum1 = x (of T + 1) . y1
+  template <int R>
+  static __device__ __forceinline__ void dots(const float (&x)[R], const float (&y0)[R], const float (&y1)[R], float& sum0, float& sum1) {
+    sum0 = lane(x[0]) * y0[0], sum1 = RowLane<T + 1>::lane(x[0]) * y1[0];
+#pragma unroll
+    for (int r = 1; r < R; ++r)
+      sum0 = __builtin_fmaf(lane(x[r]), y0[r], sum0), sum1 = __builtin_fmaf(RowLane<T + 1>::lane(x[r]), y1[r], sum1);
+  }
+  static __device__ __forceinline__ void dots(const float (&x)[4], const float (&y0)[4], const float (&y1)[4], float& sum0, float& sum1) {
+    asm("s_nop 1\n\t"
+        "v_mul_f32_dpp %0, %2, %6" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %1, %2, %10" TFA_ROW_AT("n")
+        "v_fmac_f32_dpp %0, %3, %7" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %1, %3, %11" TFA_ROW_AT("n")
+        "v_fmac_f32_dpp %0, %4, %8" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %1, %4, %12" TFA_ROW_AT("n")
+        "v_fmac_f32_dpp %0, %5, %9" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %1, %5, %13" TFA_ROW_AT("n")
+        : "=&v"(sum0), "=&v"(sum1)
+        : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(y0[0]), "v"(y0[1]), "v"(y0[2]), "v"(y0[3]), "v"(y1[0]), "v"(y1[1]),
+          "v"(y1[2]), "v"(y1[3]), [t] "n"(T), [n] "n"(T + 1));
+  }
+  // sum += x (of T) u
   template <int R>
   static __device__ __forceinline__ void add(const float (&x)[R], float u, float (&sum)[R]) {
 #pragma unroll
     for (int r = 0; r < R; ++r) sum[r] = __builtin_fmaf(lane(x[r]), u, sum[r]);
   }
-  template <int R>
-  static __device__ __forceinline__ float dot(const float (&x)[R], const float (&y)[R]) {
-    float sum = lane(x[0]) * y[0];
-#pragma unroll
-    for (int r = 1; r < R; ++r) sum = __builtin_fmaf(lane(x[r]), y[r], sum);
-    return sum;
-  }
-  static __device__ __forceinline__ float lane(float x) {
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x150 + T, 15, 15, true));
-  }
-  // four at once without a move for each
-#define TFA_ROW " row_newbcast:%c[t] row_mask:0xf bank_mask:0xf\n\t"
-  static __device__ __forceinline__ void products(const float (&x)[4], float u, float (&out)[4]) {
-    asm("s_nop 1\n\t"
-        "v_mul_f32_dpp %0, %4, %8" TFA_ROW
-        "v_mul_f32_dpp %1, %5, %8" TFA_ROW
-        "v_mul_f32_dpp %2, %6, %8" TFA_ROW
-        "v_mul_f32_dpp %3, %7, %8" TFA_ROW
-        : "=&v"(out[0]), "=&v"(out[1]), "=&v"(out[2]), "=&v"(out[3])
-        : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(u), [t] "n"(T));
-  }
   static __device__ __forceinline__ void add(const float (&x)[4], float u, float (&sum)[4]) {
     asm("s_nop 1\n\t"
-        "v_fmac_f32_dpp %0, %4, %8" TFA_ROW
-        "v_fmac_f32_dpp %1, %5, %8" TFA_ROW
-        "v_fmac_f32_dpp %2, %6, %8" TFA_ROW
-        "v_fmac_f32_dpp %3, %7, %8" TFA_ROW
+        "v_fmac_f32_dpp %0, %4, %8" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %1, %5, %8" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %2, %6, %8" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %3, %7, %8" TFA_ROW_AT("t")
         : "+&v"(sum[0]), "+&v"(sum[1]), "+&v"(sum[2]), "+&v"(sum[3])
         : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(u), [t] "n"(T));
   }
-  static __device__ __forceinline__ float dot(const float (&x)[4], const float (&y)[4]) {
-    float sum;
-    asm("s_nop 1\n\t"
-        "v_mul_f32_dpp %0, %1, %5" TFA_ROW
-        "v_fmac_f32_dpp %0, %2, %6" TFA_ROW
-        "v_fmac_f32_dpp %0, %3, %7" TFA_ROW
-        "v_fmac_f32_dpp %0, %4, %8" TFA_ROW
-        "s_nop 1"
-        : "=&v"(sum)
-        : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(y[0]), "v"(y[1]), "v"(y[2]), "v"(y[3]), [t] "n"(T));
-    return sum;
+  // g += c (of T) u;  sum_b = b (of T) . g,  sum_c = c (of T) . h
+  template <int R>
+  static __device__ __forceinline__ void reverse(const float (&b)[R], const float (&c)[R], float u, const float (&h)[R], float (&g)[R], float& sum_b,
+                                                 float& sum_c) {
+    add(c, u, g);
+    sum_b = lane(b[0]) * g[0], sum_c = lane(c[0]) * h[0];
+#pragma unroll
+    for (int r = 1; r < R; ++r) sum_b = __builtin_fmaf(lane(b[r]), g[r], sum_b), sum_c = __builtin_fmaf(lane(c[r]), h[r], sum_c);
   }
-#undef TFA_ROW
+  static __device__ __forceinline__ void reverse(const float (&b)[4], const float (&c)[4], float u, const float (&h)[4], float (&g)[4], float& sum_b,
+                                                 float& sum_c) {
+    asm("s_nop 1\n\t"
+        "v_fmac_f32_dpp %0, %10, %18" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %1, %11, %18" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %2, %12, %18" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %3, %13, %18" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %4, %6, %0" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %5, %10, %14" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %4, %7, %1" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %5, %11, %15" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %4, %8, %2" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %5, %12, %16" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %4, %9, %3" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %5, %13, %17" TFA_ROW_AT("t")
+        : "+&v"(g[0]), "+&v"(g[1]), "+&v"(g[2]), "+&v"(g[3]), "=&v"(sum_b), "=&v"(sum_c)
+        : "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "v"(c[0]), "v"(c[1]), "v"(c[2]), "v"(c[3]), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]),
+          "v"(u), [t] "n"(T));
+  }
 };
+#undef TFA_ROW_AT
+
 // f(0), f(1), ... f(N - 1) with numbers that are part of their type
 template <typename F, int... I>
 __device__ __forceinline__ void for_each_index(F f, std::integer_sequence<int, I...>) {
@@ -125,59 +173,41 @@ __device__ __forceinline__ float fold(float a) {
     return a + lane_xor<MASK>(a);
 }
 
-// fold<MASK>(v[i], v[i + N]) of N pairs.  Within rows of 16 an addition that writes the lanes of some quads alone takes two
-// instructions where selecting takes three.  (Permutations take values that are two instructions old: waits before, and behind for
-// what the compiler does with the sums, since it does not see these instructions.)
-template <int MASK, int N>
-__device__ __forceinline__ void fold_pairs(const float (&v)[2 * N], float (&w)[N]) {
-  if constexpr (MASK == 8 && N == 4) {
-    asm("s_nop 1\n\t"
-        "v_add_f32_dpp %0, %4, %4 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
-        "v_add_f32_dpp %0, %8, %8 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
-        "v_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
-        "v_add_f32_dpp %1, %9, %9 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
-        "v_add_f32_dpp %2, %6, %6 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
-        "v_add_f32_dpp %2, %10, %10 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
-        "v_add_f32_dpp %3, %7, %7 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
-        "v_add_f32_dpp %3, %11, %11 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
-        "s_nop 1"
-        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3])
-        : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(v[4]), "v"(v[5]), "v"(v[6]), "v"(v[7]));
-  } else if constexpr (MASK == 7 && N == 4) {
-    asm("s_nop 1\n\t"
-        "v_add_f32_dpp %0, %4, %4 row_half_mirror row_mask:0xf bank_mask:0x5\n\t"
-        "v_add_f32_dpp %0, %8, %8 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
-        "v_add_f32_dpp %1, %5, %5 row_half_mirror row_mask:0xf bank_mask:0x5\n\t"
-        "v_add_f32_dpp %1, %9, %9 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
-        "v_add_f32_dpp %2, %6, %6 row_half_mirror row_mask:0xf bank_mask:0x5\n\t"
-        "v_add_f32_dpp %2, %10, %10 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
-        "v_add_f32_dpp %3, %7, %7 row_half_mirror row_mask:0xf bank_mask:0x5\n\t"
-        "v_add_f32_dpp %3, %11, %11 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
-        "s_nop 1"
-        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3])
-        : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(v[4]), "v"(v[5]), "v"(v[6]), "v"(v[7]));
-  } else if constexpr (MASK == 7 && N == 2) {
-    asm("s_nop 1\n\t"
-        "v_add_f32_dpp %0, %2, %2 row_half_mirror row_mask:0xf bank_mask:0x5\n\t"
-        "v_add_f32_dpp %0, %4, %4 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
-        "v_add_f32_dpp %1, %3, %3 row_half_mirror row_mask:0xf bank_mask:0x5\n\t"
-        "v_add_f32_dpp %1, %5, %5 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
-        "s_nop 1"
-        : "=&v"(w[0]), "=&v"(w[1])
-        : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]));
-  } else if constexpr (MASK == 8 && N == 2) {
-    asm("s_nop 1\n\t"
-        "v_add_f32_dpp %0, %2, %2 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
-        "v_add_f32_dpp %0, %4, %4 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
-        "v_add_f32_dpp %1, %3, %3 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
-        "v_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
-        "s_nop 1"
-        : "=&v"(w[0]), "=&v"(w[1])
-        : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = fold<MASK>(v[i], v[i + N]);
-  }
+// Sums over a row's 16 lanes of the 8 values of two tokens: lane l receives those of value 4 (l / 8) + 2 (l / 4 % 2) + l / 2 % 2.  An addition
+// that writes the lanes of some quads alone takes two instructions where selecting takes three; below a quad lanes are selected by `odd`, those
+// with bit 1 of their number set.
+__device__ __forceinline__ void fold_row(const float (&v)[8], const float (&u)[8], unsigned long long odd, float& sum_v, float& sum_u) {
+  float w0, w1, w2, w3, x0, x1, y0, y1, y2, y3, z0, z1;
+#define TFA_HALVES(to, low, high) \
+  "v_add_f32_dpp " to ", " low ", " low " row_ror:8 row_mask:0xf bank_mask:0x3\n\t" \
+  "v_add_f32_dpp " to ", " high ", " high " row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+#define TFA_QUADS(to, low, high) \
+  "v_add_f32_dpp " to ", " low ", " low " row_half_mirror row_mask:0xf bank_mask:0x5\n\t" \
+  "v_add_f32_dpp " to ", " high ", " high " row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
+  asm("s_nop 1\n\t"
+      TFA_HALVES("%0", "%4", "%8") TFA_HALVES("%2", "%6", "%10") TFA_HALVES("%1", "%5", "%9") TFA_HALVES("%3", "%7", "%11")
+      : "=&v"(w0), "=&v"(w1), "=&v"(w2), "=&v"(w3)
+      : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(v[4]), "v"(v[5]), "v"(v[6]), "v"(v[7]));
+  asm("s_nop 1\n\t"
+      TFA_HALVES("%0", "%4", "%8") TFA_HALVES("%2", "%6", "%10") TFA_HALVES("%1", "%5", "%9") TFA_HALVES("%3", "%7", "%11")
+      : "=&v"(y0), "=&v"(y1), "=&v"(y2), "=&v"(y3)
+      : "v"(u[0]), "v"(u[1]), "v"(u[2]), "v"(u[3]), "v"(u[4]), "v"(u[5]), "v"(u[6]), "v"(u[7]));
+  float keep_v, give_v, keep_u, give_u;
+  asm("s_nop 1\n\t"
+      TFA_QUADS("%0", "%10", "%12") TFA_QUADS("%1", "%11", "%13") TFA_QUADS("%2", "%14", "%16") TFA_QUADS("%3", "%15", "%17")
+      "v_cndmask_b32 %5, %1, %0, %18\n\t"  // (what the other lane keeps)
+      "v_cndmask_b32 %7, %3, %2, %18\n\t"
+      "v_cndmask_b32 %4, %0, %1, %18\n\t"
+      "v_cndmask_b32 %6, %2, %3, %18\n\t"
+      "v_add_f32_dpp %4, %5, %4 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %6, %7, %6 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 0\n\t"
+      "v_add_f32_dpp %8, %4, %4 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %9, %6, %6 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf"
+      : "=&v"(x0), "=&v"(x1), "=&v"(z0), "=&v"(z1), "=&v"(keep_v), "=&v"(give_v), "=&v"(keep_u), "=&v"(give_u), "=&v"(sum_v), "=&v"(sum_u)
+      : "v"(w0), "v"(w1), "v"(w2), "v"(w3), "v"(y0), "v"(y1), "v"(y2), "v"(y3), "s"(odd));
+#undef TFA_HALVES
+#undef TFA_QUADS
 }
 
 }  // namespace tfa
