@@ -417,7 +417,7 @@ int tfa_causal_conv_step(const tfa_conv_desc* desc, const void* x, const float* 
  *   y_t = (c_t . h_t + d x_t) silu(z_t)
  * x, dt, z: (batch, tokens, channels) at strides of batch and token, channels contiguous; b, c: (batch, tokens, groups, states) at
  * strides of batch, token and group, states contiguous, shared by channels / groups neighbouring channels; all of one type, at any
- * address, token strides from 0 to 2^24 - 1.  a: fp32 (channels, states); d, dt_bias: fp32 (channels) or NULL (zero); z may be NULL (no gate).  State tensors are fp32
+ * address, token strides from 0 to 2^24 - 1.  a: fp32 (channels, states), -inf for no memory; d, dt_bias: fp32 (channels) or NULL (zero); z may be NULL (no gate).  State tensors are fp32
  * (batch, channels, states).  lengths: (batch) device int64 or NULL; tokens at and past a sequence's length are padding: never
  * read, zeros in y and the gradients, and the state is the one at the length.  States, exponentials and sums are fp32 for every
  * type.  What is not finite makes NaN or infinities of its channel from its token on.  Up to 64 states.
@@ -431,7 +431,7 @@ typedef struct tfa_scan_desc {
   int64_t b_stride[3], c_stride[3];               /* batch, token, group */
 } tfa_scan_desc;
 
-/* Bytes of the states that a backward needs of its forward, and of the workspaces of both. */
+/* Bytes of the states that a backward needs of its forward, and of the workspaces of both; all 16-byte aligned device memory. */
 int tfa_selective_scan_sizes(const tfa_scan_desc* desc, size_t* kept, size_t* workspace, size_t* backward_workspace);
 /* state_in may be NULL (zeros), state_out NULL (not wanted; must not be state_in), kept NULL (no backward follows). */
 int tfa_selective_scan(const tfa_scan_desc* desc, const void* x, const void* dt, const float* a, const void* b, const void* c,
@@ -458,7 +458,8 @@ int tfa_selective_scan_step(const tfa_scan_desc* desc, const void* x, const void
  * The norm of all values of many contiguous tensors, norm[0] = sqrt(sum of squares) with squares summed in 64 bits, and their
  * clipping: every value times min(1, max_norm / (norm + 1e-6)), in place.  A norm that is not finite makes gradients NaN or zero.
  * tensors[d], count[d]: those of type d (TFA_DTYPE_*); host memory, read before the call returns.  norm: device fp32.
- * parts: device workspace of the size that tfa_grad_norm_workspace_size gives.  Sums are added in one order whatever the timing.
+ * workspace: 8-byte aligned device memory of the size that tfa_grad_norm_workspace_size gives.  Sums are added in one order
+ * whatever the timing.
  */
 typedef struct tfa_grad_tensor {
   void* data;

@@ -154,7 +154,8 @@ def test_c_entries_refuse_bad_descriptors():
         (scan(states=0), _lib.TFA_ERR_INVALID),
         (scan(states=65), _lib.TFA_ERR_UNSUPPORTED),
         (scan(batch=-1), _lib.TFA_ERR_INVALID),
-        (scan(batch=2**25), _lib.TFA_ERR_UNSUPPORTED),
+        (scan(batch=2**29), _lib.TFA_ERR_UNSUPPORTED),
+        (scan(batch=2**25, tokens=2**30), _lib.TFA_ERR_UNSUPPORTED),
         (scan(tokens=2**31), _lib.TFA_ERR_UNSUPPORTED),
     ]:
         assert lib.tfa_selective_scan_sizes(desc, *sizes) == rc
@@ -163,6 +164,9 @@ def test_c_entries_refuse_bad_descriptors():
     call = lib.tfa_selective_scan
     assert call(scan(), far, far, None, far, far, None, None, None, None, None, far, None, None, None, None) == _lib.TFA_ERR_INVALID
     assert call(scan(), far, far, far, far, far, None, None, None, None, far, far, far, None, None, None) == _lib.TFA_ERR_INVALID
+    assert call(scan(), far, far, far, far, far, None, None, None, None, None, far, None, far + 8, None, None) == _lib.TFA_ERR_INVALID
+    for strides in (dict(x_stride_token=2**24), dict(b_stride_token=-1)):
+        assert call(scan(**strides), far, far, far, far, far, None, None, None, None, None, far, None, None, None, None) == _lib.TFA_ERR_UNSUPPORTED
     assert call(scan(batch=0), *[None] * 15) == _lib.TFA_OK
     assert lib.tfa_selective_scan_step(scan(), far, far, far, far, far, None, None, None, far, far, None) == _lib.TFA_ERR_INVALID
     back = lib.tfa_selective_scan_backward
@@ -180,6 +184,7 @@ def test_c_entries_refuse_bad_descriptors():
     assert lib.tfa_grad_norm_workspace_size(lists((0, 3)), size) == _lib.TFA_ERR_INVALID
     assert lib.tfa_grad_norm_workspace_size(lists((far, 20000), (far, 1)), size) == _lib.TFA_OK and size.value >= 8 * 2
     assert lib.tfa_grad_norm(lists((far, 3)), None, far, None) == _lib.TFA_ERR_INVALID
+    assert lib.tfa_grad_norm(lists((far, 3)), far, far + 4, None) == _lib.TFA_ERR_INVALID
     assert lib.tfa_clip_grads(lists((far, 3)), -1.0, far, far, None) == _lib.TFA_ERR_INVALID
     assert lib.tfa_clip_grads(lists((far, 3), (far + 8, 3)), 1.0, far, far, None) == _lib.TFA_ERR_INVALID  # overlap
     assert b"overlap" in lib.tfa_last_error()

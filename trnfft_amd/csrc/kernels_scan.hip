@@ -16,7 +16,9 @@ __global__ __launch_bounds__(64) void scan_join_kernel(ScanArgs p, int lanes, bo
   const long long row = unit / tiles / p.groups;
   const bool valid = own < each;
   const int channel = (int)(unit / tiles % p.groups) * each + (valid ? own : 0);
-  const States<R> a = load_states<R>(p.a + (long long)channel * p.n, p.n, q, valid);
+  States<R> a = load_states<R>(p.a + (long long)channel * p.n, p.n, q, valid);
+#pragma unroll
+  for (int r = 0; r < R; ++r) a.v[r] = rate_of(a.v[r]);
   const float* from = reverse ? p.dstate_out : p.state_in;
   States<R> s = {};
   if (from) s = load_states<R>(from + (row * p.channels + channel) * p.n, p.n, q, valid);
@@ -30,7 +32,7 @@ __global__ __launch_bounds__(64) void scan_join_kernel(ScanArgs p, int lanes, bo
       const int k = min(k0 + i, p.segments - 2);
       const long long at = ((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane;
       sum[i] = reinterpret_cast<const States<R>*>(p.seg_state)[at];
-      steps[i] = p.seg_steps[at] * kLog2E;
+      steps[i] = p.seg_steps[at];
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, bool whole, 
   }
   Four32 a = states_of(p.a + (long long)channel * p.n);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) a.v[r] *= kLog2E;
+  for (int r = 0; r < 4; ++r) a.v[r] = rate_of(a.v[r]);
   const float skip = p.d ? p.d[channel] : 0.0f, bias = p.dt_bias ? p.dt_bias[channel] : 0.0f;
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {

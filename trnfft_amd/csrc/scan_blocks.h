@@ -41,19 +41,43 @@ struct ScanPlace {
   int seg;
 };
 
-template <int Q>
-__device__ __forceinline__ ScanPlace<Q> scan_place(const ScanArgs& p, long long block, int waves) {
+// Ragged rows are given out by length, so that the compute units' sums of them are about the same: the longest first, and every other layer
+// of workgroups over the 256 compute units from the shortest on (a wave that starts late has little to do).  64 rows of up to 626 tokens, 512
+// channels of 16 states, two workgroups a compute unit: RAGGED us, in their own order 88.6.  Batches of more rows than threads keep their order.
+template <int THREADS>
+__device__ __forceinline__ long long scan_row(const ScanArgs& p, long long slot, int blocks) {
+  if (!p.lengths || p.batch > THREADS || p.batch == 1) return slot;
+  __shared__ int found;
+  // (layers 0, 2, ... take the ranks from the front, 1, 3, ... from the back)
+  const int layer_rows = max(1, 256 / blocks), layer = (int)slot / layer_rows, first = layer * layer_rows;
+  const int in = (int)slot - first, rank = layer % 2 == 0 ? layer / 2 * layer_rows + in : (int)p.batch - 1 - (layer / 2 * layer_rows + in);
+  const int t = threadIdx.x;
+  if (t < p.batch) {
+    const long long own = p.lengths[t];
+    int before = 0;
+    for (int i = 0; i < (int)p.batch; ++i) {
+      const long long other = p.lengths[i];
+      before += other > own || (other == own && i < t);
+    }
+    if (before == rank) found = t;
+  }
+  __syncthreads();
+  return found;
+}
+
+template <int Q, int WAVES>
+__device__ __forceinline__ ScanPlace<Q> scan_place(const ScanArgs& p, long long block) {
   ScanPlace<Q> s;
-  const int each = p.channels / p.groups, tiles = (each + s.kChannels - 1) / s.kChannels, across = (tiles + waves - 1) / waves;
+  const int each = p.channels / p.groups, tiles = (each + s.kChannels - 1) / s.kChannels, across = (tiles + WAVES - 1) / WAVES;
   s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   s.lane = threadIdx.x % 64;
   s.q = s.lane / s.kChannels;
   s.c = s.lane % s.kChannels;
-  s.tile = (int)(block % across) * waves + s.wave;
+  s.tile = (int)(block % across) * WAVES + s.wave;
   block /= across;
   s.group = (int)(block % p.groups);
   block /= p.groups;
-  s.row = block % p.batch;
+  s.row = __builtin_amdgcn_readfirstlane((int)scan_row<64 * WAVES>(p, block % p.batch, across * p.groups));
   s.seg = (int)(block / p.batch);
   s.idle = s.tile >= tiles;
   const int tile = min(s.tile, tiles - 1), left = each - tile * s.kChannels;
@@ -333,7 +357,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
   constexpr int kOwn = kScanTile / Q;
   __shared__ float rows[kScanWaves][2][kBankWords<Q, R>];
   __shared__ float planes[kScanWaves][2][kPlaneWords<Q>];
-  const ScanPlace<Q> s = scan_place<Q>(p, first_block + blockIdx.x, kScanWaves);
+  const ScanPlace<Q> s = scan_place<Q, kScanWaves>(p, first_block + blockIdx.x);
   if (s.idle) return;
   float *const lb = rows[s.wave][0], *const lc = rows[s.wave][1], *const ls = planes[s.wave][0], *const lu = planes[s.wave][1];
   const long long seg_begin = s.seg * p.seg_tokens, seg_end = min(p.tokens, seg_begin + p.seg_tokens), end = min(scan_end(p, s.row), seg_end);
@@ -349,7 +373,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
 
   States<R> a = load_states<R>(p.a + (long long)channel * p.n, p.n, s.q, s.valid), h = {};
 #pragma unroll
-  for (int r = 0; r < R; ++r) a.v[r] *= kLog2E;
+  for (int r = 0; r < R; ++r) a.v[r] = rate_of(a.v[r]);
   const float bias = p.dt_bias ? p.dt_bias[channel] : 0.0f, skip = p.d ? p.d[channel] : 0.0f;
   if (OUT) {
     if (p.segments > 1)
@@ -457,7 +481,7 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
   __shared__ float rows[kWaves][2][kBankWords<Q, R>];
   __shared__ float planes[kWaves][SUM ? 2 : 6][kPlaneWords<Q>];
   __shared__ float shares[2][SUM ? 1 : kWaves][SUM ? 1 : kScanTile * 2 * Q * R];  // of this tile and the one before
-  ScanPlace<Q> s = scan_place<Q>(p, first_block + blockIdx.x, kWaves);
+  ScanPlace<Q> s = scan_place<Q, kWaves>(p, first_block + blockIdx.x);
   if (SUM) ++s.seg;  // (nothing comes before the first segment)
   if (SUM && s.idle) return;  // (else it takes part in the barriers)
   float *const lb = rows[s.wave][0], *const lc = rows[s.wave][1];
@@ -479,7 +503,7 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
 
   States<R> a = load_states<R>(p.a + (long long)channel * p.n, p.n, s.q, s.valid), carry = {}, da = {};
 #pragma unroll
-  for (int r = 0; r < R; ++r) a.v[r] *= kLog2E;
+  for (int r = 0; r < R; ++r) a.v[r] = rate_of(a.v[r]);
   const float bias = p.dt_bias ? p.dt_bias[channel] : 0.0f, skip = p.d ? p.d[channel] : 0.0f;
   if (!SUM) {
     if (p.segments > 1)

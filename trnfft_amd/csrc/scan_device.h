@@ -14,6 +14,10 @@ constexpr float kLog2E = 1.4426950408889634f;
 // over a memory of a thousand frames more than all roundings together.  Its mean is put back into the argument, which costs nothing.
 __device__ __forceinline__ float decay_of(float s, float a2) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, a2, 6e-9f)); }
 
+// a log2(e) as decay_of takes it.  A rate of -inf (no memory) becomes one that does the same for every step of 1e-35 and more, and with a step
+// of zero, as padding has it, keeps the state instead of making NaN of it.  (NaN stays.)
+__device__ __forceinline__ float rate_of(float a) { return (a < -1e38f ? -1e38f : a) * kLog2E; }
+
 // log(1 + e^v) and its derivative, off by a few 2^-24 of themselves and of v: with e = e^-|v| and u = 1 + e, log(1 + e) = log(u) + (e - (u - 1)),
 // where the second term is what the sum u lost (the hardware's logarithm is good to its last bit next to 1 too).  Measured from -20 to 20:
 // 3e-8 of it in the mean square for v > 0, 2e-7 at -8, 1e-6 at most; a series for the artanh took twice the instructions for the same.

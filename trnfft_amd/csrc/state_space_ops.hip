@@ -20,15 +20,17 @@ size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
 // Sizes up to which no count of threads, values or bytes of a workspace passes 63 bits
 constexpr int32_t kMostChannels = 1 << 20;
-constexpr int64_t kMostBatch = 1 << 24, kMostTokens = INT32_MAX;
+constexpr int64_t kMostBatch = 1 << 28, kMostTokens = INT32_MAX;
+constexpr double kMostValues = 1LL << 44;
 
 int check_sequence(int32_t dtype, int64_t batch, int64_t tokens, int32_t channels) {
   if (!dtype_ok(dtype)) return set_error(TFA_ERR_INVALID, "dtype must be TFA_DTYPE_F32, _BF16 or _F16");
   if (batch < 0 || tokens < 0) return set_error(TFA_ERR_INVALID, "negative dimension");
   if (channels < 1) return set_error(TFA_ERR_INVALID, "need at least one channel");
   if (channels > kMostChannels) return set_error(TFA_ERR_UNSUPPORTED, "more than 2^20 channels");
-  if (batch > kMostBatch) return set_error(TFA_ERR_UNSUPPORTED, "more than 2^24 batch rows");
+  if (batch > kMostBatch) return set_error(TFA_ERR_UNSUPPORTED, "more than 2^28 batch rows");
   if (tokens > kMostTokens) return set_error(TFA_ERR_UNSUPPORTED, "more than 2^31 tokens");
+  if ((double)batch * (double)tokens * channels > kMostValues) return set_error(TFA_ERR_UNSUPPORTED, "more than 2^44 values");
   return TFA_OK;
 }
 
@@ -101,6 +103,12 @@ void scan_inputs(P& p, const tfa_scan_desc* d, const ScanInputs& in) {
   p.b_sb = rows ? d->b_stride[0] : 0, p.c_sb = rows ? d->c_stride[0] : 0;
   p.b_sg = groups ? d->b_stride[2] : 0, p.c_sg = groups ? d->c_stride[2] : 0;
 }
+// what the kernels read and write by 16 bytes
+int check_aligned(const void* kept, const void* workspace) {
+  if ((reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(workspace)) % 16)
+    return set_error(TFA_ERR_INVALID, "kept states and workspace must be 16-byte aligned");
+  return TFA_OK;
+}
 // (a lane's own part of an address has 32 bits: tokens of a tile are less than 2^32 bytes apart)
 int check_token_strides(const tfa_scan_desc* d) {
   if (d->tokens < 2) return TFA_OK;
@@ -153,6 +161,7 @@ bool overlapping(const tfa_grad_lists* g) {
 
 int grad_norm(const tfa_grad_lists* grads, float* norm, void* workspace, bool scale, double max_norm, tfa_stream stream) {
   if (!norm || !workspace) return set_error(TFA_ERR_INVALID, "null data pointer");
+  if (reinterpret_cast<uintptr_t>(workspace) % 8) return set_error(TFA_ERR_INVALID, "the workspace must be 8-byte aligned");
   const hipError_t e = tfa::launch_grad_norm(grad_lists(grads), static_cast<double*>(workspace), norm, scale, max_norm,
                                              static_cast<hipStream_t>(stream));
   if (e == hipErrorInvalidValue) return set_error(TFA_ERR_UNSUPPORTED, "tensor beyond the launch grid");
@@ -235,6 +244,7 @@ int tfa_selective_scan(const tfa_scan_desc* desc, const void* x, const void* dt,
   scan_tokens(p, desc);
   const tfa::ScanSizes size = tfa::scan_sizes(p);
   if (size.seg_state && !workspace) return set_error(TFA_ERR_INVALID, "null workspace");
+  if (const int rc = check_aligned(kept, workspace)) return rc;
   p.lengths = reinterpret_cast<const long long*>(lengths);
   p.state_in = state_in, p.state_out = state_out, p.y = y;
   p.kept = size.kept ? static_cast<float*>(kept) : nullptr;
@@ -263,6 +273,7 @@ int tfa_selective_scan_backward(const tfa_scan_desc* desc, const void* x, const 
   const tfa::ScanSizes size = tfa::scan_sizes(p);
   if (size.kept && !kept) return set_error(TFA_ERR_INVALID, "the forward's states are needed");
   if (!workspace && align256(size.seg_state) + size.shared_parts + size.channel_parts) return set_error(TFA_ERR_INVALID, "null workspace");
+  if (const int rc = check_aligned(kept, workspace)) return rc;
   p.lengths = reinterpret_cast<const long long*>(lengths);
   p.state_in = state_in, p.kept = static_cast<float*>(const_cast<void*>(kept));
   p.dy = g.grad_y, p.dstate_out = g.grad_state_out;

@@ -298,7 +298,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
 
     x, dt, z (batch, frames, channels), b, c (batch, frames, groups, states): one dtype of float32, bfloat16, float16; views of
     larger projections are taken as they are.  Neighbouring channels share a group of b and c.  a (channels, states) float32, at
-    most 0 where steps are positive (above it states grow); d (skip) and dt_bias (channels,), float32 or x's dtype.  Steps are
+    most 0 where steps are positive (above it states grow; -inf: no memory); d (skip) and dt_bias (channels,), float32 or x's dtype.  Steps are
     softplus(dt + dt_bias), or dt + dt_bias without softplus; z gates the output by silu(z).  Up to 64 states.
     initial_state: (batch, channels, states) float32.  lengths: (batch,) whole numbers; frames at and past a sequence's length
     are padding, whatever they hold: outputs and gradients are zero there.
