@@ -379,6 +379,50 @@ def test_scan_keeps_what_is_not_finite_to_its_channel_and_later_frames():
             assert not d[0, 20:].any(), name
 
 
+def test_steps_called_natively_and_from_python_agree(monkeypatch):
+    """Operands as the C ABI takes them go to it directly, others are converted or refused first: the same call either way."""
+    from trnfft_amd import state_space
+
+    rows, ch, groups, n = 5, 24, 2, 6
+    v = {k: cuda(w) for k, w in scan_inputs(rows, 1, ch, groups, n, torch.float32, 3)[0].items()}
+    frame = {k: v[k][:, 0] for k in ("x", "dt", "b", "c", "z")}
+    x2, weight, bias = torch.randn(2 * rows, ch, device="cuda")[::2], torch.randn(ch, 4, device="cuda"), torch.randn(ch, device="cuda")
+
+    def steps(x, dt, a, weight):
+        state, taps = v["state"].clone(), torch.ones(rows, 3, ch, device="cuda")
+        versions = state._version, taps._version
+        y = trnfft_amd.selective_scan_step(x, dt, a, frame["b"], frame["c"], state, d=v["d"], z=frame["z"], dt_bias=v["dt_bias"])
+        u = trnfft_amd.causal_conv_step(x2, taps, weight, bias, activation="silu")
+        assert state._version > versions[0] and taps._version > versions[1]
+        return y, state, u, taps
+
+    taken = []
+    direct = state_space.step_here
+    monkeypatch.setattr(state_space, "step_here", lambda *args: taken.append(direct(*args)) or taken[-1])
+    want = steps(frame["x"], frame["dt"], v["a"], weight)
+    assert len(taken) == 2 and all(torch.is_tensor(t) for t in taken)
+    taken.clear()
+    wide = torch.zeros(rows, 2 * ch, device="cuda")
+    wide[:, ::2] = frame["dt"]
+    got = steps(frame["x"], wide[:, ::2], v["a"].t().contiguous().t(), weight.t().contiguous().t())
+    assert taken == [None, None]
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+    monkeypatch.setattr(state_space, "step_here", lambda *args: None)
+    for g, w in zip(steps(frame["x"], frame["dt"], v["a"], weight), want):
+        assert torch.equal(g, w)
+    monkeypatch.undo()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        steps(frame["x"].clone().requires_grad_(), frame["dt"], v["a"], weight)
+    with pytest.raises(ValueError, match="state must be"):
+        trnfft_amd.causal_conv_step(x2, torch.ones(rows, 2, ch, device="cuda"), weight, bias)
+    with pytest.raises(TypeError, match="state must be"):
+        trnfft_amd.causal_conv_step(x2, torch.ones(rows, 3, ch, device="cuda", dtype=torch.float16), weight, bias)
+    with torch.inference_mode():
+        got = trnfft_amd.causal_conv_step(x2, torch.ones(rows, 3, ch, device="cuda"), weight, bias, activation="silu")
+    assert torch.equal(got, want[2])
+
+
 @pytest.mark.parametrize("rows,t", [(0, 5), (3, 0), (0, 0)])
 def test_nothing_to_do(rows, t):
     v, _ = scan_inputs(rows, t, 6, 1, 4, torch.float32, 0, extra=False)

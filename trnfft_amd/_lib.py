@@ -183,6 +183,7 @@ class GradLists(ctypes.Structure):
 
 _lib = None
 _table = None
+_steps: dict = {}
 _lock = threading.Lock()
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -304,6 +305,18 @@ def tensor_table():
                                "`python -m trnfft_amd.csrc.build`") from e
         _table = table
     return _table
+
+
+def native_step(name: str):
+    """The caller of a stream's step (csrc/tensor_table.cpp) and the address of the C entry that it calls, loaded once."""
+    step = _steps.get(name)
+    if step is None:
+        tensor_table()
+        from . import _tensor_table
+
+        entry = {"conv_step": "tfa_causal_conv_step", "scan_step": "tfa_selective_scan_step"}[name]
+        step = _steps[name] = getattr(_tensor_table, name), ctypes.cast(getattr(lib(), entry), ctypes.c_void_p).value
+    return step
 
 
 def check(rc: int, what: str) -> None:

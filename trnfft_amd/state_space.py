@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .attention import DTYPES, _features, _on
-from .dispatch import _require_hip, addr, launch, refuse_tangents, target_device
+from .dispatch import _require_hip, _use_hip, addr, launch, refuse_tangents, step_here, target_device
 from .norm import ACTIVATIONS, _channels
 
 _WHOLE = (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8)
@@ -56,19 +56,6 @@ def _wants(*tensors: torch.Tensor | None) -> bool:
 
 def _dense(g: torch.Tensor | None, dev: torch.device) -> torch.Tensor | None:
     return None if g is None else _on(g, dev).contiguous()
-
-
-# A step is a few microseconds of GPU work: operands that are as the kernels take them are passed through with as few questions as that takes.
-def _step_operand(x: torch.Tensor | None, dev: torch.device, index: int) -> torch.Tensor | None:
-    if x is None or (x.get_device() == index and x.stride(-1) == 1 and not x.is_neg()):
-        return x
-    return _features(x, dev)
-
-
-def _step_weights(w: torch.Tensor | None, dev: torch.device, index: int) -> torch.Tensor | None:
-    if w is None or (w.dtype == torch.float32 and w.get_device() == index and w.is_contiguous() and not w.is_neg()):
-        return w
-    return _channels(w, dev)
 
 
 def _tokens(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
@@ -191,6 +178,10 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     in x's dtype on the GPU.  No gradients.
     """
     what = "causal_conv_step"
+    if activation in ACTIVATIONS and _use_hip():  # (as it mostly is: nothing to convert, nothing to refuse)
+        y = step_here(what, "conv_step", state, x, state, weight, bias, ACTIVATIONS[activation])
+        if y is not None:
+            return y
     _check_conv(what, x, weight, bias, activation, 2)
     (b, c), width = x.shape, weight.shape[1]
     if state.shape != (b, width - 1, c):
@@ -202,8 +193,7 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     refuse_tangents(what, x, state, weight, bias)
     _require_hip(what)
     dev, out_dev = _check_state(what, state), x.device
-    at = dev.index
-    x, weight, bias = _step_operand(x, dev, at), _step_weights(weight, dev, at), _step_weights(bias, dev, at)
+    x, weight, bias = _features(x, dev), _channels(weight, dev), _channels(bias, dev)
     desc = _lib.ConvDesc(DTYPES[x.dtype], c, width, ACTIVATIONS[activation], b, 1, x.stride(0), 0)
     y = x.new_empty(b, c)
     launch(what, dev, _lib.lib().tfa_causal_conv_step, desc, addr(x), addr(weight), addr(bias), addr(state), addr(y))
@@ -341,6 +331,10 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     dtype.  state: contiguous float32 on the GPU.  No gradients.
     """
     what = "selective_scan_step"
+    if _use_hip():  # (as it mostly is: nothing to convert, nothing to refuse)
+        y = step_here(what, "scan_step", state, x, dt, a, b, c, state, d, z, dt_bias, softplus)
+        if y is not None:
+            return y
     _check_scan(what, x, dt, a, b, c, d, z, dt_bias, 2)
     rows, channels = x.shape
     if state.shape != (rows, *a.shape):
@@ -352,9 +346,9 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     refuse_tangents(what, x, dt, a, b, c, state, d, z, dt_bias)
     _require_hip(what)
     dev, out_dev = _check_state(what, state), x.device
-    at = dev.index
-    x, dt, b, c, z = (_step_operand(v, dev, at) for v in (x, dt, b, c, z))
-    a, d, dt_bias = _step_weights(a, dev, at), _step_weights(d, dev, at), _step_weights(dt_bias, dev, at)
+    x, dt, b, c = _features(x, dev), _features(dt, dev), _features(b, dev), _features(c, dev)
+    z = None if z is None else _features(z, dev)
+    a, d, dt_bias = _dense(a, dev), _channels(d, dev), _channels(dt_bias, dev)
     (bs, bg, _), (cs, cg, _) = b.stride(), c.stride()
     desc = _lib.ScanDesc(DTYPES[x.dtype], channels, b.shape[1], a.shape[1], int(bool(softplus)), 0, rows, 1, x.stride(0), 0,
                          dt.stride(0), 0, 0 if z is None else z.stride(0), 0, bs, 0, bg, cs, 0, cg)
