@@ -397,8 +397,8 @@ def test_steps_called_natively_and_from_python_agree(monkeypatch):
         return y, state, u, taps
 
     taken = []
-    direct = state_space.step_here
-    monkeypatch.setattr(state_space, "step_here", lambda *args: taken.append(direct(*args)) or taken[-1])
+    direct = state_space._step
+    monkeypatch.setattr(state_space, "_step", lambda *args: taken.append(direct(*args)) or taken[-1])
     want = steps(frame["x"], frame["dt"], v["a"], weight)
     assert len(taken) == 2 and all(torch.is_tensor(t) for t in taken)
     taken.clear()
@@ -408,7 +408,7 @@ def test_steps_called_natively_and_from_python_agree(monkeypatch):
     assert taken == [None, None]
     for g, w in zip(got, want):
         assert torch.equal(g, w)
-    monkeypatch.setattr(state_space, "step_here", lambda *args: None)
+    monkeypatch.setattr(state_space, "_step", lambda *args: None)
     for g, w in zip(steps(frame["x"], frame["dt"], v["a"], weight), want):
         assert torch.equal(g, w)
     monkeypatch.undo()

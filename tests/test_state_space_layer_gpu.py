@@ -9,6 +9,7 @@ import sys
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import trnfft_amd
 from trnfft_amd.nn import StateSpace
@@ -233,6 +234,43 @@ def test_gradients_are_not_differentiated_again_and_states_are_seen_to_change():
     with torch.no_grad():
         trnfft_amd.selective_scan_step(v[0][:, 0], v[1][:, 0], v[2], v[3][:, 0], v[4][:, 0], state)
     assert state._version > version
+
+
+def test_nodes_of_the_graph_are_kept_freed_hooked_and_recomputed():
+    v = operands(rows=2, t=70, ch=24)
+    leaves = [v[0].requires_grad_(), v[2].requires_grad_()]
+    weight = torch.randn(24, 4, device="cuda", requires_grad=True)
+
+    def layer():
+        return trnfft_amd.selective_scan(trnfft_amd.causal_conv(v[0], weight, activation="silu"), *v[1:])
+
+    wanted = [*leaves, weight]
+    y = layer()
+    dy = torch.randn_like(y)
+    want = torch.autograd.grad(y, wanted, dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, wanted, dy), want))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, wanted, dy)
+    # one gradient at a time, and one that is made to be differentiated and then is not
+    for i, leaf in enumerate(wanted):
+        assert torch.equal(torch.autograd.grad(layer(), leaf, dy, create_graph=i == 1)[0], want[i])
+    moved = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: moved.append(t.device.type) or t.cpu(), lambda t: t.cuda()):
+        y = layer()
+    assert len(moved) >= 7 and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, wanted, dy), want))
+    y = torch.utils.checkpoint.checkpoint(layer, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, wanted, dy), want))
+    y = layer()
+    with torch.no_grad():
+        weight.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, wanted, dy)
+
+    def broken(_):
+        raise ValueError("of a hook")
+
+    with torch.autograd.graph.saved_tensors_hooks(broken, lambda t: t), pytest.raises(ValueError, match="of a hook"):
+        layer()
 
 
 def test_the_example_with_this_layer():

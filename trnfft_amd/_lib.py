@@ -183,7 +183,7 @@ class GradLists(ctypes.Structure):
 
 _lib = None
 _table = None
-_steps: dict = {}
+_space = None
 _lock = threading.Lock()
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -307,16 +307,18 @@ def tensor_table():
     return _table
 
 
-def native_step(name: str):
-    """The caller of a stream's step (csrc/tensor_table.cpp) and the address of the C entry that it calls, loaded once."""
-    step = _steps.get(name)
-    if step is None:
-        tensor_table()
-        from . import _tensor_table
-
-        entry = {"conv_step": "tfa_causal_conv_step", "scan_step": "tfa_selective_scan_step"}[name]
-        step = _steps[name] = getattr(_tensor_table, name), ctypes.cast(getattr(lib(), entry), ctypes.c_void_p).value
-    return step
+def state_space():
+    """The native calls of the state space operators (csrc/state_space_calls.cpp), loaded once."""
+    global _space
+    if _space is None:
+        try:
+            from . import _state_space
+        except ImportError as e:
+            raise RuntimeError("trnfft_amd: _state_space.so is missing or was built for another torch; run "
+                               "`python -m trnfft_amd.csrc.build`") from e
+        _state_space.bind(*(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value for name in _state_space.ENTRIES))
+        _space = _state_space
+    return _space
 
 
 def check(rc: int, what: str) -> None:

@@ -1,6 +1,7 @@
 """Build libtrnfft_amd.so (all HIP kernels + the C ABI) for gfx950 with hipcc, in-tree, and
 libtfa_copy.so, the plain-copy kernels bench.py measures the achievable memory rate with; and, with the host compiler,
-_tensor_table.so, which reads lists of tensors for the operators that take them.
+_tensor_table.so, which reads lists of tensors for the operators that take them, and _state_space.so, which makes the state space
+operators' calls and their nodes of autograd's graph.
 
 Usage: python -m trnfft_amd.csrc.build   (or trnfft_amd.csrc.build.build()).
 """
@@ -21,6 +22,8 @@ COPY_LIB = os.path.join(PKG, "libtfa_copy.so")
 COPY_SOURCE = "bench_copy.hip"
 TABLE_LIB = os.path.join(PKG, "_tensor_table.so")
 TABLE_SOURCE = "tensor_table.cpp"
+SPACE_LIB = os.path.join(PKG, "_state_space.so")
+SPACE_SOURCE = "state_space_calls.cpp"
 SOURCES = [
     "plan.hip",
     "kernels_c2c.hip",
@@ -53,6 +56,7 @@ SOURCES = [
 
 CXX = os.environ.get("CXX", "g++")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 FLAGS = [
     "-O3",
     "--offload-arch=gfx950",
@@ -90,20 +94,29 @@ def _link(objs: list[str], out: str) -> None:
     os.replace(tmp, out)
 
 
-def _build_table() -> None:
-    """The CPython module on torch's own headers (torch is loaded before it: its libraries need no search path)."""
+def _build_module(src: str, out: str) -> None:
+    """A CPython module on torch's own headers (torch is loaded before it: its libraries need no search path)."""
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
-    tmp = TABLE_LIB + ".tmp"
-    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
-    for path in (*include_paths(), sysconfig.get_path("include")):
+    tmp = out + ".tmp"
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    for path in (*include_paths(), os.path.join(ROCM, "include"), sysconfig.get_path("include")):
         cmd += ["-isystem", path]
-    cmd += [os.path.join(HERE, TABLE_SOURCE), "-o", tmp, *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    cmd += [os.path.join(HERE, src), "-o", tmp, *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"{CXX} failed for {TABLE_SOURCE}:\n{res.stderr}")
-    os.replace(tmp, TABLE_LIB)
+        raise RuntimeError(f"{CXX} failed for {src}:\n{res.stderr}")
+    os.replace(tmp, out)
+
+
+def _build_table() -> None:
+    _build_module(TABLE_SOURCE, TABLE_LIB)
+
+
+def _build_state_space() -> None:
+    _build_module(SPACE_SOURCE, SPACE_LIB)
 
 
 def build(verbose: bool = False) -> str:
@@ -115,14 +128,15 @@ def build(verbose: bool = False) -> str:
     srcs = SOURCES + [COPY_SOURCE]
     objs = [os.path.join(objdir, s.rsplit(".", 1)[0] + ".o") for s in srcs]
     with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 1)) as ex:
-        table = ex.submit(_build_table)
+        modules = [ex.submit(_build_table), ex.submit(_build_state_space)]
         list(ex.map(lambda so: _compile(*so), zip(srcs, objs)))
-    # (the C ABI needs neither torch's headers nor Python's: it is there also where the table fails)
+    # (the C ABI needs neither torch's headers nor Python's: it is there also where a module fails)
     _link(objs[:-1], LIB)
     _link(objs[-1:], COPY_LIB)
-    table.result()
+    for module in modules:
+        module.result()
     if verbose:
-        print(f"built {LIB}, {COPY_LIB} and {TABLE_LIB}")
+        print(f"built {LIB}, {COPY_LIB}, {TABLE_LIB} and {SPACE_LIB}")
     return LIB
 
 

@@ -165,20 +165,6 @@ def launch(what: str, dev: torch.device, fn, *args) -> None:
         _lib.check(rc, what)
 
 
-def step_here(what: str, step: str, state: torch.Tensor, *args) -> torch.Tensor | None:
-    """A stream's step called natively: its result, or None where an operand has to be converted or refused first, or the state is
-    on another device than the current one."""
-    _require_hip(what)
-    index = state.get_device()
-    if index < 0 or _current_device() != index or getattr(forward_ad, "_current_level", 0) >= 0:
-        return None
-    call, entry = _lib.native_step(step)
-    y = call(entry, _raw_stream(index), index, *args)
-    if type(y) is int:
-        _lib.check(y, what)
-    return y
-
-
 def addr(t: torch.Tensor | None) -> int | None:
     """The data address as the C ABI takes it (None: NULL)."""
     return None if t is None else t.data_ptr()

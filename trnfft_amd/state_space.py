@@ -10,14 +10,12 @@ filter and a few states a channel, however long it runs.  ``causal_conv`` and ``
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
-from torch.autograd.function import once_differentiable
+from torch.autograd import forward_ad
 
 from . import _lib
 from .attention import DTYPES, _features, _on
-from .dispatch import _require_hip, _use_hip, addr, launch, refuse_tangents, step_here, target_device
+from .dispatch import _current_device, _require_hip, _use_hip, addr, launch, refuse_tangents, target_device
 from .norm import ACTIVATIONS, _channels
 
 _WHOLE = (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8)
@@ -71,6 +69,28 @@ def _check_state(what: str, state: torch.Tensor) -> torch.device:
     return state.device
 
 
+def _results(what: str, out, dev: torch.device):
+    """y, or y and the last state, on dev, of a native call's list or status."""
+    if type(out) is int:
+        _lib.check(out, what)
+    out = [v if v.device == dev else v.to(dev) for v in out]
+    return out[0] if len(out) == 1 else tuple(out)
+
+
+def _step(what: str, step: str, state: torch.Tensor, *args) -> torch.Tensor | None:
+    """A stream's step called natively: its result, or None where an operand has to be converted or refused first, or the state is
+    on another device than the current one."""
+    if not _use_hip():
+        return None
+    index = state.get_device()
+    if index < 0 or _current_device() != index or getattr(forward_ad, "_current_level", 0) >= 0:
+        return None
+    y = getattr(_lib.state_space(), step)(index, *args)
+    if type(y) is int:
+        _lib.check(y, what)
+    return y
+
+
 # ---------------------------------------------------------------------------------------------
 # causal convolution
 # ---------------------------------------------------------------------------------------------
@@ -90,47 +110,6 @@ def _check_conv(what: str, x, weight, bias, activation, dims: int) -> None:
         _check_channels(what, c, x.dtype, bias=bias)
     if activation not in ACTIVATIONS:
         raise ValueError(f"{what}: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
-
-
-def _conv_forward(x, weight, bias, state, lengths, activation, want_state: bool):
-    b, t, c = x.shape
-    width, dev, what = weight.shape[1], x.device, "causal_conv"
-    desc = _lib.ConvDesc(DTYPES[x.dtype], c, width, activation, b, t, *x.stride()[:2])
-    y = x.new_empty(b, t, c)
-    last = x.new_empty(b, width - 1, c) if want_state else None
-    launch(what, dev, _lib.lib().tfa_causal_conv, desc, addr(x), addr(weight), addr(bias), addr(lengths), addr(state), addr(y),
-           addr(last))
-    return y, last
-
-
-class _CausalConvFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, state, lengths, activation):
-        ctx.set_materialize_grads(False)
-        ctx.activation = activation
-        ctx.save_for_backward(x, weight, bias, state, lengths)
-        return _conv_forward(x, weight, bias, state, lengths, activation, True)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_y, g_last):
-        x, weight, bias, state, lengths = ctx.saved_tensors
-        (b, t, c), width, dev, what, need = x.shape, weight.shape[1], x.device, "causal_conv backward", ctx.needs_input_grad
-        desc = _lib.ConvDesc(DTYPES[x.dtype], c, width, ctx.activation, b, t, *x.stride()[:2])
-        g_y = x.new_zeros(b, t, c) if g_y is None else _dense(g_y, dev)
-        g_last = _dense(g_last, dev)
-        d_x = x.new_empty(b, t, c) if need[0] else None
-        d_w = torch.empty_like(weight) if need[1] else None
-        d_b = torch.empty_like(bias) if bias is not None and need[2] else None
-        d_s = torch.empty_like(state) if state is not None and need[3] else None
-        ws = None
-        if need[1] or need[2]:
-            nbytes = ctypes.c_size_t()
-            _lib.check(_lib.lib().tfa_causal_conv_workspace_size(desc, nbytes), what)
-            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
-        launch(what, dev, _lib.lib().tfa_causal_conv_backward, desc, addr(x), addr(weight), addr(bias), addr(lengths), addr(state),
-               addr(g_y), addr(g_last), addr(d_x), addr(d_w), addr(d_b), addr(d_s), addr(ws))
-        return d_x, d_w, d_b, d_s, None, None
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
@@ -161,13 +140,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     dev, out_dev = target_device(x), x.device
     x, weight, bias = _features(x, dev), _channels(weight, dev), _channels(bias, dev)
     state, lengths = _dense(initial_state, dev), _whole_numbers(lengths, dev)
-    if _wants(x, weight, bias, state):
-        y, last = _CausalConvFn.apply(x, weight, bias, state, lengths, ACTIVATIONS[activation])
-    else:
-        y, last = _conv_forward(x, weight, bias, state, lengths, ACTIVATIONS[activation], return_state)
-    if out_dev != dev:
-        y, last = y.to(out_dev), None if last is None else last.to(out_dev)
-    return (y, last) if return_state else y
+    grads = _wants(x, weight, bias, state)
+    return _results(what, _lib.state_space().causal_conv(x, weight, bias, state, lengths, ACTIVATIONS[activation], return_state, grads), out_dev)
 
 
 def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -178,9 +152,9 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     in x's dtype on the GPU.  No gradients.
     """
     what = "causal_conv_step"
-    if activation in ACTIVATIONS and _use_hip():  # (as it mostly is: nothing to convert, nothing to refuse)
-        y = step_here(what, "conv_step", state, x, state, weight, bias, ACTIVATIONS[activation])
-        if y is not None:
+    if activation in ACTIVATIONS:
+        y = _step(what, "conv_step", state, x, state, weight, bias, ACTIVATIONS[activation])
+        if y is not None:  # (as it mostly is: nothing to convert, nothing to refuse)
             return y
     _check_conv(what, x, weight, bias, activation, 2)
     (b, c), width = x.shape, weight.shape[1]
@@ -231,55 +205,6 @@ def _check_scan(what: str, x, dt, a, b, c, d, z, dt_bias, dims: int) -> None:
         _check_channels(what, channels, dtype, d=d, dt_bias=dt_bias)
 
 
-def _scan_desc(x, dt, b, c, z, softplus: bool) -> _lib.ScanDesc:
-    (rows, t, channels), (groups, n) = x.shape, b.shape[2:]
-    return _lib.ScanDesc(DTYPES[x.dtype], channels, groups, n, int(softplus), 0, rows, t, *x.stride()[:2], *dt.stride()[:2],
-                         *((0, 0) if z is None else z.stride()[:2]), *b.stride()[:3], *c.stride()[:3])
-
-
-def _scan_forward(x, dt, a, b, c, d, z, dt_bias, state, lengths, softplus: bool, want_state: bool, want_kept: bool):
-    (rows, t, channels), n, dev, what = x.shape, a.shape[1], x.device, "selective_scan"
-    desc = _scan_desc(x, dt, b, c, z, softplus)
-    sizes = [ctypes.c_size_t() for _ in range(3)]
-    _lib.check(_lib.lib().tfa_selective_scan_sizes(desc, *sizes), what)
-    kept, ws = (torch.empty(s.value, dtype=torch.uint8, device=dev) if s.value and want else None
-                for s, want in zip(sizes, (want_kept, True)))
-    y = x.new_empty(rows, t, channels)
-    last = torch.empty(rows, channels, n, dtype=torch.float32, device=dev) if want_state else None
-    launch(what, dev, _lib.lib().tfa_selective_scan, desc, addr(x), addr(dt), addr(a), addr(b), addr(c), addr(d), addr(z),
-           addr(dt_bias), addr(lengths), addr(state), addr(y), addr(last), addr(kept), addr(ws))
-    return y, last, kept
-
-
-class _SelectiveScanFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, dt, a, b, c, d, z, dt_bias, state, lengths, softplus):
-        ctx.set_materialize_grads(False)
-        ctx.softplus = softplus
-        y, last, kept = _scan_forward(x, dt, a, b, c, d, z, dt_bias, state, lengths, softplus, True, True)
-        ctx.save_for_backward(x, dt, a, b, c, d, z, dt_bias, state, lengths, kept)
-        return y, last
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_y, g_last):
-        x, dt, a, b, c, d, z, dt_bias, state, lengths, kept = ctx.saved_tensors
-        dev, what = x.device, "selective_scan backward"
-        desc = _scan_desc(x, dt, b, c, z, ctx.softplus)
-        sizes = [ctypes.c_size_t() for _ in range(3)]
-        _lib.check(_lib.lib().tfa_selective_scan_sizes(desc, *sizes), what)
-        ws = torch.empty(sizes[2].value, dtype=torch.uint8, device=dev) if sizes[2].value else None
-        g_y = torch.zeros(x.shape, dtype=x.dtype, device=dev) if g_y is None else _dense(g_y, dev)
-        g_last = _dense(g_last, dev)
-        grads = [torch.empty(v.shape, dtype=v.dtype, device=dev) if v is not None and need else None
-                 for v, need in zip((x, dt, a, b, c, d, z, dt_bias, state), ctx.needs_input_grad)]
-        d_x, d_dt, d_a, d_b, d_c, d_d, d_z, d_bias, d_state = map(addr, grads)
-        table = _lib.ScanGrads(addr(g_y), addr(g_last), d_x, d_dt, d_b, d_c, d_z, d_a, d_d, d_bias, d_state)
-        launch(what, dev, _lib.lib().tfa_selective_scan_backward, desc, addr(x), addr(dt), addr(a), addr(b), addr(c), addr(d),
-               addr(z), addr(dt_bias), addr(lengths), addr(state), addr(kept), table, addr(ws))
-        return *grads, None, None
-
-
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, *,
                    d: torch.Tensor | None = None, z: torch.Tensor | None = None, dt_bias: torch.Tensor | None = None,
                    softplus: bool = True, initial_state: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
@@ -313,13 +238,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     z = None if z is None else _tokens(z, dev)
     a, d, dt_bias = _dense(a, dev), _channels(d, dev), _channels(dt_bias, dev)
     state, lengths = _dense(initial_state, dev), _whole_numbers(lengths, dev)
-    if _wants(x, dt, a, b, c, d, z, dt_bias, state):
-        y, last = _SelectiveScanFn.apply(x, dt, a, b, c, d, z, dt_bias, state, lengths, bool(softplus))
-    else:
-        y, last, _ = _scan_forward(x, dt, a, b, c, d, z, dt_bias, state, lengths, bool(softplus), return_state, False)
-    if out_dev != dev:
-        y, last = y.to(out_dev), None if last is None else last.to(out_dev)
-    return (y, last) if return_state else y
+    grads = _wants(x, dt, a, b, c, d, z, dt_bias, state)
+    return _results(what, _lib.state_space().selective_scan(x, dt, a, b, c, d, z, dt_bias, state, lengths, softplus, return_state, grads), out_dev)
 
 
 def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor,
@@ -331,10 +251,9 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     dtype.  state: contiguous float32 on the GPU.  No gradients.
     """
     what = "selective_scan_step"
-    if _use_hip():  # (as it mostly is: nothing to convert, nothing to refuse)
-        y = step_here(what, "scan_step", state, x, dt, a, b, c, state, d, z, dt_bias, softplus)
-        if y is not None:
-            return y
+    y = _step(what, "scan_step", state, x, dt, a, b, c, state, d, z, dt_bias, softplus)
+    if y is not None:  # (as it mostly is: nothing to convert, nothing to refuse)
+        return y
     _check_scan(what, x, dt, a, b, c, d, z, dt_bias, 2)
     rows, channels = x.shape
     if state.shape != (rows, *a.shape):
