@@ -200,6 +200,40 @@ def test_a_captured_training_pass():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_a_capture_refuses_leaves_whose_eager_graph_lives():
+    """(Its backward pass would end the process.)  Leaves that are used through other nodes are found as well."""
+    v = operands(t=40)
+    x = v[0].requires_grad_()
+    w = torch.randn(24, 4, device="cuda", dtype=torch.float64, requires_grad=True)
+    eager = trnfft_amd.selective_scan(trnfft_amd.causal_conv(x * 2.0, w.float()), *v[1:])
+    eager.sum().backward(retain_graph=True)
+    graph, mark = torch.cuda.CUDAGraph(), torch.zeros(3, device="cuda")
+    with torch.cuda.graph(graph):
+        mark.add_(1.0)
+        with pytest.raises(RuntimeError, match="eager pass"):
+            trnfft_amd.selective_scan(x, *v[1:])
+        with pytest.raises(RuntimeError, match="eager pass"):
+            trnfft_amd.causal_conv(v[1], w.float())
+        with pytest.raises(RuntimeError, match="eager pass"):
+            trnfft_amd.causal_conv(x.tanh(), w.detach().float())
+        with torch.no_grad():
+            y = trnfft_amd.selective_scan(x, *v[1:])
+    graph.replay()
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        assert torch.equal(y, trnfft_amd.selective_scan(x, *v[1:])) and torch.equal(mark, torch.ones_like(mark))
+    want = torch.autograd.grad(trnfft_amd.selective_scan(x, *v[1:]).square().sum(), x)[0]
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = trnfft_amd.selective_scan(x, *v[1:])
+        g, = torch.autograd.grad(y, x, 2.0 * y.detach())
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(g, want)
+
+
 def test_results_do_not_depend_on_timing():
     leaves = [v.requires_grad_() for v in operands(rows=3, t=900, ch=130, seed=4)]
 

@@ -11,11 +11,14 @@
 
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/trnfft_amd.h"
@@ -25,6 +28,8 @@
 #include <iterator>
 #include <optional>
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 namespace {
 
@@ -84,6 +89,31 @@ variable_list once(variable_list grads) {
       if (g.defined()) g = Once::apply(g.requires_grad_());
   }
   return grads;
+}
+
+// A leaf's gradients go to a node that belongs to the stream on which the leaf was first used, for as long as any graph with it lives.
+// A backward pass that is captured cannot reach one of the default stream: the attempt ends the process.  So a captured call refuses to
+// become part of such a graph.
+void refuse_eager_graphs(const at::Tensor* tensors, size_t count) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+  std::unordered_set<torch::autograd::Node*> seen;
+  const auto add = [&](const std::shared_ptr<torch::autograd::Node>& node) {
+    if (node && seen.insert(node.get()).second) todo.push_back(node);
+  };
+  for (size_t i = 0; i < count; ++i)
+    if (tensors[i].defined() && tensors[i].requires_grad())
+      add(tensors[i].grad_fn() ? tensors[i].grad_fn() : torch::autograd::impl::try_get_grad_accumulator(tensors[i]));
+  while (!todo.empty()) {
+    const auto node = todo.back();
+    todo.pop_back();
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) {
+      const auto stream = node->stream();
+      TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(stream->device_index()).id(),
+                  "a graph of an eager pass through these tensors lives: delete its results before a pass through them is captured");
+    }
+    for (const auto& edge : node->next_edges()) add(edge.function);
+  }
 }
 
 // Room for the gradients of the first N of a node's operands, where they are wanted (operands that were left out have no edge in the graph).
@@ -274,6 +304,7 @@ PyObject* conv_of(PyObject* args) {
   if (!PyArg_ParseTuple(args, "OOOOOipp", o, o + 1, o + 2, o + 3, o + 4, &activation, &want_state, &grads)) return nullptr;
   at::Tensor t[5];
   for (int i = 0; i < 5; ++i) t[i] = argument(o[i]);
+  if (grads) refuse_eager_graphs(t, 4);
   variable_list out;
   {
     const WithoutGil released;
@@ -290,6 +321,7 @@ PyObject* scan_of(PyObject* args) {
     return nullptr;
   at::Tensor t[10];
   for (int i = 0; i < 10; ++i) t[i] = argument(o[i]);
+  if (grads) refuse_eager_graphs(t, 9);
   variable_list out;
   {
     const WithoutGil released;
