@@ -184,6 +184,7 @@ class GradLists(ctypes.Structure):
 _lib = None
 _table = None
 _space = None
+_norm = None
 _lock = threading.Lock()
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -305,6 +306,19 @@ def tensor_table():
                                "`python -m trnfft_amd.csrc.build`") from e
         _table = table
     return _table
+
+
+def grad_norm_call(*args):
+    """The norm or clipping of a list of gradients, called natively (csrc/tensor_table.cpp)."""
+    global _norm
+    if _norm is None:
+        tensor_table()
+        from ._tensor_table import norm
+
+        _norm = norm, tuple(ctypes.cast(getattr(lib(), name), ctypes.c_void_p).value
+                            for name in ("tfa_grad_norm_workspace_size", "tfa_grad_norm", "tfa_clip_grads"))
+    call, entries = _norm
+    return call(*args, *entries)
 
 
 def state_space():

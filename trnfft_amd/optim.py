@@ -8,13 +8,12 @@ s (c / 255)^4 of uint8 codes (at least 1 where there is any).  The reference has
 
 from __future__ import annotations
 
-import ctypes
 
 import torch
 
 from . import _lib
 from .attention import DTYPES, _on
-from .dispatch import _require_hip, launch
+from .dispatch import _raw_stream, _require_hip, launch
 
 BLOCK = 256  # values that share a scale
 
@@ -97,23 +96,12 @@ def _norm_call(what: str, grads: list, max_norm: float | None) -> torch.Tensor:
     if not types <= DTYPES.keys():
         raise TypeError(f"{what}: float32, bfloat16 or float16 gradients expected, got {(types - DTYPES.keys()).pop()}")
     _require_hip(what)
-    dev, lib = grads[0].device, _lib.lib()
+    dev = grads[0].device
     if dev.type != "cuda":
         raise ValueError(f"{what}: the gradients must be on the GPU")
-    lists, table = _lib.GradLists(), _lib.tensor_table()
-    for dtype in types:
-        own = grads if len(types) == 1 else [g for g in grads if g.dtype == dtype]
-        lists.tensors[DTYPES[dtype]] = table(what, ("gradients",), (own,), (dtype,), dev.index)
-        lists.count[DTYPES[dtype]] = len(own)
-    nbytes = ctypes.c_size_t()
-    _lib.check(lib.tfa_grad_norm_workspace_size(lists, nbytes), what)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-    if max_norm is None:
-        launch(what, dev, lib.tfa_grad_norm, lists, norm.data_ptr(), ws.data_ptr())
-    else:
-        launch(what, dev, lib.tfa_clip_grads, lists, max_norm, norm.data_ptr(), ws.data_ptr())
-        torch.autograd.graph.increment_version(grads)
+    norm = _lib.grad_norm_call(what, grads, max_norm, dev.index, _raw_stream(dev.index))
+    if type(norm) is int:
+        _lib.check(norm, what)
     return norm
 
 
