@@ -271,6 +271,22 @@ def test_scan_of_steps_as_they_are(shape, extra):
     check_scan(shape, torch.float32, extra, softplus=False, seed=5)
 
 
+@pytest.mark.parametrize("dtype", list(TOL))
+@pytest.mark.parametrize("shape", [(2, 45, 33, 1, 9), (3, 33, 40, 2, 11), (2, 130, 18, 1, 15), (1, 255, 17, 1, 10), (2, 64, 32, 1, 16),
+                                   (2, 32, 130, 1, 14)], ids=str)
+def test_scan_of_two_waves_a_channel(shape, dtype):
+    """9 to 16 states: half of them to a wave each, with odd and even numbers of tiles and halves of one state to eight."""
+    for extra in (False, True):
+        check_scan(shape, dtype, extra, softplus=True, seed=11)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(161, 8, 250, 1, 16), (41, 31, 1000, 8, 16)], ids=str)
+def test_scan_of_many_rows_and_channels(shape, dtype):
+    """More waves than that is done for."""
+    check_scan(shape, dtype, True, softplus=True, seed=12)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shape", [(1, 1300, 20, 1, 16), (2, 700, 5, 1, 6), (3, 513, 36, 2, 40)], ids=str)
 def test_scan_in_segments(shape, dtype):

@@ -109,6 +109,8 @@ static long long scan_tiles(const ScanArgs& p) {
 }
 long long scan_waves(const ScanArgs& p) { return p.batch * p.groups * scan_tiles(p); }
 
+bool scan_has_pairs(const ScanArgs& p) { return scan_shape(p.n).lanes == 4 && scan_shape(p.n).each == 4; }
+
 static long long share_parts(const ScanArgs& p) {
   const int lanes = scan_shape(p.n).lanes, waves = lanes == 4 ? kBackWaves<4> : lanes == 8 ? kBackWaves<8> : kBackWaves<16>;
   return (scan_tiles(p) + waves - 1) / waves;

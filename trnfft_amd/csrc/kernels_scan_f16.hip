@@ -1,5 +1,5 @@
-// The selective scan over whole sequences (scan_blocks.h): fp16 operands.
-#include "scan_blocks.h"
+// The selective scan over whole sequences (scan_blocks.h, scan_pairs.h): fp16 operands.
+#include "scan_pairs.h"
 
 namespace tfa {
 

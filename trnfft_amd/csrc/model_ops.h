@@ -264,6 +264,7 @@ struct ScanSizes {
   size_t kept, seg_state, seg_steps, shared_parts, channel_parts;
 };
 long long scan_waves(const ScanArgs& p);  // of a segment
+bool scan_has_pairs(const ScanArgs& p);   // whether two waves can take the same channels, forward
 ScanSizes scan_sizes(const ScanArgs& p);
 hipError_t launch_scan_forward(const ScanArgs& p);
 hipError_t launch_scan_backward(const ScanArgs& p);

@@ -6,6 +6,8 @@
 //   ds_t = x_t sum_n g_t[n] b_t[n] + sum_n a[n] f_t[n],  dx_t = s_t sum_n g_t[n] b_t[n] + d v_t,  da[n] = sum_t s_t f_t[n],
 //   where f_t = g_t e_t h_{t-1},  dz_t = dy_t silu'(z_t) (sum_n c_t[n] h_t[n] + d x_t)
 //
+// (scan_pairs.h: two waves for the same channels.)
+//
 // A wave takes 64 / Q channels of a row and group, Q lanes a channel with R states each (4 x 1, 2 or 4 up to 16 states, 8 and 16 x 4 above), and walks
 // along the tokens in tiles of 16.  For what belongs to a channel and token alone (softplus, gates, loads, stores) lane q of a channel takes
 // every Q-th token, so nothing of it is done twice; the tokens' s and s x go to the channel's lanes through LDS, as do b and
@@ -43,7 +45,8 @@ struct ScanPlace {
 
 // Ragged rows are given out by length, so that the compute units' sums of them are about the same: the longest first, and every other layer
 // of workgroups over the 256 compute units from the shortest on (a wave that starts late has little to do).  64 rows of up to 626 tokens, 512
-// channels of 16 states, two workgroups a compute unit: 80.5 us, in their own order 88.6.  Batches of more rows than threads keep their order.
+// channels of 16 states by scan_forward_kernel, two workgroups a compute unit: 80.5 us, in their own order 88.6.  Batches of more rows than threads
+// keep their order.
 template <int THREADS>
 __device__ __forceinline__ long long scan_row(const ScanArgs& p, long long slot, int blocks) {
   if (!p.lengths || p.batch > THREADS || p.batch == 1) return slot;
@@ -65,15 +68,15 @@ __device__ __forceinline__ long long scan_row(const ScanArgs& p, long long slot,
   return found;
 }
 
-template <int Q, int WAVES>
+template <int Q, int WAVES, int SPLIT = 1>
 __device__ __forceinline__ ScanPlace<Q> scan_place(const ScanArgs& p, long long block) {
   ScanPlace<Q> s;
-  const int each = p.channels / p.groups, tiles = (each + s.kChannels - 1) / s.kChannels, across = (tiles + WAVES - 1) / WAVES;
+  const int each = p.channels / p.groups, tiles = (each + s.kChannels - 1) / s.kChannels, across = (tiles + WAVES / SPLIT - 1) / (WAVES / SPLIT);
   s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   s.lane = threadIdx.x % 64;
   s.q = s.lane / s.kChannels;
   s.c = s.lane % s.kChannels;
-  s.tile = (int)(block % across) * WAVES + s.wave;
+  s.tile = (int)(block % across) * (WAVES / SPLIT) + s.wave / SPLIT;
   block /= across;
   s.group = (int)(block % p.groups);
   block /= p.groups;
@@ -93,6 +96,13 @@ __device__ __forceinline__ ScanPlace<Q> scan_place(const ScanArgs& p, long long 
 __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
+}
+
+// A workgroup's barrier for what it shares in LDS: loads and stores of memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 constexpr int kPlaneRow = kScanTile + 4;  // words of a channel's tokens: rows at 16 bytes that spread over the banks
@@ -542,7 +552,7 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
     if (p.ddt) store_tokens<T, Q>(static_cast<T*>(p.ddt) + at, p.channels, s, left, all, ga);
     if (p.dz) store_tokens<T, Q>(static_cast<T*>(p.dz) + at, p.channels, s, left, all, ys);
     if (!p.shared_parts) return;
-    __syncthreads();
+    lds_barrier();
     constexpr int kRow = 2 * Q * R;
     float* const to = p.shared_parts + (((s.tile / kWaves * p.batch + s.row) * p.tokens + t0) * p.groups + s.group) * kRow;
     for (int i = threadIdx.x; i < left * kRow; i += 64 * kWaves) {
@@ -732,40 +742,12 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
 
 enum ScanMode { kScanSums, kScanForward, kScanBackSums, kScanBackward };
 
-template <typename T, int Q, int R>
-hipError_t scan_launch(const ScanArgs& p, ScanMode mode) {
-  const int waves = mode == kScanBackSums || mode == kScanBackward ? kBackWaves<Q> : kScanWaves;
-  const long long tiles = (p.channels / p.groups + 64 / Q - 1) / (64 / Q);
-  // (the last segment's sums are not needed, nor are the first's backwards)
-  const int segments = mode == kScanSums || mode == kScanBackSums ? p.segments - 1 : p.segments;
-  const long long blocks = (tiles + waves - 1) / waves * p.groups * p.batch * segments;
-  for (long long first = 0; first < blocks; first += max_blocks(64 * waves)) {
-    const dim3 grid((unsigned)std::min(blocks - first, max_blocks(64 * waves))), block(64 * waves);
-    if (mode == kScanSums) hipLaunchKernelGGL((scan_forward_kernel<T, Q, R, false>), grid, block, 0, p.stream, p, first);
-    if (mode == kScanForward) hipLaunchKernelGGL((scan_forward_kernel<T, Q, R, true>), grid, block, 0, p.stream, p, first);
-    if (mode == kScanBackSums) hipLaunchKernelGGL((scan_backward_kernel<T, Q, R, true>), grid, block, 0, p.stream, p, first);
-    if (mode == kScanBackward) hipLaunchKernelGGL((scan_backward_kernel<T, Q, R, false>), grid, block, 0, p.stream, p, first);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  return hipSuccess;
-}
-
 // Lanes of a channel, and the states that each has
 struct ScanShape {
   int lanes, each;
 };
 inline ScanShape scan_shape(int n) {
   return n <= 4 ? ScanShape{4, 1} : n <= 8 ? ScanShape{4, 2} : n <= 16 ? ScanShape{4, 4} : n <= 32 ? ScanShape{8, 4} : ScanShape{16, 4};
-}
-
-template <typename T>
-hipError_t scan_typed(const ScanArgs& p, ScanMode mode) {
-  const ScanShape s = scan_shape(p.n);
-  if (s.lanes == 4 && s.each == 1) return scan_launch<T, 4, 1>(p, mode);
-  if (s.lanes == 4 && s.each == 2) return scan_launch<T, 4, 2>(p, mode);
-  if (s.lanes == 4) return scan_launch<T, 4, 4>(p, mode);
-  return s.lanes == 8 ? scan_launch<T, 8, 4>(p, mode) : scan_launch<T, 16, 4>(p, mode);
 }
 
 hipError_t scan_f32(const ScanArgs& p, ScanMode mode);

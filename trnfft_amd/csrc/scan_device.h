@@ -75,6 +75,15 @@ struct RowLane {
         : "=&v"(out0[0]), "=&v"(out0[1]), "=&v"(out0[2]), "=&v"(out0[3]), "=&v"(out1[0]), "=&v"(out1[1]), "=&v"(out1[2]), "=&v"(out1[3])
         : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(u0), "v"(u1), [t] "n"(T), [n] "n"(T + 1));
   }
+  static __device__ __forceinline__ void products(const float (&x)[2], float u0, float u1, float (&out0)[2], float (&out1)[2]) {
+    asm("s_nop 1\n\t"
+        "v_mul_f32_dpp %0, %4, %6" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %1, %5, %6" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %2, %4, %7" TFA_ROW_AT("n")
+        "v_mul_f32_dpp %3, %5, %7" TFA_ROW_AT("n")
+        : "=&v"(out0[0]), "=&v"(out0[1]), "=&v"(out1[0]), "=&v"(out1[1])
+        : "v"(x[0]), "v"(x[1]), "v"(u0), "v"(u1), [t] "n"(T), [n] "n"(T + 1));
+  }
   // sum0 = x (of T) . y0, sum1 = x (of T + 1) . y1
   template <int R>
   static __device__ __forceinline__ void dots(const float (&x)[R], const float (&y0)[R], const float (&y1)[R], float& sum0, float& sum1) {
@@ -96,6 +105,15 @@ struct RowLane {
         : "=&v"(sum0), "=&v"(sum1)
         : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(y0[0]), "v"(y0[1]), "v"(y0[2]), "v"(y0[3]), "v"(y1[0]), "v"(y1[1]),
           "v"(y1[2]), "v"(y1[3]), [t] "n"(T), [n] "n"(T + 1));
+  }
+  static __device__ __forceinline__ void dots(const float (&x)[2], const float (&y0)[2], const float (&y1)[2], float& sum0, float& sum1) {
+    asm("s_nop 1\n\t"
+        "v_mul_f32_dpp %0, %2, %4" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %1, %2, %6" TFA_ROW_AT("n")
+        "v_fmac_f32_dpp %0, %3, %5" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %1, %3, %7" TFA_ROW_AT("n")
+        : "=&v"(sum0), "=&v"(sum1)
+        : "v"(x[0]), "v"(x[1]), "v"(y0[0]), "v"(y0[1]), "v"(y1[0]), "v"(y1[1]), [t] "n"(T), [n] "n"(T + 1));
   }
   // sum += x (of T) u
   template <int R>
@@ -139,6 +157,18 @@ struct RowLane {
         : "+&v"(g[0]), "+&v"(g[1]), "+&v"(g[2]), "+&v"(g[3]), "=&v"(sum_b), "=&v"(sum_c)
         : "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "v"(c[0]), "v"(c[1]), "v"(c[2]), "v"(c[3]), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]),
           "v"(u), [t] "n"(T));
+  }
+  static __device__ __forceinline__ void reverse(const float (&b)[2], const float (&c)[2], float u, const float (&h)[2], float (&g)[2], float& sum_b,
+                                                 float& sum_c) {
+    asm("s_nop 1\n\t"
+        "v_fmac_f32_dpp %0, %6, %10" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %1, %7, %10" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %3, %6, %8" TFA_ROW_AT("t")
+        "v_mul_f32_dpp %2, %4, %0" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %3, %7, %9" TFA_ROW_AT("t")
+        "v_fmac_f32_dpp %2, %5, %1" TFA_ROW_AT("t")
+        : "+&v"(g[0]), "+&v"(g[1]), "=&v"(sum_b), "=&v"(sum_c)
+        : "v"(b[0]), "v"(b[1]), "v"(c[0]), "v"(c[1]), "v"(h[0]), "v"(h[1]), "v"(u), [t] "n"(T));
   }
 };
 #undef TFA_ROW_AT
