@@ -526,8 +526,10 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
   ScanTokens<T, Q> x, dt, z, dy;
   ScanRows<T, Q, R> b, c;
   States<R> h0 = {};
+  unsigned kept_lane = s.lane * (unsigned)sizeof(h0);
   const auto fetch = [&](long long t0) {
     const int left = tile_left(end, t0);
+    asm volatile("" : "+v"(kept_lane));
     dt.load(pdt + t0 * p.dt_st, p.dt_st, s, left);
     dy.load(pdy + t0 * p.channels, p.channels, s, left);
     c.load(pc + t0 * p.c_st, p.c_st, p.n, c_whole, s.lane, left);
@@ -536,7 +538,8 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
       x.load(px + t0 * p.x_st, p.x_st, s, left);
       b.load(pb + t0 * p.b_st, p.b_st, p.n, b_whole, s.lane, left);
       if (t0 > 0)
-        h0 = *lane_address(kept + (t0 / kScanStretch - 1) * 64, s.lane * (unsigned)sizeof(h0));
+        // (kept_lane: a register of its own.  An address in one that the other way loads into is waited for, and with it the loads above.)
+        h0 = *reinterpret_cast<const States<R>*>(reinterpret_cast<const char*>(kept + (t0 / kScanStretch - 1) * 64) + kept_lane);
       else
         h0 = p.state_in ? load_states<R>(p.state_in + (s.row * p.channels + channel) * p.n, p.n, s.q, s.valid) : States<R>{};
     }
