@@ -294,6 +294,29 @@ def test_scan_in_segments(shape, dtype):
     check_scan(shape, dtype, True, softplus=True, seed=7)
 
 
+@pytest.mark.parametrize("t,end", [(1056, 1056), (1090, 1071), (1090, 300)])
+def test_scan_in_long_segments(t, end):
+    """Two segments backwards, whose sums are made in halves (the definition on the GPU, in float64)."""
+    ch = 16400
+    v, _ = scan_inputs(1, t, ch, 1, 1, torch.float32, 8, extra=False)
+    names = list(k for k in v if v[k] is not None)
+    ref = {k: v[k].double().cuda().requires_grad_() for k in names}
+    h, ys = torch.zeros(1, ch, 1, dtype=torch.float64, device="cuda"), []
+    for x, dt, b, c in list(zip(*(ref[k].unbind(1) for k in ("x", "dt", "b", "c"))))[:end]:
+        s = torch.logaddexp(dt, torch.zeros_like(dt))
+        h = torch.exp(s[..., None] * ref["a"]) * h + (s * x)[..., None] * b
+        ys.append((h * c).sum(-1))
+    y_ref = torch.nn.functional.pad(torch.stack(ys, 1), (0, 0, 0, t - end))
+    own = {k: cuda(v[k]).requires_grad_() for k in names}
+    y, last = scan(own, torch.tensor([end]))
+    dy, dlast = torch.randn_like(y), torch.randn_like(last)
+    want = torch.autograd.grad([y_ref, h], list(ref.values()), [dy.double(), dlast.double()])
+    got = torch.autograd.grad([y, last], list(own.values()), [dy, dlast])
+    assert rel(y, y_ref.cpu()) <= 2e-6 and rel(last, h.cpu()) <= 2e-6
+    for name, w, g in zip(names, want, got):
+        assert rel(g, w.cpu()) <= (SUMS if name == "a" else 4e-6), name
+
+
 @pytest.mark.parametrize("dtype", list(TOL))
 @pytest.mark.parametrize("ch,groups,n,softplus", [(48, 1, 16, True), (10, 2, 3, True), (7, 1, 21, False), (33, 3, 64, True),
                                                   (260, 1, 8, True)])

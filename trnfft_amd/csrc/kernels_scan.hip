@@ -22,23 +22,24 @@ __global__ __launch_bounds__(64) void scan_join_kernel(ScanArgs p, int lanes, bo
   const float* from = reverse ? p.dstate_out : p.state_in;
   States<R> s = {};
   if (from) s = load_states<R>(from + (row * p.channels + channel) * p.n, p.n, q, valid);
-  // sixteen segments' sums on their way at a time (the last one has none, and nothing comes behind it)
+  // sixteen segments' sums on their way at a time
   constexpr int U = 16;
-  for (int k0 = 0; k0 < p.segments; k0 += U) {
+  const int parts = p.segments * p.fine, sums = parts - p.fine;  // (the last segment's have none)
+  for (int k0 = 0; k0 <= sums; k0 += U) {
     States<R> sum[U];
     float steps[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int k = min(k0 + i, p.segments - 2);
-      const long long at = ((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane;
+      const int k = min(k0 + i, sums - 1);
+      const long long at = ((reverse ? parts - 1 - k : k) * units + unit) * 64 + lane;
       sum[i] = reinterpret_cast<const States<R>*>(p.seg_state)[at];
       steps[i] = p.seg_steps[at];
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int k = k0 + i;
-      if (k >= p.segments) break;
-      reinterpret_cast<States<R>*>(p.seg_state)[((reverse ? p.segments - 1 - k : k) * units + unit) * 64 + lane] = s;
+      if (k > sums) break;
+      reinterpret_cast<States<R>*>(p.seg_state)[((reverse ? parts - 1 - k : k) * units + unit) * 64 + lane] = s;
 #pragma unroll
       for (int r = 0; r < R; ++r) s.v[r] = __builtin_fmaf(__builtin_amdgcn_exp2f(steps[i] * a.v[r]), s.v[r], sum[i].v[r]);
     }
@@ -119,7 +120,7 @@ static long long share_parts(const ScanArgs& p) {
 ScanSizes scan_sizes(const ScanArgs& p) {
   ScanSizes s;
   const ScanShape shape = scan_shape(p.n);
-  const size_t lanes = (size_t)scan_waves(p) * 64, of_segments = p.segments > 1 ? p.segments * lanes : 0;
+  const size_t lanes = (size_t)scan_waves(p) * 64, of_segments = p.segments > 1 ? p.segments * p.fine * lanes : 0;
   s.kept = p.tokens > 0 ? (p.tokens - 1) / kScanStretch * lanes * shape.each * sizeof(float) : 0;
   s.seg_state = of_segments * shape.each * sizeof(float);
   s.seg_steps = of_segments * sizeof(float);

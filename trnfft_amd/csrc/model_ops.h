@@ -253,7 +253,8 @@ struct ScanArgs {
   float* shared_parts;   // sums over workgroups' channels of db and dc
   float* channel_parts;  // sums over rows and segments of da, dd and ddt_bias
   int segments;
-  long long seg_tokens;  // a multiple of kScanStretch
+  long long seg_tokens;  // a multiple of kScanStretch, and of as many times `fine`
+  int fine;              // parts of a segment whose sums are made by themselves
   hipStream_t stream;
 };
 constexpr int kScanTile = 16;     // tokens that are worked on together

@@ -370,7 +370,8 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
   const ScanPlace<Q> s = scan_place<Q, kScanWaves>(p, first_block + blockIdx.x);
   if (s.idle) return;
   float *const lb = rows[s.wave][0], *const lc = rows[s.wave][1], *const ls = planes[s.wave][0], *const lu = planes[s.wave][1];
-  const long long seg_begin = s.seg * p.seg_tokens, seg_end = min(p.tokens, seg_begin + p.seg_tokens), end = min(scan_end(p, s.row), seg_end);
+  const long long seg_tokens = OUT ? p.seg_tokens : p.seg_tokens / p.fine;
+  const long long seg_begin = s.seg * seg_tokens, seg_end = min(p.tokens, seg_begin + seg_tokens), end = min(scan_end(p, s.row), seg_end);
 
   const T* px = static_cast<const T*>(p.x) + s.row * p.x_sb + seg_begin * p.x_st + s.base;
   const T* pdt = static_cast<const T*>(p.dt) + s.row * p.dt_sb + seg_begin * p.dt_st + s.base;
@@ -387,7 +388,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
   const float bias = p.dt_bias ? p.dt_bias[channel] : 0.0f, skip = p.d ? p.d[channel] : 0.0f;
   if (OUT) {
     if (p.segments > 1)
-      h = reinterpret_cast<const States<R>*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane];
+      h = reinterpret_cast<const States<R>*>(p.seg_state)[(s.seg * p.fine * s.units + s.unit) * 64 + s.lane];
     else if (p.state_in)
       h = load_states<R>(p.state_in + (s.row * p.channels + channel) * p.n, p.n, s.q, s.valid);
   }
@@ -492,13 +493,14 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
   __shared__ float planes[kWaves][SUM ? 2 : 6][kPlaneWords<Q>];
   __shared__ float shares[2][SUM ? 1 : kWaves][SUM ? 1 : kScanTile * 2 * Q * R];  // of this tile and the one before
   ScanPlace<Q> s = scan_place<Q, kWaves>(p, first_block + blockIdx.x);
-  if (SUM) ++s.seg;  // (nothing comes before the first segment)
+  if (SUM) s.seg += p.fine;  // (nothing comes before the first segment)
   if (SUM && s.idle) return;  // (else it takes part in the barriers)
   float *const lb = rows[s.wave][0], *const lc = rows[s.wave][1];
   // of every channel and token: s, dy silu(z), s x, and what its own lane needs again: x, the slope of s by dt, dy silu'(z)
   float *const ls = planes[s.wave][0], *const lv = planes[s.wave][1], *const lu = planes[s.wave][SUM ? 0 : 2];
   float *const lx = planes[s.wave][SUM ? 0 : 3], *const lslope = planes[s.wave][SUM ? 0 : 4], *const lz = planes[s.wave][SUM ? 0 : 5];
-  const long long seg_begin = s.seg * p.seg_tokens, seg_end = min(p.tokens, seg_begin + p.seg_tokens), end = min(scan_end(p, s.row), seg_end);
+  const long long seg_tokens = SUM ? p.seg_tokens / p.fine : p.seg_tokens;
+  const long long seg_begin = s.seg * seg_tokens, seg_end = min(p.tokens, seg_begin + seg_tokens), end = min(scan_end(p, s.row), seg_end);
 
   const T* const px = static_cast<const T*>(p.x) + s.row * p.x_sb + s.base;
   const T* const pdt = static_cast<const T*>(p.dt) + s.row * p.dt_sb + s.base;
@@ -517,7 +519,7 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
   const float bias = p.dt_bias ? p.dt_bias[channel] : 0.0f, skip = p.d ? p.d[channel] : 0.0f;
   if (!SUM) {
     if (p.segments > 1)
-      carry = reinterpret_cast<const States<R>*>(p.seg_state)[(s.seg * s.units + s.unit) * 64 + s.lane];
+      carry = reinterpret_cast<const States<R>*>(p.seg_state)[(((long long)(s.seg + 1) * p.fine - 1) * s.units + s.unit) * 64 + s.lane];
     else if (p.dstate_out)
       carry = load_states<R>(p.dstate_out + (s.row * p.channels + channel) * p.n, p.n, s.q, s.valid);
   }

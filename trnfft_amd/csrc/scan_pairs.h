@@ -230,7 +230,7 @@ hipError_t scan_launch(const ScanArgs& p, ScanMode mode) {
   }
   const int waves = mode == kScanBackSums || mode == kScanBackward ? kBackWaves<Q> : kScanWaves;
   // (the last segment's sums are not needed, nor are the first's backwards)
-  const int segments = mode == kScanSums || mode == kScanBackSums ? p.segments - 1 : p.segments;
+  const int segments = mode == kScanSums || mode == kScanBackSums ? (p.segments - 1) * p.fine : p.segments;
   return scan_grid(p, 64 / Q, waves, waves, segments, [&](dim3 grid, dim3 block, long long first) {
     if (mode == kScanSums) hipLaunchKernelGGL((scan_forward_kernel<T, Q, R, false>), grid, block, 0, p.stream, p, first);
     if (mode == kScanForward) hipLaunchKernelGGL((scan_forward_kernel<T, Q, R, true>), grid, block, 0, p.stream, p, first);

@@ -76,13 +76,15 @@ int check_scan(const tfa_scan_desc* d) {
 // 381 and 354, 12 x 1024 of 1024 (768) 97 and 100, 16 x 300 of 512 (512) 27 and 34.
 constexpr int64_t kForwardWaves = 1024, kForwardWant = 4096, kBackwardWaves = 2048, kBackwardWant = 2048;
 constexpr int64_t kMostSegments = 64, kSegTokens = 64, kSplitTokens = 256;
+// Sums of so few long segments are made in halves: 8 x 4096 of 2048, whose sums backwards are 1024 waves', 173 and 132 us.
+constexpr int64_t kFineTokens = 512;  // of such a segment
 constexpr int64_t kPairWaves = 924, kPairWork = 150000;  // tokens times the waves that are missing
 
 tfa::ScanArgs scan_args(const tfa_scan_desc* d, bool backward) {
   tfa::ScanArgs p{};
   p.dtype = d->dtype, p.channels = d->channels, p.groups = d->groups, p.n = d->states;
   p.batch = d->batch, p.tokens = d->tokens, p.softplus = d->softplus != 0;
-  p.segments = 1;
+  p.segments = 1, p.fine = 1;
   p.seg_tokens = std::max<int64_t>(1, (d->tokens + tfa::kScanStretch - 1) / tfa::kScanStretch) * tfa::kScanStretch;
   if (d->batch == 0) return p;
   const int64_t waves = tfa::scan_waves(p);
@@ -90,7 +92,9 @@ tfa::ScanArgs scan_args(const tfa_scan_desc* d, bool backward) {
   if (!backward && tfa::scan_has_pairs(p) && (waves >= kPairWaves || d->tokens <= kPairWork / (kPairWaves - waves))) return p;
   const int64_t want = std::min({((backward ? kBackwardWant : kForwardWant) + waves - 1) / waves, d->tokens / kSegTokens, kMostSegments});
   if (want > 1) {
-    p.seg_tokens = ((d->tokens + want - 1) / want + tfa::kScanStretch - 1) / tfa::kScanStretch * tfa::kScanStretch;
+    if (backward && waves * (want - 1) < kBackwardWant && d->tokens / want >= kFineTokens) p.fine = 2;
+    const int64_t step = tfa::kScanStretch * p.fine;
+    p.seg_tokens = ((d->tokens + want - 1) / want + step - 1) / step * step;
     p.segments = (int)((d->tokens + p.seg_tokens - 1) / p.seg_tokens);
   }
   return p;
