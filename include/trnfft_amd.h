@@ -417,10 +417,12 @@ int tfa_causal_conv_step(const tfa_conv_desc* desc, const void* x, const float* 
  *   y_t = (c_t . h_t + d x_t) silu(z_t)
  * x, dt, z: (batch, tokens, channels) at strides of batch and token, channels contiguous; b, c: (batch, tokens, groups, states) at
  * strides of batch, token and group, states contiguous, shared by channels / groups neighbouring channels; all of one type, at any
- * address, token strides from 0 to 2^24 - 1.  a: fp32 (channels, states), -inf for no memory; d, dt_bias: fp32 (channels) or NULL (zero); z may be NULL (no gate).  State tensors are fp32
- * (batch, channels, states).  lengths: (batch) device int64 or NULL; tokens at and past a sequence's length are padding: never
- * read, zeros in y and the gradients, and the state is the one at the length.  States, exponentials and sums are fp32 for every
- * type.  What is not finite makes NaN or infinities of its channel from its token on.  Up to 64 states.
+ * address, token strides from 0 to 2^24 - 1.  a: fp32 (channels, states), -inf for no memory; d, dt_bias: fp32 (channels) or NULL
+ * (zero); z may be NULL (no gate).  State tensors are fp32 (batch, channels, states).  lengths: (batch) device int64 or NULL; tokens
+ * at and past a sequence's length are padding: never read, zeros in y and the gradients, and the state is the one at the length.
+ * States, exponentials and sums are fp32 for every type: a decay is rounded once a token, so over a memory of m tokens (exponents of
+ * steps that are the same from token to token) a state can be off by m 2^-25 of itself.  What is not finite makes NaN or infinities
+ * of its channel from its token on.  Up to 64 states.
  */
 typedef struct tfa_scan_desc {
   int32_t dtype; /* TFA_DTYPE_* of x, dt, z, b, c, y and their gradients */

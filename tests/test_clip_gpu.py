@@ -122,3 +122,17 @@ def test_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert abs(float(norm) - want) <= 2.0**-23 * want and abs(norm_of(grads) - 1.0) <= 1e-5
+
+
+def test_refusals_of_the_native_call():
+    good = torch.ones(8, device="cuda")
+    for bad, error, text in ((torch.ones(8, device="cuda", dtype=torch.float64), TypeError, "got torch.float64"),
+                             (torch.ones(4, 4, device="cuda").t()[1:], ValueError, "contiguous"),
+                             (torch.ones(8), ValueError, "GPU of the first"), (3, TypeError, "tensors")):
+        version = good._version
+        for call in (lambda g: trnfft_amd.grad_norm(g), lambda g: trnfft_amd.clip_grads(g, 0.5)):
+            with pytest.raises(error, match=text):
+                call([good, bad])
+        assert good._version == version and torch.equal(good, torch.ones_like(good))
+    version = good._version
+    assert float(trnfft_amd.clip_grads([good], 100.0)) == pytest.approx(8.0**0.5, rel=1e-6) and good._version > version

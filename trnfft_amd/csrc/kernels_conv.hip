@@ -7,6 +7,8 @@
 // channels over a run of frames, with its window of frames in registers, so a frame is read once but for the W - 1 in front of
 // (and, backward, behind) a run.  Each filter width is a kernel of its own: a wider one with taps of zero would make NaN of
 // infinities outside the filter.  Frames at and past lengths[n] are padding: not read, zeros in y and dx.
+// 8 x 4096 tokens of 2048 channels, bf16, 4 taps: forward 52 us (5.1 TB/s, the rate of a copy), backward 101 and its join 5 (4.0 TB/s);
+// 64 x 626 of 1024 with rows of all lengths 33.
 #include "model_ops.h"
 #include "activations.h"
 

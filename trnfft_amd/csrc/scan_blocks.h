@@ -6,15 +6,17 @@
 //   ds_t = x_t sum_n g_t[n] b_t[n] + sum_n a[n] f_t[n],  dx_t = s_t sum_n g_t[n] b_t[n] + d v_t,  da[n] = sum_t s_t f_t[n],
 //   where f_t = g_t e_t h_{t-1},  dz_t = dy_t silu'(z_t) (sum_n c_t[n] h_t[n] + d x_t)
 //
-// (scan_pairs.h: two waves for the same channels.)
-//
 // A wave takes 64 / Q channels of a row and group, Q lanes a channel with R states each (4 x 1, 2 or 4 up to 16 states, 8 and 16 x 4 above), and walks
 // along the tokens in tiles of 16.  For what belongs to a channel and token alone (softplus, gates, loads, stores) lane q of a channel takes
 // every Q-th token, so nothing of it is done twice; the tokens' s and s x go to the channel's lanes through LDS, as do b and
 // c, whose rows all channels of a group share.  Sums over the lanes of a channel are folded: Q tokens' sums at once, each ending in
 // the lane of its token.
 //
-// Bound by vector instructions (an exponential takes two instructions' time), not by memory.
+// Bound by vector instructions (an exponential takes two instructions' time), not by memory.  A token and wave of 16 channels of 16 states take 39
+// of them forward, 24 for the recurrence and its dot products alone, and about 100 backward.  8 x 4096 tokens of 2048 channels, bf16: backward
+// 900 us in two segments (and 132 for their sums), forward 443 with one wave a SIMD, 400 in scan_pairs.h; 1 x 65536 of 1024 in 64 segments,
+// four waves a SIMD, 315 and 220 for the sums.  Products b u by 4 x 4 matrix instructions are 16 instructions fewer in two tokens and took
+// the same time, 8 lanes a channel of two states 557 and 1190 us.
 #pragma once
 #include "scan_device.h"
 

@@ -156,13 +156,14 @@ tfa::GradLists grad_lists(const tfa_grad_lists* g) {
 // whether two of the tensors share memory, which two workgroups would then scale
 bool overlapping(const tfa_grad_lists* g) {
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  spans.reserve(g->count[0] + g->count[1] + g->count[2]);
   for (int d = 0; d < 3; ++d)
     for (int64_t i = 0; i < g->count[d]; ++i)
       if (g->tensors[d][i].n > 0) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(g->tensors[d][i].data);
         spans.emplace_back(at, at + (uintptr_t)g->tensors[d][i].n * (d == TFA_DTYPE_F32 ? 4 : 2));
       }
-  std::sort(spans.begin(), spans.end());
+  if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());  // (as a model's gradients mostly lie, at a third of the time)
   for (size_t i = 1; i < spans.size(); ++i)
     if (spans[i].first < spans[i - 1].second) return true;
   return false;

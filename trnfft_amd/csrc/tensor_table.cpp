@@ -142,12 +142,17 @@ PyObject* norm_of(PyObject* args) {
   std::vector<tfa_grad_tensor> rows[3];
   std::vector<at::Tensor> tensors;
   tensors.reserve(PyList_GET_SIZE(list));
+  for (auto& r : rows) r.reserve(PyList_GET_SIZE(list));
   for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
     PyObject* const item = PyList_GET_ITEM(list, i);
     if (!THPVariable_Check(item)) return refuse(PyExc_TypeError, what, name, "must be tensors");
     const at::Tensor& t = THPVariable_Unpack(item);
     const int type = t.scalar_type() == at::kFloat ? TFA_DTYPE_F32 : t.scalar_type() == at::kBFloat16 ? TFA_DTYPE_BF16 : TFA_DTYPE_F16;
-    if (type == TFA_DTYPE_F16 && t.scalar_type() != at::kHalf) return refuse(PyExc_TypeError, what, name, "must be float32, bfloat16 or float16");
+    if (type == TFA_DTYPE_F16 && t.scalar_type() != at::kHalf) {
+      PyErr_Format(PyExc_TypeError, "%U: float32, bfloat16 or float16 gradients expected, got %S", what,
+                   reinterpret_cast<PyObject*>(torch::getTHPDtype(t.scalar_type())));
+      return nullptr;
+    }
     if (const char* text = misplaced(t, device)) return refuse(PyExc_ValueError, what, name, text);
     rows[type].push_back({t.data_ptr(), t.numel()});
     tensors.push_back(t);

@@ -111,13 +111,14 @@ class StateSpace(nn.Module):
         """Frames at and past a row's length are padding.  state: where the sequences go on from; return_state: where they end."""
         signal, gate = self.enter(x).chunk(2, dim=-1)
         before, start = (None, None) if state is None else state
-        signal, last = causal_conv(signal, self.conv_weight, self.conv_bias, activation="silu", initial_state=before, lengths=lengths,
-                                   return_state=True)
+        signal = causal_conv(signal, self.conv_weight, self.conv_bias, activation="silu", initial_state=before, lengths=lengths,
+                             return_state=return_state)
+        signal, last = signal if return_state else (signal, None)
         dt, a, b, c = self._operands(signal)
-        y, end = selective_scan(signal, dt, a, b, c, d=self.skip, z=gate, dt_bias=self.dt_bias, initial_state=start, lengths=lengths,
-                                return_state=True)
-        y = self.leave(y)
-        return (y, (last, end)) if return_state else y
+        y = selective_scan(signal, dt, a, b, c, d=self.skip, z=gate, dt_bias=self.dt_bias, initial_state=start, lengths=lengths,
+                           return_state=return_state)
+        y, end = y if return_state else (y, None)
+        return (self.leave(y), (last, end)) if return_state else self.leave(y)
 
     def step(self, x: torch.Tensor, state: tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
         """The next frame (batch, features) of every stream; both parts of the state are updated in place.  No gradients."""

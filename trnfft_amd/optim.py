@@ -8,12 +8,11 @@ s (c / 255)^4 of uint8 codes (at least 1 where there is any).  The reference has
 
 from __future__ import annotations
 
-
 import torch
 
 from . import _lib
 from .attention import DTYPES, _on
-from .dispatch import _raw_stream, _require_hip, launch
+from .dispatch import _raw_stream, _require_hip, _use_hip, launch
 
 BLOCK = 256  # values that share a scale
 
@@ -92,10 +91,11 @@ def adamw_state_values(codes, scales, out=None) -> list[torch.Tensor]:
 
 
 def _norm_call(what: str, grads: list, max_norm: float | None) -> torch.Tensor:
-    types = {g.dtype for g in grads}
-    if not types <= DTYPES.keys():
-        raise TypeError(f"{what}: float32, bfloat16 or float16 gradients expected, got {(types - DTYPES.keys()).pop()}")
-    _require_hip(what)
+    if not _use_hip():  # (else the native call sees to it)
+        types = {g.dtype for g in grads}
+        if not types <= DTYPES.keys():
+            raise TypeError(f"{what}: float32, bfloat16 or float16 gradients expected, got {(types - DTYPES.keys()).pop()}")
+        _require_hip(what)
     dev = grads[0].device
     if dev.type != "cuda":
         raise ValueError(f"{what}: the gradients must be on the GPU")

@@ -219,7 +219,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     are padding, whatever they hold: outputs and gradients are zero there.
 
     Returns y (batch, frames, channels) in x's dtype, and with return_state the state after each sequence's last frame (float32).
-    States and sums are fp32.  Gradients cannot be differentiated again, and there is no forward mode.
+    States and sums are fp32.  A decay is rounded once a frame: where steps are the same from frame to frame, a state with a memory
+    of m frames can be off by m 2^-25 of itself.  Gradients cannot be differentiated again, and there is no forward mode.  In a captured pass
+    leaves are refused whose graph of an eager pass still lives: autograd would leave the capture for them.
     A value that is not finite makes NaN or infinities of its channel from its frame on (of b and c: of its group's channels).
     """
     what = "selective_scan"
