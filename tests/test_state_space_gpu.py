@@ -462,6 +462,51 @@ def test_steps_called_natively_and_from_python_agree(monkeypatch):
     assert torch.equal(got, want[2])
 
 
+@pytest.mark.parametrize("extra", [False, True])
+def test_sequences_called_natively_and_from_python_agree(extra, monkeypatch):
+    """The same for whole sequences, with and without gradients: what has to be converted goes through Python."""
+    from trnfft_amd import state_space
+
+    v, lengths = scan_inputs(3, 21, 24, 2, 6, torch.float32, 4, extra)
+    v, lengths = {k: cuda(w) for k, w in v.items()}, cuda(lengths)
+    conv = conv_inputs(3, 21, 24, 4, torch.float32, 5, bias=extra, state=extra, lengths=False)
+    conv = {k: cuda(conv.get(k)) for k in ("x", "weight", "bias", "state")}
+
+    def passes(v, conv, lengths):
+        leaves = [w.detach().requires_grad_() for w in (*v.values(), *conv.values()) if torch.is_tensor(w)]
+        own = iter(leaves)
+        v = {k: next(own) if torch.is_tensor(w) else None for k, w in v.items()}
+        conv = {k: next(own) if torch.is_tensor(w) else None for k, w in conv.items()}
+        outs = []
+        for grads in (True, False):
+            with torch.set_grad_enabled(grads):
+                y, last = scan(v, lengths)
+                u, end = trnfft_amd.causal_conv(conv["x"], conv["weight"], conv["bias"], activation="gelu", initial_state=conv["state"],
+                                                lengths=lengths, return_state=True)
+                alone = scan(v, lengths, return_state=False)
+                assert torch.is_tensor(alone) and torch.equal(alone, y)
+            outs += [y, last, u, end]
+            assert y.requires_grad == grads and end.requires_grad == grads
+        return [*outs, *torch.autograd.grad([outs[0].sum(), outs[2].square().sum(), outs[3].sum()], leaves, allow_unused=True)]
+
+    taken = []
+    direct = state_space._direct
+    monkeypatch.setattr(state_space, "_direct", lambda *args: taken.append(direct(*args)) or taken[-1])
+    want = passes(v, conv, lengths)
+    assert len(taken) == 6 and all(t is not None for t in taken)
+    taken.clear()
+    turned = {**v, "a": v["a"].t().contiguous().t()}
+    got = passes(turned, {**conv, "weight": conv["weight"].t().contiguous().t()}, None if lengths is None else lengths.int())
+    assert taken == [None] * 6
+    monkeypatch.setattr(state_space, "_direct", lambda *args: None)
+    for other in (got, passes(v, conv, lengths)):
+        for a, b in zip(other, want):
+            assert (a is None and b is None) or torch.equal(a, b)
+    with pytest.raises(NotImplementedError, match="64 states"):
+        monkeypatch.undo()
+        trnfft_amd.selective_scan(v["x"], v["dt"], torch.zeros(24, 65, device="cuda"), *(torch.zeros(3, 21, 2, 65, device="cuda"),) * 2)
+
+
 @pytest.mark.parametrize("rows,t", [(0, 5), (3, 0), (0, 0)])
 def test_nothing_to_do(rows, t):
     v, _ = scan_inputs(rows, t, 6, 1, 4, torch.float32, 0, extra=False)

@@ -120,13 +120,15 @@ def test_native_calls_are_bound_to_the_library():
     native = _lib.state_space()
     assert native is _lib.state_space() and set(native.ENTRIES) - {"tfa_last_error"} <= set(_lib.EXPORTS)
     with pytest.raises(RuntimeError, match="tensor or None"):
-        native.causal_conv(1, None, None, None, None, 0, False, False)
+        native.causal_conv(1, None, None, None, None, 0, False, True)
     with pytest.raises(TypeError):
         native.selective_scan()
     x, state = torch.zeros(2, 8), torch.zeros(2, 3, 8)  # on the CPU: left to Python
     assert native.conv_step(0, x, state, torch.zeros(8, 4), None, 0) is None
     assert native.scan_step(0, x, x, torch.zeros(8, 2), x, x, state, None, None, None, True) is None
     assert native.conv_step(0, 3, state, None, None, 0) is None
+    assert native.causal_conv(x[None], torch.zeros(8, 4), None, None, None, 0, False, False) is None
+    assert native.selective_scan(3, x, x, x, x, None, None, None, None, None, True, False, False) is None
 
 
 def test_c_entries_refuse_bad_descriptors():

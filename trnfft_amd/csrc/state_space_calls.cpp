@@ -4,9 +4,9 @@
 // Steps of streams: where every operand is as the C ABI takes it, the call is made from here; asked from Python nine tensors cost 8 of the
 // 13.8 us of a small scan's step.  Anything else is left to Python, which converts or refuses it.
 //
-// Whole sequences and their nodes of autograd's graph: Python has checked and converted the operands.  A backward
+// Whole sequences likewise (a scan takes 15 us of the host from Python, 7.6 from here), and their nodes of autograd's graph: a backward
 // pass in Python took 70 us on autograd's thread, which had to wake up for it and to take Python's lock; a small training pass of the scan takes
-// 132 us of the host instead of 218 (a layer norm's: 66).
+// 123 us of the host instead of 218 (a layer norm's: 66).
 #include <Python.h>
 
 #include <torch/csrc/Exceptions.h>
@@ -246,11 +246,11 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
 
 const char kBindDoc[] = "bind(addresses): the C ABI's entries in the order of ENTRIES.";
 const char kConvDoc[] =
-    "causal_conv(x, weight, bias, state, lengths, activation, want_state, grads) -> [y] or [y, last], or an error's status.  Operands as the\n"
-    "C ABI takes them, on one device; grads: with a node of the graph.";
+    "causal_conv(x, weight, bias, state, lengths, activation, want_state, checked) -> y or (y, last), an error's status, or None where operands\n"
+    "that are not checked are not as the C ABI takes them.";
 const char kScanDoc[] =
-    "selective_scan(x, dt, a, b, c, d, z, dt_bias, state, lengths, softplus, want_state, grads) -> [y] or [y, last], or an error's status,\n"
-    "as causal_conv.";
+    "selective_scan(x, dt, a, b, c, d, z, dt_bias, state, lengths, softplus, want_state, checked) -> y or (y, last), an error's status, or\n"
+    "None, as causal_conv.";
 const char kConvStepDoc[] =
     "conv_step(device, x, state, weight, bias, activation) -> y, an error's status, or None where an operand is not as the C ABI takes it\n"
     "(or needs a gradient).";
@@ -284,57 +284,7 @@ at::Tensor argument(PyObject* o) {
   return THPVariable_Unpack(o);
 }
 
-PyObject* list_of(const variable_list& v) {
-  PyObject* const list = PyList_New((Py_ssize_t)v.size());
-  if (!list) return nullptr;
-  for (size_t i = 0; i < v.size(); ++i) {
-    PyObject* const item = THPVariable_Wrap(v[i]);
-    if (!item) {
-      Py_DECREF(list);
-      return nullptr;
-    }
-    PyList_SET_ITEM(list, (Py_ssize_t)i, item);
-  }
-  return list;
-}
-
-PyObject* conv_of(PyObject* args) {
-  PyObject* o[5];
-  int activation, want_state, grads;
-  if (!PyArg_ParseTuple(args, "OOOOOipp", o, o + 1, o + 2, o + 3, o + 4, &activation, &want_state, &grads)) return nullptr;
-  at::Tensor t[5];
-  for (int i = 0; i < 5; ++i) t[i] = argument(o[i]);
-  if (grads) refuse_eager_graphs(t, 4);
-  variable_list out;
-  {
-    const WithoutGil released;
-    out = grads ? ConvFn::apply(t[0], t[1], optional_of(t[2]), optional_of(t[3]), optional_of(t[4]), (int64_t)activation, (bool)want_state)
-                : conv_forward(t[0], t[1], t[2], t[3], t[4], activation, want_state);
-  }
-  return list_of(out);
-}
-
-PyObject* scan_of(PyObject* args) {
-  PyObject* o[10];
-  int softplus, want_state, grads;
-  if (!PyArg_ParseTuple(args, "OOOOOOOOOOppp", o, o + 1, o + 2, o + 3, o + 4, o + 5, o + 6, o + 7, o + 8, o + 9, &softplus, &want_state, &grads))
-    return nullptr;
-  at::Tensor t[10];
-  for (int i = 0; i < 10; ++i) t[i] = argument(o[i]);
-  if (grads) refuse_eager_graphs(t, 9);
-  variable_list out;
-  {
-    const WithoutGil released;
-    if (grads)
-      out = ScanFn::apply(t[0], t[1], t[2], t[3], t[4], optional_of(t[5]), optional_of(t[6]), optional_of(t[7]), optional_of(t[8]),
-                          optional_of(t[9]), (bool)softplus, (bool)want_state);
-    else
-      out = std::get<0>(scan_forward(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], softplus, want_state, false));
-  }
-  return list_of(out);
-}
-
-// A tensor of the device with contiguous last axis that needs no gradient; None gives an undefined one where it may be left out.
+// A tensor of the device with contiguous last axis, which (grads) needs no gradient; None gives an undefined one where it may be left out.
 struct Operand {
   const at::Tensor* t = nullptr;
   bool good = false;
@@ -346,7 +296,7 @@ struct Operand {
     if (!THPVariable_CheckExact(o) && !THPVariable_Check(o)) return;
     const at::Tensor& v = THPVariable_Unpack(o);
     if (!v.defined() || v.layout() != at::kStrided || !v.is_cuda() || v.get_device() != device || v.is_neg() || (grads && v.requires_grad())) return;
-    if (v.dim() < 1 || v.dim() > 3 || (v.size(v.dim() - 1) != 1 && v.stride(v.dim() - 1) != 1)) return;
+    if (v.dim() < 1 || v.dim() > 4 || (v.size(v.dim() - 1) != 1 && v.stride(v.dim() - 1) != 1)) return;
     t = &v;
     good = true;
   }
@@ -356,6 +306,103 @@ struct Operand {
 };
 
 PyObject* none() { Py_RETURN_NONE; }
+
+// y, or y and the last state
+PyObject* result_of(const variable_list& v) {
+  PyObject* const y = THPVariable_Wrap(v[0]);
+  if (!y || v.size() == 1) return y;
+  PyObject* const last = THPVariable_Wrap(v[1]);
+  PyObject* const both = last ? PyTuple_Pack(2, y, last) : nullptr;
+  Py_DECREF(y);
+  Py_XDECREF(last);
+  return both;
+}
+
+bool want_gradients(const at::Tensor* t, size_t count) {
+  if (c10::GradMode::is_enabled())
+    for (size_t i = 0; i < count; ++i)
+      if (t[i].defined() && t[i].requires_grad()) return true;
+  return false;
+}
+// a sequence's operand whose frames are as close as the kernels' addresses take them
+bool close_frames(const Operand& o) { return !o.t || o.t->size(1) < 2 || (o.t->stride(1) >= 0 && o.t->stride(1) < 1 << 24); }
+
+// Whole sequences: operands x, weight, bias, state and lengths.  `checked`: by Python, which has made them what the C ABI takes; else they are left
+// to it unless they are so already.
+PyObject* conv_of(PyObject* args) {
+  PyObject* o[5];
+  int activation, want_state, checked;
+  if (!PyArg_ParseTuple(args, "OOOOOipp", o, o + 1, o + 2, o + 3, o + 4, &activation, &want_state, &checked)) return nullptr;
+  if (!checked) {
+    if (!THPVariable_Check(o[0])) return none();
+    const int64_t device = THPVariable_Unpack(o[0]).get_device();
+    const Operand x(o[0], device, false), weight(o[1], device, false), bias(o[2], device, false, true), state(o[3], device, false, true),
+        lengths(o[4], device, false, true);
+    for (const Operand* v : {&x, &weight, &bias, &state, &lengths})
+      if (!v->good) return none();
+    if (x.t->dim() != 3 || weight.t->dim() != 2 || !close_frames(x)) return none();
+    const at::ScalarType type = x.t->scalar_type();
+    const int64_t b = x.t->size(0), c = x.t->size(2), width = weight.t->size(1);
+    if (dtype_of(type) < 0 || c < 1 || width < 1 || c > INT32_MAX || width > INT32_MAX) return none();
+    if (!weight.whole(at::kFloat, {c, width}) || !bias.whole(at::kFloat, {c}) || !state.whole(type, {b, width - 1, c}) ||
+        !lengths.whole(at::kLong, {b}))
+      return none();
+  }
+  at::Tensor t[5];
+  for (int i = 0; i < 5; ++i) t[i] = argument(o[i]);
+  const bool grads = want_gradients(t, 4);
+  if (grads) refuse_eager_graphs(t, 4);
+  variable_list out;
+  {
+    const WithoutGil released;
+    out = grads ? ConvFn::apply(t[0], t[1], optional_of(t[2]), optional_of(t[3]), optional_of(t[4]), (int64_t)activation, (bool)want_state)
+                : conv_forward(t[0], t[1], t[2], t[3], t[4], activation, want_state);
+  }
+  return result_of(out);
+}
+
+// as conv_of: x, dt, a, b, c, d, z, dt_bias, state and lengths
+PyObject* scan_of(PyObject* args) {
+  PyObject* o[10];
+  int softplus, want_state, checked;
+  if (!PyArg_ParseTuple(args, "OOOOOOOOOOppp", o, o + 1, o + 2, o + 3, o + 4, o + 5, o + 6, o + 7, o + 8, o + 9, &softplus, &want_state, &checked))
+    return nullptr;
+  if (!checked) {
+    if (!THPVariable_Check(o[0])) return none();
+    const int64_t device = THPVariable_Unpack(o[0]).get_device();
+    const Operand x(o[0], device, false), dt(o[1], device, false), a(o[2], device, false), b(o[3], device, false), c(o[4], device, false),
+        d(o[5], device, false, true), z(o[6], device, false, true), bias(o[7], device, false, true), state(o[8], device, false, true),
+        lengths(o[9], device, false, true);
+    for (const Operand* v : {&x, &dt, &a, &b, &c, &d, &z, &bias, &state, &lengths})
+      if (!v->good) return none();
+    if (x.t->dim() != 3 || a.t->dim() != 2 || b.t->dim() != 4) return none();
+    const at::ScalarType type = x.t->scalar_type();
+    const int64_t rows = x.t->size(0), tokens = x.t->size(1), channels = x.t->size(2), n = a.t->size(1), groups = b.t->size(2);
+    if (dtype_of(type) < 0 || channels < 1 || n < 1 || groups < 1 || channels % groups || channels > INT32_MAX || n > INT32_MAX) return none();
+    if (!dt.is(type, {rows, tokens, channels}) || !z.is(type, {rows, tokens, channels}) || !b.is(type, {rows, tokens, groups, n}) ||
+        !c.is(type, {rows, tokens, groups, n}))
+      return none();
+    for (const Operand* v : {&x, &dt, &b, &c, &z})
+      if (!close_frames(*v)) return none();
+    if (!a.whole(at::kFloat, {channels, n}) || !d.whole(at::kFloat, {channels}) || !bias.whole(at::kFloat, {channels}) ||
+        !state.whole(at::kFloat, {rows, channels, n}) || !lengths.whole(at::kLong, {rows}))
+      return none();
+  }
+  at::Tensor t[10];
+  for (int i = 0; i < 10; ++i) t[i] = argument(o[i]);
+  const bool grads = want_gradients(t, 9);
+  if (grads) refuse_eager_graphs(t, 9);
+  variable_list out;
+  {
+    const WithoutGil released;
+    if (grads)
+      out = ScanFn::apply(t[0], t[1], t[2], t[3], t[4], optional_of(t[5]), optional_of(t[6]), optional_of(t[7]), optional_of(t[8]),
+                          optional_of(t[9]), (bool)softplus, (bool)want_state);
+    else
+      out = std::get<0>(scan_forward(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], t[9], softplus, want_state, false));
+  }
+  return result_of(out);
+}
 
 // y where the call went well, its status otherwise; the state has changed
 PyObject* stepped(int rc, const at::Tensor& y, const at::Tensor& state) {

@@ -70,11 +70,22 @@ def _check_state(what: str, state: torch.Tensor) -> torch.device:
 
 
 def _results(what: str, out, dev: torch.device):
-    """y, or y and the last state, on dev, of a native call's list or status."""
+    """A native call's results on dev; raises for a status."""
     if type(out) is int:
         _lib.check(out, what)
-    out = [v if v.device == dev else v.to(dev) for v in out]
-    return out[0] if len(out) == 1 else tuple(out)
+    if type(out) is tuple:
+        return tuple(v if v.device == dev else v.to(dev) for v in out)
+    return out if out.device == dev else out.to(dev)
+
+
+def _direct(what: str, name: str, *args):
+    """A sequence's call made natively: its results, or None where an operand has to be converted or refused first."""
+    if not _use_hip() or getattr(forward_ad, "_current_level", 0) >= 0:
+        return None
+    out = getattr(_lib.state_space(), name)(*args, False)
+    if type(out) is int:
+        _lib.check(out, what)
+    return out
 
 
 def _step(what: str, step: str, state: torch.Tensor, *args) -> torch.Tensor | None:
@@ -127,6 +138,10 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     length.  Sums are fp32.  Gradients cannot be differentiated again, and there is no forward mode.
     """
     what = "causal_conv"
+    if activation in ACTIVATIONS:
+        out = _direct(what, what, x, weight, bias, initial_state, lengths, ACTIVATIONS[activation], return_state)
+        if out is not None:  # (as it mostly is: nothing to convert, nothing to refuse)
+            return out
     _check_conv(what, x, weight, bias, activation, 3)
     (b, _, c), width = x.shape, weight.shape[1]
     if initial_state is not None:
@@ -140,8 +155,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     dev, out_dev = target_device(x), x.device
     x, weight, bias = _features(x, dev), _channels(weight, dev), _channels(bias, dev)
     state, lengths = _dense(initial_state, dev), _whole_numbers(lengths, dev)
-    grads = _wants(x, weight, bias, state)
-    return _results(what, _lib.state_space().causal_conv(x, weight, bias, state, lengths, ACTIVATIONS[activation], return_state, grads), out_dev)
+    return _results(what, _lib.state_space().causal_conv(x, weight, bias, state, lengths, ACTIVATIONS[activation], return_state, True), out_dev)
 
 
 def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -225,6 +239,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     A value that is not finite makes NaN or infinities of its channel from its frame on (of b and c: of its group's channels).
     """
     what = "selective_scan"
+    out = _direct(what, what, x, dt, a, b, c, d, z, dt_bias, initial_state, lengths, softplus, return_state)
+    if out is not None:  # (as it mostly is: nothing to convert, nothing to refuse)
+        return out
     _check_scan(what, x, dt, a, b, c, d, z, dt_bias, 3)
     rows = x.shape[0]
     if initial_state is not None:
@@ -240,8 +257,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     z = None if z is None else _tokens(z, dev)
     a, d, dt_bias = _dense(a, dev), _channels(d, dev), _channels(dt_bias, dev)
     state, lengths = _dense(initial_state, dev), _whole_numbers(lengths, dev)
-    grads = _wants(x, dt, a, b, c, d, z, dt_bias, state)
-    return _results(what, _lib.state_space().selective_scan(x, dt, a, b, c, d, z, dt_bias, state, lengths, softplus, return_state, grads), out_dev)
+    return _results(what, _lib.state_space().selective_scan(x, dt, a, b, c, d, z, dt_bias, state, lengths, softplus, return_state, True), out_dev)
 
 
 def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor,
