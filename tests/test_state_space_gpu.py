@@ -294,6 +294,12 @@ def test_scan_in_segments(shape, dtype):
     check_scan(shape, dtype, True, softplus=True, seed=7)
 
 
+@pytest.mark.parametrize("shape", [(257, 3, 20, 1, 16), (600, 2, 40, 5, 3), (640, 2, 17, 1, 33)], ids=str)
+def test_gradients_over_many_rows(shape):
+    """Sums over rows in two passes."""
+    check_scan(shape, torch.float32, True, softplus=True, seed=13)
+
+
 @pytest.mark.parametrize("t,end", [(1056, 1056), (1090, 1071), (1090, 300)])
 def test_scan_in_long_segments(t, end):
     """Two segments backwards, whose sums are made in halves (the definition on the GPU, in float64)."""

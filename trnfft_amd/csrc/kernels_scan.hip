@@ -63,30 +63,54 @@ __global__ __launch_bounds__(256) void scan_shares_kernel(ScanArgs p, int states
   out[(cell * p.groups + group) * p.n + k] = from_f32<T>(sum);
 }
 
-// da, dd and ddt_bias from the rows' and segments' sums
+// da, dd and ddt_bias from the rows' and segments' sums: a workgroup for a wave's channels, whose waves take every kSumWaves-th sum.  Many sums are
+// added in two passes: `span` neighbours by a workgroup, which leaves theirs in place of the first, then (span 0) every `step`-th.
+// 8 x 4096 tokens of 2048 channels 4.9 us; 10000 rows of 64 channels 20 in two passes, 241 in one, 1273 by one thread for all sums of a state.
+constexpr int kSumWaves = 16;
+constexpr long long kSumsAtOnce = 256;
 template <int R>
-__global__ __launch_bounds__(256) void scan_channels_kernel(ScanArgs p, int lanes) {
+__global__ __launch_bounds__(64 * kSumWaves) void scan_channels_kernel(ScanArgs p, int lanes, long long span, long long step) {
+  __shared__ States<R> of_a[kSumWaves][64];
+  __shared__ States<2> of_rest[kSumWaves][64];
   const int channels = 64 / lanes, each = p.channels / p.groups, tiles = (each + channels - 1) / channels;
-  const long long id = blockIdx.x * 256LL + threadIdx.x, of_row = (long long)p.groups * tiles * 64;
-  if (id >= of_row) return;
-  const int lane = (int)(id % 64), q = lane / channels, own = (int)(id / 64 % tiles) * channels + lane % channels;
-  if (own >= each) return;
-  const int channel = (int)(id / 64 / tiles) * each + own;
+  const int tile = (int)(blockIdx.x % (p.groups * tiles)), lane = threadIdx.x % 64, wave = threadIdx.x / 64, q = lane / channels;
+  const int own = tile % tiles * channels + lane % channels;
+  const long long of_row = (long long)p.groups * tiles * 64, id = tile * 64LL + lane;
   const long long count = p.segments * p.batch, all = count * of_row;
+  const long long begin = blockIdx.x / (p.groups * tiles) * span, end = span ? min(begin + span, count) : count;
   States<R> da = {};
-  float dd = 0.0f, dbias = 0.0f;
+  States<2> rest = {};
 #pragma unroll 4
-  for (long long i = 0; i < count; ++i) {
+  for (long long i = begin + wave * step; i < end; i += kSumWaves * step) {
     const long long at = i * of_row + id;
     const States<R> v = reinterpret_cast<const States<R>*>(p.channel_parts)[at];
 #pragma unroll
     for (int r = 0; r < R; ++r) da.v[r] += v.v[r];
-    dd += p.channel_parts[R * all + at];
-    dbias += p.channel_parts[(R + 1) * all + at];
+    rest.v[0] += p.channel_parts[R * all + at];
+    rest.v[1] += p.channel_parts[(R + 1) * all + at];
   }
+  of_a[wave][lane] = da;
+  of_rest[wave][lane] = rest;
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int w = 1; w < kSumWaves; ++w) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) da.v[r] += of_a[w][lane].v[r];
+    rest.v[0] += of_rest[w][lane].v[0], rest.v[1] += of_rest[w][lane].v[1];
+  }
+  if (span) {
+    const long long at = begin * of_row + id;
+    reinterpret_cast<States<R>*>(p.channel_parts)[at] = da;
+    p.channel_parts[R * all + at] = rest.v[0];
+    p.channel_parts[(R + 1) * all + at] = rest.v[1];
+    return;
+  }
+  if (own >= each) return;
+  const int channel = tile / tiles * each + own;
   if (p.da) store_states<R>(p.da + (long long)channel * p.n, p.n, q, true, da);
-  if (q == 0 && p.dd) p.dd[channel] = dd;
-  if (q == 0 && p.ddt_bias) p.ddt_bias[channel] = dbias;
+  if (q == 0 && p.dd) p.dd[channel] = rest.v[0];
+  if (q == 0 && p.ddt_bias) p.ddt_bias[channel] = rest.v[1];
 }
 
 template <int BLOCK = 256, typename F>
@@ -160,9 +184,16 @@ hipError_t launch_scan_backward(const ScanArgs& p) {
     if (e != hipSuccess) return e;
   }
   if (!p.da && !p.dd && !p.ddt_bias) return hipSuccess;
-  const long long threads = p.groups * scan_tiles(p) * 64;
   const auto kernel = s.each == 1 ? scan_channels_kernel<1> : s.each == 2 ? scan_channels_kernel<2> : scan_channels_kernel<4>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, p.stream, p, s.lanes);
+  const long long tiles = p.groups * scan_tiles(p), count = p.segments * p.batch;
+  long long step = 1;
+  if (count > kSumsAtOnce) {
+    // (as many workgroups as a grid holds, of 64 sums at least)
+    step = std::max({64LL, (count + kSumsAtOnce - 1) / kSumsAtOnce, count / std::max(1LL, max_blocks(64 * kSumWaves) / tiles - 1)});
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * ((count + step - 1) / step))), dim3(64 * kSumWaves), 0, p.stream, p, s.lanes, step, 1LL);
+    if (const hipError_t failed = hipGetLastError(); failed != hipSuccess) return failed;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(64 * kSumWaves), 0, p.stream, p, s.lanes, 0LL, step);
   return hipGetLastError();
 }
 
