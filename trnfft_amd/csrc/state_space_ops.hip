@@ -67,18 +67,16 @@ int check_scan(const tfa_scan_desc* d) {
 
 // A sequence is cut into segments where its rows and channels alone leave the vector units idle, at a cost: the segments' sums are 0.6 (forward)
 // and 0.25 (backward) of the pass itself.  Forward below 1024 waves into segments that make about 4096, backward below 2048 into
-// such that make 2048 (a wave takes half of a SIMD's registers there), at most 64 of at least 32 (backward 64) tokens, of sequences of at
-// least 256.
+// such that make 2048 (a wave takes half of a SIMD's registers there), at most 64 of at least 32 tokens, of sequences of at least 256.
 // 16 states, bf16: 8 x 4096 tokens of 2048 channels (1024 waves) forward 400 us whole, 505 in 4 segments; backward 1340 whole, 1100 in 2,
 // 1140 in 4.  1 x 65536 of 1024 (64 waves) 753 in 16, 544 in 32, 491 in 64.  1 x 16384 of 256 (16 waves) 83 in 64, 131 in 256.  1 x 1000 of 512
-// 73 in 3, 40 in 7, 27 in 15, 24 in 31; 4 x 1001 of 384 36 in 15, 30 in 31.  1 x 128 of 1024 21 whole, 27
-// in 2.
+// 73 in 3, 40 in 7, 27 in 15, 24 in 31; 4 x 1001 of 384 in 15 and 31: forward 36 and 30, backward with its sums 54 and 40.  1 x 128 of 1024 21
+// whole, 27 in 2.
 // Where two waves take the same channels (scan_pairs.h) a token takes 0.1 us whole up to 1024 waves; segments take as much at 924, less in
 // proportion to the waves below, and some 15 us for their launches: whole and in segments 7 x 4096 of 2048 (896 waves) 392 and 445, 6 rows (768)
 // 381 and 354, 12 x 1024 of 1024 (768) 97 and 100, 16 x 300 of 512 (512) 27 and 34.
 constexpr int64_t kForwardWaves = 1024, kForwardWant = 4096, kBackwardWaves = 2048, kBackwardWant = 2048;
-constexpr int64_t kMostSegments = 64, kSplitTokens = 256;
-constexpr int64_t kForwardTokens = 32, kBackwardTokens = 64;  // of a segment at least
+constexpr int64_t kMostSegments = 64, kSegTokens = 32, kSplitTokens = 256;
 // Sums of so few long segments are made in halves: 8 x 4096 of 2048, whose sums backwards are 1024 waves', 173 and 132 us.
 constexpr int64_t kFineTokens = 512;  // of such a segment
 constexpr int64_t kPairWaves = 924, kPairWork = 150000;  // tokens times the waves that are missing
@@ -93,7 +91,7 @@ tfa::ScanArgs scan_args(const tfa_scan_desc* d, bool backward) {
   const int64_t waves = tfa::scan_waves(p);
   if (waves >= (backward ? kBackwardWaves : kForwardWaves) || d->tokens < kSplitTokens) return p;
   if (!backward && tfa::scan_has_pairs(p) && (waves >= kPairWaves || d->tokens <= kPairWork / (kPairWaves - waves))) return p;
-  const int64_t want = std::min({((backward ? kBackwardWant : kForwardWant) + waves - 1) / waves, d->tokens / (backward ? kBackwardTokens : kForwardTokens), kMostSegments});
+  const int64_t want = std::min({((backward ? kBackwardWant : kForwardWant) + waves - 1) / waves, d->tokens / kSegTokens, kMostSegments});
   if (want > 1) {
     if (backward && waves * (want - 1) < kBackwardWant && d->tokens / want >= kFineTokens) p.fine = 2;
     const int64_t step = tfa::kScanStretch * p.fine;
