@@ -74,7 +74,6 @@ class Block(nn.Module):
         q, k, v = self._split(x)
         return self._join(x, trnfft_amd.linear_attention_step(q, k, v, self._log_decay(), state, scale=1.0))
 
-
     def state(self, streams: int, device) -> torch.Tensor:
         return torch.zeros(streams, self.heads, self.key_dim, self.value_dim, device=device)
 

@@ -149,39 +149,25 @@ struct ScanTokens {
 };
 // A tile's rows of b or c, 16 by Q R, zeros past n and past the end.  With 4 lanes a channel a row of 16 lanes has one q: lane l of it
 // keeps the R states of token l % 16, and products take them from there.  Else they go through LDS.
-template <int BYTES>
-struct WordsOf {
-  typedef unsigned Type __attribute__((ext_vector_type(BYTES / 4)));
-};
-template <>
-struct WordsOf<4> {
-  typedef unsigned Type;
-};
-template <>
-struct WordsOf<2> {
-  typedef unsigned short Type;
-};
 template <typename T, int Q, int R>
 struct ScanRows {
   static constexpr int kParts = Q == 4 ? 1 : Q / 4, kBytes = R * (int)sizeof(T), kWords = kBytes < 4 ? 1 : kBytes / 4;
   unsigned w[kParts][kWords];  // as they lie in memory, so that nothing waits for them before they are put to use
   static __device__ __forceinline__ int token(int lane, int i) { return Q == 4 ? lane % 16 : (lane + 64 * i) / Q; }
   static __device__ __forceinline__ int state(int lane, int i) { return (Q == 4 ? lane / 16 : (lane + 64 * i) % Q) * R; }
-  // p: the tile's first token; whole: R neighbours can be read at once, and n is a multiple of R
+  // p: the tile's first token; whole: n is a multiple of R
   __device__ __forceinline__ void load(const T* p, long long st, int n, bool whole, int lane, int left) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
       const int k = state(lane, i);
       const unsigned at = __umul24(min(token(lane, i), left - 1), st);
       if (whole) {
-        typedef typename WordsOf<kBytes>::Type Words;
-        const Words v = *reinterpret_cast<const Words*>(lane_address(p, (at + min(k, n - R)) * (unsigned)sizeof(T)));
-        if constexpr (kWords == 1) {
-          w[i][0] = v;
-        } else {
-#pragma unroll
-          for (int j = 0; j < kWords; ++j) w[i][j] = v[j];
-        }
+        // (one access, which the memory takes at any address of an element)
+        const T* const from = lane_address(p, (at + min(k, n - R)) * (unsigned)sizeof(T));
+        if constexpr (kBytes < 4)
+          w[i][0] = *reinterpret_cast<const unsigned short*>(from);
+        else
+          __builtin_memcpy(w[i], from, kBytes);
       } else {
 #pragma unroll
         for (int j = 0; j < kWords; ++j) w[i][j] = 0;
@@ -278,10 +264,6 @@ __device__ __forceinline__ void reverse_token(const ScanBank<Q, R>& b, const flo
 }
 template <int Q, int R>
 constexpr int kBankWords = Q == 4 ? 1 : 16 * Q * R;
-template <typename T, int R>
-__device__ __forceinline__ bool rows_whole(const void* p, long long sb, long long st, long long sg, int n) {
-  return (reinterpret_cast<uintptr_t>(p) % (R * sizeof(T)) | (sb | st | sg | n) % R) == 0;
-}
 
 // sums over a channel's lanes of Q values: lane q receives the q-th
 template <int Q, int MASK = 32>
@@ -380,7 +362,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
   const T* pz = p.z ? static_cast<const T*>(p.z) + s.row * p.z_sb + seg_begin * p.z_st + s.base : nullptr;
   const T* pb = static_cast<const T*>(p.b) + s.row * p.b_sb + seg_begin * p.b_st + s.group * p.b_sg;
   const T* pc = static_cast<const T*>(p.c) + s.row * p.c_sb + seg_begin * p.c_st + s.group * p.c_sg;
-  const bool b_whole = rows_whole<T, R>(p.b, p.b_sb, p.b_st, p.b_sg, p.n), c_whole = rows_whole<T, R>(p.c, p.c_sb, p.c_st, p.c_sg, p.n);
+  const bool whole = p.n % R == 0;  // rows of b and c can be read by R neighbours
   T* const y = OUT ? static_cast<T*>(p.y) + s.row * p.tokens * p.channels + s.base : nullptr;
   const int channel = s.base + s.own;
 
@@ -403,9 +385,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
   const auto fetch = [&](int left) {
     x.load(px, p.x_st, s, left);
     dt.load(pdt, p.dt_st, s, left);
-    b.load(pb, p.b_st, p.n, b_whole, s.lane, left);
+    b.load(pb, p.b_st, p.n, whole, s.lane, left);
     if (OUT) {
-      c.load(pc, p.c_st, p.n, c_whole, s.lane, left);
+      c.load(pc, p.c_st, p.n, whole, s.lane, left);
       if (pz) z.load(pz, p.z_st, s, left), pz += kScanTile * p.z_st;
     }
     px += kScanTile * p.x_st, pdt += kScanTile * p.dt_st, pb += kScanTile * p.b_st, pc += kScanTile * p.c_st;
@@ -511,7 +493,7 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
   const T* const pc = static_cast<const T*>(p.c) + s.row * p.c_sb + s.group * p.c_sg;
   const long long plane = s.row * p.tokens * p.channels + s.base;  // of contiguous (batch, tokens, channels)
   const T* const pdy = static_cast<const T*>(p.dy) + plane;
-  const bool b_whole = rows_whole<T, R>(p.b, p.b_sb, p.b_st, p.b_sg, p.n), c_whole = rows_whole<T, R>(p.c, p.c_sb, p.c_st, p.c_sg, p.n);
+  const bool whole = p.n % R == 0;  // rows of b and c can be read by R neighbours
   const States<R>* const kept = reinterpret_cast<const States<R>*>(p.kept) + s.unit * kept_states(p) * 64;
   const int channel = s.base + s.own;
 
@@ -536,11 +518,11 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
     asm volatile("" : "+v"(kept_lane));
     dt.load(pdt + t0 * p.dt_st, p.dt_st, s, left);
     dy.load(pdy + t0 * p.channels, p.channels, s, left);
-    c.load(pc + t0 * p.c_st, p.c_st, p.n, c_whole, s.lane, left);
+    c.load(pc + t0 * p.c_st, p.c_st, p.n, whole, s.lane, left);
     if (pz) z.load(pz + t0 * p.z_st, p.z_st, s, left);
     if (!SUM) {
       x.load(px + t0 * p.x_st, p.x_st, s, left);
-      b.load(pb + t0 * p.b_st, p.b_st, p.n, b_whole, s.lane, left);
+      b.load(pb + t0 * p.b_st, p.b_st, p.n, whole, s.lane, left);
       if (t0 > 0)
         // (kept_lane: a register of its own.  An address in one that the other way loads into is waited for, and with it the loads above.)
         h0 = *reinterpret_cast<const States<R>*>(reinterpret_cast<const char*>(kept + (t0 / kScanStretch - 1) * 64) + kept_lane);

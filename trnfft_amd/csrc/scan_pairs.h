@@ -98,7 +98,7 @@ __global__ __launch_bounds__(64 * kPairWaves) void scan_pair_kernel(ScanArgs p, 
   const T* pz = p.z ? static_cast<const T*>(p.z) + s.row * p.z_sb + s.base : nullptr;
   const T* pb = static_cast<const T*>(p.b) + s.row * p.b_sb + s.group * p.b_sg + 8 * half;
   const T* pc = static_cast<const T*>(p.c) + s.row * p.c_sb + s.group * p.c_sg + 8 * half;
-  const bool b_whole = rows_whole<T, 2>(p.b, p.b_sb, p.b_st, p.b_sg, p.n), c_whole = rows_whole<T, 2>(p.c, p.c_sb, p.c_st, p.c_sg, p.n);
+  const bool whole = p.n % 2 == 0;
   T* const y = static_cast<T*>(p.y) + s.row * p.tokens * p.channels + s.base;
   const int channel = s.base + s.own;
   const long long states = (s.row * p.channels + channel) * p.n + 8 * half;
@@ -124,8 +124,8 @@ __global__ __launch_bounds__(64 * kPairWaves) void scan_pair_kernel(ScanArgs p, 
     if (left < kScanTile) place(left);
     o.x.load(px, x_at);
     o.dt.load(pdt, dt_at);
-    o.b.load(pb, p.b_st, n, b_whole, s.lane, left);
-    o.c.load(pc, p.c_st, n, c_whole, s.lane, left);
+    o.b.load(pb, p.b_st, n, whole, s.lane, left);
+    o.c.load(pc, p.c_st, n, whole, s.lane, left);
     if (pz) o.z.load(pz, z_at), pz += kScanTile * p.z_st;
     px += kScanTile * p.x_st, pdt += kScanTile * p.dt_st, pb += kScanTile * p.b_st, pc += kScanTile * p.c_st;
   };
