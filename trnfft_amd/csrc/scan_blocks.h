@@ -155,32 +155,32 @@ struct ScanRows {
   unsigned w[kParts][kWords];  // as they lie in memory, so that nothing waits for them before they are put to use
   static __device__ __forceinline__ int token(int lane, int i) { return Q == 4 ? lane % 16 : (lane + 64 * i) / Q; }
   static __device__ __forceinline__ int state(int lane, int i) { return (Q == 4 ? lane / 16 : (lane + 64 * i) % Q) * R; }
-  // p: the tile's first token; whole: n is a multiple of R
-  __device__ __forceinline__ void load(const T* p, long long st, int n, bool whole, int lane, int left) {
+  // p: the tile's first token; first: the state that lane 0 begins with; n: all states, at least R.  Behind the last R a lane reads these.
+  __device__ __forceinline__ void load(const T* p, long long st, int n, int first, int lane, int left) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
-      const int k = state(lane, i);
       const unsigned at = __umul24(min(token(lane, i), left - 1), st);
-      if (whole) {
-        // (one access, which the memory takes at any address of an element)
-        const T* const from = lane_address(p, (at + min(k, n - R)) * (unsigned)sizeof(T));
-        if constexpr (kBytes < 4)
-          w[i][0] = *reinterpret_cast<const unsigned short*>(from);
-        else
-          __builtin_memcpy(w[i], from, kBytes);
-      } else {
+      // (one access, which the memory takes at any address of an element)
+      const T* const from = lane_address(p, (at + min(first + state(lane, i), n - R)) * (unsigned)sizeof(T));
+      if constexpr (kBytes < 4)
+        w[i][0] = *reinterpret_cast<const unsigned short*>(from);
+      else
+        __builtin_memcpy(w[i], from, kBytes);
+    }
+  }
+  // `ahead` values more from the front dropped
+  __device__ __forceinline__ void drop(int i, int ahead) {
+    if constexpr (R == 4 && sizeof(T) == 2) {
+      const unsigned long long v = (w[i][0] | (unsigned long long)w[i][1] << 32) >> 16 * (ahead & 3);
+      w[i][0] = (unsigned)v, w[i][1] = (unsigned)(v >> 32);
+    } else if constexpr (R == 2 && sizeof(T) == 2) {
+      w[i][0] >>= 16 * (ahead & 1);
+    } else if constexpr (R > 1) {
+      // (by masks: a choice between two of them would become a choice between their places in memory)
+      const unsigned one = -(unsigned)(ahead & 1), two = -(unsigned)(ahead >> 1 & 1);
 #pragma unroll
-        for (int j = 0; j < kWords; ++j) w[i][j] = 0;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const T v = *lane_address(p, (at + min(k + r, n - 1)) * (unsigned)sizeof(T));
-          if constexpr (sizeof(T) == 4)
-            w[i][r] = __builtin_bit_cast(unsigned, v);
-          else
-            w[i][r / 2] |= (unsigned)__builtin_bit_cast(unsigned short, v) << 16 * (r % 2);
-        }
-        asm volatile("");  // (as above)
-      }
+      for (int r = 0; r < R - 1; ++r) w[i][r] = (w[i][r + 1] & one) | (w[i][r] & ~one);
+      if constexpr (R == 4) w[i][0] = (w[i][2] & two) | (w[i][0] & ~two), w[i][1] = (w[i][3] & two) | (w[i][1] & ~two);
     }
   }
   __device__ __forceinline__ float value(int i, int r) const {
@@ -194,14 +194,15 @@ template <int Q, int R>
 struct ScanBank {
   States<R> own;
   template <typename T>
-  __device__ __forceinline__ void put(const ScanRows<T, Q, R>& rows, float* lds, int n, int lane, int left) {
-    const bool all = n == Q * R && left == kScanTile;
+  __device__ __forceinline__ void put(ScanRows<T, Q, R> rows, float* lds, int n, int first, int lane, int left) {
+    const bool all = n - first >= Q * R && left == kScanTile;
 #pragma unroll
     for (int i = 0; i < rows.kParts; ++i) {
+      const int t = rows.token(lane, i), k = first + rows.state(lane, i);
+      if (n % R) rows.drop(i, max(k + R - n, 0));  // (the lane that has the last states has read some before its own)
 #pragma unroll
       for (int r = 0; r < R; ++r) own.v[r] = rows.value(i, r);
       if (!all) {
-        const int t = rows.token(lane, i), k = rows.state(lane, i);
 #pragma unroll
         for (int r = 0; r < R; ++r) own.v[r] = k + r < n && t < left ? own.v[r] : 0.0f;
       }
@@ -362,7 +363,6 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
   const T* pz = p.z ? static_cast<const T*>(p.z) + s.row * p.z_sb + seg_begin * p.z_st + s.base : nullptr;
   const T* pb = static_cast<const T*>(p.b) + s.row * p.b_sb + seg_begin * p.b_st + s.group * p.b_sg;
   const T* pc = static_cast<const T*>(p.c) + s.row * p.c_sb + seg_begin * p.c_st + s.group * p.c_sg;
-  const bool whole = p.n % R == 0;  // rows of b and c can be read by R neighbours
   T* const y = OUT ? static_cast<T*>(p.y) + s.row * p.tokens * p.channels + s.base : nullptr;
   const int channel = s.base + s.own;
 
@@ -385,9 +385,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
   const auto fetch = [&](int left) {
     x.load(px, p.x_st, s, left);
     dt.load(pdt, p.dt_st, s, left);
-    b.load(pb, p.b_st, p.n, whole, s.lane, left);
+    b.load(pb, p.b_st, p.n, 0, s.lane, left);
     if (OUT) {
-      c.load(pc, p.c_st, p.n, whole, s.lane, left);
+      c.load(pc, p.c_st, p.n, 0, s.lane, left);
       if (pz) z.load(pz, p.z_st, s, left), pz += kScanTile * p.z_st;
     }
     px += kScanTile * p.x_st, pdt += kScanTile * p.dt_st, pb += kScanTile * p.b_st, pc += kScanTile * p.c_st;
@@ -413,9 +413,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void scan_forward_kernel(ScanArgs 
       if (!OUT) steps += own[i];
     }
     ScanBank<Q, R> bs, cs;
-    bs.put(b, lb, p.n, s.lane, left);
+    bs.put(b, lb, p.n, 0, s.lane, left);
     if (OUT) {
-      cs.put(c, lc, p.n, s.lane, left);
+      cs.put(c, lc, p.n, 0, s.lane, left);
       if (pz) {
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) zs[i] = activate(to_f32(z.v[i]), kActSilu);
@@ -493,7 +493,6 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
   const T* const pc = static_cast<const T*>(p.c) + s.row * p.c_sb + s.group * p.c_sg;
   const long long plane = s.row * p.tokens * p.channels + s.base;  // of contiguous (batch, tokens, channels)
   const T* const pdy = static_cast<const T*>(p.dy) + plane;
-  const bool whole = p.n % R == 0;  // rows of b and c can be read by R neighbours
   const States<R>* const kept = reinterpret_cast<const States<R>*>(p.kept) + s.unit * kept_states(p) * 64;
   const int channel = s.base + s.own;
 
@@ -518,11 +517,11 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
     asm volatile("" : "+v"(kept_lane));
     dt.load(pdt + t0 * p.dt_st, p.dt_st, s, left);
     dy.load(pdy + t0 * p.channels, p.channels, s, left);
-    c.load(pc + t0 * p.c_st, p.c_st, p.n, whole, s.lane, left);
+    c.load(pc + t0 * p.c_st, p.c_st, p.n, 0, s.lane, left);
     if (pz) z.load(pz + t0 * p.z_st, p.z_st, s, left);
     if (!SUM) {
       x.load(px + t0 * p.x_st, p.x_st, s, left);
-      b.load(pb + t0 * p.b_st, p.b_st, p.n, whole, s.lane, left);
+      b.load(pb + t0 * p.b_st, p.b_st, p.n, 0, s.lane, left);
       if (t0 > 0)
         // (kept_lane: a register of its own.  An address in one that the other way loads into is waited for, and with it the loads above.)
         h0 = *reinterpret_cast<const States<R>*>(reinterpret_cast<const char*>(kept + (t0 / kScanStretch - 1) * 64) + kept_lane);
@@ -622,8 +621,8 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
       }
     }
     ScanBank<Q, R> bs, cs;
-    cs.put(c, lc, p.n, s.lane, left);
-    if (!SUM) bs.put(b, lb, p.n, s.lane, left);
+    cs.put(c, lc, p.n, 0, s.lane, left);
+    if (!SUM) bs.put(b, lb, p.n, 0, s.lane, left);
     wave_order();
     const States<R> start = s.valid ? h0 : States<R>{};
     if (!SUM && t0 < last) results(t0 + kScanTile);

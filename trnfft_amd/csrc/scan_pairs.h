@@ -96,9 +96,8 @@ __global__ __launch_bounds__(64 * kPairWaves) void scan_pair_kernel(ScanArgs p, 
   const T* px = static_cast<const T*>(p.x) + s.row * p.x_sb + s.base;
   const T* pdt = static_cast<const T*>(p.dt) + s.row * p.dt_sb + s.base;
   const T* pz = p.z ? static_cast<const T*>(p.z) + s.row * p.z_sb + s.base : nullptr;
-  const T* pb = static_cast<const T*>(p.b) + s.row * p.b_sb + s.group * p.b_sg + 8 * half;
-  const T* pc = static_cast<const T*>(p.c) + s.row * p.c_sb + s.group * p.c_sg + 8 * half;
-  const bool whole = p.n % 2 == 0;
+  const T* pb = static_cast<const T*>(p.b) + s.row * p.b_sb + s.group * p.b_sg;
+  const T* pc = static_cast<const T*>(p.c) + s.row * p.c_sb + s.group * p.c_sg;
   T* const y = static_cast<T*>(p.y) + s.row * p.tokens * p.channels + s.base;
   const int channel = s.base + s.own;
   const long long states = (s.row * p.channels + channel) * p.n + 8 * half;
@@ -124,8 +123,8 @@ __global__ __launch_bounds__(64 * kPairWaves) void scan_pair_kernel(ScanArgs p, 
     if (left < kScanTile) place(left);
     o.x.load(px, x_at);
     o.dt.load(pdt, dt_at);
-    o.b.load(pb, p.b_st, n, whole, s.lane, left);
-    o.c.load(pc, p.c_st, n, whole, s.lane, left);
+    o.b.load(pb, p.b_st, p.n, 8 * half, s.lane, left);
+    o.c.load(pc, p.c_st, p.n, 8 * half, s.lane, left);
     if (pz) o.z.load(pz, z_at), pz += kScanTile * p.z_st;
     px += kScanTile * p.x_st, pdt += kScanTile * p.dt_st, pb += kScanTile * p.b_st, pc += kScanTile * p.c_st;
   };
@@ -155,8 +154,8 @@ __global__ __launch_bounds__(64 * kPairWaves) void scan_pair_kernel(ScanArgs p, 
       put_pair_token(lu, s, half, i, own[i] * xs[i]);
     }
     ScanBank<4, 2> bs, cs;
-    bs.put(o.b, nullptr, n, s.lane, left);
-    cs.put(o.c, nullptr, n, s.lane, left);
+    bs.put(o.b, nullptr, p.n, 8 * half, s.lane, left);
+    cs.put(o.c, nullptr, p.n, 8 * half, s.lane, left);
     if (pz) {
 #pragma unroll
       for (int i = 0; i < kPairOwn; ++i) zs[i] = activate(o.z.value(i), kActSilu);
