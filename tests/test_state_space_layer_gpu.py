@@ -234,6 +234,43 @@ def test_a_capture_refuses_leaves_whose_eager_graph_lives():
         assert torch.equal(g, want)
 
 
+def test_threads_and_streams_do_not_share():
+    """Calls of several threads, each on a stream of its own: the native calls give up Python's lock."""
+    import threading
+
+    cases = [[v.requires_grad_() for v in operands(rows=2, t=t, ch=ch, seed=seed)] for seed, (t, ch) in enumerate([(300, 24), (700, 40), (33, 130)])]
+
+    def passes(leaves):
+        y, last = trnfft_amd.selective_scan(*leaves, return_state=True)
+        u = trnfft_amd.causal_conv(y, torch.ones(y.shape[2], 3, device="cuda"), activation="relu")
+        grads = torch.autograd.grad([u, last], leaves, [torch.ones_like(u), torch.ones_like(last)])
+        norm = trnfft_amd.grad_norm([g.contiguous() for g in grads])
+        return [y.detach(), last.detach(), u.detach(), *grads, norm]
+
+    want = [passes(leaves) for leaves in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(leaves, expected):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = passes(leaves)
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, expected)):
+                        wrong.append("results differ")
+        except Exception as e:  # (of the thread)
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=pair) for pair in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_results_do_not_depend_on_timing():
     leaves = [v.requires_grad_() for v in operands(rows=3, t=900, ch=130, seed=4)]
 
