@@ -212,22 +212,28 @@ __device__ __forceinline__ float sum_lanes(float v) {
 // Q neighbouring lanes a channel, 4 states each, so that a wave reads and writes its states in one piece; ROWS streams a thread, whose states
 // are on their way together and for which a, d and dt_bias are read once.  Memory bound by the states.  256 streams of 2048 channels of 16
 // states, bf16: 16.9 us (72 MB); with one stream a thread 19.0, four 19.7, eight 28.0.
-// whole: states and a, b and c can be read by fours
+// States, a, b and c are read by fours where n is a multiple of that: the memory takes one access at any address of an element.
 template <typename T, int Q, int ROWS>
-__global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, bool whole, bool rows_whole, long long first) {
+__global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, long long first) {
   const long long id = ((first + blockIdx.x) * 256 + threadIdx.x) / Q, row0 = id / p.channels * ROWS;
   const int q = threadIdx.x % Q;
   if (row0 >= p.batch) return;
   const int channel = (int)(id % p.channels), group = channel / (p.channels / p.groups), k0 = 4 * q;
-  const bool all = whole && k0 < p.n;
-  const auto states_of = [&](const float* at) { return all ? *reinterpret_cast<const Four32*>(at + k0) : load_states<4>(at, p.n, q, true); };
+  const bool all = p.n % 4 == 0 && k0 < p.n;
+  const auto states_of = [&](const float* at) {
+    if (!all) return load_states<4>(at, p.n, q, true);
+    Four32 v;
+    __builtin_memcpy(v.v, at + k0, sizeof(v));
+    return v;
+  };
   const auto rows_of = [&](const void* base, long long at) {
     const T* const from = static_cast<const T*>(base) + at;
     Four32 v;
-    if (rows_whole && k0 < p.n) {
-      const Pack<T, 4> u = *reinterpret_cast<const Pack<T, 4>*>(from + k0);
+    if (all) {
+      T u[4];
+      __builtin_memcpy(u, from + k0, sizeof(u));
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v.v[r] = to_f32(u.v[r]);
+      for (int r = 0; r < 4; ++r) v.v[r] = to_f32(u[r]);
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r) v.v[r] = k0 + r < p.n ? to_f32(from[k0 + r]) : 0.0f;
@@ -266,7 +272,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, bool whole, 
     }
     float* const state = p.state + (row * p.channels + channel) * p.n;
     if (all)
-      *reinterpret_cast<Four32*>(state + k0) = h[i];
+      __builtin_memcpy(state + k0, h[i].v, sizeof(h[i]));
     else
       store_states<4>(state, p.n, q, true, h[i]);
     y = sum_lanes<Q>(y);
@@ -279,11 +285,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p, bool whole, 
 
 template <typename T, int Q, int ROWS>
 static hipError_t step_rows(const ScanStep& p) {
-  const bool whole = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.state) | reinterpret_cast<uintptr_t>(p.a)) % 16 == 0;
-  const bool rows = (reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.c)) % (4 * sizeof(T)) == 0 &&
-                    (p.b_sb | p.b_sg | p.c_sb | p.c_sg | p.n) % 4 == 0;
   return scan_launches((p.batch + ROWS - 1) / ROWS * p.channels * Q, [&](long long first, unsigned n) {
-    hipLaunchKernelGGL((scan_step_kernel<T, Q, ROWS>), dim3(n), dim3(256), 0, p.stream, p, whole, rows, first);
+    hipLaunchKernelGGL((scan_step_kernel<T, Q, ROWS>), dim3(n), dim3(256), 0, p.stream, p, first);
   });
 }
 // Two streams a thread where that leaves 2048 waves
