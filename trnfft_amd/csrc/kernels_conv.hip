@@ -24,6 +24,27 @@ constexpr int kRunMost = 64;
 // tokens of 2048 bf16 channels and 4 taps: 101 us, 4 tokens 122)
 constexpr int kConvBatch = 4, kConvBackBatch = 2;
 
+// V neighbouring values in one access, which the memory takes at any address of an element
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> pack_at(const T* p) {
+  Pack<T, V> u;
+  __builtin_memcpy(&u, p, sizeof(u));
+  return u;
+}
+template <typename T, int V>
+__device__ __forceinline__ void load_any(const T* p, float (&x)[V]) {
+  const Pack<T, V> u = pack_at<T, V>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = to_f32(u.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_any(T* p, const float (&x)[V]) {
+  Pack<T, V> u;
+#pragma unroll
+  for (int i = 0; i < V; ++i) u.v[i] = from_f32<T>(x[i]);
+  __builtin_memcpy(p, &u, sizeof(u));
+}
+
 __device__ __forceinline__ long long conv_end(const long long* lengths, long long row, long long tokens) {
   return lengths ? min(max(lengths[row], 0LL), tokens) : tokens;
 }
@@ -32,9 +53,9 @@ __device__ __forceinline__ long long conv_end(const long long* lengths, long lon
 template <typename T, int V, int W>
 __device__ __forceinline__ void conv_frame(const T* x, long long st, const T* state, long long channels, long long t, float (&v)[V]) {
   if (t >= 0) {
-    load_pack<T, V>(x + t * st, v);
+    load_any<T, V>(x + t * st, v);
   } else if (state) {
-    load_pack<T, V>(state + (t + W - 1) * channels, v);
+    load_any<T, V>(state + (t + W - 1) * channels, v);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = 0.0f;
@@ -93,7 +114,7 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a, int vecto
     for (int j = 0; j < W - 1; ++j) {
       float v[V];
       conv_frame<T, V, W>(x, a.x_st, state, a.channels, end + j - (W - 1), v);
-      store_pack<T, V>(out + (long long)j * a.channels, v);
+      store_any<T, V>(out + (long long)j * a.channels, v);
     }
   }
   if (s.t0 < live) {
@@ -112,19 +133,19 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(ConvArgs a, int vecto
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
     }
-    store_pack<T, V>(y + t * a.channels, z);
+    store_any<T, V>(y + t * a.channels, z);
   };
   long long t = s.t0;
   for (; t + kConvBatch <= live; t += kConvBatch) {
     Pack<T, V> u[kConvBatch];
 #pragma unroll
-    for (int k = 0; k < kConvBatch; ++k) u[k] = *reinterpret_cast<const Pack<T, V>*>(x + (t + k) * a.x_st);
+    for (int k = 0; k < kConvBatch; ++k) u[k] = pack_at<T, V>(x + (t + k) * a.x_st);
 #pragma unroll
     for (int k = 0; k < kConvBatch; ++k) token(t + k, u[k]);
   }
-  for (; t < live; ++t) token(t, *reinterpret_cast<const Pack<T, V>*>(x + t * a.x_st));
+  for (; t < live; ++t) token(t, pack_at<T, V>(x + t * a.x_st));
   const float none[V] = {};
-  for (t = max(s.t0, live); t < s.t1; ++t) store_pack<T, V>(y + t * a.channels, none);
+  for (t = max(s.t0, live); t < s.t1; ++t) store_any<T, V>(y + t * a.channels, none);
 }
 
 // The workgroup's filter gradients are added in LDS.  parts: (workgroups along the runs, channels, W + 1)
@@ -188,21 +209,21 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a, int vect
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) dpre[j][i] = dpre[j + 1][i];
       }
-      if (to) store_pack<T, V>(to, d);
+      if (to) store_any<T, V>(to, d);
     };
     const float none[V] = {};
     // The first W - 1 tokens complete frames of the run before, or of the state before the first
     long long t = s.t0;
     for (; t < live && t < s.t0 + W - 1; ++t) {
-      token(*reinterpret_cast<const Pack<T, V>*>(x + t * a.x_st), *reinterpret_cast<const Pack<T, V>*>(dy + t * a.channels), std::true_type());
+      token(pack_at<T, V>(x + t * a.x_st), pack_at<T, V>(dy + t * a.channels), std::true_type());
       frame(s.t0 == 0 && dstate ? dstate + t * a.channels : nullptr, none);
     }
     for (; t + kConvBackBatch <= live; t += kConvBackBatch) {
       Pack<T, V> u[kConvBackBatch], g[kConvBackBatch];
 #pragma unroll
       for (int k = 0; k < kConvBackBatch; ++k) {
-        u[k] = *reinterpret_cast<const Pack<T, V>*>(x + (t + k) * a.x_st);
-        g[k] = *reinterpret_cast<const Pack<T, V>*>(dy + (t + k) * a.channels);
+        u[k] = pack_at<T, V>(x + (t + k) * a.x_st);
+        g[k] = pack_at<T, V>(dy + (t + k) * a.channels);
       }
 #pragma unroll
       for (int k = 0; k < kConvBackBatch; ++k) {
@@ -213,7 +234,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a, int vect
     // the rest of the run, the W - 1 tokens behind it, and padding
     for (; t < s.t1 + W - 1; ++t) {
       if (t < end) {
-        const Pack<T, V> u = *reinterpret_cast<const Pack<T, V>*>(x + t * a.x_st), g = *reinterpret_cast<const Pack<T, V>*>(dy + t * a.channels);
+        const Pack<T, V> u = pack_at<T, V>(x + t * a.x_st), g = pack_at<T, V>(dy + t * a.channels);
         if (t < s.t1)
           token(u, g, std::true_type());
         else
@@ -224,7 +245,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(ConvArgs a, int vect
       }
       const long long at = t - (W - 1), k = t - end;  // the frame, and its place in the state at the end
       float more[V] = {};
-      if (dlast && k >= 0 && k < W - 1) load_pack<T, V>(dlast + k * a.channels, more);
+      if (dlast && k >= 0 && k < W - 1) load_any<T, V>(dlast + k * a.channels, more);
       T* to = nullptr;
       if (at >= 0 ? at >= s.t0 : s.t0 == 0) to = at >= 0 ? (dx ? dx + at * a.channels : nullptr) : (dstate ? dstate + (at + W - 1) * a.channels : nullptr);
       frame(to, more);
@@ -279,8 +300,8 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, int vectors,
   T* const state = static_cast<T*>(a.state_out) + row * (W - 1) * a.channels + c;
   float win[W][V], z[V];
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) load_pack<T, V>(state + (long long)j * a.channels, win[j]);
-  load_pack<T, V>(static_cast<const T*>(a.x) + row * a.x_sb + c, win[W - 1]);
+  for (int j = 0; j < W - 1; ++j) load_any<T, V>(state + (long long)j * a.channels, win[j]);
+  load_any<T, V>(static_cast<const T*>(a.x) + row * a.x_sb + c, win[W - 1]);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float s = a.bias ? a.bias[c + i] : 0.0f;
@@ -289,8 +310,8 @@ __global__ __launch_bounds__(256) void conv_step_kernel(ConvArgs a, int vectors,
     z[i] = activate(s, a.act);
   }
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) store_pack<T, V>(state + (long long)j * a.channels, win[j + 1]);
-  store_pack<T, V>(static_cast<T*>(a.y) + row * a.channels + c, z);
+  for (int j = 0; j < W - 1; ++j) store_any<T, V>(state + (long long)j * a.channels, win[j + 1]);
+  store_any<T, V>(static_cast<T*>(a.y) + row * a.channels + c, z);
 }
 
 struct ConvRuns {
@@ -312,23 +333,12 @@ static ConvRuns conv_runs(const ConvArgs& a, int v) {
   return r;
 }
 
-static size_t type_size(int dtype) { return dtype == 0 ? 4 : 2; }
-
-// whether vectors of v values can be read and written
-static bool conv_whole(const ConvArgs& a, int v) {
-  const uintptr_t bytes = v * type_size(a.dtype);
-  const void* const all[] = {a.x, a.y, a.state_in, a.state_out, a.dy, a.dstate_out, a.dx, a.dstate_in};
-  for (const void* p : all)
-    if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
-  return a.channels % v == 0 && a.x_sb % v == 0 && a.x_st % v == 0;
-}
 // Values a vector backward: 4, so that the windows of x and dpre, the filters and their gradients stay in registers
 constexpr int kConvBackwardVector = 4;
 static int conv_backward_vector(const ConvArgs& a) { return a.channels % kConvBackwardVector == 0 ? kConvBackwardVector : 1; }
 
 size_t conv_workspace_bytes(const ConvArgs& a) {
-  // (the vector that the addresses allow may be narrower than the sizes do: as many parts as the more of both)
-  const long long parts = std::max(conv_runs(a, conv_backward_vector(a)).parts, conv_runs(a, 1).parts);
+  const long long parts = conv_runs(a, conv_backward_vector(a)).parts;
   return (size_t)parts * a.channels * (a.width + 1) * sizeof(float);
 }
 
@@ -385,7 +395,7 @@ static hipError_t conv_vector(const ConvArgs& a) {
 template <ConvMode MODE, typename T>
 static hipError_t conv_typed(const ConvArgs& a) {
   constexpr int V = MODE == kConvBackward ? kConvBackwardVector : 16 / (int)sizeof(T);
-  return conv_whole(a, V) ? conv_vector<MODE, T, V>(a) : conv_vector<MODE, T, 1>(a);
+  return a.channels % V == 0 ? conv_vector<MODE, T, V>(a) : conv_vector<MODE, T, 1>(a);
 }
 
 template <ConvMode MODE>
