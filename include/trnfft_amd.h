@@ -422,7 +422,8 @@ int tfa_causal_conv_step(const tfa_conv_desc* desc, const void* x, const float* 
  * at and past a sequence's length are padding: never read, zeros in y and the gradients, and the state is the one at the length.
  * States, exponentials and sums are fp32 for every type: a decay is rounded once a token, so over a memory of m tokens (exponents of
  * steps that are the same from token to token) a state can be off by m 2^-25 of itself.  What is not finite makes NaN or infinities
- * of its channel from its token on.  Up to 64 states.
+ * of its channel from its token on, but for dt_t + dt_bias of -inf under softplus: a step of 0, which leaves the state.  Up to 64
+ * states.
  */
 typedef struct tfa_scan_desc {
   int32_t dtype; /* TFA_DTYPE_* of x, dt, z, b, c, y and their gradients */

@@ -1,0 +1,82 @@
+"""The state space operators where steps are zero.  References and tolerances are those of test_state_space_gpu.py: what is not masked
+passes the same operations, and what is masked is zero or the same bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import trnfft_amd
+from test_state_space_gpu import SUMS, TOL, cuda, rel, scan, scan_inputs, scan_reference, tol
+
+pytestmark = pytest.mark.gpu
+
+# rows, t, channels, groups, states: 1, 2 and 4 states a lane, two waves a channel, segments, 8 and 16 lanes a channel
+SHAPES = [(2, 37, 24, 1, 4), (2, 21, 12, 2, 7), (2, 50, 70, 2, 12), (1, 600, 20, 1, 16), (2, 35, 12, 1, 20), (2, 33, 9, 1, 40)]
+INF = float("inf")
+
+
+def check(v, lengths):
+    """Outputs and all gradients against the definition; returns y, the last state and the gradients."""
+    dtype, names = v["x"].dtype, list(v)
+    ref = {k: x.double().requires_grad_() for k, x in v.items()}
+    y_ref, last_ref = scan_reference(**ref, softplus=True, lengths=lengths)
+    own = {k: cuda(x).requires_grad_() for k, x in v.items()}
+    y, last = scan(own, cuda(lengths))
+    assert rel(y, y_ref) <= tol(y_ref, dtype) and rel(last, last_ref) <= 2e-6
+    g = torch.Generator().manual_seed(1)
+    dy, dlast = torch.randn(y.shape, generator=g).to(dtype), torch.randn(last.shape, generator=g)
+    want = torch.autograd.grad([y_ref, last_ref], list(ref.values()), [dy.double(), dlast.double()])
+    got = torch.autograd.grad([y, last], list(own.values()), [cuda(dy), cuda(dlast)])
+    for name, w, d in zip(names, want, got):
+        assert torch.isfinite(w).all(), name
+        bound = SUMS if name in ("a", "d", "dt_bias") else 2e-6 if name == "state" else tol(w, dtype)
+        if dtype == torch.float32 and name in ("dt", "b", "c", "z", "x"):
+            bound = 4e-6
+        assert rel(d, w) <= bound, name
+    return y, last, dict(zip(names, got))
+
+
+@pytest.mark.parametrize("dtype", list(TOL))
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_a_step_before_softplus_of_minus_infinity_is_none(shape, dtype):
+    """Frames masked by dt, for a channel or for all of them, and channels masked by dt_bias leave the state."""
+    v, _ = scan_inputs(*shape, dtype, 3)
+    t = shape[1]
+    lengths = torch.tensor([t, t - 5][:shape[0]])
+    v["dt"][0, t // 2, 1] = v["dt"][:, 3] = v["dt"][-1, t - 7:] = -INF
+    v["dt_bias"][2] = -INF
+    y, last, grads = check(v, lengths)
+    assert torch.equal(last[:, 2].cpu(), v["state"][:, 2])
+    for at in ((0, t // 2, 1), (slice(None), 3), (slice(None), slice(None), 2)):
+        assert not grads["dt"][at].any()
+    assert not grads["dt_bias"][2].any()
+
+
+@pytest.mark.parametrize("value", [-INF, torch.finfo(torch.float32).min, -200.0, 200.0, 1.8e38, 3e38])
+def test_softplus_far_out(value):
+    """Zero on one side and the value itself on the other, up to the type's ends."""
+    one = torch.ones(1, 3, 16, device="cuda")
+    b = torch.ones(1, 3, 1, 4, device="cuda")
+    a = torch.zeros(16, 4, device="cuda")
+    want = max(value, 0.0)
+    for dt, bias in ((one * value, None), (one * 0.0, torch.full((16,), value, device="cuda"))):
+        y, last = trnfft_amd.selective_scan(one * 2.0**-8, dt, a, b, b, dt_bias=bias, return_state=True)
+        assert torch.equal(last, torch.full_like(last, 3 * 2.0**-8 * torch.tensor(want).item()))
+        state = torch.zeros(1, 16, 4, device="cuda")
+        trnfft_amd.selective_scan_step(one[:, 0] * 2.0**-8, dt[:, 0], a, b[:, 0], b[:, 0], state, dt_bias=bias)
+        assert torch.equal(state, torch.full_like(state, 2.0**-8 * torch.tensor(want).item()))
+
+
+@pytest.mark.parametrize("dtype", list(TOL))
+@pytest.mark.parametrize("states", [4, 7, 16, 20, 40])
+def test_masked_steps_leave_the_state_of_a_stream(states, dtype):
+    v, _ = scan_inputs(5, 1, 24, 2, states, dtype, 4)
+    one = {k: cuda(x)[:, 0] for k, x in v.items() if k in ("x", "dt", "b", "c", "z")}
+    a, d, bias, state = (cuda(v[k]) for k in ("a", "d", "dt_bias", "state"))
+    one["dt"][1], one["dt"][3, 7], bias[5] = -INF, -INF, -INF
+    before = state.clone()
+    y = trnfft_amd.selective_scan_step(one["x"], one["dt"], a, one["b"], one["c"], state, d=d, z=one["z"], dt_bias=bias)
+    assert torch.isfinite(y).all() and torch.isfinite(state).all()
+    assert torch.equal(state[1], before[1]) and torch.equal(state[3, 7], before[3, 7]) and torch.equal(state[:, 5], before[:, 5])
+    assert not torch.equal(state[0], before[0])

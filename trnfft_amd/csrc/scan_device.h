@@ -21,12 +21,13 @@ __device__ __forceinline__ float rate_of(float a) { return (a < -1e38f ? -1e38f 
 // log(1 + e^v) and its derivative, off by a few 2^-24 of themselves and of v: with e = e^-|v| and u = 1 + e, log(1 + e) = log(u) + (e - (u - 1)),
 // where the second term is what the sum u lost (the hardware's logarithm is good to its last bit next to 1 too).  Measured from -20 to 20:
 // 3e-8 of it in the mean square for v > 0, 2e-7 at -8, 1e-6 at most; a series for the artanh took twice the instructions for the same.
+// -inf gives a step of 0 with slope 0: a frame that is masked so leaves the state.
 __device__ __forceinline__ float softplus(float v, float& slope) {
   const float e = __builtin_amdgcn_exp2f(-fabsf(v) * kLog2E), u = 1.0f + e;
   const float r = __builtin_fmaf(__builtin_amdgcn_logf(u), 0.69314718055994531f, e - (u - 1.0f));
   const float part = __builtin_amdgcn_rcpf(u);
   slope = v < 0.0f ? e * part : part;
-  return __builtin_fmaf(v + fabsf(v), 0.5f, r);  // (NaN stays)
+  return fmaxf(v, 0.0f) + r;  // (NaN stays: it is in r)
 }
 
 // x of the lane whose number differs by MASK (1, 2, 3, 7, 8: permutations within rows of 16 lanes; 4 is 7 after 3)

@@ -236,7 +236,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     States and sums are fp32.  A decay is rounded once a frame: where steps are the same from frame to frame, a state with a memory
     of m frames can be off by m 2^-25 of itself.  Gradients cannot be differentiated again, and there is no forward mode.  In a captured pass
     leaves are refused whose graph of an eager pass still lives: autograd would leave the capture for them.
-    A value that is not finite makes NaN or infinities of its channel from its frame on (of b and c: of its group's channels).
+    A value that is not finite makes NaN or infinities of its channel from its frame on (of b and c: of its group's channels), but for
+    dt + dt_bias of -inf under softplus, a step of 0: such a frame leaves the state.
     """
     what = "selective_scan"
     out = _direct(what, what, x, dt, a, b, c, d, z, dt_bias, initial_state, lengths, softplus, return_state)
