@@ -1,5 +1,5 @@
-"""The state space operators where steps are zero.  References and tolerances are those of test_state_space_gpu.py: what is not masked
-passes the same operations, and what is masked is zero or the same bits."""
+"""The state space operators where steps are zero or there is no memory.  References and tolerances are those of
+test_state_space_gpu.py: what is not masked passes the same operations, and what is masked is zero or the same bits."""
 
 from __future__ import annotations
 
@@ -16,16 +16,17 @@ SHAPES = [(2, 37, 24, 1, 4), (2, 21, 12, 2, 7), (2, 50, 70, 2, 12), (1, 600, 20,
 INF = float("inf")
 
 
-def check(v, lengths):
+def check(v, lengths, dlast_scale=1.0, of_reference=None):
     """Outputs and all gradients against the definition; returns y, the last state and the gradients."""
     dtype, names = v["x"].dtype, list(v)
-    ref = {k: x.double().requires_grad_() for k, x in v.items()}
+    ref = {**{k: x.double() for k, x in v.items()}, **(of_reference or {})}
+    ref = {k: x.requires_grad_() for k, x in ref.items()}
     y_ref, last_ref = scan_reference(**ref, softplus=True, lengths=lengths)
     own = {k: cuda(x).requires_grad_() for k, x in v.items()}
     y, last = scan(own, cuda(lengths))
     assert rel(y, y_ref) <= tol(y_ref, dtype) and rel(last, last_ref) <= 2e-6
     g = torch.Generator().manual_seed(1)
-    dy, dlast = torch.randn(y.shape, generator=g).to(dtype), torch.randn(last.shape, generator=g)
+    dy, dlast = torch.randn(y.shape, generator=g).to(dtype), torch.randn(last.shape, generator=g) * dlast_scale
     want = torch.autograd.grad([y_ref, last_ref], list(ref.values()), [dy.double(), dlast.double()])
     got = torch.autograd.grad([y, last], list(own.values()), [cuda(dy), cuda(dlast)])
     for name, w, d in zip(names, want, got):
@@ -80,3 +81,19 @@ def test_masked_steps_leave_the_state_of_a_stream(states, dtype):
     assert torch.isfinite(y).all() and torch.isfinite(state).all()
     assert torch.equal(state[1], before[1]) and torch.equal(state[3, 7], before[3, 7]) and torch.equal(state[:, 5], before[:, 5])
     assert not torch.equal(state[0], before[0])
+
+
+@pytest.mark.parametrize("dtype", list(TOL))
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_padding_has_no_gradient_where_there_is_no_memory(shape, dtype):
+    """Rates of -inf (in 64 bits, of -1e300: the same without 0 times infinity) before padding that ends inside a tile, and a large
+    gradient of a large last state: the steps' bias sums up frames, not padding."""
+    v, _ = scan_inputs(*shape, dtype, 5)
+    lengths = torch.tensor([shape[1], shape[1] - 9][:shape[0]])
+    v["state"] *= 30.0
+    v["b"] *= 30.0
+    far = v["a"].double()
+    v["a"][1], v["a"][3, 0] = -INF, -INF
+    far[1], far[3, 0] = -1e300, -1e300
+    _, _, grads = check(v, lengths, dlast_scale=30.0, of_reference={"a": far})
+    assert not grads["a"][1].any() and not grads["a"][3, 0].any()
