@@ -428,13 +428,16 @@ int tfa_causal_conv_step(const tfa_conv_desc* desc, const void* x, const float* 
 typedef struct tfa_scan_desc {
   int32_t dtype; /* TFA_DTYPE_* of x, dt, z, b, c, y and their gradients */
   int32_t channels, groups, states;
-  int32_t softplus, reserved;
+  int32_t softplus;
+  int32_t bc_fixed; /* not 0: no gradients of b and c are asked of the backward, whose sums are most of its workspace */
   int64_t batch, tokens;
   int64_t x_stride[2], dt_stride[2], z_stride[2]; /* batch, token */
   int64_t b_stride[3], c_stride[3];               /* batch, token, group */
 } tfa_scan_desc;
 
-/* Bytes of the states that a backward needs of its forward, and of the workspaces of both; all 16-byte aligned device memory. */
+/* Bytes of the states that a backward needs of its forward, and of the workspaces of both; all 16-byte aligned device memory.  For every
+ * token and channel: kept states n / 4, n being the states filled up to 4, 8, 16, 32 or 64; sums of the gradients of b and c n / 8
+ * (32 at 64: two fp32 states for 16 channels). */
 int tfa_selective_scan_sizes(const tfa_scan_desc* desc, size_t* kept, size_t* workspace, size_t* backward_workspace);
 /* state_in may be NULL (zeros), state_out NULL (not wanted; must not be state_in), kept NULL (no backward follows). */
 int tfa_selective_scan(const tfa_scan_desc* desc, const void* x, const void* dt, const float* a, const void* b, const void* c,

@@ -97,3 +97,25 @@ def test_padding_has_no_gradient_where_there_is_no_memory(shape, dtype):
     far[1], far[3, 0] = -1e300, -1e300
     _, _, grads = check(v, lengths, dlast_scale=30.0, of_reference={"a": far})
     assert not grads["a"][1].any() and not grads["a"][3, 0].any()
+
+
+@pytest.mark.parametrize("states", [4, 16, 20, 40])
+def test_no_memory_for_gradients_that_are_not_wanted(states):
+    """Fixed b and c: the others' gradients are the same, and the room that adds up b's and c's is not taken."""
+    v, _ = scan_inputs(2, 1024, 512, 1, states, torch.bfloat16, 8, extra=False)
+    own = {k: cuda(x) for k, x in v.items() if x is not None}
+    peaks, grads = [], []  # (bytes as they are asked for: blocks that the allocator has at hand may be larger)
+    for names in (("x", "dt", "a", "b", "c"), ("x", "dt", "a")):
+        leaves = {k: x.detach().requires_grad_(k in names) for k, x in own.items()}
+        y, _ = scan(leaves)
+        dy = torch.ones_like(y)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_stats()["requested_bytes.all.current"]
+        grads.append(torch.autograd.grad(y, [leaves[k] for k in names], dy))
+        peaks.append(torch.cuda.memory_stats()["requested_bytes.all.peak"] - before)
+    for name, one, two in zip(("x", "dt", "a"), *grads):
+        assert torch.equal(one, two), name
+    # values of two sets of states for every token and 64 (16 above 32 states) channels, and the gradients of b and c themselves
+    filled, channels = (64, 16) if states > 32 else (32, 64) if states > 16 else (16, 64) if states > 8 else (4, 64)
+    assert peaks[0] - peaks[1] >= 2 * 1024 * 2 * filled * 4 * (512 // channels)

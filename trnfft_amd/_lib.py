@@ -164,7 +164,7 @@ class ScanDesc(ctypes.Structure):
         ("groups", ctypes.c_int32),
         ("states", ctypes.c_int32),
         ("softplus", ctypes.c_int32),
-        ("reserved", ctypes.c_int32),
+        ("bc_fixed", ctypes.c_int32),
         ("batch", ctypes.c_int64),
         ("tokens", ctypes.c_int64),
         *((f"{name}_stride_{axis}", ctypes.c_int64) for name in ("x", "dt", "z") for axis in ("batch", "token")),

@@ -222,12 +222,13 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
       const at::Tensor &x = saved[0], &dt = saved[1], &a = saved[2], &b = saved[3], &c = saved[4], &d = saved[5], &z = saved[6], &bias = saved[7],
                        &state = saved[8], &lengths = saved[9], &kept = saved[10];
       const c10::DeviceGuard guard(x.device());
-      const tfa_scan_desc desc = scan_desc(x, dt, a, b, c, z, ctx->saved_data["softplus"].toBool());
+      tfa_scan_desc desc = scan_desc(x, dt, a, b, c, z, ctx->saved_data["softplus"].toBool());
+      make_grads(ctx, saved, 9, grads);
+      desc.bc_fixed = !grads[3].defined() && !grads[4].defined();
       size_t kept_size = 0, forward_size = 0, size = 0;
       run_backward(entries.scan_sizes(&desc, &kept_size, &forward_size, &size), "selective_scan");
       const at::Tensor workspace = bytes_like(x, size);
       const at::Tensor dy = g[0].defined() ? dense(g[0]) : at::zeros(x.sizes(), x.options()), dlast = g.size() > 1 ? dense(g[1]) : at::Tensor();
-      make_grads(ctx, saved, 9, grads);
       tfa_scan_grads out{};
       out.grad_y = data(dy), out.grad_state_out = floats(dlast);
       out.x = data(grads[0]), out.dt = data(grads[1]), out.a = floats(grads[2]), out.b = data(grads[3]), out.c = data(grads[4]);

@@ -238,7 +238,7 @@ int tfa_selective_scan_sizes(const tfa_scan_desc* desc, size_t* kept, size_t* wo
   const tfa::ScanSizes f = tfa::scan_sizes(scan_args(desc, false)), b = tfa::scan_sizes(scan_args(desc, true));
   *kept = f.kept;
   *workspace = align256(f.seg_state) + align256(f.seg_steps);
-  *backward_workspace = align256(b.seg_state) + align256(b.seg_steps) + align256(b.shared_parts) + align256(b.channel_parts);
+  *backward_workspace = align256(b.seg_state) + align256(b.seg_steps) + align256(b.channel_parts) + (desc->bc_fixed ? 0 : align256(b.shared_parts));
   return TFA_OK;
 }
 
@@ -277,13 +277,14 @@ int tfa_selective_scan_backward(const tfa_scan_desc* desc, const void* x, const 
   if (desc->batch > 0 && !a) return set_error(TFA_ERR_INVALID, "null data pointer");
   if (some && (!x || !dt || !b || !c || !g.grad_y)) return set_error(TFA_ERR_INVALID, "null data pointer");
   if (g.z && !z) return set_error(TFA_ERR_INVALID, "no gate, no gradient of one");
+  if (desc->bc_fixed && (g.b || g.c)) return set_error(TFA_ERR_INVALID, "bc_fixed leaves no room for gradients of b and c");
   if (g.state_in && g.state_in == g.grad_state_out) return set_error(TFA_ERR_INVALID, "the states' gradients must not be one");
   tfa::ScanArgs p = scan_args(desc, true);
   scan_inputs(p, desc, {x, dt, b, c, z, a, d, dt_bias});
   scan_tokens(p, desc);
   const tfa::ScanSizes size = tfa::scan_sizes(p);
   if (size.kept && !kept) return set_error(TFA_ERR_INVALID, "the forward's states are needed");
-  if (!workspace && align256(size.seg_state) + size.shared_parts + size.channel_parts) return set_error(TFA_ERR_INVALID, "null workspace");
+  if (!workspace && size.seg_state + size.channel_parts + (desc->bc_fixed ? 0 : size.shared_parts)) return set_error(TFA_ERR_INVALID, "null workspace");
   if (const int rc = check_aligned(kept, workspace)) return rc;
   p.lengths = reinterpret_cast<const long long*>(lengths);
   p.state_in = state_in, p.kept = static_cast<float*>(const_cast<void*>(kept));
@@ -293,9 +294,9 @@ int tfa_selective_scan_backward(const tfa_scan_desc* desc, const void* x, const 
   char* space = static_cast<char*>(workspace);
   p.seg_state = reinterpret_cast<float*>(space), space += align256(size.seg_state);
   p.seg_steps = reinterpret_cast<float*>(space), space += align256(size.seg_steps);
-  if (g.b || g.c) p.shared_parts = reinterpret_cast<float*>(space);
-  space += align256(size.shared_parts);
   if (g.a || g.d || g.dt_bias) p.channel_parts = reinterpret_cast<float*>(space);
+  space += align256(size.channel_parts);
+  if (g.b || g.c) p.shared_parts = reinterpret_cast<float*>(space);
   p.stream = static_cast<hipStream_t>(stream);
   return launched(tfa::launch_scan_backward(p));
 }
