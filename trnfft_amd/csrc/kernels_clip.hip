@@ -4,7 +4,7 @@
 //
 // Squares are summed in 64 bits: they neither overflow nor vanish for any finite fp32 gradient, and a sum over 10^8 of them
 // is exact to the norm's last bit (conversions and 64-bit products run at the vector units' ordinary rate, and one a value is
-// far below what the memory's rate leaves room for).  Every workgroup leaves one sum; they are added in one order by one workgroup: the
+// far below what the memory's rate leaves room for).  Every workgroup leaves one sum; they are added in one order: the
 // norm does not depend on timing.  Memory bound: one reading for the norm, one reading and writing where gradients are scaled.
 // 120M bf16 values in 320 tensors: 51 us for the squares (4.7 TB/s), 80 for scaling (6.0 TB/s: a part is in the caches still); 24 tensors of 0.5M
 // fp32 values together 4.0 and 4.3, which is two launches.
@@ -19,6 +19,10 @@ constexpr int kGradTensors = 180;  // per launch: their table travels in the ker
 // loads of a next batch cover the sums of this one)
 constexpr int kLeastChunk = 4096, kMostChunk = 65536;
 constexpr long long kGradBlocks = 2048;
+// Parts that every scaling workgroup adds up by itself; more are added in a launch of its own before.  bf16, norm and scaling: 120M values (1831
+// parts) 126 us both ways, 12M fp32 17 by themselves and 19 in a launch, 1000M (15258) 1185 and 1181, 2000M (30517) 2366 and 2277, 7000M (106811)
+// 10283 and 7903: together they read the square of their number.
+constexpr long long kGradParts = 16384;
 
 struct GradTable {
   GradTensor t[kGradTensors];
@@ -108,19 +112,26 @@ __global__ __launch_bounds__(256) void grad_squares_kernel(GradTable tab, double
   if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 
-__device__ __forceinline__ double norm_of_parts(const double* parts, long long count) {
+__device__ __forceinline__ double sum_of_parts(const double* parts, long long count) {
   double sum = 0.0;
 #pragma unroll 8
   for (long long i = threadIdx.x; i < count; i += 256) sum += parts[i];
-  return sqrt(block_sum(sum));
+  return block_sum(sum);
 }
+__device__ __forceinline__ double norm_of_parts(const double* parts, long long count) { return sqrt(sum_of_parts(parts, count)); }
 
 __global__ __launch_bounds__(256) void grad_norm_kernel(const double* parts, long long count, float* norm) {
   const double root = norm_of_parts(parts, count);
   if (threadIdx.x == 0) norm[0] = (float)root;
 }
 
-// Every workgroup adds the parts itself, in the same order: one launch less, for some 2000 values out of the caches.
+// the sum in place of the first part
+__global__ __launch_bounds__(256) void grad_sum_kernel(double* parts, long long count) {
+  const double sum = sum_of_parts(parts, count);
+  if (threadIdx.x == 0) parts[0] = sum;
+}
+
+// Every workgroup adds the parts itself, in the same order: one launch less, for up to kGradParts values out of the caches.
 template <typename T>
 __global__ __launch_bounds__(256) void grad_scale_kernel(GradTable tab, const double* parts, long long count, double max_norm, float* norm) {
   constexpr int V = GradStretch<T>::V;
@@ -207,6 +218,11 @@ hipError_t launch_grad_norm(const GradLists& g, double* parts, float* norm, bool
   if (!scale || !done) {
     hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(256), 0, stream, parts, done, norm);
     return hipGetLastError();
+  }
+  if (done > kGradParts) {
+    hipLaunchKernelGGL(grad_sum_kernel, dim3(1), dim3(256), 0, stream, parts, done);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    done = 1;
   }
   for (int d = 0; d < 3; ++d) {
     long long before = 0;
