@@ -698,11 +698,9 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
         ga[i] = __builtin_fmaf(xi, gb[i], ga[i] * (1.0f / kLog2E)) * lslope[at];
         gb[i] = __builtin_fmaf(ls[at], gb[i], skip * vi);
         dskip_tile = __builtin_fmaf(vi, xi, dskip_tile);
+        // (past the end the slope is 0, and so is ga, unless a rate of no memory has made an infinity of what it is taken times)
+        dbias_tile += s.q + Q * i < left ? ga[i] : 0.0f;
       }
-      // (where there is no token or channel the slope is 0, and so is ga, unless a rate of no memory has made an infinity of what it is taken times)
-      if (!full) clear_dead<Q>(s, left, ga);
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) dbias_tile += ga[i];
       // (a tile's terms by themselves first: long sums keep their last bits)
       dskip += dskip_tile;
       dbias += dbias_tile;
