@@ -14,9 +14,14 @@
 //
 // Bound by vector instructions (an exponential takes two instructions' time), not by memory.  A token and wave of 16 channels of 16 states take 39
 // of them forward, 24 for the recurrence and its dot products alone, and about 100 backward.  8 x 4096 tokens of 2048 channels, bf16: backward
-// 900 us in two segments (and 132 for their sums), forward 443 with one wave a SIMD, 400 in scan_pairs.h; 1 x 65536 of 1024 in 64 segments,
-// four waves a SIMD, 315 and 220 for the sums.  Products b u by 4 x 4 matrix instructions are 16 instructions fewer in two tokens and took
+// 900 to 924 us in two segments (and 130 to 134 for their sums), forward 443 with one wave a SIMD, 400 in scan_pairs.h; 1 x 65536 of 1024 in 64
+// segments, four waves a SIMD, 317 and 222 for the sums.  Products b u by 4 x 4 matrix instructions are 16 instructions fewer in two tokens and took
 // the same time, 8 lanes a channel of two states 557 and 1190 us.
+// The backward also runs out of scalar registers: 53 to 70 of them (34 to 43 at 33 to 64 states) lie in lanes of vector registers and are read back
+// in every tile, a part of its instructions.  At 33 to 64 states its LDS of 106 KB leaves a compute unit one workgroup, one wave a SIMD, and 16
+// channels whose shares of db and dc are added there: 32 B of workspace a value of the sequence where up to 16 states take 2.
+// A group of channels that does not fill a workgroup (4 waves, 8 at 17 to 32 states) leaves waves without channels, which backward run the pass for
+// its barriers: 64 x 626 tokens of 64 channels of 16 states, bf16, training 112 us in one group, 231 in four of 16 channels.
 #pragma once
 #include "scan_device.h"
 

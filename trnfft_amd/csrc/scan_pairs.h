@@ -7,8 +7,8 @@
 // barrier a tile: behind it both find the tile's s and s x in LDS, and what the other wave's states have added to the tile before.  Buffers
 // alternate from tile to tile, so nothing is written that is still read.
 //
-// Bound by issue: some 380 instructions a tile and wave, 3500 clocks for two waves' (8 x 4096 tokens of 2048 channels, bf16: 400 us, and 420 with states
-// kept).  Loads two tiles ahead made it no faster.
+// Bound by issue: some 380 instructions a tile and wave, 3500 clocks for two waves' (8 x 4096 tokens of 2048 channels, bf16: 400 us, and 418 to 426 with
+// states kept).  Loads two tiles ahead made it no faster.
 //
 // States that are kept or handed on lie as the kernels of four states a lane (scan_blocks.h) lay them out.
 #pragma once

@@ -2,7 +2,8 @@
 // on autograd's thread, would take longer than their work on the GPU.
 //
 // Steps of streams: where every operand is as the C ABI takes it, the call is made from here; asked from Python nine tensors cost 8 of the
-// 13.8 us of a small scan's step.  Anything else is left to Python, which converts or refuses it.
+// 13.8 us of a small scan's step.  Anything else is left to Python, which converts or refuses it: filters, biases, d and dt_bias of 16 bits are
+// converted to fp32 by a launch each (1 x 1024: convolution's step 20.5 us for 5.2, scan's 24.5 for 5.3).
 //
 // Whole sequences likewise (a scan takes 15 us of the host from Python, 7.6 from here), and their nodes of autograd's graph: a backward
 // pass in Python took 70 us on autograd's thread, which had to wake up for it and to take Python's lock; a small training pass of the scan takes

@@ -75,6 +75,12 @@ int check_scan(const tfa_scan_desc* d) {
 // Where two waves take the same channels (scan_pairs.h) a token takes 0.1 us whole up to 1024 waves; segments take as much at 924, less in
 // proportion to the waves below, and some 15 us for their launches: whole and in segments 7 x 4096 of 2048 (896 waves) 392 and 445, 6 rows (768)
 // 381 and 354, 12 x 1024 of 1024 (768) 97 and 100, 16 x 300 of 512 (512) 27 and 34.
+// Other numbers of states, bf16, forward and whole training passes (the backward's segments beside the rule's own forward), the rule's, then the
+// best of 1, 2, 4 ... 64 segments: 4 states, 8 x 4096 of 1024 (512 waves) 144 and 503, 128 (in 32) and 466 (in 16); 2 x 4096 of 1024 (128) 47 and
+// 150, 48 and 141; 1 x 65536 of 256 (16) 183 and 450, 184 and 449.  8 states, 1 x 16384 of 1024 (64) 97 and 320, 97 and 317.  32 states,
+// 8 x 4096 of 512 (512) 229 and 784, 199 and 784; 1 x 1000 of 512 (64) 26 and 111, 26 and 110.  64 states, 8 x 4096 of 256 (512) 221 and
+// 1043, 209 and 1041; 4 x 1001 of 384 (384) 55 and 261, 55 and 231 (in 8).  It does not fit where other numbers than 9 to 16 states make 1024 waves
+// exactly: 8 x 4096 of 2048 whole 597 (4 states) and 551 (8), 283 and 327 in 16 segments; 8 x 4096 of 512 of 64 states 512, 383.
 constexpr int64_t kForwardWaves = 1024, kForwardWant = 4096, kBackwardWaves = 2048, kBackwardWant = 2048;
 constexpr int64_t kMostSegments = 64, kSegTokens = 32, kSplitTokens = 256;
 // Sums of so few long segments are made in halves: 8 x 4096 of 2048, whose sums backwards are 1024 waves', 173 and 132 us.
