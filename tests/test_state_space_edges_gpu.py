@@ -99,6 +99,23 @@ def test_padding_has_no_gradient_where_there_is_no_memory(shape, dtype):
     assert not grads["a"][1].any() and not grads["a"][3, 0].any()
 
 
+@pytest.mark.parametrize("dtype", list(TOL))
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_masked_steps_have_no_gradient_where_there_is_no_memory(shape, dtype):
+    """Frames of no step keep the state at rates of -inf too, and give steps no gradient, however large state and gradient are."""
+    v, _ = scan_inputs(*shape, dtype, 6)
+    t = shape[1]
+    lengths = torch.tensor([t, t - 9][:shape[0]])
+    v["state"] *= 30.0
+    v["b"] *= 30.0
+    far = v["a"].double()
+    v["a"][1], v["a"][3, 0] = -INF, -INF
+    far[1], far[3, 0] = -1e300, -1e300
+    v["dt"][:, t - 12:] = v["dt"][:, 2] = -INF
+    _, _, grads = check(v, lengths, dlast_scale=30.0, of_reference={"a": far})
+    assert not grads["dt"][:, t - 12:].any() and not grads["dt"][:, 2].any()
+
+
 @pytest.mark.parametrize("states", [4, 16, 20, 40])
 def test_no_memory_for_gradients_that_are_not_wanted(states):
     """Fixed b and c: the others' gradients are the same, and the room that adds up b's and c's is not taken."""

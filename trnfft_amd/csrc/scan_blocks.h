@@ -17,7 +17,7 @@
 // 900 to 924 us in two segments (and 130 to 134 for their sums), forward 443 with one wave a SIMD, 400 in scan_pairs.h; 1 x 65536 of 1024 in 64
 // segments, four waves a SIMD, 317 and 222 for the sums.  Products b u by 4 x 4 matrix instructions are 16 instructions fewer in two tokens and took
 // the same time, 8 lanes a channel of two states 557 and 1190 us.
-// The backward also runs out of scalar registers: 53 to 70 of them (34 to 43 at 33 to 64 states) lie in lanes of vector registers and are read back
+// The backward also runs out of scalar registers: 54 to 70 of them (34 to 39 at 33 to 64 states) lie in lanes of vector registers and are read back
 // in every tile, a part of its instructions.  At 33 to 64 states its LDS of 106 KB leaves a compute unit one workgroup, one wave a SIMD, and 16
 // channels whose shares of db and dc are added there: 32 B of workspace a value of the sequence where up to 16 states take 2.
 // A group of channels that does not fill a workgroup (4 waves, 8 at 17 to 32 states) leaves waves without channels, which backward run the pass for
@@ -700,11 +700,12 @@ __global__ __launch_bounds__(64 * kBackWaves<Q>, 2) void scan_backward_kernel(Sc
         const int at = s.c * kPlaneRow + s.q + Q * i;
         const float xi = lx[at], vi = lv[at];
         ys[i] = lz[at] * __builtin_fmaf(skip, xi, ys[i]);
-        ga[i] = __builtin_fmaf(xi, gb[i], ga[i] * (1.0f / kLog2E)) * lslope[at];
+        // (a slope of 0, past the end and where steps are masked: no gradient, also where a rate of no memory has made an infinity of the sum)
+        const float slope_i = lslope[at], of_step = __builtin_fmaf(xi, gb[i], ga[i] * (1.0f / kLog2E)) * slope_i;
+        ga[i] = slope_i == 0.0f ? 0.0f : of_step;
         gb[i] = __builtin_fmaf(ls[at], gb[i], skip * vi);
         dskip_tile = __builtin_fmaf(vi, xi, dskip_tile);
-        // (past the end the slope is 0, and so is ga, unless a rate of no memory has made an infinity of what it is taken times)
-        dbias_tile += s.q + Q * i < left ? ga[i] : 0.0f;
+        dbias_tile += ga[i];
       }
       // (a tile's terms by themselves first: long sums keep their last bits)
       dskip += dskip_tile;
